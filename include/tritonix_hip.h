@@ -332,6 +332,112 @@ const char* tnx_strerror(int status);
 int tnx_last_hip_error(void); /* hipError_t of the last TNX_E_HIP on this thread */
 int tnx_version(void);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Microscaled 4-bit tensors.  Rows of k elements, quantised along k in blocks of 32: a 4-bit float per element (0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6 and a sign bit), a scale byte s per block that stands for 2^(s - 127) (255: NaN, for a block that held an
+ * infinity or a NaN).  Layout: k is padded to slabs of 256 with zeros; codes are row-major, 128 bytes per row and slab, the
+ * even element of a byte in its low half; scales are 8 bytes per row and slab, 32 rows together: [row / 32][slab][row % 32][8].
+ * Both buffers are 16-byte aligned; a batch of matrices follows one another without gaps.
+ */
+#define TNX_MX_MAX_K (1 << 22)
+
+typedef struct tnx_mx_args {
+  void* data;    /* the matrix: read by tnx_mx_quantize, written by tnx_mx_dequantize */
+  void* codes;   /* batch x tnx_mx_code_bytes(rows, k) */
+  void* scales;  /* batch x tnx_mx_scale_bytes(rows, k) */
+  int64_t batch, rows, k;
+  int64_t stride_batch, stride_row, stride_k;   /* of data, in elements; stride_k == 1 or stride_row == 1 are the fast layouts */
+  int32_t dtype;                                /* of data: TNX_F16, TNX_BF16 or TNX_F32 */
+  int32_t reserved;
+  void* stream;
+} tnx_mx_args;
+
+/* bytes of the two buffers of one matrix */
+size_t tnx_mx_code_bytes(int64_t rows, int64_t k);
+size_t tnx_mx_scale_bytes(int64_t rows, int64_t k);
+
+/* scale = 2^(floor(log2 of the block's largest magnitude) - 2), elements rounded to the nearest code, ties to the even code,
+ * above 6 to 6 */
+int tnx_mx_quantize(const tnx_mx_args* args);
+int tnx_mx_dequantize(const tnx_mx_args* args);
+
+/* from the row-major form of files: ceil(k / 2) bytes of codes and ceil(k / 32) scale bytes per row */
+int tnx_mx_import(const void* codes, const void* scales, int64_t batch, int64_t rows, int64_t k, void* out_codes, void* out_scales,
+                  void* stream);
+
+/* Products of two such tensors, both quantised along the k they are multiplied over: out[m, n] = a[m, k] . b[n, k], 32-bit
+ * sums, rounded once.  With a GLU epilogue n is the interleaved width (even rows of b are the gate) and out has n / 2 columns.
+ *
+ * experts > 0: b holds `experts` matrices one after another, and row r of the product (0 <= r < m) belongs to the expert e with
+ * offsets[e] <= r < offsets[e + 1] (device memory, offsets[0] = 0, not decreasing, offsets[experts] <= m).  Row r of the product takes
+ * row r of a or, with `order` given (device memory, one entry per row), row order[r] / top_k of the a_rows rows of a; entries outside are taken
+ * as the nearest row inside.  Rows from offsets[experts] on are written as zeros. */
+typedef struct tnx_mx_gemm_args {
+  const void *a_codes, *a_scales, *b_codes, *b_scales;
+  void* out;
+  int64_t m, n, k;
+  int64_t a_rows;            /* rows that a has: m, or the tokens that order chooses from */
+  int64_t stride_out;        /* elements from row to row of out (columns are neighbours) */
+  const int32_t* offsets;
+  const int32_t* order;
+  int32_t experts, top_k;
+  int32_t out_dtype;         /* TNX_F16, TNX_BF16 or TNX_F32 */
+  int32_t epilogue;          /* tnx_epilogue */
+  void* stream;
+} tnx_mx_gemm_args;
+
+int tnx_mx_gemm(const tnx_mx_gemm_args* args);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Routing of tokens to experts.
+ *
+ * scores s = softmax or sigmoid of a row of logits.  Experts are ranked by s + bias where there is a bias, by their logit where
+ * there is none; a logit of -inf cannot be chosen (nor a biased score of -inf or NaN).  With num_groups > 1 the experts come in
+ * that many equal groups, of which the top_groups best stay: a group is worth the sum of its group_top largest keys (those of them that
+ * can be chosen).  The top_k largest keys are chosen, the lower expert first where they are equal; slots left over hold expert -1 and weight 0.
+ * weight = scale * s, divided by the sum of the chosen s if renormalize.  A row with a NaN (for softmax also +inf) has experts
+ * -1 and weights NaN.
+ *
+ * The plan: `order` lists the pairs token * top_k + slot by expert, within an expert by pair, then -1 for the empty
+ * slots; expert e owns order[offsets[e] .. offsets[e + 1]); rows[pair] is the pair's place in order, -1 for an empty slot. */
+#define TNX_MOE_MAX_EXPERTS 1024
+#define TNX_MOE_MAX_TOP_K 32
+#define TNX_MOE_MAX_GROUPS 64
+
+enum tnx_moe_scoring { TNX_MOE_SOFTMAX = 0, TNX_MOE_SIGMOID = 1 };
+
+typedef struct tnx_moe_args {
+  const void* logits;        /* [tokens, num_experts], rows stride_logits elements apart */
+  const float* bias;         /* [num_experts] or null */
+  float* weights;            /* [tokens, top_k]: written by tnx_moe_route, read by the backward pass */
+  int32_t* experts;          /* [tokens, top_k]: written by tnx_moe_route, read by tnx_moe_plan and the backward pass */
+  int32_t* offsets;          /* [num_experts + 1] */
+  int32_t* order;            /* [tokens * top_k] */
+  int32_t* rows;             /* [tokens * top_k] */
+  const float* grad;         /* backward: gradient of weights, [tokens, top_k] */
+  void* grad_logits;         /* backward: [tokens, num_experts], contiguous, of the logits' dtype */
+  int64_t tokens, stride_logits;
+  int32_t num_experts, top_k, dtype, scoring;
+  int32_t num_groups, top_groups, group_top, renormalize;
+  float scale;
+  int32_t reserved;
+  void* workspace;           /* tnx_moe_workspace_bytes, 16-byte aligned, no initialisation */
+  size_t workspace_bytes;
+  void* stream;
+} tnx_moe_args;
+
+size_t tnx_moe_workspace_bytes(int64_t tokens, int32_t top_k, int32_t num_experts);
+/* experts, weights and the plan */
+int tnx_moe_route(const tnx_moe_args* args);
+/* the plan alone, for experts that the caller chose; numbers outside [0, num_experts) are empty slots */
+int tnx_moe_plan(const tnx_moe_args* args);
+/* grad_logits from grad: the choice is held fixed, as it is almost everywhere */
+int tnx_moe_route_backward(const tnx_moe_args* args);
+
+/* out[t, :] = sum over j of weights[t, j] * y[rows[t, j], :], empty slots left out; y [tokens * top_k, n] and out [tokens, n] contiguous.  32-bit sums. */
+int tnx_moe_combine(const void* y, const int32_t* rows, const float* weights, void* out, int64_t tokens, int32_t top_k, int64_t n,
+                    int32_t y_dtype, int32_t out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

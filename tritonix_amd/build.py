@@ -349,6 +349,7 @@ _resources = {}
 def _compile(src, obj, verbose, force=True):
     deps = [src, os.path.join(CSRC, "gemm_tile.h"), os.path.join(CSRC, "gemm_skinny.h"), os.path.join(CSRC, "registry.h"),
             os.path.join(CSRC, "conv_tile.h"), os.path.join(CSRC, "conv_pack.h"),
+            *([os.path.join(CSRC, "mx.h")] if os.path.basename(src).startswith(("mx_", "moe")) else []),
             *([os.path.join(CSRC, "conv_halo.h")] if os.path.basename(src).startswith(("halo_", "conv.hip")) else []),
             os.path.join(ROOT, "include", "tritonix_hip.h"), os.path.abspath(__file__)]
     if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(d) for d in deps):
@@ -399,7 +400,8 @@ def build(jobs=None, quick=False, verbose=True, force=True, only=None, out=None,
         GATHER_TILES if not (only or only_conv) or only == "gather" else (), os.path.join(BUILD, "gen")) + generate_halo(
         HALO_TILES if not (only or only_conv) or only == "gather" else (), os.path.join(BUILD, "gen")) + [
         os.path.join(CSRC, "capi.hip"), os.path.join(CSRC, "skinny.hip"),
-        os.path.join(CSRC, "conv.hip"), os.path.join(CSRC, "f32.hip")]
+        os.path.join(CSRC, "conv.hip"), os.path.join(CSRC, "f32.hip"), os.path.join(CSRC, "mx_quant.hip"), os.path.join(CSRC, "mx_gemm.hip"),
+        os.path.join(CSRC, "moe.hip")]
     if lib == LIB:
         try:
             build_launch(verbose)
