@@ -336,7 +336,8 @@ int tnx_version(void);
  * Microscaled 4-bit tensors.  Rows of k elements, quantised along k in blocks of 32: a 4-bit float per element (0, 0.5, 1,
  * 1.5, 2, 3, 4, 6 and a sign bit), a scale byte s per block that stands for 2^(s - 127) (255: NaN, for a block that held an
  * infinity or a NaN).  Layout: k is padded to slabs of 256 with zeros; codes are row-major, 128 bytes per row and slab, the
- * even element of a byte in its low half; scales are 8 bytes per row and slab, 32 rows together: [row / 32][slab][row % 32][8].
+ * even element of a byte in its low half; scales are 8 bytes per row and slab, two slabs and 32 rows together:
+ * [row / 32][slab / 2][row % 32][slab % 2][8].
  * Both buffers are 16-byte aligned; a batch of matrices follows one another without gaps.
  */
 #define TNX_MX_MAX_K (1 << 22)

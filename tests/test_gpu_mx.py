@@ -71,20 +71,20 @@ def test_extreme_blocks(device, dtype, dim):
 
 def test_codes_are_the_documented_bytes(device):
     """The two buffers byte by byte, and the padding: codes zero, scales 127 (rows past the last one excepted)."""
-    rows, k = 37, 300
+    rows, k = 37, 600
     x = make((rows, k), torch.bfloat16, 7)
     t = tritonix.mx_quantize(x.to(device))
     code, e, _ = ref.quantize(x.double().numpy())
-    slabs = 2
+    slabs = 3
     want = np.zeros((rows, slabs * 256), dtype=np.int64)
     want[:, :code.shape[1]] = code
     want = want[:, 0::2] + 16 * want[:, 1::2]
     np.testing.assert_array_equal(t.codes.cpu().numpy().reshape(rows, slabs * 128), want)
-    scales = t.scales.cpu().numpy().reshape(2, slabs, 32, 8)
+    scales = t.scales.cpu().numpy().reshape(2, 2, 32, 2, 8)       # row / 32, slab / 2, row % 32, slab % 2
     for r in range(rows):
-        got = scales[r // 32, :, r % 32, :].reshape(-1)
-        np.testing.assert_array_equal(got[:10], e[r] + 127)
-        assert (got[10:] == 127).all()
+        got = scales[r // 32, :, r % 32].reshape(-1)[:slabs * 8]
+        np.testing.assert_array_equal(got[:19], e[r] + 127)
+        assert (got[19:] == 127).all()
 
 
 @pytest.mark.parametrize("k", [1, 31, 32, 63, 100, 256, 1000])

@@ -32,8 +32,8 @@ def test_limits_are_the_headers():
 
 def test_buffer_sizes():
     lib = _C.load()
-    assert lib.tnx_mx_code_bytes(1, 1) == 128 and lib.tnx_mx_scale_bytes(1, 1) == 256
-    assert lib.tnx_mx_code_bytes(33, 257) == 33 * 256 and lib.tnx_mx_scale_bytes(33, 257) == 2 * 2 * 256
+    assert lib.tnx_mx_code_bytes(1, 1) == 128 and lib.tnx_mx_scale_bytes(1, 1) == 512
+    assert lib.tnx_mx_code_bytes(33, 257) == 33 * 256 and lib.tnx_mx_scale_bytes(33, 257) == 2 * 512 and lib.tnx_mx_scale_bytes(32, 513) == 2 * 512
     assert lib.tnx_mx_code_bytes(80000, 131072) == 80000 * 65536
     assert lib.tnx_mx_code_bytes(0, 5) == lib.tnx_mx_scale_bytes(5, 0) == 0
     t = tritonix.MXTensor.empty(3, 33, 257, -2, "cpu")

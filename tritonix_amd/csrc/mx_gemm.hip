@@ -126,22 +126,86 @@ __device__ __forceinline__ void store_columns(const MxParams& p, int64_t row, in
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Tiles: BN columns of the output (rows of the weights) x BM rows, four waves of half of each, slabs of 256 k in two LDS
-// buffers filled by direct loads.  Slab s + 1 has to be there, and slab s be read by all, when the last step of slab s
+// Tiles: BN columns of the output (rows of the weights) x BM rows, WGN x WGM waves, slabs of 256 k in two LDS buffers
+// filled by direct loads.  Slab s + 1 has to be there, and slab s be read by all, when the last step of slab s
 // begins: one barrier per slab, its wait hidden behind that step's products.
-template <int BN, int BM> struct MxTile {
-  static constexpr int WTN = BN / 2, WTM = BM / 2, TN = WTN / 32, TM = WTM / 32;
-  static constexpr int B_BYTES = BN * MX_ROWB, A_BYTES = BM * MX_ROWB, BS_BYTES = BN * MX_SCALEB, AS_BYTES = BM * MX_SCALEB;
-  static constexpr int SLOT = B_BYTES + A_BYTES + BS_BYTES + AS_BYTES;
-  static constexpr int B_OPS = B_BYTES / 4096, A_OPS = A_BYTES / 4096;      // 16-byte loads per lane and slab
-  // the epilogue's strip of a wave: 32 rows of its columns in binary32 at most
-  static constexpr int PITCH = WTN * 4 + 16, STRIP = 32 * PITCH;
-  static constexpr int LDS = 2 * SLOT > 4 * STRIP ? 2 * SLOT : 4 * STRIP;
+template <int BN_, int BM_, int WGN, int WGM> struct MxTile {
+  static constexpr int BN = BN_, BM = BM_, NW = WGN * WGM, THREADS = NW * 64, WAVES_M = WGM;
+  static constexpr int WTN = BN / WGN, WTM = BM / WGM, TN = WTN / 32, TM = WTM / 32;
+  static constexpr int B_BYTES = BN * MX_ROWB, A_BYTES = BM * MX_ROWB;
+  static constexpr int SLOT = B_BYTES + A_BYTES, S_BYTES = (BN + BM) * 2 * MX_SCALEB;      // codes of a slab; scales of two
+  static constexpr int B_OPS = B_BYTES / (1024 * NW), A_OPS = A_BYTES / (1024 * NW);      // 16-byte loads per lane and slab
+  static constexpr int LDS = 2 * SLOT + 2 * S_BYTES;
+  // waves per SIMD that the LDS leaves room for
+  static constexpr int OCC = (163840 / LDS) * NW / 4;
 };
 
-template <int BN, int BM, bool EXPERTS>
-__global__ __launch_bounds__(256) void mx_tile_kernel(MxParams p) {
-  typedef MxTile<BN, BM> C;
+// x: words of an even q, y: of the odd q after it.  Lanes 0-31 keep x and get its upper lanes' as y; lanes 32-63 the same of y.
+__device__ __forceinline__ void exchange_halves(uint32_t& x, uint32_t& y) {
+  const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  x = r[0];
+  y = r[1];
+}
+template <class O> __device__ __forceinline__ uint32_t two(float a, float b) { return (uint32_t)O::cvt(a) | (uint32_t)O::cvt(b) << 16; }
+
+// a lane's words of a row, or as many of their elements (of ES bytes) as the row still has
+template <bool WHOLE, int ES, int WORDS> __device__ __forceinline__ void store_words(uint8_t* d, const uint32_t (&w)[WORDS], int left) {
+  if (WHOLE || left >= WORDS * 4 / ES) {
+    typedef i32x2 __attribute__((aligned(2))) loose2;
+    if constexpr (WORDS == 4) *(i32x4_loose*)d = i32x4{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+    else *(loose2*)d = i32x2{(int)w[0], (int)w[1]};
+  } else {
+#pragma unroll
+    for (int e = 0; e < WORDS * 4 / ES; ++e)
+      if (e < left) {
+        if constexpr (ES == 4) ((uint32_t*)d)[e] = w[e];
+        else ((uint16_t*)d)[e] = (uint16_t)(w[e / 2] >> (e & 1) * 16);
+      }
+  }
+}
+
+// One 32x32 product into its place (out: row 0, column 0 of it; m_left, left_cols: what there is of it).  A lane has, of row lane % 32, the columns
+// 8 q + 4 half + 0 .. 3.  Rounded, four columns are two words; exchanging the halves' words of an even q with those of the odd q after it leaves
+// lanes 0-31 with all eight columns of the one and lanes 32-63 with those of the other: 16 bytes a lane.  (With the gate two columns are a word,
+// 8 bytes a lane; binary32 needs no exchange.)
+template <bool WHOLE, class O, bool GLU>
+__device__ __forceinline__ void store_product(const f32x16& v, uint8_t* out, int64_t ldo, int r32, int half, int m_left, int left_cols, int epi) {
+  constexpr int ES = sizeof(typename O::raw);
+  uint8_t* row = out + (int64_t)r32 * ldo * ES;
+  const bool have = WHOLE || r32 < m_left;
+#pragma unroll
+  for (int q = 0; q < 4; q += 2) {
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < (GLU ? 4 : 8); ++e) o[e] = GLU ? glu_gate<true>(v[4 * q + 2 * e], epi) * v[4 * q + 2 * e + 1] : v[4 * q + e];
+    if constexpr (ES == 4) {
+      constexpr int W = GLU ? 2 : 4;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = 2 * W * (q + h) + W * half;
+        uint32_t w[W];
+#pragma unroll
+        for (int e = 0; e < W; ++e) w[e] = __builtin_bit_cast(uint32_t, o[W * h + e]);
+        if (have) store_words<WHOLE, 4, W>(row + c * 4, w, left_cols - c);
+      }
+    } else if constexpr (GLU) {
+      uint32_t w[2] = {two<O>(o[0], o[1]), two<O>(o[2], o[3])};
+      exchange_halves(w[0], w[1]);
+      const int c = 4 * (q + half);
+      if (have) store_words<WHOLE, 2, 2>(row + c * 2, w, left_cols - c);
+    } else {
+      uint32_t w[4] = {two<O>(o[0], o[1]), two<O>(o[2], o[3]), two<O>(o[4], o[5]), two<O>(o[6], o[7])};
+      exchange_halves(w[0], w[2]);
+      exchange_halves(w[1], w[3]);
+      const int c = 8 * (q + half);
+      if (have) store_words<WHOLE, 2, 4>(row + c * 2, w, left_cols - c);
+    }
+  }
+}
+
+template <class C, bool EXPERTS, class O, bool GLU>
+__global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_kernel(MxParams p) {
+  constexpr int BN = C::BN, BM = C::BM, NW = C::NW;
   extern __shared__ __attribute__((aligned(1024))) uint8_t mx_smem[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(uint8_t __attribute__((address_space(3)))*)mx_smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -158,7 +222,7 @@ __global__ __launch_bounds__(256) void mx_tile_kernel(MxParams p) {
   } else {
     const int id = xcd_remap(blockIdx.x, p.tiles_m * p.tiles_n, 8);
     int tm;
-    swizzle2d(id / p.tiles_n, id % p.tiles_n, p.tiles_m, p.tiles_n, 8, &tm, &tn);
+    swizzle2d(id / p.tiles_n, id % p.tiles_n, p.tiles_m, p.tiles_n, 4, &tm, &tn);
     rt.expert = 0;
     rt.row0 = tm * BM;
     rt.rows = p.m - rt.row0 < BM ? p.m - rt.row0 : BM;
@@ -166,19 +230,19 @@ __global__ __launch_bounds__(256) void mx_tile_kernel(MxParams p) {
   const int n0 = tn * BN, ncols = p.n - n0 < BN ? p.n - n0 : BN;
   if (EXPERTS && rt.expert == p.experts) {               // rows of no expert
     const int c0 = p.epi != EPI_NONE ? n0 / 2 : n0, nc = p.epi != EPI_NONE ? ncols / 2 : ncols;
-    for (int i = tid; i < rt.rows * nc; i += 256) store_out<float>(p.out, (int64_t)(rt.row0 + i / nc) * p.ldo + c0 + i % nc, 0.0f, p.out_dtype);
+    for (int i = tid; i < rt.rows * nc; i += C::THREADS) store_out<float>(p.out, (int64_t)(rt.row0 + i / nc) * p.ldo + c0 + i % nc, 0.0f, p.out_dtype);
     return;
   }
   const uint8_t* b = uniform_ptr(p.b + (int64_t)rt.expert * p.b_expert + (int64_t)n0 * p.slabs * MX_ROWB);
-  const uint8_t* bs = uniform_ptr(p.bs + (int64_t)rt.expert * p.bs_expert + (int64_t)(n0 >> 5) * p.slabs * 256);
+  const uint8_t* bs = uniform_ptr(p.bs + (int64_t)rt.expert * p.bs_expert + (int64_t)(n0 >> 5) * ((p.slabs + 1) >> 1) * 512);
 
-  // Direct loads.  Instruction q of wave w fills rows 8 (4 q + w) .. + 7 of a side, lane l the 16-byte place l % 8 of row l / 8,
+  // Direct loads.  Instruction q of wave w fills rows 8 (NW q + w) .. + 7 of a side, lane l the 16-byte place l % 8 of row l / 8,
   // which holds the chunk place ^ (row / 2 % 8): a fragment read (16 lanes a cycle, rows {0-3, 12-15, 20-27} or the others, one chunk)
   // then falls on 16 different places of 256 bytes.  Rows past the end are the last row again; nobody stores what they give.
   uint32_t b_off[C::B_OPS];
 #pragma unroll
   for (int q = 0; q < C::B_OPS; ++q) {
-    const int row = 8 * (4 * q + wave) + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
+    const int row = 8 * (NW * q + wave) + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
     b_off[q] = (uint32_t)(row < ncols ? row : ncols - 1) * (uint32_t)(p.slabs * MX_ROWB) + chunk * 16;
   }
   uint32_t a_off[C::A_OPS];
@@ -187,79 +251,51 @@ __global__ __launch_bounds__(256) void mx_tile_kernel(MxParams p) {
   if (EXPERTS) {
 #pragma unroll
     for (int q = 0; q < C::A_OPS; ++q) {
-      const int row = 8 * (4 * q + wave) + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
+      const int row = 8 * (NW * q + wave) + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
       a_at[q] = p.a + (int64_t)source_row(p, rt.row0 + (row < rt.rows ? row : rt.rows - 1)) * p.slabs * MX_ROWB + chunk * 16;
     }
   } else {
     a = uniform_ptr(p.a + (int64_t)rt.row0 * p.slabs * MX_ROWB);
 #pragma unroll
     for (int q = 0; q < C::A_OPS; ++q) {
-      const int row = 8 * (4 * q + wave) + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
+      const int row = 8 * (NW * q + wave) + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
       a_off[q] = (uint32_t)(row < rt.rows ? row : rt.rows - 1) * (uint32_t)(p.slabs * MX_ROWB) + chunk * 16;
     }
   }
-  // Scales: 16 lanes a group of 32 rows (256 bytes); a wave's instruction takes four groups.  BN / 128 instructions of 1 KiB in all.  With
-  // experts the rows of a lie anywhere: two words per row, 32 rows an instruction.
-  constexpr int BS_OPS = (C::BS_BYTES + 1023) / 1024, AS_OPS = EXPERTS ? C::AS_BYTES / 256 : (C::AS_BYTES + 1023) / 1024;
-  uint32_t bs_off[BS_OPS];
-#pragma unroll
-  for (int q = 0; q < BS_OPS; ++q) {
-    const int last = (ncols - 1) >> 5, g = 4 * q + (lane >> 4);
-    bs_off[q] = (uint32_t)(g < last ? g : last) * (uint32_t)(p.slabs * 256) + (lane & 15) * 16;
-  }
-  uint32_t as_off[EXPERTS ? 1 : AS_OPS];
-  const uint8_t* as_at[EXPERTS ? (AS_OPS + 3) / 4 : 1];
-  const uint8_t* as = nullptr;
-  if (EXPERTS) {
-#pragma unroll
-    for (int q = 0; q < (AS_OPS + 3) / 4; ++q) {
-      const int row = 32 * (4 * q + wave) + (lane >> 1);
-      const int src = source_row(p, rt.row0 + (row < rt.rows ? row : rt.rows - 1));
-      as_at[q] = p.as + mx_scale_at(src, 0, p.slabs) + (lane & 1) * 4;
-    }
-  } else {
-    as = uniform_ptr(p.as + (int64_t)(rt.row0 >> 5) * p.slabs * 256);
-#pragma unroll
-    for (int q = 0; q < AS_OPS; ++q) {
-      const int last = (rt.rows - 1) >> 5, g = 4 * q + (lane >> 4);
-      as_off[q] = (uint32_t)(g < last ? g : last) * (uint32_t)(p.slabs * 256) + (lane & 15) * 16;
+  // Scales: 16 bytes a row, for two slabs; wave w brings those of 64 rows, of the weights' first, then of a's
+  constexpr int S_WAVES = (BN + BM) / 64;
+  static_assert(S_WAVES <= NW, "a wave has one load of scales");
+  const uint8_t* s_at;
+  {
+    const int row = 64 * wave + lane, ar = row - BN;
+    if (64 * wave < BN) s_at = bs + mx_scale_at(row < ncols ? row : ncols - 1, 0, p.slabs);
+    else {
+      const int r = rt.row0 + (ar < rt.rows ? ar : rt.rows - 1);
+      s_at = p.as + mx_scale_at(EXPERTS ? source_row(p, r) : r, 0, p.slabs);
     }
   }
 
-  auto fetch = [&](int slab) __attribute__((always_inline)) {
+  // one slab is OPS loads of a wave: op q of them (a constant after unrolling) into the slab's buffer
+  constexpr int OPS = C::B_OPS + C::A_OPS + 1;
+  auto fetch_op = [&](int slab, int q) __attribute__((always_inline)) {
     const uint32_t slot = lds0 + (slab & 1) * C::SLOT;
-    const uint8_t* bk = b + (int64_t)slab * MX_ROWB;
-#pragma unroll
-    for (int q = 0; q < C::B_OPS; ++q) dma16_from(bk, b_off[q], slot + (4 * q + wave) * 1024);
-    if (EXPERTS) {
-#pragma unroll
-      for (int q = 0; q < C::A_OPS; ++q) dma16_at(a_at[q] + (int64_t)slab * MX_ROWB, slot + C::B_BYTES + (4 * q + wave) * 1024);
-    } else {
-      const uint8_t* ak = a + (int64_t)slab * MX_ROWB;
-#pragma unroll
-      for (int q = 0; q < C::A_OPS; ++q) dma16_from(ak, a_off[q], slot + C::B_BYTES + (4 * q + wave) * 1024);
-    }
-    const uint32_t sb = slot + C::B_BYTES + C::A_BYTES, sa = sb + C::BS_BYTES;
-    const uint8_t* bsk = bs + (int64_t)slab * 256;
-    // (every branch below is uniform over the wave)
-#pragma unroll
-    for (int q = 0; q < BS_OPS; ++q)
-      if (wave == q) { if (C::BS_BYTES >= 1024 || lane < C::BS_BYTES / 16) dma16_from(bsk, bs_off[q], sb + q * 1024); }
-    if (EXPERTS) {
-#pragma unroll
-      for (int q = 0; q < (AS_OPS + 3) / 4; ++q)
-        if (AS_OPS >= 4 || wave < AS_OPS) dma4_at(as_at[q] + (int64_t)slab * 256, sa + (4 * q + wave) * 256);
-    } else {
-      const uint8_t* ask = as + (int64_t)slab * 256;
-#pragma unroll
-      for (int q = 0; q < AS_OPS; ++q)
-        if (wave == 3 - q) { if (C::AS_BYTES >= 1024 || lane < C::AS_BYTES / 16) dma16_from(ask, as_off[q], sa + q * 1024); }
+    if (q < C::B_OPS) dma16_from(b + (int64_t)slab * MX_ROWB, b_off[q], slot + (NW * q + wave) * 1024);
+    else if (q < C::B_OPS + C::A_OPS) {
+      const int i = q - C::B_OPS;
+      const uint32_t to = slot + C::B_BYTES + (NW * i + wave) * 1024;
+      if (EXPERTS) dma16_at(a_at[i] + (int64_t)slab * MX_ROWB, to);
+      else dma16_from(a + (int64_t)slab * MX_ROWB, a_off[i], to);
+    } else if ((slab & 1) == 0 && wave < S_WAVES) {
+      dma16_at(s_at + (int64_t)(slab >> 1) * 512, lds0 + 2 * C::SLOT + (slab >> 1 & 1) * C::S_BYTES + wave * 1024);
     }
   };
 
-  const int wn = (wave >> 1) * C::WTN, wm = (wave & 1) * C::WTM, half = lane >> 5, r32 = lane & 31;
-  // place of chunk 4 half + step in this lane's row
+  const int wn = wave / C::WAVES_M * C::WTN, wm = wave % C::WAVES_M * C::WTM, half = lane >> 5, r32 = lane & 31;
+  // place of chunk 4 half + step in this lane's row; the weights' and a's products further on are constants from here
   const uint32_t place = (uint32_t)r32 * MX_ROWB + (((4 * half) ^ ((r32 >> 1) & 7)) << 4);
+  const uint32_t place_b = lds0 + place + wn * MX_ROWB, place_a = lds0 + place + C::B_BYTES + wm * MX_ROWB;
+  const uint32_t place_s = lds0 + 2 * C::SLOT + r32 * 2 * MX_SCALEB + half * 4;
+  constexpr int NM = C::TN * C::TM;
   f32x16 acc[C::TN][C::TM];
 #pragma unroll
   for (int i = 0; i < C::TN; ++i)
@@ -267,112 +303,110 @@ __global__ __launch_bounds__(256) void mx_tile_kernel(MxParams p) {
     for (int j = 0; j < C::TM; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-  i32x4 fb[2][C::TN], fa[2][C::TM];
-  int sb[2][C::TN], sa[2][C::TM];
-  auto read_step = [&](int slab, int step, int set) __attribute__((always_inline)) {
-    const uint32_t at = lds0 + (slab & 1) * C::SLOT + (place ^ (step << 4));
-#pragma unroll
-    for (int i = 0; i < C::TN; ++i) fb[set][i] = *TNX_LDS(i32x4, at + (wn + 32 * i) * MX_ROWB);
-#pragma unroll
-    for (int j = 0; j < C::TM; ++j) fa[set][j] = *TNX_LDS(i32x4, at + C::B_BYTES + (wm + 32 * j) * MX_ROWB);
+  // Fragments and scales.  A slab is four steps (blocks 4 half + step); a step goes through the products column by column of a's
+  // fragments.  So a's fragment j is free once column j is done and takes the next step's at once; the weights' are in use to
+  // a step's end and have two sets.
+  i32x4 fb[2][C::TN], fa[C::TM];
+  int sb[2][C::TN], sa[C::TM];
+  auto read_b = [&](uint32_t slot, int step, int i) __attribute__((always_inline)) {
+    fb[step & 1][i] = *TNX_LDS(i32x4, (place_b ^ (step << 4)) + slot + i * 32 * MX_ROWB);
   };
-  auto read_scales = [&](int slab, int set) __attribute__((always_inline)) {
-    const uint32_t at = lds0 + (slab & 1) * C::SLOT + C::B_BYTES + C::A_BYTES + r32 * MX_SCALEB + half * 4;
-#pragma unroll
-    for (int i = 0; i < C::TN; ++i) sb[set][i] = *TNX_LDS(int, at + (wn + 32 * i) * MX_SCALEB);
-#pragma unroll
-    for (int j = 0; j < C::TM; ++j) sa[set][j] = *TNX_LDS(int, at + C::BS_BYTES + (wm + 32 * j) * MX_SCALEB);
+  auto read_a = [&](uint32_t slot, int step, int j) __attribute__((always_inline)) {
+    fa[j] = *TNX_LDS(i32x4, (place_a ^ (step << 4)) + slot + j * 32 * MX_ROWB);
   };
-
-  const int slabs = p.slabs;
-  fetch(0);
-  TNX_WAIT_VM(0);
-  __syncthreads();
-  if (slabs > 1) fetch(1);
-  read_scales(0, 0);
-  read_step(0, 0, 0);
-  for (int s = 0; s < slabs; ++s) {
+  // (at: of the slab, in the scales' buffers)
+  auto read_sb = [&](uint32_t at, int set, int i) __attribute__((always_inline)) { sb[set][i] = *TNX_LDS(int, place_s + at + (wn + 32 * i) * 2 * MX_SCALEB); };
+  auto read_sa = [&](uint32_t at, int j) __attribute__((always_inline)) { sa[j] = *TNX_LDS(int, place_s + at + (BN + wm + 32 * j) * 2 * MX_SCALEB); };
+  // A slab's products, in the order written: the compiler, left to itself, moves each fragment's read in front of its use and waits for it.
+  // After the last step's first column comes the barrier; from there on the reads are the next slab's.  From there on, too, and far into the next
+  // slab, one direct load every STRIDE products: a load of a wave takes the address unit 16 cycles, and a wave whose
+  // load has to queue for it issues no products meanwhile.
+  constexpr int BAR = C::TM > 1 ? C::TN : 0, EARLY = NM - BAR, ROOM = EARLY + 2 * NM;
+  constexpr int STRIDE = ROOM / OPS > 0 ? ROOM / OPS : 1, DPER = (OPS * STRIDE + ROOM - 1) / ROOM;
+  constexpr int FIRST_OPS = (EARLY + STRIDE - 1) / STRIDE * DPER < C::B_OPS + C::A_OPS ? (EARLY + STRIDE - 1) / STRIDE * DPER : C::B_OPS + C::A_OPS;
+  constexpr int PER = (C::TN + EARLY - 1) / EARLY;
+  auto products = [&](int s, auto next_tag, auto fetch_tag) __attribute__((always_inline)) {
+    constexpr bool NEXT = decltype(next_tag)::value, FETCH = decltype(fetch_tag)::value;
+    const uint32_t slot = (s & 1) * C::SLOT, other = C::SLOT - slot, scales = ((s + 1) >> 1 & 1) * C::S_BYTES + ((s + 1) & 1) * MX_SCALEB;
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      if (step < 3) read_step(s, step + 1, (step + 1) & 1);
-      constexpr int HALF = C::TN * C::TM / 2;
 #pragma unroll
-      for (int e = 0; e < C::TN * C::TM; ++e) {
-        if (step == 3 && e == HALF) {
-          // The fragments of this slab are in registers and the loads of the next one have landed, in every wave.  (After the
-          // last slab the reads fetch what the other buffer still holds, and nothing uses it.)
-          __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < NM; ++e) {
+        if (NEXT && step == 3 && e == BAR) {
+          // the fragments of this slab are in registers and the loads of the next one have landed, in every wave
           asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
-          read_step(s + 1, 0, 0);
-          read_scales(s + 1, 1);
-          if (s + 2 < slabs) fetch(s + 2);
           __builtin_amdgcn_sched_barrier(0);
         }
-        const int i = e / C::TM, j = (i & 1) ? C::TM - 1 - e % C::TM : e % C::TM;
-        acc[i][j] = mfma32(fb[step & 1][i], fa[step & 1][j], acc[i][j], sb[0][i], sa[0][j], step);
+        const int j = e / C::TN, i = (j & 1) ? C::TN - 1 - e % C::TN : e % C::TN;
+        acc[i][j] = mfma32(fb[step & 1][i], fa[j], acc[i][j], sb[0][i], sa[j], step);
+        if (step < 3) {
+          if (e < C::TN) read_b(slot, step + 1, e);
+          if (e % C::TN == C::TN - 1) read_a(slot, step + 1, j);
+        } else if (NEXT && e >= BAR) {
+#pragma unroll
+          for (int r = (e - BAR) * PER; r < (e - BAR) * PER + PER && r < C::TN; ++r) {
+            read_b(other, 0, r);
+            read_sb(scales, 1, r);
+          }
+          if (BAR > 0 && e == BAR) { read_a(other, 0, 0); read_sa(scales, 0); }
+          if (e % C::TN == C::TN - 1) { read_a(other, 0, j); read_sa(scales, j); }
+        }
+        if (step == 3 ? FETCH && e >= BAR : NEXT) {
+          const int at = step == 3 ? e - BAR : EARLY + step * NM + e;
+          if (at % STRIDE == 0) {
+#pragma unroll
+            for (int q = at / STRIDE * DPER; q < at / STRIDE * DPER + DPER; ++q)
+              if (step == 3 ? q < FIRST_OPS : q >= FIRST_OPS && q < OPS) fetch_op(step == 3 ? s + 2 : s + 1, q);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+    if (NEXT) {
 #pragma unroll
-    for (int i = 0; i < C::TN; ++i) sb[0][i] = sb[1][i];
-#pragma unroll
-    for (int j = 0; j < C::TM; ++j) sa[0][j] = sa[1][j];
-  }
+      for (int i = 0; i < C::TN; ++i) sb[0][i] = sb[1][i];
+    }
+  };
 
-  // Epilogue.  A lane has, of output row lane % 32 of each 32x32 product, the columns 8 q + 4 half + 0 .. 3: they go to the wave's own strip of
-  // LDS (rows of outputs, gated and rounded), and leave as 16-byte pieces of whole rows.
-  __syncthreads();
-  const uint32_t strip = lds0 + wave * C::STRIP;
-  const bool glu = p.epi != EPI_NONE;
-  const int es = p.out_dtype == DT_F32 ? 4 : 2;
-  const int ocols = glu ? C::WTN / 2 : C::WTN;
-  const int row_bytes = ocols * es, pieces = row_bytes / 16;          // a power of two
-  const int left_cols = (glu ? ncols / 2 : ncols) - (glu ? wn / 2 : wn);
-  const int64_t col0 = (glu ? n0 / 2 : n0) + (glu ? wn / 2 : wn);
-  const int shift = 31 - __clz(pieces);
+  const int slabs = p.slabs;
 #pragma unroll
-  for (int j = 0; j < C::TM; ++j) {
+  for (int q = 0; q < OPS; ++q) fetch_op(0, q);
+  if (slabs > 1) {
 #pragma unroll
-    for (int i = 0; i < C::TN; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float v0 = acc[i][j][4 * q], v1 = acc[i][j][4 * q + 1], v2 = acc[i][j][4 * q + 2], v3 = acc[i][j][4 * q + 3];
-        const int c = 32 * i + 8 * q + 4 * half;
-        const uint32_t at = strip + r32 * C::PITCH;
-        if (glu) {
-          const float o0 = glu_gate<true>(v0, p.epi) * v1, o1 = glu_gate<true>(v2, p.epi) * v3;
-          if (es == 4) *TNX_LDS(i32x2, at + c * 2) = i32x2{__builtin_bit_cast(int, o0), __builtin_bit_cast(int, o1)};
-          else if (p.out_dtype == DT_BF16) *TNX_LDS(int, at + c) = (int)((uint32_t)OutBF16::cvt(o0) | (uint32_t)OutBF16::cvt(o1) << 16);
-          else *TNX_LDS(int, at + c) = (int)((uint32_t)OutF16::cvt(o0) | (uint32_t)OutF16::cvt(o1) << 16);
-        } else if (es == 4) {
-          *TNX_LDS(i32x4, at + c * 4) = i32x4{__builtin_bit_cast(int, v0), __builtin_bit_cast(int, v1), __builtin_bit_cast(int, v2), __builtin_bit_cast(int, v3)};
-        } else if (p.out_dtype == DT_BF16) {
-          *TNX_LDS(i32x2, at + c * 2) = i32x2{(int)((uint32_t)OutBF16::cvt(v0) | (uint32_t)OutBF16::cvt(v1) << 16),
-                                              (int)((uint32_t)OutBF16::cvt(v2) | (uint32_t)OutBF16::cvt(v3) << 16)};
-        } else {
-          *TNX_LDS(i32x2, at + c * 2) = i32x2{(int)((uint32_t)OutF16::cvt(v0) | (uint32_t)OutF16::cvt(v1) << 16),
-                                              (int)((uint32_t)OutF16::cvt(v2) | (uint32_t)OutF16::cvt(v3) << 16)};
-        }
-      }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the strip is the wave's own: its LDS operations are in order
-    const int m_left = rt.rows - (wm + 32 * j);
-    for (int t = lane; t < 32 * pieces; t += 64) {
-      const int row = t >> shift, piece = t & (pieces - 1), c = piece * 16 / es;
-      const i32x4 v = *TNX_LDS(i32x4, strip + row * C::PITCH + piece * 16);
-      if (row >= m_left || c >= left_cols) continue;
-      uint8_t* d = p.out + ((int64_t)(rt.row0 + wm + 32 * j + row) * p.ldo + col0 + c) * es;
-      if (c + 16 / es <= left_cols) *(i32x4_loose*)d = v;
-      else {
-        for (int e = 0; c + e < left_cols; ++e) {        // (constant places of v only: no array in scratch memory)
-          const uint32_t w = (uint32_t)(e * es < 4 ? v[0] : e * es < 8 ? v[1] : e * es < 12 ? v[2] : v[3]);
-          if (es == 4) ((uint32_t*)d)[e] = w;
-          else ((uint16_t*)d)[e] = (uint16_t)(e & 1 ? w >> 16 : w);
-        }
-      }
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    for (int q = 0; q < FIRST_OPS; ++q) fetch_op(1, q);
+    TNX_WAIT_VM(FIRST_OPS);                // (these go out in every wave: what is older has landed)
+  } else {
+    TNX_WAIT_VM(0);
   }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < C::TN; ++i) { read_b(0, 0, i); read_sb(0, 0, i); }
+#pragma unroll
+  for (int j = 0; j < C::TM; ++j) { read_a(0, 0, j); read_sa(0, j); }
+  int s = 0;
+  for (; s < slabs - 2; ++s) products(s, BoolTag<true>(), BoolTag<true>());
+  if (s < slabs - 1) products(s++, BoolTag<true>(), BoolTag<false>());
+  products(s, BoolTag<false>(), BoolTag<false>());
+
+  // Epilogue, from the registers (LDS is not touched: nothing waits for the other waves).  The sums stay where the matrix instructions
+  // left them until their turn: without the empty asm all 256 are copied out at once, to scratch memory for the most part.
+  constexpr int ES = sizeof(typename O::raw), W = GLU ? 16 : 32;          // output columns of a product
+  const int left_cols = GLU ? (ncols - wn) >> 1 : ncols - wn;
+  uint8_t* out = p.out + ((int64_t)(rt.row0 + wm) * p.ldo + (GLU ? (n0 + wn) >> 1 : n0 + wn)) * ES;
+  const bool whole = rt.rows - wm >= C::WTM && ncols - wn >= C::WTN;
+#pragma unroll
+  for (int j = 0; j < C::TM; ++j)
+#pragma unroll
+    for (int i = 0; i < C::TN; ++i) {
+      f32x16 v = acc[i][j];
+      asm volatile("" : "+a"(v));
+      uint8_t* at = out + ((int64_t)(32 * j) * p.ldo + W * i) * ES;
+      if (whole) store_product<true, O, GLU>(v, at, p.ldo, r32, half, 32, W, p.epi);
+      else store_product<false, O, GLU>(v, at, p.ldo, r32, half, rt.rows - wm - 32 * j, left_cols - W * i, p.epi);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -431,7 +465,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
           for (int i = 0; i < NT; ++i) {
             fb[d][i][0] = *(const i32x4*)(b_at[i] + s * MX_ROWB);
             fb[d][i][1] = *(const i32x4*)(b_at[i] + s * MX_ROWB + 16);
-            sb[d][i] = *(const uint16_t*)(bs_at[i] + s * 256);
+            sb[d][i] = *(const uint16_t*)(bs_at[i] + (s >> 1) * 512 + (s & 1) * 8);
           }
         }
       }
@@ -446,7 +480,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
             if (a_have[j]) {
               fa0 = *(const i32x4*)(a_at[j] + s * MX_ROWB);
               fa1 = *(const i32x4*)(a_at[j] + s * MX_ROWB + 16);
-              sa = *(const uint16_t*)(as_at[j] + s * 256);
+              sa = *(const uint16_t*)(as_at[j] + (s >> 1) * 512 + (s & 1) * 8);
             }
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
@@ -474,14 +508,19 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-template <int BN, int BM, bool EXPERTS> int launch_tile(MxParams p, int64_t row_tiles, hipStream_t stream) {
-  typedef MxTile<BN, BM> C;
-  p.tiles_n = (p.n + BN - 1) / BN;
-  p.tiles_m = (p.m + BM - 1) / BM;
+template <class C, bool EXPERTS> int launch_tile(MxParams p, int64_t row_tiles, hipStream_t stream) {
+  p.tiles_n = (p.n + C::BN - 1) / C::BN;
+  p.tiles_m = (p.m + C::BM - 1) / C::BM;
   const int64_t grid = row_tiles * p.tiles_n;
   if (grid > 0x7fffffff) return TNX_E_UNSUPPORTED;
-  hipLaunchKernelGGL((mx_tile_kernel<BN, BM, EXPERTS>), dim3((unsigned)grid), dim3(256), C::LDS, stream, p);
-  return mx_launched();
+  auto go = [&](auto out_tag, auto glu_tag) {
+    typedef typename decltype(out_tag)::type O;
+    hipLaunchKernelGGL((mx_tile_kernel<C, EXPERTS, O, decltype(glu_tag)::value>), dim3((unsigned)grid), dim3(C::THREADS), C::LDS, stream, p);
+    return mx_launched();
+  };
+  auto gated = [&](auto out_tag) { return p.epi != EPI_NONE ? go(out_tag, BoolTag<true>()) : go(out_tag, BoolTag<false>()); };
+  if (p.out_dtype == DT_BF16) return gated(TypeTag<OutBF16>());
+  return p.out_dtype == DT_F16 ? gated(TypeTag<OutF16>()) : gated(TypeTag<OutF32>());
 }
 
 template <int NT, int MT, bool EXPERTS> int launch_few(MxParams p, int64_t row_tiles, hipStream_t stream) {
@@ -499,10 +538,10 @@ template <bool EXPERTS> int launch(const MxParams& p, hipStream_t stream) {
   if (each <= 32 && tiles(32) <= 65535) return launch_few<2, 2, EXPERTS>(p, tiles(32), stream);
   if (each <= 64 && tiles(64) <= 65535) return launch_few<2, 4, EXPERTS>(p, tiles(64), stream);
   const int64_t big = tiles(256) * ((p.n + 255) / 256);
-  if (big >= 200) return launch_tile<256, 256, EXPERTS>(p, tiles(256), stream);
+  if (big >= 200) return launch_tile<MxTile<256, 256, 4, 2>, EXPERTS>(p, tiles(256), stream);
   const int64_t mid = tiles(128) * ((p.n + 127) / 128);
-  if (mid >= 256) return launch_tile<128, 128, EXPERTS>(p, tiles(128), stream);
-  return launch_tile<64, 64, EXPERTS>(p, tiles(64), stream);
+  if (mid >= 256) return launch_tile<MxTile<128, 128, 2, 2>, EXPERTS>(p, tiles(128), stream);
+  return launch_tile<MxTile<64, 64, 2, 2>, EXPERTS>(p, tiles(64), stream);
 }
 
 }  // namespace

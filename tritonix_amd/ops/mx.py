@@ -90,7 +90,7 @@ class MXTensor:
         slabs = -(-k // SLAB)
         count = 1 if batch is None else batch
         code_bytes = count * rows * slabs * (SLAB // 2)
-        scale_bytes = count * (-(-rows // 32)) * slabs * 32 * (SLAB // BLOCK)
+        scale_bytes = count * (-(-rows // 32)) * (-(-slabs // 2)) * 32 * 2 * (SLAB // BLOCK)
         return MXTensor(torch.empty(code_bytes + scale_bytes, dtype=torch.uint8, device=device), batch, rows, k, dim, code_bytes)
 
     @staticmethod
