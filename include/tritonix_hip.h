@@ -366,6 +366,9 @@ int tnx_mx_dequantize(const tnx_mx_args* args);
 int tnx_mx_import(const void* codes, const void* scales, int64_t batch, int64_t rows, int64_t k, void* out_codes, void* out_scales,
                   void* stream);
 
+/* one or two rows of a (k up to 30720) may be given as floats in a_data, with a_codes and a_scales null: the kernel quantises them itself */
+int tnx_mx_gemm_takes_rows(int64_t a_rows, int64_t k);
+
 /* Products of two such tensors, both quantised along the k they are multiplied over: out[m, n] = a[m, k] . b[n, k], 32-bit
  * sums, rounded once.  With a GLU epilogue n is the interleaved width (even rows of b are the gate) and out has n / 2 columns.
  *
@@ -375,15 +378,19 @@ int tnx_mx_import(const void* codes, const void* scales, int64_t batch, int64_t 
  * as the nearest row inside.  Rows from offsets[experts] on are written as zeros. */
 typedef struct tnx_mx_gemm_args {
   const void *a_codes, *a_scales, *b_codes, *b_scales;
+  const void* a_data;        /* see tnx_mx_gemm_takes_rows; otherwise null */
   void* out;
   int64_t m, n, k;
   int64_t a_rows;            /* rows that a has: m, or the tokens that order chooses from */
+  int64_t stride_a;          /* elements from row to row of a_data (columns are neighbours) */
   int64_t stride_out;        /* elements from row to row of out (columns are neighbours) */
   const int32_t* offsets;
   const int32_t* order;
   int32_t experts, top_k;
   int32_t out_dtype;         /* TNX_F16, TNX_BF16 or TNX_F32 */
   int32_t epilogue;          /* tnx_epilogue */
+  int32_t a_dtype;           /* of a_data: TNX_F16, TNX_BF16 or TNX_F32 */
+  int32_t reserved;
   void* stream;
 } tnx_mx_gemm_args;
 

@@ -124,7 +124,7 @@ def check_product(out, a, b, dtype, k):
 
 
 SIZES = [(1, 16, 32), (1, 1, 1), (3, 17, 31), (16, 64, 256), (17, 100, 300), (33, 130, 600), (64, 64, 64), (65, 257, 513), (100, 300, 1000),
-         (200, 2000, 260), (257, 259, 2049), (1, 4096, 2048), (1000, 520, 777), (300, 4100, 512), (2049, 2100, 256), (3600, 3700, 300)]
+         (200, 2000, 260), (257, 259, 2049), (1, 4096, 2048), (2, 300, 1000), (1, 130, 30720), (2, 70, 31000), (1, 20, 70000), (40, 50, 9000), (1000, 520, 777), (300, 4100, 512), (2049, 2100, 256), (3600, 3700, 300)]
 
 
 @pytest.mark.parametrize("size", SIZES, ids=str)
@@ -165,6 +165,16 @@ def test_a_nan_block_reaches_its_row_or_column_only(device, m):
     want[1] = True
     want[:, 50] = True
     assert torch.equal(bad, want)
+
+
+def test_two_rows_of_a_wider_tensor(device):
+    """Rows that the kernel quantises itself, with a stride and an odd start."""
+    base, w = make((4, 700), torch.float32, 5), make((600, 200), torch.bfloat16, 6)
+    q = tritonix.mx_quantize(w.to(device), dim=0)
+    for dtype in TYPES:
+        x = base.to(dtype)[1::2, 33:633]
+        out = tritonix.mx_matmul(base.to(dtype).to(device)[1::2, 33:633], q, torch.float32)
+        check_product(out, ref.values(x, -1), ref.values(w, -2), torch.float32, 600)
 
 
 def test_empty_sizes(device):

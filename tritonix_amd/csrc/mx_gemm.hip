@@ -26,6 +26,8 @@ struct MxParams {
   int experts, tiles_n, tiles_m;           // experts == 0: one matrix; tiles_m: of one matrix
   FastDiv top_k;
   int out_dtype, epi;
+  int64_t lda;                             // few rows as floats: their stride, type and k; parts of k (log2)
+  int a_dtype, k, wk_log;
 };
 
 __device__ __forceinline__ f32x16 mfma32(i32x4 a, i32x4 b, f32x16 c, int sa, int sb, int step) {
@@ -107,13 +109,21 @@ __device__ __forceinline__ int source_row(const MxParams& p, int r) {
   return t < p.a_rows ? t : p.a_rows - 1;
 }
 
+// act(g) * l.  The reciprocal is the instruction's own, good to a unit in the last place of 32 bits: the results are rounded from there.  (Its
+// corrected form and the division cost 256x128 gates of a tile 2 us more.)
+__device__ __forceinline__ float gated(float g, float l, int epi) {
+  if (epi == EPI_GLU_IDENTITY) return g * l;
+  const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+  return (epi == EPI_GLU_SILU ? g * s : s) * l;
+}
+
 // `count` of four neighbouring columns of a row (two with the gate), as many as there are
 __device__ __forceinline__ void store_columns(const MxParams& p, int64_t row, int col, int cols, const f32x4& v) {
   float o[4];
   int c = col, n = 4;
   if (p.epi != EPI_NONE) {
-    o[0] = glu_gate<true>(v[0], p.epi) * v[1];
-    o[1] = glu_gate<true>(v[2], p.epi) * v[3];
+    o[0] = gated(v[0], v[1], p.epi);
+    o[1] = gated(v[2], v[3], p.epi);
     o[2] = o[3] = 0.0f;
     c = col >> 1; n = 2; cols >>= 1;
   } else {
@@ -130,7 +140,7 @@ __device__ __forceinline__ void store_columns(const MxParams& p, int64_t row, in
 // filled by direct loads.  Slab s + 1 has to be there, and slab s be read by all, when the last step of slab s
 // begins: one barrier per slab, its wait hidden behind that step's products.
 template <int BN_, int BM_, int WGN, int WGM> struct MxTile {
-  static constexpr int BN = BN_, BM = BM_, NW = WGN * WGM, THREADS = NW * 64, WAVES_M = WGM;
+  static constexpr int BN = BN_, BM = BM_, NW = WGN * WGM, THREADS = NW * 64, WAVES_N = WGN;
   static constexpr int WTN = BN / WGN, WTM = BM / WGM, TN = WTN / 32, TM = WTM / 32;
   static constexpr int B_BYTES = BN * MX_ROWB, A_BYTES = BM * MX_ROWB;
   static constexpr int SLOT = B_BYTES + A_BYTES, S_BYTES = (BN + BM) * 2 * MX_SCALEB;      // codes of a slab; scales of two
@@ -177,7 +187,7 @@ __device__ __forceinline__ void store_product(const f32x16& v, uint8_t* out, int
   for (int q = 0; q < 4; q += 2) {
     float o[8];
 #pragma unroll
-    for (int e = 0; e < (GLU ? 4 : 8); ++e) o[e] = GLU ? glu_gate<true>(v[4 * q + 2 * e], epi) * v[4 * q + 2 * e + 1] : v[4 * q + e];
+    for (int e = 0; e < (GLU ? 4 : 8); ++e) o[e] = GLU ? gated(v[4 * q + 2 * e], v[4 * q + 2 * e + 1], epi) : v[4 * q + e];
     if constexpr (ES == 4) {
       constexpr int W = GLU ? 2 : 4;
 #pragma unroll
@@ -290,7 +300,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
     }
   };
 
-  const int wn = wave / C::WAVES_M * C::WTN, wm = wave % C::WAVES_M * C::WTM, half = lane >> 5, r32 = lane & 31;
+  const int wn = wave % C::WAVES_N * C::WTN, wm = wave / C::WAVES_N * C::WTM, half = lane >> 5, r32 = lane & 31;
   // place of chunk 4 half + step in this lane's row; the weights' and a's products further on are constants from here
   const uint32_t place = (uint32_t)r32 * MX_ROWB + (((4 * half) ^ ((r32 >> 1) & 7)) << 4);
   const uint32_t place_b = lds0 + place + wn * MX_ROWB, place_a = lds0 + place + C::B_BYTES + wm * MX_ROWB;
@@ -385,6 +395,22 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
   for (int i = 0; i < C::TN; ++i) { read_b(0, 0, i); read_sb(0, 0, i); }
 #pragma unroll
   for (int j = 0; j < C::TM; ++j) { read_a(0, 0, j); read_sa(0, j); }
+  if (wm >= rt.rows) {
+    // A wave without rows (an expert's last tile, mostly) does its share of the loads and keeps the barriers; the wave of the other half on
+    // its SIMD has the matrix unit to itself.
+    for (int s = 0; s < slabs - 1; ++s) {
+#pragma unroll
+      for (int q = FIRST_OPS; q < OPS; ++q) fetch_op(s + 1, q);
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (s + 2 < slabs) {
+#pragma unroll
+        for (int q = 0; q < FIRST_OPS; ++q) fetch_op(s + 2, q);
+      }
+    }
+    return;
+  }
   int s = 0;
   for (; s < slabs - 2; ++s) products(s, BoolTag<true>(), BoolTag<true>());
   if (s < slabs - 1) products(s++, BoolTag<true>(), BoolTag<false>());
@@ -410,77 +436,136 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Few rows: bound by streaming the weights, so nothing goes through LDS on the way in.  A workgroup has 16 NT rows of the
-// weights and up to 16 MT rows of a; its eight waves each take every eighth slab, all of a turn's loads in flight together, and meet in
-// LDS.  16x16x128 instructions: lane group g (lane / 16) takes the blocks 2 g and 2 g + 1 of a slab, 32 neighbouring bytes and
-// two neighbouring scales.
-constexpr int FEW_WAVES = 8;
+// Few rows: bound by streaming the weights, so nothing of them goes through LDS.  A wave has 16 NT rows of the weights and up to 16 MT rows of a; a
+// workgroup's eight waves are wk parts of k (slabs kpart, kpart + wk, ...) times 8 / wk groups of weight rows, and the parts meet in LDS.  All of
+// a turn's loads are in flight together.  16x16x128 instructions: lane group g (lane / 16) takes the blocks 2 g and 2 g + 1 of a slab, 32 neighbouring
+// bytes and two neighbouring scales.
+//
+// RAW: one or two rows of a, as 16- or 32-bit floats: every workgroup quantises them into LDS while its first weights are on
+// their way (one token: 14336 elements are 28 a thread), which saves a launch of 3 us and its gap.
+constexpr int FEW_WAVES = 8, FEW_RAW_ROWS = 2, FEW_RAW_LDS = 32768;
 
-template <int NT, int MT, bool EXPERTS>
+template <class T> __device__ __forceinline__ void quantize_to_lds(const MxParams& p, uint32_t codes, uint32_t scales, int tid) {
+  typedef typename Elem<T>::raw raw;
+  const int per_row = p.slabs * 32, items = p.a_rows * per_row;
+  for (int i0 = 0; i0 < items; i0 += FEW_WAVES * 64) {                    // (whole blocks of four lanes take each turn)
+    const int i = i0 + tid, row = i >= per_row ? 1 : 0, at = i - row * per_row;
+    if (i >= items) continue;
+    const int left = p.k - at * 8;
+    const raw* src = (const raw*)p.a + (int64_t)row * p.lda + (int64_t)at * 8;
+    Run8<T> x;
+    if (left >= 8) x = *(const Run8<T>*)src;
+    else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x.v[e] = e < left ? src[e] : (raw)0;
+    }
+    float v[8], factor;
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = Elem<T>::get(x.v[e]);
+      const uint32_t b = __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu;
+      top = top > b ? top : b;
+    }
+    const uint32_t s = scale_byte(quad_max(top), &factor);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = scaled(v[e], factor);
+    *TNX_LDS(uint32_t, codes + i * 4) = codes8(v);
+    if ((at & 3) == 0) *TNX_LDS(uint8_t, scales + (i >> 2)) = (uint8_t)s;      // (a block of padding: codes 0, any finite scale)
+  }
+}
+
+template <int NT, int MT, bool EXPERTS, bool RAW>
 __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
-  __shared__ __attribute__((aligned(16))) f32x4 part[FEW_WAVES][NT * MT][64];
+  extern __shared__ __attribute__((aligned(16))) uint8_t mx_smem[];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(uint8_t __attribute__((address_space(3)))*)mx_smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wk = 1 << p.wk_log, kpart = wave & (wk - 1);
+  const int n0 = (blockIdx.x * (FEW_WAVES >> p.wk_log) + (wave >> p.wk_log)) * (16 * NT);
   RowTile rt;
   if (EXPERTS) {
-    if (!find_rows<16 * MT>(p, blockIdx.y, lane, &rt)) return;
+    if (!find_rows<16 * MT>(p, blockIdx.y, lane, &rt)) return;            // (the same answer in every wave)
   } else {
     rt.expert = 0;
     rt.row0 = blockIdx.y * (16 * MT);
     rt.rows = p.m - rt.row0 < 16 * MT ? p.m - rt.row0 : 16 * MT;
   }
-  const int n0 = blockIdx.x * (16 * NT);
   const int row = lane & 15, g = lane >> 4;
+  const bool empty = EXPERTS && rt.expert == p.experts;
+  const uint32_t raw_scales = lds0 + FEW_RAW_ROWS * p.slabs * MX_ROWB;
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (!EXPERTS || rt.expert < p.experts) {
-    const uint8_t* b = p.b + (int64_t)rt.expert * p.b_expert;
-    const uint8_t* bs = p.bs + (int64_t)rt.expert * p.bs_expert;
-    const uint8_t *b_at[NT], *bs_at[NT], *a_at[MT], *as_at[MT];
-    bool a_have[MT];
+
+  constexpr int DEPTH = NT == 1 ? 8 : 4;                 // slabs of a turn
+  const uint8_t *b_at[NT], *bs_at[NT];
+  i32x4 fb[DEPTH][NT][2];
+  int sb[DEPTH][NT];
+  auto load_weights = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int64_t s = s0 + d * wk;
+      if (s < p.slabs) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          fb[d][i][0] = *(const i32x4*)(b_at[i] + s * MX_ROWB);
+          fb[d][i][1] = *(const i32x4*)(b_at[i] + s * MX_ROWB + 16);
+          sb[d][i] = *(const uint16_t*)(bs_at[i] + (s >> 1) * 512 + (s & 1) * 8);
+        }
+      }
+    }
+  };
+  if (!empty) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int n = n0 + 16 * i + row < p.n ? n0 + 16 * i + row : p.n - 1;
-      b_at[i] = b + (int64_t)n * p.slabs * MX_ROWB + 32 * g;
-      bs_at[i] = bs + mx_scale_at(n, 0, p.slabs) + 2 * g;
+      b_at[i] = p.b + (int64_t)rt.expert * p.b_expert + (int64_t)n * p.slabs * MX_ROWB + 32 * g;
+      bs_at[i] = p.bs + (int64_t)rt.expert * p.bs_expert + mx_scale_at(n, 0, p.slabs) + 2 * g;
     }
+    load_weights(kpart);
+  }
+  if (RAW) {
+    if (p.a_dtype == DT_BF16) quantize_to_lds<__bf16>(p, lds0, raw_scales, tid);
+    else if (p.a_dtype == DT_F16) quantize_to_lds<_Float16>(p, lds0, raw_scales, tid);
+    else quantize_to_lds<float>(p, lds0, raw_scales, tid);
+    __syncthreads();
+  }
+  if (!empty) {
+    const uint8_t *a_at[MT], *as_at[MT];
+    bool a_have[MT];
+    int src[MT];
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       a_have[j] = 16 * j + row < rt.rows;
-      const int src = EXPERTS ? source_row(p, rt.row0 + (a_have[j] ? 16 * j + row : 0)) : rt.row0 + (a_have[j] ? 16 * j + row : 0);
-      a_at[j] = p.a + (int64_t)src * p.slabs * MX_ROWB + 32 * g;
-      as_at[j] = p.as + mx_scale_at(src, 0, p.slabs) + 2 * g;
-    }
-    constexpr int DEPTH = 4;                             // slabs of a turn
-    for (int s0 = wave; s0 < p.slabs; s0 += FEW_WAVES * DEPTH) {
-      i32x4 fb[DEPTH][NT][2];
-      int sb[DEPTH][NT];
-#pragma unroll
-      for (int d = 0; d < DEPTH; ++d) {
-        const int64_t s = s0 + d * FEW_WAVES;
-        if (s < p.slabs) {
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            fb[d][i][0] = *(const i32x4*)(b_at[i] + s * MX_ROWB);
-            fb[d][i][1] = *(const i32x4*)(b_at[i] + s * MX_ROWB + 16);
-            sb[d][i] = *(const uint16_t*)(bs_at[i] + (s >> 1) * 512 + (s & 1) * 8);
-          }
-        }
+      const int r = rt.row0 + (a_have[j] ? 16 * j + row : 0);
+      src[j] = EXPERTS ? source_row(p, r) : r;
+      if (!RAW) {
+        a_at[j] = p.a + (int64_t)src[j] * p.slabs * MX_ROWB + 32 * g;
+        as_at[j] = p.as + mx_scale_at(src[j], 0, p.slabs) + 2 * g;
       }
+    }
+    for (int s0 = kpart;;) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
-        const int64_t s = s0 + d * FEW_WAVES;
+        const int64_t s = s0 + d * wk;
         if (s < p.slabs) {
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
             i32x4 fa0 = {0, 0, 0, 0}, fa1 = {0, 0, 0, 0};
             int sa = 0x7f7f;
             if (a_have[j]) {
-              fa0 = *(const i32x4*)(a_at[j] + s * MX_ROWB);
-              fa1 = *(const i32x4*)(a_at[j] + s * MX_ROWB + 16);
-              sa = *(const uint16_t*)(as_at[j] + (s >> 1) * 512 + (s & 1) * 8);
+              if (RAW) {
+                const uint32_t at = (uint32_t)(src[j] * p.slabs + s);
+                fa0 = *TNX_LDS(i32x4, lds0 + at * MX_ROWB + 32 * g);
+                fa1 = *TNX_LDS(i32x4, lds0 + at * MX_ROWB + 32 * g + 16);
+                sa = *TNX_LDS(uint16_t, raw_scales + at * MX_SCALEB + 2 * g);
+              } else {
+                fa0 = *(const i32x4*)(a_at[j] + s * MX_ROWB);
+                fa1 = *(const i32x4*)(a_at[j] + s * MX_ROWB + 16);
+                sa = *(const uint16_t*)(as_at[j] + (s >> 1) * 512 + (s & 1) * 8);
+              }
             }
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
@@ -490,21 +575,35 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
           }
         }
       }
+      s0 += wk * DEPTH;
+      if (s0 >= p.slabs) break;
+      load_weights(s0);
     }
   }
+  if (wk > 1) {
+    // part k of a group of weight rows beside the others': [wave][product][lane]
+    if (RAW) __syncthreads();                            // (the rows of a lie there)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) *TNX_LDS(f32x4, lds0 + ((wave * NT * MT + i * MT + j) * 64 + lane) * 16) = acc[i][j];
+    __syncthreads();
+  }
+  // with parts, product ij of the group is summed and stored by part ij % wk (in the order of the parts)
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) part[wave][i * MT + j][lane] = acc[i][j];
-  __syncthreads();
-  for (int t = tid; t < NT * MT * 64; t += FEW_WAVES * 64) {
-    const int ij = t >> 6, l = t & 63;
-    f32x4 v = part[0][ij][l];
-#pragma unroll
-    for (int w = 1; w < FEW_WAVES; ++w) v += part[w][ij][l];
-    const int r = 16 * (ij % MT) + (l & 15), c = n0 + 16 * (ij / MT) + 4 * (l >> 4);
-    if (r < rt.rows && c < p.n) store_columns(p, rt.row0 + r, c, p.n, v);
-  }
+    for (int j = 0; j < MT; ++j) {
+      if (((i * MT + j) & (wk - 1)) != kpart) continue;
+      f32x4 v = acc[i][j];
+      if (wk > 1) {
+        const int w0 = wave - kpart;
+        v = *TNX_LDS(f32x4, lds0 + ((w0 * NT * MT + i * MT + j) * 64 + lane) * 16);
+        for (int w = 1; w < wk; ++w) v += *TNX_LDS(f32x4, lds0 + (((w0 + w) * NT * MT + i * MT + j) * 64 + lane) * 16);
+      }
+      const int r = 16 * j + row, c = n0 + 16 * i + 4 * g;
+      if (r < rt.rows && c < p.n) store_columns(p, rt.row0 + r, c, p.n, v);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -523,20 +622,28 @@ template <class C, bool EXPERTS> int launch_tile(MxParams p, int64_t row_tiles, 
   return p.out_dtype == DT_F16 ? gated(TypeTag<OutF16>()) : gated(TypeTag<OutF32>());
 }
 
-template <int NT, int MT, bool EXPERTS> int launch_few(MxParams p, int64_t row_tiles, hipStream_t stream) {
-  if (row_tiles > 65535) return TNX_E_UNSUPPORTED;
-  hipLaunchKernelGGL((mx_few_kernel<NT, MT, EXPERTS>), dim3((unsigned)((p.n + 16 * NT - 1) / (16 * NT)), (unsigned)row_tiles), dim3(FEW_WAVES * 64), 0,
-                     stream, p);
+template <int NT, int MT, bool EXPERTS, bool RAW> int launch_few(MxParams p, int64_t row_tiles, hipStream_t stream) {
+  // as few parts of k as give every SIMD two waves: a part less is a sum less, and its wave has more loads in flight
+  const int64_t groups = (p.n + 16 * NT - 1) / (16 * NT);
+  p.wk_log = 0;
+  while (p.wk_log < 3 && (2 << p.wk_log) <= p.slabs && (groups * row_tiles << p.wk_log) < 2048) ++p.wk_log;
+  const int64_t per = FEW_WAVES >> p.wk_log;
+  size_t lds = p.wk_log ? (size_t)FEW_WAVES * NT * MT * 1024 : 0;
+  const size_t raw = RAW ? (size_t)FEW_RAW_ROWS * p.slabs * (MX_ROWB + MX_SCALEB) : 0;
+  if (raw > lds) lds = raw;
+  hipLaunchKernelGGL((mx_few_kernel<NT, MT, EXPERTS, RAW>), dim3((unsigned)((groups + per - 1) / per), (unsigned)row_tiles), dim3(FEW_WAVES * 64), lds, stream, p);
   return mx_launched();
 }
 
-template <bool EXPERTS> int launch(const MxParams& p, hipStream_t stream) {
+template <bool EXPERTS> int launch(const MxParams& p, bool raw, hipStream_t stream) {
   // rows that a workgroup can expect, and how many tiles of BM there are at most
   const int64_t each = EXPERTS ? (p.m + p.experts - 1) / p.experts : p.m;
   auto tiles = [&](int bm) { return EXPERTS ? (int64_t)p.m / bm + 1 + (p.experts < p.m ? p.experts : p.m) : ((int64_t)p.m + bm - 1) / bm; };
-  if (each <= 16 && tiles(16) <= 65535) return launch_few<1, 1, EXPERTS>(p, tiles(16), stream);
-  if (each <= 32 && tiles(32) <= 65535) return launch_few<2, 2, EXPERTS>(p, tiles(32), stream);
-  if (each <= 64 && tiles(64) <= 65535) return launch_few<2, 4, EXPERTS>(p, tiles(64), stream);
+  if (raw) return tiles(16) <= 65535 ? launch_few<1, 1, EXPERTS, true>(p, tiles(16), stream) : TNX_E_UNSUPPORTED;
+  // (experts' rows are uneven: an expert with more than a tile's reads its weights again, from the L2 mostly)
+  if (each <= (EXPERTS ? 4 : 16) && tiles(16) <= 65535) return launch_few<1, 1, EXPERTS, false>(p, tiles(16), stream);
+  if (each <= (EXPERTS ? 16 : 32) && tiles(32) <= 65535) return launch_few<1, 2, EXPERTS, false>(p, tiles(32), stream);
+  if (each <= (EXPERTS ? 40 : 64) && tiles(64) <= 65535) return launch_few<2, 4, EXPERTS, false>(p, tiles(64), stream);
   const int64_t big = tiles(256) * ((p.n + 255) / 256);
   if (big >= 200) return launch_tile<MxTile<256, 256, 4, 2>, EXPERTS>(p, tiles(256), stream);
   const int64_t mid = tiles(128) * ((p.n + 127) / 128);
@@ -544,7 +651,11 @@ template <bool EXPERTS> int launch(const MxParams& p, hipStream_t stream) {
   return launch_tile<MxTile<64, 64, 2, 2>, EXPERTS>(p, tiles(64), stream);
 }
 
+bool takes_rows(int64_t a_rows, int64_t k) { return a_rows <= FEW_RAW_ROWS && FEW_RAW_ROWS * mx_slabs(k) * (MX_ROWB + MX_SCALEB) <= FEW_RAW_LDS; }
+
 }  // namespace
+
+extern "C" int tnx_mx_gemm_takes_rows(int64_t a_rows, int64_t k) { return a_rows > 0 && k > 0 && takes_rows(a_rows, k); }
 
 extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
   if (!a || a->m < 0 || a->n < 0 || a->k < 0 || a->experts < 0 || a->epilogue < TNX_EPI_NONE || a->epilogue > TNX_EPI_GLU_IDENTITY) return TNX_E_INVALID;
@@ -554,12 +665,18 @@ extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
   const int64_t cols = a->epilogue != TNX_EPI_NONE ? a->n / 2 : a->n;
   if (!a->out || a->stride_out < cols || ((uintptr_t)a->out & (a->out_dtype == TNX_F32 ? 3 : 1))) return TNX_E_INVALID;
   if (a->k == 0 || a->k > TNX_MX_MAX_K || a->m > 0x3fffffff || a->n > 0x3fffffff || a->a_rows > 0x3fffffff) return TNX_E_UNSUPPORTED;
-  if (!a->a_codes || !a->a_scales || !a->b_codes || !a->b_scales) return TNX_E_INVALID;
-  if (((uintptr_t)a->a_codes | (uintptr_t)a->a_scales | (uintptr_t)a->b_codes | (uintptr_t)a->b_scales) & 15) return TNX_E_INVALID;
+  const bool raw = a->a_data != nullptr;
+  if (!a->b_codes || !a->b_scales || (((uintptr_t)a->b_codes | (uintptr_t)a->b_scales) & 15)) return TNX_E_INVALID;
+  if (raw) {
+    if (a->a_codes || a->a_scales) return TNX_E_INVALID;
+    if (a->a_dtype != TNX_BF16 && a->a_dtype != TNX_F16 && a->a_dtype != TNX_F32) return TNX_E_UNSUPPORTED;
+    if ((uintptr_t)a->a_data & (a->a_dtype == TNX_F32 ? 3 : 1)) return TNX_E_INVALID;
+    if (!takes_rows(a->a_rows, a->k)) return TNX_E_UNSUPPORTED;
+  } else if (!a->a_codes || !a->a_scales || (((uintptr_t)a->a_codes | (uintptr_t)a->a_scales) & 15)) return TNX_E_INVALID;
   if (a->experts > 0 ? (!a->offsets || a->experts > TNX_MOE_MAX_EXPERTS) : (a->offsets || a->order)) return TNX_E_INVALID;
   if (a->order ? (a->top_k < 1 || a->a_rows < 1) : a->a_rows != a->m) return TNX_E_INVALID;
   MxParams p;
-  p.a = (const uint8_t*)a->a_codes; p.as = (const uint8_t*)a->a_scales;
+  p.a = (const uint8_t*)(raw ? a->a_data : a->a_codes); p.as = (const uint8_t*)a->a_scales;
   p.b = (const uint8_t*)a->b_codes; p.bs = (const uint8_t*)a->b_scales;
   p.out = (uint8_t*)a->out;
   p.offsets = a->offsets; p.order = a->order;
@@ -570,5 +687,6 @@ extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
   p.experts = a->experts; p.tiles_n = p.tiles_m = 0;
   p.top_k = make_fastdiv((uint32_t)(a->order ? a->top_k : 1));
   p.out_dtype = a->out_dtype; p.epi = a->epilogue;
-  return a->experts > 0 ? launch<true>(p, (hipStream_t)a->stream) : launch<false>(p, (hipStream_t)a->stream);
+  p.a_dtype = a->a_dtype; p.lda = a->stride_a; p.k = (int)a->k; p.wk_log = 0;
+  return a->experts > 0 ? launch<true>(p, raw, (hipStream_t)a->stream) : launch<false>(p, raw, (hipStream_t)a->stream);
 }

@@ -20,63 +20,12 @@ using namespace tnx;
 
 namespace {
 
-template <class T> struct Elem;
-template <> struct Elem<float> {
-  static __device__ __forceinline__ float get(uint32_t v) { return __builtin_bit_cast(float, v); }
-  typedef uint32_t raw;
-  static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(uint32_t, v); }
-};
-template <> struct Elem<__bf16> {
-  typedef uint16_t raw;
-  static __device__ __forceinline__ float get(raw v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
-  static __device__ __forceinline__ raw put(float v) { return f32_to_bf16(v); }
-};
-template <> struct Elem<_Float16> {
-  typedef uint16_t raw;
-  static __device__ __forceinline__ float get(raw v) { return (float)__builtin_bit_cast(_Float16, v); }
-  static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
-};
-
-// scale byte of a block whose largest magnitude has the bits `top` (an integer maximum orders magnitudes, infinities and
-// NaNs last), and the factor 2^-e (0 for a block without finite values: its codes are zero)
-__device__ __forceinline__ uint32_t scale_byte(uint32_t top, float* factor) {
-  const int exponent = (int)(top >> 23);                 // biased; 0: zero or subnormal, below 2^-126: e is -127 there
-  if (exponent == 255) { *factor = 0.0f; return 255; }
-  const int s = exponent > 2 ? exponent - 2 : 0;         // e + 127
-  *factor = __builtin_bit_cast(float, (uint32_t)(254 - s) << 23);      // s <= 252: a normal number
-  return (uint32_t)s;
-}
-
-__device__ __forceinline__ float scale_value(uint32_t s) {
-  return __builtin_bit_cast(float, s == 255 ? 0x7fc00000u : s == 0 ? 0x00400000u : s << 23);
-}
-
-// eight values already divided by the scale -> eight codes; the first in the low bits
-__device__ __forceinline__ uint32_t codes8(const float* v) {
-  uint32_t r = 0;
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], 1.0f, 0);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], 1.0f, 1);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], 1.0f, 2);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], 1.0f, 3);
-  return r;
-}
-
-// an element times the block's factor; in a block without finite values everything becomes 0
-__device__ __forceinline__ float scaled(float x, float factor) { return factor == 0.0f ? 0.0f : x * factor; }
-
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void values8(uint32_t c, float scale, float* v) {
   const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
   const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
   v[0] = a.x * scale; v[1] = a.y * scale; v[2] = b.x * scale; v[3] = b.y * scale;
   v[4] = d.x * scale; v[5] = d.y * scale; v[6] = f.x * scale; v[7] = f.y * scale;
-}
-
-__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
-  const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);      // lane ^ 1
-  v = v > a ? v : a;
-  const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true);      // lane ^ 2
-  return v > b ? v : b;
 }
 
 struct QuantParams {
@@ -89,7 +38,6 @@ struct QuantParams {
 
 constexpr int ROW_ITEMS = 4;                             // runs of 8 elements a lane takes, 256 lanes apart
 
-template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Run8 { typename Elem<T>::raw v[8]; };
 
 template <class T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantParams p) {

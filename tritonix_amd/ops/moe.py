@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from tritonix_amd import _C
-from tritonix_amd.ops.mx import MXTensor, dtype_code, epilogue_of, gemm_args, launch, on_device, operand, raise_for_status
+from tritonix_amd.ops.mx import MXTensor, dtype_code, epilogue_of, gemm_args, launch, on_device, operand, raise_for_status, takes_rows
 from tritonix_amd.kernel import _stream_of
 
 __all__ = ["Routing", "moe_route", "moe_route_backward", "moe_plan", "moe_glu", "moe_down", "moe_ffn"]
@@ -210,7 +210,7 @@ def _check_experts(name: str, x, w, routing: Routing, rows: int) -> None:
         raise ValueError(f"{name} expects [{rows}, {w.k}] rows, got {tuple(x.shape)}")
 
 
-def _grouped(name: str, x: MXTensor, w: MXTensor, routing: Routing, out: torch.Tensor, gather: bool, epilogue: int, index: int) -> None:
+def _grouped(name: str, x, w: MXTensor, routing: Routing, out: torch.Tensor, gather: bool, epilogue: int, index: int) -> None:
     g = gemm_args(x, w, out, epilogue)
     g.experts, g.offsets, g.top_k = routing.num_experts, routing.offsets.data_ptr(), routing.top_k
     if gather:
@@ -228,8 +228,8 @@ def moe_glu(x, w12: MXTensor, routing: Routing, activation: str = "silu", out_dt
         out_dtype = torch.bfloat16 if isinstance(x, MXTensor) else x.dtype
     dtype_code("moe_glu", out_dtype)
     index = on_device("moe_glu", x, w12, routing.order)
-    xq = operand("moe_glu", "x", x, -1)
-    out = torch.empty((routing.tokens * routing.top_k, w12.rows // 2), dtype=out_dtype, device=xq.device)
+    xq = x if takes_rows(x) else operand("moe_glu", "x", x, -1)
+    out = torch.empty((routing.tokens * routing.top_k, w12.rows // 2), dtype=out_dtype, device=w12.device)
     _grouped("moe_glu", xq, w12, routing, out, True, epilogue_of(activation), index)
     return out
 
@@ -244,11 +244,11 @@ def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
         out_dtype = torch.bfloat16 if isinstance(h, MXTensor) else h.dtype
     code = dtype_code("moe_down", out_dtype)
     index = on_device("moe_down", h, w3, routing.order)
-    hq = operand("moe_down", "h", h, -1)
+    hq = h if takes_rows(h) else operand("moe_down", "h", h, -1)
     n = w3.rows
-    y = torch.empty((routing.tokens * routing.top_k, n), dtype=out_dtype, device=hq.device)
+    y = torch.empty((routing.tokens * routing.top_k, n), dtype=out_dtype, device=w3.device)
     _grouped("moe_down", hq, w3, routing, y, False, _C.EPI_NONE, index)
-    out = torch.empty((routing.tokens, n), dtype=out_dtype, device=hq.device)
+    out = torch.empty((routing.tokens, n), dtype=out_dtype, device=w3.device)
     with torch.cuda.device(index):
         status = _C.load().tnx_moe_combine(y.data_ptr(), routing.rows.data_ptr(), routing.weights.data_ptr(), out.data_ptr(), routing.tokens,
                                            routing.top_k, n, code, code, _stream_of(index))

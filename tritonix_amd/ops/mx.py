@@ -206,11 +206,21 @@ def operand(name: str, side: str, x, dim: int) -> MXTensor:
     return mx_quantize(x, dim=dim)
 
 
-def gemm_args(a: MXTensor, b: MXTensor, out: torch.Tensor, epilogue: int) -> _C.MxGemmArgs:
+def takes_rows(x) -> bool:
+    """Whether a product takes these rows as they are: one or two rows of floats are quantised by the kernel itself."""
+    return (not isinstance(x, MXTensor) and 0 < x.shape[0] <= 2 and (x.stride(1) == 1 or x.shape[1] == 1) and x.dtype in _DTYPES
+            and bool(_C.load().tnx_mx_gemm_takes_rows(x.shape[0], x.shape[1])))
+
+
+def gemm_args(a, b: MXTensor, out: torch.Tensor, epilogue: int) -> _C.MxGemmArgs:
     g = _C.MxGemmArgs()
-    g.a_codes, g.a_scales, g.b_codes, g.b_scales = a.codes_ptr, a.scales_ptr, b.codes_ptr, b.scales_ptr
+    if isinstance(a, MXTensor):
+        g.a_codes, g.a_scales, g.a_rows = a.codes_ptr, a.scales_ptr, a.rows
+    else:
+        g.a_data, g.a_dtype, g.stride_a, g.a_rows = a.data_ptr(), _DTYPES[a.dtype], a.stride(0), a.shape[0]
+    g.b_codes, g.b_scales = b.codes_ptr, b.scales_ptr
     g.out = out.data_ptr()
-    g.m, g.n, g.k, g.a_rows = out.shape[0], b.rows, b.k, a.rows
+    g.m, g.n, g.k = out.shape[0], b.rows, b.k
     g.stride_out = out.stride(0)
     g.out_dtype, g.epilogue = _DTYPES[out.dtype], epilogue
     return g
@@ -223,15 +233,18 @@ def _product(name: str, a, b, out_dtype, epilogue: int) -> torch.Tensor:
         out_dtype = torch.bfloat16 if isinstance(a, MXTensor) else a.dtype
     dtype_code(name, out_dtype)
     index = on_device(name, a, b)
-    a, b = operand(name, "a", a, -1), operand(name, "b", b, -2)
+    m, k = a.shape
+    if not takes_rows(a):
+        a = operand(name, "a", a, -1)
+    b = operand(name, "b", b, -2)
     n = b.rows
     if epilogue != _C.EPI_NONE:
         if n % 2:
             raise ValueError("the interleaved weight must have an even number of columns")
         n //= 2
-    if a.k == 0:
-        return torch.zeros((a.rows, n), dtype=out_dtype, device=a.device)
-    out = torch.empty((a.rows, n), dtype=out_dtype, device=a.device)
+    if k == 0:
+        return torch.zeros((m, n), dtype=out_dtype, device=b.device)
+    out = torch.empty((m, n), dtype=out_dtype, device=b.device)
     launch(name, index, _C.load().tnx_mx_gemm, gemm_args(a, b, out, epilogue))
     return out
 
