@@ -39,7 +39,9 @@ def test_buffer_sizes():
     t = tritonix.MXTensor.empty(3, 33, 257, -2, "cpu")
     assert t.code_bytes == 3 * lib.tnx_mx_code_bytes(33, 257) and t.buffer.numel() - t.code_bytes == 3 * lib.tnx_mx_scale_bytes(33, 257)
     assert t.shape == (3, 257, 33) and t.t().shape == (3, 33, 257) and t.t().t().shape == t.shape
-    assert lib.tnx_moe_workspace_bytes(64, 8, 16) == 0 and lib.tnx_moe_workspace_bytes(65, 8, 16) == 16 * 2 * 4 + 16 * 4
+    # up to four tokens one workgroup does it all; then a count per block (four tokens, later 32) and expert, and a total per expert
+    assert lib.tnx_moe_workspace_bytes(4, 8, 16) == 0 and lib.tnx_moe_workspace_bytes(5, 8, 16) == 16 * 2 * 4 + 16 * 4
+    assert lib.tnx_moe_workspace_bytes(65536, 8, 128) == 2048 * 128 * 4 + 128 * 4
 
 
 def mx(**kw):
@@ -104,7 +106,7 @@ def moe(**kw):
     (dict(tokens=-1), _C.E_INVALID), (dict(top_k=0), _C.E_INVALID), (dict(top_k=9), _C.E_INVALID), (dict(num_experts=2000), _C.E_UNSUPPORTED),
     (dict(num_experts=64, top_k=40), _C.E_UNSUPPORTED), (dict(dtype=_C.I8), _C.E_UNSUPPORTED), (dict(scoring=2), _C.E_INVALID),
     (dict(num_groups=3), _C.E_INVALID), (dict(num_groups=4, top_groups=5), _C.E_INVALID), (dict(group_top=3), _C.E_INVALID),
-    (dict(tokens=1 << 30), _C.E_UNSUPPORTED), (dict(tokens=1000), _C.E_WORKSPACE), (dict(tokens=1000, workspace=256, workspace_bytes=16), _C.E_WORKSPACE),
+    (dict(tokens=1 << 30), _C.E_UNSUPPORTED), (dict(tokens=5), _C.E_WORKSPACE), (dict(tokens=1000, workspace=256, workspace_bytes=16), _C.E_WORKSPACE),
     (dict(logits=257), _C.E_INVALID)])
 def test_routing_refuses(change, status):
     lib = _C.load()

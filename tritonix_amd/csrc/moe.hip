@@ -19,6 +19,8 @@ struct RouteParams {
   int64_t tokens, stride;
   int e, k, dtype, scoring, groups, top_groups, group_top, renorm, group_size;
   float scale;
+  int runs_at;                             // bytes of LDS before the runs of keys
+  bool vec, vec_out;                       // rows of the logits (of their gradient) in aligned runs of four
 };
 
 struct PlanParams {
@@ -26,7 +28,8 @@ struct PlanParams {
   int32_t *offsets, *order, *rows;
   int32_t *counts, *totals;                // workspace: [experts][blocks] and [experts]
   int64_t pairs;
-  int e, blocks;
+  int e, block, blocks, words;             // pairs of a block, blocks, 64-bit words of a block's bits
+  bool fused;                              // the routing kernel's workgroups are the blocks, and count
 };
 
 __device__ __forceinline__ float load_logit(const uint8_t* p, int64_t i, int dtype) {
@@ -35,15 +38,22 @@ __device__ __forceinline__ float load_logit(const uint8_t* p, int64_t i, int dty
   return dtype == DT_BF16 ? __builtin_bit_cast(float, (uint32_t)v << 16) : (float)__builtin_bit_cast(_Float16, v);
 }
 
-// the value of lane ^ D (D a power of two up to 32) as every group of 2 D lanes needs it for a sum or maximum that all
-// its lanes end up with: D = 4 and 8 mirror instead, which is the same once the smaller groups agree
+// The value of lane ^ D for sums and maxima that every lane of a group of 2 D ends up with: D = 4 and 8 mirror instead, which is
+// the same once the smaller groups agree.  All without LDS: these are the steps of latency in the choice.
 template <int D> __device__ __forceinline__ int lane_xor(int v) {
   if constexpr (D == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);
   else if constexpr (D == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);
   else if constexpr (D == 4) return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true);      // mirror of 8
   else if constexpr (D == 8) return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, true);      // mirror of 16
-  else return __shfl_xor(v, D);
+  else if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);       // even rows twice, odd rows twice
+    return (int)(threadIdx.x & 16 ? r[0] : r[1]);
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+    return (int)(threadIdx.x & 32 ? r[0] : r[1]);
+  }
 }
+template <int D> __device__ __forceinline__ float lane_xor(float v) { return __builtin_bit_cast(float, lane_xor<D>(__builtin_bit_cast(int, v))); }
 template <int L, class F> __device__ __forceinline__ void over_lanes(F f) {
   if constexpr (L > 1) f(IntTag<1>());
   if constexpr (L > 2) f(IntTag<2>());
@@ -53,54 +63,79 @@ template <int L, class F> __device__ __forceinline__ void over_lanes(F f) {
   if constexpr (L > 32) f(IntTag<32>());
 }
 template <int L> __device__ __forceinline__ float lanes_max(float v) {
-  over_lanes<L>([&](auto d) { v = __builtin_fmaxf(v, __builtin_bit_cast(float, lane_xor<decltype(d)::value>(__builtin_bit_cast(int, v)))); });
+  over_lanes<L>([&](auto d) { v = __builtin_fmaxf(v, lane_xor<decltype(d)::value>(v)); });
   return v;
 }
 template <int L> __device__ __forceinline__ float lanes_sum(float v) {
-  over_lanes<L>([&](auto d) { v += __builtin_bit_cast(float, lane_xor<decltype(d)::value>(__builtin_bit_cast(int, v))); });
+  over_lanes<L>([&](auto d) { v += lane_xor<decltype(d)::value>(v); });
   return v;
 }
-template <int L> __device__ __forceinline__ bool lanes_any(bool v) {
-  int x = v;
-  over_lanes<L>([&](auto d) { x |= lane_xor<decltype(d)::value>(x); });
-  return x != 0;
+template <int L> __device__ __forceinline__ int lanes_min(int v) {
+  over_lanes<L>([&](auto d) {
+    const int o = lane_xor<decltype(d)::value>(v);
+    v = o < v ? o : v;
+  });
+  return v;
+}
+template <int L> __device__ __forceinline__ int lanes_or(int v) {
+  over_lanes<L>([&](auto d) { v |= lane_xor<decltype(d)::value>(v); });
+  return v;
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
 
-constexpr int PLAN_PAIRS = 512;            // pairs of token and slot a workgroup of 256 threads places
+// Expert i of lane j where L lanes hold a row: four neighbours a lane, so that a load or store is 16 bytes.
+template <int L> __device__ __forceinline__ int expert_of(int i, int j) { return (i >> 2) * (4 * L) + 4 * j + (i & 3); }
 
-// The places of PLAN_PAIRS pairs among their experts, without atomics whose order could show: a bit per pair and expert
+// a row of logits; past the end -inf.  vec: four neighbours in one load
+template <int L, int EPL> __device__ __forceinline__ void load_row(const uint8_t* row, int e_count, int dtype, bool vec, int j, float (&l)[EPL]) {
+#pragma unroll
+  for (int i = 0; i < EPL; i += 4) {
+    const int e = expert_of<L>(i, j);
+    if (vec) {
+      if (e < e_count) {
+        if (dtype == DT_F32) {
+          const f32x4 v = *(const f32x4*)((const float*)row + e);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) l[i + x] = v[x];
+        } else {
+          typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+          const u16x4 v = *(const u16x4*)((const uint16_t*)row + e);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) l[i + x] = dtype == DT_BF16 ? Elem<__bf16>::get(v[x]) : Elem<_Float16>::get(v[x]);
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) l[i + x] = -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) l[i + x] = e + x < e_count ? load_logit(row, e + x, dtype) : -INFINITY;
+    }
+  }
+}
+
+// Places of pairs among their experts, without atomics whose order could show: a bit per pair of a block and expert
 // (setting bits commutes); a pair's rank is the number of bits below its own.
 struct PairBits {
-  unsigned long long* words;               // [experts][PLAN_PAIRS / 64]
+  unsigned long long* words;               // [experts][n]
+  int n;
   __device__ __forceinline__ int rank(int e, int i) const {
-    const unsigned long long* w = words + e * (PLAN_PAIRS / 64);
+    const unsigned long long* w = words + e * n;
     int r = 0;
     for (int q = 0; q < i / 64; ++q) r += __popcll(w[q]);
     return r + __popcll(w[i / 64] & ((1ull << (i & 63)) - 1));
   }
   __device__ __forceinline__ int count(int e) const {
     int r = 0;
-#pragma unroll
-    for (int q = 0; q < PLAN_PAIRS / 64; ++q) r += __popcll(words[e * (PLAN_PAIRS / 64) + q]);
+    for (int q = 0; q < n; ++q) r += __popcll(words[e * n + q]);
     return r;
   }
-};
-
-// the experts of a block's pairs into bits; expert[] of this thread's pairs (-1: none)
-__device__ __forceinline__ void mark_pairs(const PlanParams& p, int64_t first, const PairBits& bits, int tid, int (&expert)[PLAN_PAIRS / 256]) {
-  for (int i = tid; i < p.e * (PLAN_PAIRS / 64); i += 256) bits.words[i] = 0;
-  __syncthreads();
-#pragma unroll
-  for (int u = 0; u < PLAN_PAIRS / 256; ++u) {
-    const int i = u * 256 + tid;
-    expert[u] = first + i < p.pairs ? p.experts[first + i] : -1;
-    if (expert[u] < 0 || expert[u] >= p.e) expert[u] = -1;
-    else atomicOr(bits.words + expert[u] * (PLAN_PAIRS / 64) + (i >> 6), 1ull << (i & 63));
+  __device__ __forceinline__ void clear(int e_count, int tid) const {
+    for (int i = tid; i < e_count * n; i += 256) words[i] = 0;
   }
-  __syncthreads();
-}
+  __device__ __forceinline__ void mark(int e, int i) const { atomicOr(words + e * n + (i >> 6), 1ull << (i & 63)); }
+};
 
 // exclusive sums of n values in LDS (n <= TNX_MOE_MAX_EXPERTS) over a workgroup of 256 threads; returns the whole sum
 __device__ __forceinline__ int scan_experts(int* v, int n, int tid) {
@@ -138,58 +173,58 @@ __device__ __forceinline__ int scan_experts(int* v, int n, int tid) {
   return total;
 }
 
-// all of the plan of at most PLAN_PAIRS pairs, by one workgroup.  smem: the pairs' bits, then an int per expert
-__device__ __forceinline__ void plan_alone(const PlanParams& p, uint8_t* smem, int tid) {
-  const PairBits bits{(unsigned long long*)smem};
-  int* base = (int*)(smem + (size_t)p.e * PLAN_PAIRS / 8);
-  int expert[PLAN_PAIRS / 256];
-  mark_pairs(p, 0, bits, tid, expert);
-  for (int e = tid; e < p.e; e += 256) base[e] = bits.count(e);
-  __syncthreads();
-  const int total = scan_experts(base, p.e, tid);
-  for (int e = tid; e <= p.e; e += 256) p.offsets[e] = e < p.e ? base[e] : total;
-#pragma unroll
-  for (int u = 0; u < PLAN_PAIRS / 256; ++u) {
-    const int i = u * 256 + tid;
-    if (i >= p.pairs) continue;
-    if (expert[u] >= 0) {
-      const int at = base[expert[u]] + bits.rank(expert[u], i);
-      p.order[at] = i;
-      p.rows[i] = at;
-    } else p.rows[i] = -1;
-    if (i >= total) p.order[i] = -1;
+// All of a plan of at most PLAN_ALONE pairs by one workgroup, from the experts in LDS (ids, -1: none).  A pair's place is the number of pairs
+// before it: counted one by one, which for so few is quicker than sums over the experts.
+constexpr int PLAN_ALONE = 128;
+__device__ __forceinline__ void plan_alone(const PlanParams& p, const int* ids, int tid) {
+  const int pairs = (int)p.pairs;
+  if (tid < pairs) {
+    const int mine = ids[tid];
+    int at = 0, total = 0;
+    for (int i = 0; i < pairs; ++i) {
+      const int e = ids[i];
+      total += e >= 0;
+      at += e >= 0 && (e < mine || (e == mine && i < tid));
+    }
+    p.rows[tid] = mine >= 0 ? at : -1;
+    if (mine >= 0) p.order[at] = tid;
+    if (tid >= total) p.order[tid] = -1;
+  }
+  for (int e = tid; e <= p.e; e += 256) {
+    int before = 0;
+    for (int i = 0; i < pairs; ++i) before += ids[i] >= 0 && ids[i] < e;
+    p.offsets[e] = before;
   }
 }
 
-// Scores and choice.  L lanes share a token and hold EPL experts each, expert i L + j in lane j: a load instruction reads
-// neighbouring logits.  The choice is top_k rounds of a maximum over the lanes' best; a round costs EPL compares and log2 L DPP
-// steps, so as few lanes a token as the registers allow are best (128 experts: 8 lanes of 16).
-template <int L, int EPL, bool GROUPS>
-__device__ __forceinline__ void route_tokens(const RouteParams& p, int tid, int64_t token0, uint8_t* smem) {
+// Scores and choice.  L lanes share a token and hold EPL experts each.  The choice is top_k rounds of a maximum over all keys, then the lowest expert that
+// has it.  Bound by its instructions: eight lanes of sixteen experts where there are tokens enough to fill the card, a wave per token
+// where there are few and a token's own time counts.  65536 tokens, 8 of 128 experts: 0 us; with a search through all sixteen registers
+// each round 22, with the lanes' keys sorted first as doubles that hold key and expert 84 (a compare is one instruction, but not a fast one).
+// FULL: with a bias or groups.  smem: a workgroup's own.
+template <int L, int EPL, bool FULL>
+__device__ __forceinline__ void route_tokens(const RouteParams& p, int tid, int64_t token0, uint8_t* smem, int (&id)[(TNX_MOE_MAX_TOP_K + L - 1) / L]) {
   const int j = tid % L, slot = tid / L;
   const int64_t token = token0 + slot;
   const bool live = token < p.tokens;
   const uint8_t* row = p.logits + (live ? token : p.tokens - 1) * p.stride * (p.dtype == DT_F32 ? 4 : 2);
-  float l[EPL], key[EPL];
+  float l[EPL];
+  load_row<L, EPL>(row, p.e, p.dtype, p.vec, j, l);
   float top = -INFINITY;
-  bool bad = false;
+  int bad_bit = 0;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    const int e = i * L + j;
-    l[i] = e < p.e ? load_logit(row, e, p.dtype) : -INFINITY;
-  }
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    bad |= l[i] != l[i];
+    bad_bit |= l[i] != l[i];
     top = __builtin_fmaxf(top, l[i]);
   }
   top = lanes_max<L>(top);
   const bool soft = p.scoring == TNX_MOE_SOFTMAX;
-  bad = lanes_any<L>(bad) || (soft && top == INFINITY);
+  const bool bad = lanes_or<L>(bad_bit) || (soft && top == INFINITY);
   // softmax: score = exp(l - top) * inv (a row of -inf throughout has no score: nothing is chosen)
-  float inv = 0.0f;
+  // Where the weights are divided by their own sum, and no bias asks for the scores themselves, the sum over all falls out.
+  float inv = 1.0f;
   const float off = top == -INFINITY ? 0.0f : top;
-  if (soft) {
+  if (soft && (!p.renorm || (FULL && p.bias))) {
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) sum += __expf(l[i] - off);
@@ -197,84 +232,143 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int tid, int6
     inv = sum > 0.0f ? 1.0f / sum : 0.0f;
   }
   auto score = [&](float x) { return soft ? __expf(x - off) * inv : sigmoid(x); };
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = i * L + j;
-    key[i] = l[i];
-    if (p.bias && e < p.e && l[i] > -INFINITY) {
-      key[i] = score(l[i]) + p.bias[e];
-      if (!(key[i] > -INFINITY)) key[i] = -INFINITY;
-    }
-    if (bad) key[i] = -INFINITY;
-  }
-  if (GROUPS) {
-    // the keys of the workgroup's tokens in LDS; a lane ranks groups j, j + L, ... of its token
-    float* keys = (float*)smem + slot * (p.e + TNX_MOE_MAX_GROUPS);
-    float* worth = keys + p.e;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (i * L + j < p.e) keys[i * L + j] = key[i];
-    __syncthreads();
-    for (int g = j; g < p.groups; g += L) {
-      // the sum of the group_top (1 or 2) largest keys that can be chosen
-      float a = -INFINITY, b = -INFINITY;
-      for (int i = 0; i < p.group_size; ++i) {
-        const float x = keys[g * p.group_size + i];
-        b = __builtin_fmaxf(b, __builtin_fminf(a, x));
-        a = __builtin_fmaxf(a, x);
-      }
-      worth[g] = p.group_top == 2 && b > -INFINITY ? a + b : a;
-    }
-    __syncthreads();
-    unsigned long long stay = 0;           // the groups with fewer than top_groups better ones
-    for (int g = j; g < p.groups; g += L) {
-      const float w = worth[g];
-      int better = 0;
-      for (int o = 0; o < p.groups; ++o) better += worth[o] > w || (worth[o] == w && o < g);
-      if (better < p.top_groups) stay |= 1ull << g;
-    }
-    int lo = (int)(uint32_t)stay, hi = (int)(uint32_t)(stay >> 32);
-    over_lanes<L>([&](auto d) { lo |= lane_xor<decltype(d)::value>(lo); hi |= lane_xor<decltype(d)::value>(hi); });
-    stay = (unsigned long long)(uint32_t)hi << 32 | (uint32_t)lo;
+  float key[EPL];
+  if (FULL) {
+    float (&f)[EPL] = key;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const int e = i * L + j;
-      if (e < p.e && !(stay >> (e / p.group_size) & 1)) key[i] = -INFINITY;
-    }
-    __syncthreads();                       // (the plan's bits take the same memory)
-  }
-  constexpr int KR = (TNX_MOE_MAX_TOP_K + L - 1) / L;
-  float w[KR];
-  int id[KR];
-  float total = 0.0f;
-#pragma unroll
-  for (int r = 0; r < KR; ++r) {
-    w[r] = 0.0f;
-    id[r] = -1;
-    for (int q = r * L; q < p.k && q < r * L + L; ++q) {
-      float best = key[0], best_l = l[0];
-      int best_e = j;
-#pragma unroll
-      for (int i = 1; i < EPL; ++i)
-        if (key[i] > best) { best = key[i]; best_l = l[i]; best_e = i * L + j; }
-      over_lanes<L>([&](auto d) {
-        constexpr int D = decltype(d)::value;
-        const float o = __builtin_bit_cast(float, lane_xor<D>(__builtin_bit_cast(int, best)));
-        const float ol = __builtin_bit_cast(float, lane_xor<D>(__builtin_bit_cast(int, best_l)));
-        const int oe = lane_xor<D>(best_e);
-        if (o > best || (o == best && oe < best_e)) { best = o; best_l = ol; best_e = oe; }
-      });
-      const bool found = best > -INFINITY;
-      const float s = found ? score(best_l) : 0.0f;
-      total += s;
-      if (j == q - r * L) { w[r] = s; id[r] = found ? best_e : -1; }
-      if (best_e % L == j) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-          if (i * L + j == best_e) key[i] = -INFINITY;
+      const int e = expert_of<L>(i, j);
+      f[i] = l[i];
+      if (p.bias && e < p.e && l[i] > -INFINITY) {
+        f[i] = score(l[i]) + p.bias[e];
+        if (!(f[i] > -INFINITY)) f[i] = -INFINITY;
       }
     }
+    if (p.top_groups < p.groups) {
+      // The token's keys in LDS, its own lanes' only: they are in one wave, whose LDS operations are in order.
+      float* keys = (float*)smem + slot * (p.e + TNX_MOE_MAX_GROUPS);
+      float* worth = keys + p.e;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (expert_of<L>(i, j) < p.e) keys[expert_of<L>(i, j)] = f[i];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      // several lanes a group: the sum of the group_top (1 or 2) largest keys that can be chosen
+      int per = 1;
+      while (per < 16 && 2 * per * p.groups <= L) per *= 2;
+      for (int g0 = 0; g0 < p.groups; g0 += L / per) {
+        const int g = g0 + j / per;
+        float a = -INFINITY, b = -INFINITY;
+        if (g < p.groups)
+          for (int i = j % per; i < p.group_size; i += per) {
+            const float x = keys[g * p.group_size + i];
+            b = __builtin_fmaxf(b, __builtin_fminf(a, x));
+            a = __builtin_fmaxf(a, x);
+          }
+        auto merge = [&](auto d) {
+          const float oa = lane_xor<decltype(d)::value>(a), ob = lane_xor<decltype(d)::value>(b);
+          b = __builtin_fmaxf(__builtin_fminf(a, oa), __builtin_fmaxf(b, ob));
+          a = __builtin_fmaxf(a, oa);
+        };
+        if (per > 1) merge(IntTag<1>());
+        if (per > 2) merge(IntTag<2>());
+        if (per > 4) merge(IntTag<4>());
+        if (per > 8) merge(IntTag<8>());
+        if (g < p.groups && j % per == 0) worth[g] = p.group_top == 2 && b > -INFINITY ? a + b : a;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      int lo = 0, hi = 0;                  // the groups with fewer than top_groups better ones
+      for (int g = j; g < p.groups; g += L) {
+        const float w = worth[g];
+        int better = 0;
+        for (int o = 0; o < p.groups; ++o) better += worth[o] > w || (worth[o] == w && o < g);
+        if (better < p.top_groups) (g < 32 ? lo : hi) |= 1 << (g & 31);
+      }
+      lo = lanes_or<L>(lo);
+      hi = lanes_or<L>(hi);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const int e = expert_of<L>(i, j), g = e / p.group_size;
+        if (e < p.e && !((g < 32 ? lo : hi) >> (g & 31) & 1)) f[i] = -INFINITY;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) key[i] = l[i];
   }
+  constexpr int KR = (TNX_MOE_MAX_TOP_K + L - 1) / L, NG = EPL / 4;
+  float won[KR];
+  if constexpr (NG == 1) {
+#pragma unroll
+    for (int r = 0; r < KR; ++r) {
+      won[r] = -INFINITY;
+      id[r] = 0;
+#pragma unroll 1
+      for (int q = r * L; q < p.k && q < r * L + L; ++q) {
+        const float best = lanes_max<L>(__builtin_fmaxf(__builtin_fmaxf(key[0], key[1]), __builtin_fmaxf(key[2], key[3])));
+        int at = key[3] == best ? 3 : -1;  // this lane's first place that has it
+        at = key[2] == best ? 2 : at;
+        at = key[1] == best ? 1 : at;
+        at = key[0] == best ? 0 : at;
+        const int mine = at >= 0 ? 4 * j + at : 0x7fffffff, e = lanes_min<L>(mine);
+        if (j == q - r * L) { won[r] = best; id[r] = e; }
+        at = mine == e ? at : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) key[i] = i == at ? -INFINITY : key[i];
+      }
+    }
+  } else {
+    // Runs of four keys in LDS, the runs' maxima in registers: run g L + j (experts 4 (g L + j) + 0 .. 3) is lane j's g-th.  Only the lane that holds the
+    // round's key looks into its run.  (All in one wave, whose LDS operations are in order.)
+    f32x4* runs = (f32x4*)(smem + p.runs_at) + tid;                       // [NG][256]
+    int* chosen = (int*)(smem + p.runs_at + NG * 4096) + slot * TNX_MOE_MAX_TOP_K;
+    float top4[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      runs[g * 256] = f32x4{key[4 * g], key[4 * g + 1], key[4 * g + 2], key[4 * g + 3]};
+      top4[g] = __builtin_fmaxf(__builtin_fmaxf(key[4 * g], key[4 * g + 1]), __builtin_fmaxf(key[4 * g + 2], key[4 * g + 3]));
+    }
+#pragma unroll
+    for (int r = 0; r < KR; ++r) {
+      won[r] = -INFINITY;
+#pragma unroll 1
+      for (int q = r * L; q < p.k && q < r * L + L; ++q) {
+        float best = top4[0];
+#pragma unroll
+        for (int g = 1; g < NG; ++g) best = __builtin_fmaxf(best, top4[g]);
+        best = lanes_max<L>(best);
+        int at = -1;
+#pragma unroll
+        for (int g = NG - 1; g >= 0; --g) at = top4[g] == best ? g : at;
+        const int mine = at >= 0 ? at * L + j : 0x7fffffff, run = lanes_min<L>(mine);
+        if (j == q - r * L) won[r] = best;
+        if (at >= 0 && mine == run) {
+          f32x4 v = runs[at * 256];
+          const int x = v[0] == best ? 0 : v[1] == best ? 1 : v[2] == best ? 2 : 3;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = i == x ? -INFINITY : v[i];
+          const float rest = __builtin_fmaxf(__builtin_fmaxf(v[0], v[1]), __builtin_fmaxf(v[2], v[3]));
+          ((float*)(runs + at * 256))[x] = -INFINITY;
+          chosen[q] = 4 * run + x;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) top4[g] = g == at ? rest : top4[g];
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int r = 0; r < KR; ++r) id[r] = r * L + j < p.k ? chosen[r * L + j] : 0;
+  }
+  float w[KR], total = 0.0f;
+#pragma unroll
+  for (int r = 0; r < KR; ++r) {
+    const bool found = won[r] > -INFINITY && !bad;        // (a row with a NaN may have chosen nothing at all)
+    id[r] = found ? id[r] : -1;
+    // (with a bias the key is not the logit: read again)
+    const float x = found ? (FULL && p.bias ? load_logit(row, id[r], p.dtype) : won[r]) : 0.0f;
+    w[r] = found ? score(x) : 0.0f;
+    total += w[r];
+  }
+  total = lanes_sum<L>(total);
   const float f = p.renorm ? (total > 0.0f ? p.scale / total : 0.0f) : p.scale;
 #pragma unroll
   for (int r = 0; r < KR; ++r) {
@@ -286,79 +380,136 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int tid, int6
   }
 }
 
-// ALONE: one workgroup has all the tokens, and places their pairs too
-template <int L, int EPL, bool GROUPS, bool ALONE>
+// What a workgroup's tokens chose, for the plan: ALONE places the pairs of the only workgroup, otherwise each counts its own per expert.
+template <int L, int EPL, bool FULL, bool ALONE>
 __global__ __launch_bounds__(256) void route_kernel(RouteParams p, PlanParams q) {
   extern __shared__ __attribute__((aligned(16))) uint8_t moe_smem[];
-  route_tokens<L, EPL, GROUPS>(p, threadIdx.x, (int64_t)blockIdx.x * (256 / L), moe_smem);
+  constexpr int KR = (TNX_MOE_MAX_TOP_K + L - 1) / L;
+  const int tid = threadIdx.x, j = tid % L, slot = tid / L;
+  int id[KR];
+  route_tokens<L, EPL, FULL>(p, tid, (int64_t)blockIdx.x * (256 / L), moe_smem, id);
+  if (FULL || EPL > 4) __syncthreads();    // (the keys lay where the plan's memory is)
   if (ALONE) {
-    __threadfence_block();                 // the experts just written are read back through memory by this workgroup
+    int* ids = (int*)moe_smem;
+#pragma unroll
+    for (int r = 0; r < KR; ++r)
+      if (slot < p.tokens && r * L + j < p.k) ids[slot * p.k + r * L + j] = id[r];
     __syncthreads();
-    plan_alone(q, moe_smem, threadIdx.x);
+    plan_alone(q, ids, tid);
+  } else if (q.fused) {
+    const PairBits bits{(unsigned long long*)moe_smem, q.words};
+    bits.clear(q.e, tid);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < KR; ++r)
+      if ((int64_t)blockIdx.x * (256 / L) + slot < p.tokens && r * L + j < p.k && id[r] >= 0) bits.mark(id[r], slot * p.k + r * L + j);
+    __syncthreads();
+    for (int e = tid; e < q.e; e += 256) q.counts[(int64_t)e * q.blocks + blockIdx.x] = bits.count(e);
   }
 }
 
-__global__ __launch_bounds__(256) void plan_alone_kernel(PlanParams p) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t moe_smem[];
-  plan_alone(p, moe_smem, threadIdx.x);
+// the experts of a block's pairs into bits; anything outside the range is an empty slot
+__device__ __forceinline__ void mark_pairs(const PlanParams& p, const PairBits& bits, int tid) {
+  bits.clear(p.e, tid);
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * p.block;
+  for (int i = tid; i < p.block && first + i < p.pairs; i += 256) {
+    const int e = p.experts[first + i];
+    if (e >= 0 && e < p.e) bits.mark(e, i);
+  }
+  __syncthreads();
 }
 
-// Many pairs, three launches: how many pairs of each block an expert has; sums over the blocks; places.
+__global__ __launch_bounds__(256) void plan_alone_kernel(PlanParams p) {
+  __shared__ int ids[PLAN_ALONE];
+  if ((int)threadIdx.x < PLAN_ALONE) {
+    const int e = (int)threadIdx.x < p.pairs ? p.experts[threadIdx.x] : -1;
+    ids[threadIdx.x] = e >= 0 && e < p.e ? e : -1;
+  }
+  __syncthreads();
+  plan_alone(p, ids, threadIdx.x);
+}
+
+// Many pairs: how many of each block an expert has (with the routing, or here); sums over the blocks, where there are more than a placing
+// workgroup should add up by itself; places.
 __global__ __launch_bounds__(256) void plan_count_kernel(PlanParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t moe_smem[];
-  const PairBits bits{(unsigned long long*)moe_smem};
-  int expert[PLAN_PAIRS / 256];
-  mark_pairs(p, (int64_t)blockIdx.x * PLAN_PAIRS, bits, threadIdx.x, expert);
+  const PairBits bits{(unsigned long long*)moe_smem, p.words};
+  mark_pairs(p, bits, threadIdx.x);
   for (int e = threadIdx.x; e < p.e; e += 256) p.counts[(int64_t)e * p.blocks + blockIdx.x] = bits.count(e);
 }
 
+// counts[e][block] -> pairs of e in the blocks before it; a workgroup per expert, eight neighbouring blocks a thread (65536 tokens of 8 pairs: 2048 blocks,
+// one turn).  With the experts next to each other instead, 8.5 us, most of it for lines of which a workgroup uses 16 bytes.
 __global__ __launch_bounds__(256) void plan_sum_kernel(PlanParams p) {
   __shared__ int waves[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int32_t* c = p.counts + (int64_t)blockIdx.x * p.blocks;
-  const int tid = threadIdx.x, lane = tid & 63;
   int carry = 0;
-  for (int b0 = 0; b0 < p.blocks; b0 += 256) {
-    const int v = b0 + tid < p.blocks ? c[b0 + tid] : 0;
-    int upto = v;
+  for (int b0 = 0; b0 < p.blocks; b0 += 2048) {
+    int v[8], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = b0 + tid * 8 + i < p.blocks ? c[b0 + tid * 8 + i] : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += v[i];
+    int upto = sum;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const int x = __shfl_up(upto, d);
       if (lane >= d) upto += x;
     }
-    if (lane == 63) waves[tid >> 6] = upto;
     __syncthreads();
-    int before = carry + upto - v, all = 0;
+    if (lane == 63) waves[wave] = upto;
+    __syncthreads();
+    int before = carry + upto - sum;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      if (w < (tid >> 6)) before += waves[w];
-      all += waves[w];
+      if (w < wave) before += waves[w];
+      carry += waves[w];
     }
-    if (b0 + tid < p.blocks) c[b0 + tid] = before;
-    carry += all;
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (b0 + tid * 8 + i < p.blocks) c[b0 + tid * 8 + i] = before;
+      before += v[i];
+    }
   }
   if (tid == 0) p.totals[blockIdx.x] = carry;
 }
 
+// SUMMED: the counts are sums over the blocks before already
+template <bool SUMMED>
 __global__ __launch_bounds__(256) void plan_place_kernel(PlanParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t moe_smem[];
-  const PairBits bits{(unsigned long long*)moe_smem};
-  int* base = (int*)(moe_smem + (size_t)p.e * PLAN_PAIRS / 8);
+  const PairBits bits{(unsigned long long*)moe_smem, p.words};
+  int* base = (int*)(moe_smem + (size_t)p.e * p.words * 8);
+  int* own = base + p.e;                   // pairs of the expert in the blocks before this one
   const int tid = threadIdx.x;
-  const int64_t first = (int64_t)blockIdx.x * PLAN_PAIRS;
-  for (int e = tid; e < p.e; e += 256) base[e] = p.totals[e];
-  int expert[PLAN_PAIRS / 256];
-  mark_pairs(p, first, bits, tid, expert);
+  const int64_t first = (int64_t)blockIdx.x * p.block;
+  for (int e = tid; e < p.e; e += 256) {
+    if (SUMMED) {
+      base[e] = p.totals[e];
+      own[e] = p.counts[(int64_t)e * p.blocks + blockIdx.x];
+    } else {
+      int all = 0, before = 0;
+#pragma unroll 8
+      for (int b = 0; b < p.blocks; ++b) {
+        const int c = p.counts[(int64_t)e * p.blocks + b];
+        all += c;
+        before += b < (int)blockIdx.x ? c : 0;
+      }
+      base[e] = all;
+      own[e] = before;
+    }
+  }
+  mark_pairs(p, bits, tid);
   const int total = scan_experts(base, p.e, tid);
   if (blockIdx.x == 0)
     for (int e = tid; e <= p.e; e += 256) p.offsets[e] = e < p.e ? base[e] : total;
-#pragma unroll
-  for (int u = 0; u < PLAN_PAIRS / 256; ++u) {
-    const int i = u * 256 + tid;
+  for (int i = tid; i < p.block && first + i < p.pairs; i += 256) {
     const int64_t pair = first + i;
-    if (pair >= p.pairs) continue;
-    if (expert[u] >= 0) {
-      const int at = base[expert[u]] + p.counts[(int64_t)expert[u] * p.blocks + blockIdx.x] + bits.rank(expert[u], i);
+    const int e = p.experts[pair];
+    if (e >= 0 && e < p.e) {
+      const int at = base[e] + own[e] + bits.rank(e, i);
       p.order[at] = (int32_t)pair;
       p.rows[pair] = at;
     } else p.rows[pair] = -1;
@@ -371,28 +522,29 @@ __global__ __launch_bounds__(256) void plan_place_kernel(PlanParams p) {
 //   softmax: dl_i = s_i (ds_i - sum_j s_j ds_j) over all i; with renormalised weights the sum is zero and s_j / S = weight / scale, so
 //            neither the logits nor the other experts enter: dl_j = w_j (g_j - sum_i (w_i / scale) g_i)
 //   sigmoid: dl_j = ds_j s_j (1 - s_j), of the chosen alone
+// The chosen experts' values go through a row in LDS that starts as zeros, and the row leaves in runs of four.  Bound by writing the
+// gradient: 65536 x 128, float32, renormalised softmax: 0 us for 33.5 MB.  (Compared one by one with every lane's experts: 13.6 us.)
 template <int L, int EPL>
 __global__ __launch_bounds__(256) void route_backward_kernel(RouteParams p) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t moe_smem[];
   const int tid = threadIdx.x, j = tid % L;
   const int64_t token = (int64_t)blockIdx.x * (256 / L) + tid / L;
   const bool live = token < p.tokens;
   const int64_t t = live ? token : p.tokens - 1;
   const uint8_t* row = p.logits + t * p.stride * (p.dtype == DT_F32 ? 4 : 2);
-  const bool soft = p.scoring == TNX_MOE_SOFTMAX;
-  float l[EPL], d[EPL];
-  float off = 0.0f, inv = 0.0f;
-  const bool dense = soft && !p.renorm;
+  const bool soft = p.scoring == TNX_MOE_SOFTMAX, dense = soft && !p.renorm;
+  f32x4* mine = (f32x4*)moe_smem + (tid / L) * (EPL / 4 * L);              // [EPL / 4][L] runs of four
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) d[i] = 0.0f;
+  for (int i = 0; i < EPL; i += 4) mine[i / 4 * L + j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float l[EPL];
+  float inv = 0.0f;
   if (dense) {
+    load_row<L, EPL>(row, p.e, p.dtype, p.vec, j, l);
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      l[i] = i * L + j < p.e ? load_logit(row, i * L + j, p.dtype) : -INFINITY;
-      top = __builtin_fmaxf(top, l[i]);
-    }
+    for (int i = 0; i < EPL; ++i) top = __builtin_fmaxf(top, l[i]);
     top = lanes_max<L>(top);
-    off = top == -INFINITY ? 0.0f : top;
+    const float off = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) sum += l[i] = __expf(l[i] - off);
@@ -404,7 +556,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteParams p) {
   float g[KR], s[KR], w[KR];
   int id[KR];
   float wg = 0.0f, total = 0.0f;
-  bool bad = false;
+  int bad_bit = 0;
 #pragma unroll
   for (int r = 0; r < KR; ++r) {
     const int q = r * L + j;
@@ -412,7 +564,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteParams p) {
     g[r] = s[r] = w[r] = 0.0f;
     if (q < p.k) {
       w[r] = p.weights[t * p.k + q];
-      bad |= w[r] != w[r];
+      bad_bit |= w[r] != w[r];
       id[r] = p.experts[t * p.k + q];
       if (id[r] >= p.e) id[r] = -1;
       if (id[r] >= 0) {
@@ -423,40 +575,47 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteParams p) {
     total += s[r];
     wg += soft ? w[r] * g[r] : s[r] * g[r];
   }
-  bad = lanes_any<L>(bad);
+  const bool bad = lanes_or<L>(bad_bit) != 0;
   wg = lanes_sum<L>(wg);
   total = lanes_sum<L>(total);
-  float value[KR];                         // of the chosen: dl (dense: without the common term)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the row is its own lanes' only, and they are in one wave
 #pragma unroll
   for (int r = 0; r < KR; ++r) {
-    if (soft && p.renorm) value[r] = w[r] * (g[r] - (p.scale != 0.0f ? wg / p.scale : 0.0f));
-    else if (soft) value[r] = w[r] * g[r];                  // s ds: weight is scale s
+    float value;                           // dl (dense: without the common term)
+    if (soft && p.renorm) value = w[r] * (g[r] - (p.scale != 0.0f ? wg / p.scale : 0.0f));
+    else if (soft) value = w[r] * g[r];                    // s ds: weight is scale s
     else {
       float ds = p.scale * g[r];
       if (p.renorm) ds = total > 0.0f ? p.scale * (g[r] - wg / total) / total : 0.0f;
-      value[r] = ds * s[r] * (1.0f - s[r]);
+      value = ds * s[r] * (1.0f - s[r]);
     }
+    if (id[r] >= 0) ((float*)mine)[id[r]] = value;
   }
-  if (dense) {
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) d[i] = -(l[i] * inv) * wg;
-  }
-#pragma unroll
-  for (int r = 0; r < KR; ++r) {
-    for (int q = r * L; q < p.k && q < r * L + L; ++q) {
-      // slot q's expert and value from the lane that has them
-      const int from = (tid & 63) - j + (q - r * L);
-      const int e = __shfl(id[r], from);
-      const float v = __shfl(value[r], from);
-#pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (e == i * L + j) d[i] += v;
-    }
-  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   if (!live) return;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i)
-    if (i * L + j < p.e) store_out<float>(p.grad_logits, token * p.e + i * L + j, bad ? __builtin_nanf("") : d[i], p.dtype);
+  for (int i = 0; i < EPL; i += 4) {
+    const int e = expert_of<L>(i, j);
+    f32x4 d = mine[i / 4 * L + j];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (dense) d[x] -= l[i + x] * inv * wg;
+      if (bad) d[x] = __builtin_nanf("");
+    }
+    const int64_t at = token * p.e + e;
+    if (e + 4 <= p.e && p.vec_out) {
+      if (p.dtype == DT_F32) *(f32x4*)((float*)p.grad_logits + at) = d;
+      else {
+        const uint32_t a = p.dtype == DT_BF16 ? (uint32_t)OutBF16::cvt(d[0]) | (uint32_t)OutBF16::cvt(d[1]) << 16 : (uint32_t)OutF16::cvt(d[0]) | (uint32_t)OutF16::cvt(d[1]) << 16;
+        const uint32_t b = p.dtype == DT_BF16 ? (uint32_t)OutBF16::cvt(d[2]) | (uint32_t)OutBF16::cvt(d[3]) << 16 : (uint32_t)OutF16::cvt(d[2]) | (uint32_t)OutF16::cvt(d[3]) << 16;
+        *(i32x2*)((uint16_t*)p.grad_logits + at) = i32x2{(int)a, (int)b};
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (e + x < p.e) store_out<float>(p.grad_logits, at + x, d[x], p.dtype);
+    }
+  }
 }
 
 // The join: 16 bytes of a token's output per lane, the top_k rows one after another.
@@ -510,42 +669,73 @@ __global__ __launch_bounds__(256) void combine_kernel(const uint8_t* y, const in
 
 // ------------------------------------------------------------------------------------------------------------------
 int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
-int64_t plan_blocks(int64_t pairs) { return (pairs + PLAN_PAIRS - 1) / PLAN_PAIRS; }
-size_t plan_lds(int e) { return (size_t)e * (PLAN_PAIRS / 8) + (size_t)e * 4; }
+
+// Lanes a token: one wave for few tokens or many experts
+int route_lanes(int64_t tokens, int e) {
+  if (e > 512 || tokens <= 1024) return 64;
+  return e <= 128 ? 8 : e <= 256 ? 16 : 32;
+}
+constexpr int SUM_BLOCKS = 128;            // more blocks than this are summed by a launch of their own
+
+// The plan's blocks are the pairs of a routing workgroup's 256 / lanes tokens; many tokens at four a workgroup are counted apart, in larger blocks.
+void plan_shape(PlanParams* q, int64_t tokens, int k, int e) {
+  const int lanes = route_lanes(tokens, e);
+  q->pairs = tokens * k;
+  q->e = e;
+  q->fused = lanes < 64 || tokens <= 1024;
+  q->block = q->fused ? 256 / lanes * k : 512;
+  q->blocks = (int)((q->pairs + q->block - 1) / q->block);
+  q->words = (q->block + 63) / 64;
+}
+bool plan_is_alone(const PlanParams& q) { return q.blocks <= 1 && q.pairs <= PLAN_ALONE; }
+size_t bits_lds(const PlanParams& q) { return (size_t)q.e * q.words * 8; }
+
+size_t plan_bytes(const PlanParams& q) {
+  if (q.pairs <= PLAN_ALONE && q.blocks <= 1) return 0;
+  return (size_t)(up16((int64_t)q.e * q.blocks * 4) + up16((int64_t)q.e * 4));
+}
 
 int check_plan(const tnx_moe_args* a) {
   if (!a || a->tokens < 0 || a->top_k < 1 || a->num_experts < 1) return TNX_E_INVALID;
   if (a->num_experts > TNX_MOE_MAX_EXPERTS || a->top_k > TNX_MOE_MAX_TOP_K || a->tokens > 0x3fffffff / a->top_k) return TNX_E_UNSUPPORTED;
   if (!a->offsets) return TNX_E_INVALID;
   if (a->tokens > 0 && (!a->experts || !a->order || !a->rows)) return TNX_E_INVALID;
-  if (a->tokens * a->top_k > PLAN_PAIRS && (!a->workspace || ((uintptr_t)a->workspace & 15) ||
-      a->workspace_bytes < tnx_moe_workspace_bytes(a->tokens, a->top_k, a->num_experts))) return TNX_E_WORKSPACE;
+  const size_t need = tnx_moe_workspace_bytes(a->tokens, a->top_k, a->num_experts);
+  if (need && (!a->workspace || ((uintptr_t)a->workspace & 15) || a->workspace_bytes < need)) return TNX_E_WORKSPACE;
   return TNX_OK;
 }
 
 PlanParams plan_params(const tnx_moe_args* a) {
   PlanParams q;
   q.experts = a->experts; q.offsets = a->offsets; q.order = a->order; q.rows = a->rows;
-  q.pairs = a->tokens * a->top_k;
-  q.e = a->num_experts;
-  q.blocks = (int)plan_blocks(q.pairs);
+  plan_shape(&q, a->tokens, a->top_k, a->num_experts);
   q.counts = (int32_t*)a->workspace;
   q.totals = q.counts ? (int32_t*)((uint8_t*)q.counts + up16((int64_t)q.e * q.blocks * 4)) : nullptr;
   return q;
 }
 
+// the launches after the counts
+int place_pairs(const PlanParams& q, hipStream_t stream) {
+  const size_t lds = bits_lds(q) + (size_t)q.e * 8;
+  if (q.blocks > SUM_BLOCKS) {
+    hipLaunchKernelGGL(plan_sum_kernel, dim3((unsigned)q.e), dim3(256), 0, stream, q);
+    const int st = mx_launched();
+    if (st) return st;
+    hipLaunchKernelGGL((plan_place_kernel<true>), dim3((unsigned)q.blocks), dim3(256), lds, stream, q);
+  } else {
+    hipLaunchKernelGGL((plan_place_kernel<false>), dim3((unsigned)q.blocks), dim3(256), lds, stream, q);
+  }
+  return mx_launched();
+}
+
 int launch_plan(const PlanParams& q, hipStream_t stream) {
-  if (q.pairs <= PLAN_PAIRS) {
-    hipLaunchKernelGGL(plan_alone_kernel, dim3(1), dim3(256), plan_lds(q.e), stream, q);
+  if (plan_is_alone(q)) {
+    hipLaunchKernelGGL(plan_alone_kernel, dim3(1), dim3(256), 0, stream, q);
     return mx_launched();
   }
-  hipLaunchKernelGGL(plan_count_kernel, dim3((unsigned)q.blocks), dim3(256), plan_lds(q.e), stream, q);
-  int st = mx_launched();
-  if (st) return st;
-  hipLaunchKernelGGL(plan_sum_kernel, dim3((unsigned)q.e), dim3(256), 0, stream, q);
-  if ((st = mx_launched())) return st;
-  hipLaunchKernelGGL(plan_place_kernel, dim3((unsigned)q.blocks), dim3(256), plan_lds(q.e), stream, q);
-  return mx_launched();
+  hipLaunchKernelGGL(plan_count_kernel, dim3((unsigned)q.blocks), dim3(256), bits_lds(q), stream, q);
+  const int st = mx_launched();
+  return st ? st : place_pairs(q, stream);
 }
 
 int check_route(const tnx_moe_args* a) {
@@ -568,36 +758,52 @@ RouteParams route_params(const tnx_moe_args* a) {
   p.groups = a->num_groups; p.top_groups = a->top_groups; p.group_top = a->group_top; p.renorm = a->renormalize;
   p.group_size = a->num_experts / a->num_groups;
   p.scale = a->scale;
+  p.runs_at = 0;
+  const int es = a->dtype == TNX_F32 ? 4 : 2;
+  p.vec = p.e % 4 == 0 && p.stride % 4 == 0 && ((uintptr_t)a->logits & (4 * es - 1)) == 0;
+  p.vec_out = p.e % 4 == 0 && ((uintptr_t)a->grad_logits & (4 * es - 1)) == 0;
   return p;
 }
 
-template <int L, int EPL> int launch_route(const RouteParams& p, const PlanParams& q, hipStream_t stream) {
+template <int L, int EPL> int launch_route(const RouteParams& in, const PlanParams& q, hipStream_t stream) {
   constexpr int TOKENS = 256 / L;
-  const unsigned blocks = (unsigned)((p.tokens + TOKENS - 1) / TOKENS);
-  const bool groups = p.groups > 1 && p.top_groups < p.groups;
-  const bool alone = blocks == 1 && q.pairs <= PLAN_PAIRS;
-  const size_t keys = groups ? (size_t)TOKENS * (p.e + TNX_MOE_MAX_GROUPS) * 4 : 0, bits = alone ? plan_lds(p.e) : 0;
-  const size_t lds = keys > bits ? keys : bits;
-  if (groups && alone) hipLaunchKernelGGL((route_kernel<L, EPL, true, true>), dim3(blocks), dim3(256), lds, stream, p, q);
-  else if (groups) hipLaunchKernelGGL((route_kernel<L, EPL, true, false>), dim3(blocks), dim3(256), lds, stream, p, q);
+  const unsigned blocks = (unsigned)((in.tokens + TOKENS - 1) / TOKENS);
+  const bool groups = in.top_groups < in.groups, full = groups || in.bias, alone = plan_is_alone(q);
+  const size_t keys = groups ? (size_t)up16((int64_t)TOKENS * (in.e + TNX_MOE_MAX_GROUPS) * 4) : 0, plan = alone ? PLAN_ALONE * 4 : bits_lds(q);
+  RouteParams p = in;
+  p.runs_at = (int)keys;
+  const size_t choice = keys + (EPL > 4 ? (size_t)EPL * 1024 + TOKENS * TNX_MOE_MAX_TOP_K * 4 : 0), lds = choice > plan ? choice : plan;
+  if (full && alone) hipLaunchKernelGGL((route_kernel<L, EPL, true, true>), dim3(blocks), dim3(256), lds, stream, p, q);
+  else if (full) hipLaunchKernelGGL((route_kernel<L, EPL, true, false>), dim3(blocks), dim3(256), lds, stream, p, q);
   else if (alone) hipLaunchKernelGGL((route_kernel<L, EPL, false, true>), dim3(blocks), dim3(256), lds, stream, p, q);
   else hipLaunchKernelGGL((route_kernel<L, EPL, false, false>), dim3(blocks), dim3(256), lds, stream, p, q);
   const int st = mx_launched();
-  return st || alone ? st : launch_plan(q, stream);
+  return st || alone ? st : q.fused ? place_pairs(q, stream) : launch_plan(q, stream);
 }
 
 template <int L, int EPL> int launch_backward(const RouteParams& p, hipStream_t stream) {
   constexpr int TOKENS = 256 / L;
-  hipLaunchKernelGGL((route_backward_kernel<L, EPL>), dim3((unsigned)((p.tokens + TOKENS - 1) / TOKENS)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((route_backward_kernel<L, EPL>), dim3((unsigned)((p.tokens + TOKENS - 1) / TOKENS)), dim3(256), (size_t)256 * EPL * 4, stream, p);
   return mx_launched();
+}
+
+// f(lanes, experts a lane) of the smallest built pair that holds e experts
+template <class F> int with_lanes(int lanes, int e, F f) {
+  switch (lanes) {
+    case 8: return e <= 32 ? f(IntTag<8>(), IntTag<4>()) : e <= 64 ? f(IntTag<8>(), IntTag<8>()) : f(IntTag<8>(), IntTag<16>());
+    case 16: return f(IntTag<16>(), IntTag<16>());
+    case 32: return f(IntTag<32>(), IntTag<16>());
+    default: return e <= 256 ? f(IntTag<64>(), IntTag<4>()) : f(IntTag<64>(), IntTag<16>());
+  }
 }
 
 }  // namespace
 
 extern "C" size_t tnx_moe_workspace_bytes(int64_t tokens, int32_t top_k, int32_t num_experts) {
-  const int64_t pairs = tokens * top_k;
-  if (tokens <= 0 || top_k <= 0 || num_experts <= 0 || pairs <= PLAN_PAIRS) return 0;
-  return (size_t)(up16((int64_t)num_experts * plan_blocks(pairs) * 4) + up16((int64_t)num_experts * 4));
+  if (tokens <= 0 || top_k <= 0 || num_experts <= 0) return 0;
+  PlanParams q;
+  plan_shape(&q, tokens, top_k, num_experts);
+  return plan_bytes(q);
 }
 
 extern "C" int tnx_moe_plan(const tnx_moe_args* a) {
@@ -612,12 +818,7 @@ extern "C" int tnx_moe_route(const tnx_moe_args* a) {
   const PlanParams q = plan_params(a);
   const hipStream_t stream = (hipStream_t)a->stream;
   if (a->tokens == 0) return launch_plan(q, stream);
-  if (p.e <= 32) return launch_route<8, 4>(p, q, stream);
-  if (p.e <= 64) return launch_route<8, 8>(p, q, stream);
-  if (p.e <= 128) return launch_route<8, 16>(p, q, stream);
-  if (p.e <= 256) return launch_route<16, 16>(p, q, stream);
-  if (p.e <= 512) return launch_route<32, 16>(p, q, stream);
-  return launch_route<64, 16>(p, q, stream);
+  return with_lanes(route_lanes(p.tokens, p.e), p.e, [&](auto l, auto n) { return launch_route<decltype(l)::value, decltype(n)::value>(p, q, stream); });
 }
 
 extern "C" int tnx_moe_route_backward(const tnx_moe_args* a) {
@@ -628,13 +829,9 @@ extern "C" int tnx_moe_route_backward(const tnx_moe_args* a) {
   if (a->tokens == 0) return TNX_OK;
   if (!a->experts || !a->grad || !a->grad_logits) return TNX_E_INVALID;
   const RouteParams p = route_params(a);
-  const hipStream_t stream = (hipStream_t)a->stream;
-  if (p.e <= 32) return launch_backward<8, 4>(p, stream);
-  if (p.e <= 64) return launch_backward<8, 8>(p, stream);
-  if (p.e <= 128) return launch_backward<8, 16>(p, stream);
-  if (p.e <= 256) return launch_backward<16, 16>(p, stream);
-  if (p.e <= 512) return launch_backward<32, 16>(p, stream);
-  return launch_backward<64, 16>(p, stream);
+  return with_lanes(route_lanes(p.tokens, p.e), p.e, [&](auto l, auto n) {
+    return launch_backward<decltype(l)::value, decltype(n)::value>(p, (hipStream_t)a->stream);
+  });
 }
 
 extern "C" int tnx_moe_combine(const void* y, const int32_t* rows, const float* weights, void* out, int64_t tokens, int32_t top_k, int64_t n,

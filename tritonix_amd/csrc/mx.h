@@ -46,8 +46,11 @@ template <> struct Elem<_Float16> {
   static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 };
 
-// scale byte of a block whose largest magnitude has the bits `top` (an integer maximum orders magnitudes, infinities and
-// NaNs last), and the factor 2^-e (0 for a block without finite values: its codes are zero)
+// magnitude of an element as an integer (these order as the magnitudes do, infinities and NaNs last), and the binary32 bits of one
+template <class R> __device__ __forceinline__ R magnitude(R v) { return v & (R)(sizeof(R) == 4 ? 0x7fffffffu : 0x7fffu); }
+template <class T> __device__ __forceinline__ uint32_t top_bits(typename Elem<T>::raw m) { return __builtin_bit_cast(uint32_t, Elem<T>::get(m)); }
+
+// scale byte of a block whose largest magnitude has the binary32 bits `top`, and the factor 2^-e (0 for a block without finite values: its codes are zero)
 __device__ __forceinline__ uint32_t scale_byte(uint32_t top, float* factor) {
   const int exponent = (int)(top >> 23);                 // biased; 0: zero or subnormal, below 2^-126: e is -127 there
   if (exponent == 255) { *factor = 0.0f; return 255; }
@@ -73,6 +76,7 @@ __device__ __forceinline__ uint32_t codes8(const float* v) {
 // an element times the block's factor; in a block without finite values everything becomes 0
 __device__ __forceinline__ float scaled(float x, float factor) { return factor == 0.0f ? 0.0f : x * factor; }
 
+// the largest of the four lanes that share a block
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);      // lane ^ 1
   v = v > a ? v : a;

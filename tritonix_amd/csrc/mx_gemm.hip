@@ -460,16 +460,15 @@ template <class T> __device__ __forceinline__ void quantize_to_lds(const MxParam
       for (int e = 0; e < 8; ++e) x.v[e] = e < left ? src[e] : (raw)0;
     }
     float v[8], factor;
-    uint32_t top = 0;
+    raw top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] = Elem<T>::get(x.v[e]);
-      const uint32_t b = __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu;
+      const raw b = magnitude(x.v[e]);
       top = top > b ? top : b;
     }
-    const uint32_t s = scale_byte(quad_max(top), &factor);
+    const uint32_t s = scale_byte(top_bits<T>((raw)quad_max(top)), &factor);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = scaled(v[e], factor);
+    for (int e = 0; e < 8; ++e) v[e] = scaled(Elem<T>::get(x.v[e]), factor);
     *TNX_LDS(uint32_t, codes + i * 4) = codes8(v);
     if ((at & 3) == 0) *TNX_LDS(uint8_t, scales + (i >> 2)) = (uint8_t)s;      // (a block of padding: codes 0, any finite scale)
   }

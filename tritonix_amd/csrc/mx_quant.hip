@@ -8,9 +8,9 @@
 // Both directions are bound by memory: 2 (4) bytes and 17/32 of one per element.  Two layouts of the source:
 //   k contiguous   a lane takes 8 neighbouring elements (16 or 32 bytes), four lanes share a block, and the largest magnitude goes round the
 //                  four in two DPP steps; the codes of a lane are one aligned word, so loads and stores are whole runs of a row
-//   anything else  (rows contiguous: a matrix quantised down its columns.)  A lane takes two neighbouring rows and walks
-//                  the 32 k of its block, loads of 64 neighbouring pairs; the largest magnitude needs no other lane.  The codes of
-//                  128 rows x 256 k meet in LDS and leave as rows of 128 bytes.
+//   anything else  (rows contiguous: a matrix quantised down its columns.)  A lane takes 8 bytes of neighbouring rows and walks
+//                  the 32 k of its block; the largest magnitude needs no other lane.  The codes of the rows x 256 k meet in LDS
+//                  and leave as rows of 128 bytes.
 #include <hip/hip_runtime.h>
 
 #include "../../include/tritonix_hip.h"
@@ -36,106 +36,120 @@ struct QuantParams {
   int64_t codes_b, scales_b;                             // bytes from one matrix of the batch to the next
 };
 
-constexpr int ROW_ITEMS = 4;                             // runs of 8 elements a lane takes, 256 lanes apart
+// Runs that a lane takes, 256 lanes apart.  8192 x 8192 bfloat16: quantising 30.9 us with two, 35.6 with four (the next workgroups' loads begin sooner).
+constexpr int QUANT_RUNS = 2, BACK_RUNS = 4;
 
 
-template <class T>
+// STREAM: a source that the memory-side cache of 256 MiB cannot hold is read past the caches (8192 x 28672 bfloat16: 108 us, so 123; a smaller one
+// that was just written is there: 8192 x 8192 31 us, past the caches 34).  For 2-byte elements; float32 is the same either way.
+template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantParams p) {
   typedef typename Elem<T>::raw raw;
   const int64_t total = p.rows * p.slabs * 32;           // runs of one matrix
-  const int64_t first = (int64_t)blockIdx.x * (256 * ROW_ITEMS) + threadIdx.x;
+  const int64_t first = (int64_t)blockIdx.x * (256 * QUANT_RUNS) + threadIdx.x;
   const raw* src = (const raw*)p.src + (int64_t)blockIdx.y * p.stride_b;
   uint8_t* codes = p.codes + (int64_t)blockIdx.y * p.codes_b;
   uint8_t* scales = p.scales + (int64_t)blockIdx.y * p.scales_b;
-  Run8<T> x[ROW_ITEMS];
-  int64_t row[ROW_ITEMS];
-  int at[ROW_ITEMS];
+  Run8<T> x[QUANT_RUNS];
+  int64_t row[QUANT_RUNS];
+  int at[QUANT_RUNS];
 #pragma unroll
-  for (int u = 0; u < ROW_ITEMS; ++u) {
+  for (int u = 0; u < QUANT_RUNS; ++u) {
     const int64_t i = first + u * 256;
     const int64_t item = i < total ? i : 0;
     row[u] = total < 0x7fffffff ? (int64_t)((uint32_t)item / (uint32_t)(p.slabs * 32)) : item / (p.slabs * 32);
     at[u] = (int)(item - row[u] * p.slabs * 32);
     const int64_t left = p.k - (int64_t)at[u] * 8;
     const raw* s = src + row[u] * p.stride_r + (int64_t)at[u] * 8;
-    if (left >= 8) x[u] = *(const Run8<T>*)s;
+    if (left >= 8) {
+      if constexpr (STREAM && sizeof(raw) == 2) {
+        const i32x4 w = __builtin_nontemporal_load((const i32x4_loose*)s);
+        __builtin_memcpy(&x[u], &w, 16);
+      } else x[u] = *(const Run8<T>*)s;
+    }
     else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[u].v[e] = e < left ? s[e] : (raw)0;
     }
   }
 #pragma unroll
-  for (int u = 0; u < ROW_ITEMS; ++u) {
+  for (int u = 0; u < QUANT_RUNS; ++u) {
     float v[8];
-    uint32_t top = 0;
+    raw top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] = Elem<T>::get(x[u].v[e]);
-      const uint32_t b = __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu;
+      const raw b = magnitude(x[u].v[e]);
       top = top > b ? top : b;
     }
-    top = quad_max(top);                                 // (all four lanes of a block are here: runs come in whole slabs)
+    top = (raw)quad_max(top);                            // (all four lanes of a block are here: runs come in whole slabs)
     float factor;
-    uint32_t s = scale_byte(top, &factor);
+    uint32_t s = scale_byte(top_bits<T>(top), &factor);
     if ((int64_t)(at[u] & ~3) * 8 >= p.k) s = 127;       // a block of padding
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = scaled(v[e], factor);
+    for (int e = 0; e < 8; ++e) v[e] = scaled(Elem<T>::get(x[u].v[e]), factor);
     if (first + u * 256 >= total) continue;
     *(uint32_t*)(codes + (row[u] * p.slabs * 32 + at[u]) * 4) = codes8(v);
     if ((at[u] & 3) == 0) scales[mx_scale_at(row[u], at[u] >> 5, p.slabs) + ((at[u] >> 2) & 7)] = (uint8_t)s;
   }
 }
 
+// Back: a lane's run is 16 bytes of the result (8 elements of 2 bytes, 4 of 4), stored past the caches: written through them, the lines that
+// the stores only fill in part for a while push out the codes (8192 x 28672: 197 us, so 128; float32 with 32 bytes a lane 339 us).
 template <class T>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(QuantParams p) {
   typedef typename Elem<T>::raw raw;
-  const int64_t total = p.rows * p.slabs * 32;
-  const int64_t first = (int64_t)blockIdx.x * (256 * ROW_ITEMS) + threadIdx.x;
+  constexpr int RUN = 16 / sizeof(raw), PER_SLAB = MX_SLAB / RUN;
+  const int64_t per_row = p.slabs * PER_SLAB, total = p.rows * per_row;
+  const int64_t first = (int64_t)blockIdx.x * (256 * BACK_RUNS) + threadIdx.x;
   raw* dst = (raw*)p.dst + (int64_t)blockIdx.y * p.stride_b;
   const uint8_t* codes = p.codes + (int64_t)blockIdx.y * p.codes_b;
   const uint8_t* scales = p.scales + (int64_t)blockIdx.y * p.scales_b;
-  uint32_t c[ROW_ITEMS], s[ROW_ITEMS];
-  int64_t row[ROW_ITEMS];
-  int at[ROW_ITEMS];
+  uint32_t c[BACK_RUNS], s[BACK_RUNS];
+  int64_t row[BACK_RUNS];
+  int at[BACK_RUNS];
 #pragma unroll
-  for (int u = 0; u < ROW_ITEMS; ++u) {
+  for (int u = 0; u < BACK_RUNS; ++u) {
     const int64_t i = first + u * 256;
     const int64_t item = i < total ? i : 0;
-    row[u] = total < 0x7fffffff ? (int64_t)((uint32_t)item / (uint32_t)(p.slabs * 32)) : item / (p.slabs * 32);
-    at[u] = (int)(item - row[u] * p.slabs * 32);
-    c[u] = *(const uint32_t*)(codes + (row[u] * p.slabs * 32 + at[u]) * 4);
-    s[u] = scales[mx_scale_at(row[u], at[u] >> 5, p.slabs) + ((at[u] >> 2) & 7)];
+    row[u] = total < 0x7fffffff ? (int64_t)((uint32_t)item / (uint32_t)per_row) : item / per_row;
+    at[u] = (int)(item - row[u] * per_row);
+    const uint8_t* from = codes + (row[u] * per_row + at[u]) * (RUN / 2);
+    c[u] = RUN == 8 ? *(const uint32_t*)from : *(const uint16_t*)from;
+    s[u] = scales[mx_scale_at(row[u], at[u] / PER_SLAB, p.slabs) + (at[u] / (32 / RUN)) % 8];
   }
 #pragma unroll
-  for (int u = 0; u < ROW_ITEMS; ++u) {
-    const int64_t left = p.k - (int64_t)at[u] * 8;
+  for (int u = 0; u < BACK_RUNS; ++u) {
+    const int64_t left = p.k - (int64_t)at[u] * RUN;
     if (first + u * 256 >= total || left <= 0) continue;
     float v[8];
     values8(c[u], scale_value(s[u]), v);
-    Run8<T> out;
+    raw o[RUN];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out.v[e] = Elem<T>::put(v[e]);
-    raw* d = dst + row[u] * p.stride_r + (int64_t)at[u] * 8;
-    if (left >= 8) *(Run8<T>*)d = out;
-    else {
+    for (int e = 0; e < RUN; ++e) o[e] = Elem<T>::put(v[e]);
+    raw* d = dst + row[u] * p.stride_r + (int64_t)at[u] * RUN;
+    if (left >= RUN) {
+      i32x4 w;
+      __builtin_memcpy(&w, o, 16);
+      store16_stream_loose(d, w);
+    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) d[e] = out.v[e];
+      for (int e = 0; e < RUN; ++e)
+        if (e < left) d[e] = o[e];
     }
   }
 }
 
-// Columns: a workgroup takes 128 rows and one slab, wave b the block b of it, a lane the rows 2 lane and 2 lane + 1.
-// Pitch of a row of codes in LDS: 16 bytes more than 128, so that the lanes' 16-byte pieces of neighbouring rows fall on
-// different banks.
-constexpr int COL_ROWS = 128, COL_PITCH = MX_ROWB + 16;
+// Columns: a workgroup takes 256 rows (128 of float32) and one slab, wave b the block b of it, a lane 8 bytes of neighbouring rows: a load
+// instruction is 512 bytes of one k.  (4 bytes a lane: 8192 x 8192 bfloat16 57 us, with 8 37.)  Pitch of a row of codes in LDS: 16 bytes more than 128, so that the lanes' 16-byte pieces fall on different banks.
+constexpr int COL_PITCH = MX_ROWB + 16;
+template <class T> constexpr int col_lane = 8 / sizeof(typename Elem<T>::raw);
+template <class T> struct __attribute__((packed, aligned(sizeof(T)))) RunC { typename Elem<T>::raw v[col_lane<T>]; };
 
-template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Pair { typename Elem<T>::raw v[2]; };
-
-// PAIRED: rows are neighbours in memory (stride_r == 1); otherwise any strides, an element at a time
-template <class T, bool PAIRED>
+// RUNS: rows are neighbours in memory (stride_r == 1); otherwise any strides, an element at a time
+template <class T, bool RUNS>
 __global__ __launch_bounds__(512) void quantize_columns_kernel(QuantParams p) {
   typedef typename Elem<T>::raw raw;
+  constexpr int COL_LANE = col_lane<T>, COL_ROWS = 64 * COL_LANE;
   __shared__ __attribute__((aligned(16))) uint8_t tile[COL_ROWS * COL_PITCH];
   __shared__ __attribute__((aligned(16))) uint8_t tile_s[COL_ROWS * MX_SCALEB];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -144,45 +158,46 @@ __global__ __launch_bounds__(512) void quantize_columns_kernel(QuantParams p) {
   uint8_t* codes = p.codes + (int64_t)blockIdx.z * p.codes_b;
   uint8_t* scales = p.scales + (int64_t)blockIdx.z * p.scales_b;
   const int64_t k0 = slab * MX_SLAB + wave * 32, left = p.k - k0;
-  const int64_t r = row0 + 2 * lane;
-  const bool have0 = r < p.rows, have1 = r + 1 < p.rows;
-  raw x0[32], x1[32];
+  const int64_t r = row0 + COL_LANE * lane, rows_left = p.rows - r;
+  // the lane's 8 bytes of each k, as two words (the empty asm keeps them so: 32 x 4 unpacked elements spill)
+  uint32_t x[32][2];
   const raw* s = src + k0 * p.stride_k + r * p.stride_r;
+  const bool whole = RUNS && rows_left >= COL_LANE && left >= 32;
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
-    x0[i] = x1[i] = 0;
-    if (i < left) {
-      if (PAIRED && have1) {
-        const Pair<T> t = *(const Pair<T>*)(s + i * p.stride_k);
-        x0[i] = t.v[0];
-        x1[i] = t.v[1];
-      } else {
-        if (have0) x0[i] = s[i * p.stride_k];
-        if (have1) x1[i] = s[i * p.stride_k + p.stride_r];
-      }
+    RunC<T> t;
+    if (whole) t = *(const RunC<T>*)(s + i * p.stride_k);
+    else {
+#pragma unroll
+      for (int h = 0; h < COL_LANE; ++h) t.v[h] = i < left && h < rows_left ? s[i * p.stride_k + h * p.stride_r] : (raw)0;
     }
+    __builtin_memcpy(x[i], &t, 8);
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t top = 0;
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(x[i][0]), "+v"(x[i][1]));
+  auto element = [&](int i, int h) __attribute__((always_inline)) { return sizeof(raw) == 4 ? (raw)x[i][h & 1] : (raw)(x[i][h >> 1 & 1] >> (h & 1) * 16); };
+#pragma unroll
+  for (int h = 0; h < COL_LANE; ++h) {
+    raw top = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const uint32_t b = __builtin_bit_cast(uint32_t, Elem<T>::get(h ? x1[i] : x0[i])) & 0x7fffffffu;
+      const raw b = magnitude(element(i, h));
       top = top > b ? top : b;
     }
     float factor;
-    const uint32_t sb = left <= 0 ? 127u : scale_byte(top, &factor);
+    const uint32_t sb = left <= 0 ? 127u : scale_byte(top_bits<T>(top), &factor);
     if (left <= 0) factor = 0.0f;
     i32x4 c;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = scaled(Elem<T>::get(h ? x1[q * 8 + e] : x0[q * 8 + e]), factor);
+      for (int e = 0; e < 8; ++e) v[e] = scaled(Elem<T>::get(element(q * 8 + e, h)), factor);
       c[q] = (int)codes8(v);
     }
-    *(i32x4*)(tile + (2 * lane + h) * COL_PITCH + wave * 16) = c;
-    tile_s[(2 * lane + h) * MX_SCALEB + wave] = (uint8_t)sb;
+    *(i32x4*)(tile + (COL_LANE * lane + h) * COL_PITCH + wave * 16) = c;
+    tile_s[(COL_LANE * lane + h) * MX_SCALEB + wave] = (uint8_t)sb;
+    __builtin_amdgcn_sched_barrier(0);                   // (one row's 32 floats at a time: all four at once spill)
   }
   __syncthreads();
 #pragma unroll
@@ -196,15 +211,21 @@ __global__ __launch_bounds__(512) void quantize_columns_kernel(QuantParams p) {
     *(uint64_t*)(scales + mx_scale_at(row0 + tid, slab, p.slabs)) = *(const uint64_t*)(tile_s + tid * MX_SCALEB);
 }
 
-template <class T, bool PAIRED>
+template <class T, bool RUNS>
 __global__ __launch_bounds__(512) void dequantize_columns_kernel(QuantParams p) {
   typedef typename Elem<T>::raw raw;
+  constexpr int COL_LANE = col_lane<T>, COL_ROWS = 64 * COL_LANE;
   __shared__ __attribute__((aligned(16))) uint8_t tile[COL_ROWS * COL_PITCH];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t slab = blockIdx.y, row0 = (int64_t)blockIdx.x * COL_ROWS;
   raw* dst = (raw*)p.dst + (int64_t)blockIdx.z * p.stride_b;
   const uint8_t* codes = p.codes + (int64_t)blockIdx.z * p.codes_b;
   const uint8_t* scales = p.scales + (int64_t)blockIdx.z * p.scales_b;
+  const int64_t k0 = slab * MX_SLAB + wave * 32, left = p.k - k0;
+  const int64_t r = row0 + COL_LANE * lane, rows_left = p.rows - r;
+  float f[COL_LANE];
+#pragma unroll
+  for (int h = 0; h < COL_LANE; ++h) f[h] = h < rows_left ? scale_value(scales[mx_scale_at(r + h, slab, p.slabs) + wave]) : 0.0f;
 #pragma unroll
   for (int u = 0; u < COL_ROWS * 8 / 512; ++u) {
     const int i = u * 512 + tid, row = i >> 3, chunk = i & 7;
@@ -212,32 +233,30 @@ __global__ __launch_bounds__(512) void dequantize_columns_kernel(QuantParams p) 
       *(i32x4*)(tile + row * COL_PITCH + chunk * 16) = *(const i32x4*)(codes + ((row0 + row) * p.slabs + slab) * MX_ROWB + chunk * 16);
   }
   __syncthreads();
-  const int64_t k0 = slab * MX_SLAB + wave * 32, left = p.k - k0;
-  const int64_t r = row0 + 2 * lane;
-  const bool have0 = r < p.rows, have1 = r + 1 < p.rows;
-  if (!have0 || left <= 0) return;
-  const float f0 = scale_value(scales[mx_scale_at(r, slab, p.slabs) + wave]);
-  const float f1 = have1 ? scale_value(scales[mx_scale_at(r + 1, slab, p.slabs) + wave]) : 0.0f;
-  const i32x4 c0 = *(const i32x4*)(tile + 2 * lane * COL_PITCH + wave * 16);
-  const i32x4 c1 = *(const i32x4*)(tile + (2 * lane + (have1 ? 1 : 0)) * COL_PITCH + wave * 16);
+  if (rows_left <= 0 || left <= 0) return;
   raw* d = dst + k0 * p.stride_k + r * p.stride_r;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    float v0[8], v1[8];
-    values8((uint32_t)c0[q], f0, v0);
-    values8((uint32_t)c1[q], f1, v1);
+    float v[COL_LANE][8];
+#pragma unroll
+    for (int h = 0; h < COL_LANE; ++h)                   // (rows past the end: what LDS holds, times 0, and not stored)
+      values8(*(const uint32_t*)(tile + (COL_LANE * lane + h) * COL_PITCH + wave * 16 + q * 4), f[h], v[h]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = q * 8 + e;
       if (i >= left) continue;
-      if (PAIRED && have1) {
-        Pair<T> t;
-        t.v[0] = Elem<T>::put(v0[e]);
-        t.v[1] = Elem<T>::put(v1[e]);
-        *(Pair<T>*)(d + i * p.stride_k) = t;
+      if (RUNS && rows_left >= COL_LANE) {
+        RunC<T> t;
+#pragma unroll
+        for (int h = 0; h < COL_LANE; ++h) t.v[h] = Elem<T>::put(v[h][e]);
+        typedef i32x2 __attribute__((aligned(2))) loose2;
+        i32x2 w;
+        __builtin_memcpy(&w, &t, 8);
+        __builtin_nontemporal_store(w, (loose2*)(d + i * p.stride_k));
       } else {
-        d[i * p.stride_k] = Elem<T>::put(v0[e]);
-        if (have1) d[i * p.stride_k + p.stride_r] = Elem<T>::put(v1[e]);
+#pragma unroll
+        for (int h = 0; h < COL_LANE; ++h)
+          if (h < rows_left) d[i * p.stride_k + h * p.stride_r] = Elem<T>::put(v[h][e]);
       }
     }
   }
@@ -270,20 +289,22 @@ __global__ __launch_bounds__(256) void import_kernel(const uint8_t* codes, const
 
 template <class T, bool BACK> int launch(const QuantParams& p, hipStream_t stream) {
   if (p.stride_k == 1) {
-    const int64_t blocks = (p.rows * p.slabs * 32 + 256 * ROW_ITEMS - 1) / (256 * ROW_ITEMS);
+    const int64_t per_block = 256 * (BACK ? BACK_RUNS : QUANT_RUNS), runs = p.rows * p.slabs * (BACK && sizeof(typename Elem<T>::raw) == 4 ? 64 : 32);
+    const int64_t blocks = (runs + per_block - 1) / per_block;
     if (blocks > 0x7fffffff) return TNX_E_UNSUPPORTED;
     const dim3 grid((unsigned)blocks, (unsigned)p.batch);
     if (BACK) hipLaunchKernelGGL((dequantize_rows_kernel<T>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((quantize_rows_kernel<T>), grid, dim3(256), 0, stream, p);
+    else if (sizeof(typename Elem<T>::raw) == 2 && p.batch * p.rows * p.k > (256 << 20) / 2) hipLaunchKernelGGL((quantize_rows_kernel<T, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((quantize_rows_kernel<T, false>), grid, dim3(256), 0, stream, p);
     return mx_launched();
   }
-  const int64_t tiles = (p.rows + COL_ROWS - 1) / COL_ROWS;
+  const int64_t tiles = (p.rows + 64 * col_lane<T> - 1) / (64 * col_lane<T>);
   if (tiles > 0x7fffff || p.slabs > 65535) return TNX_E_UNSUPPORTED;
   const dim3 grid((unsigned)tiles, (unsigned)p.slabs, (unsigned)p.batch);
-  const bool paired = p.stride_r == 1;
-  if (BACK && paired) hipLaunchKernelGGL((dequantize_columns_kernel<T, true>), grid, dim3(512), 0, stream, p);
+  const bool runs = p.stride_r == 1;
+  if (BACK && runs) hipLaunchKernelGGL((dequantize_columns_kernel<T, true>), grid, dim3(512), 0, stream, p);
   else if (BACK) hipLaunchKernelGGL((dequantize_columns_kernel<T, false>), grid, dim3(512), 0, stream, p);
-  else if (paired) hipLaunchKernelGGL((quantize_columns_kernel<T, true>), grid, dim3(512), 0, stream, p);
+  else if (runs) hipLaunchKernelGGL((quantize_columns_kernel<T, true>), grid, dim3(512), 0, stream, p);
   else hipLaunchKernelGGL((quantize_columns_kernel<T, false>), grid, dim3(512), 0, stream, p);
   return mx_launched();
 }
