@@ -347,6 +347,310 @@ PyObject* stream_of(PyObject*, PyObject* arg) {
   return PyLong_FromUnsignedLongLong((unsigned long long)(uintptr_t)c10::hip::getCurrentHIPStream((c10::DeviceIndex)index).stream());
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------
+// Microscaled products and routing.  These calls have nothing to keep between them: the kernels' choice is the library's host arithmetic.
+// What is saved is the interpreter's work around them, checks, torch.empty and the filling of structs: one token's routing 16.5 us -> 0, its
+// product 10 -> 0, an ordinary product with its quantisation 16 -> 0.  As above, None hands the call to the ordinary path, which
+// raises what is to be raised; a status other than TNX_OK does too (nothing is left behind by such a launch).
+struct OpEntries {
+  size_t (*code_bytes)(int64_t, int64_t);
+  size_t (*scale_bytes)(int64_t, int64_t);
+  int (*quantize)(const tnx_mx_args*);
+  int (*dequantize)(const tnx_mx_args*);
+  int (*takes_rows)(int64_t, int64_t);
+  int (*gemm)(const tnx_mx_gemm_args*);
+  size_t (*workspace_bytes)(int64_t, int32_t, int32_t);
+  int (*route)(const tnx_moe_args*);
+  int (*backward)(const tnx_moe_args*);
+  int (*combine)(const void*, const int32_t*, const float*, void*, int64_t, int32_t, int64_t, int32_t, int32_t, void*);
+} ops = {};
+
+// bind_ops(addresses of the above, in their order)
+PyObject* bind_ops(PyObject*, PyObject* arg) {
+  constexpr int N = sizeof(OpEntries) / sizeof(void*);
+  if (!PyTuple_Check(arg) || PyTuple_GET_SIZE(arg) != N) {
+    PyErr_SetString(PyExc_ValueError, "bind_ops: not the entry points");
+    return nullptr;
+  }
+  void* at[N];
+  for (int i = 0; i < N; ++i) at[i] = (void*)(uintptr_t)PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(arg, i));
+  if (PyErr_Occurred()) return nullptr;
+  static_assert(sizeof ops == sizeof at, "one pointer each");
+  std::memcpy(&ops, at, sizeof ops);
+  Py_RETURN_NONE;
+}
+
+// tnx_dtype of a float type that has kernels, or -1
+int float_code(at::ScalarType t) {
+  return t == at::kHalf ? TNX_F16 : t == at::kBFloat16 ? TNX_BF16 : t == at::kFloat ? TNX_F32 : -1;
+}
+at::ScalarType type_of(int code) { return code == TNX_F16 ? at::kHalf : code == TNX_BF16 ? at::kBFloat16 : at::kFloat; }
+
+// integers from Python objects; false: not integers (and no error set)
+template <int N> bool integers(PyObject* const* args, int64_t (&out)[N]) {
+  for (int i = 0; i < N; ++i) {
+    if (!PyLong_Check(args[i])) return false;
+    out[i] = PyLong_AsLongLong(args[i]);
+  }
+  if (!PyErr_Occurred()) return true;
+  PyErr_Clear();
+  return false;
+}
+
+// a dense tensor of the current device; what it is for may be asked of it
+bool here(PyObject* o, int64_t dim, const at::Tensor** t, c10::DeviceIndex* device) {
+  if (!own_tensor(o)) return false;
+  const at::Tensor& x = THPVariable_Unpack(o);
+  if (!plain(x, dim)) return false;
+  if (*device < 0) *device = (c10::DeviceIndex)x.get_device();
+  *t = &x;
+  return x.get_device() == *device && c10::hip::current_device() == *device;
+}
+
+// buffer of a quantised matrix of `rows` rows of k: codes, then scales
+struct Quantised {
+  at::Tensor buffer;
+  int64_t code_bytes = 0;
+  int status = TNX_OK;
+};
+Quantised quantised(const at::Tensor& x, bool along_last, c10::DeviceIndex device, void* stream) {
+  const int64_t rows = x.size(along_last ? 0 : 1), k = x.size(along_last ? 1 : 0);
+  Quantised q;
+  q.code_bytes = (int64_t)ops.code_bytes(rows, k);
+  q.buffer = fresh({q.code_bytes + (int64_t)ops.scale_bytes(rows, k)}, at::kByte, device);
+  tnx_mx_args a = {};
+  a.data = x.data_ptr();
+  a.codes = q.buffer.data_ptr();
+  a.scales = (uint8_t*)a.codes + q.code_bytes;
+  a.batch = 1; a.rows = rows; a.k = k;
+  a.stride_row = x.stride(along_last ? 0 : 1); a.stride_k = x.stride(along_last ? 1 : 0);
+  a.dtype = float_code(x.scalar_type());
+  a.stream = stream;
+  q.status = ops.quantize(&a);
+  return q;
+}
+
+// mx_quantize(x, along its last dimension) -> (buffer, bytes of codes), or None
+PyObject* mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2) Py_RETURN_NONE;
+  try {
+    const at::Tensor* x;
+    c10::DeviceIndex device = -1;
+    if (!here(args[0], 2, &x, &device) || float_code(x->scalar_type()) < 0) Py_RETURN_NONE;
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    const bool along_last = PyObject_IsTrue(args[1]) == 1;
+    Quantised q;
+    {
+      const Unlocked unlocked;
+      q = quantised(*x, along_last, device, stream);
+    }
+    if (q.status != TNX_OK) Py_RETURN_NONE;
+    const Object t = taken(THPVariable_Wrap(q.buffer)), bytes = taken(PyLong_FromLongLong(q.code_bytes));
+    if (!t.p || !bytes.p) return nullptr;
+    return PyTuple_Pack(2, t.p, bytes.p);
+  } catch (...) {
+    return none();
+  }
+}
+
+// mx_dequantize(buffer, bytes of codes, rows, k, along its last dimension, tnx_dtype) -> the matrix, or None
+PyObject* mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) Py_RETURN_NONE;
+  try {
+    const at::Tensor* b;
+    c10::DeviceIndex device = -1;
+    int64_t v[5];
+    if (!here(args[0], 1, &b, &device) || !integers(args + 1, v) || v[1] < 0 || v[2] < 0) Py_RETURN_NONE;
+    tnx_mx_args a = {};
+    a.codes = b->data_ptr();
+    a.scales = (uint8_t*)a.codes + v[0];
+    a.batch = 1; a.rows = v[1]; a.k = v[2];
+    const bool along_last = v[3] != 0;
+    a.stride_row = along_last ? v[2] : 1; a.stride_k = along_last ? 1 : v[1];
+    a.dtype = (int32_t)v[4];
+    a.stream = c10::hip::getCurrentHIPStream(device).stream();
+    at::Tensor out;
+    int status;
+    {
+      const Unlocked unlocked;
+      out = fresh({along_last ? v[1] : v[2], along_last ? v[2] : v[1]}, type_of(a.dtype), device);
+      a.data = out.data_ptr();
+      status = ops.dequantize(&a);
+    }
+    if (status != TNX_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(out);
+  } catch (...) {
+    return none();
+  }
+}
+
+// mx_product(a, buffer, bytes of codes, n, k, epilogue[, experts, top_k, offsets, order or None, rows or None, weights or None]) -> the product of
+// the rows of a, quantised on the way in, or None.  With experts: of `order`'s pairs (gathered), or of a's rows as they lie, and
+// with rows and weights the join of it
+PyObject* mx_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6 && n != 12) Py_RETURN_NONE;
+  try {
+    const at::Tensor *a, *b, *offsets = nullptr, *order = nullptr, *rows = nullptr, *weights = nullptr;
+    c10::DeviceIndex device = -1;
+    int64_t v[4], ev[2] = {0, 1};
+    if (!here(args[0], 2, &a, &device) || !here(args[1], 1, &b, &device) || !integers(args + 2, v)) Py_RETURN_NONE;
+    const int code = float_code(a->scalar_type());
+    const int64_t k = v[2], epilogue = v[3];
+    if (code < 0 || a->size(1) != k || k <= 0 || (epilogue != TNX_EPI_NONE && v[1] % 2)) Py_RETURN_NONE;
+    if (n == 12) {
+      const int64_t most = a->size(0);
+      if (!integers(args + 6, ev) || ev[0] <= 0 || ev[1] <= 0 || !here(args[8], 1, &offsets, &device) || offsets->numel() != ev[0] + 1 ||
+          offsets->scalar_type() != at::kInt || !offsets->is_contiguous())
+        Py_RETURN_NONE;
+      if (args[9] != Py_None && (!here(args[9], 1, &order, &device) || order->numel() != most * ev[1] || order->scalar_type() != at::kInt || !order->is_contiguous()))
+        Py_RETURN_NONE;
+      if (args[10] != Py_None) {
+        if (order || !here(args[10], 2, &rows, &device) || !here(args[11], 2, &weights, &device) || rows->numel() != most || rows->size(1) != ev[1] ||
+            weights->sizes() != rows->sizes() || rows->scalar_type() != at::kInt || weights->scalar_type() != at::kFloat || !rows->is_contiguous() ||
+            !weights->is_contiguous())
+          Py_RETURN_NONE;
+      }
+    }
+    tnx_mx_gemm_args g = {};
+    g.b_codes = b->data_ptr();
+    g.b_scales = (const uint8_t*)g.b_codes + v[0];
+    g.a_rows = a->size(0);
+    g.m = order ? order->numel() : g.a_rows;
+    g.n = v[1]; g.k = k;
+    g.stride_out = epilogue != TNX_EPI_NONE ? g.n / 2 : g.n;
+    g.out_dtype = code; g.epilogue = (int32_t)epilogue;
+    if (n == 12) {
+      g.experts = (int32_t)ev[0]; g.top_k = (int32_t)ev[1];
+      g.offsets = (const int32_t*)offsets->data_ptr();
+      g.order = order ? (const int32_t*)order->data_ptr() : nullptr;
+    }
+    g.stream = c10::hip::getCurrentHIPStream(device).stream();
+    at::Tensor out, joined;
+    int status;
+    {
+      const Unlocked unlocked;
+      Quantised q;
+      if ((a->stride(1) == 1 || k == 1) && ops.takes_rows(g.a_rows, k)) {
+        g.a_data = a->data_ptr(); g.a_dtype = code; g.stride_a = a->stride(0);
+      } else {
+        q = quantised(*a, true, device, g.stream);
+        g.a_codes = q.buffer.data_ptr();
+        g.a_scales = (const uint8_t*)g.a_codes + q.code_bytes;
+      }
+      out = fresh({g.m, g.stride_out}, a->scalar_type(), device);
+      g.out = out.data_ptr();
+      status = q.status != TNX_OK ? q.status : ops.gemm(&g);
+      if (status == TNX_OK && rows) {
+        joined = fresh({rows->size(0), g.n}, a->scalar_type(), device);
+        status = ops.combine(out.data_ptr(), (const int32_t*)rows->data_ptr(), (const float*)weights->data_ptr(), joined.data_ptr(), rows->size(0),
+                             (int32_t)rows->size(1), g.n, code, code, g.stream);
+      }
+    }
+    if (status != TNX_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(rows ? joined : out);
+  } catch (...) {
+    return none();
+  }
+}
+
+// moe_route(logits, bias or None, top_k, scoring, num_groups, top_groups, group_top, renormalize, scale) -> (weights, experts, offsets, order,
+// rows), or None
+PyObject* moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9 || !PyFloat_Check(args[8])) Py_RETURN_NONE;
+  try {
+    const at::Tensor *logits, *bias = nullptr;
+    c10::DeviceIndex device = -1;
+    int64_t v[6];
+    if (!here(args[0], 2, &logits, &device) || !integers(args + 2, v)) Py_RETURN_NONE;
+    if (args[1] != Py_None && (!here(args[1], 1, &bias, &device) || !bias->is_contiguous() || bias->scalar_type() != at::kFloat || bias->numel() != logits->size(1)))
+      Py_RETURN_NONE;
+    const int64_t tokens = logits->size(0), experts = logits->size(1), top_k = v[0];
+    if (float_code(logits->scalar_type()) < 0 || experts < 1 || experts > TNX_MOE_MAX_EXPERTS || top_k < 1 || top_k > experts ||
+        top_k > TNX_MOE_MAX_TOP_K || (logits->stride(1) != 1 && experts > 1))
+      Py_RETURN_NONE;
+    tnx_moe_args a = {};
+    a.logits = logits->data_ptr();
+    a.bias = bias ? (const float*)bias->data_ptr() : nullptr;
+    a.tokens = tokens; a.stride_logits = logits->stride(0);
+    a.num_experts = (int32_t)experts; a.top_k = (int32_t)top_k; a.dtype = float_code(logits->scalar_type());
+    a.scoring = (int32_t)v[1]; a.num_groups = (int32_t)v[2]; a.top_groups = (int32_t)v[3]; a.group_top = (int32_t)v[4]; a.renormalize = (int32_t)v[5];
+    a.scale = (float)PyFloat_AS_DOUBLE(args[8]);
+    a.stream = c10::hip::getCurrentHIPStream(device).stream();
+    at::Tensor weights, chosen, offsets, order, rows;
+    int status;
+    {
+      const Unlocked unlocked;
+      weights = fresh({tokens, top_k}, at::kFloat, device);
+      chosen = fresh({tokens, top_k}, at::kInt, device);
+      offsets = fresh({experts + 1}, at::kInt, device);
+      order = fresh({tokens * top_k}, at::kInt, device);
+      rows = fresh({tokens, top_k}, at::kInt, device);
+      at::Tensor scratch;
+      const size_t bytes = ops.workspace_bytes(tokens, a.top_k, a.num_experts);
+      if (bytes) {
+        scratch = fresh({(int64_t)bytes}, at::kByte, device);
+        a.workspace = scratch.data_ptr();
+        a.workspace_bytes = bytes;
+      }
+      a.weights = (float*)weights.data_ptr();
+      a.experts = (int32_t*)chosen.data_ptr();
+      a.offsets = (int32_t*)offsets.data_ptr();
+      a.order = (int32_t*)order.data_ptr();
+      a.rows = (int32_t*)rows.data_ptr();
+      status = ops.route(&a);
+    }
+    if (status != TNX_OK) Py_RETURN_NONE;
+    const Object o[5] = {taken(THPVariable_Wrap(weights)), taken(THPVariable_Wrap(chosen)), taken(THPVariable_Wrap(offsets)),
+                         taken(THPVariable_Wrap(order)), taken(THPVariable_Wrap(rows))};
+    for (const Object& x : o)
+      if (!x.p) return nullptr;
+    return PyTuple_Pack(5, o[0].p, o[1].p, o[2].p, o[3].p, o[4].p);
+  } catch (...) {
+    return none();
+  }
+}
+
+// moe_backward(grad, logits, weights, experts, scoring, renormalize, scale) -> gradient of the logits, or None
+PyObject* moe_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7 || !PyFloat_Check(args[6])) Py_RETURN_NONE;
+  try {
+    const at::Tensor *grad, *logits, *weights, *chosen;
+    c10::DeviceIndex device = -1;
+    int64_t v[2];
+    if (!here(args[0], 2, &grad, &device) || !here(args[1], 2, &logits, &device) || !here(args[2], 2, &weights, &device) ||
+        !here(args[3], 2, &chosen, &device) || !integers(args + 4, v))
+      Py_RETURN_NONE;
+    const int64_t tokens = logits->size(0), experts = logits->size(1);
+    if (grad->sizes() != weights->sizes() || chosen->sizes() != weights->sizes() || weights->size(0) != tokens || grad->scalar_type() != at::kFloat ||
+        weights->scalar_type() != at::kFloat || chosen->scalar_type() != at::kInt || !grad->is_contiguous() || !weights->is_contiguous() ||
+        !chosen->is_contiguous() || (logits->stride(1) != 1 && experts > 1) || float_code(logits->scalar_type()) < 0)
+      Py_RETURN_NONE;
+    tnx_moe_args a = {};
+    a.logits = logits->data_ptr();
+    a.weights = (float*)weights->data_ptr();
+    a.experts = (int32_t*)chosen->data_ptr();
+    a.grad = (const float*)grad->data_ptr();
+    a.tokens = tokens; a.stride_logits = logits->stride(0);
+    a.num_experts = (int32_t)experts; a.top_k = (int32_t)weights->size(1); a.dtype = float_code(logits->scalar_type());
+    a.scoring = (int32_t)v[0]; a.renormalize = (int32_t)v[1];
+    a.num_groups = a.top_groups = a.group_top = 1;
+    a.scale = (float)PyFloat_AS_DOUBLE(args[6]);
+    a.stream = c10::hip::getCurrentHIPStream(device).stream();
+    at::Tensor out;
+    int status;
+    {
+      const Unlocked unlocked;
+      out = fresh({tokens, experts}, logits->scalar_type(), device);
+      a.grad_logits = out.data_ptr();
+      status = ops.backward(&a);
+    }
+    if (status != TNX_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(out);
+  } catch (...) {
+    return none();
+  }
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
     {"keep", keep, METH_VARARGS, nullptr},
@@ -356,6 +660,12 @@ PyMethodDef methods[] = {
     {"forget", forget, METH_NOARGS, nullptr},
     {"forget_convs", forget_convs, METH_NOARGS, nullptr},
     {"stream_of", stream_of, METH_O, nullptr},
+    {"bind_ops", bind_ops, METH_O, nullptr},
+    {"mx_quantize", (PyCFunction)(void (*)(void))mx_quantize, METH_FASTCALL, nullptr},
+    {"mx_dequantize", (PyCFunction)(void (*)(void))mx_dequantize, METH_FASTCALL, nullptr},
+    {"mx_product", (PyCFunction)(void (*)(void))mx_product, METH_FASTCALL, nullptr},
+    {"moe_route", (PyCFunction)(void (*)(void))moe_route, METH_FASTCALL, nullptr},
+    {"moe_backward", (PyCFunction)(void (*)(void))moe_backward, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -16,6 +16,7 @@ from typing import Optional
 import torch
 
 from tritonix_amd import _C
+from tritonix_amd.ops import mx as _mx
 from tritonix_amd.ops.mx import MXTensor, dtype_code, epilogue_of, gemm_args, launch, on_device, operand, raise_for_status, takes_rows
 from tritonix_amd.kernel import _stream_of
 
@@ -152,6 +153,12 @@ def moe_route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: 
     them).  A row with a NaN (softmax: or +inf) gets experts -1 and NaN weights.  ``weights`` carries a gradient if ``logits`` does; the choice is held fixed."""
     if logits.dim() != 2:
         raise ValueError(f"moe_route expects logits[t,e], got {tuple(logits.shape)}")
+    renormalize, scale = bool(renormalize), float(scale)
+    number = _SCORING.get(scoring)
+    if number is not None and (group_top == 1 or bias is not None) and not (logits.requires_grad and torch.is_grad_enabled()):
+        out = (_mx.native or _mx.find_native()).moe_route(logits, bias, top_k, number, num_groups, top_groups, group_top, renormalize, scale)
+        if out is not None:
+            return Routing(*out, logits.shape[1], scoring, renormalize, scale)
     tokens, num_experts = logits.shape
     _check_counts("moe_route", top_k, num_experts)
     if top_k > num_experts:
@@ -170,15 +177,18 @@ def moe_route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: 
         logits = logits.contiguous()
     if bias is not None:
         bias = bias.detach().contiguous()
-    options = (scoring, num_groups, top_groups, group_top, bool(renormalize), float(scale))
+    options = (scoring, num_groups, top_groups, group_top, renormalize, scale)
     if logits.requires_grad and torch.is_grad_enabled():
         out = _Route.apply(logits, bias, top_k, options)
     else:
         out = _route(logits, bias, top_k, options)
-    return Routing(*out, num_experts, scoring, bool(renormalize), float(scale))
+    return Routing(*out, num_experts, scoring, renormalize, scale)
 
 
 def _backward(grad, logits, weights, experts, options):
+    out = (_mx.native or _mx.find_native()).moe_backward(grad, logits, weights, experts, _SCORING[options[0]], options[4], options[5])
+    if out is not None:
+        return out
     index = on_device("moe_route_backward", grad, logits, weights, experts)
     a = _route_args(logits, None, experts.shape[1], options)
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -221,6 +231,11 @@ def _grouped(name: str, x, w: MXTensor, routing: Routing, out: torch.Tensor, gat
 def moe_glu(x, w12: MXTensor, routing: Routing, activation: str = "silu", out_dtype=None) -> torch.Tensor:
     """Gated up-projections of each token's experts: row r of the result, ``[t * k, f]``, belongs to the pair ``routing.order[r]``; rows
     of empty slots come last and are zero.  ``x[t, d]`` is a torch tensor or an ``MXTensor``, ``w12`` an ``MXTensor`` ``[e, d, 2f]``."""
+    if out_dtype is None and type(w12) is MXTensor and w12.batch == routing.num_experts and w12.dim == -2 and x.shape[:1] == (routing.tokens,):
+        out = (_mx.native or _mx.find_native()).mx_product(x, w12.buffer, w12.code_bytes, w12.rows, w12.k, epilogue_of(activation), routing.num_experts,
+                                                           routing.top_k, routing.offsets, routing.order, None, None)
+        if out is not None:
+            return out
     _check_experts("moe_glu", x, w12, routing, routing.tokens)
     if w12.rows % 2:
         raise ValueError("the interleaved weight must have an even number of columns")
@@ -239,6 +254,11 @@ def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
 
     The products are rounded to the result's type before the join (they are k times the result's size, and the join is bound by
     reading them); the join sums in 32 bits."""
+    if out_dtype is None and type(w3) is MXTensor and w3.batch == routing.num_experts and w3.dim == -2:
+        out = (_mx.native or _mx.find_native()).mx_product(h, w3.buffer, w3.code_bytes, w3.rows, w3.k, _C.EPI_NONE, routing.num_experts, routing.top_k,
+                                                           routing.offsets, None, routing.rows, routing.weights)
+        if out is not None:
+            return out
     _check_experts("moe_down", h, w3, routing, routing.tokens * routing.top_k)
     if out_dtype is None:
         out_dtype = torch.bfloat16 if isinstance(h, MXTensor) else h.dtype

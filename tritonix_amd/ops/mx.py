@@ -18,7 +18,7 @@ from typing import Optional, Tuple
 import torch
 
 from tritonix_amd import _C
-from tritonix_amd.kernel import _stream_of
+from tritonix_amd.kernel import _stream_of, launch_module
 
 __all__ = ["MXTensor", "mx_quantize", "mx_dequantize", "mx_matmul", "mx_glu", "mx_linear"]
 
@@ -26,6 +26,34 @@ BLOCK = 32
 SLAB = 256                      # k is padded to whole slabs (csrc/mx.h)
 _DTYPES = {torch.float16: _C.F16, torch.bfloat16: _C.BF16, torch.float32: _C.F32}
 _EPILOGUES = {"silu": _C.EPI_GLU_SILU, "sigmoid": _C.EPI_GLU_SIGMOID}
+
+
+class _Interpreter:
+    """Stands in for ``_launch`` where it cannot be used: every call takes the ordinary path below."""
+
+    @staticmethod
+    def _none(*_):
+        return None
+
+    mx_quantize = mx_dequantize = mx_product = moe_route = moe_backward = _none
+
+
+# csrc/launch.cpp, which makes the ordinary calls without the interpreter's share of them; found with the first call
+native = None
+
+
+def find_native():
+    global native
+    module = launch_module()
+    if module is None:
+        native = _Interpreter
+    else:
+        lib = _C.load()
+        module.bind_ops(tuple(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+            lib.tnx_mx_code_bytes, lib.tnx_mx_scale_bytes, lib.tnx_mx_quantize, lib.tnx_mx_dequantize, lib.tnx_mx_gemm_takes_rows, lib.tnx_mx_gemm,
+            lib.tnx_moe_workspace_bytes, lib.tnx_moe_route, lib.tnx_moe_route_backward, lib.tnx_moe_combine)))
+        native = module
+    return native
 
 
 def dtype_code(name: str, dtype) -> int:
@@ -177,6 +205,12 @@ def mx_quantize(x: torch.Tensor, dim: int = -1) -> MXTensor:
 
     A block's scale is 2^(floor(log2 of its largest magnitude) - 2); elements round to the nearest 4-bit float, ties to
     the even code, and those past 6 scales to 6.  A block with an infinity or a NaN becomes NaN throughout."""
+    if dim in (0, 1, -1, -2):
+        last = dim in (1, -1)
+        got = (native or find_native()).mx_quantize(x, last)             # (a matrix of the current device)
+        if got is not None:
+            m, n = x.shape
+            return MXTensor(got[0], None, m if last else n, n if last else m, -1 if last else -2, got[1])
     if x.dim() not in (2, 3):
         raise ValueError(f"mx_quantize expects a matrix or a batch of them, got {tuple(x.shape)}")
     dim = _dim("mx_quantize", dim, x.dim())
@@ -191,6 +225,10 @@ def mx_quantize(x: torch.Tensor, dim: int = -1) -> MXTensor:
 def mx_dequantize(t: MXTensor, dtype=torch.bfloat16) -> torch.Tensor:
     """The values that ``t`` stands for, contiguous in its logical shape.  (Exact in bfloat16 and float32.)"""
     code = dtype_code("mx_dequantize", dtype)
+    if t.batch is None:
+        out = (native or find_native()).mx_dequantize(t.buffer, t.code_bytes, t.rows, t.k, int(t.dim == -1), code)
+        if out is not None:
+            return out
     index = on_device("mx_dequantize", t)
     out = torch.empty(t.shape, dtype=dtype, device=t.device)
     launch("mx_dequantize", index, _C.load().tnx_mx_dequantize, _mx_args(out, t, code))
@@ -227,6 +265,12 @@ def gemm_args(a, b: MXTensor, out: torch.Tensor, epilogue: int) -> _C.MxGemmArgs
 
 
 def _product(name: str, a, b, out_dtype, epilogue: int) -> torch.Tensor:
+    if type(b) is not MXTensor and not isinstance(a, MXTensor) and len(a.shape) == len(b.shape) == 2 and a.shape[1] == b.shape[0]:
+        b = mx_quantize(b, dim=0)
+    if type(b) is MXTensor and b.batch is None and b.dim == -2 and (out_dtype is None or out_dtype is getattr(a, "dtype", None)):
+        out = (native or find_native()).mx_product(a, b.buffer, b.code_bytes, b.rows, b.k, epilogue)
+        if out is not None:
+            return out
     if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[0]:
         raise ValueError(f"{name} expects a[m,k] and b[k,n], got {tuple(a.shape)} and {tuple(b.shape)}")
     if out_dtype is None:
