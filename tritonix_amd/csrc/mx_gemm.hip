@@ -136,18 +136,19 @@ __device__ __forceinline__ void store_columns(const MxParams& p, int64_t row, in
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Tiles: BN columns of the output (rows of the weights) x BM rows, WGN x WGM waves, slabs of 256 k in two LDS buffers
+// Tiles: BN columns of the output (rows of the weights) x BM rows, WGN x WGM waves, slabs of 256 k in a ring of S LDS buffers
 // filled by direct loads.  Slab s + 1 has to be there, and slab s be read by all, when the last step of slab s
-// begins: one barrier per slab, its wait hidden behind that step's products.
-template <int BN_, int BM_, int WGN, int WGM> struct MxTile {
-  static constexpr int BN = BN_, BM = BM_, NW = WGN * WGM, THREADS = NW * 64, WAVES_N = WGN;
+// begins: one barrier per slab, its wait hidden behind that step's products.  Slab s + S then goes where s was.
+template <int BN_, int BM_, int WGN, int WGM, int S_> struct MxTile {
+  static constexpr int BN = BN_, BM = BM_, NW = WGN * WGM, THREADS = NW * 64, WAVES_N = WGN, S = S_;
   static constexpr int WTN = BN / WGN, WTM = BM / WGM, TN = WTN / 32, TM = WTM / 32;
   static constexpr int B_BYTES = BN * MX_ROWB, A_BYTES = BM * MX_ROWB;
   static constexpr int SLOT = B_BYTES + A_BYTES, S_BYTES = (BN + BM) * 2 * MX_SCALEB;      // codes of a slab; scales of two
   static constexpr int B_OPS = B_BYTES / (1024 * NW), A_OPS = A_BYTES / (1024 * NW);      // 16-byte loads per lane and slab
-  static constexpr int LDS = 2 * SLOT + 2 * S_BYTES;
+  static constexpr int LDS = S * (SLOT + S_BYTES);       // (slabs s .. s + S are of S / 2 + 1 pairs: S buffers are enough)
   // waves per SIMD that the LDS leaves room for
   static constexpr int OCC = (163840 / LDS) * NW / 4;
+  static_assert((S & (S - 1)) == 0 && S >= 2 && LDS <= 163840, "a ring of 2, 4, 8 buffers");
 };
 
 // x: words of an even q, y: of the odd q after it.  Lanes 0-31 keep x and get its upper lanes' as y; lanes 32-63 the same of y.
@@ -215,7 +216,7 @@ __device__ __forceinline__ void store_product(const f32x16& v, uint8_t* out, int
 
 template <class C, bool EXPERTS, class O, bool GLU>
 __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_kernel(MxParams p) {
-  constexpr int BN = C::BN, BM = C::BM, NW = C::NW;
+  constexpr int BN = C::BN, BM = C::BM, NW = C::NW, S = C::S;
   extern __shared__ __attribute__((aligned(1024))) uint8_t mx_smem[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(uint8_t __attribute__((address_space(3)))*)mx_smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
   // one slab is OPS loads of a wave: op q of them (a constant after unrolling) into the slab's buffer
   constexpr int OPS = C::B_OPS + C::A_OPS + 1;
   auto fetch_op = [&](int slab, int q) __attribute__((always_inline)) {
-    const uint32_t slot = lds0 + (slab & 1) * C::SLOT;
+    const uint32_t slot = lds0 + (slab & (S - 1)) * C::SLOT;
     if (q < C::B_OPS) dma16_from(b + (int64_t)slab * MX_ROWB, b_off[q], slot + (NW * q + wave) * 1024);
     else if (q < C::B_OPS + C::A_OPS) {
       const int i = q - C::B_OPS;
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
       if (EXPERTS) dma16_at(a_at[i] + (int64_t)slab * MX_ROWB, to);
       else dma16_from(a + (int64_t)slab * MX_ROWB, a_off[i], to);
     } else if ((slab & 1) == 0 && wave < S_WAVES) {
-      dma16_at(s_at + (int64_t)(slab >> 1) * 512, lds0 + 2 * C::SLOT + (slab >> 1 & 1) * C::S_BYTES + wave * 1024);
+      dma16_at(s_at + (int64_t)(slab >> 1) * 512, lds0 + S * C::SLOT + (slab >> 1 & (S - 1)) * C::S_BYTES + wave * 1024);
     }
   };
 
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
   // place of chunk 4 half + step in this lane's row; the weights' and a's products further on are constants from here
   const uint32_t place = (uint32_t)r32 * MX_ROWB + (((4 * half) ^ ((r32 >> 1) & 7)) << 4);
   const uint32_t place_b = lds0 + place + wn * MX_ROWB, place_a = lds0 + place + C::B_BYTES + wm * MX_ROWB;
-  const uint32_t place_s = lds0 + 2 * C::SLOT + r32 * 2 * MX_SCALEB + half * 4;
+  const uint32_t place_s = lds0 + S * C::SLOT + r32 * 2 * MX_SCALEB + half * 4;
   constexpr int NM = C::TN * C::TM;
   f32x16 acc[C::TN][C::TM];
 #pragma unroll
@@ -335,16 +336,21 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
   constexpr int STRIDE = ROOM / OPS > 0 ? ROOM / OPS : 1, DPER = (OPS * STRIDE + ROOM - 1) / ROOM;
   constexpr int FIRST_OPS = (EARLY + STRIDE - 1) / STRIDE * DPER < C::B_OPS + C::A_OPS ? (EARLY + STRIDE - 1) / STRIDE * DPER : C::B_OPS + C::A_OPS;
   constexpr int PER = (C::TN + EARLY - 1) / EARLY;
-  auto products = [&](int s, auto next_tag, auto fetch_tag) __attribute__((always_inline)) {
-    constexpr bool NEXT = decltype(next_tag)::value, FETCH = decltype(fetch_tag)::value;
-    const uint32_t slot = (s & 1) * C::SLOT, other = C::SLOT - slot, scales = ((s + 1) >> 1 & 1) * C::S_BYTES + ((s + 1) & 1) * MX_SCALEB;
+  // NEXT: there is a slab s + 1.  LATE: slab s + S - 1 is there, and the rest of its loads go out; FETCH: slab s + S is, and its first do.
+  auto products = [&](int s, auto next_tag, auto late_tag, auto fetch_tag) __attribute__((always_inline)) {
+    constexpr bool NEXT = decltype(next_tag)::value, LATE = decltype(late_tag)::value, FETCH = decltype(fetch_tag)::value;
+    const uint32_t slot = (s & (S - 1)) * C::SLOT, other = ((s + 1) & (S - 1)) * C::SLOT;
+    const uint32_t scales = ((s + 1) >> 1 & (S - 1)) * C::S_BYTES + ((s + 1) & 1) * MX_SCALEB;
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
 #pragma unroll
       for (int e = 0; e < NM; ++e) {
         if (NEXT && step == 3 && e == BAR) {
-          // the fragments of this slab are in registers and the loads of the next one have landed, in every wave
-          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          // The fragments of this slab are in registers and the loads of the next one have landed, in every wave.  (Younger are at least the code
+          // loads of the S - 2 slabs after it, where those exist.)
+          if (FETCH) TNX_WAIT_VM((S - 2) * (OPS - 1));
+          else TNX_WAIT_VM(0);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
           __builtin_amdgcn_sched_barrier(0);
@@ -363,12 +369,12 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
           if (BAR > 0 && e == BAR) { read_a(other, 0, 0); read_sa(scales, 0); }
           if (e % C::TN == C::TN - 1) { read_a(other, 0, j); read_sa(scales, j); }
         }
-        if (step == 3 ? FETCH && e >= BAR : NEXT) {
+        if (step == 3 ? FETCH && e >= BAR : LATE) {
           const int at = step == 3 ? e - BAR : EARLY + step * NM + e;
           if (at % STRIDE == 0) {
 #pragma unroll
             for (int q = at / STRIDE * DPER; q < at / STRIDE * DPER + DPER; ++q)
-              if (step == 3 ? q < FIRST_OPS : q >= FIRST_OPS && q < OPS) fetch_op(step == 3 ? s + 2 : s + 1, q);
+              if (step == 3 ? q < FIRST_OPS : q >= FIRST_OPS && q < OPS) fetch_op(step == 3 ? s + S : s + S - 1, q);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -381,12 +387,17 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
   };
 
   const int slabs = p.slabs;
+  static_assert((S - 2) * (OPS - 1) + FIRST_OPS < 64, "the counter of loads in flight");
 #pragma unroll
-  for (int q = 0; q < OPS; ++q) fetch_op(0, q);
-  if (slabs > 1) {
+  for (int t = 0; t < S - 1; ++t)
+    if (t < slabs) {
 #pragma unroll
-    for (int q = 0; q < FIRST_OPS; ++q) fetch_op(1, q);
-    TNX_WAIT_VM(FIRST_OPS);                // (these go out in every wave: what is older has landed)
+      for (int q = 0; q < OPS; ++q) fetch_op(t, q);
+    }
+  if (slabs >= S) {
+#pragma unroll
+    for (int q = 0; q < FIRST_OPS; ++q) fetch_op(S - 1, q);
+    TNX_WAIT_VM((S - 2) * (OPS - 1) + FIRST_OPS);          // (these go out in every wave: what is older has landed)
   } else {
     TNX_WAIT_VM(0);
   }
@@ -399,22 +410,28 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
     // A wave without rows (an expert's last tile, mostly) does its share of the loads and keeps the barriers; the wave of the other half on
     // its SIMD has the matrix unit to itself.
     for (int s = 0; s < slabs - 1; ++s) {
+      if (s + S - 1 < slabs) {
 #pragma unroll
-      for (int q = FIRST_OPS; q < OPS; ++q) fetch_op(s + 1, q);
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        for (int q = FIRST_OPS; q < OPS; ++q) fetch_op(s + S - 1, q);
+      }
+      if (s + S < slabs) TNX_WAIT_VM((S - 2) * (OPS - 1));
+      else TNX_WAIT_VM(0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (s + 2 < slabs) {
+      if (s + S < slabs) {
 #pragma unroll
-        for (int q = 0; q < FIRST_OPS; ++q) fetch_op(s + 2, q);
+        for (int q = 0; q < FIRST_OPS; ++q) fetch_op(s + S, q);
       }
     }
     return;
   }
   int s = 0;
-  for (; s < slabs - 2; ++s) products(s, BoolTag<true>(), BoolTag<true>());
-  if (s < slabs - 1) products(s++, BoolTag<true>(), BoolTag<false>());
-  products(s, BoolTag<false>(), BoolTag<false>());
+  for (; s < slabs - S; ++s) products(s, BoolTag<true>(), BoolTag<true>(), BoolTag<true>());
+  if (s == slabs - S) products(s++, BoolTag<true>(), BoolTag<true>(), BoolTag<false>());
+  if (S > 2)
+    for (; s < slabs - 1; ++s) products(s, BoolTag<true>(), BoolTag<false>(), BoolTag<false>());
+  products(s, BoolTag<false>(), BoolTag<false>(), BoolTag<false>());
 
   // Epilogue, from the registers (LDS is not touched: nothing waits for the other waves).  The sums stay where the matrix instructions
   // left them until their turn: without the empty asm all 256 are copied out at once, to scratch memory for the most part.
@@ -436,7 +453,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Few rows: bound by streaming the weights, so nothing of them goes through LDS.  A wave has 16 NT rows of the weights and up to 16 MT rows of a; a
+// Few rows: bound by streaming the weights, so nothing of them goes through LDS.  A wave has 16 rows of the weights and up to 16 rows of a; a
 // workgroup's eight waves are wk parts of k (slabs kpart, kpart + wk, ...) times 8 / wk groups of weight rows, and the parts meet in LDS.  All of
 // a turn's loads are in flight together.  16x16x128 instructions: lane group g (lane / 16) takes the blocks 2 g and 2 g + 1 of a slab, 32 neighbouring
 // bytes and two neighbouring scales.
@@ -474,55 +491,45 @@ template <class T> __device__ __forceinline__ void quantize_to_lds(const MxParam
   }
 }
 
-template <int NT, int MT, bool EXPERTS, bool RAW>
+template <bool EXPERTS, bool RAW>
 __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t mx_smem[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(uint8_t __attribute__((address_space(3)))*)mx_smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = 1 << p.wk_log, kpart = wave & (wk - 1);
-  const int n0 = (blockIdx.x * (FEW_WAVES >> p.wk_log) + (wave >> p.wk_log)) * (16 * NT);
+  const int n0 = (blockIdx.x * (FEW_WAVES >> p.wk_log) + (wave >> p.wk_log)) * 16;
   RowTile rt;
   if (EXPERTS) {
-    if (!find_rows<16 * MT>(p, blockIdx.y, lane, &rt)) return;            // (the same answer in every wave)
+    if (!find_rows<16>(p, blockIdx.y, lane, &rt)) return;                 // (the same answer in every wave)
   } else {
     rt.expert = 0;
-    rt.row0 = blockIdx.y * (16 * MT);
-    rt.rows = p.m - rt.row0 < 16 * MT ? p.m - rt.row0 : 16 * MT;
+    rt.row0 = blockIdx.y * 16;
+    rt.rows = p.m - rt.row0 < 16 ? p.m - rt.row0 : 16;
   }
   const int row = lane & 15, g = lane >> 4;
   const bool empty = EXPERTS && rt.expert == p.experts;
   const uint32_t raw_scales = lds0 + FEW_RAW_ROWS * p.slabs * MX_ROWB;
-  f32x4 acc[NT][MT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 
-  constexpr int DEPTH = NT == 1 ? 8 : 4;                 // slabs of a turn
-  const uint8_t *b_at[NT], *bs_at[NT];
-  i32x4 fb[DEPTH][NT][2];
-  int sb[DEPTH][NT];
+  constexpr int DEPTH = 8;                               // slabs of a turn
+  const uint8_t *b_at = nullptr, *bs_at = nullptr;
+  i32x4 fb[DEPTH][2];
+  int sb[DEPTH];
   auto load_weights = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       const int64_t s = s0 + d * wk;
       if (s < p.slabs) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          fb[d][i][0] = *(const i32x4*)(b_at[i] + s * MX_ROWB);
-          fb[d][i][1] = *(const i32x4*)(b_at[i] + s * MX_ROWB + 16);
-          sb[d][i] = *(const uint16_t*)(bs_at[i] + (s >> 1) * 512 + (s & 1) * 8);
-        }
+        fb[d][0] = *(const i32x4*)(b_at + s * MX_ROWB);
+        fb[d][1] = *(const i32x4*)(b_at + s * MX_ROWB + 16);
+        sb[d] = *(const uint16_t*)(bs_at + (s >> 1) * 512 + (s & 1) * 8);
       }
     }
   };
   if (!empty) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int n = n0 + 16 * i + row < p.n ? n0 + 16 * i + row : p.n - 1;
-      b_at[i] = p.b + (int64_t)rt.expert * p.b_expert + (int64_t)n * p.slabs * MX_ROWB + 32 * g;
-      bs_at[i] = p.bs + (int64_t)rt.expert * p.bs_expert + mx_scale_at(n, 0, p.slabs) + 2 * g;
-    }
+    const int n = n0 + row < p.n ? n0 + row : p.n - 1;
+    b_at = p.b + (int64_t)rt.expert * p.b_expert + (int64_t)n * p.slabs * MX_ROWB + 32 * g;
+    bs_at = p.bs + (int64_t)rt.expert * p.bs_expert + mx_scale_at(n, 0, p.slabs) + 2 * g;
     load_weights(kpart);
   }
   if (RAW) {
@@ -532,46 +539,31 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
     __syncthreads();
   }
   if (!empty) {
-    const uint8_t *a_at[MT], *as_at[MT];
-    bool a_have[MT];
-    int src[MT];
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      a_have[j] = 16 * j + row < rt.rows;
-      const int r = rt.row0 + (a_have[j] ? 16 * j + row : 0);
-      src[j] = EXPERTS ? source_row(p, r) : r;
-      if (!RAW) {
-        a_at[j] = p.a + (int64_t)src[j] * p.slabs * MX_ROWB + 32 * g;
-        as_at[j] = p.as + mx_scale_at(src[j], 0, p.slabs) + 2 * g;
-      }
-    }
+    const bool have = row < rt.rows;
+    const int r = rt.row0 + (have ? row : 0), src = EXPERTS ? source_row(p, r) : r;
+    const uint8_t* a_at = RAW ? nullptr : p.a + (int64_t)src * p.slabs * MX_ROWB + 32 * g;
+    const uint8_t* as_at = RAW ? nullptr : p.as + mx_scale_at(src, 0, p.slabs) + 2 * g;
     for (int s0 = kpart;;) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
         const int64_t s = s0 + d * wk;
         if (s < p.slabs) {
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            i32x4 fa0 = {0, 0, 0, 0}, fa1 = {0, 0, 0, 0};
-            int sa = 0x7f7f;
-            if (a_have[j]) {
-              if (RAW) {
-                const uint32_t at = (uint32_t)(src[j] * p.slabs + s);
-                fa0 = *TNX_LDS(i32x4, lds0 + at * MX_ROWB + 32 * g);
-                fa1 = *TNX_LDS(i32x4, lds0 + at * MX_ROWB + 32 * g + 16);
-                sa = *TNX_LDS(uint16_t, raw_scales + at * MX_SCALEB + 2 * g);
-              } else {
-                fa0 = *(const i32x4*)(a_at[j] + s * MX_ROWB);
-                fa1 = *(const i32x4*)(a_at[j] + s * MX_ROWB + 16);
-                sa = *(const uint16_t*)(as_at[j] + (s >> 1) * 512 + (s & 1) * 8);
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              acc[i][j] = mfma16<0>(fb[d][i][0], fa0, acc[i][j], sb[d][i], sa);
-              acc[i][j] = mfma16<1>(fb[d][i][1], fa1, acc[i][j], sb[d][i], sa);
+          i32x4 fa0 = {0, 0, 0, 0}, fa1 = {0, 0, 0, 0};
+          int sa = 0x7f7f;
+          if (have) {
+            if (RAW) {
+              const uint32_t at = (uint32_t)(src * p.slabs + s);
+              fa0 = *TNX_LDS(i32x4, lds0 + at * MX_ROWB + 32 * g);
+              fa1 = *TNX_LDS(i32x4, lds0 + at * MX_ROWB + 32 * g + 16);
+              sa = *TNX_LDS(uint16_t, raw_scales + at * MX_SCALEB + 2 * g);
+            } else {
+              fa0 = *(const i32x4*)(a_at + s * MX_ROWB);
+              fa1 = *(const i32x4*)(a_at + s * MX_ROWB + 16);
+              sa = *(const uint16_t*)(as_at + (s >> 1) * 512 + (s & 1) * 8);
             }
           }
+          acc = mfma16<0>(fb[d][0], fa0, acc, sb[d], sa);
+          acc = mfma16<1>(fb[d][1], fa1, acc, sb[d], sa);
         }
       }
       s0 += wk * DEPTH;
@@ -580,29 +572,15 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
     }
   }
   if (wk > 1) {
-    // part k of a group of weight rows beside the others': [wave][product][lane]
+    // a part's sums beside the others', and the first part adds them up in order
     if (RAW) __syncthreads();                            // (the rows of a lie there)
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < MT; ++j) *TNX_LDS(f32x4, lds0 + ((wave * NT * MT + i * MT + j) * 64 + lane) * 16) = acc[i][j];
+    *TNX_LDS(f32x4, lds0 + (wave * 64 + lane) * 16) = acc;
     __syncthreads();
+    if (kpart > 0) return;
+    for (int w = 1; w < wk; ++w) acc += *TNX_LDS(f32x4, lds0 + ((wave + w) * 64 + lane) * 16);
   }
-  // with parts, product ij of the group is summed and stored by part ij % wk (in the order of the parts)
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      if (((i * MT + j) & (wk - 1)) != kpart) continue;
-      f32x4 v = acc[i][j];
-      if (wk > 1) {
-        const int w0 = wave - kpart;
-        v = *TNX_LDS(f32x4, lds0 + ((w0 * NT * MT + i * MT + j) * 64 + lane) * 16);
-        for (int w = 1; w < wk; ++w) v += *TNX_LDS(f32x4, lds0 + (((w0 + w) * NT * MT + i * MT + j) * 64 + lane) * 16);
-      }
-      const int r = 16 * j + row, c = n0 + 16 * i + 4 * g;
-      if (r < rt.rows && c < p.n) store_columns(p, rt.row0 + r, c, p.n, v);
-    }
+  const int c = n0 + 4 * g;
+  if (row < rt.rows && c < p.n) store_columns(p, rt.row0 + row, c, p.n, acc);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -621,33 +599,52 @@ template <class C, bool EXPERTS> int launch_tile(MxParams p, int64_t row_tiles, 
   return p.out_dtype == DT_F16 ? gated(TypeTag<OutF16>()) : gated(TypeTag<OutF32>());
 }
 
-template <int NT, int MT, bool EXPERTS, bool RAW> int launch_few(MxParams p, int64_t row_tiles, hipStream_t stream) {
+template <bool EXPERTS, bool RAW> int launch_few(MxParams p, int64_t row_tiles, hipStream_t stream) {
   // as few parts of k as give every SIMD two waves: a part less is a sum less, and its wave has more loads in flight
-  const int64_t groups = (p.n + 16 * NT - 1) / (16 * NT);
+  const int64_t groups = (p.n + 15) / 16;
   p.wk_log = 0;
   while (p.wk_log < 3 && (2 << p.wk_log) <= p.slabs && (groups * row_tiles << p.wk_log) < 2048) ++p.wk_log;
   const int64_t per = FEW_WAVES >> p.wk_log;
-  size_t lds = p.wk_log ? (size_t)FEW_WAVES * NT * MT * 1024 : 0;
+  size_t lds = p.wk_log ? (size_t)FEW_WAVES * 1024 : 0;
   const size_t raw = RAW ? (size_t)FEW_RAW_ROWS * p.slabs * (MX_ROWB + MX_SCALEB) : 0;
   if (raw > lds) lds = raw;
-  hipLaunchKernelGGL((mx_few_kernel<NT, MT, EXPERTS, RAW>), dim3((unsigned)((groups + per - 1) / per), (unsigned)row_tiles), dim3(FEW_WAVES * 64), lds, stream, p);
+  hipLaunchKernelGGL((mx_few_kernel<EXPERTS, RAW>), dim3((unsigned)((groups + per - 1) / per), (unsigned)row_tiles), dim3(FEW_WAVES * 64), lds, stream, p);
   return mx_launched();
 }
 
+// Microseconds of `tiles` tiles, `slots` of them on the card at a time: a slab costs t, less (t_few) where at most half of the slots are taken, a
+// tile o beside its slabs.
+double tiles_us(int64_t tiles, int slots, double t, double t_few, double o, int64_t slabs) {
+  const int64_t rounds = tiles / slots, rest = tiles % slots;
+  return rounds * (slabs * t + o) + (rest ? slabs * (2 * rest <= slots ? t_few : t) + o : 0.0);
+}
+
+// The tile with the lowest estimate.  Fitted to products of 8 to 4096 rows with 256 x 1024 to 14336 x 14336 weights, and of 4 to 4096 tokens with 8 to
+// 128 experts.  What it decides, measured in us: 1024 x 4096 x 4096 tiles of 64 18.5, of 128 15.6 (one on a CU, four buffers) and 16.0 (two on a
+// CU, two buffers), of 256 25.6; 2048 x 14336 x 4096 117, 88, 73 and 66; 512 x 4096 x 14336 27, 30, 46 and 69; 64 tokens through
+// the up-projections of 64 experts (4096 -> 1024) 49, 56, 49 and 56, through the down-projections 44, 55, 37 and 44.
 template <bool EXPERTS> int launch(const MxParams& p, bool raw, hipStream_t stream) {
-  // rows that a workgroup can expect, and how many tiles of BM there are at most
-  const int64_t each = EXPERTS ? (p.m + p.experts - 1) / p.experts : p.m;
-  auto tiles = [&](int bm) { return EXPERTS ? (int64_t)p.m / bm + 1 + (p.experts < p.m ? p.experts : p.m) : ((int64_t)p.m + bm - 1) / bm; };
-  if (raw) return tiles(16) <= 65535 ? launch_few<1, 1, EXPERTS, true>(p, tiles(16), stream) : TNX_E_UNSUPPORTED;
-  // (experts' rows are uneven: an expert with more than a tile's reads its weights again, from the L2 mostly)
-  if (each <= (EXPERTS ? 4 : 16) && tiles(16) <= 65535) return launch_few<1, 1, EXPERTS, false>(p, tiles(16), stream);
-  if (each <= (EXPERTS ? 16 : 32) && tiles(32) <= 65535) return launch_few<1, 2, EXPERTS, false>(p, tiles(32), stream);
-  if (each <= (EXPERTS ? 40 : 64) && tiles(64) <= 65535) return launch_few<2, 4, EXPERTS, false>(p, tiles(64), stream);
-  const int64_t big = tiles(256) * ((p.n + 255) / 256);
-  if (big >= 200) return launch_tile<MxTile<256, 256, 4, 2>, EXPERTS>(p, tiles(256), stream);
-  const int64_t mid = tiles(128) * ((p.n + 127) / 128);
-  if (mid >= 256) return launch_tile<MxTile<128, 128, 2, 2>, EXPERTS>(p, tiles(128), stream);
-  return launch_tile<MxTile<64, 64, 2, 2>, EXPERTS>(p, tiles(64), stream);
+  // tiles of BM rows: how many there are at most, and how many to expect (an expert's last is half full)
+  auto most = [&](int bm) { return EXPERTS ? (int64_t)p.m / bm + 1 + (p.experts < p.m ? p.experts : p.m) : ((int64_t)p.m + bm - 1) / bm; };
+  auto expect = [&](int bm) {
+    if (!EXPERTS) return most(bm);
+    const int64_t some = p.experts < p.m ? p.experts : p.m, n = (int64_t)p.m / bm + some / 2;
+    return n > some ? n : some;
+  };
+  auto cols = [&](int bn) { return ((int64_t)p.n + bn - 1) / bn; };
+  if (raw) return most(16) <= 65535 ? launch_few<EXPERTS, true>(p, most(16), stream) : TNX_E_UNSUPPORTED;
+  const double us64 = tiles_us(expect(64) * cols(64), 512, 0.5, 0.35, EXPERTS ? 3.8 : 1.5, p.slabs);
+  const double us128 = tiles_us(expect(128) * cols(128), 512, 1.1, 0.76, 4.5, p.slabs);
+  const double us128_deep = tiles_us(expect(128) * cols(128), 256, 0.5, 0.45, 6.0, p.slabs);
+  const double us256 = tiles_us(expect(256) * cols(256), 256, 1.77, 1.15, 9.0, p.slabs);
+  // Up to 16 rows: the streaming kernel brings 3.3 MB a us and has a short way to the first load.  4 x 4096 x 8192: 9.6 us, tiles of 64 13.0; 4 x
+  // 14336 x 14336: 29 and 24.5.
+  const double us_few = 5.0 + (double)p.n * p.slabs * (MX_ROWB + MX_SCALEB) / 3.3e6;
+  if (!EXPERTS && p.m <= 16 && us_few < us64) return launch_few<EXPERTS, false>(p, most(16), stream);
+  if (us256 <= us128 && us256 <= us128_deep && us256 <= us64) return launch_tile<MxTile<256, 256, 4, 2, 2>, EXPERTS>(p, most(256), stream);
+  if (us64 <= us128 && us64 <= us128_deep) return launch_tile<MxTile<64, 64, 2, 2, 4>, EXPERTS>(p, most(64), stream);
+  if (us128_deep < us128) return launch_tile<MxTile<128, 128, 2, 2, 4>, EXPERTS>(p, most(128), stream);
+  return launch_tile<MxTile<128, 128, 2, 2, 2>, EXPERTS>(p, most(128), stream);
 }
 
 bool takes_rows(int64_t a_rows, int64_t k) { return a_rows <= FEW_RAW_ROWS && FEW_RAW_ROWS * mx_slabs(k) * (MX_ROWB + MX_SCALEB) <= FEW_RAW_LDS; }
