@@ -28,6 +28,7 @@ struct MxParams {
   int out_dtype, epi;
   int64_t lda;                             // few rows as floats: their stride, type and k; parts of k (log2)
   int a_dtype, k, wk_log;
+  bool stream_b;                           // the weights are read by one tile of rows each: past the caches (tiles of up to 128 rows)
 };
 
 __device__ __forceinline__ f32x16 mfma32(i32x4 a, i32x4 b, f32x16 c, int sa, int sb, int step) {
@@ -290,13 +291,16 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
   constexpr int OPS = C::B_OPS + C::A_OPS + 1;
   auto fetch_op = [&](int slab, int q) __attribute__((always_inline)) {
     const uint32_t slot = lds0 + (slab & (S - 1)) * C::SLOT;
-    if (q < C::B_OPS) dma16_from(b + (int64_t)slab * MX_ROWB, b_off[q], slot + (NW * q + wave) * 1024);
-    else if (q < C::B_OPS + C::A_OPS) {
+    if (q < C::B_OPS) {
+      if (BM <= 128 && p.stream_b) dma16_nt(b + (int64_t)slab * MX_ROWB, b_off[q], __builtin_amdgcn_readfirstlane(slot + (NW * q + wave) * 1024));
+      else dma16_from(b + (int64_t)slab * MX_ROWB, b_off[q], slot + (NW * q + wave) * 1024);
+    }
+    if (q >= C::B_OPS && q < C::B_OPS + C::A_OPS) {
       const int i = q - C::B_OPS;
       const uint32_t to = slot + C::B_BYTES + (NW * i + wave) * 1024;
       if (EXPERTS) dma16_at(a_at[i] + (int64_t)slab * MX_ROWB, to);
       else dma16_from(a + (int64_t)slab * MX_ROWB, a_off[i], to);
-    } else if ((slab & 1) == 0 && wave < S_WAVES) {
+    } else if (q == C::B_OPS + C::A_OPS && (slab & 1) == 0 && wave < S_WAVES) {
       dma16_at(s_at + (int64_t)(slab >> 1) * 512, lds0 + S * C::SLOT + (slab >> 1 & (S - 1)) * C::S_BYTES + wave * 1024);
     }
   };
@@ -587,6 +591,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
 template <class C, bool EXPERTS> int launch_tile(MxParams p, int64_t row_tiles, hipStream_t stream) {
   p.tiles_n = (p.n + C::BN - 1) / C::BN;
   p.tiles_m = (p.m + C::BM - 1) / C::BM;
+  // 64 tokens through 64 experts' up-projections, weights not in the caches: 62 us, so 55; with 1024 tokens, two tiles an expert, 99 and 104
+  p.stream_b = EXPERTS ? (int64_t)p.m * 2 <= (int64_t)p.experts * C::BM : p.tiles_m == 1;
   const int64_t grid = row_tiles * p.tiles_n;
   if (grid > 0x7fffffff) return TNX_E_UNSUPPORTED;
   auto go = [&](auto out_tag, auto glu_tag) {
@@ -683,6 +689,6 @@ extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
   p.experts = a->experts; p.tiles_n = p.tiles_m = 0;
   p.top_k = make_fastdiv((uint32_t)(a->order ? a->top_k : 1));
   p.out_dtype = a->out_dtype; p.epi = a->epilogue;
-  p.a_dtype = a->a_dtype; p.lda = a->stride_a; p.k = (int)a->k; p.wk_log = 0;
+  p.a_dtype = a->a_dtype; p.lda = a->stride_a; p.k = (int)a->k; p.wk_log = 0; p.stream_b = false;
   return a->experts > 0 ? launch<true>(p, raw, (hipStream_t)a->stream) : launch<false>(p, raw, (hipStream_t)a->stream);
 }
