@@ -373,7 +373,8 @@ int tnx_mx_gemm_takes_rows(int64_t a_rows, int64_t k);
  * sums, rounded once.  With a GLU epilogue n is the interleaved width (even rows of b are the gate) and out has n / 2 columns.
  *
  * experts > 0: b holds `experts` matrices one after another, and row r of the product (0 <= r < m) belongs to the expert e with
- * offsets[e] <= r < offsets[e + 1] (device memory, offsets[0] = 0, not decreasing, offsets[experts] <= m).  Row r of the product takes
+ * offsets[e] <= r < offsets[e + 1] (device memory, offsets[0] = 0, not decreasing, offsets[experts] <= m; anything else is taken
+ * into that range).  Row r of the product takes
  * row r of a or, with `order` given (device memory, one entry per row), row order[r] / top_k of the a_rows rows of a; entries outside are taken
  * as the nearest row inside.  Rows from offsets[experts] on are written as zeros. */
 typedef struct tnx_mx_gemm_args {

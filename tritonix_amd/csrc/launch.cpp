@@ -364,17 +364,20 @@ struct OpEntries {
   int (*backward)(const tnx_moe_args*);
   int (*combine)(const void*, const int32_t*, const float*, void*, int64_t, int32_t, int64_t, int32_t, int32_t, void*);
 } ops = {};
+int64_t join_bytes = 0;
 
-// bind_ops(addresses of the above, in their order)
+// bind_ops(addresses of the above, in their order, and the most bytes of a join's rows in 32 bits)
 PyObject* bind_ops(PyObject*, PyObject* arg) {
   constexpr int N = sizeof(OpEntries) / sizeof(void*);
-  if (!PyTuple_Check(arg) || PyTuple_GET_SIZE(arg) != N) {
+  if (!PyTuple_Check(arg) || PyTuple_GET_SIZE(arg) != N + 1) {
     PyErr_SetString(PyExc_ValueError, "bind_ops: not the entry points");
     return nullptr;
   }
   void* at[N];
   for (int i = 0; i < N; ++i) at[i] = (void*)(uintptr_t)PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(arg, i));
+  const long long most = PyLong_AsLongLong(PyTuple_GET_ITEM(arg, N));
   if (PyErr_Occurred()) return nullptr;
+  join_bytes = most;
   static_assert(sizeof ops == sizeof at, "one pointer each");
   std::memcpy(&ops, at, sizeof ops);
   Py_RETURN_NONE;
@@ -537,17 +540,91 @@ PyObject* mx_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
         g.a_codes = q.buffer.data_ptr();
         g.a_scales = (const uint8_t*)g.a_codes + q.code_bytes;
       }
-      out = fresh({g.m, g.stride_out}, a->scalar_type(), device);
+      // (the rows of a join: in 32 bits up to the size that moe.py has)
+      if (rows && g.m * g.n * 4 <= join_bytes) g.out_dtype = TNX_F32;
+      out = fresh({g.m, g.stride_out}, type_of(g.out_dtype), device);
       g.out = out.data_ptr();
       status = q.status != TNX_OK ? q.status : ops.gemm(&g);
       if (status == TNX_OK && rows) {
         joined = fresh({rows->size(0), g.n}, a->scalar_type(), device);
         status = ops.combine(out.data_ptr(), (const int32_t*)rows->data_ptr(), (const float*)weights->data_ptr(), joined.data_ptr(), rows->size(0),
-                             (int32_t)rows->size(1), g.n, code, code, g.stream);
+                             (int32_t)rows->size(1), g.n, g.out_dtype, code, g.stream);
       }
     }
     if (status != TNX_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(rows ? joined : out);
+  } catch (...) {
+    return none();
+  }
+}
+
+// out[m, n] = a[m, k] b[k, n] of float tensors, both quantised along k
+struct Multiplied {
+  at::Tensor out;
+  int status;
+};
+Multiplied multiplied(const Quantised& a, const Quantised& b, int64_t m, int64_t n, int64_t k, at::ScalarType type, c10::DeviceIndex device, void* stream) {
+  Multiplied r{fresh({m, n}, type, device), a.status != TNX_OK ? a.status : b.status};
+  if (r.status != TNX_OK) return r;
+  tnx_mx_gemm_args g = {};
+  g.a_codes = a.buffer.data_ptr(); g.a_scales = (const uint8_t*)g.a_codes + a.code_bytes;
+  g.b_codes = b.buffer.data_ptr(); g.b_scales = (const uint8_t*)g.b_codes + b.code_bytes;
+  g.out = r.out.data_ptr();
+  g.m = g.a_rows = m; g.n = n; g.k = k; g.stride_out = n;
+  g.out_dtype = float_code(type);
+  g.stream = stream;
+  r.status = ops.gemm(&g);
+  return r;
+}
+
+// mx_linear(x, w) -> x w; mx_linear_backward(dy, x, w, wants dx, wants dw) -> (dx or None, dw or None); or None
+bool linear_operands(PyObject* x, PyObject* w, const at::Tensor** tx, const at::Tensor** tw, c10::DeviceIndex* device) {
+  return here(x, 2, tx, device) && here(w, 2, tw, device) && (*tx)->size(1) == (*tw)->size(0) && (*tx)->scalar_type() == (*tw)->scalar_type() &&
+         float_code((*tx)->scalar_type()) >= 0 && (*tx)->numel() > 0 && (*tw)->numel() > 0;
+}
+
+PyObject* mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2) Py_RETURN_NONE;
+  try {
+    const at::Tensor *x, *w;
+    c10::DeviceIndex device = -1;
+    if (!linear_operands(args[0], args[1], &x, &w, &device)) Py_RETURN_NONE;
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    Multiplied y;
+    {
+      const Unlocked unlocked;
+      y = multiplied(quantised(*x, true, device, stream), quantised(*w, false, device, stream), x->size(0), w->size(1), x->size(1), x->scalar_type(), device, stream);
+    }
+    if (y.status != TNX_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(y.out);
+  } catch (...) {
+    return none();
+  }
+}
+
+PyObject* mx_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) Py_RETURN_NONE;
+  try {
+    const at::Tensor *x, *w, *dy;
+    c10::DeviceIndex device = -1;
+    if (!linear_operands(args[1], args[2], &x, &w, &device) || !here(args[0], 2, &dy, &device) || dy->size(0) != x->size(0) || dy->size(1) != w->size(1) ||
+        dy->scalar_type() != x->scalar_type())
+      Py_RETURN_NONE;
+    const bool wants_dx = args[3] == Py_True, wants_dw = args[4] == Py_True;
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    const int64_t m = x->size(0), k = x->size(1), cols = w->size(1);
+    Multiplied dx{{}, TNX_OK}, dw{{}, TNX_OK};
+    {
+      const Unlocked unlocked;
+      // dx = dy w^T along the columns of w, dw = x^T dy along the rows of x
+      if (wants_dx) dx = multiplied(quantised(*dy, true, device, stream), quantised(*w, true, device, stream), m, k, cols, x->scalar_type(), device, stream);
+      if (wants_dw) dw = multiplied(quantised(*x, false, device, stream), quantised(*dy, false, device, stream), k, cols, m, x->scalar_type(), device, stream);
+    }
+    if (dx.status != TNX_OK || dw.status != TNX_OK) Py_RETURN_NONE;
+    const Object ox = taken(wants_dx ? THPVariable_Wrap(dx.out) : (Py_INCREF(Py_None), Py_None));
+    const Object ow = taken(wants_dw ? THPVariable_Wrap(dw.out) : (Py_INCREF(Py_None), Py_None));
+    if (!ox.p || !ow.p) return nullptr;
+    return PyTuple_Pack(2, ox.p, ow.p);
   } catch (...) {
     return none();
   }
@@ -664,6 +741,8 @@ PyMethodDef methods[] = {
     {"mx_quantize", (PyCFunction)(void (*)(void))mx_quantize, METH_FASTCALL, nullptr},
     {"mx_dequantize", (PyCFunction)(void (*)(void))mx_dequantize, METH_FASTCALL, nullptr},
     {"mx_product", (PyCFunction)(void (*)(void))mx_product, METH_FASTCALL, nullptr},
+    {"mx_linear", (PyCFunction)(void (*)(void))mx_linear, METH_FASTCALL, nullptr},
+    {"mx_linear_backward", (PyCFunction)(void (*)(void))mx_linear_backward, METH_FASTCALL, nullptr},
     {"moe_route", (PyCFunction)(void (*)(void))moe_route, METH_FASTCALL, nullptr},
     {"moe_backward", (PyCFunction)(void (*)(void))moe_backward, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -634,7 +634,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const uint8_t* y, const in
   const bool whole = c + 8 <= n;
   for (int j = 0; j < k; ++j) {
     const int r = rows[t * k + j];
-    if (r < 0) continue;
+    if (r < 0 || r >= tokens * k) continue;
     const float w = weights[t * k + j];
     const int64_t at = (int64_t)r * n + c;
     if (whole) {
@@ -675,7 +675,7 @@ int route_lanes(int64_t tokens, int e) {
   if (e > 512 || tokens <= 1024) return 64;
   return e <= 128 ? 8 : e <= 256 ? 16 : 32;
 }
-constexpr int SUM_BLOCKS = 128;            // more blocks than this are summed by a launch of their own
+constexpr int SUM_BLOCKS = 256;            // more blocks than this are summed by a launch of their own
 
 // The plan's blocks are the pairs of a routing workgroup's 256 / lanes tokens; many tokens at four a workgroup are counted apart, in larger blocks.
 void plan_shape(PlanParams* q, int64_t tokens, int k, int e) {

@@ -60,13 +60,20 @@ __device__ __forceinline__ void dma4_at(const uint8_t* src, uint32_t lds_base) {
 // own.  All 64 lanes take part; the answer is uniform.  expert == experts: rows past the last expert's; false: no such tile.
 struct RowTile { int expert, row0, rows; };
 
+// (Offsets are taken inside [0, m] and as not decreasing, whatever they hold: no row outside of the product is touched.)
+__device__ __forceinline__ int rows_upto(const MxParams& p, int e) {
+  const int v = e > p.experts ? p.m : p.offsets[e];
+  return v < 0 ? 0 : v < p.m ? v : p.m;
+}
+
+template <int BM> __device__ __forceinline__ int tiles_between(int lo, int hi) { return hi > lo ? (hi - lo + BM - 1) / BM : 0; }
+
 template <int BM> __device__ __forceinline__ int expert_tiles(const MxParams& p, int lane) {
   int total = 0;
   for (int e0 = 0; e0 <= p.experts; e0 += 64) {
     const int e = e0 + lane;
     int t = 0;
-    if (e < p.experts) t = (p.offsets[e + 1] - p.offsets[e] + BM - 1) / BM;
-    else if (e == p.experts) t = (p.m - p.offsets[e] + BM - 1) / BM;
+    if (e <= p.experts) t = tiles_between<BM>(rows_upto(p, e), rows_upto(p, e + 1));
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) t += __shfl_xor(t, d);
     total += t;
@@ -79,8 +86,8 @@ template <int BM> __device__ __forceinline__ bool find_rows(const MxParams& p, i
   for (int e0 = 0; e0 <= p.experts; e0 += 64) {
     const int e = e0 + lane;
     int lo = 0, hi = 0;
-    if (e <= p.experts) { lo = p.offsets[e]; hi = e < p.experts ? p.offsets[e + 1] : p.m; }
-    const int t = (hi - lo + BM - 1) / BM;
+    if (e <= p.experts) { lo = rows_upto(p, e); hi = rows_upto(p, e + 1); }
+    const int t = tiles_between<BM>(lo, hi);
     int upto = t;                                        // tiles of the lanes up to this one
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {

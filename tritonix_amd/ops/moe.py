@@ -252,8 +252,8 @@ def moe_glu(x, w12: MXTensor, routing: Routing, activation: str = "silu", out_dt
 def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
     """Down-projections of the rows that ``moe_glu`` made, joined: ``out[t] = sum_j weights[t, j] * (h[rows[t, j]] @ w3[e])``, ``[t, d]``.
 
-    The products are rounded to the result's type before the join (they are k times the result's size, and the join is bound by
-    reading them); the join sums in 32 bits."""
+    The join sums in 32 bits.  The products it sums are in 32 bits too where they take at most 32 MiB; larger ones are rounded to the result's
+    type first (they are k times the result's size, and writing and reading them is what the join costs)."""
     if out_dtype is None and type(w3) is MXTensor and w3.batch == routing.num_experts and w3.dim == -2:
         out = (_mx.native or _mx.find_native()).mx_product(h, w3.buffer, w3.code_bytes, w3.rows, w3.k, _C.EPI_NONE, routing.num_experts, routing.top_k,
                                                            routing.offsets, None, routing.rows, routing.weights)
@@ -266,12 +266,13 @@ def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
     index = on_device("moe_down", h, w3, routing.order)
     hq = h if takes_rows(h) else operand("moe_down", "h", h, -1)
     n = w3.rows
-    y = torch.empty((routing.tokens * routing.top_k, n), dtype=out_dtype, device=w3.device)
+    rows = routing.tokens * routing.top_k
+    y = torch.empty((rows, n), dtype=torch.float32 if rows * n * 4 <= _mx.JOIN_BYTES else out_dtype, device=w3.device)
     _grouped("moe_down", hq, w3, routing, y, False, _C.EPI_NONE, index)
     out = torch.empty((routing.tokens, n), dtype=out_dtype, device=w3.device)
     with torch.cuda.device(index):
         status = _C.load().tnx_moe_combine(y.data_ptr(), routing.rows.data_ptr(), routing.weights.data_ptr(), out.data_ptr(), routing.tokens,
-                                           routing.top_k, n, code, code, _stream_of(index))
+                                           routing.top_k, n, dtype_code("moe_down", y.dtype), code, _stream_of(index))
     raise_for_status(status, "moe_down")
     return out
 

@@ -24,6 +24,9 @@ __all__ = ["MXTensor", "mx_quantize", "mx_dequantize", "mx_matmul", "mx_glu", "m
 
 BLOCK = 32
 SLAB = 256                      # k is padded to whole slabs (csrc/mx.h)
+# Rows that moe_down joins are kept in 32 bits up to this many bytes, which the L2 caches hold together; larger ones, whose writing and reading is
+# what the join costs, are rounded to the result's type first (8192 tokens of 8 experts, 4096 wide: 1 GB each way in 32 bits).
+JOIN_BYTES = 32 << 20
 _DTYPES = {torch.float16: _C.F16, torch.bfloat16: _C.BF16, torch.float32: _C.F32}
 _EPILOGUES = {"silu": _C.EPI_GLU_SILU, "sigmoid": _C.EPI_GLU_SIGMOID}
 
@@ -35,7 +38,7 @@ class _Interpreter:
     def _none(*_):
         return None
 
-    mx_quantize = mx_dequantize = mx_product = moe_route = moe_backward = _none
+    mx_quantize = mx_dequantize = mx_product = mx_linear = mx_linear_backward = moe_route = moe_backward = _none
 
 
 # csrc/launch.cpp, which makes the ordinary calls without the interpreter's share of them; found with the first call
@@ -51,7 +54,7 @@ def find_native():
         lib = _C.load()
         module.bind_ops(tuple(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
             lib.tnx_mx_code_bytes, lib.tnx_mx_scale_bytes, lib.tnx_mx_quantize, lib.tnx_mx_dequantize, lib.tnx_mx_gemm_takes_rows, lib.tnx_mx_gemm,
-            lib.tnx_moe_workspace_bytes, lib.tnx_moe_route, lib.tnx_moe_route_backward, lib.tnx_moe_combine)))
+            lib.tnx_moe_workspace_bytes, lib.tnx_moe_route, lib.tnx_moe_route_backward, lib.tnx_moe_combine)) + (JOIN_BYTES,))
         native = module
     return native
 
@@ -314,11 +317,15 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w):
         ctx.save_for_backward(x, w)
-        return mx_matmul(x, w)
+        y = (native or find_native()).mx_linear(x, w)
+        return mx_matmul(x, w) if y is None else y
 
     @staticmethod
     def backward(ctx, dy):
         x, w = ctx.saved_tensors
+        both = (native or find_native()).mx_linear_backward(dy, x, w, *ctx.needs_input_grad)
+        if both is not None:
+            return both
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = mx_matmul(dy, w.t(), out_dtype=x.dtype)
