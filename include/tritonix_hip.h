@@ -360,6 +360,9 @@ size_t tnx_mx_scale_bytes(int64_t rows, int64_t k);
 /* scale = 2^(floor(log2 of the block's largest magnitude) - 2), elements rounded to the nearest code, ties to the even code,
  * above 6 to 6 */
 int tnx_mx_quantize(const tnx_mx_args* args);
+/* one matrix (batch == 1) along both dimensions, read once: along k into args' buffers, and its transpose, k rows quantised along `rows`, into
+ * codes_t and scales_t */
+int tnx_mx_quantize_both(const tnx_mx_args* args, void* codes_t, void* scales_t);
 int tnx_mx_dequantize(const tnx_mx_args* args);
 
 /* from the row-major form of files: ceil(k / 2) bytes of codes and ceil(k / 32) scale bytes per row */

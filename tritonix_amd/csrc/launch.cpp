@@ -17,6 +17,7 @@
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/headeronly/version.h>
 
@@ -356,6 +357,7 @@ struct OpEntries {
   size_t (*code_bytes)(int64_t, int64_t);
   size_t (*scale_bytes)(int64_t, int64_t);
   int (*quantize)(const tnx_mx_args*);
+  int (*quantize_both)(const tnx_mx_args*, void*, void*);
   int (*dequantize)(const tnx_mx_args*);
   int (*takes_rows)(int64_t, int64_t);
   int (*gemm)(const tnx_mx_gemm_args*);
@@ -416,21 +418,41 @@ struct Quantised {
   int64_t code_bytes = 0;
   int status = TNX_OK;
 };
-Quantised quantised(const at::Tensor& x, bool along_last, c10::DeviceIndex device, void* stream) {
-  const int64_t rows = x.size(along_last ? 0 : 1), k = x.size(along_last ? 1 : 0);
+Quantised room(int64_t rows, int64_t k, c10::DeviceIndex device) {
   Quantised q;
   q.code_bytes = (int64_t)ops.code_bytes(rows, k);
   q.buffer = fresh({q.code_bytes + (int64_t)ops.scale_bytes(rows, k)}, at::kByte, device);
+  return q;
+}
+tnx_mx_args quantising(const at::Tensor& x, bool along_last, const Quantised& q, void* stream) {
   tnx_mx_args a = {};
   a.data = x.data_ptr();
   a.codes = q.buffer.data_ptr();
   a.scales = (uint8_t*)a.codes + q.code_bytes;
-  a.batch = 1; a.rows = rows; a.k = k;
+  a.batch = 1;
+  a.rows = x.size(along_last ? 0 : 1); a.k = x.size(along_last ? 1 : 0);
   a.stride_row = x.stride(along_last ? 0 : 1); a.stride_k = x.stride(along_last ? 1 : 0);
   a.dtype = float_code(x.scalar_type());
   a.stream = stream;
+  return a;
+}
+Quantised quantised(const at::Tensor& x, bool along_last, c10::DeviceIndex device, void* stream) {
+  Quantised q = room(x.size(along_last ? 0 : 1), x.size(along_last ? 1 : 0), device);
+  const tnx_mx_args a = quantising(x, along_last, q, stream);
   q.status = ops.quantize(&a);
   return q;
+}
+// along its last dimension, and along its first
+struct QuantisedBoth {
+  Quantised last, first;
+};
+QuantisedBoth quantised(const at::Tensor& x, bool last, bool first, c10::DeviceIndex device, void* stream) {
+  if (!last || !first) return {last ? quantised(x, true, device, stream) : Quantised(), first ? quantised(x, false, device, stream) : Quantised()};
+  QuantisedBoth b{room(x.size(0), x.size(1), device), room(x.size(1), x.size(0), device)};
+  const tnx_mx_args a = quantising(x, true, b.last, stream);
+  uint8_t* other = (uint8_t*)b.first.buffer.data_ptr();
+  b.last.status = b.first.status = ops.quantize_both(&a, other, other + b.first.code_bytes);
+  return b;
 }
 
 // mx_quantize(x, along its last dimension) -> (buffer, bytes of codes), or None
@@ -577,54 +599,61 @@ Multiplied multiplied(const Quantised& a, const Quantised& b, int64_t m, int64_t
   return r;
 }
 
-// mx_linear(x, w) -> x w; mx_linear_backward(dy, x, w, wants dx, wants dw) -> (dx or None, dw or None); or None
-bool linear_operands(PyObject* x, PyObject* w, const at::Tensor** tx, const at::Tensor** tw, c10::DeviceIndex* device) {
-  return here(x, 2, tx, device) && here(w, 2, tw, device) && (*tx)->size(1) == (*tw)->size(0) && (*tx)->scalar_type() == (*tw)->scalar_type() &&
-         float_code((*tx)->scalar_type()) >= 0 && (*tx)->numel() > 0 && (*tw)->numel() > 0;
-}
+// The training step of a linear layer as a node of the autograd graph: y = x w, dx = dy w^T, dw = x^T dy.  Each matrix is read once, for both of
+// its quantisations; kept for the backward pass are the quantised x and w (17/32 of a byte an element) that its products take.
+struct LinearStep : torch::autograd::Function<LinearStep> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, bool wants_dx, bool wants_dw) {
+    const c10::DeviceIndex device = (c10::DeviceIndex)x.get_device();
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    const int64_t m = x.size(0), k = x.size(1), n = w.size(1);
+    QuantisedBoth qx, qw;
+    Multiplied y;
+    {
+      const Unlocked unlocked;
+      qx = quantised(x, true, wants_dw, device, stream);
+      qw = quantised(w, wants_dx, true, device, stream);
+      y = multiplied(qx.last, qw.first, m, n, k, x.scalar_type(), device, stream);
+    }
+    if (y.status != TNX_OK || (wants_dw && qx.first.status != TNX_OK) || (wants_dx && qw.last.status != TNX_OK)) throw std::runtime_error("mx_linear");
+    if (wants_dx || wants_dw) {
+      ctx->save_for_backward({qx.first.buffer, qw.last.buffer});
+      ctx->saved_data["m"] = m;
+      ctx->saved_data["k"] = k;
+      ctx->saved_data["n"] = n;
+      ctx->saved_data["type"] = (int64_t)x.scalar_type();
+    }
+    return y.out;
+  }
+  // (on a thread of the engine's, with the streams and the device of the forward call)
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const at::Tensor& dy = grads[0];
+    const auto saved = ctx->get_saved_variables();
+    const int64_t m = ctx->saved_data["m"].toInt(), k = ctx->saved_data["k"].toInt(), n = ctx->saved_data["n"].toInt();
+    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+    TORCH_CHECK(plain(dy, 2) && dy.size(0) == m && dy.size(1) == n && dy.scalar_type() == type, "mx_linear: a gradient that is not an ordinary tensor of the result's size and type");
+    const bool wants_dx = ctx->needs_input_grad(0) && saved[1].defined(), wants_dw = ctx->needs_input_grad(1) && saved[0].defined();
+    const c10::DeviceIndex device = (c10::DeviceIndex)dy.get_device();
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    const QuantisedBoth qy = quantised(dy, wants_dx, wants_dw, device, stream);
+    Multiplied dx{{}, TNX_OK}, dw{{}, TNX_OK};
+    if (wants_dx) dx = multiplied(qy.last, {saved[1], (int64_t)ops.code_bytes(k, n), TNX_OK}, m, k, n, type, device, stream);
+    if (wants_dw) dw = multiplied({saved[0], (int64_t)ops.code_bytes(k, m), TNX_OK}, qy.first, k, n, m, type, device, stream);
+    TORCH_CHECK(dx.status == TNX_OK && dw.status == TNX_OK, "mx_linear: status ", dx.status != TNX_OK ? dx.status : dw.status, " in the backward pass");
+    return {dx.out, dw.out, at::Tensor(), at::Tensor()};
+  }
+};
 
+// mx_linear(x, w) -> x w with its place in the graph, or None
 PyObject* mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 2) Py_RETURN_NONE;
   try {
     const at::Tensor *x, *w;
     c10::DeviceIndex device = -1;
-    if (!linear_operands(args[0], args[1], &x, &w, &device)) Py_RETURN_NONE;
-    void* stream = c10::hip::getCurrentHIPStream(device).stream();
-    Multiplied y;
-    {
-      const Unlocked unlocked;
-      y = multiplied(quantised(*x, true, device, stream), quantised(*w, false, device, stream), x->size(0), w->size(1), x->size(1), x->scalar_type(), device, stream);
-    }
-    if (y.status != TNX_OK) Py_RETURN_NONE;
-    return THPVariable_Wrap(y.out);
-  } catch (...) {
-    return none();
-  }
-}
-
-PyObject* mx_linear_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 5) Py_RETURN_NONE;
-  try {
-    const at::Tensor *x, *w, *dy;
-    c10::DeviceIndex device = -1;
-    if (!linear_operands(args[1], args[2], &x, &w, &device) || !here(args[0], 2, &dy, &device) || dy->size(0) != x->size(0) || dy->size(1) != w->size(1) ||
-        dy->scalar_type() != x->scalar_type())
+    if (!here(args[0], 2, &x, &device) || !here(args[1], 2, &w, &device) || x->size(1) != w->size(0) || x->scalar_type() != w->scalar_type() ||
+        float_code(x->scalar_type()) < 0 || x->numel() == 0 || w->numel() == 0)
       Py_RETURN_NONE;
-    const bool wants_dx = args[3] == Py_True, wants_dw = args[4] == Py_True;
-    void* stream = c10::hip::getCurrentHIPStream(device).stream();
-    const int64_t m = x->size(0), k = x->size(1), cols = w->size(1);
-    Multiplied dx{{}, TNX_OK}, dw{{}, TNX_OK};
-    {
-      const Unlocked unlocked;
-      // dx = dy w^T along the columns of w, dw = x^T dy along the rows of x
-      if (wants_dx) dx = multiplied(quantised(*dy, true, device, stream), quantised(*w, true, device, stream), m, k, cols, x->scalar_type(), device, stream);
-      if (wants_dw) dw = multiplied(quantised(*x, false, device, stream), quantised(*dy, false, device, stream), k, cols, m, x->scalar_type(), device, stream);
-    }
-    if (dx.status != TNX_OK || dw.status != TNX_OK) Py_RETURN_NONE;
-    const Object ox = taken(wants_dx ? THPVariable_Wrap(dx.out) : (Py_INCREF(Py_None), Py_None));
-    const Object ow = taken(wants_dw ? THPVariable_Wrap(dw.out) : (Py_INCREF(Py_None), Py_None));
-    if (!ox.p || !ow.p) return nullptr;
-    return PyTuple_Pack(2, ox.p, ow.p);
+    const bool graph = at::GradMode::is_enabled();
+    return THPVariable_Wrap(LinearStep::apply(*x, *w, graph && x->requires_grad(), graph && w->requires_grad()));
   } catch (...) {
     return none();
   }
@@ -742,7 +771,6 @@ PyMethodDef methods[] = {
     {"mx_dequantize", (PyCFunction)(void (*)(void))mx_dequantize, METH_FASTCALL, nullptr},
     {"mx_product", (PyCFunction)(void (*)(void))mx_product, METH_FASTCALL, nullptr},
     {"mx_linear", (PyCFunction)(void (*)(void))mx_linear, METH_FASTCALL, nullptr},
-    {"mx_linear_backward", (PyCFunction)(void (*)(void))mx_linear_backward, METH_FASTCALL, nullptr},
     {"moe_route", (PyCFunction)(void (*)(void))moe_route, METH_FASTCALL, nullptr},
     {"moe_backward", (PyCFunction)(void (*)(void))moe_backward, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -84,6 +84,18 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   return v > b ? v : b;
 }
 
+// the largest of the N lanes (8 or 16) that share a block
+template <int N> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  v = quad_max(v);
+  const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true);     // the mirrored lane of eight: of the other quad
+  v = v > a ? v : a;
+  if (N == 16) {
+    const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true);   // of sixteen
+    v = v > b ? v : b;
+  }
+  return v;
+}
+
 // eight neighbouring elements, at any alignment of an element
 template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Run8 { typename Elem<T>::raw v[8]; };
 

@@ -34,6 +34,7 @@ struct QuantParams {
   int64_t rows, k, slabs, batch;
   int64_t stride_b, stride_r, stride_k;                  // elements of src / dst
   int64_t codes_b, scales_b;                             // bytes from one matrix of the batch to the next
+  uint8_t *codes2, *scales2;                             // the same matrix quantised along its rows instead (quantize_columns_kernel)
 };
 
 // Runs that a lane takes, 256 lanes apart.  8192 x 8192 bfloat16: quantising 30.9 us with two, 35.6 with four (the next workgroups' loads begin sooner).
@@ -146,10 +147,15 @@ template <class T> constexpr int col_lane = 8 / sizeof(typename Elem<T>::raw);
 template <class T> struct __attribute__((packed, aligned(sizeof(T)))) RunC { typename Elem<T>::raw v[col_lane<T>]; };
 
 // RUNS: rows are neighbours in memory (stride_r == 1); otherwise any strides, an element at a time
-template <class T, bool RUNS>
+// BOTH: the matrix quantised along its rows as well, from the registers: a block of 32 neighbouring rows is 8 lanes (16 of float32), whose
+// largest magnitude goes round them for each k.  In the words of the other tensor, a row's codes are 2 bytes (1) a lane.
+template <class T, bool RUNS, bool BOTH>
 __global__ __launch_bounds__(512) void quantize_columns_kernel(QuantParams p) {
   typedef typename Elem<T>::raw raw;
   constexpr int COL_LANE = col_lane<T>, COL_ROWS = 64 * COL_LANE;
+  constexpr int BYTES2 = COL_ROWS / 2, PITCH2 = BYTES2 + 16, BLOCKS2 = COL_ROWS / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t tile2[BOTH ? MX_SLAB * PITCH2 : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t tile2_s[BOTH ? MX_SLAB * BLOCKS2 : 16];
   __shared__ __attribute__((aligned(16))) uint8_t tile[COL_ROWS * COL_PITCH];
   __shared__ __attribute__((aligned(16))) uint8_t tile_s[COL_ROWS * MX_SCALEB];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -212,7 +218,47 @@ __global__ __launch_bounds__(512) void quantize_columns_kernel(QuantParams p) {
     tile_s[(COL_LANE * lane + h) * MX_SCALEB + wave] = (uint8_t)sb;
     __builtin_amdgcn_sched_barrier(0);                   // (one row's 32 floats at a time: all four at once spill)
   }
+  if (BOTH) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(x[i][0]), "+v"(x[i][1]));       // (unpacked once more, not kept unpacked)
+    const bool padding = row0 + (COL_LANE * lane & ~31) >= p.rows;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      raw top = 0;
+#pragma unroll
+      for (int h = 0; h < COL_LANE; ++h) {
+        const raw b = magnitude(element(i, h));
+        top = top > b ? top : b;
+      }
+      top = (raw)lanes_max<32 / COL_LANE>(top);
+      float factor;
+      const uint32_t sb = scale_byte(top_bits<T>(top), &factor);
+      uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, scaled(Elem<T>::get(element(i, 0)), factor), scaled(Elem<T>::get(element(i, 1)), factor), 1.0f, 0);
+      if (COL_LANE == 4)
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, scaled(Elem<T>::get(element(i, 2)), factor), scaled(Elem<T>::get(element(i, 3)), factor), 1.0f, 1);
+      uint8_t* at = tile2 + (wave * 32 + i) * PITCH2 + lane * (COL_LANE / 2);
+      if (COL_LANE == 4) *(uint16_t*)at = (uint16_t)c;
+      else *at = (uint8_t)c;
+      if (lane % (32 / COL_LANE) == 0) tile2_s[(wave * 32 + i) * BLOCKS2 + lane / (32 / COL_LANE)] = (uint8_t)(padding ? 127u : sb);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+  }
   __syncthreads();
+  if (BOTH) {
+    const int64_t slabs2 = mx_slabs(p.rows), slab2 = row0 / MX_SLAB, k2 = slab * MX_SLAB;
+    const int part = (int)(row0 % MX_SLAB) / COL_ROWS;
+#pragma unroll
+    for (int u = 0; u < MX_SLAB * (BYTES2 / 16) / 512; ++u) {
+      const int i = u * 512 + tid, row = i / (BYTES2 / 16), chunk = i % (BYTES2 / 16);
+      if (k2 + row < p.k)
+        *(i32x4*)(p.codes2 + ((k2 + row) * slabs2 + slab2) * MX_ROWB + part * BYTES2 + chunk * 16) = *(const i32x4*)(tile2 + row * PITCH2 + chunk * 16);
+    }
+    if (tid < MX_SLAB && k2 + tid < p.k) {
+      uint8_t* at = p.scales2 + mx_scale_at(k2 + tid, slab2, slabs2) + part * BLOCKS2;
+      if (BLOCKS2 == 8) *(uint64_t*)at = *(const uint64_t*)(tile2_s + tid * 8);
+      else *(uint32_t*)at = *(const uint32_t*)(tile2_s + tid * 4);
+    }
+  }
 #pragma unroll
   for (int u = 0; u < COL_ROWS * 8 / 512; ++u) {
     const int i = u * 512 + tid, row = i >> 3, chunk = i & 7;
@@ -317,9 +363,29 @@ template <class T, bool BACK> int launch(const QuantParams& p, hipStream_t strea
   const bool runs = p.stride_r == 1;
   if (BACK && runs) hipLaunchKernelGGL((dequantize_columns_kernel<T, true>), grid, dim3(512), 0, stream, p);
   else if (BACK) hipLaunchKernelGGL((dequantize_columns_kernel<T, false>), grid, dim3(512), 0, stream, p);
-  else if (runs) hipLaunchKernelGGL((quantize_columns_kernel<T, true>), grid, dim3(512), 0, stream, p);
-  else hipLaunchKernelGGL((quantize_columns_kernel<T, false>), grid, dim3(512), 0, stream, p);
+  else if (runs) hipLaunchKernelGGL((quantize_columns_kernel<T, true, false>), grid, dim3(512), 0, stream, p);
+  else hipLaunchKernelGGL((quantize_columns_kernel<T, false, false>), grid, dim3(512), 0, stream, p);
   return mx_launched();
+}
+
+// p: the matrix's columns, neighbours in memory
+template <class T> int launch_both(const QuantParams& p, hipStream_t stream) {
+  const int64_t tiles = mx_slabs(p.rows) * (MX_SLAB / (64 * col_lane<T>));         // (whole slabs of the rows too)
+  if (tiles > 0x7fffff || p.slabs > 65535) return TNX_E_UNSUPPORTED;
+  hipLaunchKernelGGL((quantize_columns_kernel<T, true, true>), dim3((unsigned)tiles, (unsigned)p.slabs), dim3(512), 0, stream, p);
+  return mx_launched();
+}
+
+void fill(const tnx_mx_args* a, QuantParams* p) {
+  p->src = (const uint8_t*)a->data;
+  p->dst = (uint8_t*)a->data;
+  p->codes = (uint8_t*)a->codes;
+  p->scales = (uint8_t*)a->scales;
+  p->rows = a->rows; p->k = a->k; p->slabs = mx_slabs(a->k); p->batch = a->batch;
+  p->stride_b = a->stride_batch; p->stride_r = a->stride_row; p->stride_k = a->k == 1 ? 1 : a->stride_k;
+  p->codes_b = mx_code_bytes(a->rows, a->k);
+  p->scales_b = mx_scale_bytes(a->rows, a->k);
+  p->codes2 = p->scales2 = nullptr;
 }
 
 template <bool BACK> int convert(const tnx_mx_args* a) {
@@ -330,14 +396,7 @@ template <bool BACK> int convert(const tnx_mx_args* a) {
   const unsigned size = a->dtype == TNX_F32 ? 4 : 2;
   if ((uintptr_t)a->data & (size - 1)) return TNX_E_INVALID;
   QuantParams p;
-  p.src = (const uint8_t*)a->data;
-  p.dst = (uint8_t*)a->data;
-  p.codes = (uint8_t*)a->codes;
-  p.scales = (uint8_t*)a->scales;
-  p.rows = a->rows; p.k = a->k; p.slabs = mx_slabs(a->k); p.batch = a->batch;
-  p.stride_b = a->stride_batch; p.stride_r = a->stride_row; p.stride_k = a->k == 1 ? 1 : a->stride_k;
-  p.codes_b = mx_code_bytes(a->rows, a->k);
-  p.scales_b = mx_scale_bytes(a->rows, a->k);
+  fill(a, &p);
   const hipStream_t stream = (hipStream_t)a->stream;
   switch (a->dtype) {
     case TNX_BF16: return launch<__bf16, BACK>(p, stream);
@@ -353,6 +412,36 @@ extern "C" size_t tnx_mx_code_bytes(int64_t rows, int64_t k) { return rows > 0 &
 extern "C" size_t tnx_mx_scale_bytes(int64_t rows, int64_t k) { return rows > 0 && k > 0 ? (size_t)mx_scale_bytes(rows, k) : 0; }
 
 extern "C" int tnx_mx_quantize(const tnx_mx_args* a) { return convert<false>(a); }
+extern "C" int tnx_mx_quantize_both(const tnx_mx_args* a, void* codes2, void* scales2) {
+  if (!a || a->batch != 1 || a->rows < 0 || a->k < 0) return TNX_E_INVALID;
+  if (a->rows == 0 || a->k == 0) return TNX_OK;
+  if (!codes2 || !scales2 || ((uintptr_t)codes2 & 15) || ((uintptr_t)scales2 & 15)) return TNX_E_INVALID;
+  if (a->rows > TNX_MX_MAX_K) return TNX_E_UNSUPPORTED;
+  tnx_mx_args other = *a;                                // the same matrix with the parts of its two dimensions exchanged
+  other.codes = codes2; other.scales = scales2;
+  other.rows = a->k; other.k = a->rows;
+  other.stride_row = a->stride_k; other.stride_k = a->stride_row;
+  const bool along = a->stride_k == 1 && a->rows > 1 && a->k > 1;      // k is the contiguous one: the columns are the other tensor's
+  const tnx_mx_args *columns = along ? &other : a, *rows = along ? a : &other;
+  if (columns->stride_row != 1 || columns->rows == 1 || columns->k == 1) {       // neither is, or a vector
+    const int status = tnx_mx_quantize(a);
+    return status != TNX_OK ? status : tnx_mx_quantize(&other);
+  }
+  if (!a->data || !a->codes || !a->scales || ((uintptr_t)a->codes & 15) || ((uintptr_t)a->scales & 15)) return TNX_E_INVALID;
+  if (a->k > TNX_MX_MAX_K) return TNX_E_UNSUPPORTED;
+  if ((uintptr_t)a->data & (a->dtype == TNX_F32 ? 3 : 1)) return TNX_E_INVALID;
+  QuantParams p;
+  fill(columns, &p);
+  p.codes2 = (uint8_t*)rows->codes;
+  p.scales2 = (uint8_t*)rows->scales;
+  const hipStream_t stream = (hipStream_t)a->stream;
+  switch (a->dtype) {
+    case TNX_BF16: return launch_both<__bf16>(p, stream);
+    case TNX_F16: return launch_both<_Float16>(p, stream);
+    case TNX_F32: return launch_both<float>(p, stream);
+    default: return TNX_E_UNSUPPORTED;
+  }
+}
 extern "C" int tnx_mx_dequantize(const tnx_mx_args* a) { return convert<true>(a); }
 
 extern "C" int tnx_mx_import(const void* codes, const void* scales, int64_t batch, int64_t rows, int64_t k, void* out_codes, void* out_scales,

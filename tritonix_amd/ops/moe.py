@@ -7,6 +7,9 @@
 joined per token).  ``w12[e, d, 2f]`` is interleaved column-wise like ``glu``'s; both weights are ``MXTensor`` batches quantised along the dimension
 that is summed over (``mx_quantize(w, dim=-2)`` or ``MXTensor.from_codes(..., dim=-2)``).  Nothing here waits for the GPU: the
 rows of each expert are counted and found on it.
+
+The router is trained through ``Routing.weights``, which carries its gradient; the experts' products are for answering and
+carry none, neither to x nor to the weights.
 """
 from __future__ import annotations
 
@@ -189,6 +192,8 @@ def _backward(grad, logits, weights, experts, options):
     out = (_mx.native or _mx.find_native()).moe_backward(grad, logits, weights, experts, _SCORING[options[0]], options[4], options[5])
     if out is not None:
         return out
+    _check_field("moe_route_backward", "weights", weights, torch.float32, tuple(grad.shape))
+    _check_field("moe_route_backward", "experts", experts, torch.int32, tuple(grad.shape))
     index = on_device("moe_route_backward", grad, logits, weights, experts)
     a = _route_args(logits, None, experts.shape[1], options)
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -209,7 +214,18 @@ def moe_route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, routing
     return _backward(grad_weights, logits, routing.weights, routing.experts, (routing.scoring, 1, 1, 1, routing.renormalize, routing.scale))
 
 
+def _check_field(name: str, field: str, t: torch.Tensor, dtype, shape) -> None:
+    """The kernels read a routing as it was made: one that was changed since has to have kept its types and sizes."""
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: routing.{field} is contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
 def _check_experts(name: str, x, w, routing: Routing, rows: int) -> None:
+    slots = tuple(routing.experts.shape)
+    _check_field(name, "offsets", routing.offsets, torch.int32, (routing.num_experts + 1,))
+    _check_field(name, "order", routing.order, torch.int32, (routing.tokens * routing.top_k,))
+    _check_field(name, "rows", routing.rows, torch.int32, slots)
+    _check_field(name, "weights", routing.weights, torch.float32, slots)
     if not isinstance(w, MXTensor) or w.batch is None:
         raise ValueError(f"{name}: the experts' weights are an MXTensor of shape [experts, k, n]")
     if w.batch != routing.num_experts:
@@ -242,7 +258,7 @@ def moe_glu(x, w12: MXTensor, routing: Routing, activation: str = "silu", out_dt
     if out_dtype is None:
         out_dtype = torch.bfloat16 if isinstance(x, MXTensor) else x.dtype
     dtype_code("moe_glu", out_dtype)
-    index = on_device("moe_glu", x, w12, routing.order)
+    index = on_device("moe_glu", x, w12, routing.offsets, routing.order)
     xq = x if takes_rows(x) else operand("moe_glu", "x", x, -1)
     out = torch.empty((routing.tokens * routing.top_k, w12.rows // 2), dtype=out_dtype, device=w12.device)
     _grouped("moe_glu", xq, w12, routing, out, True, epilogue_of(activation), index)
@@ -263,7 +279,7 @@ def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
     if out_dtype is None:
         out_dtype = torch.bfloat16 if isinstance(h, MXTensor) else h.dtype
     code = dtype_code("moe_down", out_dtype)
-    index = on_device("moe_down", h, w3, routing.order)
+    index = on_device("moe_down", h, w3, routing.offsets, routing.rows, routing.weights)
     hq = h if takes_rows(h) else operand("moe_down", "h", h, -1)
     n = w3.rows
     rows = routing.tokens * routing.top_k

@@ -38,7 +38,7 @@ class _Interpreter:
     def _none(*_):
         return None
 
-    mx_quantize = mx_dequantize = mx_product = mx_linear = mx_linear_backward = moe_route = moe_backward = _none
+    mx_quantize = mx_dequantize = mx_product = mx_linear = moe_route = moe_backward = _none
 
 
 # csrc/launch.cpp, which makes the ordinary calls without the interpreter's share of them; found with the first call
@@ -53,7 +53,7 @@ def find_native():
     else:
         lib = _C.load()
         module.bind_ops(tuple(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
-            lib.tnx_mx_code_bytes, lib.tnx_mx_scale_bytes, lib.tnx_mx_quantize, lib.tnx_mx_dequantize, lib.tnx_mx_gemm_takes_rows, lib.tnx_mx_gemm,
+            lib.tnx_mx_code_bytes, lib.tnx_mx_scale_bytes, lib.tnx_mx_quantize, lib.tnx_mx_quantize_both, lib.tnx_mx_dequantize, lib.tnx_mx_gemm_takes_rows, lib.tnx_mx_gemm,
             lib.tnx_moe_workspace_bytes, lib.tnx_moe_route, lib.tnx_moe_route_backward, lib.tnx_moe_combine)) + (JOIN_BYTES,))
         native = module
     return native
@@ -314,18 +314,16 @@ def mx_glu(x, w12, activation: str = "silu", out_dtype=None) -> torch.Tensor:
 
 
 class _Linear(torch.autograd.Function):
+    """What the native side has not taken; it keeps x and w themselves."""
+
     @staticmethod
     def forward(ctx, x, w):
         ctx.save_for_backward(x, w)
-        y = (native or find_native()).mx_linear(x, w)
-        return mx_matmul(x, w) if y is None else y
+        return mx_matmul(x, w)
 
     @staticmethod
     def backward(ctx, dy):
         x, w = ctx.saved_tensors
-        both = (native or find_native()).mx_linear_backward(dy, x, w, *ctx.needs_input_grad)
-        if both is not None:
-            return both
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = mx_matmul(dy, w.t(), out_dtype=x.dtype)
@@ -338,7 +336,11 @@ def mx_linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """``x[m, k] @ w[k, n]`` with all three products of a training step microscaled.
 
     Forward: x and w quantised along k.  Backward: ``dx = dy @ w^T`` with both quantised along n, ``dw = x^T @ dy`` with both
-    quantised along m; the rounding of the operands counts as the identity.  x and w are kept in their own types."""
+    quantised along m; the rounding of the operands counts as the identity.  For the backward pass x and w are kept quantised, as its products
+    take them."""
+    y = (native or find_native()).mx_linear(x, w)
+    if y is not None:
+        return y
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[0]:
         raise ValueError(f"mx_linear expects x[m,k] and w[k,n], got {tuple(x.shape)} and {tuple(w.shape)}")
     if x.dtype != w.dtype:
