@@ -26,10 +26,12 @@ struct RouteParams {
 struct PlanParams {
   const int32_t* experts;
   int32_t *offsets, *order, *rows;
-  int32_t *counts, *totals;                // workspace: [experts][blocks] and [experts]
+  int32_t *counts, *totals;                // workspace: [experts][blocks] where they are summed first, else [blocks][experts]; and [experts]
   int64_t pairs;
   int e, block, blocks, words;             // pairs of a block, blocks, 64-bit words of a block's bits
   bool fused;                              // the routing kernel's workgroups are the blocks, and count
+  bool summed;                             // the counts are summed over the blocks by a launch of their own
+  __device__ __forceinline__ int64_t count_at(int expert, int at) const { return summed ? (int64_t)expert * blocks + at : (int64_t)at * e + expert; }
 };
 
 __device__ __forceinline__ float load_logit(const uint8_t* p, int64_t i, int dtype) {
@@ -199,7 +201,7 @@ __device__ __forceinline__ void plan_alone(const PlanParams& p, const int* ids, 
 
 // Scores and choice.  L lanes share a token and hold EPL experts each.  The choice is top_k rounds of a maximum over all keys, then the lowest expert that
 // has it.  Bound by its instructions: eight lanes of sixteen experts where there are tokens enough to fill the card, a wave per token
-// where there are few and a token's own time counts.  65536 tokens, 8 of 128 experts: 0 us; with a search through all sixteen registers
+// where there are few and a token's own time counts.  65536 tokens, 8 of 128 experts: 18.4 us; with a search through all sixteen registers
 // each round 22, with the lanes' keys sorted first as doubles that hold key and expert 84 (a compare is one instruction, but not a fast one).
 // FULL: with a bias or groups.  smem: a workgroup's own.
 template <int L, int EPL, bool FULL>
@@ -404,7 +406,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p, PlanParams q)
     for (int r = 0; r < KR; ++r)
       if ((int64_t)blockIdx.x * (256 / L) + slot < p.tokens && r * L + j < p.k && id[r] >= 0) bits.mark(id[r], slot * p.k + r * L + j);
     __syncthreads();
-    for (int e = tid; e < q.e; e += 256) q.counts[(int64_t)e * q.blocks + blockIdx.x] = bits.count(e);
+    for (int e = tid; e < q.e; e += 256) q.counts[q.count_at(e, blockIdx.x)] = bits.count(e);
   }
 }
 
@@ -436,7 +438,7 @@ __global__ __launch_bounds__(256) void plan_count_kernel(PlanParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t moe_smem[];
   const PairBits bits{(unsigned long long*)moe_smem, p.words};
   mark_pairs(p, bits, threadIdx.x);
-  for (int e = threadIdx.x; e < p.e; e += 256) p.counts[(int64_t)e * p.blocks + blockIdx.x] = bits.count(e);
+  for (int e = threadIdx.x; e < p.e; e += 256) p.counts[p.count_at(e, blockIdx.x)] = bits.count(e);
 }
 
 // counts[e][block] -> pairs of e in the blocks before it; a workgroup per expert, eight neighbouring blocks a thread (65536 tokens of 8 pairs: 2048 blocks,
@@ -485,20 +487,36 @@ __global__ __launch_bounds__(256) void plan_place_kernel(PlanParams p) {
   int* own = base + p.e;                   // pairs of the expert in the blocks before this one
   const int tid = threadIdx.x;
   const int64_t first = (int64_t)blockIdx.x * p.block;
-  for (int e = tid; e < p.e; e += 256) {
-    if (SUMMED) {
+  if (SUMMED) {
+    for (int e = tid; e < p.e; e += 256) {
       base[e] = p.totals[e];
       own[e] = p.counts[(int64_t)e * p.blocks + blockIdx.x];
-    } else {
+    }
+  } else {
+    // Neighbouring threads have neighbouring experts, and where there are threads left over, several share an expert's blocks.  129 blocks of 60
+    // experts: 5.4 us for all of it; with a thread per expert and the counts of an expert's blocks side by side 8.0.
+    for (int e = tid; e < p.e; e += 256) base[e] = own[e] = 0;
+    __syncthreads();
+    const int shares = p.e < 256 ? 256 / p.e : 1;
+    for (int i = tid; i < p.e * shares; i += 256) {
+      const int share = i / p.e, e = i - share * p.e;
       int all = 0, before = 0;
-#pragma unroll 8
-      for (int b = 0; b < p.blocks; ++b) {
-        const int c = p.counts[(int64_t)e * p.blocks + b];
-        all += c;
-        before += b < (int)blockIdx.x ? c : 0;
+      for (int b0 = share; b0 < p.blocks; b0 += 16 * shares) {
+        int c[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const int b = b0 + u * shares;
+          c[u] = p.counts[(int64_t)(b < p.blocks ? b : b0) * p.e + e];
+        }
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const int b = b0 + u * shares;
+          all += b < p.blocks ? c[u] : 0;
+          before += b < (int)blockIdx.x ? c[u] : 0;
+        }
       }
-      base[e] = all;
-      own[e] = before;
+      atomicAdd(&base[e], all);                            // (in LDS, and of integers: any order gives the same)
+      atomicAdd(&own[e], before);
     }
   }
   mark_pairs(p, bits, tid);
@@ -523,7 +541,7 @@ __global__ __launch_bounds__(256) void plan_place_kernel(PlanParams p) {
 //            neither the logits nor the other experts enter: dl_j = w_j (g_j - sum_i (w_i / scale) g_i)
 //   sigmoid: dl_j = ds_j s_j (1 - s_j), of the chosen alone
 // The chosen experts' values go through a row in LDS that starts as zeros, and the row leaves in runs of four.  Bound by writing the
-// gradient: 65536 x 128, float32, renormalised softmax: 0 us for 33.5 MB.  (Compared one by one with every lane's experts: 13.6 us.)
+// gradient: 65536 x 128, float32, renormalised softmax: 7.7 us for 33.5 MB.  (Compared one by one with every lane's experts: 13.6 us.)
 template <int L, int EPL>
 __global__ __launch_bounds__(256) void route_backward_kernel(RouteParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t moe_smem[];
@@ -675,7 +693,9 @@ int route_lanes(int64_t tokens, int e) {
   if (e > 512 || tokens <= 1024) return 64;
   return e <= 128 ? 8 : e <= 256 ? 16 : 32;
 }
-constexpr int SUM_BLOCKS = 256;            // more blocks than this are summed by a launch of their own
+// Counts of more blocks, or more of them for a thread, are summed by a launch of their own.  A placing workgroup reads 16 at a time, and that takes what
+// memory takes: 161 blocks of 512 experts (322 a thread) 17.5 us, summed first 7.3; 111 of 160 (111 a thread) 7.7, 75 of 256 6.4.
+constexpr int SUM_BLOCKS = 256, SUM_LOADS = 160;
 
 // The plan's blocks are the pairs of a routing workgroup's 256 / lanes tokens; many tokens at four a workgroup are counted apart, in larger blocks.
 void plan_shape(PlanParams* q, int64_t tokens, int k, int e) {
@@ -686,6 +706,7 @@ void plan_shape(PlanParams* q, int64_t tokens, int k, int e) {
   q->block = q->fused ? 256 / lanes * k : 512;
   q->blocks = (int)((q->pairs + q->block - 1) / q->block);
   q->words = (q->block + 63) / 64;
+  q->summed = q->blocks > SUM_BLOCKS || (int64_t)q->blocks * q->e > SUM_LOADS * 256;
 }
 bool plan_is_alone(const PlanParams& q) { return q.blocks <= 1 && q.pairs <= PLAN_ALONE; }
 size_t bits_lds(const PlanParams& q) { return (size_t)q.e * q.words * 8; }
@@ -717,7 +738,7 @@ PlanParams plan_params(const tnx_moe_args* a) {
 // the launches after the counts
 int place_pairs(const PlanParams& q, hipStream_t stream) {
   const size_t lds = bits_lds(q) + (size_t)q.e * 8;
-  if (q.blocks > SUM_BLOCKS) {
+  if (q.summed) {
     hipLaunchKernelGGL(plan_sum_kernel, dim3((unsigned)q.e), dim3(256), 0, stream, q);
     const int st = mx_launched();
     if (st) return st;

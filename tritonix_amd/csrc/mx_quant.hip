@@ -140,63 +140,102 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(QuantParams p) {
   }
 }
 
-// Columns: a workgroup takes 256 rows (128 of float32) and one slab, wave b the block b of it, a lane 8 bytes of neighbouring rows: a load
-// instruction is 512 bytes of one k.  (4 bytes a lane: 8192 x 8192 bfloat16 57 us, with 8 37.)  Pitch of a row of codes in LDS: 16 bytes more than 128, so that the lanes' 16-byte pieces fall on different banks.
-constexpr int COL_PITCH = MX_ROWB + 16;
-template <class T> constexpr int col_lane = 8 / sizeof(typename Elem<T>::raw);
-template <class T> struct __attribute__((packed, aligned(sizeof(T)))) RunC { typename Elem<T>::raw v[col_lane<T>]; };
+// Columns: wave b of a workgroup takes the b-th 32 k of its part of a slab, a lane LANE neighbouring rows, which it reads 32 times: a load
+// instruction is one k.  Two shapes.  WIDE: a whole slab by 8 bytes a lane, 256 rows (128 of float32), so that loads are runs of 512 bytes (4 bytes a lane:
+// 8192 x 8192 bfloat16 57 us, with 8 37) and stores whole rows of a slab.  Small, where that makes fewer workgroups than the card has
+// CUs: 64 k by 128 rows (512 x 512 bfloat16, quantised, back and both ways at once: 3.0, 6.0 and 5.8 us, wide 5.9, 10.4 and 11.0;
+// 8192 x 4096: 18.8, 17.4 and 27.3, wide 16.4, 16.2 and 24.3).  Pitch of a row of codes in LDS: 16 bytes more, so that the lanes' 16-byte pieces fall on different banks.
+template <class T, bool WIDE> struct Columns {
+  static constexpr int LANE = WIDE ? 8 / sizeof(typename Elem<T>::raw) : 2, WAVES = WIDE ? 8 : 2, THREADS = 64 * WAVES;
+  static constexpr int ROWS = 64 * LANE, K = 32 * WAVES, PARTS = 8 / WAVES;      // of a workgroup; workgroups along a slab
+  static constexpr int CHUNKS = WAVES, PITCH = 16 * WAVES + 16;                   // a row's 16-byte pieces
+  static constexpr int WORDS = LANE * (int)sizeof(typename Elem<T>::raw) / 4;     // of a lane and k
+};
+template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) RunC { typename Elem<T>::raw v[N]; };
 
 // RUNS: rows are neighbours in memory (stride_r == 1); otherwise any strides, an element at a time
-// BOTH: the matrix quantised along its rows as well, from the registers: a block of 32 neighbouring rows is 8 lanes (16 of float32), whose
-// largest magnitude goes round them for each k.  In the words of the other tensor, a row's codes are 2 bytes (1) a lane.
-template <class T, bool RUNS, bool BOTH>
-__global__ __launch_bounds__(512) void quantize_columns_kernel(QuantParams p) {
+// BOTH: the matrix quantised along its rows as well, from the registers: a block of 32 neighbouring rows is 8 lanes (16 with two rows each), whose
+// largest magnitude goes round them for each k.  In the words of the other tensor, a row's codes are 2 bytes (1) a lane.  8192 x 4096 bfloat16: 24.3 us,
+// one after the other 18.6 + 16.4.
+template <class T, bool WIDE, bool RUNS, bool BOTH>
+__global__ __launch_bounds__((Columns<T, WIDE>::THREADS)) void quantize_columns_kernel(QuantParams p) {
   typedef typename Elem<T>::raw raw;
-  constexpr int COL_LANE = col_lane<T>, COL_ROWS = 64 * COL_LANE;
-  constexpr int BYTES2 = COL_ROWS / 2, PITCH2 = BYTES2 + 16, BLOCKS2 = COL_ROWS / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t tile2[BOTH ? MX_SLAB * PITCH2 : 16];
-  __shared__ __attribute__((aligned(16))) uint8_t tile2_s[BOTH ? MX_SLAB * BLOCKS2 : 16];
-  __shared__ __attribute__((aligned(16))) uint8_t tile[COL_ROWS * COL_PITCH];
-  __shared__ __attribute__((aligned(16))) uint8_t tile_s[COL_ROWS * MX_SCALEB];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t slab = blockIdx.y, row0 = (int64_t)blockIdx.x * COL_ROWS;
+  typedef Columns<T, WIDE> C;
+  constexpr int LANE = C::LANE, W = C::WORDS, BITS = 8 * sizeof(raw);
+  constexpr int BYTES2 = C::ROWS / 2, PITCH2 = BYTES2 + 16, BLOCKS2 = C::ROWS / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t tile[C::ROWS * C::PITCH];
+  __shared__ __attribute__((aligned(16))) uint8_t tile_s[C::ROWS * C::WAVES];
+  __shared__ __attribute__((aligned(16))) uint8_t tile2[BOTH ? C::K * PITCH2 : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t tile2_s[BOTH ? C::K * BLOCKS2 : 16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t slab = blockIdx.y / C::PARTS, row0 = (int64_t)blockIdx.x * C::ROWS;
+  const int part = blockIdx.y % C::PARTS;
   const raw* src = (const raw*)p.src + (int64_t)blockIdx.z * p.stride_b;
   uint8_t* codes = p.codes + (int64_t)blockIdx.z * p.codes_b;
   uint8_t* scales = p.scales + (int64_t)blockIdx.z * p.scales_b;
-  const int64_t k0 = slab * MX_SLAB + wave * 32, left = p.k - k0;
-  const int64_t r = row0 + COL_LANE * lane, rows_left = p.rows - r;
-  // the lane's 8 bytes of each k, as two words (the empty asm keeps them so: 32 x 4 unpacked elements spill)
-  uint32_t x[32][2];
-  const raw* s = src + k0 * p.stride_k + r * p.stride_r;
-  if (RUNS && rows_left >= COL_LANE && left >= 32) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      // 2-byte elements past the caches: a source that is not in them comes at 2 TB/s otherwise (8192 x 4096 bfloat16 42 us, so 17; float32 is the same
-      // either way from memory, and 53 us or 70 for 8192 x 8192 where it is in the caches)
-      typedef i32x2 __attribute__((aligned(2))) loose2;
-      const loose2* at = (const loose2*)(s + i * p.stride_k);
-      const i32x2 w = sizeof(raw) == 2 ? __builtin_nontemporal_load(at) : *at;
+  const int64_t k0 = slab * MX_SLAB + part * C::K + wave * 32, left = p.k - k0;
+  const int64_t r = row0 + LANE * lane, rows_left = p.rows - r;
+  // the lane's rows of each k, as words (the empty asm keeps them so: 32 x 4 unpacked elements spill)
+  uint32_t x[32][W];
+  // 2-byte elements past the caches: a source that is not in them comes at 2 TB/s otherwise (8192 x 4096 bfloat16 42 us, so 17; float32 is the same
+  // either way from memory, and 53 us or 70 for 8192 x 8192 where it is in the caches)
+  auto load = [&](int i, const raw* at) __attribute__((always_inline)) {
+    typedef i32x2 __attribute__((aligned(2))) loose2;
+    typedef int __attribute__((aligned(2))) loose1;
+    if constexpr (W == 2) {
+      const i32x2 w = sizeof(raw) == 2 ? __builtin_nontemporal_load((const loose2*)at) : *(const loose2*)at;
       x[i][0] = (uint32_t)w[0];
       x[i][1] = (uint32_t)w[1];
+    } else {
+      x[i][0] = (uint32_t)__builtin_nontemporal_load((const loose1*)at);
     }
-  } else {
+  };
+  if (RUNS && row0 + C::ROWS <= p.rows && left >= 32) {
+    const raw* s = src + k0 * p.stride_k + r;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) load(i, s + i * p.stride_k);
+  } else if (RUNS && p.rows >= LANE && left > 0) {
+    // An edge: every lane reads whole runs inside the matrix, the last rows' moved up to end with it, k past the end the last one again; then the rows
+    // that the lane does not have are shifted out and the k cleared.  (Element by element, each load waits for the one before.)
+    const int64_t run = rows_left >= LANE ? r : p.rows - LANE;
+    const int drop = rows_left >= LANE ? 0 : rows_left > 0 ? (int)(r - run) * BITS : 64;
+    const raw* s = src + k0 * p.stride_k + run;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) load(i, s + (i < left ? i : left - 1) * p.stride_k);
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      RunC<T> t;
+      uint64_t v = x[i][0];
+      if (W == 2) v |= (uint64_t)x[i][W - 1] << 32;
+      v = drop < 64 && i < left ? v >> drop : 0;
+      x[i][0] = (uint32_t)v;
+      if (W == 2) x[i][W - 1] = (uint32_t)(v >> 32);
+    }
+  } else {
+    const raw* s = src + k0 * p.stride_k + r * p.stride_r;
 #pragma unroll
-      for (int h = 0; h < COL_LANE; ++h) t.v[h] = i < left && h < rows_left ? s[i * p.stride_k + h * p.stride_r] : (raw)0;
-      __builtin_memcpy(x[i], &t, 8);
+    for (int i = 0; i < 32; ++i) {
+      RunC<T, LANE> t;
+#pragma unroll
+      for (int h = 0; h < LANE; ++h) t.v[h] = i < left && h < rows_left ? s[i * p.stride_k + h * p.stride_r] : (raw)0;
+      __builtin_memcpy(x[i], &t, 4 * W);
       if (sizeof(raw) == 2 && i % 8 == 7) {               // (eight k at a time: the elements of all 32 spill before they are packed)
 #pragma unroll
-        for (int q = i - 7; q <= i; ++q) asm volatile("" : "+v"(x[q][0]), "+v"(x[q][1]));
+        for (int q = i - 7; q <= i; ++q)
+#pragma unroll
+          for (int w = 0; w < W; ++w) asm volatile("" : "+v"(x[q][w]));
       }
     }
   }
+  auto pin = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(x[i][0]), "+v"(x[i][1]));
-  auto element = [&](int i, int h) __attribute__((always_inline)) { return sizeof(raw) == 4 ? (raw)x[i][h & 1] : (raw)(x[i][h >> 1 & 1] >> (h & 1) * 16); };
+    for (int i = 0; i < 32; ++i)
 #pragma unroll
-  for (int h = 0; h < COL_LANE; ++h) {
+      for (int w = 0; w < W; ++w) asm volatile("" : "+v"(x[i][w]));
+  };
+  pin();
+  auto element = [&](int i, int h) __attribute__((always_inline)) { return sizeof(raw) == 4 ? (raw)x[i][h % W] : (raw)(x[i][(h >> 1) % W] >> (h & 1) * 16); };
+#pragma unroll
+  for (int h = 0; h < LANE; ++h) {
     raw top = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
@@ -214,107 +253,119 @@ __global__ __launch_bounds__(512) void quantize_columns_kernel(QuantParams p) {
       for (int e = 0; e < 8; ++e) v[e] = scaled(Elem<T>::get(element(q * 8 + e, h)), factor);
       c[q] = (int)codes8(v);
     }
-    *(i32x4*)(tile + (COL_LANE * lane + h) * COL_PITCH + wave * 16) = c;
-    tile_s[(COL_LANE * lane + h) * MX_SCALEB + wave] = (uint8_t)sb;
+    *(i32x4*)(tile + (LANE * lane + h) * C::PITCH + wave * 16) = c;
+    tile_s[(LANE * lane + h) * C::WAVES + wave] = (uint8_t)sb;
     __builtin_amdgcn_sched_barrier(0);                   // (one row's 32 floats at a time: all four at once spill)
   }
   if (BOTH) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) asm volatile("" : "+v"(x[i][0]), "+v"(x[i][1]));       // (unpacked once more, not kept unpacked)
-    const bool padding = row0 + (COL_LANE * lane & ~31) >= p.rows;
+    pin();                                               // (unpacked once more, not kept unpacked)
+    const bool padding = row0 + (LANE * lane & ~31) >= p.rows;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       raw top = 0;
 #pragma unroll
-      for (int h = 0; h < COL_LANE; ++h) {
+      for (int h = 0; h < LANE; ++h) {
         const raw b = magnitude(element(i, h));
         top = top > b ? top : b;
       }
-      top = (raw)lanes_max<32 / COL_LANE>(top);
+      top = (raw)lanes_max<32 / LANE>(top);
       float factor;
       const uint32_t sb = scale_byte(top_bits<T>(top), &factor);
-      uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, scaled(Elem<T>::get(element(i, 0)), factor), scaled(Elem<T>::get(element(i, 1)), factor), 1.0f, 0);
-      if (COL_LANE == 4)
+      uint32_t c = 0;
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, scaled(Elem<T>::get(element(i, 0)), factor), scaled(Elem<T>::get(element(i, 1)), factor), 1.0f, 0);
+      if (LANE == 4)
         c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, scaled(Elem<T>::get(element(i, 2)), factor), scaled(Elem<T>::get(element(i, 3)), factor), 1.0f, 1);
-      uint8_t* at = tile2 + (wave * 32 + i) * PITCH2 + lane * (COL_LANE / 2);
-      if (COL_LANE == 4) *(uint16_t*)at = (uint16_t)c;
+      uint8_t* at = tile2 + (wave * 32 + i) * PITCH2 + lane * (LANE / 2);
+      if (LANE == 4) *(uint16_t*)at = (uint16_t)c;
       else *at = (uint8_t)c;
-      if (lane % (32 / COL_LANE) == 0) tile2_s[(wave * 32 + i) * BLOCKS2 + lane / (32 / COL_LANE)] = (uint8_t)(padding ? 127u : sb);
+      if (lane % (32 / LANE) == 0) tile2_s[(wave * 32 + i) * BLOCKS2 + lane / (32 / LANE)] = (uint8_t)(padding ? 127u : sb);
       if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
   __syncthreads();
   if (BOTH) {
-    const int64_t slabs2 = mx_slabs(p.rows), slab2 = row0 / MX_SLAB, k2 = slab * MX_SLAB;
-    const int part = (int)(row0 % MX_SLAB) / COL_ROWS;
+    const int64_t slabs2 = mx_slabs(p.rows), slab2 = row0 / MX_SLAB, k2 = slab * MX_SLAB + part * C::K;
+    const int part2 = (int)(row0 % MX_SLAB) / C::ROWS;
 #pragma unroll
-    for (int u = 0; u < MX_SLAB * (BYTES2 / 16) / 512; ++u) {
-      const int i = u * 512 + tid, row = i / (BYTES2 / 16), chunk = i % (BYTES2 / 16);
+    for (int u = 0; u < C::K * (BYTES2 / 16) / C::THREADS; ++u) {
+      const int i = u * C::THREADS + tid, row = i / (BYTES2 / 16), chunk = i % (BYTES2 / 16);
       if (k2 + row < p.k)
-        *(i32x4*)(p.codes2 + ((k2 + row) * slabs2 + slab2) * MX_ROWB + part * BYTES2 + chunk * 16) = *(const i32x4*)(tile2 + row * PITCH2 + chunk * 16);
+        *(i32x4*)(p.codes2 + ((k2 + row) * slabs2 + slab2) * MX_ROWB + part2 * BYTES2 + chunk * 16) = *(const i32x4*)(tile2 + row * PITCH2 + chunk * 16);
     }
-    if (tid < MX_SLAB && k2 + tid < p.k) {
-      uint8_t* at = p.scales2 + mx_scale_at(k2 + tid, slab2, slabs2) + part * BLOCKS2;
+    if (tid < C::K && k2 + tid < p.k) {
+      uint8_t* at = p.scales2 + mx_scale_at(k2 + tid, slab2, slabs2) + part2 * BLOCKS2;
       if (BLOCKS2 == 8) *(uint64_t*)at = *(const uint64_t*)(tile2_s + tid * 8);
       else *(uint32_t*)at = *(const uint32_t*)(tile2_s + tid * 4);
     }
   }
 #pragma unroll
-  for (int u = 0; u < COL_ROWS * 8 / 512; ++u) {
-    const int i = u * 512 + tid, row = i >> 3, chunk = i & 7;
+  for (int u = 0; u < C::ROWS * C::CHUNKS / C::THREADS; ++u) {
+    const int i = u * C::THREADS + tid, row = i / C::CHUNKS, chunk = i % C::CHUNKS;
     if (row0 + row < p.rows)
-      *(i32x4*)(codes + ((row0 + row) * p.slabs + slab) * MX_ROWB + chunk * 16) = *(const i32x4*)(tile + row * COL_PITCH + chunk * 16);
+      *(i32x4*)(codes + ((row0 + row) * p.slabs + slab) * MX_ROWB + (part * C::CHUNKS + chunk) * 16) = *(const i32x4*)(tile + row * C::PITCH + chunk * 16);
   }
   // (the scales of the whole groups of 32 rows that the tensor's allocation has)
-  if (tid < COL_ROWS && row0 + (tid & ~31) < p.rows)
-    *(uint64_t*)(scales + mx_scale_at(row0 + tid, slab, p.slabs)) = *(const uint64_t*)(tile_s + tid * MX_SCALEB);
+  if (tid < C::ROWS && row0 + (tid & ~31) < p.rows) {
+    uint8_t* at = scales + mx_scale_at(row0 + tid, slab, p.slabs) + part * C::WAVES;
+    if (C::WAVES == 8) *(uint64_t*)at = *(const uint64_t*)(tile_s + tid * C::WAVES);
+    else *(uint16_t*)at = *(const uint16_t*)(tile_s + tid * C::WAVES);
+  }
 }
 
-template <class T, bool RUNS>
-__global__ __launch_bounds__(512) void dequantize_columns_kernel(QuantParams p) {
+template <class T, bool WIDE, bool RUNS>
+__global__ __launch_bounds__((Columns<T, WIDE>::THREADS)) void dequantize_columns_kernel(QuantParams p) {
   typedef typename Elem<T>::raw raw;
-  constexpr int COL_LANE = col_lane<T>, COL_ROWS = 64 * COL_LANE;
-  __shared__ __attribute__((aligned(16))) uint8_t tile[COL_ROWS * COL_PITCH];
+  typedef Columns<T, WIDE> C;
+  constexpr int LANE = C::LANE;
+  __shared__ __attribute__((aligned(16))) uint8_t tile[C::ROWS * C::PITCH];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t slab = blockIdx.y, row0 = (int64_t)blockIdx.x * COL_ROWS;
+  const int64_t slab = blockIdx.y / C::PARTS, row0 = (int64_t)blockIdx.x * C::ROWS;
+  const int part = blockIdx.y % C::PARTS;
   raw* dst = (raw*)p.dst + (int64_t)blockIdx.z * p.stride_b;
   const uint8_t* codes = p.codes + (int64_t)blockIdx.z * p.codes_b;
   const uint8_t* scales = p.scales + (int64_t)blockIdx.z * p.scales_b;
-  const int64_t k0 = slab * MX_SLAB + wave * 32, left = p.k - k0;
-  const int64_t r = row0 + COL_LANE * lane, rows_left = p.rows - r;
-  float f[COL_LANE];
+  const int64_t k0 = slab * MX_SLAB + part * C::K + wave * 32, left = p.k - k0;
+  const int64_t r = row0 + LANE * lane, rows_left = p.rows - r;
+  float f[LANE];
 #pragma unroll
-  for (int h = 0; h < COL_LANE; ++h) f[h] = h < rows_left ? scale_value(scales[mx_scale_at(r + h, slab, p.slabs) + wave]) : 0.0f;
+  for (int h = 0; h < LANE; ++h) f[h] = h < rows_left ? scale_value(scales[mx_scale_at(r + h, slab, p.slabs) + part * C::WAVES + wave]) : 0.0f;
 #pragma unroll
-  for (int u = 0; u < COL_ROWS * 8 / 512; ++u) {
-    const int i = u * 512 + tid, row = i >> 3, chunk = i & 7;
+  for (int u = 0; u < C::ROWS * C::CHUNKS / C::THREADS; ++u) {
+    const int i = u * C::THREADS + tid, row = i / C::CHUNKS, chunk = i % C::CHUNKS;
     if (row0 + row < p.rows)
-      *(i32x4*)(tile + row * COL_PITCH + chunk * 16) = *(const i32x4*)(codes + ((row0 + row) * p.slabs + slab) * MX_ROWB + chunk * 16);
+      *(i32x4*)(tile + row * C::PITCH + chunk * 16) = *(const i32x4*)(codes + ((row0 + row) * p.slabs + slab) * MX_ROWB + (part * C::CHUNKS + chunk) * 16);
   }
   __syncthreads();
   if (rows_left <= 0 || left <= 0) return;
   raw* d = dst + k0 * p.stride_k + r * p.stride_r;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    float v[COL_LANE][8];
+    float v[LANE][8];
 #pragma unroll
-    for (int h = 0; h < COL_LANE; ++h)                   // (rows past the end: what LDS holds, times 0, and not stored)
-      values8(*(const uint32_t*)(tile + (COL_LANE * lane + h) * COL_PITCH + wave * 16 + q * 4), f[h], v[h]);
+    for (int h = 0; h < LANE; ++h)                       // (rows past the end: what LDS holds, times 0, and not stored)
+      values8(*(const uint32_t*)(tile + (LANE * lane + h) * C::PITCH + wave * 16 + q * 4), f[h], v[h]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = q * 8 + e;
       if (i >= left) continue;
-      if (RUNS && rows_left >= COL_LANE) {
-        RunC<T> t;
+      if (RUNS && rows_left >= LANE) {
+        RunC<T, LANE> t;
 #pragma unroll
-        for (int h = 0; h < COL_LANE; ++h) t.v[h] = Elem<T>::put(v[h][e]);
+        for (int h = 0; h < LANE; ++h) t.v[h] = Elem<T>::put(v[h][e]);
         typedef i32x2 __attribute__((aligned(2))) loose2;
-        i32x2 w;
-        __builtin_memcpy(&w, &t, 8);
-        __builtin_nontemporal_store(w, (loose2*)(d + i * p.stride_k));
+        typedef int __attribute__((aligned(2))) loose1;
+        if constexpr (C::WORDS == 2) {
+          i32x2 w;
+          __builtin_memcpy(&w, &t, 8);
+          __builtin_nontemporal_store(w, (loose2*)(d + i * p.stride_k));
+        } else {
+          int w;
+          __builtin_memcpy(&w, &t, 4);
+          __builtin_nontemporal_store(w, (loose1*)(d + i * p.stride_k));
+        }
       } else {
 #pragma unroll
-        for (int h = 0; h < COL_LANE; ++h)
+        for (int h = 0; h < LANE; ++h)
           if (h < rows_left) d[i * p.stride_k + h * p.stride_r] = Elem<T>::put(v[h][e]);
       }
     }
@@ -346,6 +397,42 @@ __global__ __launch_bounds__(256) void import_kernel(const uint8_t* codes, const
   out_scales[mx_scale_at(row, block >> 3, slabs) + (block & 7)] = left > 0 ? scales[row * sb + block] : 127;
 }
 
+// whether the wide shape has a workgroup for every CU
+template <class T> bool columns_wide(int64_t rows, const QuantParams& p) {
+  typedef Columns<T, true> C;
+  return (rows + C::ROWS - 1) / C::ROWS * p.slabs * p.batch >= 256;
+}
+
+template <class C> bool columns_grid(int64_t rows, const QuantParams& p, dim3* grid) {
+  const int64_t tiles = (rows + C::ROWS - 1) / C::ROWS, parts = p.slabs * C::PARTS;
+  *grid = dim3((unsigned)tiles, (unsigned)parts, (unsigned)p.batch);
+  return tiles <= 0x7fffff && parts <= 65535;
+}
+
+template <class T, bool BACK, bool WIDE> int launch_columns(const QuantParams& p, hipStream_t stream) {
+  typedef Columns<T, WIDE> C;
+  dim3 grid;
+  if (!columns_grid<C>(p.rows, p, &grid)) return TNX_E_UNSUPPORTED;
+  const bool runs = p.stride_r == 1;
+  if (BACK && runs) hipLaunchKernelGGL((dequantize_columns_kernel<T, WIDE, true>), grid, dim3(C::THREADS), 0, stream, p);
+  else if (BACK) hipLaunchKernelGGL((dequantize_columns_kernel<T, WIDE, false>), grid, dim3(C::THREADS), 0, stream, p);
+  else if (runs) hipLaunchKernelGGL((quantize_columns_kernel<T, WIDE, true, false>), grid, dim3(C::THREADS), 0, stream, p);
+  else hipLaunchKernelGGL((quantize_columns_kernel<T, WIDE, false, false>), grid, dim3(C::THREADS), 0, stream, p);
+  return mx_launched();
+}
+
+// both quantisations; p: the matrix's columns, neighbours in memory.  (Whole slabs of the rows too: the padding of the other tensor)
+template <class T, bool WIDE> int launch_both(const QuantParams& p, hipStream_t stream) {
+  typedef Columns<T, WIDE> C;
+  dim3 grid;
+  if (!columns_grid<C>(mx_slabs(p.rows) * MX_SLAB, p, &grid)) return TNX_E_UNSUPPORTED;
+  hipLaunchKernelGGL((quantize_columns_kernel<T, WIDE, true, true>), grid, dim3(C::THREADS), 0, stream, p);
+  return mx_launched();
+}
+template <class T> int launch_both(const QuantParams& p, hipStream_t stream) {
+  return columns_wide<T>(p.rows, p) ? launch_both<T, true>(p, stream) : launch_both<T, false>(p, stream);
+}
+
 template <class T, bool BACK> int launch(const QuantParams& p, hipStream_t stream) {
   if (p.stride_k == 1) {
     const int64_t per_block = 256 * (BACK ? BACK_RUNS : QUANT_RUNS), runs = p.rows * p.slabs * (BACK && sizeof(typename Elem<T>::raw) == 4 ? 64 : 32);
@@ -357,23 +444,7 @@ template <class T, bool BACK> int launch(const QuantParams& p, hipStream_t strea
     else hipLaunchKernelGGL((quantize_rows_kernel<T, false>), grid, dim3(256), 0, stream, p);
     return mx_launched();
   }
-  const int64_t tiles = (p.rows + 64 * col_lane<T> - 1) / (64 * col_lane<T>);
-  if (tiles > 0x7fffff || p.slabs > 65535) return TNX_E_UNSUPPORTED;
-  const dim3 grid((unsigned)tiles, (unsigned)p.slabs, (unsigned)p.batch);
-  const bool runs = p.stride_r == 1;
-  if (BACK && runs) hipLaunchKernelGGL((dequantize_columns_kernel<T, true>), grid, dim3(512), 0, stream, p);
-  else if (BACK) hipLaunchKernelGGL((dequantize_columns_kernel<T, false>), grid, dim3(512), 0, stream, p);
-  else if (runs) hipLaunchKernelGGL((quantize_columns_kernel<T, true, false>), grid, dim3(512), 0, stream, p);
-  else hipLaunchKernelGGL((quantize_columns_kernel<T, false, false>), grid, dim3(512), 0, stream, p);
-  return mx_launched();
-}
-
-// p: the matrix's columns, neighbours in memory
-template <class T> int launch_both(const QuantParams& p, hipStream_t stream) {
-  const int64_t tiles = mx_slabs(p.rows) * (MX_SLAB / (64 * col_lane<T>));         // (whole slabs of the rows too)
-  if (tiles > 0x7fffff || p.slabs > 65535) return TNX_E_UNSUPPORTED;
-  hipLaunchKernelGGL((quantize_columns_kernel<T, true, true>), dim3((unsigned)tiles, (unsigned)p.slabs), dim3(512), 0, stream, p);
-  return mx_launched();
+  return columns_wide<T>(p.rows, p) ? launch_columns<T, BACK, true>(p, stream) : launch_columns<T, BACK, false>(p, stream);
 }
 
 void fill(const tnx_mx_args* a, QuantParams* p) {
