@@ -191,3 +191,13 @@ def test_linear_steps_in_threads_and_streams(device):
             got.append(torch.autograd.grad(tritonix.mx_linear(xs, w), xs, dy)[0])
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+def test_the_example_runs(device, capsys):
+    import os
+    import runpy
+
+    main = runpy.run_path(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "routed_ffn.py"))["main"]
+    worst, largest = main(tokens=300, width=256, inner=128, experts=8, top_k=2, device=device)
+    assert 0 < largest < float("inf") and 0 <= worst < float("inf")
+    assert "rows per expert" in capsys.readouterr().out

@@ -158,3 +158,15 @@ def test_python_refusals():
                  lambda: tritonix.moe_route_backward(torch.ones(4, 3), x, r)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("change,codes,scales,status", [
+    (dict(batch=2), 256, 256, _C.E_INVALID), (dict(rows=-1), 256, 256, _C.E_INVALID), ({}, None, 256, _C.E_INVALID), ({}, 256, None, _C.E_INVALID),
+    ({}, 264, 256, _C.E_INVALID), (dict(data=None), 256, 256, _C.E_INVALID), (dict(codes=None), 256, 256, _C.E_INVALID),
+    (dict(scales=8), 256, 256, _C.E_INVALID), (dict(rows=1 << 23), 256, 256, _C.E_UNSUPPORTED), (dict(k=1 << 23), 256, 256, _C.E_UNSUPPORTED),
+    (dict(dtype=_C.I8), 256, 256, _C.E_UNSUPPORTED), (dict(dtype=_C.I8, stride_row=3, stride_k=5), 256, 256, _C.E_UNSUPPORTED),
+    (dict(rows=0), None, None, _C.OK), (dict(k=0, data=None), None, None, _C.OK)])
+def test_both_quantisations_refuse(change, codes, scales, status):
+    lib = _C.load()
+    assert lib.tnx_mx_quantize_both(ctypes.byref(mx(**change)), codes, scales) == status
+    assert lib.tnx_mx_quantize_both(None, 256, 256) == _C.E_INVALID

@@ -45,17 +45,13 @@ template <int STEP> __device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f3
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, STEP, sa, STEP, sb);
 }
 
-// 16 (4) bytes per lane from a 64-bit address of its own to LDS (base + lane * 16 or 4): see dma16 for M0
+// 16 bytes per lane from a 64-bit address of its own to LDS (base + lane * 16): see dma16 for M0
 __device__ __forceinline__ void dma16_at(const uint8_t* src, uint32_t lds_base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(src) : "memory");
 }
 __device__ __forceinline__ void dma16_from(const uint8_t* sbase, uint32_t voff, uint32_t lds_base) {
   dma16(sbase, voff, __builtin_amdgcn_readfirstlane(lds_base));
 }
-__device__ __forceinline__ void dma4_at(const uint8_t* src, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(src) : "memory");
-}
-
 // Which rows a workgroup has: one matrix, or the tile-th tile of BM rows over all experts, each expert's rows cut on their
 // own.  All 64 lanes take part; the answer is uniform.  expert == experts: rows past the last expert's; false: no such tile.
 struct RowTile { int expert, row0, rows; };
@@ -147,6 +143,11 @@ __device__ __forceinline__ void store_columns(const MxParams& p, int64_t row, in
 // Tiles: BN columns of the output (rows of the weights) x BM rows, WGN x WGM waves, slabs of 256 k in a ring of S LDS buffers
 // filled by direct loads.  Slab s + 1 has to be there, and slab s be read by all, when the last step of slab s
 // begins: one barrier per slab, its wait hidden behind that step's products.  Slab s + S then goes where s was.
+//
+// What bounds them.  8192 x 8192 x 8192 on tiles of 256: 260 us, 4.2 PFLOP/s, on random values, and 190 to 215 on zeros: the board's power limit.  A tile costs
+// 1.8 us a slab and 9 beside its slabs, most of that for the burst of results that all CUs write at the end of a round; so 8192 x 4096 x 4096 74 us, 3.7
+// PFLOP/s.  Products of 16x16x128 instead, twice as many instructions for an issue slot that the reads and loads want as well: 295 us on
+// zeros.  With few rows of many weights it is the weights' bytes: 64 tokens of 8 through 64 experts' 4096 x 1024 matrices 37 us, 3.8 TB/s.
 template <int BN_, int BM_, int WGN, int WGM, int S_> struct MxTile {
   static constexpr int BN = BN_, BM = BM_, NW = WGN * WGM, THREADS = NW * 64, WAVES_N = WGN, S = S_;
   static constexpr int WTN = BN / WGN, WTM = BM / WGM, TN = WTN / 32, TM = WTM / 32;

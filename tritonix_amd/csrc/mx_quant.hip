@@ -142,8 +142,8 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(QuantParams p) {
 
 // Columns: wave b of a workgroup takes the b-th 32 k of its part of a slab, a lane LANE neighbouring rows, which it reads 32 times: a load
 // instruction is one k.  Two shapes.  WIDE: a whole slab by 8 bytes a lane, 256 rows (128 of float32), so that loads are runs of 512 bytes (4 bytes a lane:
-// 8192 x 8192 bfloat16 57 us, with 8 37) and stores whole rows of a slab.  Small, where that makes fewer workgroups than the card has
-// CUs: 64 k by 128 rows (512 x 512 bfloat16, quantised, back and both ways at once: 3.0, 6.0 and 5.8 us, wide 5.9, 10.4 and 11.0;
+// 8192 x 8192 bfloat16 57 us, with 8 37) and stores whole rows of a slab.  Small, where that makes too few workgroups for the card:
+// 64 k by 128 rows (512 x 512 bfloat16, quantised, back and both ways at once: 3.0, 6.0 and 5.8 us, wide 5.9, 10.4 and 11.0;
 // 8192 x 4096: 18.8, 17.4 and 27.3, wide 16.4, 16.2 and 24.3).  Pitch of a row of codes in LDS: 16 bytes more, so that the lanes' 16-byte pieces fall on different banks.
 template <class T, bool WIDE> struct Columns {
   static constexpr int LANE = WIDE ? 8 / sizeof(typename Elem<T>::raw) : 2, WAVES = WIDE ? 8 : 2, THREADS = 64 * WAVES;
@@ -397,10 +397,11 @@ __global__ __launch_bounds__(256) void import_kernel(const uint8_t* codes, const
   out_scales[mx_scale_at(row, block >> 3, slabs) + (block & 7)] = left > 0 ? scales[row * sb + block] : 127;
 }
 
-// whether the wide shape has a workgroup for every CU
+// Whether the wide shape has a workgroup for every CU, or for every other of float32, whose lanes have half the work.  (Quantising, small and wide: bfloat16 3000 x 2001,
+// 96 workgroups, 6.3 and 9.1 us, 4096 x 4096, 256 of them, 10.3 and 10.2; float32 1024 x 2048, 64, 4.1 and 4.8, 2048 x 2048, 128, 5.8 and 5.3.)
 template <class T> bool columns_wide(int64_t rows, const QuantParams& p) {
   typedef Columns<T, true> C;
-  return (rows + C::ROWS - 1) / C::ROWS * p.slabs * p.batch >= 256;
+  return (rows + C::ROWS - 1) / C::ROWS * p.slabs * p.batch >= 64 * C::LANE;
 }
 
 template <class C> bool columns_grid(int64_t rows, const QuantParams& p, dim3* grid) {
