@@ -369,7 +369,8 @@ int tnx_mx_dequantize(const tnx_mx_args* args);
 int tnx_mx_import(const void* codes, const void* scales, int64_t batch, int64_t rows, int64_t k, void* out_codes, void* out_scales,
                   void* stream);
 
-/* one or two rows of a (k up to 30720) may be given as floats in a_data, with a_codes and a_scales null: the kernel quantises them itself */
+/* few rows of a (one with k up to 30720, or up to 16 with at most 16384 elements) may be given as floats in a_data, with a_codes and a_scales null:
+ * the kernel quantises them itself */
 int tnx_mx_gemm_takes_rows(int64_t a_rows, int64_t k);
 
 /* Products of two such tensors, both quantised along the k they are multiplied over: out[m, n] = a[m, k] . b[n, k], 32-bit

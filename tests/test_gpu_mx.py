@@ -124,7 +124,8 @@ def check_product(out, a, b, dtype, k):
 
 
 SIZES = [(1, 16, 32), (1, 1, 1), (3, 17, 31), (16, 64, 256), (17, 100, 300), (33, 130, 600), (64, 64, 64), (65, 257, 513), (100, 300, 1000),
-         (200, 2000, 260), (257, 259, 2049), (1, 4096, 2048), (2, 300, 1000), (1, 130, 30720), (2, 70, 31000), (1, 20, 70000), (40, 50, 9000), (1000, 520, 777), (300, 4100, 512), (2049, 2100, 256), (3600, 3700, 300)]
+         (200, 2000, 260), (257, 259, 2049), (1, 4096, 2048), (2, 300, 1000), (1, 130, 30720), (2, 70, 31000), (1, 20, 70000), (40, 50, 9000), (1000, 520, 777), (300, 4100, 512), (2049, 2100, 256), (3600, 3700, 300),
+         (3, 20, 5000), (4, 70, 4096), (5, 300, 3000), (8, 257, 2048), (9, 33, 1700), (16, 100, 1024), (16, 40, 1025)]
 
 
 @pytest.mark.parametrize("size", SIZES, ids=str)

@@ -77,7 +77,7 @@ def gemm(**kw):
     (dict(offsets=256), _C.E_INVALID), (dict(experts=2, offsets=256, order=256, a_rows=0, top_k=1), _C.E_INVALID),
     (dict(experts=2, offsets=256, order=256, top_k=0), _C.E_INVALID), (dict(experts=2000, offsets=256), _C.E_INVALID),
     (dict(k=1 << 23), _C.E_UNSUPPORTED), (dict(m=0), _C.OK), (dict(n=0), _C.OK), (dict(a_data=256), _C.E_INVALID),
-    (dict(a_data=256, a_codes=None, a_scales=None, a_dtype=_C.BF16), _C.E_UNSUPPORTED),            # four rows
+    (dict(a_data=256, a_codes=None, a_scales=None, a_dtype=_C.BF16, m=17, a_rows=17), _C.E_UNSUPPORTED),
     (dict(a_data=257, a_codes=None, a_scales=None, a_dtype=_C.BF16, m=2, a_rows=2), _C.E_INVALID),
     (dict(a_data=256, a_codes=None, a_scales=None, a_dtype=_C.I8, m=2, a_rows=2), _C.E_UNSUPPORTED),
     (dict(a_data=256, a_codes=None, a_scales=None, a_dtype=_C.BF16, m=2, a_rows=2, k=31000), _C.E_UNSUPPORTED)])
@@ -89,7 +89,8 @@ def test_product_refuses(change, status):
 
 def test_rows_that_the_product_takes_as_floats():
     lib = _C.load()
-    assert [lib.tnx_mx_gemm_takes_rows(m, k) for m, k in ((1, 1), (2, 30720), (2, 30721), (3, 64), (0, 64), (1, 0))] == [1, 1, 0, 0, 0, 0]
+    assert [lib.tnx_mx_gemm_takes_rows(m, k) for m, k in (
+        (1, 1), (1, 30720), (1, 30721), (2, 8192), (2, 8193), (16, 1024), (16, 1025), (17, 64), (0, 64), (1, 0))] == [1, 1, 0, 1, 0, 1, 0, 0, 0, 0]
 
 
 def moe(**kw):

@@ -470,15 +470,19 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
 // a turn's loads are in flight together.  16x16x128 instructions: lane group g (lane / 16) takes the blocks 2 g and 2 g + 1 of a slab, 32 neighbouring
 // bytes and two neighbouring scales.
 //
-// RAW: one or two rows of a, as 16- or 32-bit floats: every workgroup quantises them into LDS while its first weights are on
-// their way (one token: 14336 elements are 28 a thread), which saves a launch of 3 us and its gap.
-constexpr int FEW_WAVES = 8, FEW_RAW_ROWS = 2, FEW_RAW_LDS = 32768;
+// RAW: the rows of a as 16- or 32-bit floats: every workgroup quantises them into LDS while its first weights are on their way, 4096 elements in about
+// 0.5 us, which saves a launch of 3 us and its gap.  In one launch and in two: 4096 x 4096 of 1, 4 and 8 rows 5.1, 6.7 and 8.6 us, 10.1 to 10.2;
+// 14336 x 4096 8.8, 11.1 and 14.2, 11.8 to 11.1; 4096 x 7000 6.9, 9.4 and 12.9, 8.9 to 9.3: up to 16384 elements, or one row.
+constexpr int FEW_WAVES = 8, FEW_RAW_ROWS = 16, FEW_RAW_K = 30720, FEW_RAW_ELEMENTS = 16384;
+// bytes of such a row: 16 more than its codes, so that the rows' chunks fall on different banks, and its scales
+__host__ __device__ inline uint32_t raw_pitch(int64_t slabs) { return (uint32_t)slabs * MX_ROWB + 16; }
+__host__ __device__ inline size_t raw_bytes(int64_t rows, int64_t slabs) { return (size_t)rows * (raw_pitch(slabs) + slabs * MX_SCALEB); }
 
 template <class T> __device__ __forceinline__ void quantize_to_lds(const MxParams& p, uint32_t codes, uint32_t scales, int tid) {
   typedef typename Elem<T>::raw raw;
   const int per_row = p.slabs * 32, items = p.a_rows * per_row;
   for (int i0 = 0; i0 < items; i0 += FEW_WAVES * 64) {                    // (whole blocks of four lanes take each turn)
-    const int i = i0 + tid, row = i >= per_row ? 1 : 0, at = i - row * per_row;
+    const int i = i0 + tid, row = (int)((uint32_t)i / (uint32_t)per_row), at = i - row * per_row;
     if (i >= items) continue;
     const int left = p.k - at * 8;
     const raw* src = (const raw*)p.a + (int64_t)row * p.lda + (int64_t)at * 8;
@@ -498,7 +502,7 @@ template <class T> __device__ __forceinline__ void quantize_to_lds(const MxParam
     const uint32_t s = scale_byte(top_bits<T>((raw)quad_max(top)), &factor);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = scaled(Elem<T>::get(x.v[e]), factor);
-    *TNX_LDS(uint32_t, codes + i * 4) = codes8(v);
+    *TNX_LDS(uint32_t, codes + row * raw_pitch(p.slabs) + at * 4) = codes8(v);
     if ((at & 3) == 0) *TNX_LDS(uint8_t, scales + (i >> 2)) = (uint8_t)s;      // (a block of padding: codes 0, any finite scale)
   }
 }
@@ -520,7 +524,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
   }
   const int row = lane & 15, g = lane >> 4;
   const bool empty = EXPERTS && rt.expert == p.experts;
-  const uint32_t raw_scales = lds0 + FEW_RAW_ROWS * p.slabs * MX_ROWB;
+  const uint32_t raw_scales = lds0 + p.a_rows * raw_pitch(p.slabs);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 
   constexpr int DEPTH = 8;                               // slabs of a turn
@@ -564,10 +568,10 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
           int sa = 0x7f7f;
           if (have) {
             if (RAW) {
-              const uint32_t at = (uint32_t)(src * p.slabs + s);
-              fa0 = *TNX_LDS(i32x4, lds0 + at * MX_ROWB + 32 * g);
-              fa1 = *TNX_LDS(i32x4, lds0 + at * MX_ROWB + 32 * g + 16);
-              sa = *TNX_LDS(uint16_t, raw_scales + at * MX_SCALEB + 2 * g);
+              const uint32_t at = lds0 + src * raw_pitch(p.slabs) + (uint32_t)s * MX_ROWB + 32 * g;
+              fa0 = *TNX_LDS(i32x4, at);
+              fa1 = *TNX_LDS(i32x4, at + 16);
+              sa = *TNX_LDS(uint16_t, raw_scales + (uint32_t)(src * p.slabs + s) * MX_SCALEB + 2 * g);
             } else {
               fa0 = *(const i32x4*)(a_at + s * MX_ROWB);
               fa1 = *(const i32x4*)(a_at + s * MX_ROWB + 16);
@@ -620,7 +624,7 @@ template <bool EXPERTS, bool RAW> int launch_few(MxParams p, int64_t row_tiles, 
   while (p.wk_log < 3 && (2 << p.wk_log) <= p.slabs && (groups * row_tiles << p.wk_log) < 2048) ++p.wk_log;
   const int64_t per = FEW_WAVES >> p.wk_log;
   size_t lds = p.wk_log ? (size_t)FEW_WAVES * 1024 : 0;
-  const size_t raw = RAW ? (size_t)FEW_RAW_ROWS * p.slabs * (MX_ROWB + MX_SCALEB) : 0;
+  const size_t raw = RAW ? raw_bytes(p.a_rows, p.slabs) : 0;
   if (raw > lds) lds = raw;
   hipLaunchKernelGGL((mx_few_kernel<EXPERTS, RAW>), dim3((unsigned)((groups + per - 1) / per), (unsigned)row_tiles), dim3(FEW_WAVES * 64), lds, stream, p);
   return mx_launched();
@@ -661,7 +665,9 @@ template <bool EXPERTS> int launch(const MxParams& p, bool raw, hipStream_t stre
   return launch_tile<MxTile<128, 128, 2, 2, 2>, EXPERTS>(p, most(128), stream);
 }
 
-bool takes_rows(int64_t a_rows, int64_t k) { return a_rows <= FEW_RAW_ROWS && FEW_RAW_ROWS * mx_slabs(k) * (MX_ROWB + MX_SCALEB) <= FEW_RAW_LDS; }
+bool takes_rows(int64_t a_rows, int64_t k) {
+  return a_rows == 1 ? k <= FEW_RAW_K : a_rows <= FEW_RAW_ROWS && a_rows * k <= FEW_RAW_ELEMENTS;
+}
 
 }  // namespace
 

@@ -1,7 +1,7 @@
 // Quantisation to microscaled 4-bit floats and back.
 //
 // A block of 32 elements with largest magnitude a gets the scale 2^e, e = floor(log2 a) - 2 (the exponent of 6, the
-// largest 4-bit value, is 2), clamped to [-127, 127], and each element x the 4-bit float nearest to x / 2^e, ties to the even
+// largest 4-bit value, is 2) but at least -127, and each element x the 4-bit float nearest to x / 2^e, ties to the even
 // code, magnitudes above 6 to 6.  The division is a multiplication by 2^-e, exact in binary32 but for results below
 // its smallest normal number, which round to code 0 either way.  A block that holds an infinity or a NaN gets the NaN scale.
 //

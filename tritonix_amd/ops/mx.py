@@ -248,8 +248,8 @@ def operand(name: str, side: str, x, dim: int) -> MXTensor:
 
 
 def takes_rows(x) -> bool:
-    """Whether a product takes these rows as they are: one or two rows of floats are quantised by the kernel itself."""
-    return (not isinstance(x, MXTensor) and 0 < x.shape[0] <= 2 and (x.stride(1) == 1 or x.shape[1] == 1) and x.dtype in _DTYPES
+    """Whether a product takes these rows as they are: a few rows of floats are quantised by the kernel itself."""
+    return (not isinstance(x, MXTensor) and 0 < x.shape[0] <= 16 and (x.stride(1) == 1 or x.shape[1] == 1) and x.dtype in _DTYPES
             and bool(_C.load().tnx_mx_gemm_takes_rows(x.shape[0], x.shape[1])))
 
 
