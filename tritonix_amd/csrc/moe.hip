@@ -201,7 +201,7 @@ __device__ __forceinline__ void plan_alone(const PlanParams& p, const int* ids, 
 
 // Scores and choice.  L lanes share a token and hold EPL experts each.  The choice is top_k rounds of a maximum over all keys, then the lowest expert that
 // has it.  Bound by its instructions: eight lanes of sixteen experts where there are tokens enough to fill the card, a wave per token
-// where there are few and a token's own time counts.  65536 tokens, 8 of 128 experts: 18.4 us; with a search through all sixteen registers
+// where there are few and a token's own time counts.  65536 tokens, 8 of 128 experts: 16.8 us; with a search through all sixteen registers
 // each round 22, with the lanes' keys sorted first as doubles that hold key and expert 84 (a compare is one instruction, but not a fast one).
 // FULL: with a bias or groups.  smem: a workgroup's own.
 template <int L, int EPL, bool FULL>
@@ -382,14 +382,19 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int tid, int6
   }
 }
 
+// The block of a workgroup.  Neighbours are on one XCD: an expert's counts and places in neighbouring blocks are neighbours in memory, a few bytes from each, and
+// meet in its L2.  (65536 x 8 of 128 experts, spread over the XCDs as they come: the choice 18.3 us instead of 16.8, places 8.6 instead of 5.6.)
+__device__ __forceinline__ int plan_block() { return xcd_remap(blockIdx.x, gridDim.x, 8); }
+
 // What a workgroup's tokens chose, for the plan: ALONE places the pairs of the only workgroup, otherwise each counts its own per expert.
 template <int L, int EPL, bool FULL, bool ALONE>
 __global__ __launch_bounds__(256) void route_kernel(RouteParams p, PlanParams q) {
   extern __shared__ __attribute__((aligned(16))) uint8_t moe_smem[];
   constexpr int KR = (TNX_MOE_MAX_TOP_K + L - 1) / L;
   const int tid = threadIdx.x, j = tid % L, slot = tid / L;
+  const int block = plan_block();
   int id[KR];
-  route_tokens<L, EPL, FULL>(p, tid, (int64_t)blockIdx.x * (256 / L), moe_smem, id);
+  route_tokens<L, EPL, FULL>(p, tid, (int64_t)block * (256 / L), moe_smem, id);
   if (FULL || EPL > 4) __syncthreads();    // (the keys lay where the plan's memory is)
   if (ALONE) {
     int* ids = (int*)moe_smem;
@@ -404,20 +409,31 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p, PlanParams q)
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < KR; ++r)
-      if ((int64_t)blockIdx.x * (256 / L) + slot < p.tokens && r * L + j < p.k && id[r] >= 0) bits.mark(id[r], slot * p.k + r * L + j);
+      if ((int64_t)block * (256 / L) + slot < p.tokens && r * L + j < p.k && id[r] >= 0) bits.mark(id[r], slot * p.k + r * L + j);
     __syncthreads();
-    for (int e = tid; e < q.e; e += 256) q.counts[q.count_at(e, blockIdx.x)] = bits.count(e);
+    for (int e = tid; e < q.e; e += 256) q.counts[q.count_at(e, block)] = bits.count(e);
   }
 }
 
-// the experts of a block's pairs into bits; anything outside the range is an empty slot
-__device__ __forceinline__ void mark_pairs(const PlanParams& p, const PairBits& bits, int tid) {
+// a thread's pairs of a block, tid, tid + 256, ..: their experts, -1 where there is none.  Anything outside the range is an empty slot.
+constexpr int PLAN_BLOCK = 1024;
+__device__ __forceinline__ void load_pairs(const PlanParams& p, int block, int tid, int (&mine)[PLAN_BLOCK / 256]) {
+  const int64_t first = (int64_t)block * p.block;
+#pragma unroll
+  for (int u = 0; u < PLAN_BLOCK / 256; ++u) {
+    const int i = tid + u * 256;
+    mine[u] = -1;
+    if (i < p.block && first + i < p.pairs) mine[u] = p.experts[first + i];
+  }
+}
+// into bits
+__device__ __forceinline__ void mark_pairs(const PlanParams& p, const PairBits& bits, int tid, int (&mine)[PLAN_BLOCK / 256]) {
   bits.clear(p.e, tid);
   __syncthreads();
-  const int64_t first = (int64_t)blockIdx.x * p.block;
-  for (int i = tid; i < p.block && first + i < p.pairs; i += 256) {
-    const int e = p.experts[first + i];
-    if (e >= 0 && e < p.e) bits.mark(e, i);
+#pragma unroll
+  for (int u = 0; u < PLAN_BLOCK / 256; ++u) {
+    if (mine[u] >= p.e) mine[u] = -1;
+    if (mine[u] >= 0) bits.mark(mine[u], tid + u * 256);
   }
   __syncthreads();
 }
@@ -437,8 +453,11 @@ __global__ __launch_bounds__(256) void plan_alone_kernel(PlanParams p) {
 __global__ __launch_bounds__(256) void plan_count_kernel(PlanParams p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t moe_smem[];
   const PairBits bits{(unsigned long long*)moe_smem, p.words};
-  mark_pairs(p, bits, threadIdx.x);
-  for (int e = threadIdx.x; e < p.e; e += 256) p.counts[p.count_at(e, blockIdx.x)] = bits.count(e);
+  const int block = plan_block();
+  int mine[PLAN_BLOCK / 256];
+  load_pairs(p, block, threadIdx.x, mine);
+  mark_pairs(p, bits, threadIdx.x, mine);
+  for (int e = threadIdx.x; e < p.e; e += 256) p.counts[p.count_at(e, block)] = bits.count(e);
 }
 
 // counts[e][block] -> pairs of e in the blocks before it; a workgroup per expert, eight neighbouring blocks a thread (65536 tokens of 8 pairs: 2048 blocks,
@@ -485,12 +504,14 @@ __global__ __launch_bounds__(256) void plan_place_kernel(PlanParams p) {
   const PairBits bits{(unsigned long long*)moe_smem, p.words};
   int* base = (int*)(moe_smem + (size_t)p.e * p.words * 8);
   int* own = base + p.e;                   // pairs of the expert in the blocks before this one
-  const int tid = threadIdx.x;
-  const int64_t first = (int64_t)blockIdx.x * p.block;
+  const int tid = threadIdx.x, block = plan_block();
+  const int64_t first = (int64_t)block * p.block;
+  int mine[PLAN_BLOCK / 256];
+  load_pairs(p, block, tid, mine);                // (on their way together with the counts)
   if (SUMMED) {
     for (int e = tid; e < p.e; e += 256) {
       base[e] = p.totals[e];
-      own[e] = p.counts[(int64_t)e * p.blocks + blockIdx.x];
+      own[e] = p.counts[p.count_at(e, block)];
     }
   } else {
     // Neighbouring threads have neighbouring experts, and where there are threads left over, several share an expert's blocks.  129 blocks of 60
@@ -512,25 +533,25 @@ __global__ __launch_bounds__(256) void plan_place_kernel(PlanParams p) {
         for (int u = 0; u < 16; ++u) {
           const int b = b0 + u * shares;
           all += b < p.blocks ? c[u] : 0;
-          before += b < (int)blockIdx.x ? c[u] : 0;
+          before += b < block ? c[u] : 0;
         }
       }
       atomicAdd(&base[e], all);                            // (in LDS, and of integers: any order gives the same)
       atomicAdd(&own[e], before);
     }
   }
-  mark_pairs(p, bits, tid);
+  mark_pairs(p, bits, tid, mine);
   const int total = scan_experts(base, p.e, tid);
-  if (blockIdx.x == 0)
+  if (block == 0)
     for (int e = tid; e <= p.e; e += 256) p.offsets[e] = e < p.e ? base[e] : total;
-  for (int i = tid; i < p.block && first + i < p.pairs; i += 256) {
+#pragma unroll
+  for (int u = 0; u < PLAN_BLOCK / 256; ++u) {
+    const int i = tid + u * 256, e = mine[u];
     const int64_t pair = first + i;
-    const int e = p.experts[pair];
-    if (e >= 0 && e < p.e) {
-      const int at = base[e] + own[e] + bits.rank(e, i);
-      p.order[at] = (int32_t)pair;
-      p.rows[pair] = at;
-    } else p.rows[pair] = -1;
+    if (i >= p.block || pair >= p.pairs) break;
+    const int at = e >= 0 ? base[e] + own[e] + bits.rank(e, i) : -1;
+    if (e >= 0) p.order[at] = (int32_t)pair;
+    p.rows[pair] = at;
     if (pair >= total) p.order[pair] = -1;
   }
 }
@@ -704,6 +725,7 @@ void plan_shape(PlanParams* q, int64_t tokens, int k, int e) {
   q->e = e;
   q->fused = lanes < 64 || tokens <= 1024;
   q->block = q->fused ? 256 / lanes * k : 512;
+  static_assert(256 / 8 * TNX_MOE_MAX_TOP_K <= PLAN_BLOCK && 512 <= PLAN_BLOCK, "a thread's pairs");
   q->blocks = (int)((q->pairs + q->block - 1) / q->block);
   q->words = (q->block + 63) / 64;
   q->summed = q->blocks > SUM_BLOCKS || (int64_t)q->blocks * q->e > SUM_LOADS * 256;

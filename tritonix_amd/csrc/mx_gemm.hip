@@ -638,7 +638,7 @@ double tiles_us(int64_t tiles, int slots, double t, double t_few, double o, int6
 }
 
 // The tile with the lowest estimate.  Fitted to products of 8 to 4096 rows with 256 x 1024 to 14336 x 14336 weights, and of 4 to 4096 tokens with 8 to
-// 128 experts.  What it decides, measured in us: 1024 x 4096 x 4096 tiles of 64 18.5, of 128 15.6 (one on a CU, four buffers) and 16.0 (two on a
+// 128 experts.  What it decides, measured in us: 1024 x 4096 x 4096 tiles of 64 18.5, of 128 15.1 (one on a CU, four buffers, eight waves; 15.6 with four) and 16.0 (two on a
 // CU, two buffers), of 256 25.6; 2048 x 14336 x 4096 117, 88, 73 and 66; 512 x 4096 x 14336 27, 30, 46 and 69; 64 tokens through
 // the up-projections of 64 experts (4096 -> 1024) 49, 56, 49 and 56, through the down-projections 44, 55, 37 and 44.
 template <bool EXPERTS> int launch(const MxParams& p, bool raw, hipStream_t stream) {
@@ -661,7 +661,7 @@ template <bool EXPERTS> int launch(const MxParams& p, bool raw, hipStream_t stre
   if (!EXPERTS && p.m <= 16 && us_few < us64) return launch_few<EXPERTS, false>(p, most(16), stream);
   if (us256 <= us128 && us256 <= us128_deep && us256 <= us64) return launch_tile<MxTile<256, 256, 4, 2, 2>, EXPERTS>(p, most(256), stream);
   if (us64 <= us128 && us64 <= us128_deep) return launch_tile<MxTile<64, 64, 2, 2, 4>, EXPERTS>(p, most(64), stream);
-  if (us128_deep < us128) return launch_tile<MxTile<128, 128, 2, 2, 4>, EXPERTS>(p, most(128), stream);
+  if (us128_deep < us128) return launch_tile<MxTile<128, 128, 4, 2, 4>, EXPERTS>(p, most(128), stream);
   return launch_tile<MxTile<128, 128, 2, 2, 2>, EXPERTS>(p, most(128), stream);
 }
 
