@@ -617,11 +617,16 @@ template <class C, bool EXPERTS> int launch_tile(MxParams p, int64_t row_tiles, 
   return p.out_dtype == DT_F16 ? gated(TypeTag<OutF16>()) : gated(TypeTag<OutF32>());
 }
 
+// as few parts of k (log2) as give every SIMD two waves: a part less is a sum less, and its wave has more loads in flight
+int few_parts(int64_t outputs, int64_t slabs) {
+  int log = 0;
+  while (log < 3 && (2 << log) <= slabs && (outputs << log) < 2048) ++log;
+  return log;
+}
+
 template <bool EXPERTS, bool RAW> int launch_few(MxParams p, int64_t row_tiles, hipStream_t stream) {
-  // as few parts of k as give every SIMD two waves: a part less is a sum less, and its wave has more loads in flight
   const int64_t groups = (p.n + 15) / 16;
-  p.wk_log = 0;
-  while (p.wk_log < 3 && (2 << p.wk_log) <= p.slabs && (groups * row_tiles << p.wk_log) < 2048) ++p.wk_log;
+  p.wk_log = few_parts(groups * row_tiles, p.slabs);
   const int64_t per = FEW_WAVES >> p.wk_log;
   size_t lds = p.wk_log ? (size_t)FEW_WAVES * 1024 : 0;
   const size_t raw = RAW ? raw_bytes(p.a_rows, p.slabs) : 0;
@@ -655,10 +660,15 @@ template <bool EXPERTS> int launch(const MxParams& p, bool raw, hipStream_t stre
   const double us128 = tiles_us(expect(128) * cols(128), 512, 1.1, 0.76, 4.5, p.slabs);
   const double us128_deep = tiles_us(expect(128) * cols(128), 256, 0.5, 0.45, 6.0, p.slabs);
   const double us256 = tiles_us(expect(256) * cols(256), 256, 1.77, 1.15, 9.0, p.slabs);
-  // Up to 16 rows: the streaming kernel brings 3.3 MB a us and has a short way to the first load.  4 x 4096 x 8192: 9.6 us, tiles of 64 13.0; 4 x
-  // 14336 x 14336: 29 and 24.5.
-  const double us_few = 5.0 + (double)p.n * p.slabs * (MX_ROWB + MX_SCALEB) / 3.3e6;
-  if (!EXPERTS && p.m <= 16 && us_few < us64) return launch_few<EXPERTS, false>(p, most(16), stream);
+  if constexpr (!EXPERTS) {
+    // The streaming kernel: a slab of a workgroup's eight waves is 35 kB of weights and rows, and a CU brings that in 1 us, however few of
+    // them are busy.  So it is for few rows, or few columns, and it shares k out.  40 x 64 x 9630: 7.7 us, tiles of 64 13.7; 8 x 4096 x 4096 4.6 and 7.4;
+    // 64 x 1024 x 4096 5.0 and 7.8, 128 rows 7.1 and 7.4; 256 x 256 x 16384 12 and 23; 48 x 4096 x 4096 11.6 and 7.6.
+    const int64_t outputs = cols(16) * most(16);
+    const int log = few_parts(outputs, p.slabs);
+    const double us_few = 2.7 + (double)(((outputs << log) + 256 * FEW_WAVES - 1) / (256 * FEW_WAVES) * ((p.slabs + (1 << log) - 1) >> log));
+    if (us_few < us64 && us_few < us128 && us_few < us128_deep && us_few < us256 && most(16) <= 65535) return launch_few<false, false>(p, most(16), stream);
+  }
   if (us256 <= us128 && us256 <= us128_deep && us256 <= us64) return launch_tile<MxTile<256, 256, 4, 2, 2>, EXPERTS>(p, most(256), stream);
   if (us64 <= us128 && us64 <= us128_deep) return launch_tile<MxTile<64, 64, 2, 2, 4>, EXPERTS>(p, most(64), stream);
   if (us128_deep < us128) return launch_tile<MxTile<128, 128, 4, 2, 4>, EXPERTS>(p, most(128), stream);
