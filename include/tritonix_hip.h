@@ -397,7 +397,12 @@ typedef struct tnx_mx_gemm_args {
   int32_t a_dtype;           /* of a_data: TNX_F16, TNX_BF16 or TNX_F32 */
   int32_t reserved;
   void* stream;
+  void* workspace;           /* tnx_mx_gemm_workspace_bytes, 16-byte aligned, no initialisation; null: k is not cut */
+  size_t workspace_bytes;
 } tnx_mx_gemm_args;
+
+/* scratch that a product is faster with (few tiles of many slabs: k is cut in parts), or 0.  Host arithmetic on m, n and k */
+size_t tnx_mx_gemm_workspace_bytes(const tnx_mx_gemm_args* args);
 
 int tnx_mx_gemm(const tnx_mx_gemm_args* args);
 

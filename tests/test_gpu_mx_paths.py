@@ -61,6 +61,31 @@ def test_products(device, monkeypatch, m, wide):
     both(monkeypatch, lambda: (tritonix.mx_matmul(x, w), tritonix.mx_glu(x, w), tritonix.mx_glu(x, w, "none")), ["mx_product"] * 3)
 
 
+@pytest.mark.parametrize("size", [(40, 500, 14336), (100, 1100, 14336), (130, 2050, 9000), (200, 1030, 17000)], ids=str)
+@pytest.mark.parametrize("epilogue", ["plain", "silu"])
+def test_products_with_k_in_parts(device, monkeypatch, size, epilogue):
+    """The same sums, added up in another order: against the product without the scratch, and the native path against the interpreter's."""
+    m, n, k = size
+    a, w = mx.mx_quantize(rand(device, m, k)), mx.mx_quantize(rand(device, k, n, seed=1), dim=0)
+    call = (lambda x: tritonix.mx_matmul(x, w, out_dtype=torch.float32)) if epilogue == "plain" else (lambda x: tritonix.mx_glu(x, w, out_dtype=torch.float32))
+    lib = _C.load()
+    got = call(a)
+    out = torch.empty_like(got)
+    g = mx.gemm_args(a, w, out, _C.EPI_NONE if epilogue == "plain" else _C.EPI_GLU_SILU)
+    g.stream = torch.cuda.current_stream().cuda_stream
+    assert lib.tnx_mx_gemm_workspace_bytes(ctypes.byref(g)) > 0
+    assert lib.tnx_mx_gemm(ctypes.byref(g)) == _C.OK            # without scratch
+    product = tritonix.mx_matmul(a, w, out_dtype=torch.float32)
+    # sums of k terms of magnitude up to the largest entry's scale, rounded in two orders of 2^-24 each; the gate's slope is at most 1.1
+    scale = (tritonix.mx_dequantize(a, torch.float32).abs() @ tritonix.mx_dequantize(w, torch.float32).abs()).max()
+    bound = float(scale) * (k // 64 + 16) * 2.0 ** -23
+    bound = bound if epilogue == "plain" else 2.2 * bound * float(product.abs().max())
+    assert float((got - out).abs().max()) <= bound
+    if epilogue == "plain":
+        x = rand(device, m, k)
+        both(monkeypatch, lambda: (tritonix.mx_matmul(x, w),), ["mx_product"])
+
+
 def test_linear(device, monkeypatch):
     x, w, dy = rand(device, 65, 130).requires_grad_(True), rand(device, 130, 66, seed=1).requires_grad_(True), rand(device, 65, 66, seed=2)
 

@@ -171,3 +171,16 @@ def test_both_quantisations_refuse(change, codes, scales, status):
     lib = _C.load()
     assert lib.tnx_mx_quantize_both(ctypes.byref(mx(**change)), codes, scales) == status
     assert lib.tnx_mx_quantize_both(None, 256, 256) == _C.E_INVALID
+
+
+def test_workspace_of_a_product():
+    lib = _C.load()
+
+    def size(**kw):
+        return lib.tnx_mx_gemm_workspace_bytes(ctypes.byref(gemm(**kw)))
+    assert size() == size(m=8192, n=8192, k=8192) == size(m=0) == size(n=0) == size(m=100, n=4096, k=512) == 0
+    bytes_of = size(m=100, n=4099, k=14336)                     # parts of 100 x 4100 floats
+    assert bytes_of % 1640000 == 0 and 2 <= bytes_of // 1640000 <= 8
+    assert size(m=100, n=4099, k=14336, experts=4, offsets=256) == 0 and size(m=1, n=4096, k=14336, a_data=256) == 0
+    assert lib.tnx_mx_gemm_workspace_bytes(None) == 0
+    assert lib.tnx_mx_gemm(ctypes.byref(gemm(workspace=264, workspace_bytes=1))) == _C.E_INVALID

@@ -361,6 +361,7 @@ struct OpEntries {
   int (*dequantize)(const tnx_mx_args*);
   int (*takes_rows)(int64_t, int64_t);
   int (*gemm)(const tnx_mx_gemm_args*);
+  size_t (*gemm_workspace)(const tnx_mx_gemm_args*);
   size_t (*workspace_bytes)(int64_t, int32_t, int32_t);
   int (*route)(const tnx_moe_args*);
   int (*backward)(const tnx_moe_args*);
@@ -453,6 +454,16 @@ QuantisedBoth quantised(const at::Tensor& x, bool last, bool first, c10::DeviceI
   uint8_t* other = (uint8_t*)b.first.buffer.data_ptr();
   b.last.status = b.first.status = ops.quantize_both(&a, other, other + b.first.code_bytes);
   return b;
+}
+
+// the product, with the scratch that it is faster with
+int multiply(tnx_mx_gemm_args* g, c10::DeviceIndex device) {
+  const size_t bytes = ops.gemm_workspace(g);
+  if (!bytes) return ops.gemm(g);
+  const at::Tensor scratch = fresh({(int64_t)bytes}, at::kByte, device);
+  g->workspace = scratch.data_ptr();
+  g->workspace_bytes = bytes;
+  return ops.gemm(g);
 }
 
 // mx_quantize(x, along its last dimension) -> (buffer, bytes of codes), or None
@@ -566,7 +577,7 @@ PyObject* mx_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (rows && g.m * g.n * 4 <= join_bytes) g.out_dtype = TNX_F32;
       out = fresh({g.m, g.stride_out}, type_of(g.out_dtype), device);
       g.out = out.data_ptr();
-      status = q.status != TNX_OK ? q.status : ops.gemm(&g);
+      status = q.status != TNX_OK ? q.status : multiply(&g, device);
       if (status == TNX_OK && rows) {
         joined = fresh({rows->size(0), g.n}, a->scalar_type(), device);
         status = ops.combine(out.data_ptr(), (const int32_t*)rows->data_ptr(), (const float*)weights->data_ptr(), joined.data_ptr(), rows->size(0),
@@ -595,7 +606,7 @@ Multiplied multiplied(const Quantised& a, const Quantised& b, int64_t m, int64_t
   g.m = g.a_rows = m; g.n = n; g.k = k; g.stride_out = n;
   g.out_dtype = float_code(type);
   g.stream = stream;
-  r.status = ops.gemm(&g);
+  r.status = multiply(&g, device);
   return r;
 }
 

@@ -28,6 +28,7 @@ struct MxParams {
   int out_dtype, epi;
   int64_t lda;                             // few rows as floats: their stride, type and k; parts of k (log2)
   int a_dtype, k, wk_log;
+  int part_slabs;                          // k cut in parts of so many slabs, an even number
   bool stream_b;                           // the weights are read by one tile of rows each: past the caches (tiles of up to 128 rows)
 };
 
@@ -223,7 +224,8 @@ __device__ __forceinline__ void store_product(const f32x16& v, uint8_t* out, int
   }
 }
 
-template <class C, bool EXPERTS, class O, bool GLU>
+// PARTS: blockIdx.y is a part of k, whose sums go to a matrix of their own in 32 bits; join_kernel adds them up.
+template <class C, bool EXPERTS, class O, bool GLU, bool PARTS>
 __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_kernel(MxParams p) {
   constexpr int BN = C::BN, BM = C::BM, NW = C::NW, S = C::S;
   extern __shared__ __attribute__((aligned(1024))) uint8_t mx_smem[];
@@ -253,7 +255,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
     for (int i = tid; i < rt.rows * nc; i += C::THREADS) store_out<float>(p.out, (int64_t)(rt.row0 + i / nc) * p.ldo + c0 + i % nc, 0.0f, p.out_dtype);
     return;
   }
-  const uint8_t* b = uniform_ptr(p.b + (int64_t)rt.expert * p.b_expert + (int64_t)n0 * p.slabs * MX_ROWB);
+  const int slab0 = PARTS ? (int)blockIdx.y * p.part_slabs : 0, slabs = PARTS && p.slabs - slab0 > p.part_slabs ? p.part_slabs : p.slabs - slab0;
+  const uint8_t* b = uniform_ptr(p.b + (int64_t)rt.expert * p.b_expert + ((int64_t)n0 * p.slabs + slab0) * MX_ROWB);
   const uint8_t* bs = uniform_ptr(p.bs + (int64_t)rt.expert * p.bs_expert + (int64_t)(n0 >> 5) * ((p.slabs + 1) >> 1) * 512);
 
   // Direct loads.  Instruction q of wave w fills rows 8 (NW q + w) .. + 7 of a side, lane l the 16-byte place l % 8 of row l / 8,
@@ -275,7 +278,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
       a_at[q] = p.a + (int64_t)source_row(p, rt.row0 + (row < rt.rows ? row : rt.rows - 1)) * p.slabs * MX_ROWB + chunk * 16;
     }
   } else {
-    a = uniform_ptr(p.a + (int64_t)rt.row0 * p.slabs * MX_ROWB);
+    a = uniform_ptr(p.a + ((int64_t)rt.row0 * p.slabs + slab0) * MX_ROWB);
 #pragma unroll
     for (int q = 0; q < C::A_OPS; ++q) {
       const int row = 8 * (NW * q + wave) + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
@@ -288,10 +291,10 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
   const uint8_t* s_at;
   {
     const int row = 64 * wave + lane, ar = row - BN;
-    if (64 * wave < BN) s_at = bs + mx_scale_at(row < ncols ? row : ncols - 1, 0, p.slabs);
+    if (64 * wave < BN) s_at = bs + mx_scale_at(row < ncols ? row : ncols - 1, slab0, p.slabs);
     else {
       const int r = rt.row0 + (ar < rt.rows ? ar : rt.rows - 1);
-      s_at = p.as + mx_scale_at(EXPERTS ? source_row(p, r) : r, 0, p.slabs);
+      s_at = p.as + mx_scale_at(EXPERTS ? source_row(p, r) : r, slab0, p.slabs);
     }
   }
 
@@ -398,7 +401,6 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
     }
   };
 
-  const int slabs = p.slabs;
   static_assert((S - 2) * (OPS - 1) + FIRST_OPS < 64, "the counter of loads in flight");
 #pragma unroll
   for (int t = 0; t < S - 1; ++t)
@@ -449,7 +451,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
   // left them until their turn: without the empty asm all 256 are copied out at once, to scratch memory for the most part.
   constexpr int ES = sizeof(typename O::raw), W = GLU ? 16 : 32;          // output columns of a product
   const int left_cols = GLU ? (ncols - wn) >> 1 : ncols - wn;
-  uint8_t* out = p.out + ((int64_t)(rt.row0 + wm) * p.ldo + (GLU ? (n0 + wn) >> 1 : n0 + wn)) * ES;
+  uint8_t* out = p.out + ((PARTS ? (int64_t)blockIdx.y * p.m * p.ldo : 0) + (int64_t)(rt.row0 + wm) * p.ldo + (GLU ? (n0 + wn) >> 1 : n0 + wn)) * ES;
   const bool whole = rt.rows - wm >= C::WTM && ncols - wn >= C::WTN;
 #pragma unroll
   for (int j = 0; j < C::TM; ++j)
@@ -600,16 +602,51 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(MxParams p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-template <class C, bool EXPERTS> int launch_tile(MxParams p, int64_t row_tiles, hipStream_t stream) {
+int parts_pitch(int64_t n) { return (int)((n + 3) & ~(int64_t)3); }
+// slabs of a part: even, since two slabs' scales lie together
+int parts_slabs(int slabs, int parts) { return ((slabs + parts - 1) / parts + 1) & ~1; }
+constexpr size_t MAX_PARTS_BYTES = (size_t)64 << 20;
+size_t parts_bytes(int64_t m, int64_t n, int parts) { return parts > 1 ? (size_t)parts * m * parts_pitch(n) * 4 : 0; }
+
+// The parts' sums, in their order, through the epilogue: four columns a thread.  sums: [parts][m][pitch]
+__global__ __launch_bounds__(256) void join_kernel(MxParams p, const float* sums, int parts, int pitch) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / (pitch >> 2);
+  if (row >= p.m) return;
+  const int col = (int)(i - row * (pitch >> 2)) * 4;
+  const f32x4* at = (const f32x4*)(sums + row * pitch + col);
+  const int64_t next = (int64_t)p.m * pitch >> 2;
+  f32x4 v = *at;
+  for (int s = 1; s < parts; ++s) v += at[s * next];
+  store_columns(p, row, col, p.n, v);
+}
+
+template <class C, bool EXPERTS> int launch_tile(MxParams p, int64_t row_tiles, hipStream_t stream, int parts = 1, void* sums = nullptr) {
   p.tiles_n = (p.n + C::BN - 1) / C::BN;
   p.tiles_m = (p.m + C::BM - 1) / C::BM;
   // 64 tokens through 64 experts' up-projections, weights not in the caches: 62 us, so 55; with 1024 tokens, two tiles an expert, 99 and 104
   p.stream_b = EXPERTS ? (int64_t)p.m * 2 <= (int64_t)p.experts * C::BM : p.tiles_m == 1;
   const int64_t grid = row_tiles * p.tiles_n;
   if (grid > 0x7fffffff) return TNX_E_UNSUPPORTED;
+  if constexpr (!EXPERTS && C::S == 4) {
+    if (parts > 1) {
+      const int pitch = parts_pitch(p.n);
+      MxParams q = p;
+      q.out = (uint8_t*)sums;
+      q.ldo = pitch;
+      q.part_slabs = parts_slabs(p.slabs, parts);
+      parts = (p.slabs + q.part_slabs - 1) / q.part_slabs;                  // (rounded up to even, fewer may do)
+      hipLaunchKernelGGL((mx_tile_kernel<C, false, OutF32, false, true>), dim3((unsigned)grid, (unsigned)parts), dim3(C::THREADS), C::LDS, stream, q);
+      const int status = mx_launched();
+      if (status != TNX_OK) return status;
+      const int64_t items = (int64_t)p.m * (pitch >> 2);
+      hipLaunchKernelGGL(join_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, stream, p, (const float*)sums, parts, pitch);
+      return mx_launched();
+    }
+  }
   auto go = [&](auto out_tag, auto glu_tag) {
     typedef typename decltype(out_tag)::type O;
-    hipLaunchKernelGGL((mx_tile_kernel<C, EXPERTS, O, decltype(glu_tag)::value>), dim3((unsigned)grid), dim3(C::THREADS), C::LDS, stream, p);
+    hipLaunchKernelGGL((mx_tile_kernel<C, EXPERTS, O, decltype(glu_tag)::value, false>), dim3((unsigned)grid), dim3(C::THREADS), C::LDS, stream, p);
     return mx_launched();
   };
   auto gated = [&](auto out_tag) { return p.epi != EPI_NONE ? go(out_tag, BoolTag<true>()) : go(out_tag, BoolTag<false>()); };
@@ -642,37 +679,72 @@ double tiles_us(int64_t tiles, int slots, double t, double t_few, double o, int6
   return rounds * (slabs * t + o) + (rest ? slabs * (2 * rest <= slots ? t_few : t) + o : 0.0);
 }
 
+enum Kind { FEW, TILE_64, TILE_128, TILE_128_DEEP, TILE_256 };
+struct Choice {
+  Kind kind;
+  int parts;
+};
+
 // The tile with the lowest estimate.  Fitted to products of 8 to 4096 rows with 256 x 1024 to 14336 x 14336 weights, and of 4 to 4096 tokens with 8 to
 // 128 experts.  What it decides, measured in us: 1024 x 4096 x 4096 tiles of 64 18.5, of 128 15.1 (one on a CU, four buffers, eight waves; 15.6 with four) and 16.0 (two on a
 // CU, two buffers), of 256 25.6; 2048 x 14336 x 4096 117, 88, 73 and 66; 512 x 4096 x 14336 27, 30, 46 and 69; 64 tokens through
 // the up-projections of 64 experts (4096 -> 1024) 49, 56, 49 and 56, through the down-projections 44, 55, 37 and 44.
-template <bool EXPERTS> int launch(const MxParams& p, bool raw, hipStream_t stream) {
+template <bool EXPERTS> struct Shape {
+  int64_t m, n, slabs, experts;
   // tiles of BM rows: how many there are at most, and how many to expect (an expert's last is half full)
-  auto most = [&](int bm) { return EXPERTS ? (int64_t)p.m / bm + 1 + (p.experts < p.m ? p.experts : p.m) : ((int64_t)p.m + bm - 1) / bm; };
-  auto expect = [&](int bm) {
+  int64_t most(int bm) const { return EXPERTS ? m / bm + 1 + (experts < m ? experts : m) : (m + bm - 1) / bm; }
+  int64_t expect(int bm) const {
     if (!EXPERTS) return most(bm);
-    const int64_t some = p.experts < p.m ? p.experts : p.m, n = (int64_t)p.m / bm + some / 2;
-    return n > some ? n : some;
-  };
-  auto cols = [&](int bn) { return ((int64_t)p.n + bn - 1) / bn; };
-  if (raw) return most(16) <= 65535 ? launch_few<EXPERTS, true>(p, most(16), stream) : TNX_E_UNSUPPORTED;
-  const double us64 = tiles_us(expect(64) * cols(64), 512, 0.5, 0.35, EXPERTS ? 3.8 : 1.5, p.slabs);
-  const double us128 = tiles_us(expect(128) * cols(128), 512, 1.1, 0.76, 4.5, p.slabs);
-  const double us128_deep = tiles_us(expect(128) * cols(128), 256, 0.5, 0.45, 6.0, p.slabs);
-  const double us256 = tiles_us(expect(256) * cols(256), 256, 1.77, 1.15, 9.0, p.slabs);
-  if constexpr (!EXPERTS) {
-    // The streaming kernel: a slab of a workgroup's eight waves is 35 kB of weights and rows, and a CU brings that in 1 us, however few of
-    // them are busy.  So it is for few rows, or few columns, and it shares k out.  40 x 64 x 9630: 7.7 us, tiles of 64 13.7; 8 x 4096 x 4096 4.6 and 7.4;
-    // 64 x 1024 x 4096 5.0 and 7.8, 128 rows 7.1 and 7.4; 256 x 256 x 16384 12 and 23; 48 x 4096 x 4096 11.6 and 7.6.
-    const int64_t outputs = cols(16) * most(16);
-    const int log = few_parts(outputs, p.slabs);
-    const double us_few = 2.7 + (double)(((outputs << log) + 256 * FEW_WAVES - 1) / (256 * FEW_WAVES) * ((p.slabs + (1 << log) - 1) >> log));
-    if (us_few < us64 && us_few < us128 && us_few < us128_deep && us_few < us256 && most(16) <= 65535) return launch_few<false, false>(p, most(16), stream);
+    const int64_t some = experts < m ? experts : m, some_tiles = m / bm + some / 2;
+    return some_tiles > some ? some_tiles : some;
   }
-  if (us256 <= us128 && us256 <= us128_deep && us256 <= us64) return launch_tile<MxTile<256, 256, 4, 2, 2>, EXPERTS>(p, most(256), stream);
-  if (us64 <= us128 && us64 <= us128_deep) return launch_tile<MxTile<64, 64, 2, 2, 4>, EXPERTS>(p, most(64), stream);
-  if (us128_deep < us128) return launch_tile<MxTile<128, 128, 4, 2, 4>, EXPERTS>(p, most(128), stream);
-  return launch_tile<MxTile<128, 128, 2, 2, 2>, EXPERTS>(p, most(128), stream);
+  int64_t cols(int bn) const { return (n + bn - 1) / bn; }
+
+  double us64(int parts = 1) const { return tiles_us(expect(64) * cols(64) * parts, 512, 0.5, 0.35, EXPERTS ? 3.8 : 1.5, (slabs + parts - 1) / parts); }
+  double us128_deep(int parts = 1) const { return tiles_us(expect(128) * cols(128) * parts, 256, 0.5, 0.45, 6.0, (slabs + parts - 1) / parts); }
+
+  Choice choose(size_t room) const {
+    Choice best{TILE_64, 1};
+    double us = us64();
+    auto offer = [&](Kind kind, int parts, double t) {
+      if (t < us) { us = t; best = {kind, parts}; }
+    };
+    offer(TILE_128_DEEP, 1, us128_deep());
+    offer(TILE_128, 1, tiles_us(expect(128) * cols(128), 512, 1.1, 0.76, 4.5, slabs));
+    offer(TILE_256, 1, tiles_us(expect(256) * cols(256), 256, 1.77, 1.15, 9.0, slabs));
+    if constexpr (!EXPERTS) {
+      // The streaming kernel: a slab of a workgroup's eight waves is 35 kB of weights and rows, and a CU brings that in 1 us, however few of
+      // them are busy.  So it is for few rows, or few columns, and it shares k out.  40 x 64 x 9630: 7.7 us, tiles of 64 13.7; 8 x 4096 x 4096 4.6 and 7.4;
+      // 64 x 1024 x 4096 5.0 and 7.8, 128 rows 7.1 and 7.4; 256 x 256 x 16384 12 and 23; 48 x 4096 x 4096 11.6 and 7.6.
+      const int64_t outputs = cols(16) * most(16);
+      const int log = few_parts(outputs, slabs);
+      if (most(16) <= 65535) offer(FEW, 1, 2.7 + (double)(((outputs << log) + 256 * FEW_WAVES - 1) / (256 * FEW_WAVES) * ((slabs + (1 << log) - 1) >> log)));
+      // Few tiles of many slabs: k in parts, a workgroup each, and a second launch that adds them up.  100 x 4096 x 14336 20.7 us, in 4 parts 15.0; 128 x 1024 x
+      // 16384 20.6, in 8 11.6; 64 x 64 x 30000 18.7 and 11.7; 64 x 4096 x 8192 13.6, in 4 11.4, 128 rows 13.1, in 2 13.5.
+      for (int parts = 2; parts <= 8; ++parts) {
+        if (slabs < 4 * parts || parts_bytes(m, n, parts) > room) break;
+        const double join = 5.0 + (double)parts_bytes(m, n, parts) / 2e6;
+        offer(TILE_64, parts, us64(parts) + join);
+        offer(TILE_128_DEEP, parts, us128_deep(parts) + join);
+      }
+    }
+    return best;
+  }
+};
+
+template <bool EXPERTS> int launch(const MxParams& p, bool raw, void* sums, size_t room, hipStream_t stream) {
+  const Shape<EXPERTS> shape{p.m, p.n, p.slabs, p.experts};
+  if (raw) return shape.most(16) <= 65535 ? launch_few<EXPERTS, true>(p, shape.most(16), stream) : TNX_E_UNSUPPORTED;
+  const Choice c = shape.choose(sums ? room : 0);
+  switch (c.kind) {
+    case TILE_256: return launch_tile<MxTile<256, 256, 4, 2, 2>, EXPERTS>(p, shape.most(256), stream);
+    case TILE_64: return launch_tile<MxTile<64, 64, 2, 2, 4>, EXPERTS>(p, shape.most(64), stream, c.parts, sums);
+    case TILE_128_DEEP: return launch_tile<MxTile<128, 128, 4, 2, 4>, EXPERTS>(p, shape.most(128), stream, c.parts, sums);
+    case TILE_128: return launch_tile<MxTile<128, 128, 2, 2, 2>, EXPERTS>(p, shape.most(128), stream);
+    default: break;
+  }
+  if constexpr (!EXPERTS) return launch_few<false, false>(p, shape.most(16), stream);
+  return TNX_E_UNSUPPORTED;
 }
 
 bool takes_rows(int64_t a_rows, int64_t k) {
@@ -682,6 +754,12 @@ bool takes_rows(int64_t a_rows, int64_t k) {
 }  // namespace
 
 extern "C" int tnx_mx_gemm_takes_rows(int64_t a_rows, int64_t k) { return a_rows > 0 && k > 0 && takes_rows(a_rows, k); }
+
+extern "C" size_t tnx_mx_gemm_workspace_bytes(const tnx_mx_gemm_args* a) {
+  if (!a || a->m <= 0 || a->n <= 0 || a->k <= 0 || a->experts != 0 || a->a_data || a->k > TNX_MX_MAX_K || a->m > 0x3fffffff || a->n > 0x3fffffff) return 0;
+  const Shape<false> shape{a->m, a->n, mx_slabs(a->k), 0};
+  return parts_bytes(a->m, a->n, shape.choose(MAX_PARTS_BYTES).parts);
+}
 
 extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
   if (!a || a->m < 0 || a->n < 0 || a->k < 0 || a->experts < 0 || a->epilogue < TNX_EPI_NONE || a->epilogue > TNX_EPI_GLU_IDENTITY) return TNX_E_INVALID;
@@ -713,6 +791,8 @@ extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
   p.experts = a->experts; p.tiles_n = p.tiles_m = 0;
   p.top_k = make_fastdiv((uint32_t)(a->order ? a->top_k : 1));
   p.out_dtype = a->out_dtype; p.epi = a->epilogue;
-  p.a_dtype = a->a_dtype; p.lda = a->stride_a; p.k = (int)a->k; p.wk_log = 0; p.stream_b = false;
-  return a->experts > 0 ? launch<true>(p, raw, (hipStream_t)a->stream) : launch<false>(p, raw, (hipStream_t)a->stream);
+  p.a_dtype = a->a_dtype; p.lda = a->stride_a; p.k = (int)a->k; p.wk_log = 0; p.part_slabs = p.slabs; p.stream_b = false;
+  if (a->workspace && ((uintptr_t)a->workspace & 15)) return TNX_E_INVALID;
+  const size_t room = a->workspace_bytes < MAX_PARTS_BYTES ? a->workspace_bytes : MAX_PARTS_BYTES;
+  return a->experts > 0 ? launch<true>(p, raw, nullptr, 0, (hipStream_t)a->stream) : launch<false>(p, raw, a->workspace, room, (hipStream_t)a->stream);
 }

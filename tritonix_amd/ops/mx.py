@@ -53,7 +53,7 @@ def find_native():
     else:
         lib = _C.load()
         module.bind_ops(tuple(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
-            lib.tnx_mx_code_bytes, lib.tnx_mx_scale_bytes, lib.tnx_mx_quantize, lib.tnx_mx_quantize_both, lib.tnx_mx_dequantize, lib.tnx_mx_gemm_takes_rows, lib.tnx_mx_gemm,
+            lib.tnx_mx_code_bytes, lib.tnx_mx_scale_bytes, lib.tnx_mx_quantize, lib.tnx_mx_quantize_both, lib.tnx_mx_dequantize, lib.tnx_mx_gemm_takes_rows, lib.tnx_mx_gemm, lib.tnx_mx_gemm_workspace_bytes,
             lib.tnx_moe_workspace_bytes, lib.tnx_moe_route, lib.tnx_moe_route_backward, lib.tnx_moe_combine)) + (JOIN_BYTES,))
         native = module
     return native
@@ -292,7 +292,13 @@ def _product(name: str, a, b, out_dtype, epilogue: int) -> torch.Tensor:
     if k == 0:
         return torch.zeros((m, n), dtype=out_dtype, device=b.device)
     out = torch.empty((m, n), dtype=out_dtype, device=b.device)
-    launch(name, index, _C.load().tnx_mx_gemm, gemm_args(a, b, out, epilogue))
+    g = gemm_args(a, b, out, epilogue)
+    nbytes = int(_C.load().tnx_mx_gemm_workspace_bytes(ctypes.byref(g)))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=b.device) if nbytes else None
+    if scratch is not None:
+        g.workspace, g.workspace_bytes = scratch.data_ptr(), nbytes
+    launch(name, index, _C.load().tnx_mx_gemm, g)
+    del scratch
     return out
 
 
