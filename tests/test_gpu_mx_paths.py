@@ -226,3 +226,24 @@ def test_the_example_runs(device, capsys):
     worst, largest = main(tokens=300, width=256, inner=128, experts=8, top_k=2, device=device)
     assert 0 < largest < float("inf") and 0 <= worst < float("inf")
     assert "rows per expert" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_second_derivatives_are_an_error(device, monkeypatch, native):
+    """Not a silent zero: the gradients are computed, and differentiating them says so."""
+    if not native:
+        monkeypatch.setattr(mx, "native", mx._Interpreter)
+    x, w = rand(device, 33, 64, dtype=torch.float32).requires_grad_(True), rand(device, 64, 40, dtype=torch.float32, seed=1).requires_grad_(True)
+    want = torch.autograd.grad(tritonix.mx_linear(x, w).square().sum(), (x, w))
+    got = torch.autograd.grad(tritonix.mx_linear(x, w).square().sum(), (x, w), create_graph=True)
+    assert all(torch.equal(g, h) for g, h in zip(got, want))
+    with pytest.raises(RuntimeError):
+        got[0].sum().backward()
+    (one,) = torch.autograd.grad(tritonix.mx_linear(x, w.detach()).square().sum(), x, create_graph=True)
+    assert torch.equal(one, want[0])
+    with pytest.raises(RuntimeError):
+        one.sum().backward()
+    logits = rand(device, 9, 16, dtype=torch.float32).requires_grad_(True)
+    (g,) = torch.autograd.grad(tritonix.moe_route(logits, 3).weights.square().sum(), logits, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

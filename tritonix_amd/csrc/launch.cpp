@@ -18,6 +18,7 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/headeronly/version.h>
 
@@ -650,7 +651,15 @@ struct LinearStep : torch::autograd::Function<LinearStep> {
     if (wants_dx) dx = multiplied(qy.last, {saved[1], (int64_t)ops.code_bytes(k, n), TNX_OK}, m, k, n, type, device, stream);
     if (wants_dw) dw = multiplied({saved[0], (int64_t)ops.code_bytes(k, m), TNX_OK}, qy.first, k, n, m, type, device, stream);
     TORCH_CHECK(dx.status == TNX_OK && dw.status == TNX_OK, "mx_linear: status ", dx.status != TNX_OK ? dx.status : dw.status, " in the backward pass");
-    return {dx.out, dw.out, at::Tensor(), at::Tensor()};
+    torch::autograd::variable_list out{dx.out, dw.out};
+    if (at::GradMode::is_enabled()) {
+      // (asked for gradients of these gradients: an error where they are differentiated, not a silent zero)
+      for (at::Tensor& t : out)
+        if (t.defined()) t.set_requires_grad(true);
+      out = (*std::make_shared<torch::autograd::DelayedError>("mx_linear has no second derivative", 2))(std::move(out));
+    }
+    out.resize(4);
+    return out;
   }
 };
 

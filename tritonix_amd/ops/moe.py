@@ -17,6 +17,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from tritonix_amd import _C
 from tritonix_amd.ops import mx as _mx
@@ -137,6 +138,7 @@ class _Route(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad, *_):
         logits, weights, experts = ctx.saved_tensors
         return _backward(grad, logits, weights, experts, ctx.options), None, None, None

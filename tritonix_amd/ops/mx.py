@@ -16,6 +16,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from tritonix_amd import _C
 from tritonix_amd.kernel import _stream_of, launch_module
@@ -328,6 +329,7 @@ class _Linear(torch.autograd.Function):
         return mx_matmul(x, w)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, w = ctx.saved_tensors
         dx = dw = None
