@@ -247,3 +247,21 @@ def test_second_derivatives_are_an_error(device, monkeypatch, native):
     (g,) = torch.autograd.grad(tritonix.moe_route(logits, 3).weights.square().sum(), logits, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("tokens,dtype", [(1, torch.float32), (40, torch.bfloat16), (2000, torch.float32)], ids=str)
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_routing_in_the_graph(device, monkeypatch, tokens, dtype, scoring):
+    logits = rand(device, tokens, 48, dtype=dtype).requires_grad_(True)
+    bias, grad = rand(device, 48, dtype=torch.float32, seed=1), rand(device, tokens, 4, dtype=torch.float32, seed=2)
+
+    def call():
+        r = tritonix.moe_route(logits, 4, scoring=scoring, bias=bias, renormalize=False, scale=2.0)
+        assert r.weights.requires_grad and not any(t.requires_grad for t in (r.experts, r.offsets, r.order, r.rows))
+        (g,) = torch.autograd.grad(r.weights, logits, grad.t().contiguous().t(), retain_graph=True)
+        (h,) = torch.autograd.grad(r.weights.sum(), logits)              # (strides of zero)
+        return r.weights.detach(), r.experts, r.offsets, r.order, r.rows, g, h
+    both(monkeypatch, call, ["moe_route"])
+    r = tritonix.moe_route(logits, 4, scoring=scoring, bias=bias, renormalize=False, scale=2.0)
+    explicit = tritonix.moe_route_backward(grad, logits.detach(), r)
+    assert torch.equal(torch.autograd.grad(r.weights, logits, grad)[0], explicit)

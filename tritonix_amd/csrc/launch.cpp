@@ -611,6 +611,19 @@ Multiplied multiplied(const Quantised& a, const Quantised& b, int64_t m, int64_t
   return r;
 }
 
+// What a backward pass returns, for a node of `inputs` inputs.  Where gradients of these gradients may be asked for, differentiating them is an error,
+// not a silent zero.
+torch::autograd::variable_list gradients(torch::autograd::variable_list out, size_t inputs, const char* message) {
+  if (at::GradMode::is_enabled()) {
+    for (at::Tensor& t : out)
+      if (t.defined()) t.set_requires_grad(true);
+    const int64_t count = (int64_t)out.size();
+    out = (*std::make_shared<torch::autograd::DelayedError>(message, count))(std::move(out));
+  }
+  out.resize(inputs);
+  return out;
+}
+
 // The training step of a linear layer as a node of the autograd graph: y = x w, dx = dy w^T, dw = x^T dy.  Each matrix is read once, for both of
 // its quantisations; kept for the backward pass are the quantised x and w (17/32 of a byte an element) that its products take.
 struct LinearStep : torch::autograd::Function<LinearStep> {
@@ -651,15 +664,7 @@ struct LinearStep : torch::autograd::Function<LinearStep> {
     if (wants_dx) dx = multiplied(qy.last, {saved[1], (int64_t)ops.code_bytes(k, n), TNX_OK}, m, k, n, type, device, stream);
     if (wants_dw) dw = multiplied({saved[0], (int64_t)ops.code_bytes(k, m), TNX_OK}, qy.first, k, n, m, type, device, stream);
     TORCH_CHECK(dx.status == TNX_OK && dw.status == TNX_OK, "mx_linear: status ", dx.status != TNX_OK ? dx.status : dw.status, " in the backward pass");
-    torch::autograd::variable_list out{dx.out, dw.out};
-    if (at::GradMode::is_enabled()) {
-      // (asked for gradients of these gradients: an error where they are differentiated, not a silent zero)
-      for (at::Tensor& t : out)
-        if (t.defined()) t.set_requires_grad(true);
-      out = (*std::make_shared<torch::autograd::DelayedError>("mx_linear has no second derivative", 2))(std::move(out));
-    }
-    out.resize(4);
-    return out;
+    return gradients({dx.out, dw.out}, 4, "mx_linear has no second derivative");
   }
 };
 
@@ -679,8 +684,86 @@ PyObject* mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
+// weights, experts, offsets, order, rows of the routing that `a` describes
+struct Routed {
+  at::Tensor weights, experts, offsets, order, rows;
+  int status;
+};
+Routed routed(tnx_moe_args a, c10::DeviceIndex device) {
+  Routed r;
+  r.weights = fresh({a.tokens, a.top_k}, at::kFloat, device);
+  r.experts = fresh({a.tokens, a.top_k}, at::kInt, device);
+  r.offsets = fresh({a.num_experts + 1}, at::kInt, device);
+  r.order = fresh({a.tokens * a.top_k}, at::kInt, device);
+  r.rows = fresh({a.tokens, a.top_k}, at::kInt, device);
+  at::Tensor scratch;
+  const size_t bytes = ops.workspace_bytes(a.tokens, a.top_k, a.num_experts);
+  if (bytes) {
+    scratch = fresh({(int64_t)bytes}, at::kByte, device);
+    a.workspace = scratch.data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  a.weights = (float*)r.weights.data_ptr();
+  a.experts = (int32_t*)r.experts.data_ptr();
+  a.offsets = (int32_t*)r.offsets.data_ptr();
+  a.order = (int32_t*)r.order.data_ptr();
+  a.rows = (int32_t*)r.rows.data_ptr();
+  r.status = ops.route(&a);
+  return r;
+}
+
+// gradient of the logits; weights and experts [tokens, top_k] and grad of the same shape are contiguous
+int route_gradient(const at::Tensor& logits, const at::Tensor& weights, const at::Tensor& experts, const at::Tensor& grad, int32_t scoring, int32_t renormalize,
+                   float scale, c10::DeviceIndex device, void* stream, at::Tensor* out) {
+  tnx_moe_args a = {};
+  a.logits = logits.data_ptr();
+  a.weights = (float*)weights.data_ptr();
+  a.experts = (int32_t*)experts.data_ptr();
+  a.grad = (const float*)grad.data_ptr();
+  a.tokens = logits.size(0); a.stride_logits = logits.stride(0);
+  a.num_experts = (int32_t)logits.size(1); a.top_k = (int32_t)weights.size(1); a.dtype = float_code(logits.scalar_type());
+  a.scoring = scoring; a.renormalize = renormalize;
+  a.num_groups = a.top_groups = a.group_top = 1;
+  a.scale = scale;
+  a.stream = stream;
+  *out = fresh({a.tokens, a.num_experts}, logits.scalar_type(), device);
+  a.grad_logits = out->data_ptr();
+  return ops.backward(&a);
+}
+
+// The routing as a node of the autograd graph: the weights carry a gradient, the choice is held fixed
+struct RouteStep : torch::autograd::Function<RouteStep> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const tnx_moe_args& a) {
+    Routed r;
+    {
+      const Unlocked unlocked;
+      r = routed(a, (c10::DeviceIndex)logits.get_device());
+    }
+    if (r.status != TNX_OK) throw std::runtime_error("moe_route");
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({r.experts, r.offsets, r.order, r.rows});
+    ctx->save_for_backward({logits, r.weights, r.experts});
+    ctx->saved_data["scoring"] = (int64_t)a.scoring;
+    ctx->saved_data["renormalize"] = (int64_t)a.renormalize;
+    ctx->saved_data["scale"] = (double)a.scale;
+    return {r.weights, r.experts, r.offsets, r.order, r.rows};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    TORCH_CHECK(plain(grads[0], 2) && grads[0].sizes() == saved[1].sizes(), "moe_route: a gradient that is not an ordinary tensor of the weights' size");
+    const at::Tensor grad = grads[0].detach().to(at::kFloat).contiguous();
+    const c10::DeviceIndex device = (c10::DeviceIndex)grad.get_device();
+    at::Tensor out;
+    const int status = route_gradient(saved[0], saved[1], saved[2], grad, (int32_t)ctx->saved_data["scoring"].toInt(), (int32_t)ctx->saved_data["renormalize"].toInt(),
+                                      (float)ctx->saved_data["scale"].toDouble(), device, c10::hip::getCurrentHIPStream(device).stream(), &out);
+    TORCH_CHECK(status == TNX_OK, "moe_route: status ", status, " in the backward pass");
+    return gradients({out}, 2, "moe_route has no second derivative");
+  }
+};
+
 // moe_route(logits, bias or None, top_k, scoring, num_groups, top_groups, group_top, renormalize, scale) -> (weights, experts, offsets, order,
-// rows), or None
+// rows), the weights with their place in the graph, or None
 PyObject* moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 9 || !PyFloat_Check(args[8])) Py_RETURN_NONE;
   try {
@@ -702,32 +785,17 @@ PyObject* moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.scoring = (int32_t)v[1]; a.num_groups = (int32_t)v[2]; a.top_groups = (int32_t)v[3]; a.group_top = (int32_t)v[4]; a.renormalize = (int32_t)v[5];
     a.scale = (float)PyFloat_AS_DOUBLE(args[8]);
     a.stream = c10::hip::getCurrentHIPStream(device).stream();
-    at::Tensor weights, chosen, offsets, order, rows;
-    int status;
-    {
+    Routed r;
+    if (at::GradMode::is_enabled() && logits->requires_grad()) {
+      const torch::autograd::variable_list out = RouteStep::apply(*logits, a);
+      r = {out[0], out[1], out[2], out[3], out[4], TNX_OK};
+    } else {
       const Unlocked unlocked;
-      weights = fresh({tokens, top_k}, at::kFloat, device);
-      chosen = fresh({tokens, top_k}, at::kInt, device);
-      offsets = fresh({experts + 1}, at::kInt, device);
-      order = fresh({tokens * top_k}, at::kInt, device);
-      rows = fresh({tokens, top_k}, at::kInt, device);
-      at::Tensor scratch;
-      const size_t bytes = ops.workspace_bytes(tokens, a.top_k, a.num_experts);
-      if (bytes) {
-        scratch = fresh({(int64_t)bytes}, at::kByte, device);
-        a.workspace = scratch.data_ptr();
-        a.workspace_bytes = bytes;
-      }
-      a.weights = (float*)weights.data_ptr();
-      a.experts = (int32_t*)chosen.data_ptr();
-      a.offsets = (int32_t*)offsets.data_ptr();
-      a.order = (int32_t*)order.data_ptr();
-      a.rows = (int32_t*)rows.data_ptr();
-      status = ops.route(&a);
+      r = routed(a, device);
     }
-    if (status != TNX_OK) Py_RETURN_NONE;
-    const Object o[5] = {taken(THPVariable_Wrap(weights)), taken(THPVariable_Wrap(chosen)), taken(THPVariable_Wrap(offsets)),
-                         taken(THPVariable_Wrap(order)), taken(THPVariable_Wrap(rows))};
+    if (r.status != TNX_OK) Py_RETURN_NONE;
+    const Object o[5] = {taken(THPVariable_Wrap(r.weights)), taken(THPVariable_Wrap(r.experts)), taken(THPVariable_Wrap(r.offsets)),
+                         taken(THPVariable_Wrap(r.order)), taken(THPVariable_Wrap(r.rows))};
     for (const Object& x : o)
       if (!x.p) return nullptr;
     return PyTuple_Pack(5, o[0].p, o[1].p, o[2].p, o[3].p, o[4].p);
@@ -751,24 +819,12 @@ PyObject* moe_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
         weights->scalar_type() != at::kFloat || chosen->scalar_type() != at::kInt || !grad->is_contiguous() || !weights->is_contiguous() ||
         !chosen->is_contiguous() || (logits->stride(1) != 1 && experts > 1) || float_code(logits->scalar_type()) < 0)
       Py_RETURN_NONE;
-    tnx_moe_args a = {};
-    a.logits = logits->data_ptr();
-    a.weights = (float*)weights->data_ptr();
-    a.experts = (int32_t*)chosen->data_ptr();
-    a.grad = (const float*)grad->data_ptr();
-    a.tokens = tokens; a.stride_logits = logits->stride(0);
-    a.num_experts = (int32_t)experts; a.top_k = (int32_t)weights->size(1); a.dtype = float_code(logits->scalar_type());
-    a.scoring = (int32_t)v[0]; a.renormalize = (int32_t)v[1];
-    a.num_groups = a.top_groups = a.group_top = 1;
-    a.scale = (float)PyFloat_AS_DOUBLE(args[6]);
-    a.stream = c10::hip::getCurrentHIPStream(device).stream();
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
     at::Tensor out;
     int status;
     {
       const Unlocked unlocked;
-      out = fresh({tokens, experts}, logits->scalar_type(), device);
-      a.grad_logits = out.data_ptr();
-      status = ops.backward(&a);
+      status = route_gradient(*logits, *weights, *chosen, *grad, (int32_t)v[0], (int32_t)v[1], (float)PyFloat_AS_DOUBLE(args[6]), device, stream, &out);
     }
     if (status != TNX_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(out);

@@ -129,6 +129,8 @@ def _route(logits, bias, top_k, options):
 
 
 class _Route(torch.autograd.Function):
+    """What the native side has not taken."""
+
     @staticmethod
     def forward(ctx, logits, bias, top_k, options):
         out = _route(logits, bias, top_k, options)
@@ -160,7 +162,7 @@ def moe_route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: 
         raise ValueError(f"moe_route expects logits[t,e], got {tuple(logits.shape)}")
     renormalize, scale = bool(renormalize), float(scale)
     number = _SCORING.get(scoring)
-    if number is not None and (group_top == 1 or bias is not None) and not (logits.requires_grad and torch.is_grad_enabled()):
+    if number is not None and (group_top == 1 or bias is not None):
         out = (_mx.native or _mx.find_native()).moe_route(logits, bias, top_k, number, num_groups, top_groups, group_top, renormalize, scale)
         if out is not None:
             return Routing(*out, logits.shape[1], scoring, renormalize, scale)
