@@ -148,12 +148,13 @@ __device__ __forceinline__ void store_columns(const MxParams& p, int64_t row, in
 // What bounds them.  8192 x 8192 x 8192 on tiles of 256: 260 us, 4.2 PFLOP/s, on random values, and 190 to 215 on zeros: the board's power limit.  A tile costs
 // 1.8 us a slab and 9 beside its slabs, most of that for the burst of results that all CUs write at the end of a round; so 8192 x 4096 x 4096 74 us, 3.7
 // PFLOP/s.  Products of 16x16x128 instead, twice as many instructions for an issue slot that the reads and loads want as well: 295 us on
-// zeros.  With few rows of many weights it is the weights' bytes: 64 tokens of 8 through 64 experts' 4096 x 1024 matrices 37 us, 3.8 TB/s.
+// zeros.  With few rows of many weights it is the weights' bytes: 64 tokens of 8 through 64 experts' 4096 x 1024 matrices 30.6 us, 4.7 TB/s.
 template <int BN_, int BM_, int WGN, int WGM, int S_> struct MxTile {
   static constexpr int BN = BN_, BM = BM_, NW = WGN * WGM, THREADS = NW * 64, WAVES_N = WGN, S = S_;
   static constexpr int WTN = BN / WGN, WTM = BM / WGM, TN = WTN / 32, TM = WTM / 32;
   static constexpr int B_BYTES = BN * MX_ROWB, A_BYTES = BM * MX_ROWB;
-  static constexpr int SLOT = B_BYTES + A_BYTES, S_BYTES = (BN + BM) * 2 * MX_SCALEB;      // codes of a slab; scales of two
+  static constexpr int S_WAVES = (BN + BM + 63) / 64;     // waves that bring the scales of 64 rows each
+  static constexpr int SLOT = B_BYTES + A_BYTES, S_BYTES = S_WAVES * 64 * 2 * MX_SCALEB;      // codes of a slab; scales of two
   static constexpr int B_OPS = B_BYTES / (1024 * NW), A_OPS = A_BYTES / (1024 * NW);      // 16-byte loads per lane and slab
   static constexpr int LDS = S * (SLOT + S_BYTES);       // (slabs s .. s + S are of S / 2 + 1 pairs: S buffers are enough)
   // waves per SIMD that the LDS leaves room for
@@ -286,8 +287,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
     }
   }
   // Scales: 16 bytes a row, for two slabs; wave w brings those of 64 rows, of the weights' first, then of a's
-  constexpr int S_WAVES = (BN + BM) / 64;
-  static_assert(S_WAVES <= NW, "a wave has one load of scales");
+  constexpr int S_WAVES = C::S_WAVES;
+  static_assert(S_WAVES <= NW && BN % 64 == 0, "a wave has one load of scales");
   const uint8_t* s_at;
   {
     const int row = 64 * wave + lane, ar = row - BN;
@@ -679,7 +680,7 @@ double tiles_us(int64_t tiles, int slots, double t, double t_few, double o, int6
   return rounds * (slabs * t + o) + (rest ? slabs * (2 * rest <= slots ? t_few : t) + o : 0.0);
 }
 
-enum Kind { FEW, TILE_64, TILE_128, TILE_128_DEEP, TILE_256 };
+enum Kind { FEW, TILE_32, TILE_64, TILE_128, TILE_128_DEEP, TILE_256 };
 struct Choice {
   Kind kind;
   int parts;
@@ -688,7 +689,7 @@ struct Choice {
 // The tile with the lowest estimate.  Fitted to products of 8 to 4096 rows with 256 x 1024 to 14336 x 14336 weights, and of 4 to 4096 tokens with 8 to
 // 128 experts.  What it decides, measured in us: 1024 x 4096 x 4096 tiles of 64 18.5, of 128 15.1 (one on a CU, four buffers, eight waves; 15.6 with four) and 16.0 (two on a
 // CU, two buffers), of 256 25.6; 2048 x 14336 x 4096 117, 88, 73 and 66; 512 x 4096 x 14336 27, 30, 46 and 69; 64 tokens through
-// the up-projections of 64 experts (4096 -> 1024) 49, 56, 49 and 56, through the down-projections 44, 55, 37 and 44.
+// the up-projections of 64 experts (4096 -> 1024) 49, 56, 49 and 56, through the down-projections 44, 55, 37 and 44, with tiles of 32 30.6.
 template <bool EXPERTS> struct Shape {
   int64_t m, n, slabs, experts;
   // tiles of BM rows: how many there are at most, and how many to expect (an expert's last is half full)
@@ -712,7 +713,12 @@ template <bool EXPERTS> struct Shape {
     offer(TILE_128_DEEP, 1, us128_deep());
     offer(TILE_128, 1, tiles_us(expect(128) * cols(128), 512, 1.1, 0.76, 4.5, slabs));
     offer(TILE_256, 1, tiles_us(expect(256) * cols(256), 256, 1.77, 1.15, 9.0, slabs));
-    if constexpr (!EXPERTS) {
+    if constexpr (EXPERTS) {
+      // Experts of a dozen rows: a tile of 32 brings 4 kB of rows with 16 of weights where one of 128 brings 16, most of it the last row over again, and three
+      // are on a CU.  64 tokens, 8 of 128 experts, 2048 to 768, up 53 us on tiles of 128 and 35, down 37 and 30; 16 of 64 experts, 4096 to 1024, up 57 and 35; 512 of
+      // them 84 and 92.
+      offer(TILE_32, 1, tiles_us(expect(32) * cols(128), 768, 1.2, 1.2, 2.5, slabs));
+    } else {
       // The streaming kernel: a slab of a workgroup's eight waves is 35 kB of weights and rows, and a CU brings that in 1 us, however few of
       // them are busy.  So it is for few rows, or few columns, and it shares k out.  40 x 64 x 9630: 7.7 us, tiles of 64 13.7; 8 x 4096 x 4096 4.6 and 7.4;
       // 64 x 1024 x 4096 5.0 and 7.8, 128 rows 7.1 and 7.4; 256 x 256 x 16384 12 and 23; 48 x 4096 x 4096 11.6 and 7.6.
@@ -743,8 +749,8 @@ template <bool EXPERTS> int launch(const MxParams& p, bool raw, void* sums, size
     case TILE_128: return launch_tile<MxTile<128, 128, 2, 2, 2>, EXPERTS>(p, shape.most(128), stream);
     default: break;
   }
-  if constexpr (!EXPERTS) return launch_few<false, false>(p, shape.most(16), stream);
-  return TNX_E_UNSUPPORTED;
+  if constexpr (EXPERTS) return launch_tile<MxTile<128, 32, 4, 1, 2>, true>(p, shape.most(32), stream);
+  else return launch_few<false, false>(p, shape.most(16), stream);
 }
 
 bool takes_rows(int64_t a_rows, int64_t k) {
