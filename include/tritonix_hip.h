@@ -452,7 +452,8 @@ int tnx_moe_plan(const tnx_moe_args* args);
 /* grad_logits from grad: the choice is held fixed, as it is almost everywhere */
 int tnx_moe_route_backward(const tnx_moe_args* args);
 
-/* out[t, :] = sum over j of weights[t, j] * y[rows[t, j], :], empty slots left out; y [tokens * top_k, n] and out [tokens, n] contiguous.  32-bit sums. */
+/* out[t, :] = sum over j of weights[t, j] * y[rows[t, j], :]; y [tokens * top_k, n] and out [tokens, n] contiguous.  32-bit sums.  Empty slots (rows
+ * outside of y) are left out, but for a NaN weight, which tnx_moe_route gives a token with a NaN among its logits: out[t, :] is NaN there. */
 int tnx_moe_combine(const void* y, const int32_t* rows, const float* weights, void* out, int64_t tokens, int32_t top_k, int64_t n,
                     int32_t y_dtype, int32_t out_dtype, void* stream);
 

@@ -657,7 +657,8 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteParams p) {
   }
 }
 
-// The join: 16 bytes of a token's output per lane, the top_k rows one after another.
+// The join: 16 bytes of a token's output per lane, the top_k rows one after another.  An empty slot counts for nothing, unless its weight is NaN: that
+// is a token whose logits were (route_tokens), and its output says so.
 typedef uint16_t u16x8_loose __attribute__((ext_vector_type(8), aligned(2)));
 typedef float f32x8_loose __attribute__((ext_vector_type(8), aligned(4)));
 
@@ -673,8 +674,14 @@ __global__ __launch_bounds__(256) void combine_kernel(const uint8_t* y, const in
   const bool whole = c + 8 <= n;
   for (int j = 0; j < k; ++j) {
     const int r = rows[t * k + j];
-    if (r < 0 || r >= tokens * k) continue;
     const float w = weights[t * k + j];
+    if (r < 0 || r >= tokens * k) {
+      if (w != w) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = w;
+      }
+      continue;
+    }
     const int64_t at = (int64_t)r * n + c;
     if (whole) {
       if constexpr (YD == DT_F32) {

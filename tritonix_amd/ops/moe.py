@@ -271,6 +271,7 @@ def moe_glu(x, w12: MXTensor, routing: Routing, activation: str = "silu", out_dt
 
 def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
     """Down-projections of the rows that ``moe_glu`` made, joined: ``out[t] = sum_j weights[t, j] * (h[rows[t, j]] @ w3[e])``, ``[t, d]``.
+    Empty slots are left out; where their weight is NaN (``moe_route`` of a row with a NaN) the token's output is NaN.
 
     The join sums in 32 bits.  The products it sums are in 32 bits too where they take at most 32 MiB; larger ones are rounded to the result's
     type first (they are k times the result's size, and writing and reading them is what the join costs)."""
