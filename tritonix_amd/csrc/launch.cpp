@@ -370,7 +370,7 @@ struct OpEntries {
 } ops = {};
 int64_t join_bytes = 0;
 
-// bind_ops(addresses of the above, in their order, and the most bytes of a join's rows in 32 bits)
+// bind_ops(addresses of the above, in their order, and the most bytes of a bfloat16 join's rows in 32 bits)
 PyObject* bind_ops(PyObject*, PyObject* arg) {
   constexpr int N = sizeof(OpEntries) / sizeof(void*);
   if (!PyTuple_Check(arg) || PyTuple_GET_SIZE(arg) != N + 1) {
@@ -574,8 +574,8 @@ PyObject* mx_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
         g.a_codes = q.buffer.data_ptr();
         g.a_scales = (const uint8_t*)g.a_codes + q.code_bytes;
       }
-      // (the rows of a join: in 32 bits up to the size that moe.py has)
-      if (rows && g.m * g.n * 4 <= join_bytes) g.out_dtype = TNX_F32;
+      // (the rows of a join: in 32 bits where moe.py has them so)
+      if (rows && (code == TNX_F16 || g.m * g.n * 4 <= join_bytes)) g.out_dtype = TNX_F32;
       out = fresh({g.m, g.stride_out}, type_of(g.out_dtype), device);
       g.out = out.data_ptr();
       status = q.status != TNX_OK ? q.status : multiply(&g, device);

@@ -273,8 +273,9 @@ def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
     """Down-projections of the rows that ``moe_glu`` made, joined: ``out[t] = sum_j weights[t, j] * (h[rows[t, j]] @ w3[e])``, ``[t, d]``.
     Empty slots are left out; where their weight is NaN (``moe_route`` of a row with a NaN) the token's output is NaN.
 
-    The join sums in 32 bits.  The products it sums are in 32 bits too where they take at most 32 MiB; larger ones are rounded to the result's
-    type first (they are k times the result's size, and writing and reading them is what the join costs)."""
+    The join sums in 32 bits, and so are the products it sums, but for bfloat16 results whose products would take more than 32 MiB: those are rounded to
+    bfloat16 first (they are k times the result's size, and writing and reading them is what the join costs), which with eight experts takes the
+    error relative to the exact sum from 0.0017 to 0.0024.  ``out_dtype=torch.float32`` keeps them in 32 bits at every size."""
     if out_dtype is None and type(w3) is MXTensor and w3.batch == routing.num_experts and w3.dim == -2:
         out = (_mx.native or _mx.find_native()).mx_product(h, w3.buffer, w3.code_bytes, w3.rows, w3.k, _C.EPI_NONE, routing.num_experts, routing.top_k,
                                                            routing.offsets, None, routing.rows, routing.weights)
@@ -288,7 +289,8 @@ def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
     hq = h if takes_rows(h) else operand("moe_down", "h", h, -1)
     n = w3.rows
     rows = routing.tokens * routing.top_k
-    y = torch.empty((rows, n), dtype=torch.float32 if rows * n * 4 <= _mx.JOIN_BYTES else out_dtype, device=w3.device)
+    in_32_bits = out_dtype != torch.bfloat16 or rows * n * 4 <= _mx.JOIN_BYTES
+    y = torch.empty((rows, n), dtype=torch.float32 if in_32_bits else out_dtype, device=w3.device)
     _grouped("moe_down", hq, w3, routing, y, False, _C.EPI_NONE, index)
     out = torch.empty((routing.tokens, n), dtype=out_dtype, device=w3.device)
     with torch.cuda.device(index):

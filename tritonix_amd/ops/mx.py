@@ -25,8 +25,10 @@ __all__ = ["MXTensor", "mx_quantize", "mx_dequantize", "mx_matmul", "mx_glu", "m
 
 BLOCK = 32
 SLAB = 256                      # k is padded to whole slabs (csrc/mx.h)
-# Rows that moe_down joins are kept in 32 bits up to this many bytes, which the L2 caches hold together; larger ones, whose writing and reading is
-# what the join costs, are rounded to the result's type first (8192 tokens of 8 experts, 4096 wide: 1 GB each way in 32 bits).
+# Rows that moe_down joins are in 32 bits, in float16 whatever their number: a row may lie past 65504 where the weighted sum does not (8192 tokens of 8
+# experts, 1024 to 4096: 686 us, rounded to 16 bits 460).  bfloat16 has the range: its rows are in 32 bits up to this many bytes, which the L2 caches hold
+# together; more of them, whose writing and reading is what the join costs (1 GB each way in 32 bits: 467 us instead of 690), are rounded first.  With eight
+# experts that takes the result's error, relative to the exact sum, from 0.0017 to 0.0024 (root mean square; the result's own rounding is the first).
 JOIN_BYTES = 32 << 20
 _DTYPES = {torch.float16: _C.F16, torch.bfloat16: _C.BF16, torch.float32: _C.F32}
 _EPILOGUES = {"silu": _C.EPI_GLU_SILU, "sigmoid": _C.EPI_GLU_SIGMOID}
