@@ -8,8 +8,8 @@ joined per token).  ``w12[e, d, 2f]`` is interleaved column-wise like ``glu``'s;
 that is summed over (``mx_quantize(w, dim=-2)`` or ``MXTensor.from_codes(..., dim=-2)``).  Nothing here waits for the GPU: the
 rows of each expert are counted and found on it.
 
-The router is trained through ``Routing.weights``, which carries its gradient; the experts' products are for answering and
-carry none, neither to x nor to the weights.
+The router is trained through ``Routing.weights``, which carries its gradient; the experts' products are for answering and pass none, neither to x nor
+to the routing's weights: where one of those asks for its gradient, differentiating their result is an error.
 """
 from __future__ import annotations
 
@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from tritonix_amd import _C
 from tritonix_amd.ops import mx as _mx
-from tritonix_amd.ops.mx import MXTensor, dtype_code, epilogue_of, gemm_args, launch, on_device, operand, raise_for_status, takes_rows
+from tritonix_amd.ops.mx import MXTensor, dtype_code, epilogue_of, gemm_args, launch, on_device, operand, raise_for_status, takes_rows, underived
 from tritonix_amd.kernel import _stream_of
 
 __all__ = ["Routing", "moe_route", "moe_route_backward", "moe_plan", "moe_glu", "moe_down", "moe_ffn"]
@@ -255,7 +255,7 @@ def moe_glu(x, w12: MXTensor, routing: Routing, activation: str = "silu", out_dt
         out = (_mx.native or _mx.find_native()).mx_product(x, w12.buffer, w12.code_bytes, w12.rows, w12.k, epilogue_of(activation), routing.num_experts,
                                                            routing.top_k, routing.offsets, routing.order, None, None)
         if out is not None:
-            return out
+            return underived("moe_glu", out, x) if x.requires_grad else out
     _check_experts("moe_glu", x, w12, routing, routing.tokens)
     if w12.rows % 2:
         raise ValueError("the interleaved weight must have an even number of columns")
@@ -266,7 +266,7 @@ def moe_glu(x, w12: MXTensor, routing: Routing, activation: str = "silu", out_dt
     xq = x if takes_rows(x) else operand("moe_glu", "x", x, -1)
     out = torch.empty((routing.tokens * routing.top_k, w12.rows // 2), dtype=out_dtype, device=w12.device)
     _grouped("moe_glu", xq, w12, routing, out, True, epilogue_of(activation), index)
-    return out
+    return underived("moe_glu", out, x)
 
 
 def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
@@ -280,7 +280,7 @@ def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
         out = (_mx.native or _mx.find_native()).mx_product(h, w3.buffer, w3.code_bytes, w3.rows, w3.k, _C.EPI_NONE, routing.num_experts, routing.top_k,
                                                            routing.offsets, None, routing.rows, routing.weights)
         if out is not None:
-            return out
+            return underived("moe_down", out, h, routing.weights) if h.requires_grad or routing.weights.requires_grad else out
     _check_experts("moe_down", h, w3, routing, routing.tokens * routing.top_k)
     if out_dtype is None:
         out_dtype = torch.bfloat16 if isinstance(h, MXTensor) else h.dtype
@@ -297,7 +297,7 @@ def moe_down(h, w3: MXTensor, routing: Routing, out_dtype=None) -> torch.Tensor:
         status = _C.load().tnx_moe_combine(y.data_ptr(), routing.rows.data_ptr(), routing.weights.data_ptr(), out.data_ptr(), routing.tokens,
                                            routing.top_k, n, dtype_code("moe_down", y.dtype), code, _stream_of(index))
     raise_for_status(status, "moe_down")
-    return out
+    return underived("moe_down", out, h, routing.weights)
 
 
 def moe_ffn(x, w12: MXTensor, w3: MXTensor, routing: Routing, activation: str = "silu", out_dtype=None) -> torch.Tensor:

@@ -107,6 +107,29 @@ def launch(what: str, index: int, fn, args) -> None:
         raise_for_status(status, what)
 
 
+class _Underived(torch.autograd.Function):
+    """``out`` as it is, with a place in the graph of its inputs: an error where a gradient is asked to pass."""
+
+    @staticmethod
+    def forward(ctx, name, out, *inputs):
+        ctx.name = name
+        return out[0]                                      # (in a list: not an input itself)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} passes no gradient to its inputs; detach them, or the result, where none is wanted (mx_linear has one)")
+
+
+def underived(name: str, out: torch.Tensor, *inputs) -> torch.Tensor:
+    """The result of an operator without a derivative.  Differentiating it is an error where an input asks for its gradient: left out of the graph, the
+    input's gradient would lack this term silently."""
+    if torch.is_grad_enabled():
+        inputs = tuple(t for t in inputs if isinstance(t, torch.Tensor) and t.requires_grad)
+        if inputs:
+            return _Underived.apply(name, [out], *inputs)
+    return out
+
+
 class MXTensor:
     """A matrix, or a batch of them, in microscaled 4-bit floats.
 
@@ -210,7 +233,8 @@ def mx_quantize(x: torch.Tensor, dim: int = -1) -> MXTensor:
     """``x`` (float16, bfloat16 or float32, a matrix or a batch of them, any strides) with blocks of 32 along ``dim``.
 
     A block's scale is 2^(floor(log2 of its largest magnitude) - 2); elements round to the nearest 4-bit float, ties to
-    the even code, and those past 6 scales to 6.  A block with an infinity or a NaN becomes NaN throughout."""
+    the even code, and those past 6 scales to 6.  A block with an infinity or a NaN becomes NaN throughout.  An ``MXTensor`` is data: it has no place in
+    the autograd graph."""
     if dim in (0, 1, -1, -2):
         last = dim in (1, -1)
         got = (native or find_native()).mx_quantize(x, last)             # (a matrix of the current device)
@@ -271,12 +295,13 @@ def gemm_args(a, b: MXTensor, out: torch.Tensor, epilogue: int) -> _C.MxGemmArgs
 
 
 def _product(name: str, a, b, out_dtype, epilogue: int) -> torch.Tensor:
+    given = b
     if type(b) is not MXTensor and not isinstance(a, MXTensor) and len(a.shape) == len(b.shape) == 2 and a.shape[1] == b.shape[0]:
         b = mx_quantize(b, dim=0)
     if type(b) is MXTensor and b.batch is None and b.dim == -2 and (out_dtype is None or out_dtype is getattr(a, "dtype", None)):
         out = (native or find_native()).mx_product(a, b.buffer, b.code_bytes, b.rows, b.k, epilogue)
         if out is not None:
-            return out
+            return out if given is b and not a.requires_grad else underived(name, out, a, given)
     if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[0]:
         raise ValueError(f"{name} expects a[m,k] and b[k,n], got {tuple(a.shape)} and {tuple(b.shape)}")
     if out_dtype is None:
@@ -284,6 +309,7 @@ def _product(name: str, a, b, out_dtype, epilogue: int) -> torch.Tensor:
     dtype_code(name, out_dtype)
     index = on_device(name, a, b)
     m, k = a.shape
+    inputs = (a, given)
     if not takes_rows(a):
         a = operand(name, "a", a, -1)
     b = operand(name, "b", b, -2)
@@ -293,7 +319,7 @@ def _product(name: str, a, b, out_dtype, epilogue: int) -> torch.Tensor:
             raise ValueError("the interleaved weight must have an even number of columns")
         n //= 2
     if k == 0:
-        return torch.zeros((m, n), dtype=out_dtype, device=b.device)
+        return underived(name, torch.zeros((m, n), dtype=out_dtype, device=b.device), *inputs)
     out = torch.empty((m, n), dtype=out_dtype, device=b.device)
     g = gemm_args(a, b, out, epilogue)
     nbytes = int(_C.load().tnx_mx_gemm_workspace_bytes(ctypes.byref(g)))
@@ -302,14 +328,14 @@ def _product(name: str, a, b, out_dtype, epilogue: int) -> torch.Tensor:
         g.workspace, g.workspace_bytes = scratch.data_ptr(), nbytes
     launch(name, index, _C.load().tnx_mx_gemm, g)
     del scratch
-    return out
+    return underived(name, out, *inputs)
 
 
 def mx_matmul(a, b, out_dtype=None) -> torch.Tensor:
     """``a @ b`` of microscaled operands, ``a[m, k]`` quantised along k (``dim=-1``) and ``b[k, n]`` along k (``dim=-2``).
 
     Either may be a torch tensor, quantised on the way in.  32-bit sums, rounded once to ``out_dtype`` (default: ``a``'s dtype, bfloat16 where it
-    has none).  The result carries no gradient: ``mx_linear`` does."""
+    has none).  No gradient passes: differentiating the result is an error where an operand asks for its own; ``mx_linear`` has them."""
     return _product("mx_matmul", a, b, out_dtype, _C.EPI_NONE)
 
 
@@ -318,7 +344,8 @@ def epilogue_of(activation: str) -> int:
 
 
 def mx_glu(x, w12, activation: str = "silu", out_dtype=None) -> torch.Tensor:
-    """``act(x @ w12[:, 0::2]) * (x @ w12[:, 1::2])`` of microscaled operands: ``glu`` with the gate in the product's epilogue."""
+    """``act(x @ w12[:, 0::2]) * (x @ w12[:, 1::2])`` of microscaled operands: ``glu`` with the gate in the product's epilogue.  No gradient passes, as
+    with ``mx_matmul``."""
     return _product("mx_glu", x, w12, out_dtype, epilogue_of(activation))
 
 
