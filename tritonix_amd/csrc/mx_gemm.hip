@@ -114,12 +114,23 @@ __device__ __forceinline__ int source_row(const MxParams& p, int r) {
   return t < p.a_rows ? t : p.a_rows - 1;
 }
 
-// act(g) * l.  The reciprocal is the instruction's own, good to a unit in the last place of 32 bits: the results are rounded from there.  (Its
-// corrected form and the division cost 256x128 gates of a tile 2 us more.)
-__device__ __forceinline__ float gated(float g, float l, int epi) {
-  if (epi == EPI_GLU_IDENTITY) return g * l;
-  const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
-  return (epi == EPI_GLU_SILU ? g * s : s) * l;
+// act(g) * l, to the bits of the tiles of wider types (glu_gate): a result of 16 bits from the reciprocal corrected to the division's, one of 32 from the
+// division.  Without branches, which would take the gates of a product one by one: whatever the activation, it is a factor of 1 or the sigmoid and one of 1 or
+// the gate.  SHORT: SiLU of a g that is not below -66, so that 1 + exp(-g) is where the correction needs neither a scale nor a bound and is two
+// instructions.  The empty asm makes the product a binary32 number, which is then rounded: the compiler takes it and the conversion to float16 together in
+// some of the kernels, and the same operands would give them other bits.
+template <bool ROUNDED, bool SHORT> __device__ __forceinline__ float gated(float g, float l, int epi) {
+  const float d = 1.0f + __expf(-g);
+  float v;
+  if (SHORT) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    v = g * __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) * l;
+  } else {
+    const float s = ROUNDED ? reciprocal_from_one(d) : 1.0f / d;
+    v = (epi == EPI_GLU_IDENTITY ? 1.0f : s) * (epi == EPI_GLU_SIGMOID ? 1.0f : g) * l;
+  }
+  if (ROUNDED) asm("" : "+v"(v));
+  return v;
 }
 
 // `count` of four neighbouring columns of a row (two with the gate), as many as there are
@@ -127,8 +138,9 @@ __device__ __forceinline__ void store_columns(const MxParams& p, int64_t row, in
   float o[4];
   int c = col, n = 4;
   if (p.epi != EPI_NONE) {
-    o[0] = gated(v[0], v[1], p.epi);
-    o[1] = gated(v[2], v[3], p.epi);
+    const bool rounded = p.out_dtype != DT_F32;
+    o[0] = rounded ? gated<true, false>(v[0], v[1], p.epi) : gated<false, false>(v[0], v[1], p.epi);
+    o[1] = rounded ? gated<true, false>(v[2], v[3], p.epi) : gated<false, false>(v[2], v[3], p.epi);
     o[2] = o[3] = 0.0f;
     c = col >> 1; n = 2; cols >>= 1;
   } else {
@@ -190,16 +202,24 @@ template <bool WHOLE, int ES, int WORDS> __device__ __forceinline__ void store_w
 // 8 q + 4 half + 0 .. 3.  Rounded, four columns are two words; exchanging the halves' words of an even q with those of the odd q after it leaves
 // lanes 0-31 with all eight columns of the one and lanes 32-63 with those of the other: 16 bytes a lane.  (With the gate two columns are a word,
 // 8 bytes a lane; binary32 needs no exchange.)
-template <bool WHOLE, class O, bool GLU>
+// SHORT: see gated; where that does not do, the product is stored by the other form, chosen once, by a scalar.  (bfloat16 by 4-bit 4096 x 28672 x 512 with
+// ordinary gates 69.1 us, always the other form 73.7, the bare reciprocal, whose results are not glu's, 68.0; 8192 tokens' up-projections 343, 351 and 340.)
+template <bool WHOLE, class O, bool GLU, bool SHORT = GLU && sizeof(typename O::raw) == 2>
 __device__ __forceinline__ void store_product(const f32x16& v, uint8_t* out, int64_t ldo, int r32, int half, int m_left, int left_cols, int epi) {
   constexpr int ES = sizeof(typename O::raw);
+  if constexpr (SHORT) {
+    float low = v[0];
+#pragma unroll
+    for (int e = 2; e < 16; e += 2) low = __builtin_fminf(low, v[e]);
+    if (epi != EPI_GLU_SILU || __any(low < -66.0f)) return store_product<WHOLE, O, GLU, false>(v, out, ldo, r32, half, m_left, left_cols, epi);
+  }
   uint8_t* row = out + (int64_t)r32 * ldo * ES;
   const bool have = WHOLE || r32 < m_left;
 #pragma unroll
   for (int q = 0; q < 4; q += 2) {
     float o[8];
 #pragma unroll
-    for (int e = 0; e < (GLU ? 4 : 8); ++e) o[e] = GLU ? gated(v[4 * q + 2 * e], v[4 * q + 2 * e + 1], epi) : v[4 * q + e];
+    for (int e = 0; e < (GLU ? 4 : 8); ++e) o[e] = GLU ? gated<ES == 2, SHORT>(v[4 * q + 2 * e], v[4 * q + 2 * e + 1], epi) : v[4 * q + e];
     if constexpr (ES == 4) {
       constexpr int W = GLU ? 2 : 4;
 #pragma unroll
