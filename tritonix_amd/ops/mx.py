@@ -123,10 +123,9 @@ class _Underived(torch.autograd.Function):
 def underived(name: str, out: torch.Tensor, *inputs) -> torch.Tensor:
     """The result of an operator without a derivative.  Differentiating it is an error where an input asks for its gradient: left out of the graph, the
     input's gradient would lack this term silently."""
-    if torch.is_grad_enabled():
-        inputs = tuple(t for t in inputs if isinstance(t, torch.Tensor) and t.requires_grad)
-        if inputs:
-            return _Underived.apply(name, [out], *inputs)
+    for t in inputs:
+        if t.requires_grad and torch.is_grad_enabled():
+            return _Underived.apply(name, [out], *(i for i in inputs if i.requires_grad))
     return out
 
 
@@ -138,6 +137,7 @@ class MXTensor:
     kernels read them (include/tritonix_hip.h)."""
 
     __slots__ = ("buffer", "batch", "rows", "k", "dim", "code_bytes")
+    requires_grad = False
 
     def __init__(self, buffer: torch.Tensor, batch: Optional[int], rows: int, k: int, dim: int, code_bytes: int):
         self.buffer, self.batch, self.rows, self.k, self.dim, self.code_bytes = buffer, batch, rows, k, dim, code_bytes
