@@ -85,6 +85,13 @@ template <int L> __device__ __forceinline__ int lanes_or(int v) {
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+// exp(x), x <= 0, down to the smallest number: the exponential's instruction itself gives 0 for results next to the subnormal numbers
+__device__ __forceinline__ float exp_below(float x) {
+  const float h = __expf(0.5f * x);
+  return h * h;
+}
+// What a sum of scores and its terms are multiplied by, so that neither its reciprocal nor a quotient by it leaves the range: 1 but for scores next to nothing
+__device__ __forceinline__ float lift_of(float total) { return total < 0x1p-60f ? 0x1p64f : 1.0f; }
 
 // Expert i of lane j where L lanes hold a row: four neighbours a lane, so that a load or store is 16 bytes.
 template <int L> __device__ __forceinline__ int expert_of(int i, int j) { return (i >> 2) * (4 * L) + 4 * j + (i & 3); }
@@ -233,7 +240,7 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int tid, int6
     sum = lanes_sum<L>(sum);
     inv = sum > 0.0f ? 1.0f / sum : 0.0f;
   }
-  auto score = [&](float x) { return soft ? __expf(x - off) * inv : sigmoid(x); };
+  auto score = [&](float x) { return soft ? __expf(x - off) * inv : sigmoid(x); };      // (as keys have it)
   float key[EPL];
   if (FULL) {
     float (&f)[EPL] = key;
@@ -360,23 +367,35 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int tid, int6
 #pragma unroll
     for (int r = 0; r < KR; ++r) id[r] = r * L + j < p.k ? chosen[r * L + j] : 0;
   }
-  float w[KR], total = 0.0f;
+  float w[KR], total = 0.0f, most = off;
+  const bool shares = FULL && p.bias && soft && p.renorm;  // a bias may choose experts far below the row's largest: a softmax of the chosen among themselves
 #pragma unroll
   for (int r = 0; r < KR; ++r) {
     const bool found = won[r] > -INFINITY && !bad;        // (a row with a NaN may have chosen nothing at all)
     id[r] = found ? id[r] : -1;
     // (with a bias the key is not the logit: read again)
-    const float x = found ? (FULL && p.bias ? load_logit(row, id[r], p.dtype) : won[r]) : 0.0f;
-    w[r] = found ? score(x) : 0.0f;
+    w[r] = !found ? -INFINITY : FULL && p.bias ? load_logit(row, id[r], p.dtype) : won[r];
+  }
+  if (shares) {
+    most = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < KR; ++r) most = __builtin_fmaxf(most, w[r]);
+    most = lanes_max<L>(most);
+    inv = 1.0f;
+  }
+#pragma unroll
+  for (int r = 0; r < KR; ++r) {
+    w[r] = id[r] < 0 ? 0.0f : soft ? exp_below(w[r] - most) * inv : sigmoid(w[r]);
     total += w[r];
   }
   total = lanes_sum<L>(total);
-  const float f = p.renorm ? (total > 0.0f ? p.scale / total : 0.0f) : p.scale;
+  const float lift = p.renorm ? lift_of(total) : 1.0f;
+  const float f = p.renorm ? (total > 0.0f ? p.scale / (total * lift) : 0.0f) : p.scale;
 #pragma unroll
   for (int r = 0; r < KR; ++r) {
     const int q = r * L + j;
     if (live && q < p.k) {
-      p.weights[token * p.k + q] = bad ? __builtin_nanf("") : w[r] * f;
+      p.weights[token * p.k + q] = bad ? __builtin_nanf("") : w[r] * lift * f;
       p.experts[token * p.k + q] = id[r];
     }
   }
@@ -560,7 +579,7 @@ __global__ __launch_bounds__(256) void plan_place_kernel(PlanParams p) {
 //   ds_j = scale g_j, or scale (g_j - sum_i (s_i / S) g_i) / S with renormalised weights
 //   softmax: dl_i = s_i (ds_i - sum_j s_j ds_j) over all i; with renormalised weights the sum is zero and s_j / S = weight / scale, so
 //            neither the logits nor the other experts enter: dl_j = w_j (g_j - sum_i (w_i / scale) g_i)
-//   sigmoid: dl_j = ds_j s_j (1 - s_j), of the chosen alone
+//   sigmoid: dl_j = ds_j s_j (1 - s_j), of the chosen alone (renormalised: the quotient s_j / S first, which is at most 1 where 1 / S may be past the range)
 // The chosen experts' values go through a row in LDS that starts as zeros, and the row leaves in runs of four.  Bound by writing the
 // gradient: 65536 x 128, float32, renormalised softmax: 7.7 us for 33.5 MB.  (Compared one by one with every lane's experts: 13.6 us.)
 template <int L, int EPL>
@@ -617,6 +636,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteParams p) {
   const bool bad = lanes_or<L>(bad_bit) != 0;
   wg = lanes_sum<L>(wg);
   total = lanes_sum<L>(total);
+  const float lift = lift_of(total);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the row is its own lanes' only, and they are in one wave
 #pragma unroll
   for (int r = 0; r < KR; ++r) {
@@ -624,9 +644,13 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteParams p) {
     if (soft && p.renorm) value = w[r] * (g[r] - (p.scale != 0.0f ? wg / p.scale : 0.0f));
     else if (soft) value = w[r] * g[r];                    // s ds: weight is scale s
     else {
-      float ds = p.scale * g[r];
-      if (p.renorm) ds = total > 0.0f ? p.scale * (g[r] - wg / total) / total : 0.0f;
-      value = ds * s[r] * (1.0f - s[r]);
+      float ds = p.scale * g[r], share = s[r];
+      if (p.renorm) {
+        const float by = total > 0.0f ? 1.0f / (total * lift) : 0.0f;
+        ds = p.scale * (g[r] - wg * lift * by);
+        share = s[r] * lift * by;
+      }
+      value = ds * share * (1.0f - s[r]);
     }
     if (id[r] >= 0) ((float*)mine)[id[r]] = value;
   }
