@@ -154,8 +154,9 @@ class MXTensor:
     def from_codes(codes: torch.Tensor, scales: torch.Tensor, k: int, dim: int = -1) -> "MXTensor":
         """From the form of checkpoints: ``codes[..., rows, ceil(k / 2)]`` (two a byte, the even element low) and
         ``scales[..., rows, ceil(k / 32)]`` (exponent + 127), uint8, quantised along ``k``.  ``dim=-1`` gives a tensor of shape
-        ``[..., rows, k]``, ``dim=-2`` its transpose ``[..., k, rows]``, the right operand of a product.  The data is copied."""
-        dim = _dim("MXTensor.from_codes", dim)
+        ``[..., rows, k]``, ``dim=-2`` its transpose ``[..., k, rows]``, the right operand of a product; from 0 on it counts the dimensions of that
+        shape, as in ``mx_quantize``.  The data is copied."""
+        dim = _dim("MXTensor.from_codes", dim, max(codes.dim(), 2))
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise ValueError("MXTensor.from_codes: codes and scales are uint8")
         if codes.dim() not in (2, 3) or k < 1 or codes.shape[-1] != -(-k // 2) or tuple(scales.shape) != (*codes.shape[:-1], -(-k // BLOCK)):
