@@ -41,7 +41,7 @@ class Routing:
     order: torch.Tensor
     rows: torch.Tensor
     num_experts: int
-    scoring: str = "softmax"
+    scoring: Optional[str] = "softmax"         # None: the choice was made elsewhere (moe_plan), its scores are not known
     renormalize: bool = True
     scale: float = 1.0
 
@@ -100,7 +100,7 @@ def moe_plan(experts: torch.Tensor, weights: torch.Tensor, num_experts: int) -> 
     ws = _scratch(a, tokens, top_k, num_experts, experts.device)
     launch("moe_plan", index, _C.load().tnx_moe_plan, a)
     del ws
-    return Routing(weights, experts, offsets, order, rows, num_experts)
+    return Routing(weights, experts, offsets, order, rows, num_experts, scoring=None)
 
 
 def _route_args(logits: torch.Tensor, bias: Optional[torch.Tensor], top_k: int, options) -> _C.MoeArgs:
@@ -209,6 +209,8 @@ def _backward(grad, logits, weights, experts, options):
 
 def moe_route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, routing: Routing) -> torch.Tensor:
     """Gradient of the logits from that of ``routing.weights``, for the ``routing`` that ``moe_route`` made of these logits."""
+    if routing.scoring not in _SCORING:
+        raise ValueError("moe_route_backward: the routing of moe_plan has weights from elsewhere, whose gradient of logits is not known")
     if tuple(grad_weights.shape) != (routing.tokens, routing.top_k) or logits.dim() != 2 or tuple(logits.shape) != (routing.tokens, routing.num_experts):
         raise ValueError(f"moe_route_backward: gradient {tuple(grad_weights.shape)} and logits {tuple(logits.shape)} are not of this routing "
                          f"({routing.tokens} tokens, {routing.top_k} of {routing.num_experts} experts)")
