@@ -406,6 +406,15 @@ size_t tnx_mx_gemm_workspace_bytes(const tnx_mx_gemm_args* args);
 
 int tnx_mx_gemm(const tnx_mx_gemm_args* args);
 
+/* For tests and tooling: which kernels tnx_mx_gemm runs for these args (of the pointers it counts which are given and how they are aligned), or 0
+ * where it would refuse them or has nothing to do.  info (may be NULL): columns and rows of a tile, slabs of 256 k that its ring holds (0: the weights do not
+ * go through LDS), and parts that k is cut in by a launch that adds them up. */
+enum tnx_mx_route {
+  TNX_MX_ROUTE_STREAM = 1,      /* a wave per 16 rows of b and 16 rows of the product */
+  TNX_MX_ROUTE_TILES = 2
+};
+int tnx_mx_gemm_route(const tnx_mx_gemm_args* args, int32_t info[4]);
+
 /* ------------------------------------------------------------------------------------------------------------------
  * Routing of tokens to experts.
  *

@@ -39,7 +39,7 @@ EXPORTS = ("tnx_gemm", "tnx_gemm_static_workspace", "tnx_gemm_workspace_bytes", 
            "tnx_conv2d_packed_info", "tnx_conv2d_packed_forward", "tnx_conv2d_route", "tnx_conv2d_supported",
            "tnx_conv2d_output_size",
            "tnx_conv2d_default_config", "tnx_conv2d_kernel_count", "tnx_conv2d_kernel_name",
-           "tnx_mx_code_bytes", "tnx_mx_scale_bytes", "tnx_mx_quantize", "tnx_mx_quantize_both", "tnx_mx_dequantize", "tnx_mx_import", "tnx_mx_gemm", "tnx_mx_gemm_workspace_bytes", "tnx_mx_gemm_takes_rows",
+           "tnx_mx_code_bytes", "tnx_mx_scale_bytes", "tnx_mx_quantize", "tnx_mx_quantize_both", "tnx_mx_dequantize", "tnx_mx_import", "tnx_mx_gemm", "tnx_mx_gemm_workspace_bytes", "tnx_mx_gemm_takes_rows", "tnx_mx_gemm_route",
            "tnx_moe_workspace_bytes", "tnx_moe_route", "tnx_moe_plan", "tnx_moe_route_backward", "tnx_moe_combine")
 # limits of the routing entry points
 MOE_MAX_EXPERTS, MOE_MAX_TOP_K, MOE_MAX_GROUPS = 1024, 32, 64
@@ -192,6 +192,7 @@ def load() -> ctypes.CDLL:
             ("tnx_mx_import", [ptr, ptr, i64, i64, i64, ptr, ptr, ptr], ctypes.c_int),
             ("tnx_mx_gemm_takes_rows", [i64, i64], ctypes.c_int), ("tnx_mx_gemm", [ctypes.POINTER(MxGemmArgs)], ctypes.c_int),
             ("tnx_mx_gemm_workspace_bytes", [ctypes.POINTER(MxGemmArgs)], ctypes.c_size_t),
+            ("tnx_mx_gemm_route", [ctypes.POINTER(MxGemmArgs), ctypes.POINTER(i32)], ctypes.c_int),
             ("tnx_moe_workspace_bytes", [i64, i32, i32], ctypes.c_size_t), ("tnx_moe_route", [ctypes.POINTER(MoeArgs)], ctypes.c_int),
             ("tnx_moe_plan", [ctypes.POINTER(MoeArgs)], ctypes.c_int), ("tnx_moe_route_backward", [ctypes.POINTER(MoeArgs)], ctypes.c_int),
             ("tnx_moe_combine", [ptr, ptr, ptr, ptr, i64, i32, i64, i32, i32, ptr], ctypes.c_int)):

@@ -758,19 +758,48 @@ template <bool EXPERTS> struct Shape {
   }
 };
 
+typedef MxTile<256, 256, 4, 2, 2> Tile256;
+typedef MxTile<64, 64, 2, 2, 4> Tile64;
+typedef MxTile<128, 128, 4, 2, 4> Tile128Deep;
+typedef MxTile<128, 128, 2, 2, 2> Tile128;
+typedef MxTile<128, 32, 4, 1, 2> Tile32;                 // (experts only)
+
 template <bool EXPERTS> int launch(const MxParams& p, bool raw, void* sums, size_t room, hipStream_t stream) {
   const Shape<EXPERTS> shape{p.m, p.n, p.slabs, p.experts};
   if (raw) return shape.most(16) <= 65535 ? launch_few<EXPERTS, true>(p, shape.most(16), stream) : TNX_E_UNSUPPORTED;
   const Choice c = shape.choose(sums ? room : 0);
   switch (c.kind) {
-    case TILE_256: return launch_tile<MxTile<256, 256, 4, 2, 2>, EXPERTS>(p, shape.most(256), stream);
-    case TILE_64: return launch_tile<MxTile<64, 64, 2, 2, 4>, EXPERTS>(p, shape.most(64), stream, c.parts, sums);
-    case TILE_128_DEEP: return launch_tile<MxTile<128, 128, 4, 2, 4>, EXPERTS>(p, shape.most(128), stream, c.parts, sums);
-    case TILE_128: return launch_tile<MxTile<128, 128, 2, 2, 2>, EXPERTS>(p, shape.most(128), stream);
+    case TILE_256: return launch_tile<Tile256, EXPERTS>(p, shape.most(256), stream);
+    case TILE_64: return launch_tile<Tile64, EXPERTS>(p, shape.most(64), stream, c.parts, sums);
+    case TILE_128_DEEP: return launch_tile<Tile128Deep, EXPERTS>(p, shape.most(128), stream, c.parts, sums);
+    case TILE_128: return launch_tile<Tile128, EXPERTS>(p, shape.most(128), stream);
     default: break;
   }
-  if constexpr (EXPERTS) return launch_tile<MxTile<128, 32, 4, 1, 2>, true>(p, shape.most(32), stream);
+  if constexpr (EXPERTS) return launch_tile<Tile32, true>(p, shape.most(32), stream);
   else return launch_few<false, false>(p, shape.most(16), stream);
+}
+
+// what launch() does, and tnx_mx_gemm_route's answer
+template <bool EXPERTS> int route(const MxParams& p, bool raw, void* sums, size_t room, int32_t info[4]) {
+  const Shape<EXPERTS> shape{p.m, p.n, p.slabs, p.experts};
+  const Choice c = raw ? Choice{FEW, 1} : shape.choose(sums ? room : 0);
+  auto tile = [&](auto t) {
+    typedef typename decltype(t)::type C;
+    const int per = parts_slabs(p.slabs, c.parts);
+    info[0] = C::BN; info[1] = C::BM; info[2] = C::S;
+    info[3] = c.parts > 1 ? (p.slabs + per - 1) / per : 1;
+    return TNX_MX_ROUTE_TILES;
+  };
+  switch (c.kind) {
+    case TILE_256: return tile(TypeTag<Tile256>());
+    case TILE_64: return tile(TypeTag<Tile64>());
+    case TILE_128_DEEP: return tile(TypeTag<Tile128Deep>());
+    case TILE_128: return tile(TypeTag<Tile128>());
+    case TILE_32: return tile(TypeTag<Tile32>());
+    default: break;
+  }
+  info[0] = info[1] = 16; info[2] = 0; info[3] = 1;
+  return shape.most(16) <= 65535 ? TNX_MX_ROUTE_STREAM : 0;
 }
 
 bool takes_rows(int64_t a_rows, int64_t k) {
@@ -787,7 +816,10 @@ extern "C" size_t tnx_mx_gemm_workspace_bytes(const tnx_mx_gemm_args* a) {
   return parts_bytes(a->m, a->n, shape.choose(MAX_PARTS_BYTES).parts);
 }
 
-extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
+namespace {
+
+// the arguments' checks and the kernels' parameters
+int prepare(const tnx_mx_gemm_args* a, MxParams* params) {
   if (!a || a->m < 0 || a->n < 0 || a->k < 0 || a->experts < 0 || a->epilogue < TNX_EPI_NONE || a->epilogue > TNX_EPI_GLU_IDENTITY) return TNX_E_INVALID;
   if (a->m == 0 || a->n == 0) return TNX_OK;
   if (a->out_dtype != TNX_BF16 && a->out_dtype != TNX_F16 && a->out_dtype != TNX_F32) return TNX_E_UNSUPPORTED;
@@ -805,7 +837,7 @@ extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
   } else if (!a->a_codes || !a->a_scales || (((uintptr_t)a->a_codes | (uintptr_t)a->a_scales) & 15)) return TNX_E_INVALID;
   if (a->experts > 0 ? (!a->offsets || a->experts > TNX_MOE_MAX_EXPERTS) : (a->offsets || a->order)) return TNX_E_INVALID;
   if (a->order ? (a->top_k < 1 || a->a_rows < 1) : a->a_rows != a->m) return TNX_E_INVALID;
-  MxParams p;
+  MxParams& p = *params;
   p.a = (const uint8_t*)(raw ? a->a_data : a->a_codes); p.as = (const uint8_t*)a->a_scales;
   p.b = (const uint8_t*)a->b_codes; p.bs = (const uint8_t*)a->b_scales;
   p.out = (uint8_t*)a->out;
@@ -819,6 +851,26 @@ extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
   p.out_dtype = a->out_dtype; p.epi = a->epilogue;
   p.a_dtype = a->a_dtype; p.lda = a->stride_a; p.k = (int)a->k; p.wk_log = 0; p.part_slabs = p.slabs; p.stream_b = false;
   if (a->workspace && ((uintptr_t)a->workspace & 15)) return TNX_E_INVALID;
-  const size_t room = a->workspace_bytes < MAX_PARTS_BYTES ? a->workspace_bytes : MAX_PARTS_BYTES;
-  return a->experts > 0 ? launch<true>(p, raw, nullptr, 0, (hipStream_t)a->stream) : launch<false>(p, raw, a->workspace, room, (hipStream_t)a->stream);
+  return TNX_OK;
+}
+
+size_t room_of(const tnx_mx_gemm_args* a) { return a->workspace_bytes < MAX_PARTS_BYTES ? a->workspace_bytes : MAX_PARTS_BYTES; }
+
+}  // namespace
+
+extern "C" int tnx_mx_gemm(const tnx_mx_gemm_args* a) {
+  MxParams p;
+  const int status = prepare(a, &p);
+  if (status != TNX_OK || a->m == 0 || a->n == 0) return status;
+  const bool raw = a->a_data != nullptr;
+  const hipStream_t stream = (hipStream_t)a->stream;
+  return a->experts > 0 ? launch<true>(p, raw, nullptr, 0, stream) : launch<false>(p, raw, a->workspace, room_of(a), stream);
+}
+
+extern "C" int tnx_mx_gemm_route(const tnx_mx_gemm_args* a, int32_t info[4]) {
+  MxParams p;
+  int32_t unused[4];
+  if (prepare(a, &p) != TNX_OK || a->m == 0 || a->n == 0) return 0;
+  const bool raw = a->a_data != nullptr;
+  return a->experts > 0 ? route<true>(p, raw, nullptr, 0, info ? info : unused) : route<false>(p, raw, a->workspace, room_of(a), info ? info : unused);
 }
