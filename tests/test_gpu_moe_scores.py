@@ -84,3 +84,17 @@ def test_shares_of_rows_with_masked_experts(device):
         weights, experts = ref.route(logits, 4, bias=bias, renormalize=renormalize)
         np.testing.assert_array_equal(r.experts.cpu().numpy(), experts)
         np.testing.assert_allclose(r.weights.cpu().double().numpy(), weights, rtol=REL, atol=2.0 ** -126)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tokens", [2, 1100])
+def test_the_lowest_value_is_no_score(device, dtype, scoring, tokens):
+    """Experts masked by the type's lowest value that a bias chooses all the same: weight zero, alone and beside one that has a score."""
+    logits = separated(tokens, 16, torch.float32, 3).to(dtype)
+    logits[:, 8:] = torch.finfo(dtype).min
+    bias = torch.zeros(16)
+    bias[8:12] = 3.0
+    check_route(device, logits, 4, scoring=scoring, bias=bias)
+    r = check_route(device, logits, 5, scoring=scoring, bias=bias)
+    assert bool((r.weights[:, :4] == 0).all()) and bool((r.weights[:, 4] == 1).all())

@@ -379,8 +379,12 @@ __device__ __forceinline__ void route_tokens(const RouteParams& p, int tid, int6
   if (shares) {
     most = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < KR; ++r) most = __builtin_fmaxf(most, w[r]);
+    for (int r = 0; r < KR; ++r) {
+      if (w[r] - off < -745.0f) w[r] = -INFINITY;          // (masked by the type's lowest value: no score, in 64 bits neither)
+      most = __builtin_fmaxf(most, w[r]);
+    }
     most = lanes_max<L>(most);
+    if (most == -INFINITY) most = 0.0f;
     inv = 1.0f;
   }
 #pragma unroll
