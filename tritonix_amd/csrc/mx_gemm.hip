@@ -493,8 +493,8 @@ __global__ __launch_bounds__(C::THREADS, C::OCC < 2 ? C::OCC : 2) void mx_tile_k
 // a turn's loads are in flight together.  16x16x128 instructions: lane group g (lane / 16) takes the blocks 2 g and 2 g + 1 of a slab, 32 neighbouring
 // bytes and two neighbouring scales.
 //
-// RAW: the rows of a as 16- or 32-bit floats: every workgroup quantises them into LDS while its first weights are on their way, 4096 elements in about
-// 0.5 us, which saves a launch of 3 us and its gap.  In one launch and in two: 4096 x 4096 of 1, 4 and 8 rows 5.1, 6.7 and 8.6 us, 10.1 to 10.2;
+// RAW: the rows of a as 16- or 32-bit floats: every workgroup quantises them into LDS, 4096 elements in about 0.5 us, which saves a launch of 3 us and its
+// gap.  (They are asked for after the first turn's weights and arrive behind them: loads come back in order.)  In one launch and in two: 4096 x 4096 of 1, 4 and 8 rows 5.1, 6.7 and 8.6 us, 10.1 to 10.2;
 // 14336 x 4096 8.8, 11.1 and 14.2, 11.8 to 11.1; 4096 x 7000 6.9, 9.4 and 12.9, 8.9 to 9.3: up to 16384 elements, or one row.
 constexpr int FEW_WAVES = 8, FEW_RAW_ROWS = 16, FEW_RAW_K = 30720, FEW_RAW_ELEMENTS = 16384;
 // bytes of such a row: 16 more than its codes, so that the rows' chunks fall on different banks, and its scales
@@ -739,14 +739,15 @@ template <bool EXPERTS> struct Shape {
       // them 84 and 92.
       offer(TILE_32, 1, tiles_us(expect(32) * cols(128), 768, 1.2, 1.2, 2.5, slabs));
     } else {
-      // The streaming kernel: a slab of a workgroup's eight waves is 35 kB of weights and rows, and a CU brings that in 1 us, however few of
-      // them are busy.  So it is for few rows, or few columns, and it shares k out.  40 x 64 x 9630: 7.7 us, tiles of 64 13.7; 8 x 4096 x 4096 4.6 and 7.4;
-      // 64 x 1024 x 4096 5.0 and 7.8, 128 rows 7.1 and 7.4; 256 x 256 x 16384 12 and 23; 48 x 4096 x 4096 11.6 and 7.6.
+      // The streaming kernel: a slab of a workgroup's eight waves is 35 kB of weights and rows, which it brings in 1 us, however few CUs are
+      // busy (a turn waits for all of its loads; a ring, which has some ahead, brings as much in half of that).  So it is for few rows, or few columns, and it shares
+      // k out.  40 x 64 x 9630: 7.6 us, tiles of 64 13.7; 8 x 4096 x 4096 4.5 and 7.4; 64 x 1024 x 4096 4.9 and 7.8, 128 rows 7.0 and 7.4; 256 x 256 x
+      // 16384 11.2 and 23; 48 x 4096 x 4096 11.6 and 7.2.
       const int64_t outputs = cols(16) * most(16);
       const int log = few_parts(outputs, slabs);
       if (most(16) <= 65535) offer(FEW, 1, 2.7 + (double)(((outputs << log) + 256 * FEW_WAVES - 1) / (256 * FEW_WAVES) * ((slabs + (1 << log) - 1) >> log)));
-      // Few tiles of many slabs: k in parts, a workgroup each, and a second launch that adds them up.  100 x 4096 x 14336 20.7 us, in 4 parts 15.0; 128 x 1024 x
-      // 16384 20.6, in 8 11.6; 64 x 64 x 30000 18.7 and 11.7; 64 x 4096 x 8192 13.6, in 4 11.4, 128 rows 13.1, in 2 13.5.
+      // Few tiles of many slabs: k in parts, a workgroup each, and a second launch that adds them up.  100 x 4096 x 14336 20.7 us, in 4 parts 14.5; 128 x 1024 x
+      // 16384 19.7, in 8 10.8; 64 x 64 x 30000 18.4 and 10.9; 64 x 4096 x 8192 12.4, in 4 10.1, 128 rows 12.7, in 2 13.5.
       for (int parts = 2; parts <= 8; ++parts) {
         if (slabs < 4 * parts || parts_bytes(m, n, parts) > room) break;
         const double join = 5.0 + (double)parts_bytes(m, n, parts) / 2e6;

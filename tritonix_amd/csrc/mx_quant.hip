@@ -398,7 +398,8 @@ __global__ __launch_bounds__(256) void import_kernel(const uint8_t* codes, const
 }
 
 // Whether the wide shape has a workgroup for every CU, or for every other of float32, whose lanes have half the work.  (Quantising, small and wide: bfloat16 3000 x 2001,
-// 96 workgroups, 6.3 and 9.1 us, 4096 x 4096, 256 of them, 10.3 and 10.2; float32 1024 x 2048, 64, 4.1 and 4.8, 2048 x 2048, 128, 5.8 and 5.3.)
+// 96 workgroups, 6.3 and 9.1 us, 4096 x 4096, 256 of them, 10.3 and 10.2; float32 1024 x 2048, 64, 4.1 and 4.8, 2048 x 2048, 128, 5.8 and 5.3.  The way back
+// takes the same shape.)
 template <class T> bool columns_wide(int64_t rows, const QuantParams& p) {
   typedef Columns<T, true> C;
   return (rows + C::ROWS - 1) / C::ROWS * p.slabs * p.batch >= 64 * C::LANE;
