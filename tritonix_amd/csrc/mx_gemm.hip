@@ -129,7 +129,7 @@ template <bool ROUNDED, bool SHORT> __device__ __forceinline__ float gated(float
     const float s = ROUNDED ? reciprocal_from_one(d) : 1.0f / d;
     v = (epi == EPI_GLU_IDENTITY ? 1.0f : s) * (epi == EPI_GLU_SIGMOID ? 1.0f : g) * l;
   }
-  if (ROUNDED) asm("" : "+v"(v));
+  asm("" : "+v"(v));
   return v;
 }
 
@@ -138,9 +138,8 @@ __device__ __forceinline__ void store_columns(const MxParams& p, int64_t row, in
   float o[4];
   int c = col, n = 4;
   if (p.epi != EPI_NONE) {
-    const bool rounded = p.out_dtype != DT_F32;
-    o[0] = rounded ? gated<true, false>(v[0], v[1], p.epi) : gated<false, false>(v[0], v[1], p.epi);
-    o[1] = rounded ? gated<true, false>(v[2], v[3], p.epi) : gated<false, false>(v[2], v[3], p.epi);
+    o[0] = gated<false, false>(v[0], v[1], p.epi);         // (few of them: the division for every type)
+    o[1] = gated<false, false>(v[2], v[3], p.epi);
     o[2] = o[3] = 0.0f;
     c = col >> 1; n = 2; cols >>= 1;
   } else {
