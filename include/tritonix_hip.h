@@ -466,6 +466,124 @@ int tnx_moe_route_backward(const tnx_moe_args* args);
 int tnx_moe_combine(const void* y, const int32_t* rows, const float* weights, void* out, int64_t tokens, int32_t top_k, int64_t n,
                     int32_t y_dtype, int32_t out_dtype, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Linear layers.
+ *
+ * z[m, n] = x[m, k] w[k, n] + bias[n],  y = act(z) + residual.  Sums in 32 bits (float32 operands: as tnx_gemm_f32), each output rounded
+ * once.  residual, y and z are row-major without gaps, of `dtype`; bias is of `dtype` or float32.  x and w take any strides; rows of x with w row-major or
+ * k-contiguous (stride_wk == 1, the transpose of a row-major weight) are the fast layouts.  Without bias, residual, z and activation it is a
+ * product, with x also contiguous along m (stride_xm == 1): the gradients dx = dz w^T and dw = x^T dz. */
+enum tnx_activation {
+  TNX_ACT_NONE = 0,
+  TNX_ACT_RELU = 1,
+  TNX_ACT_SILU = 2,            /* z / (1 + e^-z) */
+  TNX_ACT_GELU = 3,            /* z (1 + erf(z / sqrt 2)) / 2 */
+  TNX_ACT_GELU_TANH = 4        /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+};
+
+typedef struct tnx_linear_args {
+  const void *x, *w;
+  const void* bias;            /* or null */
+  const void* residual;        /* or null */
+  void* y;
+  void* z;                     /* or null: not wanted */
+  int64_t m, n, k;
+  int64_t stride_xm, stride_xk, stride_wk, stride_wn;
+  int32_t dtype;               /* TNX_F16, TNX_BF16 or TNX_F32 */
+  int32_t bias_dtype;
+  int32_t activation;          /* tnx_activation */
+  int32_t reserved;
+  void* workspace;             /* tnx_linear_workspace_bytes, 256-byte aligned; its first TNX_WS_COUNTER_BYTES zero when first used, and left zero */
+  size_t workspace_bytes;
+  void* scratch;               /* tnx_linear_scratch_bytes, 256-byte aligned, no initialisation */
+  size_t scratch_bytes;
+  void* stream;
+} tnx_linear_args;
+
+/* Both depend on sizes, strides, types, the alignment of x and w, and on whether there is an epilogue (z counts as one).  Calls that share a
+ * workspace or scratch must be ordered. */
+size_t tnx_linear_workspace_bytes(const tnx_linear_args* args);
+size_t tnx_linear_scratch_bytes(const tnx_linear_args* args);
+int tnx_linear(const tnx_linear_args* args);
+
+/* For tests and tooling: how tnx_linear runs these args, or 0 where it would refuse them or has nothing to do.  info (may be NULL): rows and
+ * columns of a tile, waves, ring slots, slices of k. */
+enum tnx_linear_route {
+  TNX_LINEAR_ROUTE_PRODUCT = 1,   /* no epilogue */
+  TNX_LINEAR_ROUTE_FUSED = 2,     /* the epilogue in the product's kernel */
+  TNX_LINEAR_ROUTE_APART = 3      /* a launch of its own on sums in 32 bits */
+};
+int tnx_linear_route(const tnx_linear_args* args, int32_t info[5]);
+
+/* dz = dy act'(z), and dbias, the sums of dz's columns (32-bit sums of unrounded dz, in an order that depends on the sizes alone).  All [m, n]
+ * row-major without gaps.  Either of dz and dbias may be null; without an activation z is not read. */
+typedef struct tnx_linear_gradient_args {
+  const void *dy, *z;
+  void *dz, *dbias;
+  int64_t m, n;
+  int32_t dtype, bias_dtype, activation, reserved;
+  void* workspace;             /* tnx_linear_gradient_bytes, 16-byte aligned, no initialisation */
+  size_t workspace_bytes;
+  void* stream;
+} tnx_linear_gradient_args;
+size_t tnx_linear_gradient_bytes(const tnx_linear_gradient_args* args);
+int tnx_linear_gradient(const tnx_linear_gradient_args* args);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Layer normalisation by rows: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(variance + eps), the variance being the mean square
+ * of x - mean.  In 32 bits throughout, outputs rounded once.  weight and bias (either or both may be null) are of `dtype` or float32.
+ *
+ * The backward pass takes mean and rstd as the forward pass wrote them: dx, and dweight and dbias of the parameters' types (each may be
+ * null), summed over the rows in an order that depends on the sizes alone. */
+typedef struct tnx_norm_args {
+  const void *x, *weight, *bias;
+  void* y;                     /* [rows, n] without gaps */
+  float *mean, *rstd;          /* [rows]; both null in a forward pass that no backward pass follows */
+  const void* dy;
+  void *dx, *dweight, *dbias;  /* dx [rows, n] without gaps */
+  int64_t rows, n;
+  int64_t stride_x, stride_dy; /* elements from row to row (columns are neighbours) */
+  int32_t dtype, weight_dtype, bias_dtype;
+  float eps;
+  void* workspace;             /* backward: tnx_layer_norm_workspace_bytes, 16-byte aligned, no initialisation */
+  size_t workspace_bytes;
+  void* stream;
+} tnx_norm_args;
+int tnx_layer_norm(const tnx_norm_args* args);
+size_t tnx_layer_norm_workspace_bytes(const tnx_norm_args* args);
+int tnx_layer_norm_backward(const tnx_norm_args* args);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Products grouped by ragged runs of rows.  Group g has the rows offsets[g] <= r < offsets[g + 1] (device memory, groups + 1 entries; bounds
+ * outside of [0, rows] are taken as the nearest inside, and one below an earlier one as that one).
+ *
+ * TNX_GROUPED_ROWS             c[r, n] = a[r, k] b[g][k, n]; rows of no group are written as zeros
+ * TNX_GROUPED_WEIGHT_GRADIENT  c[g][k, n] = sum over the group's rows of a[r, k] b[r, n]; zeros for a group without rows
+ *
+ * 32-bit sums (float32 on the binary32 matrix instruction), rounded once.  a has neighbouring columns (stride_ak == 1, stride_ar >= k).  b: row-major
+ * (stride_bn == 1) or, in the first form, k-contiguous matrices (stride_bk == 1); in the second form rows of n, stride_bk apart.  c has no gaps.
+ * Operands whose rows are too short for the loads (n, and in the second form k, of less than a 16-byte chunk) are refused with
+ * TNX_E_UNSUPPORTED. */
+#define TNX_GROUPED_MAX_GROUPS 4096
+enum tnx_grouped_form { TNX_GROUPED_ROWS = 0, TNX_GROUPED_WEIGHT_GRADIENT = 1 };
+
+typedef struct tnx_grouped_args {
+  const void *a, *b;
+  void* c;
+  const int32_t* offsets;
+  int64_t rows, n, k;
+  int64_t stride_ar, stride_ak;
+  int64_t stride_group;        /* elements from one group's matrix to the next: of b, in the second form of c (k * n) */
+  int64_t stride_bk, stride_bn;
+  int32_t groups, dtype, form, reserved;
+  int32_t block_m, block_n;    /* a built tile, or 0: the library chooses */
+  void* stream;
+} tnx_grouped_args;
+int tnx_grouped(const tnx_grouped_args* args);
+/* For tests and tooling: 1, or 0 where tnx_grouped would refuse these args (of the pointers only the alignment counts).  info (may be NULL): rows and
+ * columns of a tile, waves, whether each group's last slab of k is loaded apart. */
+int tnx_grouped_route(const tnx_grouped_args* args, int32_t info[4]);
+
 #ifdef __cplusplus
 }
 #endif

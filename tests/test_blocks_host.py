@@ -1,0 +1,137 @@
+"""Linear layers, layer normalisation and grouped products without a GPU: what is refused, and the host's choices."""
+import ctypes
+import itertools
+
+import pytest
+import torch
+
+import tritonix
+from tritonix_amd import _C
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def t(*shape, dtype=BF16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("call,text", [
+    (lambda: tritonix.linear(t(4, 8), t(9, 6)), "expects"),
+    (lambda: tritonix.linear(t(4, 8), t(8)), "expects"),
+    (lambda: tritonix.linear(t(4, 8), t(2, 8, 6)), "expects"),
+    (lambda: tritonix.linear(t(), t(8, 6)), "expects"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6, dtype=F16)), "float16"),
+    (lambda: tritonix.linear(t(4, 8, dtype=torch.int8), t(8, 6, dtype=torch.int8)), "int8"),
+    (lambda: tritonix.linear(t(4, 8, dtype=torch.float64), t(8, 6, dtype=torch.float64)), "float64"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6), t(8)), "bias"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6), t(1, 6)), "bias"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6), t(6, dtype=F16)), "bias"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6), residual=t(6)), "residual"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6), residual=t(1, 6)), "residual"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6), residual=t(4, 6, dtype=F32)), "residual"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6), activation="tanh"), "activation"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6), activation="none"), "activation"),
+    (lambda: tritonix.linear(t(4, 8), t(8, 6)), "HIP device"),
+    (lambda: tritonix.layer_norm(t(4, 8), t(7)), "weight"),
+    (lambda: tritonix.layer_norm(t(4, 8), t(8, dtype=F16)), "weight"),
+    (lambda: tritonix.layer_norm(t(4, 8), t(8), t(4, 8)), "bias"),
+    (lambda: tritonix.layer_norm(t(4, 8, dtype=torch.int32)), "int32"),
+    (lambda: tritonix.layer_norm(t(4, 8), eps=-1e-5), "eps"),
+    (lambda: tritonix.layer_norm(t(4, 8), eps=float("nan")), "eps"),
+    (lambda: tritonix.layer_norm(t()), "scalar"),
+    (lambda: tritonix.layer_norm(t(4, 8)), "HIP device"),
+    (lambda: tritonix.grouped_matmul(t(4, 8), t(2, 9, 6), t(3, dtype=torch.int32)), "expects"),
+    (lambda: tritonix.grouped_matmul(t(4, 8), t(8, 6), t(3, dtype=torch.int32)), "expects"),
+    (lambda: tritonix.grouped_matmul(t(1, 4, 8), t(2, 8, 6), t(3, dtype=torch.int32)), "expects"),
+    (lambda: tritonix.grouped_matmul(t(4, 8), t(2, 8, 6), t(2, dtype=torch.int32)), "offsets"),
+    (lambda: tritonix.grouped_matmul(t(4, 8), t(2, 8, 6), t(3, dtype=F32)), "offsets"),
+    (lambda: tritonix.grouped_matmul(t(4, 8), t(2, 8, 6, dtype=F16), t(3, dtype=torch.int32)), "float16"),
+    (lambda: tritonix.grouped_matmul(t(4, 8), t(0, 8, 6), t(1, dtype=torch.int32)), "groups"),
+    (lambda: tritonix.grouped_matmul(t(1, 1), t(4097, 1, 1), t(4098, dtype=torch.int32)), "groups"),
+    (lambda: tritonix.grouped_matmul(t(4, 8), t(2, 8, 6), t(3, dtype=torch.int32)), "HIP device"),
+])
+def test_refusals(call, text):
+    with pytest.raises(ValueError, match=text):
+        call()
+
+
+def linear_args(m, n, k, dtype=_C.BF16, layout="nn", epilogue=True):
+    a = _C.LinearArgs()
+    a.x, a.w = 1 << 20, 1 << 21                              # (only their alignment counts)
+    a.m, a.n, a.k, a.dtype, a.bias_dtype = m, n, k, dtype, dtype
+    a.stride_xm, a.stride_xk = k, 1
+    a.stride_wk, a.stride_wn = (n, 1) if layout == "nn" else (1, k)
+    a.activation = _C.ACT_SILU if epilogue else _C.ACT_NONE
+    return a
+
+
+@pytest.mark.parametrize("dtype", [_C.BF16, _C.F16, _C.F32])
+@pytest.mark.parametrize("layout", ["nn", "nt"])
+def test_every_choice_of_tile_has_the_epilogue(dtype, layout):
+    lib = _C.load()
+    tiles = set()
+    for m, n, k in itertools.product((1, 7, 16, 33, 64, 65, 100, 200, 300, 513, 1000, 1600, 2500, 4096, 8192), (16, 64, 96, 130, 500, 768, 1111, 2048, 3000, 4096, 14336),
+                                     (8, 64, 72, 200, 512, 1000, 2048, 4096, 5000, 14336)):
+        info = (ctypes.c_int32 * 5)()
+        assert lib.tnx_linear_route(ctypes.byref(linear_args(m, n, k, dtype, layout)), info) == _C.LINEAR_ROUTE_FUSED, (m, n, k, list(info))
+        tiles.add(tuple(info[:4]))
+    assert len(tiles) >= (5 if dtype == _C.F32 else 12), tiles
+
+
+def test_routes_of_a_linear_layer():
+    lib = _C.load()
+    route = lambda a: lib.tnx_linear_route(ctypes.byref(a), None)  # noqa: E731
+    assert route(linear_args(100, 200, 300, epilogue=False)) == _C.LINEAR_ROUTE_PRODUCT
+    a = linear_args(100, 200, 304)
+    a.stride_xm, a.stride_xk = 1, 100                         # contiguous along m
+    assert route(a) == _C.LINEAR_ROUTE_APART and lib.tnx_linear_scratch_bytes(ctypes.byref(a)) >= 100 * 200 * 4
+    assert route(linear_args(100, 200, 0)) == _C.LINEAR_ROUTE_APART
+    assert route(linear_args(0, 200, 300)) == 0
+    bad = linear_args(100, 200, 300)
+    bad.activation = 5
+    assert route(bad) == 0 and lib.tnx_linear(ctypes.byref(bad)) == _C.E_INVALID
+    other = linear_args(100, 200, 300, dtype=_C.I8)
+    assert lib.tnx_linear(ctypes.byref(other)) == _C.E_UNSUPPORTED
+    bias = linear_args(100, 200, 300)
+    bias.bias, bias.bias_dtype, bias.y = 1 << 20, _C.F16, 1 << 20
+    assert lib.tnx_linear(ctypes.byref(bias)) == _C.E_UNSUPPORTED
+    cut = linear_args(16, 512, 8192)
+    cut.y = 1 << 20
+    assert lib.tnx_linear_workspace_bytes(ctypes.byref(cut)) > _C.WS_COUNTER_BYTES and lib.tnx_linear(ctypes.byref(cut)) == _C.E_WORKSPACE
+    assert lib.tnx_linear(None) == _C.E_INVALID
+
+
+def test_entry_points_refuse():
+    lib = _C.load()
+    a = _C.NormArgs(rows=4, n=8, dtype=_C.I8)
+    assert lib.tnx_layer_norm(ctypes.byref(a)) == _C.E_UNSUPPORTED
+    a = _C.NormArgs(x=4096, y=4096, rows=4, n=8, dtype=_C.BF16, weight=4096, weight_dtype=_C.F16)
+    assert lib.tnx_layer_norm(ctypes.byref(a)) == _C.E_UNSUPPORTED
+    a = _C.NormArgs(x=4096, y=4096, rows=4, n=8, dtype=_C.BF16, mean=4096)          # one of the statistics without the other
+    assert lib.tnx_layer_norm(ctypes.byref(a)) == _C.E_INVALID
+    a = _C.NormArgs(rows=4, n=8, dtype=_C.BF16, eps=-1.0)
+    assert lib.tnx_layer_norm(ctypes.byref(a)) == _C.E_INVALID
+    a = _C.NormArgs(x=4096, dy=4096, mean=4096, rstd=4096, dx=4096, dweight=4096, rows=400, n=8, dtype=_C.BF16, weight_dtype=_C.BF16)
+    assert lib.tnx_layer_norm_workspace_bytes(ctypes.byref(a)) > 0 and lib.tnx_layer_norm_backward(ctypes.byref(a)) == _C.E_WORKSPACE
+    g = _C.LinearGradientArgs(dy=4096, dbias=4096, m=400, n=8, dtype=_C.BF16, bias_dtype=_C.BF16)
+    assert lib.tnx_linear_gradient_bytes(ctypes.byref(g)) > 0 and lib.tnx_linear_gradient(ctypes.byref(g)) == _C.E_WORKSPACE
+    g = _C.LinearGradientArgs(dy=4096, dz=4096, m=400, n=8, dtype=_C.BF16, activation=_C.ACT_SILU)
+    assert lib.tnx_linear_gradient(ctypes.byref(g)) == _C.E_INVALID                 # the derivative needs z
+
+
+def grouped_args(**more):
+    return _C.GroupedArgs(**{**dict(a=4096, b=4096, c=4096, offsets=4096, rows=100, n=64, k=64, stride_ar=64, stride_ak=1, stride_group=4096, stride_bk=64,
+                                    stride_bn=1, groups=3, dtype=_C.BF16), **more})
+
+
+def test_grouped_entry_point_refuses():
+    lib = _C.load()
+    for status, more in ((_C.E_INVALID, dict(form=2)), (_C.E_INVALID, dict(groups=0)), (_C.E_INVALID, dict(rows=-1)), (_C.E_INVALID, dict(offsets=None)),
+                         (_C.E_UNSUPPORTED, dict(dtype=_C.I8)), (_C.E_UNSUPPORTED, dict(groups=5000)), (_C.E_UNSUPPORTED, dict(stride_ak=2)),
+                         (_C.E_UNSUPPORTED, dict(stride_ar=63)), (_C.E_UNSUPPORTED, dict(stride_bn=2)), (_C.E_UNSUPPORTED, dict(block_m=96, block_n=96)),
+                         (_C.E_UNSUPPORTED, dict(form=_C.GROUPED_WEIGHT_GRADIENT, n=3, stride_bk=3)), (_C.E_UNSUPPORTED, dict(n=3, k=65, stride_ar=65, stride_bk=3))):
+        assert lib.tnx_grouped(ctypes.byref(grouped_args(**more))) == status, more
+    info = (ctypes.c_int32 * 4)()
+    assert lib.tnx_grouped_route(ctypes.byref(grouped_args()), info) == 1 and info[3] == 0
+    for more in (dict(k=63, stride_ar=63), dict(n=63, stride_bk=63), dict(a=4098), dict(b=4100), dict(stride_group=4097)):
+        assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**more)), info) == 1 and info[3] == 1, more

@@ -40,9 +40,19 @@ EXPORTS = ("tnx_gemm", "tnx_gemm_static_workspace", "tnx_gemm_workspace_bytes", 
            "tnx_conv2d_output_size",
            "tnx_conv2d_default_config", "tnx_conv2d_kernel_count", "tnx_conv2d_kernel_name",
            "tnx_mx_code_bytes", "tnx_mx_scale_bytes", "tnx_mx_quantize", "tnx_mx_quantize_both", "tnx_mx_dequantize", "tnx_mx_import", "tnx_mx_gemm", "tnx_mx_gemm_workspace_bytes", "tnx_mx_gemm_takes_rows", "tnx_mx_gemm_route",
-           "tnx_moe_workspace_bytes", "tnx_moe_route", "tnx_moe_plan", "tnx_moe_route_backward", "tnx_moe_combine")
+           "tnx_moe_workspace_bytes", "tnx_moe_route", "tnx_moe_plan", "tnx_moe_route_backward", "tnx_moe_combine",
+           "tnx_linear_workspace_bytes", "tnx_linear_scratch_bytes", "tnx_linear", "tnx_linear_route", "tnx_linear_gradient_bytes", "tnx_linear_gradient",
+           "tnx_layer_norm", "tnx_layer_norm_workspace_bytes", "tnx_layer_norm_backward", "tnx_grouped", "tnx_grouped_route")
 # limits of the routing entry points
 MOE_MAX_EXPERTS, MOE_MAX_TOP_K, MOE_MAX_GROUPS = 1024, 32, 64
+# enum tnx_activation
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3, 4
+# enum tnx_linear_route
+LINEAR_ROUTE_PRODUCT, LINEAR_ROUTE_FUSED, LINEAR_ROUTE_APART = 1, 2, 3
+# enum tnx_grouped_form
+GROUPED_ROWS, GROUPED_WEIGHT_GRADIENT = 0, 1
+GROUPED_MAX_GROUPS = 4096
+WS_COUNTER_BYTES = 65536
 
 
 class GemmArgs(ctypes.Structure):
@@ -113,6 +123,45 @@ class MoeArgs(ctypes.Structure):
         ("num_groups", ctypes.c_int32), ("top_groups", ctypes.c_int32), ("group_top", ctypes.c_int32), ("renormalize", ctypes.c_int32),
         ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class LinearArgs(ctypes.Structure):
+    """struct tnx_linear_args"""
+    _fields_ = [
+        *[(n, ctypes.c_void_p) for n in ("x", "w", "bias", "residual", "y", "z")],
+        *[(n, ctypes.c_int64) for n in ("m", "n", "k", "stride_xm", "stride_xk", "stride_wk", "stride_wn")],
+        *[(n, ctypes.c_int32) for n in ("dtype", "bias_dtype", "activation", "reserved")],
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class LinearGradientArgs(ctypes.Structure):
+    """struct tnx_linear_gradient_args"""
+    _fields_ = [
+        *[(n, ctypes.c_void_p) for n in ("dy", "z", "dz", "dbias")], ("m", ctypes.c_int64), ("n", ctypes.c_int64),
+        *[(n, ctypes.c_int32) for n in ("dtype", "bias_dtype", "activation", "reserved")],
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class NormArgs(ctypes.Structure):
+    """struct tnx_norm_args"""
+    _fields_ = [
+        *[(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "y", "mean", "rstd", "dy", "dx", "dweight", "dbias")],
+        *[(n, ctypes.c_int64) for n in ("rows", "n", "stride_x", "stride_dy")],
+        *[(n, ctypes.c_int32) for n in ("dtype", "weight_dtype", "bias_dtype")], ("eps", ctypes.c_float),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+    ]
+
+
+class GroupedArgs(ctypes.Structure):
+    """struct tnx_grouped_args"""
+    _fields_ = [
+        *[(n, ctypes.c_void_p) for n in ("a", "b", "c", "offsets")],
+        *[(n, ctypes.c_int64) for n in ("rows", "n", "k", "stride_ar", "stride_ak", "stride_group", "stride_bk", "stride_bn")],
+        *[(n, ctypes.c_int32) for n in ("groups", "dtype", "form", "reserved", "block_m", "block_n")], ("stream", ctypes.c_void_p),
     ]
 
 
@@ -195,7 +244,16 @@ def load() -> ctypes.CDLL:
             ("tnx_mx_gemm_route", [ctypes.POINTER(MxGemmArgs), ctypes.POINTER(i32)], ctypes.c_int),
             ("tnx_moe_workspace_bytes", [i64, i32, i32], ctypes.c_size_t), ("tnx_moe_route", [ctypes.POINTER(MoeArgs)], ctypes.c_int),
             ("tnx_moe_plan", [ctypes.POINTER(MoeArgs)], ctypes.c_int), ("tnx_moe_route_backward", [ctypes.POINTER(MoeArgs)], ctypes.c_int),
-            ("tnx_moe_combine", [ptr, ptr, ptr, ptr, i64, i32, i64, i32, i32, ptr], ctypes.c_int)):
+            ("tnx_moe_combine", [ptr, ptr, ptr, ptr, i64, i32, i64, i32, i32, ptr], ctypes.c_int),
+            ("tnx_linear_workspace_bytes", [ctypes.POINTER(LinearArgs)], ctypes.c_size_t),
+            ("tnx_linear_scratch_bytes", [ctypes.POINTER(LinearArgs)], ctypes.c_size_t), ("tnx_linear", [ctypes.POINTER(LinearArgs)], ctypes.c_int),
+            ("tnx_linear_route", [ctypes.POINTER(LinearArgs), ctypes.POINTER(i32)], ctypes.c_int),
+            ("tnx_linear_gradient_bytes", [ctypes.POINTER(LinearGradientArgs)], ctypes.c_size_t),
+            ("tnx_linear_gradient", [ctypes.POINTER(LinearGradientArgs)], ctypes.c_int),
+            ("tnx_layer_norm", [ctypes.POINTER(NormArgs)], ctypes.c_int),
+            ("tnx_layer_norm_workspace_bytes", [ctypes.POINTER(NormArgs)], ctypes.c_size_t),
+            ("tnx_layer_norm_backward", [ctypes.POINTER(NormArgs)], ctypes.c_int), ("tnx_grouped", [ctypes.POINTER(GroupedArgs)], ctypes.c_int),
+            ("tnx_grouped_route", [ctypes.POINTER(GroupedArgs), ctypes.POINTER(i32)], ctypes.c_int)):
         getattr(lib, name).argtypes = args
         getattr(lib, name).restype = res
     _lib = lib

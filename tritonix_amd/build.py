@@ -213,6 +213,60 @@ def generate_gather(tiles, gen):
     return files + [path]
 
 
+# (block_m, block_n, waves, ring slots) of the linear layers' kernels: what the built-in choice names (COST16 and COST32 in csrc/capi.hip, and its
+# choice for float32 as heads and tails), row-major and k-contiguous weights
+LINEAR_TILES = ((256, 256, 8, 2), (256, 192, 8, 2), (192, 256, 8, 2), (192, 192, 8, 3), (256, 128, 8, 3), (256, 128, 4, 3), (128, 256, 8, 3),
+                (128, 128, 8, 3), (128, 128, 8, 2), (64, 256, 8, 3), (128, 64, 8, 3), (64, 128, 8, 3), (64, 128, 8, 4), (64, 64, 4, 4), (32, 128, 4, 3),
+                (32, 64, 4, 4))
+LINEAR_PAIR_TILES = ((256, 256, 8, 2), (256, 192, 8, 2), (192, 256, 8, 2), (192, 192, 8, 3), (128, 128, 4, 3), (128, 128, 8, 3), (64, 128, 8, 3), (64, 64, 4, 4))
+# ... of the kernels over groups of rows: rows times row-major and k-contiguous weights, and the weights' gradient
+GROUPED_TILES = ((256, 256, 8, 2), (256, 128, 8, 3), (128, 256, 8, 3), (128, 128, 8, 3), (64, 128, 8, 3), (64, 64, 4, 4), (32, 128, 4, 3), (32, 64, 4, 4))
+
+
+def generate_family(family, rows, gen):
+    """Instance files of a kernel family (``linear``, ``grouped``), one per entry, and their table.  rows: (name, macro with its arguments)."""
+    cap = family.capitalize()
+    files, names = [], []
+    for name, entry in rows:
+        text = (f'// generated by tritonix_amd/build.py -- do not edit\n#include "{CSRC}/gemm_{family}.h"\n'
+                f"namespace tnx {{\nstatic {cap}Entry k_{name}[] = {{\n    {entry}\n}};\n{cap}Group g_{name} = {{k_{name}, 1}};\n}}\n")
+        path = os.path.join(gen, name + ".hip")
+        write_if_changed(path, text)
+        files.append(path)
+        names.append(name)
+    decl = "\n".join(f"extern {cap}Group g_{n};" for n in names)
+    ptrs = ", ".join(f"&g_{n}" for n in names) or "nullptr"
+    text = (f'// generated by tritonix_amd/build.py -- do not edit\n#include "{CSRC}/gemm_{family}.h"\nnamespace tnx {{\n{decl}\n}}\n'
+            f"using namespace tnx;\n"
+            f'extern "C" const {cap}Group* const* tnx_{family}_groups(int* n) {{\n'
+            f"  static const {cap}Group* const all[] = {{{ptrs}}};\n  *n = {len(names)};\n  return all;\n}}\n")
+    path = os.path.join(gen, f"{family}_groups.hip")
+    write_if_changed(path, text)
+    return files + [path]
+
+
+def generate_linear(gen, wanted=True):
+    rows = []
+    if wanted:
+        for dt in ("bf16", "f16"):
+            for bm, bn, nw, st in LINEAR_TILES:
+                rows.append((f"linear_{dt}_m{bm}_n{bn}_w{nw}_s{st}", f"TNX_LINEAR_ENTRY({TAGS[dt][0]}, {TAGS[dt][0]}::ID, {bm}, {bn}, {nw}, {st}, false)"))
+        for bm, bn, nw, st in LINEAR_PAIR_TILES:
+            rows.append((f"linear_pair_m{bm}_n{bn}_w{nw}_s{st}", f"TNX_LINEAR_ENTRY(TagBF16, LINEAR_PAIR, {bm}, {bn}, {nw}, {st}, true)"))
+        for bm, bn, nw, st in F32_TILES:
+            rows.append((f"linear_f32_m{bm}_n{bn}_w{nw}_s{st}", f"TNX_LINEAR_ENTRY(TagF32, DT_F32, {bm}, {bn}, {nw}, {st}, false)"))
+    return generate_family("linear", rows, gen)
+
+
+def generate_grouped(gen, wanted=True):
+    rows = []
+    if wanted:
+        for dt, tiles in (("bf16", GROUPED_TILES), ("f16", GROUPED_TILES), ("f32", F32_TILES)):
+            for bm, bn, nw, st in tiles:
+                rows.append((f"grouped_{dt}_m{bm}_n{bn}_w{nw}_s{st}", f"TNX_GROUPED_ENTRY({TAGS[dt][0]}, {bm}, {bn}, {nw}, {st})"))
+    return generate_family("grouped", rows, gen)
+
+
 def parse_only_conv(spec):
     """'bf16:128:128:64,...' (dtype:block_cout:block_pixels:block_k) for development builds."""
     out = []
@@ -350,6 +404,8 @@ def _compile(src, obj, verbose, force=True):
     deps = [src, os.path.join(CSRC, "gemm_tile.h"), os.path.join(CSRC, "gemm_skinny.h"), os.path.join(CSRC, "registry.h"),
             os.path.join(CSRC, "conv_tile.h"), os.path.join(CSRC, "conv_pack.h"),
             *([os.path.join(CSRC, "mx.h")] if os.path.basename(src).startswith(("mx_", "moe")) else []),
+            *([os.path.join(CSRC, "activation.h"), os.path.join(CSRC, "gemm_linear.h")] if os.path.basename(src).startswith(("linear", "norm", "capi")) else []),
+            *([os.path.join(CSRC, "gemm_grouped.h")] if os.path.basename(src).startswith("grouped") else []),
             *([os.path.join(CSRC, "conv_halo.h")] if os.path.basename(src).startswith(("halo_", "conv.hip")) else []),
             os.path.join(ROOT, "include", "tritonix_hip.h"), os.path.abspath(__file__)]
     if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(d) for d in deps):
@@ -380,7 +436,8 @@ def demangled_tile(name):
         return None
     _, tag, bm, bn, bk, nw, st, fast, persist, bt, conv, gather, at, pair = m.groups()
     kind = "at" if at == "1" else "packed conv" if gather == "1" else "conv" if conv == "1" else "bt" if bt == "1" else "persistent" if persist == "1" else "fast" if fast == "1" else "generic"
-    return f"{tag.lower()} {bm}x{bn}x{bk} w{nw} s{st} {kind}{' f32 pair' if pair == '1' else ''}"
+    family = " linear" if "LinearFamily" in name else " grouped" if "GroupedFamily" in name else ""
+    return f"{tag.lower()} {bm}x{bn}x{bk} w{nw} s{st} {kind}{' f32 pair' if pair == '1' else ''}{family}"
 
 
 def build(jobs=None, quick=False, verbose=True, force=True, only=None, out=None, defines=(), only_conv=None):
@@ -398,10 +455,11 @@ def build(jobs=None, quick=False, verbose=True, force=True, only=None, out=None,
     DEVICE_FLAGS.extend(f"-D{d}" for d in defines)
     srcs = generate(instances) + generate_conv(conv_instances, os.path.join(BUILD, "gen")) + generate_gather(
         GATHER_TILES if not (only or only_conv) or only == "gather" else (), os.path.join(BUILD, "gen")) + generate_halo(
-        HALO_TILES if not (only or only_conv) or only == "gather" else (), os.path.join(BUILD, "gen")) + [
+        HALO_TILES if not (only or only_conv) or only == "gather" else (), os.path.join(BUILD, "gen")) + generate_linear(
+        os.path.join(BUILD, "gen"), not (only or only_conv)) + generate_grouped(os.path.join(BUILD, "gen"), not (only or only_conv)) + [
         os.path.join(CSRC, "capi.hip"), os.path.join(CSRC, "skinny.hip"),
         os.path.join(CSRC, "conv.hip"), os.path.join(CSRC, "f32.hip"), os.path.join(CSRC, "mx_quant.hip"), os.path.join(CSRC, "mx_gemm.hip"),
-        os.path.join(CSRC, "moe.hip")]
+        os.path.join(CSRC, "moe.hip"), os.path.join(CSRC, "linear.hip"), os.path.join(CSRC, "norm.hip"), os.path.join(CSRC, "grouped.hip")]
     if lib == LIB:
         try:
             build_launch(verbose)

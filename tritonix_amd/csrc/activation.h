@@ -1,0 +1,47 @@
+// Activations of a linear layer and their derivatives, in 32 bits.
+#pragma once
+#include "gemm_tile.h"
+
+namespace tnx {
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4 };
+
+constexpr float GELU_C = 0.7978845608028654f;            // sqrt(2 / pi)
+constexpr float GELU_A = 0.044715f;
+
+// 1 / (1 + e^-z); ROUNDED: on its way to 16 bits
+template <bool ROUNDED> __device__ __forceinline__ float logistic(float z) {
+  const float d = 1.0f + __expf(-z);
+  return ROUNDED ? reciprocal_from_one(d) : 1.0f / d;
+}
+
+// gelu_tanh: z (1 + tanh u) / 2 = z / (1 + e^-2u), which keeps its relative precision where tanh is next to -1
+template <bool ROUNDED> __device__ __forceinline__ float activate(float z, int act) {
+  switch (act) {
+    case ACT_RELU: return z <= 0.0f ? 0.0f : z;          // (a NaN stays one)
+    case ACT_SILU: return z * logistic<ROUNDED>(z);
+    case ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case ACT_GELU_TANH: return z * logistic<ROUNDED>(2.0f * GELU_C * (z + GELU_A * z * z * z));
+    default: return z;
+  }
+}
+
+// The derivative.  Past +-128 each is 0 or 1 in 32 bits, and held there: products of an infinity and a zero are no number.
+__device__ __forceinline__ float activation_slope(float z, int act) {
+  if (act == ACT_RELU) return z <= 0.0f ? 0.0f : z > 0.0f ? 1.0f : z;
+  z = z > 128.0f ? 128.0f : z < -128.0f ? -128.0f : z;
+  switch (act) {
+    case ACT_SILU: {
+      const float s = logistic<false>(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    case ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * (0.3989422804014327f * __expf(-0.5f * z * z));
+    case ACT_GELU_TANH: {
+      const float z2 = z * z, s = logistic<false>(2.0f * GELU_C * z * (1.0f + GELU_A * z2));
+      return s + 2.0f * z * s * (1.0f - s) * GELU_C * (1.0f + 3.0f * GELU_A * z2);
+    }
+    default: return 1.0f;
+  }
+}
+
+}  // namespace tnx

@@ -10,10 +10,12 @@
 
 #include "../../include/tritonix_hip.h"
 #include "registry.h"
+#include "gemm_linear.h"
 
 using namespace tnx;
 
 extern "C" const KernelGroup* tnx_kernel_groups(int* ngroups);  // generated
+extern "C" const LinearGroup* const* tnx_linear_groups(int* ngroups);  // generated
 
 static thread_local int g_last_hip_error = 0;
 namespace tnx {
@@ -319,11 +321,39 @@ int tnx::gemm_check(const tnx_gemm_args* a, GemmForm form) {
   return need > 0 && (!a->workspace || a->workspace_bytes < need || ((uintptr_t)a->workspace & 255)) ? TNX_E_WORKSPACE : TNX_OK;
 }
 
-int tnx::gemm_launch(const tnx_gemm_args* a, const GemmBatch* extra, GemmForm form) {
+// the kernel of a linear layer on the tile of `a`: row-major or k-contiguous B
+static linear_fn linear_kernel(const tnx_gemm_args* a, GemmForm form, bool bt) {
+  static const std::unordered_map<uint64_t, const LinearEntry*> entries = [] {
+    std::unordered_map<uint64_t, const LinearEntry*> m;
+    int ng = 0;
+    const LinearGroup* const* g = tnx_linear_groups(&ng);
+    for (int i = 0; i < ng; ++i)
+      for (int j = 0; j < g[i]->count; ++j) {
+        const LinearEntry& e = g[i]->entries[j];
+        m.emplace(entry_key(e.dtype, e.bm, e.bn, 0, e.nw, e.stages), &e);
+      }
+    return m;
+  }();
+  const int kind = form == GEMM_PAIR ? LINEAR_PAIR : form == GEMM_F32 ? TNX_F32 : a->in_dtype;
+  if (a->block_k * (form == GEMM_F32 ? 4 : 2) != 128) return nullptr;
+  const auto hit = entries.find(entry_key(kind, a->block_m, a->block_n, 0, a->num_warps, a->num_stages));
+  return hit == entries.end() ? nullptr : bt ? hit->second->bt : hit->second->nn;
+}
+
+bool tnx::gemm_linear_fused(const tnx_gemm_args* a, GemmForm form) {
+  bool fast = false, bt = false, at = false, other_tile = false;
+  if (is_skinny_cfg(a) || (a->schedule & (TNX_SCHED_PERSISTENT | TNX_SCHED_ATOMIC_REDUCE)) || a->epilogue != TNX_EPI_NONE) return false;
+  if (supported_impl(a, nullptr, &fast, true, &bt, nullptr, &at, form, &other_tile) != TNX_OK || !fast || at || other_tile) return false;
+  const int64_t lda = a->stride_am, ldb = bt ? a->stride_bn : a->stride_bk;
+  return lda <= 0x7fffffff && ldb <= 0x7fffffff && a->stride_cm == a->n && a->stride_cn == 1 && linear_kernel(a, form, bt);
+}
+
+int tnx::gemm_launch(const tnx_gemm_args* a, const GemmBatch* extra, GemmForm form, const LinearParts* linear) {
   const KernelEntry* e = nullptr;
   bool fast = false, bt = false, at = false, tail_slab = false, other_tile = false;
   int st = supported_impl(a, &e, &fast, true, &bt, &tail_slab, &at, form, &other_tile);
   if (st != TNX_OK) return st;
+  if (linear && !gemm_linear_fused(a, form)) return TNX_E_UNSUPPORTED;
   if (extra && (form == GEMM_PAIR || e->bm * e->bn > 128 * 128 || a->split_k != 1 || (a->schedule & TNX_SCHED_PERSISTENT) || is_skinny_cfg(a) || extra->batch < 1 ||
                 a->epilogue != TNX_EPI_NONE || (extra->bias && a->in_dtype == TNX_I8)))
     return TNX_E_UNSUPPORTED;
@@ -396,7 +426,9 @@ int tnx::gemm_launch(const tnx_gemm_args* a, const GemmBatch* extra, GemmForm fo
     err = e->persist(p, (unsigned)(tiles < cus ? tiles : cus), stream);
   } else {
     unsigned grid = a->split_k > 1 ? (unsigned)(p.split_tile0 + ncut * a->split_k) : (unsigned)((int64_t)p.tiles_m * p.tiles_n * problems);
-    if (form == GEMM_PAIR)
+    if (linear)
+      err = linear_kernel(a, form, bt)(p, *linear, grid, stream);
+    else if (form == GEMM_PAIR)
       err = e->pair[at ? 2 : bt ? 1 : 0](p, grid, stream);
     else
       err = (at ? e->fast_at : bt ? e->fast_bt : fast ? e->fast : e->generic)(p, grid, stream);

@@ -184,7 +184,18 @@ extern "C" size_t tnx_gemm_f32_scratch_bytes(const tnx_gemm_args* a) {
   return plan(a, nullptr, &g, &sa, &sb, &bytes, &pair) == TNX_OK ? (size_t)bytes : 0;
 }
 
-extern "C" int tnx_gemm_f32(const tnx_gemm_args* a, void* scratch, size_t scratch_bytes) {
+bool tnx::gemm_f32_linear_fused(const tnx_gemm_args* a) {
+  if (gemm_f32_direct(a, true)) return gemm_linear_fused(a, GEMM_F32);
+  tnx_gemm_args g;
+  SplitSide sa, sb;
+  int64_t bytes = 0;
+  bool pair = false;
+  return plan(a, nullptr, &g, &sa, &sb, &bytes, &pair) == TNX_OK && pair && gemm_linear_fused(&g, GEMM_PAIR);
+}
+
+extern "C" int tnx_gemm_f32(const tnx_gemm_args* a, void* scratch, size_t scratch_bytes) { return gemm_f32(a, scratch, scratch_bytes, nullptr); }
+
+int tnx::gemm_f32(const tnx_gemm_args* a, void* scratch, size_t scratch_bytes, const LinearParts* linear) {
   tnx_gemm_args g;
   SplitSide sa, sb;
   int64_t bytes = 0;
@@ -194,11 +205,11 @@ extern "C" int tnx_gemm_f32(const tnx_gemm_args* a, void* scratch, size_t scratc
   if (a->m == 0 || a->n == 0) return TNX_OK;
   if (gemm_f32_direct(a, false)) {
     if (!a->a || !a->b || !a->c || (((uintptr_t)a->a | (uintptr_t)a->b | (uintptr_t)a->c) & 3)) return TNX_E_INVALID;
-    return gemm_launch(a, nullptr, GEMM_F32);
+    return gemm_launch(a, nullptr, GEMM_F32, linear);
   }
   if (a->k == 0) {                          // nothing to cut: the GEMM writes zeros
     g.k = 0;
-    return gemm_launch(&g, nullptr, pair ? GEMM_PAIR : GEMM_PADDED);
+    return gemm_launch(&g, nullptr, pair ? GEMM_PAIR : GEMM_PADDED, linear);
   }
   if (!a->a || !a->b || !a->c) return TNX_E_INVALID;
   if (((uintptr_t)a->a | (uintptr_t)a->b | (uintptr_t)a->c) & 3) return TNX_E_INVALID;
@@ -213,5 +224,5 @@ extern "C" int tnx_gemm_f32(const tnx_gemm_args* a, void* scratch, size_t scratc
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
   }
-  return gemm_launch(&g, nullptr, pair ? GEMM_PAIR : GEMM_PADDED);
+  return gemm_launch(&g, nullptr, pair ? GEMM_PAIR : GEMM_PADDED, linear);
 }

@@ -350,6 +350,13 @@ inline hipError_t launch_kernel(const void* kernel, unsigned grid, unsigned thre
 template <bool PLAIN> struct KernelParams { typedef GemmParams type; };
 template <> struct KernelParams<true> { typedef PlainParams type; };
 
+// What a kernel family adds to the plain product: another argument struct (at most 112 bytes), its own way from a workgroup to its tile,
+// its own epilogue.  See gemm_linear.h and gemm_grouped.h.
+struct PlainFamily {
+  static constexpr bool LINEAR = false, GROUPED = false;
+  template <bool PLAIN> using params = typename KernelParams<PLAIN>::type;
+};
+
 // Chip-level tile order for grids much larger than the CU count.  The 256 workgroups that run
 // together (one per CU) take one 16x16 super-block of tiles, so one "round" touches 16 row panels
 // of A and 16 column panels of B; super-blocks are walked in serpentine order, so consecutive
@@ -1227,11 +1234,14 @@ constexpr int GATHER_TABLE_BYTES = 8192;
 // BN output pixels.  A lane's DMA ops fetch the same 16-byte k chunk of different pixels, so an op's offset is the
 // pixel's, kept in a register, plus the chunk's (filter tap, channels), read once per slab from a table in LDS.  Chunks
 // past the end of k get an offset outside the buffer and arrive as zeros.
-template <class T, class C, bool FAST, bool PERSIST = false, bool BT = false, bool CONV = false, bool GATHER = false, bool AT = false, bool PAIR = false>
-__global__ __launch_bounds__(C::THREADS, PERSIST ? 1 : Residency<C>::WAVES) void gemm_tile_kernel(typename KernelParams<FAST && !CONV && !GATHER>::type in) {
+template <class T, class C, bool FAST, bool PERSIST = false, bool BT = false, bool CONV = false, bool GATHER = false, bool AT = false, bool PAIR = false,
+          class X = PlainFamily>
+__global__ __launch_bounds__(C::THREADS, PERSIST ? 1 : Residency<C>::WAVES) void gemm_tile_kernel(typename X::template params<FAST && !CONV && !GATHER> in) {
   GemmParams p;
-  if constexpr (FAST && !CONV && !GATHER) p = expand_params<C, BT, AT>(in);
+  if constexpr (X::LINEAR || X::GROUPED) p = X::template expand<C, BT, AT>(in);
+  else if constexpr (FAST && !CONV && !GATHER) p = expand_params<C, BT, AT>(in);
   else p = in;
+  static_assert(!(X::LINEAR || X::GROUPED) || (FAST && !PERSIST && !CONV && !GATHER), "families are built with the DMA loader");
   constexpr int ES = C::ES, BM = C::BM, BN = C::BN, BK = C::BK, NW = C::NW, STAGES = C::STAGES;
   constexpr int MI = C::MI, TM = C::TM, TN = C::TN;
   static_assert(GATHER ? C::VALID_GATHER : C::VALID, "tile configuration not supported by this kernel");
@@ -1247,7 +1257,7 @@ __global__ __launch_bounds__(C::THREADS, PERSIST ? 1 : Residency<C>::WAVES) void
   typedef typename T::acc_s acc_s;
   // Several problems in one grid and a bias per row (GemmParams::batch, cv.bias) exist in the tiles up to 128x128:
   // the 256-wide tiles have no register to spare for the extra state (measured: 20 more spilled registers, -0.4 %).
-  constexpr bool MULTI = !PERSIST && !CONV && !GATHER && !PAIR && multi_problem_tile<C>();
+  constexpr bool MULTI = !PERSIST && !CONV && !GATHER && !PAIR && !X::LINEAR && !X::GROUPED && multi_problem_tile<C>();
 
   constexpr int AT_CPR = BM * ES / 16, AT_ROWB = BM * ES;    // AT: chunks and bytes of an A slab row
 
@@ -1285,7 +1295,10 @@ __global__ __launch_bounds__(C::THREADS, PERSIST ? 1 : Residency<C>::WAVES) void
     }
   };
   int pid_m, pid_n;
-  if (PERSIST || p.split_k <= 1) {
+  if constexpr (X::GROUPED) {
+    // the workgroup's group becomes the problem; workgroups past the last tile have none
+    if (!X::template find<C, AT>(in, p, (int)blockIdx.x, (int)gridDim.x, tid & 63, &pid_m, &pid_n)) return;
+  } else if (PERSIST || p.split_k <= 1) {
     int bid = blockIdx.x;
     if constexpr (MULTI) {
       // several problems with one A in one grid (conv2d's 1x1 layers: one per image): problem after problem
@@ -2468,7 +2481,9 @@ __global__ __launch_bounds__(C::THREADS, PERSIST ? 1 : Residency<C>::WAVES) void
     auto finish = [&](auto& sums) __attribute__((always_inline)) {
       auto as = [&](auto otag) __attribute__((always_inline)) {
         typedef typename decltype(otag)::type OT;
-        if constexpr (GATHER)
+        if constexpr (X::LINEAR)
+          X::template store<C, OT>(in, sums, p, strip, elane, gm0, gn0);
+        else if constexpr (GATHER)
           epilogue_store_conv<T, C, OT>(sums, p.c, strip, elane, (int)gm0, (int)gn0, p.cv);
         else if (p.epilogue == EPI_NONE)
           epilogue_store<T, C, OT, false, MULTI>(sums, p.c, strip, elane, gm0, gn0, p.m, p.n, p.scm, p.scn, p.c_row_ok, 0,
@@ -2479,7 +2494,7 @@ __global__ __launch_bounds__(C::THREADS, PERSIST ? 1 : Residency<C>::WAVES) void
       };
       if constexpr (PAIR) {
         as(TypeTag<OutF32>{});
-      } else if constexpr (GATHER || f32_out_tile<T, C>()) {
+      } else if constexpr (!X::LINEAR && !X::GROUPED && (GATHER || f32_out_tile<T, C>())) {
         if (p.out_dtype == DT_F32) as(TypeTag<OutF32>{});
         else as(TypeTag<O>{});
       } else {

@@ -1,0 +1,448 @@
+// Layer normalisation: y = (x - mean) rstd weight + bias by rows, and its gradients.
+//
+//   unit = (x - mean) rstd,  g = dy weight
+//   dx = rstd (g - mean(g) - unit mean(g unit)),  dweight = sum over rows of dy unit,  dbias = sum over rows of dy
+//
+// Bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  A row is read once, into registers (16-byte runs,
+// one after another over the threads), the mean before the variance from the same registers: no difference of large squares.  In the backward pass a workgroup
+// keeps its rows' share of dweight and dbias, in 32 bits per column, and a second launch adds the workgroups' shares up in order.
+#include <hip/hip_runtime.h>
+
+#include "../../include/tritonix_hip.h"
+#include "registry.h"
+#include "gemm_linear.h"
+
+using namespace tnx;
+
+namespace {
+
+struct NormParams {
+  const uint8_t *x, *weight, *bias, *dy;
+  uint8_t *y, *dx;
+  float *mean, *rstd;
+  float* parts;                  // backward: [workgroups][2][n], or null where neither weight nor bias asks
+  int64_t rows, n, stride_x, stride_dy;
+  int weight_dtype, bias_dtype;
+  float eps;
+};
+
+__device__ __forceinline__ float param_at(const uint8_t* p, int64_t i, int dtype, float none) { return p ? bias_value(p, (int)i, dtype) : none; }
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+// Sums over the TPR threads of a row of NS values; every thread gets them.  TPR is a wave or the whole workgroup.  `slot` alternates from call
+// to call, so that one barrier does.
+template <int TPR, int NS> __device__ __forceinline__ void row_sums(float (&v)[NS], float* lds, int slot) {
+#pragma unroll
+  for (int s = 0; s < NS; ++s) v[s] = wave_sum(v[s]);
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    float* at = lds + slot * W * NS;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) at[(threadIdx.x >> 6) * NS + s] = v[s];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) t += at[w * NS + s];
+      v[s] = t;
+    }
+  }
+}
+
+template <class O, int V> __device__ __forceinline__ void load_run(const typename O::raw* src, int cols, float (&f)[V]) {
+  typedef typename O::raw raw;
+  raw e[V];
+  if (cols == V) {
+    const i32x4 v = *(const i32x4_loose*)src;
+    __builtin_memcpy(e, &v, 16);
+  } else {
+#pragma unroll
+    for (int x = 0; x < V; ++x) e[x] = x < cols ? src[x] : (raw)0;
+  }
+#pragma unroll
+  for (int x = 0; x < V; ++x) f[x] = x < cols ? Run<O, V>::widen(e[x]) : 0.0f;
+}
+template <class O, int V> __device__ __forceinline__ void store_run(typename O::raw* dst, int cols, const float (&f)[V]) {
+  typedef typename O::raw raw;
+  raw e[V];
+#pragma unroll
+  for (int x = 0; x < V; ++x) e[x] = O::cvt(f[x]);
+  if (cols == V) {
+    i32x4 v;
+    __builtin_memcpy(&v, e, 16);
+    *(i32x4_loose*)dst = v;
+  } else {
+#pragma unroll
+    for (int x = 0; x < V; ++x)
+      if (x < cols) dst[x] = e[x];
+  }
+}
+
+// TPR threads to a row, each with up to CH runs of V columns
+template <class O, int TPR, int CH> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormParams p) {
+  typedef typename O::raw raw;
+  constexpr int V = 16 / sizeof(raw), THREADS = TPR < 256 ? 256 : TPR;
+  __shared__ float lds[2 * THREADS / 64];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
+  if (row >= p.rows) return;                             // (whole waves; with TPR = THREADS whole workgroups)
+  const raw* src = (const raw*)p.x + row * p.stride_x;
+  float f[CH][V];
+  float s[1] = {0.0f};
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int64_t col = (int64_t)(c * TPR + t) * V, left = p.n - col;
+    load_run<O, V>(src + (left > 0 ? col : 0), left >= V ? V : left > 0 ? (int)left : 0, f[c]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[0] += f[c][e];
+  }
+  row_sums<TPR, 1>(s, lds, 0);
+  const float mean = s[0] / (float)p.n;
+  float q[1] = {0.0f};
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float d = f[c][e] - mean;
+      q[0] += (int64_t)(c * TPR + t) * V + e < p.n ? d * d : 0.0f;
+    }
+  row_sums<TPR, 1>(q, lds, 1);
+  const float rstd = 1.0f / sqrtf(q[0] / (float)p.n + p.eps);
+  if (p.mean && t == 0) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
+  raw* dst = (raw*)p.y + row * p.n;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int64_t col = (int64_t)(c * TPR + t) * V, left = p.n - col;
+    if (left <= 0) break;
+    const int cols = left >= V ? V : (int)left;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < cols) f[c][e] = (f[c][e] - mean) * rstd * param_at(p.weight, col + e, p.weight_dtype, 1.0f) + param_at(p.bias, col + e, p.bias_dtype, 0.0f);
+    store_run<O, V>(dst + col, cols, f[c]);
+  }
+}
+
+template <class O, int TPR, int CH, bool PARTS> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(NormParams p) {
+  typedef typename O::raw raw;
+  constexpr int V = 16 / sizeof(raw), THREADS = TPR < 256 ? 256 : TPR, LINES = THREADS / TPR;
+  __shared__ float lds[2 * 2 * THREADS / 64];
+  const int t = threadIdx.x % TPR, line = threadIdx.x / TPR;
+  float w[CH][V], dw[PARTS ? CH : 1][V], db[PARTS ? CH : 1][V];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int64_t col = (int64_t)(c * TPR + t) * V + e;
+      w[c][e] = col < p.n ? param_at(p.weight, col, p.weight_dtype, 1.0f) : 0.0f;
+      if (PARTS) dw[c][e] = db[c][e] = 0.0f;
+    }
+  int slot = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * LINES; row0 < p.rows; row0 += (int64_t)gridDim.x * LINES) {
+    const int64_t row = row0 + line;
+    if (row < p.rows) {                                  // (a wave's own row; with TPR = THREADS always)
+      const float mean = p.mean[row], rstd = p.rstd[row], share = 1.0f / (float)p.n;
+      float u[CH][V], g[CH][V], s[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int64_t col = (int64_t)(c * TPR + t) * V, left = p.n - col, at = left > 0 ? col : 0;
+        const int cols = left >= V ? V : left > 0 ? (int)left : 0;
+        load_run<O, V>((const raw*)p.x + row * p.stride_x + at, cols, u[c]);
+        load_run<O, V>((const raw*)p.dy + row * p.stride_dy + at, cols, g[c]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          u[c][e] = e < cols ? (u[c][e] - mean) * rstd : 0.0f;
+          if (PARTS) {
+            dw[c][e] += g[c][e] * u[c][e];
+            db[c][e] += g[c][e];
+          }
+          g[c][e] *= w[c][e];
+          s[0] += g[c][e];
+          s[1] += g[c][e] * u[c][e];
+        }
+      }
+      row_sums<TPR, 2>(s, lds, slot);
+      slot ^= 1;
+      if (p.dx) {
+        const float a = s[0] * share, b = s[1] * share;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int64_t col = (int64_t)(c * TPR + t) * V, left = p.n - col;
+          if (left <= 0) break;
+#pragma unroll
+          for (int e = 0; e < V; ++e) g[c][e] = rstd * (g[c][e] - a - u[c][e] * b);
+          store_run<O, V>((raw*)p.dx + row * p.n + col, left >= V ? V : (int)left, g[c]);
+        }
+      }
+    }
+  }
+  if constexpr (PARTS) {
+    // a share for every line of the workgroup: the second launch adds them up with the others
+    float* out = p.parts + ((int64_t)blockIdx.x * LINES + line) * 2 * p.n;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int64_t col = (int64_t)(c * TPR + t) * V + e;
+        if (col < p.n) {
+          out[col] = dw[c][e];
+          out[p.n + col] = db[c][e];
+        }
+      }
+  }
+}
+
+// Rows longer than the registers hold: read again for each of the passes.  A workgroup of 1024 threads to a row.
+template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_long_kernel(NormParams p) {
+  typedef typename O::raw raw;
+  constexpr int V = 16 / sizeof(raw), TPR = 1024;
+  __shared__ float lds[2 * 2 * 16];
+  const int64_t row = blockIdx.x;
+  const raw* src = (const raw*)p.x + row * p.stride_x;
+  auto over = [&](auto f) __attribute__((always_inline)) {
+    for (int64_t col = (int64_t)threadIdx.x * V; col < p.n; col += TPR * V) f(col, p.n - col >= V ? V : (int)(p.n - col));
+  };
+  if constexpr (!BACKWARD) {
+    float s[1] = {0.0f}, q[1] = {0.0f}, f[V];
+    over([&](int64_t col, int cols) __attribute__((always_inline)) {
+      load_run<O, V>(src + col, cols, f);
+      for (int e = 0; e < V; ++e) s[0] += f[e];
+    });
+    row_sums<TPR, 1>(s, lds, 0);
+    const float mean = s[0] / (float)p.n;
+    over([&](int64_t col, int cols) __attribute__((always_inline)) {
+      load_run<O, V>(src + col, cols, f);
+      for (int e = 0; e < V; ++e) q[0] += e < cols ? (f[e] - mean) * (f[e] - mean) : 0.0f;
+    });
+    row_sums<TPR, 1>(q, lds, 1);
+    const float rstd = 1.0f / sqrtf(q[0] / (float)p.n + p.eps);
+    if (p.mean && threadIdx.x == 0) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+    over([&](int64_t col, int cols) __attribute__((always_inline)) {
+      load_run<O, V>(src + col, cols, f);
+      for (int e = 0; e < V; ++e)
+        if (e < cols) f[e] = (f[e] - mean) * rstd * param_at(p.weight, col + e, p.weight_dtype, 1.0f) + param_at(p.bias, col + e, p.bias_dtype, 0.0f);
+      store_run<O, V>((raw*)p.y + row * p.n + col, cols, f);
+    });
+  } else {
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    const raw* dy = (const raw*)p.dy + row * p.stride_dy;
+    float s[2] = {0.0f, 0.0f}, u[V], g[V];
+    auto both = [&](int64_t col, int cols) __attribute__((always_inline)) {
+      load_run<O, V>(src + col, cols, u);
+      load_run<O, V>(dy + col, cols, g);
+      for (int e = 0; e < V; ++e) {
+        u[e] = e < cols ? (u[e] - mean) * rstd : 0.0f;
+        g[e] *= e < cols ? param_at(p.weight, col + e, p.weight_dtype, 1.0f) : 0.0f;
+      }
+    };
+    over([&](int64_t col, int cols) __attribute__((always_inline)) {
+      both(col, cols);
+      for (int e = 0; e < V; ++e) {
+        s[0] += g[e];
+        s[1] += g[e] * u[e];
+      }
+    });
+    row_sums<TPR, 2>(s, lds, 0);
+    const float a = s[0] / (float)p.n, b = s[1] / (float)p.n;
+    over([&](int64_t col, int cols) __attribute__((always_inline)) {
+      both(col, cols);
+      for (int e = 0; e < V; ++e) g[e] = rstd * (g[e] - a - u[e] * b);
+      store_run<O, V>((raw*)p.dx + row * p.n + col, cols, g);
+    });
+  }
+}
+
+// dweight and dbias of such rows: a workgroup's 32 runs of columns down 256 rows, its 8 rows of threads meet in LDS
+constexpr int LONG_ROWS = 256;
+template <class O> __global__ __launch_bounds__(256) void norm_columns_kernel(NormParams p) {
+  typedef typename O::raw raw;
+  constexpr int V = 16 / sizeof(raw);
+  __shared__ float sums[2][8][32 * V + 4];
+  const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
+  const int64_t col = ((int64_t)blockIdx.x * 32 + lane) * V, row0 = (int64_t)blockIdx.y * LONG_ROWS;
+  const int cols = p.n - col >= V ? V : p.n > col ? (int)(p.n - col) : 0;
+  float dw[V] = {}, db[V] = {};
+  for (int r = line; r < LONG_ROWS; r += 8) {
+    const int64_t row = row0 + r;
+    if (row >= p.rows || cols == 0) break;
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float u[V], g[V];
+    load_run<O, V>((const raw*)p.x + row * p.stride_x + col, cols, u);
+    load_run<O, V>((const raw*)p.dy + row * p.stride_dy + col, cols, g);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      dw[e] += e < cols ? g[e] * (u[e] - mean) * rstd : 0.0f;
+      db[e] += g[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    sums[0][line][lane * V + e] = dw[e];
+    sums[1][line][lane * V + e] = db[e];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * 32 * V; i += 256) {
+    const int which = i / (32 * V), c = i % (32 * V);
+    const int64_t at = (int64_t)blockIdx.x * 32 * V + c;
+    if (at >= p.n) continue;
+    float s = 0.0f;
+#pragma unroll
+    for (int l = 0; l < 8; ++l) s += sums[which][l][c];
+    p.parts[((int64_t)blockIdx.y * 2 + which) * p.n + at] = s;
+  }
+}
+
+// out[c] = the sum of parts[i][c] in the order of i: the first n columns are dweight, the others dbias
+__global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, int64_t count, int64_t n, uint8_t* dweight, int weight_dtype, uint8_t* dbias,
+                                                          int bias_dtype) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, line = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.0f;
+  if (col < 2 * n) {
+#pragma unroll 8
+    for (int64_t i = line; i < count; i += 16) s += parts[i * 2 * n + col];
+  }
+  sums[line][lane] = s;
+  __syncthreads();
+  if (line == 0 && col < 2 * n) {
+#pragma unroll
+    for (int l = 1; l < 16; ++l) s += sums[l][lane];
+    if (col < n && dweight) store_out<float>(dweight, col, s, weight_dtype);
+    if (col >= n && dbias) store_out<float>(dbias, col - n, s, bias_dtype);
+  }
+}
+
+constexpr int64_t MOST_GROUPS = 512;
+
+// threads and runs of a row; 0: longer than the registers hold
+struct Shape {
+  int tpr, ch;
+};
+Shape shape_of(int64_t n, int v) {
+  static const Shape shapes[] = {{64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}};
+  for (const Shape& s : shapes)
+    if (n <= (int64_t)s.tpr * s.ch * v) return s;
+  return {0, 0};
+}
+int64_t lines_of(const Shape& s) { return s.tpr < 256 ? 256 / s.tpr : 1; }
+int64_t groups_of(const tnx_norm_args* a, const Shape& s) {
+  const int64_t most = (a->rows + lines_of(s) - 1) / lines_of(s);
+  return most < MOST_GROUPS ? most : MOST_GROUPS;
+}
+int64_t shares_of(const tnx_norm_args* a) {
+  const Shape s = shape_of(a->n, a->dtype == TNX_F32 ? 4 : 8);
+  return s.tpr == 0 ? (a->rows + LONG_ROWS - 1) / LONG_ROWS : groups_of(a, s) * lines_of(s);
+}
+
+int check(const tnx_norm_args* a) {
+  if (!a || a->rows < 0 || a->n < 0 || !(a->eps >= 0.0f)) return TNX_E_INVALID;
+  if (a->dtype != TNX_F16 && a->dtype != TNX_BF16 && a->dtype != TNX_F32) return TNX_E_UNSUPPORTED;
+  if ((a->weight && a->weight_dtype != a->dtype && a->weight_dtype != TNX_F32) || (a->bias && a->bias_dtype != a->dtype && a->bias_dtype != TNX_F32))
+    return TNX_E_UNSUPPORTED;
+  if (a->rows > 0x7fffffff || a->n > 0x3fffffff) return TNX_E_UNSUPPORTED;
+  return TNX_OK;
+}
+NormParams params_of(const tnx_norm_args* a) {
+  NormParams p;
+  p.x = (const uint8_t*)a->x; p.weight = (const uint8_t*)a->weight; p.bias = (const uint8_t*)a->bias; p.dy = (const uint8_t*)a->dy;
+  p.y = (uint8_t*)a->y; p.dx = (uint8_t*)a->dx;
+  p.mean = a->mean; p.rstd = a->rstd;
+  p.parts = nullptr;
+  p.rows = a->rows; p.n = a->n; p.stride_x = a->stride_x; p.stride_dy = a->stride_dy;
+  p.weight_dtype = a->weight_dtype; p.bias_dtype = a->bias_dtype;
+  p.eps = a->eps;
+  return p;
+}
+int launched() {
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
+  return TNX_OK;
+}
+
+#define TNX_NORM_SHAPES(DO) DO(64, 1) DO(64, 2) DO(64, 4) DO(256, 2) DO(256, 4) DO(512, 4) DO(1024, 4)
+
+template <class O> int forward(const NormParams& p, hipStream_t stream) {
+  const Shape s = shape_of(p.n, 16 / sizeof(typename O::raw));
+  const unsigned grid = (unsigned)((p.rows + lines_of(s) - 1) / lines_of(s));
+#define TNX_NORM_FORWARD(TPR, CH)                                                                                       \
+  if (s.tpr == TPR && s.ch == CH) {                                                                                     \
+    hipLaunchKernelGGL((norm_kernel<O, TPR, CH>), dim3(grid), dim3(TPR < 256 ? 256 : TPR), 0, stream, p);               \
+    return launched();                                                                                                  \
+  }
+  TNX_NORM_SHAPES(TNX_NORM_FORWARD)
+  hipLaunchKernelGGL((norm_long_kernel<O, false>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+  return launched();
+}
+
+template <class O> int backward(const tnx_norm_args* a, NormParams p, hipStream_t stream) {
+  const Shape s = shape_of(p.n, 16 / sizeof(typename O::raw));
+  const int64_t shares = shares_of(a);
+  const bool wanted = a->dweight || a->dbias;
+  if (s.tpr == 0) {
+    if (p.dx) hipLaunchKernelGGL((norm_long_kernel<O, true>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+    if (wanted)
+      hipLaunchKernelGGL((norm_columns_kernel<O>), dim3((unsigned)((p.n + 32 * (16 / sizeof(typename O::raw)) - 1) / (32 * (16 / sizeof(typename O::raw)))), (unsigned)shares),
+                         dim3(256), 0, stream, p);
+  } else {
+    const unsigned grid = (unsigned)groups_of(a, s);
+#define TNX_NORM_BACKWARD(TPR, CH)                                                                                      \
+  if (s.tpr == TPR && s.ch == CH) {                                                                                     \
+    if (wanted) hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, true>), dim3(grid), dim3(TPR < 256 ? 256 : TPR), 0, stream, p); \
+    else hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, false>), dim3(grid), dim3(TPR < 256 ? 256 : TPR), 0, stream, p);       \
+  }
+    TNX_NORM_SHAPES(TNX_NORM_BACKWARD)
+  }
+  if (wanted)
+    hipLaunchKernelGGL(norm_parts_kernel, dim3((unsigned)((2 * p.n + 63) / 64)), dim3(1024), 0, stream, p.parts, shares, p.n, (uint8_t*)a->dweight, a->weight_dtype,
+                       (uint8_t*)a->dbias, a->bias_dtype);
+  return launched();
+}
+
+}  // namespace
+
+extern "C" int tnx_layer_norm(const tnx_norm_args* a) {
+  const int st = check(a);
+  if (st != TNX_OK) return st;
+  if (a->rows == 0 || a->n == 0) return TNX_OK;
+  if (!a->x || !a->y || !a->mean != !a->rstd) return TNX_E_INVALID;
+  const NormParams p = params_of(a);
+  const hipStream_t stream = (hipStream_t)a->stream;
+  return a->dtype == TNX_BF16 ? forward<OutBF16>(p, stream) : a->dtype == TNX_F16 ? forward<OutF16>(p, stream) : forward<OutF32>(p, stream);
+}
+
+extern "C" size_t tnx_layer_norm_workspace_bytes(const tnx_norm_args* a) {
+  return check(a) != TNX_OK || !(a->dweight || a->dbias) ? 0 : (size_t)shares_of(a) * 2 * a->n * 4;
+}
+
+extern "C" int tnx_layer_norm_backward(const tnx_norm_args* a) {
+  const int st = check(a);
+  if (st != TNX_OK) return st;
+  if (a->n == 0 || (!a->dx && !a->dweight && !a->dbias) || (a->rows == 0 && !a->dweight && !a->dbias)) return TNX_OK;
+  if (a->rows > 0 && (!a->x || !a->dy || !a->mean || !a->rstd)) return TNX_E_INVALID;
+  const size_t need = tnx_layer_norm_workspace_bytes(a);
+  if (need && (!a->workspace || a->workspace_bytes < need || ((uintptr_t)a->workspace & 15))) return TNX_E_WORKSPACE;
+  if (shares_of(a) > 65535) return TNX_E_UNSUPPORTED;
+  NormParams p = params_of(a);
+  p.parts = (float*)a->workspace;
+  const hipStream_t stream = (hipStream_t)a->stream;
+  if (a->rows == 0) {                                     // sums of no rows
+    hipLaunchKernelGGL(norm_parts_kernel, dim3((unsigned)((2 * p.n + 63) / 64)), dim3(1024), 0, stream, p.parts, (int64_t)0, p.n, (uint8_t*)a->dweight, a->weight_dtype,
+                       (uint8_t*)a->dbias, a->bias_dtype);
+    return launched();
+  }
+  return a->dtype == TNX_BF16 ? backward<OutBF16>(a, p, stream) : a->dtype == TNX_F16 ? backward<OutF16>(a, p, stream) : backward<OutF32>(a, p, stream);
+}

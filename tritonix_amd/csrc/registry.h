@@ -40,7 +40,14 @@ struct GemmBatch {
 // holds the heads and tails of a float32 product in blocks of 32 (KernelEntry::pair).
 // F32: float32 operands as they are, on the binary32 matrix instruction.
 enum GemmForm { GEMM_PLAIN = 0, GEMM_PADDED = 1, GEMM_PAIR = 2, GEMM_F32 = 3 };
-int gemm_launch(const tnx_gemm_args* a, const GemmBatch* extra, GemmForm form = GEMM_PLAIN);
+// linear: with that epilogue (gemm_linear.h; the tile must be built with it, the operands in a layout of the DMA loader, not m-contiguous)
+struct LinearParts;
+int gemm_launch(const tnx_gemm_args* a, const GemmBatch* extra, GemmForm form = GEMM_PLAIN, const LinearParts* linear = nullptr);
+// whether gemm_launch would take `a` with a linear layer's epilogue
+bool gemm_linear_fused(const tnx_gemm_args* a, GemmForm form);
+// tnx_gemm_f32 with that epilogue, and whether it takes it
+int gemm_f32(const tnx_gemm_args* a, void* scratch, size_t scratch_bytes, const LinearParts* linear);
+bool gemm_f32_linear_fused(const tnx_gemm_args* a);
 // the status gemm_launch would return for these arguments, the workspace included, without launching
 int gemm_check(const tnx_gemm_args* a, GemmForm form);
 // whether the tile of `a` and the layout of its float32 operands have a kernel that multiplies them as they are
