@@ -135,3 +135,18 @@ def test_grouped_entry_point_refuses():
     assert lib.tnx_grouped_route(ctypes.byref(grouped_args()), info) == 1 and info[3] == 0
     for more in (dict(k=63, stride_ar=63), dict(n=63, stride_bk=63), dict(a=4098), dict(b=4100), dict(stride_group=4097)):
         assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**more)), info) == 1 and info[3] == 1, more
+
+
+def test_accumulators_stay_in_registers():
+    """No kernel of a linear layer or a grouped product keeps its sums in memory: what the compiler reported of them."""
+    import json
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "build", "kernel_resources.json")
+    if not os.path.exists(path):
+        pytest.skip("no build report (the library was built elsewhere)")
+    with open(path) as f:
+        report = json.load(f)
+    scratch = {k: v["scratch"] for k, v in report.items() if k.endswith((" linear", " grouped"))}
+    # (256x256 on float32 heads and tails fills every register with its sums and fragments)
+    assert {k: v for k, v in scratch.items() if v > (80 if "256x256" in k and "f32 pair" in k else 0)} == {}

@@ -9,19 +9,17 @@ enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4
 constexpr float GELU_C = 0.7978845608028654f;            // sqrt(2 / pi)
 constexpr float GELU_A = 0.044715f;
 
-// 1 / (1 + e^-z); ROUNDED: on its way to 16 bits
-template <bool ROUNDED> __device__ __forceinline__ float logistic(float z) {
-  const float d = 1.0f + __expf(-z);
-  return ROUNDED ? reciprocal_from_one(d) : 1.0f / d;
-}
+// 1 / (1 + e^-z), from the reciprocal instruction: half its last bit off where the division would be exact, in 32 bits, at an eighth of the
+// instructions
+__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
 // gelu_tanh: z (1 + tanh u) / 2 = z / (1 + e^-2u), which keeps its relative precision where tanh is next to -1
-template <bool ROUNDED> __device__ __forceinline__ float activate(float z, int act) {
+__device__ __forceinline__ float activate(float z, int act) {
   switch (act) {
     case ACT_RELU: return z <= 0.0f ? 0.0f : z;          // (a NaN stays one)
-    case ACT_SILU: return z * logistic<ROUNDED>(z);
+    case ACT_SILU: return z * logistic(z);
     case ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case ACT_GELU_TANH: return z * logistic<ROUNDED>(2.0f * GELU_C * (z + GELU_A * z * z * z));
+    case ACT_GELU_TANH: return z * logistic(2.0f * GELU_C * (z + GELU_A * z * z * z));
     default: return z;
   }
 }
@@ -32,12 +30,12 @@ __device__ __forceinline__ float activation_slope(float z, int act) {
   z = z > 128.0f ? 128.0f : z < -128.0f ? -128.0f : z;
   switch (act) {
     case ACT_SILU: {
-      const float s = logistic<false>(z);
+      const float s = logistic(z);
       return s * (1.0f + z * (1.0f - s));
     }
     case ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * (0.3989422804014327f * __expf(-0.5f * z * z));
     case ACT_GELU_TANH: {
-      const float z2 = z * z, s = logistic<false>(2.0f * GELU_C * z * (1.0f + GELU_A * z2));
+      const float z2 = z * z, s = logistic(2.0f * GELU_C * z * (1.0f + GELU_A * z2));
       return s + 2.0f * z * s * (1.0f - s) * GELU_C * (1.0f + 3.0f * GELU_A * z2);
     }
     default: return 1.0f;

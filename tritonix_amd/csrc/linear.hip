@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256) void epilogue_kernel(const float* sums, Linear
     const int64_t at = row * n + col;
     float v = (sums ? sums[at] : 0.0f) + bias;
     if (x.z) store_out<float>(x.z, at, v, dtype);
-    v = dtype == DT_F32 ? activate<false>(v, x.act) : activate<true>(v, x.act);
+    v = activate(v, x.act);
     if (x.residual) v += load_float(x.residual, at, dtype);
     store_out<float>(y, at, v, dtype);
   }

@@ -26,7 +26,6 @@ struct NormParams {
   float eps;
 };
 
-__device__ __forceinline__ float param_at(const uint8_t* p, int64_t i, int dtype, float none) { return p ? bias_value(p, (int)i, dtype) : none; }
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -57,9 +56,17 @@ template <int TPR, int NS> __device__ __forceinline__ void row_sums(float (&v)[N
   }
 }
 
-template <class O, int V> __device__ __forceinline__ void load_run(const typename O::raw* src, int cols, float (&f)[V]) {
+// Runs of V columns, `cols` of which exist.  WHOLE: all or none, since n is a multiple of V.
+template <class O, int V, bool WHOLE = false> __device__ __forceinline__ void load_run(const typename O::raw* src, int cols, float (&f)[V]) {
   typedef typename O::raw raw;
   raw e[V];
+  if (WHOLE) {
+    const i32x4 v = cols ? *(const i32x4_loose*)src : i32x4{0, 0, 0, 0};
+    __builtin_memcpy(e, &v, 16);
+#pragma unroll
+    for (int x = 0; x < V; ++x) f[x] = Run<O, V>::widen(e[x]);
+    return;
+  }
   if (cols == V) {
     const i32x4 v = *(const i32x4_loose*)src;
     __builtin_memcpy(e, &v, 16);
@@ -70,12 +77,13 @@ template <class O, int V> __device__ __forceinline__ void load_run(const typenam
 #pragma unroll
   for (int x = 0; x < V; ++x) f[x] = x < cols ? Run<O, V>::widen(e[x]) : 0.0f;
 }
-template <class O, int V> __device__ __forceinline__ void store_run(typename O::raw* dst, int cols, const float (&f)[V]) {
+template <class O, int V, bool WHOLE = false> __device__ __forceinline__ void store_run(typename O::raw* dst, int cols, const float (&f)[V]) {
   typedef typename O::raw raw;
   raw e[V];
 #pragma unroll
   for (int x = 0; x < V; ++x) e[x] = O::cvt(f[x]);
-  if (cols == V) {
+  if (WHOLE && cols == 0) return;
+  if (WHOLE || cols == V) {
     i32x4 v;
     __builtin_memcpy(&v, e, 16);
     *(i32x4_loose*)dst = v;
@@ -86,8 +94,27 @@ template <class O, int V> __device__ __forceinline__ void store_run(typename O::
   }
 }
 
+// V columns of weight or bias, of the rows' type or float32; null: `none` throughout
+template <class O, int V, bool WHOLE = false> __device__ __forceinline__ void load_param(const uint8_t* p, int dtype, int64_t col, int cols, float none, float (&f)[V]) {
+  if (!p) {
+#pragma unroll
+    for (int x = 0; x < V; ++x) f[x] = none;
+  } else if (dtype != DT_F32) {
+    load_run<O, V, WHOLE>((const typename O::raw*)p + col, cols, f);
+  } else {
+    const float* src = (const float*)p + col;
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {
+      float q[4];
+      load_run<OutF32, 4, WHOLE>(src + 4 * h, cols - 4 * h >= 4 ? 4 : cols - 4 * h > 0 ? cols - 4 * h : 0, q);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) f[4 * h + x] = q[x];
+    }
+  }
+}
+
 // TPR threads to a row, each with up to CH runs of V columns
-template <class O, int TPR, int CH> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormParams p) {
+template <class O, int TPR, int CH, bool WHOLE> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_kernel(NormParams p) {
   typedef typename O::raw raw;
   constexpr int V = 16 / sizeof(raw), THREADS = TPR < 256 ? 256 : TPR;
   __shared__ float lds[2 * THREADS / 64];
@@ -100,7 +127,7 @@ template <class O, int TPR, int CH> __global__ __launch_bounds__(TPR < 256 ? 256
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int64_t col = (int64_t)(c * TPR + t) * V, left = p.n - col;
-    load_run<O, V>(src + (left > 0 ? col : 0), left >= V ? V : left > 0 ? (int)left : 0, f[c]);
+    load_run<O, V, WHOLE>(src + (left > 0 ? col : 0), left >= V ? V : left > 0 ? (int)left : 0, f[c]);
 #pragma unroll
     for (int e = 0; e < V; ++e) s[0] += f[c][e];
   }
@@ -112,7 +139,7 @@ template <class O, int TPR, int CH> __global__ __launch_bounds__(TPR < 256 ? 256
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float d = f[c][e] - mean;
-      q[0] += (int64_t)(c * TPR + t) * V + e < p.n ? d * d : 0.0f;
+      q[0] += (c * TPR + t) * V + (WHOLE ? 0 : e) < (int)p.n ? d * d : 0.0f;
     }
   row_sums<TPR, 1>(q, lds, 1);
   const float rstd = 1.0f / sqrtf(q[0] / (float)p.n + p.eps);
@@ -126,79 +153,158 @@ template <class O, int TPR, int CH> __global__ __launch_bounds__(TPR < 256 ? 256
     const int64_t col = (int64_t)(c * TPR + t) * V, left = p.n - col;
     if (left <= 0) break;
     const int cols = left >= V ? V : (int)left;
+    float w[V], b[V];
+    load_param<O, V, WHOLE>(p.weight, p.weight_dtype, col, cols, 1.0f, w);
+    load_param<O, V, WHOLE>(p.bias, p.bias_dtype, col, cols, 0.0f, b);
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (e < cols) f[c][e] = (f[c][e] - mean) * rstd * param_at(p.weight, col + e, p.weight_dtype, 1.0f) + param_at(p.bias, col + e, p.bias_dtype, 0.0f);
-    store_run<O, V>(dst + col, cols, f[c]);
+    for (int e = 0; e < V; ++e) f[c][e] = (f[c][e] - mean) * rstd * w[e] + b[e];
+    store_run<O, V, WHOLE>(dst + col, cols, f[c]);
   }
 }
 
-template <class O, int TPR, int CH, bool PARTS> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(NormParams p) {
+// V columns as they lie in memory; past the row's end zeros
+template <class O, bool WHOLE> __device__ __forceinline__ i32x4 load_packed(const typename O::raw* src, int cols) {
+  typedef typename O::raw raw;
+  constexpr int V = 16 / sizeof(raw);
+  if (WHOLE) return cols ? *(const i32x4_loose*)src : i32x4{0, 0, 0, 0};
+  if (cols == V) return *(const i32x4_loose*)src;
+  raw e[V];
+#pragma unroll
+  for (int x = 0; x < V; ++x) e[x] = x < cols ? src[x] : (raw)0;
+  i32x4 v;
+  __builtin_memcpy(&v, e, 16);
+  return v;
+}
+template <class O, int V> __device__ __forceinline__ void unpack(i32x4 v, float (&f)[V]) {
+  typename O::raw e[V];
+  __builtin_memcpy(e, &v, 16);
+#pragma unroll
+  for (int x = 0; x < V; ++x) f[x] = Run<O, V>::widen(e[x]);
+}
+
+// A workgroup walks over rows; x and dy of the row that is worked on and of the next are in registers as they lie in memory (widened
+// twice: for the sums, then for dx), which leaves room for two sums per column and for the loads to run ahead of the barrier.
+// Columns past the row's end are zeros in dy and weight and so add nothing.
+template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(NormParams p) {
   typedef typename O::raw raw;
   constexpr int V = 16 / sizeof(raw), THREADS = TPR < 256 ? 256 : TPR, LINES = THREADS / TPR;
+  constexpr bool AHEAD = CH <= 2;
   __shared__ float lds[2 * 2 * THREADS / 64];
   const int t = threadIdx.x % TPR, line = threadIdx.x / TPR;
-  float w[CH][V], dw[PARTS ? CH : 1][V], db[PARTS ? CH : 1][V];
+  float dw[PARTS ? CH : 1][V], db[PARTS ? CH : 1][V];
+  int cols[CH];
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c) {
+    const int64_t left = p.n - (int64_t)(c * TPR + t) * V;
+    cols[c] = left >= V ? V : left > 0 ? (int)left : 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int64_t col = (int64_t)(c * TPR + t) * V + e;
-      w[c][e] = col < p.n ? param_at(p.weight, col, p.weight_dtype, 1.0f) : 0.0f;
+    for (int e = 0; e < V; ++e)
       if (PARTS) dw[c][e] = db[c][e] = 0.0f;
+  }
+  i32x4 x[CH], g[CH];
+  float mean = 0.0f, rstd = 0.0f;
+  auto fetch = [&](int64_t row, i32x4 (&fx)[CH], i32x4 (&fg)[CH], float& fmean, float& frstd) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int64_t at = cols[c] ? (int64_t)(c * TPR + t) * V : 0;
+      fx[c] = load_packed<O, WHOLE>((const raw*)p.x + row * p.stride_x + at, cols[c]);
+      fg[c] = load_packed<O, WHOLE>((const raw*)p.dy + row * p.stride_dy + at, cols[c]);
     }
+    fmean = p.mean[row];
+    frstd = p.rstd[row];
+  };
+  const int64_t step = (int64_t)gridDim.x * LINES;
+  int64_t row = (int64_t)blockIdx.x * LINES + line;
+  const float share = 1.0f / (float)p.n;
   int slot = 0;
-  for (int64_t row0 = (int64_t)blockIdx.x * LINES; row0 < p.rows; row0 += (int64_t)gridDim.x * LINES) {
-    const int64_t row = row0 + line;
-    if (row < p.rows) {                                  // (a wave's own row; with TPR = THREADS always)
-      const float mean = p.mean[row], rstd = p.rstd[row], share = 1.0f / (float)p.n;
-      float u[CH][V], g[CH][V], s[2] = {0.0f, 0.0f};
+  if (AHEAD && row < p.rows) fetch(row, x, g, mean, rstd);
+  for (; row < p.rows; row += step) {                    // (a wave's own rows; with TPR = THREADS the workgroup's)
+    i32x4 nx[CH], ng[CH];
+    float nmean = 0.0f, nrstd = 0.0f;
+    if (!AHEAD) fetch(row, x, g, mean, rstd);
+    else if (row + step < p.rows) fetch(row + step, nx, ng, nmean, nrstd);
+    float s[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int64_t col = (int64_t)(c * TPR + t) * V, left = p.n - col, at = left > 0 ? col : 0;
-        const int cols = left >= V ? V : left > 0 ? (int)left : 0;
-        load_run<O, V>((const raw*)p.x + row * p.stride_x + at, cols, u[c]);
-        load_run<O, V>((const raw*)p.dy + row * p.stride_dy + at, cols, g[c]);
+    for (int c = 0; c < CH; ++c) {
+      float u[V], d[V], w[V];
+      unpack<O, V>(x[c], u);
+      unpack<O, V>(g[c], d);
+      load_param<O, V, WHOLE>(p.weight, p.weight_dtype, cols[c] ? (int64_t)(c * TPR + t) * V : 0, cols[c], 1.0f, w);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          u[c][e] = e < cols ? (u[c][e] - mean) * rstd : 0.0f;
-          if (PARTS) {
-            dw[c][e] += g[c][e] * u[c][e];
-            db[c][e] += g[c][e];
-          }
-          g[c][e] *= w[c][e];
-          s[0] += g[c][e];
-          s[1] += g[c][e] * u[c][e];
+      for (int e = 0; e < V; ++e) {
+        u[e] = (u[e] - mean) * rstd;
+        if (PARTS) {
+          dw[c][e] += d[e] * u[e];
+          db[c][e] += d[e];
         }
+        d[e] *= w[e];
+        s[0] += d[e];
+        s[1] += d[e] * u[e];
       }
+    }
+    if (p.dx) {
       row_sums<TPR, 2>(s, lds, slot);
       slot ^= 1;
-      if (p.dx) {
-        const float a = s[0] * share, b = s[1] * share;
+      const float a = s[0] * share, b = s[1] * share;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const int64_t col = (int64_t)(c * TPR + t) * V, left = p.n - col;
-          if (left <= 0) break;
+      for (int c = 0; c < CH; ++c) {
+        float u[V], d[V], w[V];
+        asm("" : "+v"(x[c]), "+v"(g[c]));               // (widened again, not kept wide since the sums)
+        unpack<O, V>(x[c], u);
+        unpack<O, V>(g[c], d);
+        load_param<O, V, WHOLE>(p.weight, p.weight_dtype, cols[c] ? (int64_t)(c * TPR + t) * V : 0, cols[c], 1.0f, w);
 #pragma unroll
-          for (int e = 0; e < V; ++e) g[c][e] = rstd * (g[c][e] - a - u[c][e] * b);
-          store_run<O, V>((raw*)p.dx + row * p.n + col, left >= V ? V : (int)left, g[c]);
-        }
+        for (int e = 0; e < V; ++e) d[e] = rstd * (d[e] * w[e] - a - (u[e] - mean) * rstd * b);
+        if (cols[c]) store_run<O, V, WHOLE>((raw*)p.dx + row * p.n + (int64_t)(c * TPR + t) * V, cols[c], d);
       }
+    }
+    if (AHEAD) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        x[c] = nx[c];
+        g[c] = ng[c];
+      }
+      mean = nmean;
+      rstd = nrstd;
     }
   }
   if constexpr (PARTS) {
-    // a share for every line of the workgroup: the second launch adds them up with the others
-    float* out = p.parts + ((int64_t)blockIdx.x * LINES + line) * 2 * p.n;
+    // the workgroup's share: its lines meet in LDS, in order
+    float* const out = p.parts + (int64_t)blockIdx.x * 2 * p.n;
+    if constexpr (LINES > 1) {
+      __shared__ float meet[LINES][2][CH * V * TPR];
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+      for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int64_t col = (int64_t)(c * TPR + t) * V + e;
-        if (col < p.n) {
-          out[col] = dw[c][e];
-          out[p.n + col] = db[c][e];
+        for (int e = 0; e < V; ++e) {
+          meet[line][0][(c * TPR + t) * V + e] = dw[c][e];
+          meet[line][1][(c * TPR + t) * V + e] = db[c][e];
+        }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * CH * V * TPR; i += THREADS) {
+        const int which = i / (CH * V * TPR), col = i % (CH * V * TPR);
+        float sum = 0.0f;
+#pragma unroll
+        for (int l = 0; l < LINES; ++l) sum += meet[l][which][col];
+        if (col < p.n) out[which * p.n + col] = sum;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int64_t col = (int64_t)(c * TPR + t) * V;
+#pragma unroll
+        for (int h = 0; h < V / 4; ++h) {
+          const int left = cols[c] - 4 * h;
+          float q[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[e] = dw[c][4 * h + e];
+          store_run<OutF32, 4, WHOLE>(out + col + 4 * h, left >= 4 ? 4 : left > 0 ? left : 0, q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[e] = db[c][4 * h + e];
+          store_run<OutF32, 4, WHOLE>(out + p.n + col + 4 * h, left >= 4 ? 4 : left > 0 ? left : 0, q);
         }
       }
+    }
   }
 }
 
@@ -232,8 +338,10 @@ template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_l
     }
     over([&](int64_t col, int cols) __attribute__((always_inline)) {
       load_run<O, V>(src + col, cols, f);
-      for (int e = 0; e < V; ++e)
-        if (e < cols) f[e] = (f[e] - mean) * rstd * param_at(p.weight, col + e, p.weight_dtype, 1.0f) + param_at(p.bias, col + e, p.bias_dtype, 0.0f);
+      float w[V], b[V];
+      load_param<O, V>(p.weight, p.weight_dtype, col, cols, 1.0f, w);
+      load_param<O, V>(p.bias, p.bias_dtype, col, cols, 0.0f, b);
+      for (int e = 0; e < V; ++e) f[e] = (f[e] - mean) * rstd * w[e] + b[e];
       store_run<O, V>((raw*)p.y + row * p.n + col, cols, f);
     });
   } else {
@@ -243,9 +351,11 @@ template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_l
     auto both = [&](int64_t col, int cols) __attribute__((always_inline)) {
       load_run<O, V>(src + col, cols, u);
       load_run<O, V>(dy + col, cols, g);
+      float w[V];
+      load_param<O, V>(p.weight, p.weight_dtype, col, cols, 1.0f, w);
       for (int e = 0; e < V; ++e) {
         u[e] = e < cols ? (u[e] - mean) * rstd : 0.0f;
-        g[e] *= e < cols ? param_at(p.weight, col + e, p.weight_dtype, 1.0f) : 0.0f;
+        g[e] *= w[e];
       }
     };
     over([&](int64_t col, int cols) __attribute__((always_inline)) {
@@ -265,7 +375,7 @@ template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_l
   }
 }
 
-// dweight and dbias of such rows: a workgroup's 32 runs of columns down 256 rows, its 8 rows of threads meet in LDS
+// dweight and dbias of such rows, and of those too long for a thread to keep its columns' sums too (CH = 4): a workgroup's 32 runs of columns down 256 rows, its 8 rows of threads meet in LDS
 constexpr int LONG_ROWS = 256;
 template <class O> __global__ __launch_bounds__(256) void norm_columns_kernel(NormParams p) {
   typedef typename O::raw raw;
@@ -326,26 +436,28 @@ __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, in
   }
 }
 
-constexpr int64_t MOST_GROUPS = 512;
-
 // threads and runs of a row; 0: longer than the registers hold
 struct Shape {
   int tpr, ch;
 };
 Shape shape_of(int64_t n, int v) {
-  static const Shape shapes[] = {{64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}};
+  static const Shape shapes[] = {{64, 1}, {64, 2}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
   for (const Shape& s : shapes)
     if (n <= (int64_t)s.tpr * s.ch * v) return s;
   return {0, 0};
 }
 int64_t lines_of(const Shape& s) { return s.tpr < 256 ? 256 / s.tpr : 1; }
+// Workgroups of the backward pass.  Each costs a share of 8 n bytes, written and read, where a row of 16 bits costs 6 n: so 16 rows or
+// more to a line where that leaves every CU a workgroup, and not more than run together.
 int64_t groups_of(const tnx_norm_args* a, const Shape& s) {
-  const int64_t most = (a->rows + lines_of(s) - 1) / lines_of(s);
-  return most < MOST_GROUPS ? most : MOST_GROUPS;
+  const int64_t lines = lines_of(s), most = (a->rows + lines - 1) / lines, together = 256 * (1024 / (s.tpr < 256 ? 256 : s.tpr));
+  int64_t groups = most / 16;
+  groups = groups < 256 ? 256 : groups > together ? together : groups;
+  return groups < most ? groups : most;
 }
 int64_t shares_of(const tnx_norm_args* a) {
   const Shape s = shape_of(a->n, a->dtype == TNX_F32 ? 4 : 8);
-  return s.tpr == 0 ? (a->rows + LONG_ROWS - 1) / LONG_ROWS : groups_of(a, s) * lines_of(s);
+  return s.tpr == 0 || s.ch > 2 ? (a->rows + LONG_ROWS - 1) / LONG_ROWS : groups_of(a, s);
 }
 
 int check(const tnx_norm_args* a) {
@@ -373,14 +485,16 @@ int launched() {
   return TNX_OK;
 }
 
-#define TNX_NORM_SHAPES(DO) DO(64, 1) DO(64, 2) DO(64, 4) DO(256, 2) DO(256, 4) DO(512, 4) DO(1024, 4)
+#define TNX_NORM_SHAPES(DO) DO(64, 1) DO(64, 2) DO(256, 1) DO(512, 1) DO(1024, 1) DO(1024, 2) DO(1024, 4)
 
 template <class O> int forward(const NormParams& p, hipStream_t stream) {
   const Shape s = shape_of(p.n, 16 / sizeof(typename O::raw));
   const unsigned grid = (unsigned)((p.rows + lines_of(s) - 1) / lines_of(s));
+  const bool whole = p.n % (16 / sizeof(typename O::raw)) == 0;
 #define TNX_NORM_FORWARD(TPR, CH)                                                                                       \
   if (s.tpr == TPR && s.ch == CH) {                                                                                     \
-    hipLaunchKernelGGL((norm_kernel<O, TPR, CH>), dim3(grid), dim3(TPR < 256 ? 256 : TPR), 0, stream, p);               \
+    if (whole) hipLaunchKernelGGL((norm_kernel<O, TPR, CH, true>), dim3(grid), dim3(TPR < 256 ? 256 : TPR), 0, stream, p); \
+    else hipLaunchKernelGGL((norm_kernel<O, TPR, CH, false>), dim3(grid), dim3(TPR < 256 ? 256 : TPR), 0, stream, p);   \
     return launched();                                                                                                  \
   }
   TNX_NORM_SHAPES(TNX_NORM_FORWARD)
@@ -391,21 +505,23 @@ template <class O> int forward(const NormParams& p, hipStream_t stream) {
 template <class O> int backward(const tnx_norm_args* a, NormParams p, hipStream_t stream) {
   const Shape s = shape_of(p.n, 16 / sizeof(typename O::raw));
   const int64_t shares = shares_of(a);
-  const bool wanted = a->dweight || a->dbias;
-  if (s.tpr == 0) {
-    if (p.dx) hipLaunchKernelGGL((norm_long_kernel<O, true>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
-    if (wanted)
-      hipLaunchKernelGGL((norm_columns_kernel<O>), dim3((unsigned)((p.n + 32 * (16 / sizeof(typename O::raw)) - 1) / (32 * (16 / sizeof(typename O::raw)))), (unsigned)shares),
-                         dim3(256), 0, stream, p);
-  } else {
-    const unsigned grid = (unsigned)groups_of(a, s);
+  const bool wanted = a->dweight || a->dbias, whole = p.n % (16 / sizeof(typename O::raw)) == 0;
+  const bool apart = s.tpr == 0 || s.ch > 2;             // the parameters' sums by a launch of their own
+  const unsigned grid = (unsigned)(s.tpr ? groups_of(a, s) : 0);
+  if (s.tpr == 0 && p.dx) hipLaunchKernelGGL((norm_long_kernel<O, true>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
 #define TNX_NORM_BACKWARD(TPR, CH)                                                                                      \
-  if (s.tpr == TPR && s.ch == CH) {                                                                                     \
-    if (wanted) hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, true>), dim3(grid), dim3(TPR < 256 ? 256 : TPR), 0, stream, p); \
-    else hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, false>), dim3(grid), dim3(TPR < 256 ? 256 : TPR), 0, stream, p);       \
+  if (s.tpr == TPR && s.ch == CH && (p.dx || !apart)) {                                                                 \
+    constexpr bool SUMS = CH <= 2;                                                                                      \
+    const dim3 threads(TPR < 256 ? 256 : TPR);                                                                          \
+    if (SUMS && wanted && whole) hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, SUMS, true>), dim3(grid), threads, 0, stream, p);  \
+    else if (SUMS && wanted) hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, SUMS, false>), dim3(grid), threads, 0, stream, p);     \
+    else if (whole) hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, false, true>), dim3(grid), threads, 0, stream, p);       \
+    else hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, false, false>), dim3(grid), threads, 0, stream, p);       \
   }
-    TNX_NORM_SHAPES(TNX_NORM_BACKWARD)
-  }
+  TNX_NORM_SHAPES(TNX_NORM_BACKWARD)
+  constexpr int SPAN = 32 * (16 / sizeof(typename O::raw));
+  if (apart && wanted)
+    hipLaunchKernelGGL((norm_columns_kernel<O>), dim3((unsigned)((p.n + SPAN - 1) / SPAN), (unsigned)shares), dim3(256), 0, stream, p);
   if (wanted)
     hipLaunchKernelGGL(norm_parts_kernel, dim3((unsigned)((2 * p.n + 63) / 64)), dim3(1024), 0, stream, p.parts, shares, p.n, (uint8_t*)a->dweight, a->weight_dtype,
                        (uint8_t*)a->dbias, a->bias_dtype);
