@@ -249,3 +249,37 @@ def test_only_what_is_asked_for(device):
     (g,) = torch.autograd.grad(y, both, dy, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_the_residuals_gradient_is_its_own(device):
+    """A gradient that is handed on as it is, accumulated into twice, leaves the caller's tensor alone."""
+    x, w, r = (ref.draw(device, *s, dtype=torch.float32, seed=i).requires_grad_(True) for i, s in enumerate(((4, 16), (16, 32), (4, 32))))
+    dy = ref.draw(device, 4, 32, dtype=torch.float32, seed=5)
+    kept = dy.clone()
+    for _ in range(2):
+        tritonix.linear(x, w, None, "silu", r).backward(dy)
+    assert torch.equal(r.grad, kept + kept) and torch.equal(dy, kept)
+    assert r.grad.data_ptr() != dy.data_ptr()
+
+
+def test_the_interpreters_path_gives_the_same(device, monkeypatch):
+    """Calls that csrc/launch.cpp does not take: the same kernels, the same bits."""
+    from tritonix_amd.ops import mx, native
+
+    x, w, b, r, dy = (ref.draw(device, *s, seed=i) for i, s in enumerate(((40, 64), (64, 2304), (2304,), (40, 2304), (40, 2304))))
+    bounds, e = torch.tensor([0, 7, 7, 40], dtype=torch.int32, device=device), ref.draw(device, 3, 64, 48, seed=9)
+
+    def everything():
+        out = step(x, w, b, "gelu", r, dy)
+        leaves = [t.detach().requires_grad_(True) for t in (x, e)]
+        y = tritonix.grouped_matmul(*leaves, bounds)
+        more = [y.detach(), *torch.autograd.grad(y, leaves, dy[:, :48])]
+        leaves = [t.detach().requires_grad_(True) for t in (r, b, b)]
+        y = tritonix.layer_norm(*leaves)
+        return [*out.values(), *more, y.detach(), *torch.autograd.grad(y, leaves, dy), tritonix.linear(x, w, b), tritonix.layer_norm(x), tritonix.grouped_matmul(x, e, bounds)]
+
+    first = everything()
+    assert native.module is not mx._Interpreter, "the native side is not in use"
+    monkeypatch.setattr(native, "module", mx._Interpreter)
+    for a, c in zip(first, everything()):
+        assert torch.equal(a, c)

@@ -16,7 +16,7 @@ import sys
 import tritonix_amd
 
 _ALIASED = ("autotune", "dispatcher", "testing", "kernel", "ops", "ops.matmul", "ops.swiglu", "ops.conv2d",
-            "ops.conv2d.forward", "ops.mx", "ops.moe", "ops.linear", "ops.norm", "ops.grouped", "utils", "utils.spaces", "utils.pruners")
+            "ops.conv2d.forward", "ops.mx", "ops.moe", "ops.linear", "ops.norm", "ops.grouped", "ops.native", "utils", "utils.spaces", "utils.pruners")
 
 for _name in _ALIASED:
     sys.modules[f"{__name__}.{_name}"] = importlib.import_module(f"tritonix_amd.{_name}")

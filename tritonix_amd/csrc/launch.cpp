@@ -833,6 +833,418 @@ PyObject* moe_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------
+// Linear layers, layer normalisation, grouped products: as above, with their nodes of the autograd graph.  A training step of a small
+// layer was four launches of 10 us each under 110 us of the interpreter's; XX.
+struct BlockEntries {
+  size_t (*linear_workspace)(const tnx_linear_args*);
+  size_t (*linear_scratch)(const tnx_linear_args*);
+  int (*linear)(const tnx_linear_args*);
+  size_t (*gradient_bytes)(const tnx_linear_gradient_args*);
+  int (*gradient)(const tnx_linear_gradient_args*);
+  int (*norm)(const tnx_norm_args*);
+  size_t (*norm_workspace)(const tnx_norm_args*);
+  int (*norm_backward)(const tnx_norm_args*);
+  int (*grouped)(const tnx_grouped_args*);
+  int (*grouped_route)(const tnx_grouped_args*, int32_t*);
+} blocks = {};
+PyObject* fn_counted = nullptr;          // (device index, stream, bytes) -> scratch whose counters are zero
+PyObject* fn_dropped = nullptr;          // (device index, stream): a launch on it reported an error
+
+// bind_blocks(addresses of the above, in their order, counted workspace, its dropping)
+PyObject* bind_blocks(PyObject*, PyObject* arg) {
+  constexpr int N = sizeof(BlockEntries) / sizeof(void*);
+  if (!PyTuple_Check(arg) || PyTuple_GET_SIZE(arg) != N + 2) {
+    PyErr_SetString(PyExc_ValueError, "bind_blocks: not the entry points");
+    return nullptr;
+  }
+  void* at[N];
+  for (int i = 0; i < N; ++i) at[i] = (void*)(uintptr_t)PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(arg, i));
+  if (PyErr_Occurred()) return nullptr;
+  Object counted(PyTuple_GET_ITEM(arg, N)), dropped(PyTuple_GET_ITEM(arg, N + 1));
+  std::swap(fn_counted, counted.p);
+  std::swap(fn_dropped, dropped.p);
+  static_assert(sizeof blocks == sizeof at, "one pointer each");
+  std::memcpy(&blocks, at, sizeof blocks);
+  Py_RETURN_NONE;
+}
+
+// the interpreter lock, on whatever thread this is
+struct Locked {
+  PyGILState_STATE state = PyGILState_Ensure();
+  ~Locked() { PyGILState_Release(state); }
+};
+
+// rows with neighbouring columns that do not overlap
+bool row_major(const at::Tensor& t) { return (t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) == 1 || t.stride(0) >= t.size(1)); }
+bool column_major(const at::Tensor& t) { return t.stride(0) == 1 && t.stride(1) >= t.size(0); }
+
+struct Made {
+  at::Tensor y, z;
+  int status = TNX_OK;
+};
+// y = act(x w + bias) + residual of operands as they lie, and z.  Called without the interpreter lock, which it takes where K is cut.
+Made made_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor* bias, const at::Tensor* residual, int act, bool want_z, c10::DeviceIndex device,
+                 void* stream) {
+  tnx_linear_args a = {};
+  a.x = x.data_ptr(); a.w = w.data_ptr();
+  a.m = x.size(0); a.k = x.size(1); a.n = w.size(1);
+  a.stride_xm = a.m == 1 ? a.k : x.stride(0); a.stride_xk = a.k == 1 ? 1 : x.stride(1);
+  a.stride_wn = a.n == 1 ? 1 : w.stride(1);
+  a.stride_wk = a.k == 1 && a.stride_wn == 1 ? a.n : w.stride(0);
+  a.dtype = float_code(x.scalar_type());
+  if (bias) { a.bias = bias->data_ptr(); a.bias_dtype = float_code(bias->scalar_type()); }
+  if (residual) a.residual = residual->data_ptr();
+  a.activation = act;
+  a.stream = stream;
+  Made r;
+  r.y = fresh({a.m, a.n}, x.scalar_type(), device);
+  if (want_z) r.z = fresh({a.m, a.n}, x.scalar_type(), device);
+  a.y = r.y.data_ptr();
+  a.z = want_z ? r.z.data_ptr() : nullptr;
+  const size_t counted = blocks.linear_workspace(&a), bytes = blocks.linear_scratch(&a);
+  at::Tensor ws, scratch;
+  if (counted) {
+    const Locked locked;
+    const Object got = taken(PyObject_CallFunction(fn_counted, "iKL", (int)device, (unsigned long long)(uintptr_t)stream, (long long)counted));
+    if (!got.p || !tensor_arg(got.p)) {
+      PyErr_Clear();
+      r.status = TNX_E_WORKSPACE;
+      return r;
+    }
+    ws = THPVariable_Unpack(got.p);
+    a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.nbytes();
+  }
+  if (bytes) {
+    scratch = fresh({(int64_t)bytes}, at::kByte, device);
+    a.scratch = scratch.data_ptr(); a.scratch_bytes = bytes;
+  }
+  r.status = blocks.linear(&a);
+  if (r.status == TNX_E_HIP && counted) {
+    const Locked locked;
+    taken(PyObject_CallFunction(fn_dropped, "iK", (int)device, (unsigned long long)(uintptr_t)stream));
+    PyErr_Clear();
+  }
+  return r;
+}
+
+at::Tensor product_of(const at::Tensor& a, const at::Tensor& b, c10::DeviceIndex device, void* stream) {
+  const at::Tensor x = row_major(a) || column_major(a) ? a : a.contiguous(), w = row_major(b) || column_major(b) ? b : b.contiguous();
+  Made r = made_linear(x, w, nullptr, nullptr, TNX_ACT_NONE, false, device, stream);
+  TORCH_CHECK(r.status == TNX_OK, "linear: status ", r.status, " in the backward pass");
+  return r.y;
+}
+
+typedef std::optional<at::Tensor> MaybeTensor;
+
+struct LinearLayer : torch::autograd::Function<LinearLayer> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const MaybeTensor& bias, const MaybeTensor& residual,
+                            int64_t act) {
+    const c10::DeviceIndex device = (c10::DeviceIndex)x.get_device();
+    const bool derived = act != TNX_ACT_NONE && (x.requires_grad() || w.requires_grad() || (bias && bias->requires_grad()));
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    Made r;
+    {
+      const Unlocked unlocked;
+      r = made_linear(x, w, bias ? &*bias : nullptr, residual ? &*residual : nullptr, (int)act, derived, device, stream);
+    }
+    if (r.status != TNX_OK) throw std::runtime_error("linear");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), w, r.z});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = bias ? (int64_t)bias->scalar_type() : (int64_t)-1;
+    ctx->saved_data["residual"] = residual.has_value();
+    return r.y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return torch::autograd::variable_list(5);
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w = saved[1], &z = saved[2];
+    const at::Tensor given = grads[0].detach();
+    TORCH_CHECK(plain(given, 2) && given.size(1) == w.size(1) && given.scalar_type() == w.scalar_type(),
+                "linear: a gradient that is not an ordinary tensor of the result's size and type");
+    const int act = (int)ctx->saved_data["act"].toInt();
+    const int64_t bias_type = ctx->saved_data["bias"].toInt();
+    // (inputs that were not given are not counted)
+    const bool wants_x = ctx->needs_input_grad(0), wants_w = ctx->needs_input_grad(1), wants_bias = bias_type >= 0 && ctx->needs_input_grad(2);
+    const bool wants_residual = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(bias_type >= 0 ? 3 : 2);
+    const c10::DeviceIndex device = (c10::DeviceIndex)given.get_device();
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    at::Tensor dx, dw, dbias;
+    if (wants_x || wants_w || wants_bias) {
+      const at::Tensor dy = given.contiguous();
+      at::Tensor dz = dy;
+      if (act != TNX_ACT_NONE || wants_bias) {
+        tnx_linear_gradient_args a = {};
+        a.dy = dy.data_ptr();
+        a.m = dy.size(0); a.n = dy.size(1);
+        a.dtype = float_code(dy.scalar_type());
+        a.activation = act;
+        if (act != TNX_ACT_NONE) {
+          a.z = z.data_ptr();
+          if (wants_x || wants_w) {
+            dz = fresh({a.m, a.n}, dy.scalar_type(), device);
+            a.dz = dz.data_ptr();
+          }
+        }
+        if (wants_bias) {
+          dbias = fresh({a.n}, (at::ScalarType)bias_type, device);
+          a.dbias = dbias.data_ptr();
+          a.bias_dtype = float_code((at::ScalarType)bias_type);
+        }
+        at::Tensor scratch;
+        if (const size_t bytes = blocks.gradient_bytes(&a)) {
+          scratch = fresh({(int64_t)bytes}, at::kByte, device);
+          a.workspace = scratch.data_ptr(); a.workspace_bytes = bytes;
+        }
+        a.stream = stream;
+        const int status = blocks.gradient(&a);
+        TORCH_CHECK(status == TNX_OK, "linear: status ", status, " in the backward pass");
+      }
+      if (wants_x) dx = product_of(dz, w.t(), device, stream);
+      // (a weight that is the transpose of a row-major one has its gradient so too)
+      if (wants_w) dw = w.stride(0) == 1 && w.stride(1) != 1 ? product_of(dz.t(), x, device, stream).t() : product_of(x.t(), dz, device, stream);
+    }
+    torch::autograd::variable_list out = gradients({dx, dw, dbias}, 5, "linear has no second derivative");
+    // (the gradient itself, not another tensor of its memory: who takes it as his own looks whether others hold the tensor)
+    if (wants_residual) out[3] = grads[0];
+    return out;
+  }
+};
+
+// linear(x, w, bias or None, residual or None, tnx_activation) -> y with its place in the graph, or None
+PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) Py_RETURN_NONE;
+  try {
+    const at::Tensor *x, *w, *bias = nullptr, *residual = nullptr;
+    c10::DeviceIndex device = -1;
+    int64_t v[1];
+    if (!here(args[0], 2, &x, &device) || !here(args[1], 2, &w, &device) || !integers(args + 4, v)) Py_RETURN_NONE;
+    const at::ScalarType type = x->scalar_type();
+    if (x->size(1) != w->size(0) || type != w->scalar_type() || float_code(type) < 0 || x->numel() == 0 || w->size(0) < 16 || w->size(1) < 16 || !row_major(*x) ||
+        !(row_major(*w) || column_major(*w)))
+      Py_RETURN_NONE;
+    if (args[2] != Py_None && (!here(args[2], 1, &bias, &device) || bias->size(0) != w->size(1) || !bias->is_contiguous() ||
+                               (bias->scalar_type() != type && bias->scalar_type() != at::kFloat)))
+      Py_RETURN_NONE;
+    if (args[3] != Py_None && (!here(args[3], 2, &residual, &device) || residual->size(0) != x->size(0) || residual->size(1) != w->size(1) ||
+                               !residual->is_contiguous() || residual->scalar_type() != type))
+      Py_RETURN_NONE;
+    if (at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad() || (bias && bias->requires_grad()) || (residual && residual->requires_grad())))
+      return THPVariable_Wrap(LinearLayer::apply(*x, *w, bias ? MaybeTensor(*bias) : MaybeTensor(), residual ? MaybeTensor(*residual) : MaybeTensor(), v[0]));
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    Made r;
+    {
+      const Unlocked unlocked;
+      r = made_linear(*x, *w, bias, residual, (int)v[0], false, device, stream);
+    }
+    if (r.status != TNX_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(r.y);
+  } catch (...) {
+    return none();
+  }
+}
+
+tnx_norm_args norm_args(const at::Tensor& x, const at::Tensor* weight, const at::Tensor* bias, float eps, void* stream) {
+  tnx_norm_args a = {};
+  a.x = x.data_ptr();
+  a.rows = x.size(0); a.n = x.size(1); a.stride_x = x.stride(0);
+  a.dtype = float_code(x.scalar_type());
+  a.eps = eps;
+  if (weight) { a.weight = weight->data_ptr(); a.weight_dtype = float_code(weight->scalar_type()); }
+  if (bias) { a.bias = bias->data_ptr(); a.bias_dtype = float_code(bias->scalar_type()); }
+  a.stream = stream;
+  return a;
+}
+
+struct NormLayer : torch::autograd::Function<NormLayer> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
+    const c10::DeviceIndex device = (c10::DeviceIndex)x.get_device();
+    tnx_norm_args a = norm_args(x, weight ? &*weight : nullptr, bias ? &*bias : nullptr, (float)eps, c10::hip::getCurrentHIPStream(device).stream());
+    at::Tensor y, statistics;
+    int status;
+    {
+      const Unlocked unlocked;
+      y = fresh({a.rows, a.n}, x.scalar_type(), device);
+      statistics = fresh({2, a.rows}, at::kFloat, device);
+      a.y = y.data_ptr();
+      a.mean = (float*)statistics.data_ptr();
+      a.rstd = a.mean + a.rows;
+      status = blocks.norm(&a);
+    }
+    if (status != TNX_OK) throw std::runtime_error("layer_norm");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, weight ? *weight : at::Tensor(), bias ? *bias : at::Tensor(), statistics});
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return torch::autograd::variable_list(4);
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &statistics = saved[3];
+    const at::Tensor given = grads[0].detach();
+    TORCH_CHECK(plain(given, 2) && given.sizes() == x.sizes() && given.scalar_type() == x.scalar_type(),
+                "layer_norm: a gradient that is not an ordinary tensor of the result's size and type");
+    const at::Tensor dy = given.stride(1) == 1 || given.size(1) <= 1 ? given : given.contiguous();
+    const c10::DeviceIndex device = (c10::DeviceIndex)dy.get_device();
+    tnx_norm_args a = norm_args(x, weight.defined() ? &weight : nullptr, bias.defined() ? &bias : nullptr, (float)ctx->saved_data["eps"].toDouble(),
+                                c10::hip::getCurrentHIPStream(device).stream());
+    a.mean = (float*)statistics.data_ptr();
+    a.rstd = a.mean + a.rows;
+    a.dy = dy.data_ptr();
+    a.stride_dy = dy.stride(0);
+    at::Tensor dx, dweight, dbias, scratch;
+    if (ctx->needs_input_grad(0)) {
+      dx = fresh({a.rows, a.n}, x.scalar_type(), device);
+      a.dx = dx.data_ptr();
+    }
+    if (weight.defined() && ctx->needs_input_grad(1)) {
+      dweight = fresh({a.n}, weight.scalar_type(), device);
+      a.dweight = dweight.data_ptr();
+    }
+    if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1)) {       // (inputs that were not given are not counted)
+      dbias = fresh({a.n}, bias.scalar_type(), device);
+      a.dbias = dbias.data_ptr();
+    }
+    if (const size_t bytes = blocks.norm_workspace(&a)) {
+      scratch = fresh({(int64_t)bytes}, at::kByte, device);
+      a.workspace = scratch.data_ptr(); a.workspace_bytes = bytes;
+    }
+    const int status = blocks.norm_backward(&a);
+    TORCH_CHECK(status == TNX_OK, "layer_norm: status ", status, " in the backward pass");
+    return gradients({dx, dweight, dbias}, 4, "layer_norm has no second derivative");
+  }
+};
+
+// layer_norm(x, weight or None, bias or None, eps) -> y with its place in the graph, or None
+PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4 || !PyFloat_Check(args[3])) Py_RETURN_NONE;
+  try {
+    const at::Tensor *x, *p[2] = {nullptr, nullptr};
+    c10::DeviceIndex device = -1;
+    const double eps = PyFloat_AS_DOUBLE(args[3]);
+    if (!here(args[0], 2, &x, &device) || float_code(x->scalar_type()) < 0 || x->numel() == 0 || !(x->stride(1) == 1 || x->size(1) == 1) || !(eps >= 0.0))
+      Py_RETURN_NONE;
+    for (int i = 0; i < 2; ++i) {
+      if (args[1 + i] == Py_None) continue;
+      if (!here(args[1 + i], 1, &p[i], &device) || p[i]->size(0) != x->size(1) || !p[i]->is_contiguous() ||
+          (p[i]->scalar_type() != x->scalar_type() && p[i]->scalar_type() != at::kFloat))
+        Py_RETURN_NONE;
+    }
+    if (at::GradMode::is_enabled() && (x->requires_grad() || (p[0] && p[0]->requires_grad()) || (p[1] && p[1]->requires_grad())))
+      return THPVariable_Wrap(NormLayer::apply(*x, p[0] ? MaybeTensor(*p[0]) : MaybeTensor(), p[1] ? MaybeTensor(*p[1]) : MaybeTensor(), eps));
+    tnx_norm_args a = norm_args(*x, p[0], p[1], (float)eps, c10::hip::getCurrentHIPStream(device).stream());
+    at::Tensor y;
+    int status;
+    {
+      const Unlocked unlocked;
+      y = fresh({a.rows, a.n}, x->scalar_type(), device);
+      a.y = y.data_ptr();
+      status = blocks.norm(&a);
+    }
+    if (status != TNX_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(y);
+  } catch (...) {
+    return none();
+  }
+}
+
+// Operands of a grouped product as they lie: a with rows that do not overlap, matrices that are row-major or k-contiguous.
+bool grouped_weights(const at::Tensor& w) {
+  return (w.stride(2) == 1 && w.stride(1) >= w.size(2)) || (w.stride(1) == 1 && w.stride(2) >= w.size(1));
+}
+tnx_grouped_args grouped_args(int form, const at::Tensor& a, const at::Tensor& b, const at::Tensor& offsets, int64_t n, int64_t k, int64_t group, int64_t bk,
+                              int64_t bn, void* stream) {
+  tnx_grouped_args g = {};
+  g.a = a.data_ptr(); g.b = b.data_ptr();
+  g.offsets = (const int32_t*)offsets.data_ptr();
+  g.rows = a.size(0); g.n = n; g.k = k;
+  g.stride_ar = a.size(0) == 1 ? a.size(1) : a.stride(0); g.stride_ak = 1;
+  g.stride_group = group; g.stride_bk = bk; g.stride_bn = bn;
+  g.groups = (int32_t)(offsets.numel() - 1); g.dtype = float_code(a.scalar_type()); g.form = form;
+  g.stream = stream;
+  return g;
+}
+int rows_product(const at::Tensor& x, const at::Tensor& w, const at::Tensor& offsets, c10::DeviceIndex device, void* stream, at::Tensor* y) {
+  tnx_grouped_args g = grouped_args(TNX_GROUPED_ROWS, x, w, offsets, w.size(2), x.size(1), w.stride(0), w.stride(1), w.stride(2), stream);
+  *y = fresh({g.rows, g.n}, x.scalar_type(), device);
+  g.c = y->data_ptr();
+  return blocks.grouped(&g);
+}
+int weight_gradient(const at::Tensor& x, const at::Tensor& dy, const at::Tensor& offsets, c10::DeviceIndex device, void* stream, at::Tensor* dw) {
+  const int64_t k = x.size(1), n = dy.size(1);
+  tnx_grouped_args g = grouped_args(TNX_GROUPED_WEIGHT_GRADIENT, x, dy, offsets, n, k, k * n, dy.size(0) == 1 ? n : dy.stride(0), 1, stream);
+  *dw = fresh({(int64_t)g.groups, k, n}, x.scalar_type(), device);
+  g.c = dw->data_ptr();
+  return blocks.grouped(&g);
+}
+
+struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& offsets) {
+    const c10::DeviceIndex device = (c10::DeviceIndex)x.get_device();
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    at::Tensor y;
+    int status;
+    {
+      const Unlocked unlocked;
+      status = rows_product(x, w, offsets, device, stream, &y);
+    }
+    if (status != TNX_OK) throw std::runtime_error("grouped_matmul");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), w, offsets});
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return torch::autograd::variable_list(3);
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
+    at::Tensor dy = grads[0].detach();
+    TORCH_CHECK(plain(dy, 2) && dy.size(1) == w.size(2) && dy.scalar_type() == w.scalar_type(),
+                "grouped_matmul: a gradient that is not an ordinary tensor of the result's size and type");
+    if (!row_major(dy)) dy = dy.contiguous();
+    const c10::DeviceIndex device = (c10::DeviceIndex)dy.get_device();
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    at::Tensor dx, dw;
+    int status = TNX_OK;
+    if (ctx->needs_input_grad(0)) status = rows_product(dy, w.transpose(1, 2), offsets, device, stream, &dx);
+    if (status == TNX_OK && ctx->needs_input_grad(1)) {
+      // (as a linear layer's)
+      const bool transposed = w.stride(1) == 1 && w.stride(2) != 1;
+      status = transposed ? weight_gradient(dy, x, offsets, device, stream, &dw) : weight_gradient(x, dy, offsets, device, stream, &dw);
+      if (transposed) dw = dw.transpose(1, 2);
+    }
+    TORCH_CHECK(status == TNX_OK, "grouped_matmul: status ", status, " in the backward pass");
+    return gradients({dx, dw}, 3, "grouped_matmul has no second derivative");
+  }
+};
+
+// grouped_matmul(x, w, offsets) -> y with its place in the graph, or None
+PyObject* grouped_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 3) Py_RETURN_NONE;
+  try {
+    const at::Tensor *x, *w, *offsets;
+    c10::DeviceIndex device = -1;
+    if (!here(args[0], 2, &x, &device) || !here(args[1], 3, &w, &device) || !here(args[2], 1, &offsets, &device)) Py_RETURN_NONE;
+    // (rows shorter than a chunk may have to be padded)
+    if (x->size(1) != w->size(1) || w->size(1) < 8 || w->size(2) < 8 || x->size(0) == 0 || w->size(0) < 1 || w->size(0) > TNX_GROUPED_MAX_GROUPS ||
+        offsets->size(0) != w->size(0) + 1 || offsets->scalar_type() != at::kInt || !offsets->is_contiguous() || float_code(x->scalar_type()) < 0 ||
+        w->scalar_type() != x->scalar_type() || !row_major(*x) || !grouped_weights(*w))
+      Py_RETURN_NONE;
+    if (at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad())) return THPVariable_Wrap(GroupedProduct::apply(*x, *w, *offsets));
+    void* stream = c10::hip::getCurrentHIPStream(device).stream();
+    at::Tensor y;
+    int status;
+    {
+      const Unlocked unlocked;
+      status = rows_product(*x, *w, *offsets, device, stream, &y);
+    }
+    if (status != TNX_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(y);
+  } catch (...) {
+    return none();
+  }
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
     {"keep", keep, METH_VARARGS, nullptr},
@@ -849,6 +1261,10 @@ PyMethodDef methods[] = {
     {"mx_linear", (PyCFunction)(void (*)(void))mx_linear, METH_FASTCALL, nullptr},
     {"moe_route", (PyCFunction)(void (*)(void))moe_route, METH_FASTCALL, nullptr},
     {"moe_backward", (PyCFunction)(void (*)(void))moe_backward, METH_FASTCALL, nullptr},
+    {"bind_blocks", bind_blocks, METH_O, nullptr},
+    {"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, nullptr},
+    {"layer_norm", (PyCFunction)(void (*)(void))layer_norm, METH_FASTCALL, nullptr},
+    {"grouped_matmul", (PyCFunction)(void (*)(void))grouped_matmul, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -13,6 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tritonix_amd import _C
+from tritonix_amd.ops import native as _native
 from tritonix_amd.ops.mx import dtype_code, launch, on_device
 
 __all__ = ["grouped_matmul"]
@@ -93,6 +94,8 @@ def _weight_gradient(x, dy, offsets) -> torch.Tensor:
 
 
 class _Grouped(torch.autograd.Function):
+    """What the native side has not taken."""
+
     @staticmethod
     def forward(ctx, x, w, offsets):
         ctx.set_materialize_grads(False)
@@ -123,6 +126,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> t
     ``offsets[groups]`` on, are zero.  w may be the transpose of row-major ``[groups, n, k]`` weights.
 
     Differentiable in x and w: rows of no group have zero gradients, and so has the weight of a group without rows."""
+    y = (_native.module or _native.find()).grouped_matmul(x, w, offsets)
+    if y is not None:
+        return y
     if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[1]:
         raise ValueError(f"grouped_matmul expects x[rows, k] and w[groups, k, n], got {tuple(x.shape)} and {tuple(w.shape)}")
     groups = w.shape[0]

@@ -17,6 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from tritonix_amd import _C
 from tritonix_amd import kernel as _kernel
+from tritonix_amd.ops import native as _native
 from tritonix_amd.ops.mx import dtype_code, on_device, raise_for_status
 
 _mm = importlib.import_module("tritonix_amd.ops.matmul")
@@ -24,17 +25,6 @@ _mm = importlib.import_module("tritonix_amd.ops.matmul")
 __all__ = ["linear"]
 
 ACTIVATIONS = {None: _C.ACT_NONE, "relu": _C.ACT_RELU, "silu": _C.ACT_SILU, "gelu": _C.ACT_GELU, "gelu_tanh": _C.ACT_GELU_TANH}
-
-
-def counted_workspace(index: int, stream: int, nbytes: int) -> torch.Tensor:
-    """Scratch of products whose K is cut, its counters zero: the stream's own buffer or, for a launch that is recorded into a HIP graph, one
-    of the graph's (two graphs of one stream may be replayed on two)."""
-    device = torch.device("cuda", index)
-    if _kernel._capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        ws[:_C.WS_COUNTER_BYTES].zero_()
-        return ws
-    return _kernel._workspace(device, stream, nbytes)
 
 
 def _go(index: int, x, w, bias, residual, activation: int, want_z: bool):
@@ -57,7 +47,7 @@ def _go(index: int, x, w, bias, residual, activation: int, want_z: bool):
     need, scratch_bytes = int(lib.tnx_linear_workspace_bytes(ctypes.byref(a))), int(lib.tnx_linear_scratch_bytes(ctypes.byref(a)))
     ws = scratch = None
     if need:
-        ws = counted_workspace(index, stream, need)
+        ws = _native.counted_workspace(index, stream, need)
         a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     if scratch_bytes:
         scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=x.device)
@@ -108,6 +98,8 @@ def _transposed(w) -> bool:
 
 
 class _Linear(torch.autograd.Function):
+    """What the native side has not taken."""
+
     @staticmethod
     def forward(ctx, x, w, bias, residual, activation):
         derived = activation != _C.ACT_NONE and any(ctx.needs_input_grad[:3])
@@ -150,7 +142,11 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     Differentiable in x, w, bias and residual.  act' is taken at z = x @ w + bias as it was kept, rounded to x's dtype; dz = dy * act'(z) is
     rounded to it for the products dx = dz @ w.t() and dw = x.t() @ dz, the bias' gradient sums it in 32 bits, in an order that depends on the sizes alone."""
     act = ACTIVATIONS.get(activation)
-    if act is None:
+    if act is not None:
+        y = (_native.module or _native.find()).linear(x, w, bias, residual, act)
+        if y is not None:
+            return y
+    else:
         raise ValueError(f"linear: activation is None, 'relu', 'silu', 'gelu' or 'gelu_tanh', got {activation!r}")
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[0]:
         raise ValueError(f"linear expects x[..., k] and w[k, n], got {tuple(x.shape)} and {tuple(w.shape)}")

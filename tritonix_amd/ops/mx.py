@@ -42,6 +42,7 @@ class _Interpreter:
         return None
 
     mx_quantize = mx_dequantize = mx_product = mx_linear = moe_route = moe_backward = _none
+    linear = layer_norm = grouped_matmul = _none
 
 
 # csrc/launch.cpp, which makes the ordinary calls without the interpreter's share of them; found with the first call

@@ -15,6 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from tritonix_amd import _C
 from tritonix_amd import kernel as _kernel
+from tritonix_amd.ops import native as _native
 from tritonix_amd.ops.mx import dtype_code, launch, on_device, raise_for_status
 
 __all__ = ["layer_norm"]
@@ -49,6 +50,8 @@ def _forward(x, weight, bias, eps: float, statistics: bool):
 
 
 class _LayerNorm(torch.autograd.Function):
+    """What the native side has not taken."""
+
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         y, mean, rstd = _forward(x, weight, bias, eps, True)
@@ -90,6 +93,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     ``weight[n]`` and ``bias[n]``, of x's dtype or float32, may be left out.  The result has x's dtype and shape, rounded once.  A row with a
     NaN or an infinity is NaN.  Differentiable in x, weight and bias."""
+    y = (_native.module or _native.find()).layer_norm(x, weight, bias, eps)
+    if y is not None:
+        return y
     if x.dim() < 1:
         raise ValueError("layer_norm expects x[..., n], got a scalar")
     n = x.shape[-1]
