@@ -577,12 +577,17 @@ typedef struct tnx_grouped_args {
   int64_t stride_bk, stride_bn;
   int32_t groups, dtype, form, reserved;
   int32_t block_m, block_n;    /* a built tile, or 0: the library chooses */
+  int32_t parts, reserved2;    /* with a tile given: parts that k is cut in, each a workgroup's, added up in order by a second launch (0: one) */
   void* stream;
+  void* workspace;             /* tnx_grouped_workspace_bytes, 16-byte aligned, no initialisation; null: k is not cut */
+  size_t workspace_bytes;
 } tnx_grouped_args;
+/* scratch that a product is faster with (few tiles of a long k), or 0.  Host arithmetic on the sizes */
+size_t tnx_grouped_workspace_bytes(const tnx_grouped_args* args);
 int tnx_grouped(const tnx_grouped_args* args);
 /* For tests and tooling: 1, or 0 where tnx_grouped would refuse these args (of the pointers only the alignment counts).  info (may be NULL): rows and
- * columns of a tile, waves, whether each group's last slab of k is loaded apart. */
-int tnx_grouped_route(const tnx_grouped_args* args, int32_t info[4]);
+ * columns of a tile, waves, whether each group's last slab of k is loaded apart, parts of k (given a workspace). */
+int tnx_grouped_route(const tnx_grouped_args* args, int32_t info[5]);
 
 #ifdef __cplusplus
 }

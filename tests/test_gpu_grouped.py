@@ -103,6 +103,33 @@ def test_every_tile(device, dtype, tile, aligned, monkeypatch):
         ref.check("dw", module._weight_gradient(x, dy, offsets), want["dw"], dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tile", range(6))
+@pytest.mark.parametrize("parts", [2, 3, 7, 40])
+def test_k_in_parts(device, dtype, tile, parts, monkeypatch):
+    """k, or a group's rows, cut in parts: more of them than a group has slabs, the last one short."""
+    tiles = [(128, 128), (64, 128), (64, 64), (32, 128), (32, 64), (64, 64)] if dtype != torch.float32 else TILES[torch.float32] * 2
+    made, (bm, bn) = module._args, tiles[tile]
+
+    def with_parts(form, *args):
+        g = made(form, *args)
+        g.block_m, g.block_n, g.parts = bm, bn, parts
+        return g
+
+    monkeypatch.setattr(module, "_args", with_parts)
+    counts, ahead, behind = [bm + 1, 0, 1, 3, 530], 5, 9
+    rows = ahead + sum(counts) + behind
+    offsets = offsets_of(device, counts, ahead)
+    for k, n in ((512, bn + 64), (333, bn + 37), (40, 72)):
+        x, dy = ref.draw(device, rows, k, dtype=dtype, seed=1), ref.draw(device, rows, n, dtype=dtype, seed=3)
+        for layout in ("nn", "nt"):
+            w = weights(device, len(counts), k, n, dtype, layout, 2)
+            want = ref.grouped(x, w, offsets, dy)
+            ref.check(f"y {k} {layout}", module._rows_product(x, w, offsets), want["y"], dtype)
+        if bm >= 64 or dtype == torch.float32:
+            ref.check(f"dw {k}", module._weight_gradient(x, dy, offsets), want["dw"], dtype)
+
+
 @pytest.mark.parametrize("bounds", [[-5, 10, 20, 30], [0, 30, 10, 40], [50, 40, 30, 20], [0, 2 ** 31 - 1, 5, 7], [7, 7, 7, 7], [-(2 ** 31), -1, 0, 0], [40, 40, 40, 99]])
 def test_bounds_outside_of_the_rows(device, bounds):
     """Whatever the bounds hold, they are taken into the rows and to a sequence that does not decrease."""

@@ -42,7 +42,7 @@ EXPORTS = ("tnx_gemm", "tnx_gemm_static_workspace", "tnx_gemm_workspace_bytes", 
            "tnx_mx_code_bytes", "tnx_mx_scale_bytes", "tnx_mx_quantize", "tnx_mx_quantize_both", "tnx_mx_dequantize", "tnx_mx_import", "tnx_mx_gemm", "tnx_mx_gemm_workspace_bytes", "tnx_mx_gemm_takes_rows", "tnx_mx_gemm_route",
            "tnx_moe_workspace_bytes", "tnx_moe_route", "tnx_moe_plan", "tnx_moe_route_backward", "tnx_moe_combine",
            "tnx_linear_workspace_bytes", "tnx_linear_scratch_bytes", "tnx_linear", "tnx_linear_route", "tnx_linear_gradient_bytes", "tnx_linear_gradient",
-           "tnx_layer_norm", "tnx_layer_norm_workspace_bytes", "tnx_layer_norm_backward", "tnx_grouped", "tnx_grouped_route")
+           "tnx_layer_norm", "tnx_layer_norm_workspace_bytes", "tnx_layer_norm_backward", "tnx_grouped", "tnx_grouped_workspace_bytes", "tnx_grouped_route")
 # limits of the routing entry points
 MOE_MAX_EXPERTS, MOE_MAX_TOP_K, MOE_MAX_GROUPS = 1024, 32, 64
 # enum tnx_activation
@@ -161,7 +161,8 @@ class GroupedArgs(ctypes.Structure):
     _fields_ = [
         *[(n, ctypes.c_void_p) for n in ("a", "b", "c", "offsets")],
         *[(n, ctypes.c_int64) for n in ("rows", "n", "k", "stride_ar", "stride_ak", "stride_group", "stride_bk", "stride_bn")],
-        *[(n, ctypes.c_int32) for n in ("groups", "dtype", "form", "reserved", "block_m", "block_n")], ("stream", ctypes.c_void_p),
+        *[(n, ctypes.c_int32) for n in ("groups", "dtype", "form", "reserved", "block_m", "block_n", "parts", "reserved2")], ("stream", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -253,6 +254,7 @@ def load() -> ctypes.CDLL:
             ("tnx_layer_norm", [ctypes.POINTER(NormArgs)], ctypes.c_int),
             ("tnx_layer_norm_workspace_bytes", [ctypes.POINTER(NormArgs)], ctypes.c_size_t),
             ("tnx_layer_norm_backward", [ctypes.POINTER(NormArgs)], ctypes.c_int), ("tnx_grouped", [ctypes.POINTER(GroupedArgs)], ctypes.c_int),
+            ("tnx_grouped_workspace_bytes", [ctypes.POINTER(GroupedArgs)], ctypes.c_size_t),
             ("tnx_grouped_route", [ctypes.POINTER(GroupedArgs), ctypes.POINTER(i32)], ctypes.c_int)):
         getattr(lib, name).argtypes = args
         getattr(lib, name).restype = res

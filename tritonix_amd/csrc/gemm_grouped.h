@@ -7,6 +7,9 @@
 // finds its tile in the bounds, 64 groups at a time by a scan over the wave, then the tile kernel runs on the group as if it were the
 // whole problem.  Nothing waits for the host, nothing is launched ahead.
 //
+// Few tiles of a long k: PARTS workgroups to a tile, each over a part of k (of the group's rows), 32-bit sums in a workspace, and a launch that
+// adds the parts up in order (grouped.hip).
+//
 // The bounds are data: taken into [0, rows] and to a sequence that does not decrease, so that whatever they hold every row belongs to
 // one group or to none, is written once, and nothing outside the tensors is touched.  Rows of no group, ahead of the first and behind the
 // last, are written as zeros: a tile whose k is 0.
@@ -24,6 +27,8 @@ struct GroupedParams {
   int64_t group_stride;      // elements from a group's matrix to the next: of b, AT: of c
   int32_t rows, n, k;        // AT: k is the number of a's columns, the rows of c
   int32_t groups, group_m;
+  int32_t parts, per_part;   // PARTS: workgroups to a tile, slabs of k of each (rows times weights)
+  int64_t part_stride;       // PARTS: elements from a part of c to the next
   uint32_t flags;            // PF_TAIL
 };
 static_assert(sizeof(GroupedParams) <= 112, "a longer argument list costs every launch 0.7 us");
@@ -46,8 +51,16 @@ __device__ __forceinline__ int scan_max(int x) {
 }
 __device__ __forceinline__ int clamp_to(int v, int most) { return v < 0 ? 0 : v > most ? most : v; }
 
-struct GroupedFamily {
-  static constexpr bool LINEAR = false, GROUPED = true;
+// Workgroups are dealt to the 8 XCDs in turn.  In windows of W of them each XCD takes W / 8 neighbouring tiles, which share rows or weights through
+// its L2, and all XCDs are in the same few groups: with a run of the whole list for each XCD instead, the XCD of the longest groups is
+// the last one (weights' gradient, 16384 rows in 8 uneven groups, 4096 x 4096: 786 us, in windows of 64 451; 32768 in 32, 2048 x 2048: 395, 291).
+template <int W> __device__ __forceinline__ int windowed(int bid, int total) {
+  const int first = bid - bid % W, size = total - first < W ? total - first : W;
+  return first + xcd_remap(bid - first, size, 8);
+}
+
+template <bool PARTS> struct GroupedFamily {
+  static constexpr bool LINEAR = false, GROUPED = true, SUMS = PARTS;
   template <bool> using params = GroupedParams;
 
   template <class C, bool BT, bool AT> static __device__ __forceinline__ GemmParams expand(const GroupedParams& q) {
@@ -104,9 +117,19 @@ struct GroupedFamily {
 
   template <class C, bool AT>
   static __device__ __forceinline__ bool find(const GroupedParams& q, GemmParams& p, int bid, int grid, int lane, int* pid_m, int* pid_n) {
+    constexpr int OUT = PARTS ? 4 : C::ES;
+    int part = 0;
+    if constexpr (PARTS) {
+      // (part after part, each over all tiles)
+      grid /= q.parts;
+      const int tile = bid % grid;
+      part = bid / grid;
+      bid = tile;
+      p.c += (int64_t)part * q.part_stride * 4;
+    }
     if constexpr (AT) {
       const int per = p.tiles_m * p.tiles_n;
-      const int id = xcd_remap(bid, grid, 8), g = id / per, r = id - g * per;
+      const int id = windowed<64>(bid, grid), g = id / per, r = id - g * per;
       swizzle2d(r / p.tiles_n, r % p.tiles_n, p.tiles_m, p.tiles_n, p.group_m, pid_m, pid_n);
       int first = 0;
       for (int base = 0; base <= g; base += 64) {
@@ -114,11 +137,17 @@ struct GroupedFamily {
         const int top = __builtin_amdgcn_readlane(scan_max(i <= g ? clamp_to(q.offsets[i], q.rows) : 0), 63);
         first = top > first ? top : first;
       }
-      const int next = clamp_to(q.offsets[g + 1], q.rows), end = __builtin_amdgcn_readfirstlane(next > first ? next : first);
+      const int next = clamp_to(q.offsets[g + 1], q.rows);
+      int end = __builtin_amdgcn_readfirstlane(next > first ? next : first);
+      if constexpr (PARTS) {
+        const int slabs = (int)((uint32_t)(end - first + C::BK - 1) / C::BK), span = (int)((uint32_t)(slabs + q.parts - 1) / (uint32_t)q.parts) * C::BK;
+        first = first + part * span < end ? first + part * span : end;
+        end = first + span < end ? first + span : end;
+      }
       p.k = end - first;
       p.a += (int64_t)first * q.lda * C::ES;
       p.b += (int64_t)first * q.ldb * C::ES;
-      p.c += (int64_t)g * q.group_stride * C::ES;
+      p.c += (int64_t)g * q.group_stride * OUT;
       p.tail_slab = p.tail_slab || p.k % C::BK != 0;
       return true;
     } else {
@@ -126,17 +155,23 @@ struct GroupedFamily {
       stretch_of<C::BM>(q, lane, -1, &total);
       const int tiles = total * p.tiles_n;
       if (bid >= tiles) return false;
-      const int id = xcd_remap(bid, tiles, 8);
+      const int id = windowed<128>(bid, tiles);
       const Stretch s = stretch_of<C::BM>(q, lane, id / p.tiles_n, &total);
       const int r = id - s.before * p.tiles_n;
       p.tiles_m = (int)(((uint32_t)s.rows + C::BM - 1) / C::BM);
       swizzle2d(r / p.tiles_n, r % p.tiles_n, p.tiles_m, p.tiles_n, p.group_m, pid_m, pid_n);
       const bool none = s.number == 0 || s.number == q.groups + 1;
       p.m = p.m_load = s.rows;
-      p.k = none ? 0 : p.k;
       p.a += (int64_t)s.first * q.lda * C::ES;
       p.b += none ? 0 : (int64_t)(s.number - 1) * q.group_stride * C::ES;
-      p.c += (int64_t)s.first * q.n * C::ES;
+      if constexpr (PARTS) {
+        const int64_t start = (int64_t)part * q.per_part * C::BK, span = (int64_t)q.per_part * C::BK;
+        p.a += start * C::ES;
+        p.b += start * (p.sbk == 1 ? 1 : p.sbk) * C::ES;
+        p.k = p.k - start < span ? p.k - start : span;
+      }
+      p.k = none ? 0 : p.k;
+      p.c += (int64_t)s.first * q.n * OUT;
       p.b_once = p.tiles_m == 1;
       return true;
     }
@@ -147,26 +182,35 @@ typedef hipError_t (*grouped_fn)(const GroupedParams& p, unsigned grid, hipStrea
 struct GroupedEntry {
   int dtype, bm, bn, nw, stages;
   grouped_fn nn, bt, at;      // row-major and k-contiguous weights; the weights' gradient
+  grouped_fn parts[3];        // the same in parts; may be null
 };
 struct GroupedGroup {
   GroupedEntry* entries;
   int count;
 };
 
-template <class T, class C, bool BT, bool AT> hipError_t launch_grouped(const GroupedParams& p, unsigned grid, hipStream_t stream) {
+template <class T, class C, bool BT, bool AT, bool PARTS = false> hipError_t launch_grouped(const GroupedParams& p, unsigned grid, hipStream_t stream) {
   GroupedParams q = p;
-  return launch_kernel((const void*)&gemm_tile_kernel<T, C, true, false, BT, false, false, AT, false, GroupedFamily>, grid, C::THREADS, 0, stream, &q);
+  return launch_kernel((const void*)&gemm_tile_kernel<T, C, true, false, BT, false, false, AT, false, GroupedFamily<PARTS>>, grid, C::THREADS, 0, stream, &q);
 }
-template <class T, class C, bool OK = C::VALID_AT> struct GroupedAt {
+template <class T, class C, bool PARTS, bool OK = C::VALID_AT> struct GroupedAt {
   static constexpr grouped_fn fn = nullptr;
 };
-template <class T, class C> struct GroupedAt<T, C, true> {
-  static constexpr grouped_fn fn = &launch_grouped<T, C, false, true>;
+template <class T, class C, bool PARTS> struct GroupedAt<T, C, PARTS, true> {
+  static constexpr grouped_fn fn = &launch_grouped<T, C, false, true, PARTS>;
+};
+template <class T, class C, bool OK = (C::BM * C::BN <= 128 * 128)> struct GroupedParts {
+  static constexpr grouped_fn nn = nullptr, bt = nullptr, at = nullptr;
+};
+template <class T, class C> struct GroupedParts<T, C, true> {
+  static constexpr grouped_fn nn = &launch_grouped<T, C, false, false, true>, bt = &launch_grouped<T, C, true, false, true>, at = GroupedAt<T, C, true>::fn;
 };
 
 #define TNX_GROUPED_ENTRY(TAG, BM, BN, NW, ST)                                                                     \
   {TAG::ID, BM, BN, NW, ST, &launch_grouped<TAG, TileCfg<TAG, BM, BN, 128 / TAG::ES, NW, ST>, false, false>,       \
    &launch_grouped<TAG, TileCfg<TAG, BM, BN, 128 / TAG::ES, NW, ST>, true, false>,                                 \
-   GroupedAt<TAG, TileCfg<TAG, BM, BN, 128 / TAG::ES, NW, ST>>::fn}
+   GroupedAt<TAG, TileCfg<TAG, BM, BN, 128 / TAG::ES, NW, ST>, false>::fn,                                         \
+   {GroupedParts<TAG, TileCfg<TAG, BM, BN, 128 / TAG::ES, NW, ST>>::nn, GroupedParts<TAG, TileCfg<TAG, BM, BN, 128 / TAG::ES, NW, ST>>::bt, \
+    GroupedParts<TAG, TileCfg<TAG, BM, BN, 128 / TAG::ES, NW, ST>>::at}}
 
 }  // namespace tnx

@@ -60,7 +60,7 @@ template <class O, int N> struct Run {
 };
 
 struct LinearFamily {
-  static constexpr bool LINEAR = true, GROUPED = false;
+  static constexpr bool LINEAR = true, GROUPED = false, SUMS = false;
   template <bool> using params = LinearParams;
 
   template <class C, bool BT, bool AT> static __device__ __forceinline__ GemmParams expand(const LinearParams& q) {

@@ -353,7 +353,7 @@ template <> struct KernelParams<true> { typedef PlainParams type; };
 // What a kernel family adds to the plain product: another argument struct (at most 112 bytes), its own way from a workgroup to its tile,
 // its own epilogue.  See gemm_linear.h and gemm_grouped.h.
 struct PlainFamily {
-  static constexpr bool LINEAR = false, GROUPED = false;
+  static constexpr bool LINEAR = false, GROUPED = false, SUMS = false;      // SUMS: binary32 results whatever the operands
   template <bool PLAIN> using params = typename KernelParams<PLAIN>::type;
 };
 
@@ -2469,7 +2469,7 @@ __global__ __launch_bounds__(C::THREADS, PERSIST ? 1 : Residency<C>::WAVES) void
     // slots: 4096^3 164 -> 141 us, three: 125 -> 120, two: even; int8 with two: 165 -> 118, with three and four 1 and 5 % the other way).
     // Tiles with registers to spare lose by it (4032 x 1696 x 1536 bf16 on 128x256 22.5 -> 23.7), and so does the one of four waves and
     // two k steps, which spills outside its loop only (8192^3 698 -> 717).
-    constexpr bool NEW_LANE = PAIR || (C::KSTEPS == 1 && NW == 4 && BM == 256 && BN == 256 && (ES == 2 || STAGES == 2));
+    constexpr bool NEW_LANE = PAIR || (X::GROUPED && BM == 256 && BN == 256) || (C::KSTEPS == 1 && NW == 4 && BM == 256 && BN == 256 && (ES == 2 || STAGES == 2));
     const int elane = NEW_LANE ? __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)) : lane;
     if constexpr (CONV) {
       if (p.out_dtype == DT_F32) epilogue_store_conv<T, C, OutF32>(acc, p.c, strip, elane, (int)gm0, (int)gn0, p.cv);
@@ -2492,7 +2492,7 @@ __global__ __launch_bounds__(C::THREADS, PERSIST ? 1 : Residency<C>::WAVES) void
           epilogue_store<T, C, OT, true>(sums, p.c, strip, elane, gm0, gn0 >> 1, p.m, p.n >> 1, p.scm, p.scn, p.c_row_ok,
                                          p.epilogue);
       };
-      if constexpr (PAIR) {
+      if constexpr (PAIR || X::SUMS) {
         as(TypeTag<OutF32>{});
       } else if constexpr (!X::LINEAR && !X::GROUPED && (GATHER || f32_out_tile<T, C>())) {
         if (p.out_dtype == DT_F32) as(TypeTag<OutF32>{});

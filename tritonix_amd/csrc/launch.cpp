@@ -846,7 +846,7 @@ struct BlockEntries {
   size_t (*norm_workspace)(const tnx_norm_args*);
   int (*norm_backward)(const tnx_norm_args*);
   int (*grouped)(const tnx_grouped_args*);
-  int (*grouped_route)(const tnx_grouped_args*, int32_t*);
+  size_t (*grouped_workspace)(const tnx_grouped_args*);
 } blocks = {};
 PyObject* fn_counted = nullptr;          // (device index, stream, bytes) -> scratch whose counters are zero
 PyObject* fn_dropped = nullptr;          // (device index, stream): a launch on it reported an error
@@ -1165,18 +1165,27 @@ tnx_grouped_args grouped_args(int form, const at::Tensor& a, const at::Tensor& b
   g.stream = stream;
   return g;
 }
+// the product, with the scratch that it is faster with
+int grouped_launch(tnx_grouped_args* g, c10::DeviceIndex device) {
+  at::Tensor scratch;
+  if (const size_t bytes = blocks.grouped_workspace(g)) {
+    scratch = fresh({(int64_t)bytes}, at::kByte, device);
+    g->workspace = scratch.data_ptr(); g->workspace_bytes = bytes;
+  }
+  return blocks.grouped(g);
+}
 int rows_product(const at::Tensor& x, const at::Tensor& w, const at::Tensor& offsets, c10::DeviceIndex device, void* stream, at::Tensor* y) {
   tnx_grouped_args g = grouped_args(TNX_GROUPED_ROWS, x, w, offsets, w.size(2), x.size(1), w.stride(0), w.stride(1), w.stride(2), stream);
   *y = fresh({g.rows, g.n}, x.scalar_type(), device);
   g.c = y->data_ptr();
-  return blocks.grouped(&g);
+  return grouped_launch(&g, device);
 }
 int weight_gradient(const at::Tensor& x, const at::Tensor& dy, const at::Tensor& offsets, c10::DeviceIndex device, void* stream, at::Tensor* dw) {
   const int64_t k = x.size(1), n = dy.size(1);
   tnx_grouped_args g = grouped_args(TNX_GROUPED_WEIGHT_GRADIENT, x, dy, offsets, n, k, k * n, dy.size(0) == 1 ? n : dy.stride(0), 1, stream);
   *dw = fresh({(int64_t)g.groups, k, n}, x.scalar_type(), device);
   g.c = dw->data_ptr();
-  return blocks.grouped(&g);
+  return grouped_launch(&g, device);
 }
 
 struct GroupedProduct : torch::autograd::Function<GroupedProduct> {

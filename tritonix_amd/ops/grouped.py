@@ -71,7 +71,7 @@ def _rows_product(x, w, offsets) -> torch.Tensor:
     if n < 8 and not lib.tnx_grouped_route(ctypes.byref(args(None)), None):
         w = _padded(w, 2)
     y = torch.empty((rows, w.shape[2]), dtype=x.dtype, device=x.device)
-    launch("grouped_matmul", x.get_device(), lib.tnx_grouped, args(y))
+    _launch(args(y), x)
     return y if w.shape[2] == n else y[:, :n].contiguous()
 
 
@@ -89,8 +89,18 @@ def _weight_gradient(x, dy, offsets) -> torch.Tensor:
     if min(n, k) < 8 and not lib.tnx_grouped_route(ctypes.byref(args(None)), None):
         x, dy = _padded(x, 1), _padded(dy, 1)
     dw = torch.empty((groups, x.shape[1], dy.shape[1]), dtype=x.dtype, device=x.device)
-    launch("grouped_matmul", x.get_device(), lib.tnx_grouped, args(dw))
+    _launch(args(dw), x)
     return dw if dw.shape[1:] == (k, n) else dw[:, :k, :n].contiguous()
+
+
+def _launch(g, device_of) -> None:
+    """``tnx_grouped`` with the scratch that it is faster with."""
+    need = int(_C.load().tnx_grouped_workspace_bytes(ctypes.byref(g)))
+    scratch = torch.empty(need, dtype=torch.uint8, device=device_of.device) if need else None
+    if need:
+        g.workspace, g.workspace_bytes = scratch.data_ptr(), need
+    launch("grouped_matmul", device_of.get_device(), _C.load().tnx_grouped, g)
+    del scratch
 
 
 class _Grouped(torch.autograd.Function):

@@ -38,7 +38,7 @@ def find():
         lib = _C.load()
         native.bind_blocks(tuple(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
             lib.tnx_linear_workspace_bytes, lib.tnx_linear_scratch_bytes, lib.tnx_linear, lib.tnx_linear_gradient_bytes, lib.tnx_linear_gradient,
-            lib.tnx_layer_norm, lib.tnx_layer_norm_workspace_bytes, lib.tnx_layer_norm_backward, lib.tnx_grouped, lib.tnx_grouped_route))
+            lib.tnx_layer_norm, lib.tnx_layer_norm_workspace_bytes, lib.tnx_layer_norm_backward, lib.tnx_grouped, lib.tnx_grouped_workspace_bytes))
             + (counted_workspace, _dropped))
         module = native
     return module
