@@ -4,7 +4,8 @@
 //   dx = rstd (g - mean(g) - unit mean(g unit)),  dweight = sum over rows of dy unit,  dbias = sum over rows of dy
 //
 // Bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  A row is read once, into registers (16-byte runs,
-// one after another over the threads), the mean before the variance from the same registers: no difference of large squares.  In the backward pass a workgroup
+// one after another over the threads), the mean before the variance from the same registers: no difference of large squares.  16384 x 8192
+// bf16: 107 us (5.0 TB/s; a copy reaches 5.1), backward 182 (4.4 TB/s, and 8 us for the parameters' shares).  In the backward pass a workgroup
 // keeps its rows' share of dweight and dbias, in 32 bits per column, and a second launch adds the workgroups' shares up in order.
 #include <hip/hip_runtime.h>
 
@@ -27,17 +28,34 @@ struct NormParams {
 };
 
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+// the sum over 2, 4, 8, 16, 32 or 64 neighbouring lanes, in each of them, without LDS: exchanges within a row of 16 lanes (from 4 on mirrored,
+// which is the same once the smaller groups agree), then of rows and of halves
+template <int L> __device__ __forceinline__ float lanes_sum(float v) {
+  auto with = [&](int other) __attribute__((always_inline)) { v += __builtin_bit_cast(float, other); };
+  const auto bits = [&]() __attribute__((always_inline)) { return __builtin_bit_cast(int, v); };
+  if constexpr (L >= 2) with(__builtin_amdgcn_update_dpp(0, bits(), 0xB1, 0xF, 0xF, true));
+  if constexpr (L >= 4) with(__builtin_amdgcn_update_dpp(0, bits(), 0x4E, 0xF, 0xF, true));
+  if constexpr (L >= 8) with(__builtin_amdgcn_update_dpp(0, bits(), 0x141, 0xF, 0xF, true));
+  if constexpr (L >= 16) with(__builtin_amdgcn_update_dpp(0, bits(), 0x140, 0xF, 0xF, true));
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap((unsigned)bits(), (unsigned)bits(), false, false);
+    const unsigned one = r[0], other = r[1];             // (__builtin_bit_cast of a vector's element reads its first)
+    v = __builtin_bit_cast(float, one) + __builtin_bit_cast(float, other);
+  }
+  if constexpr (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap((unsigned)bits(), (unsigned)bits(), false, false);
+    const unsigned one = r[0], other = r[1];             // (__builtin_bit_cast of a vector's element reads its first)
+    v = __builtin_bit_cast(float, one) + __builtin_bit_cast(float, other);
+  }
   return v;
 }
 
 // Sums over the TPR threads of a row of NS values; every thread gets them.  TPR is a wave or the whole workgroup.  `slot` alternates from call
-// to call, so that one barrier does.
+// to call, so that one barrier does.  The waves' sums are read a lane each and added up over lanes: read by every thread in turn they took 64
+// registers of 16 waves' four sums (16384 x 8192 bf16 backward: 1142 us, now 182).
 template <int TPR, int NS> __device__ __forceinline__ void row_sums(float (&v)[NS], float* lds, int slot) {
 #pragma unroll
-  for (int s = 0; s < NS; ++s) v[s] = wave_sum(v[s]);
+  for (int s = 0; s < NS; ++s) v[s] = lanes_sum<64>(v[s]);
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
     float* at = lds + slot * W * NS;
@@ -47,12 +65,7 @@ template <int TPR, int NS> __device__ __forceinline__ void row_sums(float (&v)[N
     }
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      float t = 0.0f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) t += at[w * NS + s];
-      v[s] = t;
-    }
+    for (int s = 0; s < NS; ++s) v[s] = lanes_sum<W>(at[(threadIdx.x & (W - 1)) * NS + s]);
   }
 }
 
@@ -182,14 +195,15 @@ template <class O, int V> __device__ __forceinline__ void unpack(i32x4 v, float 
   for (int x = 0; x < V; ++x) f[x] = Run<O, V>::widen(e[x]);
 }
 
-// A workgroup walks over rows; x and dy of the row that is worked on and of the next are in registers as they lie in memory (widened
-// twice: for the sums, then for dx), which leaves room for two sums per column and for the loads to run ahead of the barrier.
-// Columns past the row's end are zeros in dy and weight and so add nothing.
-template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_backward_kernel(NormParams p) {
+// A workgroup walks over rows, R of them at a step (one barrier for their sums; two where a workgroup is alone on its CU or the
+// values are few: 16384 x 8192 bf16 214 us with one, 182 with two, float32 65536 x 1024 172 and 154; elsewhere two spill); x and dy of these and of the next R are in registers as they
+// lie in memory (widened twice: for the sums, then for dx), which leaves room for two sums per column and lets the loads run ahead of the
+// barrier.  Columns past the row's end are zeros in dy and weight and so add nothing.
+template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_bounds__(TPR < 128 ? 256 : TPR, 4) void norm_backward_kernel(NormParams p) {
   typedef typename O::raw raw;
-  constexpr int V = 16 / sizeof(raw), THREADS = TPR < 256 ? 256 : TPR, LINES = THREADS / TPR;
+  constexpr int V = 16 / sizeof(raw), THREADS = TPR < 128 ? 256 : TPR, LINES = THREADS / TPR, R = CH == 1 && (V == 4 || TPR == 1024) ? 2 : 1;
   constexpr bool AHEAD = CH <= 2;
-  __shared__ float lds[2 * 2 * THREADS / 64];
+  __shared__ float lds[2 * 2 * R * THREADS / 64];
   const int t = threadIdx.x % TPR, line = threadIdx.x / TPR;
   float dw[PARTS ? CH : 1][V], db[PARTS ? CH : 1][V];
   int cols[CH];
@@ -201,71 +215,91 @@ template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_
     for (int e = 0; e < V; ++e)
       if (PARTS) dw[c][e] = db[c][e] = 0.0f;
   }
-  i32x4 x[CH], g[CH];
-  float mean = 0.0f, rstd = 0.0f;
-  auto fetch = [&](int64_t row, i32x4 (&fx)[CH], i32x4 (&fg)[CH], float& fmean, float& frstd) __attribute__((always_inline)) {
+  i32x4 x[R][CH], g[R][CH];
+  float mean[R], rstd[R];
+  const int64_t step = (int64_t)gridDim.x * LINES;       // from one of a line's rows to its next
+  auto fetch = [&](int64_t first, i32x4 (&fx)[R][CH], i32x4 (&fg)[R][CH], float (&fmean)[R], float (&frstd)[R]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int64_t at = cols[c] ? (int64_t)(c * TPR + t) * V : 0;
-      fx[c] = load_packed<O, WHOLE>((const raw*)p.x + row * p.stride_x + at, cols[c]);
-      fg[c] = load_packed<O, WHOLE>((const raw*)p.dy + row * p.stride_dy + at, cols[c]);
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = first + r * step;
+      const bool there = row < p.rows;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int64_t at = cols[c] ? (int64_t)(c * TPR + t) * V : 0;
+        const int count = there ? cols[c] : 0;
+        fx[r][c] = load_packed<O, WHOLE>((const raw*)p.x + (there ? row : 0) * p.stride_x + at, count);
+        fg[r][c] = load_packed<O, WHOLE>((const raw*)p.dy + (there ? row : 0) * p.stride_dy + at, count);
+      }
+      fmean[r] = there ? p.mean[row] : 0.0f;
+      frstd[r] = there ? p.rstd[row] : 0.0f;
     }
-    fmean = p.mean[row];
-    frstd = p.rstd[row];
   };
-  const int64_t step = (int64_t)gridDim.x * LINES;
   int64_t row = (int64_t)blockIdx.x * LINES + line;
   const float share = 1.0f / (float)p.n;
   int slot = 0;
   if (AHEAD && row < p.rows) fetch(row, x, g, mean, rstd);
-  for (; row < p.rows; row += step) {                    // (a wave's own rows; with TPR = THREADS the workgroup's)
-    i32x4 nx[CH], ng[CH];
-    float nmean = 0.0f, nrstd = 0.0f;
+  for (; row < p.rows; row += R * step) {                // (a wave's own rows; with TPR = THREADS the workgroup's)
+    i32x4 nx[R][CH], ng[R][CH];
+    float nmean[R] = {}, nrstd[R] = {};
     if (!AHEAD) fetch(row, x, g, mean, rstd);
-    else if (row + step < p.rows) fetch(row + step, nx, ng, nmean, nrstd);
-    float s[2] = {0.0f, 0.0f};
+    else if (row + R * step < p.rows) fetch(row + R * step, nx, ng, nmean, nrstd);
+    float s[2 * R];
+#pragma unroll
+    for (int i = 0; i < 2 * R; ++i) s[i] = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      float u[V], d[V], w[V];
-      unpack<O, V>(x[c], u);
-      unpack<O, V>(g[c], d);
+      float w[V];
       load_param<O, V, WHOLE>(p.weight, p.weight_dtype, cols[c] ? (int64_t)(c * TPR + t) * V : 0, cols[c], 1.0f, w);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        u[e] = (u[e] - mean) * rstd;
-        if (PARTS) {
-          dw[c][e] += d[e] * u[e];
-          db[c][e] += d[e];
+      for (int r = 0; r < R; ++r) {
+        float u[V], d[V];
+        unpack<O, V>(x[r][c], u);
+        unpack<O, V>(g[r][c], d);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          u[e] = (u[e] - mean[r]) * rstd[r];
+          if (PARTS) {
+            dw[c][e] += d[e] * u[e];
+            db[c][e] += d[e];
+          }
+          d[e] *= w[e];
+          s[2 * r] += d[e];
+          s[2 * r + 1] += d[e] * u[e];
         }
-        d[e] *= w[e];
-        s[0] += d[e];
-        s[1] += d[e] * u[e];
       }
     }
     if (p.dx) {
-      row_sums<TPR, 2>(s, lds, slot);
+      row_sums<TPR, 2 * R>(s, lds, slot);
       slot ^= 1;
-      const float a = s[0] * share, b = s[1] * share;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        float u[V], d[V], w[V];
-        asm("" : "+v"(x[c]), "+v"(g[c]));               // (widened again, not kept wide since the sums)
-        unpack<O, V>(x[c], u);
-        unpack<O, V>(g[c], d);
+        float w[V];
         load_param<O, V, WHOLE>(p.weight, p.weight_dtype, cols[c] ? (int64_t)(c * TPR + t) * V : 0, cols[c], 1.0f, w);
 #pragma unroll
-        for (int e = 0; e < V; ++e) d[e] = rstd * (d[e] * w[e] - a - (u[e] - mean) * rstd * b);
-        if (cols[c]) store_run<O, V, WHOLE>((raw*)p.dx + row * p.n + (int64_t)(c * TPR + t) * V, cols[c], d);
+        for (int r = 0; r < R; ++r) {
+          float u[V], d[V];
+          asm("" : "+v"(x[r][c]), "+v"(g[r][c]));         // (widened again, not kept wide since the sums)
+          unpack<O, V>(x[r][c], u);
+          unpack<O, V>(g[r][c], d);
+          const float a = s[2 * r] * share, b = s[2 * r + 1] * share;
+#pragma unroll
+          for (int e = 0; e < V; ++e) d[e] = rstd[r] * (d[e] * w[e] - a - (u[e] - mean[r]) * rstd[r] * b);
+          if (cols[c] && (R == 1 || row + r * step < p.rows))
+            store_run<O, V, WHOLE>((raw*)p.dx + (row + r * step) * p.n + (int64_t)(c * TPR + t) * V, cols[c], d);
+        }
       }
     }
     if (AHEAD) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        x[c] = nx[c];
-        g[c] = ng[c];
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          x[r][c] = nx[r][c];
+          g[r][c] = ng[r][c];
+        }
+        mean[r] = nmean[r];
+        rstd[r] = nrstd[r];
       }
-      mean = nmean;
-      rstd = nrstd;
     }
   }
   if constexpr (PARTS) {
@@ -375,7 +409,7 @@ template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_l
   }
 }
 
-// dweight and dbias of such rows, and of those too long for a thread to keep its columns' sums too (CH = 4): a workgroup's 32 runs of columns down 256 rows, its 8 rows of threads meet in LDS
+// dweight and dbias of such rows, and of those too long for a thread to keep its columns' sums too (sums_apart): a workgroup's 32 runs of columns down 256 rows, its 8 rows of threads meet in LDS
 constexpr int LONG_ROWS = 256;
 template <class O> __global__ __launch_bounds__(256) void norm_columns_kernel(NormParams p) {
   typedef typename O::raw raw;
@@ -436,28 +470,37 @@ __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, in
   }
 }
 
-// threads and runs of a row; 0: longer than the registers hold
+// Threads and runs of a row; 0: longer than the registers hold.
 struct Shape {
   int tpr, ch;
 };
-Shape shape_of(int64_t n, int v) {
-  static const Shape shapes[] = {{64, 1}, {64, 2}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
-  for (const Shape& s : shapes)
-    if (n <= (int64_t)s.tpr * s.ch * v) return s;
+Shape shape_of(const Shape* shapes, int count, int64_t n, int v) {
+  for (int i = 0; i < count; ++i)
+    if (n <= (int64_t)shapes[i].tpr * shapes[i].ch * v) return shapes[i];
   return {0, 0};
 }
+const Shape FORWARD[] = {{64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}};
+const Shape BACKWARD[] = {{64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
+#define TNX_NORM_FORWARD_SHAPES(DO) DO(64, 1) DO(64, 2) DO(64, 4) DO(256, 2) DO(256, 4) DO(512, 4) DO(1024, 4)
+#define TNX_NORM_BACKWARD_SHAPES(DO) DO(64, 1) DO(128, 1) DO(256, 1) DO(512, 1) DO(1024, 1) DO(1024, 2) DO(1024, 4)
+Shape forward_shape(int64_t n, int v) { return shape_of(FORWARD, sizeof FORWARD / sizeof *FORWARD, n, v); }
+Shape backward_shape(int64_t n, int v) { return shape_of(BACKWARD, sizeof BACKWARD / sizeof *BACKWARD, n, v); }
+// rows that a workgroup has at a time
 int64_t lines_of(const Shape& s) { return s.tpr < 256 ? 256 / s.tpr : 1; }
+int64_t backward_lines(const Shape& s) { return s.tpr < 128 ? 256 / s.tpr : 1; }
+// more columns' sums than that a thread's registers do not hold: they are a launch of their own
+bool sums_apart(const Shape& s, int v) { return s.tpr == 0 || s.ch * v > 8; }
 // Workgroups of the backward pass.  Each costs a share of 8 n bytes, written and read, where a row of 16 bits costs 6 n: so 16 rows or
 // more to a line where that leaves every CU a workgroup, and not more than run together.
 int64_t groups_of(const tnx_norm_args* a, const Shape& s) {
-  const int64_t lines = lines_of(s), most = (a->rows + lines - 1) / lines, together = 256 * (1024 / (s.tpr < 256 ? 256 : s.tpr));
+  const int64_t lines = backward_lines(s), most = (a->rows + lines - 1) / lines, together = 256 * 16 / (s.tpr < 128 ? 4 : s.tpr / 64);
   int64_t groups = most / 16;
   groups = groups < 256 ? 256 : groups > together ? together : groups;
   return groups < most ? groups : most;
 }
 int64_t shares_of(const tnx_norm_args* a) {
-  const Shape s = shape_of(a->n, a->dtype == TNX_F32 ? 4 : 8);
-  return s.tpr == 0 || s.ch > 2 ? (a->rows + LONG_ROWS - 1) / LONG_ROWS : groups_of(a, s);
+  const Shape s = backward_shape(a->n, a->dtype == TNX_F32 ? 4 : 8);
+  return sums_apart(s, a->dtype == TNX_F32 ? 4 : 8) ? (a->rows + LONG_ROWS - 1) / LONG_ROWS : groups_of(a, s);
 }
 
 int check(const tnx_norm_args* a) {
@@ -485,10 +528,8 @@ int launched() {
   return TNX_OK;
 }
 
-#define TNX_NORM_SHAPES(DO) DO(64, 1) DO(64, 2) DO(256, 1) DO(512, 1) DO(1024, 1) DO(1024, 2) DO(1024, 4)
-
 template <class O> int forward(const NormParams& p, hipStream_t stream) {
-  const Shape s = shape_of(p.n, 16 / sizeof(typename O::raw));
+  const Shape s = forward_shape(p.n, 16 / sizeof(typename O::raw));
   const unsigned grid = (unsigned)((p.rows + lines_of(s) - 1) / lines_of(s));
   const bool whole = p.n % (16 / sizeof(typename O::raw)) == 0;
 #define TNX_NORM_FORWARD(TPR, CH)                                                                                       \
@@ -497,29 +538,30 @@ template <class O> int forward(const NormParams& p, hipStream_t stream) {
     else hipLaunchKernelGGL((norm_kernel<O, TPR, CH, false>), dim3(grid), dim3(TPR < 256 ? 256 : TPR), 0, stream, p);   \
     return launched();                                                                                                  \
   }
-  TNX_NORM_SHAPES(TNX_NORM_FORWARD)
+  TNX_NORM_FORWARD_SHAPES(TNX_NORM_FORWARD)
   hipLaunchKernelGGL((norm_long_kernel<O, false>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
   return launched();
 }
 
 template <class O> int backward(const tnx_norm_args* a, NormParams p, hipStream_t stream) {
-  const Shape s = shape_of(p.n, 16 / sizeof(typename O::raw));
+  const Shape s = backward_shape(p.n, 16 / sizeof(typename O::raw));
   const int64_t shares = shares_of(a);
   const bool wanted = a->dweight || a->dbias, whole = p.n % (16 / sizeof(typename O::raw)) == 0;
-  const bool apart = s.tpr == 0 || s.ch > 2;             // the parameters' sums by a launch of their own
+  constexpr int V = 16 / sizeof(typename O::raw);
+  const bool apart = sums_apart(s, V);
   const unsigned grid = (unsigned)(s.tpr ? groups_of(a, s) : 0);
   if (s.tpr == 0 && p.dx) hipLaunchKernelGGL((norm_long_kernel<O, true>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
 #define TNX_NORM_BACKWARD(TPR, CH)                                                                                      \
   if (s.tpr == TPR && s.ch == CH && (p.dx || !apart)) {                                                                 \
-    constexpr bool SUMS = CH <= 2;                                                                                      \
-    const dim3 threads(TPR < 256 ? 256 : TPR);                                                                          \
+    constexpr bool SUMS = CH * V <= 8;                                                                                  \
+    const dim3 threads(TPR < 128 ? 256 : TPR);                                                                          \
     if (SUMS && wanted && whole) hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, SUMS, true>), dim3(grid), threads, 0, stream, p);  \
     else if (SUMS && wanted) hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, SUMS, false>), dim3(grid), threads, 0, stream, p);     \
     else if (whole) hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, false, true>), dim3(grid), threads, 0, stream, p);       \
     else hipLaunchKernelGGL((norm_backward_kernel<O, TPR, CH, false, false>), dim3(grid), threads, 0, stream, p);       \
   }
-  TNX_NORM_SHAPES(TNX_NORM_BACKWARD)
-  constexpr int SPAN = 32 * (16 / sizeof(typename O::raw));
+  TNX_NORM_BACKWARD_SHAPES(TNX_NORM_BACKWARD)
+  constexpr int SPAN = 32 * V;
   if (apart && wanted)
     hipLaunchKernelGGL((norm_columns_kernel<O>), dim3((unsigned)((p.n + SPAN - 1) / SPAN), (unsigned)shares), dim3(256), 0, stream, p);
   if (wanted)
