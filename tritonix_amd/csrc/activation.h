@@ -13,12 +13,31 @@ constexpr float GELU_A = 0.044715f;
 // instructions
 __device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
+// erfc(|z| / sqrt 2), and e = exp(-z^2 / 2) on the way: t P(t) e with t = 1 / (1 + p |z| / sqrt 2), the rational approximation of Hastings
+// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26), off by at most 1.5e-7.  A call of erff, with its branches, took the gated and
+// activated epilogues 6 to 10 percent of a launch (4096 x 14336 x 4096 bf16, gelu: 1.19 times the plain product's time, 1.12 with this).
+__device__ __forceinline__ float erfc_abs(float z, float* e) {
+  const float x = __builtin_fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  p = __builtin_fmaf(p, t, 1.421413741f);
+  p = __builtin_fmaf(p, t, -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.254829592f);
+  *e = __expf(-x * x);
+  return p * t * *e;
+}
+
+// gelu: z (1 + erf(z / sqrt 2)) / 2 is z q / 2 below zero and z - z q / 2 above, with q = erfc(|z| / sqrt 2): no cancellation next to -1.
 // gelu_tanh: z (1 + tanh u) / 2 = z / (1 + e^-2u), which keeps its relative precision where tanh is next to -1
 __device__ __forceinline__ float activate(float z, int act) {
   switch (act) {
     case ACT_RELU: return z <= 0.0f ? 0.0f : z;          // (a NaN stays one)
     case ACT_SILU: return z * logistic(z);
-    case ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case ACT_GELU: {
+      float e;
+      const float half = 0.5f * z * erfc_abs(z, &e);
+      return z > 0.0f ? z - half : half;
+    }
     case ACT_GELU_TANH: return z * logistic(2.0f * GELU_C * (z + GELU_A * z * z * z));
     default: return z;
   }
@@ -33,7 +52,11 @@ __device__ __forceinline__ float activation_slope(float z, int act) {
       const float s = logistic(z);
       return s * (1.0f + z * (1.0f - s));
     }
-    case ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * (0.3989422804014327f * __expf(-0.5f * z * z));
+    case ACT_GELU: {
+      float e;
+      const float half = 0.5f * erfc_abs(z, &e);
+      return (z > 0.0f ? 1.0f - half : half) + 0.3989422804014327f * z * e;
+    }
     case ACT_GELU_TANH: {
       const float z2 = z * z, s = logistic(2.0f * GELU_C * z * (1.0f + GELU_A * z2));
       return s + 2.0f * z * s * (1.0f - s) * GELU_C * (1.0f + 3.0f * GELU_A * z2);

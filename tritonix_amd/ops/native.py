@@ -25,10 +25,6 @@ def counted_workspace(index: int, stream: int, nbytes: int) -> torch.Tensor:
     return _kernel._workspace(device, stream, nbytes)
 
 
-def _dropped(index: int, stream: int) -> None:
-    _kernel.drop_workspace(torch.device("cuda", index), stream)
-
-
 def find():
     global module
     native = launch_module()
@@ -38,7 +34,6 @@ def find():
         lib = _C.load()
         native.bind_blocks(tuple(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
             lib.tnx_linear_workspace_bytes, lib.tnx_linear_scratch_bytes, lib.tnx_linear, lib.tnx_linear_gradient_bytes, lib.tnx_linear_gradient,
-            lib.tnx_layer_norm, lib.tnx_layer_norm_workspace_bytes, lib.tnx_layer_norm_backward, lib.tnx_grouped, lib.tnx_grouped_workspace_bytes))
-            + (counted_workspace, _dropped))
+            lib.tnx_layer_norm, lib.tnx_layer_norm_workspace_bytes, lib.tnx_layer_norm_backward, lib.tnx_grouped, lib.tnx_grouped_workspace_bytes)))
         module = native
     return module
