@@ -73,7 +73,10 @@ def test_every_choice_of_tile_has_the_epilogue(dtype, layout):
     for m, n, k in itertools.product((1, 7, 16, 33, 64, 65, 100, 200, 300, 513, 1000, 1600, 2500, 4096, 8192), (16, 64, 96, 130, 500, 768, 1111, 2048, 3000, 4096, 14336),
                                      (8, 64, 72, 200, 512, 1000, 2048, 4096, 5000, 14336)):
         info = (ctypes.c_int32 * 5)()
-        assert lib.tnx_linear_route(ctypes.byref(linear_args(m, n, k, dtype, layout)), info) == _C.LINEAR_ROUTE_FUSED, (m, n, k, list(info))
+        route = lib.tnx_linear_route(ctypes.byref(linear_args(m, n, k, dtype, layout)), info)
+        if m <= 16 and layout == "nt" and dtype != _C.F32 and route == _C.LINEAR_ROUTE_STREAM:
+            continue
+        assert route == _C.LINEAR_ROUTE_FUSED, (m, n, k, list(info))
         tiles.add(tuple(info[:4]))
     assert len(tiles) >= (5 if dtype == _C.F32 else 12), tiles
 
@@ -86,6 +89,11 @@ def test_routes_of_a_linear_layer():
     a.stride_xm, a.stride_xk = 1, 100                         # contiguous along m
     assert route(a) == _C.LINEAR_ROUTE_APART and lib.tnx_linear_scratch_bytes(ctypes.byref(a)) >= 100 * 200 * 4
     assert route(linear_args(100, 200, 0)) == _C.LINEAR_ROUTE_APART
+    for m, n, k in ((1, 1, 1), (4, 100000, 64), (8, 200, 8192), (16, 4096, 4096)):
+        few = linear_args(m, n, k, layout="nt")
+        assert route(few) == _C.LINEAR_ROUTE_STREAM and lib.tnx_linear_workspace_bytes(ctypes.byref(few)) == 0
+    assert route(linear_args(17, 200, 304, layout="nt")) == route(linear_args(16, 512, 8192, layout="nt")) == _C.LINEAR_ROUTE_FUSED
+    assert route(linear_args(4, 200, 304, _C.F32, "nt")) == route(linear_args(4, 200, 304)) == _C.LINEAR_ROUTE_FUSED
     assert route(linear_args(0, 200, 300)) == 0
     bad = linear_args(100, 200, 300)
     bad.activation = 5

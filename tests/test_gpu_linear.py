@@ -1,4 +1,5 @@
 """Linear layers against the definition in 64 bits: values and gradients, every activation, type and layout, sizes off every tile."""
+import ctypes
 import itertools
 
 import pytest
@@ -169,19 +170,55 @@ ROUTED = [(8, 512, 512), (24, 4096, 4096), (48, 512, 4096), (64, 8192, 512), (10
 @pytest.mark.parametrize("m,n,k", ROUTED)
 @pytest.mark.parametrize("layout", ["nn", "nt"])
 def test_tiles_of_the_built_in_choice(device, dtype, m, n, k, layout):
-    import ctypes
-
     x, w = ref.draw(device, m, k, dtype=dtype, seed=1), weight(device, k, n, dtype, layout, 2)
     bias, residual = ref.draw(device, n, dtype=dtype, seed=3), ref.draw(device, m, n, dtype=dtype, seed=4)
     info = (ctypes.c_int32 * 5)()
     route = _C.load().tnx_linear_route(ctypes.byref(args_of(x, w, bias, "silu")), info)
-    assert route == _C.LINEAR_ROUTE_FUSED, (route, list(info))
+    few = m <= 16 and layout == "nt" and dtype != torch.float32
+    assert route == (_C.LINEAR_ROUTE_STREAM if few else _C.LINEAR_ROUTE_FUSED), (route, list(info))
     for _ in range(2):                     # (a second call finds the counters of a cut as the first left them)
         y = tritonix.linear(x, w, bias, "silu", residual)
     # a sample of rows: the definition of all of them would take the CPU minutes
     rows = torch.unique(torch.cat([torch.arange(0, m, max(1, m // 37)), torch.tensor([m - 1])]))
     at = rows.to(device)
     ref.check(f"tile {list(info)}", y[at], ref.linear(x[at], w, bias, "silu", residual[at])["y"], dtype)
+
+
+def strided(device, rows, cols, dtype, seed, pitch, offset, scale=1.0):
+    """Rows of cols elements, pitch apart, the first offset elements into its storage; NaN between and around them."""
+    whole = torch.full((offset + rows * pitch + 8,), float("nan"), dtype=dtype, device=device)
+    out = whole[offset:offset + rows * pitch].view(rows, pitch)[:, :cols]
+    out.copy_(ref.draw(device, rows, cols, dtype=dtype, seed=seed, scale=scale))
+    return out
+
+
+FEW = [(1, 1, 1), (1, 5, 7), (3, 9, 63), (4, 100, 257), (4, 4095, 520), (1, 4097, 136), (4, 4100, 1100), (5, 4104, 640), (8, 4099, 1026), (8, 33, 8192), (5, 17, 31), (8, 300, 2050),
+       (9, 50, 64), (16, 129, 1025), (13, 4500, 513), (16, 16, 4608), (1, 70, 9000)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+@pytest.mark.parametrize("m,n,k", FEW)
+@pytest.mark.parametrize("pad,offset", [(0, 0), (64, 64), (1, 3), (8, 8)])
+def test_few_rows_by_a_k_contiguous_weight(device, dtype, m, n, k, pad, offset):
+    """Blocks and steps that end inside the matrix, rows of the weight on lines of memory and off them; what lies between rows is never used."""
+    pitch = (k + 63) // 64 * 64 if pad == 64 else k + pad
+    x = strided(device, m, k, dtype, 1, k + pad, offset)
+    w = strided(device, n, k, dtype, 2, pitch, offset, k ** -0.5).t()
+    bias, residual = ref.draw(device, n, dtype=dtype, seed=3), ref.draw(device, m, n, dtype=dtype, seed=4)
+    args = args_of(x, w, bias, "gelu")
+    assert _C.load().tnx_linear_route(ctypes.byref(args), None) == _C.LINEAR_ROUTE_STREAM
+    ref.check("y", tritonix.linear(x, w, bias, "gelu", residual), ref.linear(x, w, bias, "gelu", residual)["y"], dtype)
+    plain = tritonix.linear(x, w)
+    ref.check("product", plain, ref.linear(x, w)["y"], dtype)
+    # a row's numbers are its own: one that is not a number stays in its row, and in its column of the weight
+    x[m // 2, k - 1] = float("inf")
+    y = tritonix.linear(x, w)
+    others = torch.arange(m, device=device) != m // 2
+    assert torch.equal(y[others], plain[others]) and not y[m // 2].isfinite().any()
+    x[m // 2, k - 1] = 1.0
+    w[0, n - 1] = float("nan")
+    y = tritonix.linear(x, w)
+    assert torch.equal(y[others, :n - 1], plain[others, :n - 1]) and y[:, n - 1].isnan().all()
 
 
 def test_same_bits_every_time_and_from_a_graph(device):
