@@ -512,7 +512,8 @@ enum tnx_linear_route {
   TNX_LINEAR_ROUTE_PRODUCT = 1,   /* no epilogue */
   TNX_LINEAR_ROUTE_FUSED = 2,     /* the epilogue in the product's kernel */
   TNX_LINEAR_ROUTE_APART = 3,     /* a launch of its own on sums in 32 bits */
-  TNX_LINEAR_ROUTE_STREAM = 4     /* few rows by a k-contiguous weight, with or without an epilogue; info is all zero */
+  TNX_LINEAR_ROUTE_STREAM = 4,    /* few rows by a k-contiguous weight, with or without an epilogue; info is all zero */
+  TNX_LINEAR_ROUTE_STREAM_ROWS = 5 /* the same by a row-major weight */
 };
 int tnx_linear_route(const tnx_linear_args* args, int32_t info[5]);
 

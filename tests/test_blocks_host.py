@@ -74,7 +74,7 @@ def test_every_choice_of_tile_has_the_epilogue(dtype, layout):
                                      (8, 64, 72, 200, 512, 1000, 2048, 4096, 5000, 14336)):
         info = (ctypes.c_int32 * 5)()
         route = lib.tnx_linear_route(ctypes.byref(linear_args(m, n, k, dtype, layout)), info)
-        if m <= 16 and layout == "nt" and dtype != _C.F32 and route == _C.LINEAR_ROUTE_STREAM:
+        if dtype != _C.F32 and route == (_C.LINEAR_ROUTE_STREAM if layout == "nt" else _C.LINEAR_ROUTE_STREAM_ROWS) and m <= (16 if layout == "nt" else 8):
             continue
         assert route == _C.LINEAR_ROUTE_FUSED, (m, n, k, list(info))
         tiles.add(tuple(info[:4]))
@@ -93,7 +93,20 @@ def test_routes_of_a_linear_layer():
         few = linear_args(m, n, k, layout="nt")
         assert route(few) == _C.LINEAR_ROUTE_STREAM and lib.tnx_linear_workspace_bytes(ctypes.byref(few)) == 0
     assert route(linear_args(17, 200, 304, layout="nt")) == route(linear_args(16, 512, 8192, layout="nt")) == _C.LINEAR_ROUTE_FUSED
-    assert route(linear_args(4, 200, 304, _C.F32, "nt")) == route(linear_args(4, 200, 304)) == _C.LINEAR_ROUTE_FUSED
+    assert route(linear_args(4, 200, 304, _C.F32, "nt")) == route(linear_args(4, 200, 304, _C.F32)) == _C.LINEAR_ROUTE_FUSED
+    for m, n, k in ((1, 8, 1), (4, 200, 304), (4, 4096, 4096), (8, 16000, 2048)):
+        few = linear_args(m, n, k)
+        assert route(few) == _C.LINEAR_ROUTE_STREAM_ROWS
+        need = lib.tnx_linear_workspace_bytes(ctypes.byref(few))
+        assert (need >= _C.WS_COUNTER_BYTES + 4 * m * n) == (k >= 1024 and n < 16000), (m, n, k, need)
+        if need:                                              # refused before any launch: without its workspace, with one too short, with one off 16 bytes
+            few.y = 1 << 22
+            assert lib.tnx_linear(ctypes.byref(few)) == _C.E_WORKSPACE
+            few.workspace, few.workspace_bytes = 1 << 23, need - 1
+            assert lib.tnx_linear(ctypes.byref(few)) == _C.E_WORKSPACE
+            few.workspace, few.workspace_bytes = (1 << 23) + 8, need
+            assert lib.tnx_linear(ctypes.byref(few)) == _C.E_WORKSPACE
+    assert route(linear_args(9, 200, 4096)) == route(linear_args(8, 200, 304)) == route(linear_args(1, 16384, 64)) == route(linear_args(1, 7, 64)) == _C.LINEAR_ROUTE_FUSED
     assert route(linear_args(0, 200, 300)) == 0
     bad = linear_args(100, 200, 300)
     bad.activation = 5

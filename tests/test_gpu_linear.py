@@ -174,8 +174,8 @@ def test_tiles_of_the_built_in_choice(device, dtype, m, n, k, layout):
     bias, residual = ref.draw(device, n, dtype=dtype, seed=3), ref.draw(device, m, n, dtype=dtype, seed=4)
     info = (ctypes.c_int32 * 5)()
     route = _C.load().tnx_linear_route(ctypes.byref(args_of(x, w, bias, "silu")), info)
-    few = m <= 16 and layout == "nt" and dtype != torch.float32
-    assert route == (_C.LINEAR_ROUTE_STREAM if few else _C.LINEAR_ROUTE_FUSED), (route, list(info))
+    if m > 16:
+        assert route == _C.LINEAR_ROUTE_FUSED, (route, list(info))
     for _ in range(2):                     # (a second call finds the counters of a cut as the first left them)
         y = tritonix.linear(x, w, bias, "silu", residual)
     # a sample of rows: the definition of all of them would take the CPU minutes
@@ -192,21 +192,27 @@ def strided(device, rows, cols, dtype, seed, pitch, offset, scale=1.0):
     return out
 
 
-FEW = [(1, 1, 1), (1, 5, 7), (3, 9, 63), (4, 100, 257), (4, 4095, 520), (1, 4097, 136), (4, 4100, 1100), (5, 4104, 640), (8, 4099, 1026), (8, 33, 8192), (5, 17, 31), (8, 300, 2050),
+FEW = [(1, 1, 1), (1, 8, 1), (2, 64, 64), (1, 72, 4100), (8, 520, 2500), (6, 1001, 5000), (3, 9000, 1025), (1, 5, 7), (3, 9, 63), (4, 100, 257), (4, 4095, 520), (1, 4097, 136), (4, 4100, 1100), (5, 4104, 640), (8, 4099, 1026), (8, 33, 8192), (5, 17, 31), (8, 300, 2050),
        (9, 50, 64), (16, 129, 1025), (13, 4500, 513), (16, 16, 4608), (1, 70, 9000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES[:2])
 @pytest.mark.parametrize("m,n,k", FEW)
 @pytest.mark.parametrize("pad,offset", [(0, 0), (64, 64), (1, 3), (8, 8)])
-def test_few_rows_by_a_k_contiguous_weight(device, dtype, m, n, k, pad, offset):
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+def test_few_rows(device, dtype, m, n, k, pad, offset, layout):
     """Blocks and steps that end inside the matrix, rows of the weight on lines of memory and off them; what lies between rows is never used."""
-    pitch = (k + 63) // 64 * 64 if pad == 64 else k + pad
     x = strided(device, m, k, dtype, 1, k + pad, offset)
-    w = strided(device, n, k, dtype, 2, pitch, offset, k ** -0.5).t()
+    rows, cols = (n, k) if layout == "nt" else (k, n)
+    w = strided(device, rows, cols, dtype, 2, (cols + 63) // 64 * 64 if pad == 64 else cols + pad, offset, k ** -0.5)
+    w = w.t() if layout == "nt" else w
     bias, residual = ref.draw(device, n, dtype=dtype, seed=3), ref.draw(device, m, n, dtype=dtype, seed=4)
     args = args_of(x, w, bias, "gelu")
-    assert _C.load().tnx_linear_route(ctypes.byref(args), None) == _C.LINEAR_ROUTE_STREAM
+    route = _C.load().tnx_linear_route(ctypes.byref(args), None)
+    if layout == "nt":
+        assert route == _C.LINEAR_ROUTE_STREAM
+    elif m <= 4 and n >= 8:
+        assert route == _C.LINEAR_ROUTE_STREAM_ROWS
     ref.check("y", tritonix.linear(x, w, bias, "gelu", residual), ref.linear(x, w, bias, "gelu", residual)["y"], dtype)
     plain = tritonix.linear(x, w)
     ref.check("product", plain, ref.linear(x, w)["y"], dtype)
@@ -221,9 +227,10 @@ def test_few_rows_by_a_k_contiguous_weight(device, dtype, m, n, k, pad, offset):
     assert torch.equal(y[others, :n - 1], plain[others, :n - 1]) and y[:, n - 1].isnan().all()
 
 
-def test_same_bits_every_time_and_from_a_graph(device):
+@pytest.mark.parametrize("m", [40, 3])
+def test_same_bits_every_time_and_from_a_graph(device, m):
     """Values and gradients from a captured graph, replayed with the program's own work between, are the eager ones bit for bit."""
-    m, n, k = 40, 1000, 2304                                # K is cut: counters in the graph's own workspace
+    n, k = 1000, 2304                                # K is cut: counters in the graph's own workspace
     x, w, b, r, dy = (ref.draw(device, *s, seed=i, scale=0.1) for i, s in enumerate(((m, k), (k, n), (n,), (m, n), (m, n))))
     leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
 

@@ -48,7 +48,7 @@ MOE_MAX_EXPERTS, MOE_MAX_TOP_K, MOE_MAX_GROUPS = 1024, 32, 64
 # enum tnx_activation
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3, 4
 # enum tnx_linear_route
-LINEAR_ROUTE_PRODUCT, LINEAR_ROUTE_FUSED, LINEAR_ROUTE_APART, LINEAR_ROUTE_STREAM = 1, 2, 3, 4
+LINEAR_ROUTE_PRODUCT, LINEAR_ROUTE_FUSED, LINEAR_ROUTE_APART, LINEAR_ROUTE_STREAM, LINEAR_ROUTE_STREAM_ROWS = 1, 2, 3, 4, 5
 # enum tnx_grouped_form
 GROUPED_ROWS, GROUPED_WEIGHT_GRADIENT = 0, 1
 GROUPED_MAX_GROUPS = 4096

@@ -148,4 +148,154 @@ template <class T> hipError_t stream_columns(const StreamParams& p, hipStream_t 
   return stream_lines<T, 16, 1, 4>(p, stream);
 }
 
+// The same for a row-major weight, up to 8 rows.  A workgroup owns 64 columns (a line of memory of each row of the weight), a step is 64 of k: a lane
+// reads 8 columns of 8 rows of the weight and picks the 8 numbers of a column together with v_perm_b32, half an instruction a number.  Column e of
+// every lane makes one matrix instruction: 8 columns in two groups, as C = 8 above.  64 columns are few workgroups (narrower ones would leave parts of
+// lines), so that `parts` of them share a block's k: each writes its sums through its L2, and the one that arrives last adds them up in the order of the parts.
+// That costs 3 to 4 us, less than a CU's slow pace.  bf16, cold weights, us, against the tile kernels': 1 x 4096 x 4096 11.6 and 13.2, 1 x 8192 x 8192 27.2 (4.9 TB/s)
+// and 31.4, 1 x 512 x 8192 8.3 and 11.0, 8 x 4096 x 4096 12.8 and 13.7, 8 x 1024 x 1024 8.5 and 8.2; a k-contiguous weight's kernel 7.6, -, 4.9, 9.2 and 3.6.
+struct StreamRowsParams {
+  const uint8_t* x;
+  const uint8_t* w;
+  uint8_t* y;
+  uint8_t* z;
+  const uint8_t* bias;
+  const uint8_t* residual;
+  uint8_t* workspace;        // counters, all zero, then the parts' sums; null without parts
+  int64_t ldx, ldw;
+  int32_t m, n, k, parts;
+  int32_t flags;             // activation | bias_dtype << 8
+};
+static_assert(sizeof(StreamRowsParams) <= 112, "a longer argument list costs every launch 0.7 us");
+
+template <class T, int W, int U> __global__ __launch_bounds__(W * 64) void gemm_stream_rows_kernel(StreamRowsParams p) {
+  static_assert(T::ES == 2, "16-bit element types only");
+  typedef Mma<T, 16> MMA;
+  typedef typename OutOf<T>::type O;
+  typedef typename O::raw raw;
+  __shared__ f32x4 sums[W][8][32];
+  __shared__ int arrived;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int li = lane & 15, octet = (li >> 3) * 4 + (lane >> 4), c = li & 7;
+  const int tiles = (p.n + 63) / 64, id = xcd_remap(blockIdx.x, tiles * p.parts, 8), tile = id / p.parts, part = id - tile * p.parts, n0 = tile * 64;
+  // (the last run of 8 columns begins where it ends with the row)
+  const int col = n0 + c * 8 < p.n - 8 ? n0 + c * 8 : p.n - 8;
+  const raw* const xp = (const raw*)p.x + (int64_t)(c < p.m ? c : p.m - 1) * p.ldx + octet * 8;
+  const raw* const wp = (const raw*)p.w + (int64_t)(octet * 8) * p.ldw + col;
+  f32x4 acc[8] = {};
+  auto multiply = [&](const i32x4 (&b)[8], i32x4 a) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      i32x4 v;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[d] = (int)__builtin_amdgcn_perm((uint32_t)b[2 * d + 1][e / 2], (uint32_t)b[2 * d][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+      acc[e] = MMA::run(v, a, acc[e]);
+    }
+  };
+  const int whole = p.k / 64, turn = W * p.parts;
+  auto steps = [&](int s, auto count) __attribute__((always_inline)) {
+    constexpr int N = decltype(count)::value;
+    i32x4 b[N][8], a[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const raw* const from = wp + (int64_t)(s + u * turn) * 64 * p.ldw;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[u][j] = (i32x4)__builtin_nontemporal_load((const i32x4_loose*)(from + j * p.ldw));
+      a[u] = *(const i32x4_loose*)(xp + (int64_t)(s + u * turn) * 64);
+    }
+#pragma unroll
+    for (int u = 0; u < N; ++u) multiply(b[u], a[u]);
+  };
+  int s = part * W + wave;
+  for (; s + (U - 1) * turn < whole; s += U * turn) steps(s, std::integral_constant<int, U>());
+  for (; s < whole; s += turn) steps(s, std::integral_constant<int, 1>());
+  if (s == whole && whole * 64 < p.k) {
+    const int left = p.k - whole * 64 - octet * 8;
+    i32x4 b[8], a = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      b[j] = i32x4{0, 0, 0, 0};
+      if (j < left) b[j] = *(const i32x4_loose*)(wp + ((int64_t)whole * 64 + j) * p.ldw);
+    }
+    const raw* const from = xp + (int64_t)whole * 64;
+    if (left >= 8) a = *(const i32x4_loose*)from;
+    else {
+      raw e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = i < left ? from[i] : (raw)0;
+      __builtin_memcpy(&a, e, 16);
+    }
+    multiply(b, a);
+  }
+  // rows 0 to 7 of the sums are the first group's columns, whose x is in columns 0 to 7, the others the second's
+  if ((lane >> 5) == (li >> 3)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[wave][e][(lane >> 4) * 8 + c] = acc[e];
+  }
+  __syncthreads();
+  auto sum_of = [&](int o) __attribute__((always_inline)) {
+    const int m = o >> 6, cc = (o >> 3) & 7, e = o & 7;
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) v += ((const float*)&sums[w][e][(g * 2 + (cc >> 2)) * 8 + m])[cc & 3];
+    return v;
+  };
+  float* const slab = p.workspace ? (float*)(p.workspace + WS_COUNTER_BYTES) + (int64_t)tile * p.parts * p.m * 64 : nullptr;
+  if (p.parts > 1) {
+    for (int o = threadIdx.x; o < p.m * 64; o += W * 64)
+      __hip_atomic_store(slab + (int64_t)part * p.m * 64 + o, sum_of(o), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int* const counter = (int*)p.workspace + tile;
+      const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      // the last arrival re-arms the counter for the next launch
+      if (before == p.parts - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      arrived = before;
+    }
+    __syncthreads();
+    if (arrived != p.parts - 1) return;
+  }
+  const int act = p.flags & 255, bias_dtype = p.flags >> 8;
+  for (int o = threadIdx.x; o < p.m * 64; o += W * 64) {
+    const int m = o >> 6, own = n0 + (o & 56), n = (own < p.n - 8 ? own : p.n - 8) + (o & 7);
+    if (n < own || own >= p.n) continue;                   // (another lane's run has it)
+    float v = 0.0f;
+    if (p.parts > 1) {
+#pragma unroll 8
+      for (int q = 0; q < p.parts; ++q) v += __hip_atomic_load(slab + (int64_t)q * p.m * 64 + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+      v = sum_of(o);
+    }
+    const int64_t at = (int64_t)m * p.n + n;
+    if (p.bias) v += bias_value(p.bias, n, bias_dtype);
+    if (p.z) ((raw*)p.z)[at] = O::cvt(v);
+    v = activate(v, act);
+    if (p.residual) v += Run<O, 8>::widen(((const raw*)p.residual)[at]);
+    ((raw*)p.y)[at] = O::cvt(v);
+  }
+}
+
+// Workgroups to a block of 64 columns: one for each CU, twice as many where a wave then has no more than two steps (1 x 4096 x 4096, us: 4 parts 12.2, 8
+// parts 11.6; 1 x 8192 x 8192 2 parts 27.2, 4 parts 30.0), and a step at least for each wave.
+constexpr int STREAM_ROWS_WAVES = 8;
+inline int stream_rows_parts(int64_t n, int64_t k) {
+  const int64_t tiles = (n + 63) / 64, most = k / (64 * STREAM_ROWS_WAVES);
+  int64_t parts = tiles < 256 ? 256 / tiles : 1;
+  if (k <= parts * STREAM_ROWS_WAVES * 128) parts *= 2;
+  if (parts > most) parts = most;
+  return parts < 1 ? 1 : (int)parts;
+}
+inline size_t stream_rows_workspace(int64_t m, int64_t n, int64_t k) {
+  const int parts = stream_rows_parts(n, k);
+  return parts > 1 ? WS_COUNTER_BYTES + (size_t)((n + 63) / 64) * parts * m * 64 * 4 : 0;
+}
+
+template <class T> hipError_t stream_rows(const StreamRowsParams& p, hipStream_t stream) {
+  StreamRowsParams q = p;
+  return launch_kernel((const void*)&gemm_stream_rows_kernel<T, STREAM_ROWS_WAVES, 2>, (unsigned)((p.n + 63) / 64 * p.parts), STREAM_ROWS_WAVES * 64, 0, stream, &q);
+}
+
 }  // namespace tnx
