@@ -53,6 +53,20 @@ def test_normalisation_past_32_bits(device):
     assert (dbias[-1].double() - column.sum()).abs() <= bound
 
 
+def test_more_rows_than_a_launch_has_threads_for(device):
+    """70 million short rows, a wave's worth of threads to each."""
+    rows, n = 70000000, 8
+    x, weight, dy = random(device, rows, n), random(device, n, seed=1), random(device, rows, n, seed=2)
+    leaves = [t.requires_grad_(True) for t in (x, weight)]
+    y = tritonix.layer_norm(x, weight)
+    dx, _ = torch.autograd.grad(y, leaves, dy)
+    for first in (0, (1 << 24) - 20, (1 << 26) - 70, rows - 50):        # (around the ends of launches, and the last)
+        part = slice(first, first + 50)
+        want = ref.layer_norm(x[part], weight, None, 1e-5, dy[part])
+        ref.check("y", y[part], want["y"], BF16)
+        ref.check("dx", dx[part], want["dx"], BF16)
+
+
 def test_a_grouped_product_past_32_bits(device):
     """Rows past 32 bits, and of the weights and their gradient."""
     k = 64

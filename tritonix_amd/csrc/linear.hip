@@ -146,7 +146,7 @@ bool with_epilogue(const tnx_linear_args* a) { return a->bias || a->residual || 
 // 8 x 4096 x 14336 26.3 and 25.1), 9 to 16 where n and k are small (16 x 2050 x 4100 8.1 and 13.6, 16 x 4096 x 4096 10.9 and 12.5; 16 x 512 x 8192
 // 16.4 and 10.6, 16 x 30000 x 512 10.8 and 9.2).
 bool takes_stream(const tnx_linear_args* a) {
-  if (a->dtype == TNX_F32 || a->stride_xk != 1 || a->stride_wk != 1 || a->m > 16 || a->n > 0x40000000 || a->k > 0x40000000) return false;
+  if (a->dtype == TNX_F32 || a->stride_xk != 1 || a->stride_wk != 1 || a->m > 16 || a->n > 0x1000000 || a->k > 0x40000000) return false;
   return a->m <= 4 || (a->m <= 8 && a->k <= 8192) || (a->n <= 4608 && a->k <= 4608);
 }
 

@@ -528,7 +528,8 @@ int launched() {
   return TNX_OK;
 }
 
-template <class O> int forward(const NormParams& p, hipStream_t stream) {
+// One launch's rows: the threads of a grid are counted in 32 bits.
+template <class O> int forward_rows(const NormParams& p, hipStream_t stream) {
   const Shape s = forward_shape(p.n, 16 / sizeof(typename O::raw));
   const unsigned grid = (unsigned)((p.rows + lines_of(s) - 1) / lines_of(s));
   const bool whole = p.n % (16 / sizeof(typename O::raw)) == 0;
@@ -541,6 +542,22 @@ template <class O> int forward(const NormParams& p, hipStream_t stream) {
   TNX_NORM_FORWARD_SHAPES(TNX_NORM_FORWARD)
   hipLaunchKernelGGL((norm_long_kernel<O, false>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
   return launched();
+}
+
+template <class O> int forward(NormParams p, hipStream_t stream) {
+  constexpr int64_t MOST = (1 << 22) - 4, ES = sizeof(typename O::raw);       // of 1024 threads, if a row takes that many
+  const int64_t at_once = p.n <= 64 * 4 * (16 / ES) ? MOST * 4 : MOST;
+  for (int64_t left = p.rows; left > 0; left -= at_once) {
+    p.rows = left < at_once ? left : at_once;
+    if (const int status = forward_rows<O>(p, stream)) return status;
+    p.x += p.rows * p.stride_x * ES;
+    p.y += p.rows * p.n * ES;
+    if (p.mean) {
+      p.mean += p.rows;
+      p.rstd += p.rows;
+    }
+  }
+  return TNX_OK;
 }
 
 template <class O> int backward(const tnx_norm_args* a, NormParams p, hipStream_t stream) {
