@@ -587,8 +587,9 @@ typedef struct tnx_grouped_args {
 /* scratch that a product is faster with (few tiles of a long k), or 0.  Host arithmetic on the sizes */
 size_t tnx_grouped_workspace_bytes(const tnx_grouped_args* args);
 int tnx_grouped(const tnx_grouped_args* args);
-/* For tests and tooling: 1, or 0 where tnx_grouped would refuse these args (of the pointers only the alignment counts).  info (may be NULL): rows and
- * columns of a tile, waves, whether each group's last slab of k is loaded apart, parts of k (given a workspace). */
+/* For tests and tooling: 1, 2 where few rows by k-contiguous weights are streamed, or 0 where tnx_grouped would refuse these args (of the pointers only the
+ * alignment counts).  info (may be NULL): rows and columns of a tile, waves, whether each group's last slab of k is loaded apart, parts of k (given a
+ * workspace); all zero for 2. */
 int tnx_grouped_route(const tnx_grouped_args* args, int32_t info[5]);
 
 #ifdef __cplusplus

@@ -154,6 +154,13 @@ def test_grouped_entry_point_refuses():
         assert lib.tnx_grouped(ctypes.byref(grouped_args(**more))) == status, more
     info = (ctypes.c_int32 * 5)()
     assert lib.tnx_grouped_route(ctypes.byref(grouped_args()), info) == 1 and info[3] == 0
+    few = dict(rows=12, stride_bk=1, stride_bn=64)
+    assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**few)), info) == 2 and list(info) == [0] * 5
+    assert lib.tnx_grouped_workspace_bytes(ctypes.byref(grouped_args(**{**few, "k": 4096, "stride_ar": 4096, "stride_bn": 4096}))) == 0
+    for more in (dict(rows=13), dict(dtype=_C.F32), dict(block_m=64, block_n=64), dict(form=_C.GROUPED_WEIGHT_GRADIENT, stride_bk=64, stride_bn=1)):
+        assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**{**few, **more})), info) == 1, more
+    for more in (dict(stride_ar=63), dict(stride_bn=63), dict(stride_ak=2)):
+        assert lib.tnx_grouped(ctypes.byref(grouped_args(**{**few, **more}))) == _C.E_UNSUPPORTED, more
     for more in (dict(k=63, stride_ar=63), dict(n=63, stride_bk=63), dict(a=4098), dict(b=4100), dict(stride_group=4097)):
         assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**more)), info) == 1 and info[3] == 1, more
 

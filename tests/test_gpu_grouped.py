@@ -130,6 +130,47 @@ def test_k_in_parts(device, dtype, tile, parts, monkeypatch):
             ref.check(f"dw {k}", module._weight_gradient(x, dy, offsets), want["dw"], dtype)
 
 
+# counts of the groups' rows, rows ahead and behind, k, n: a row each, runs longer than 8 rows, many groups, short and long k
+FEW = [([1], 0, 0, 1, 1), ([0, 3, 0], 0, 0, 7, 5), ([1, 0, 1], 1, 2, 65, 9), ([0, 8], 0, 0, 640, 200), ([2, 0, 9, 1, 0], 3, 2, 1024, 136), ([0, 0, 0, 17, 0, 0, 0], 1, 2, 300, 77),
+       ([1, 0] * 60, 0, 3, 520, 600), ([4] * 9, 0, 0, 1030, 70), ([0] * 130 + [25, 3], 9, 40, 72, 40), ([3, 5], 0, 0, 8200, 24), ([1, 2, 0, 8, 4, 5], 2, 1, 9000, 20),
+       ([1, 0] * 60, 0, 3, 2050, 600)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+@pytest.mark.parametrize("case", range(len(FEW)))
+@pytest.mark.parametrize("pad,offset", [(0, 0), (64, 64), (1, 3)])
+def test_few_rows_by_k_contiguous_weights(device, dtype, case, pad, offset):
+    """Few rows, streamed: groups of none to 25 rows, rows of the weights on lines of memory and off them, NaN between them that nothing may read."""
+    counts, ahead, behind, k, n = FEW[case]
+    rows, groups = ahead + sum(counts) + behind, len(counts)
+
+    def strided(m, columns, pitch, seed, scale=1.0):
+        whole = torch.full((offset + m * pitch + 8,), float("nan"), dtype=dtype, device=device)
+        out = whole[offset:offset + m * pitch].view(m, pitch)[:, :columns]
+        out.copy_(ref.draw(device, m, columns, dtype=dtype, seed=seed, scale=scale))
+        return out
+
+    pitch = (k + 63) // 64 * 64 if pad == 64 else k + pad
+    x, flat = strided(rows, k, k + pad, 1), strided(groups * n, k, pitch, 2, k ** -0.5)
+    w = flat.as_strided((groups, k, n), (n * pitch, 1, pitch), flat.storage_offset())
+    offsets = offsets_of(device, counts, ahead)
+    if n > 1 and k > 1:
+        g = module._args(_C.GROUPED_ROWS, x, w, None, offsets, n, k, *w.stride())
+        streamed = k >= 2048 or min(rows, groups) * n <= 16384
+        assert _C.load().tnx_grouped_route(ctypes.byref(g), None) == (2 if streamed else 1)
+    y = tritonix.grouped_matmul(x, w, offsets)
+    ref.check("y", y, ref.grouped(x, w, offsets)["y"], dtype)
+    assert not y[:ahead].any() and not y[rows - behind:].any()
+    again = tritonix.grouped_matmul(x, w, offsets)
+    assert torch.equal(y, again)
+    # a row's numbers are its own
+    bad = ahead + sum(counts) - 1
+    x[bad] = float("nan")
+    got = tritonix.grouped_matmul(x, w, offsets)
+    others = torch.arange(rows, device=device) != bad
+    assert torch.equal(got[others], y[others]) and got[bad].isnan().all()
+
+
 @pytest.mark.parametrize("bounds", [[-5, 10, 20, 30], [0, 30, 10, 40], [50, 40, 30, 20], [0, 2 ** 31 - 1, 5, 7], [7, 7, 7, 7], [-(2 ** 31), -1, 0, 0], [40, 40, 40, 99]])
 def test_bounds_outside_of_the_rows(device, bounds):
     """Whatever the bounds hold, they are taken into the rows and to a sequence that does not decrease."""

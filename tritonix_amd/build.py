@@ -405,7 +405,8 @@ def _compile(src, obj, verbose, force=True):
             os.path.join(CSRC, "conv_tile.h"), os.path.join(CSRC, "conv_pack.h"),
             *([os.path.join(CSRC, "mx.h")] if os.path.basename(src).startswith(("mx_", "moe")) else []),
             *([os.path.join(CSRC, "activation.h"), os.path.join(CSRC, "gemm_linear.h"), os.path.join(CSRC, "gemm_stream.h")] if os.path.basename(src).startswith(("linear", "norm", "capi")) else []),
-            *([os.path.join(CSRC, "gemm_grouped.h")] if os.path.basename(src).startswith("grouped") else []),
+            *([os.path.join(CSRC, "gemm_grouped.h")] if os.path.basename(src).startswith(("grouped", "linear.hip")) else []),
+            *([os.path.join(CSRC, h) for h in ("activation.h", "gemm_linear.h", "gemm_stream.h")] if os.path.basename(src) == "grouped.hip" else []),
             *([os.path.join(CSRC, "conv_halo.h")] if os.path.basename(src).startswith(("halo_", "conv.hip")) else []),
             os.path.join(ROOT, "include", "tritonix_hip.h"), os.path.abspath(__file__)]
     if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(d) for d in deps):

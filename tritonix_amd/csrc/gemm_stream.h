@@ -10,6 +10,7 @@
 // bf16, cold weights, us: 1 x 4096 x 4096 7.6 (4.4 TB/s; the tile kernels, which cut k and hand slices over, 12.4), 1 x 14336 x 4096 19 (6.2 TB/s; 25),
 // 1 x 1024 x 1024 2.5 (7.4), 8 x 4096 x 4096 9.2 (12.5), 16 x 1024 x 1024 3.9 (7.5).
 #pragma once
+#include "gemm_grouped.h"
 #include "gemm_linear.h"
 
 namespace tnx {
@@ -30,7 +31,7 @@ static_assert(sizeof(StreamParams) <= 112, "a longer argument list costs every l
 // C: columns of the weight and rows of x at most; W: waves; U: steps of 64 x 16 / C of k in flight; LINES: rows of the weight begin on lines of memory,
 // of which nothing is left for another instruction to read (with C = 8, us: 1 x 4096 x 4096 7.6 past the caches and 8.1 through them; rows that begin
 // anywhere, 1 x 2050 x 4100 7.5 and 6.4).
-template <class T, int C, int NT, int W, int U, bool LINES> __global__ __launch_bounds__(W * 64) void gemm_stream_kernel(StreamParams p) {
+template <class T, int C, int NT, int W, int U, bool LINES> __device__ __forceinline__ void stream_block(const StreamParams& p, int block) {
   static_assert(T::ES == 2, "16-bit element types only");
   typedef Mma<T, 16> MMA;
   typedef typename OutOf<T>::type O;
@@ -39,7 +40,7 @@ template <class T, int C, int NT, int W, int U, bool LINES> __global__ __launch_
   __shared__ f32x4 sums[W][NT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, kg = lane >> 4;
-  const int tiles = (p.n + C * NT - 1) / (C * NT), n0 = xcd_remap(blockIdx.x, tiles, 8) * (C * NT);
+  const int n0 = block * (C * NT);
   const int koff = li / C * 32 + kg * 8;
   const raw* const xp = (const raw*)p.x + (int64_t)(li % C < p.m ? li % C : p.m - 1) * p.ldx + koff;
   const raw* wp[NT];
@@ -122,6 +123,10 @@ template <class T, int C, int NT, int W, int U, bool LINES> __global__ __launch_
   }
 }
 
+template <class T, int C, int NT, int W, int U, bool LINES> __global__ __launch_bounds__(W * 64) void gemm_stream_kernel(StreamParams p) {
+  stream_block<T, C, NT, W, U, LINES>(p, xcd_remap(blockIdx.x, (p.n + C * NT - 1) / (C * NT), 8));
+}
+
 template <class T, int C, int NT, int W, int U, bool LINES> hipError_t stream_launch(const StreamParams& p, hipStream_t stream) {
   StreamParams q = p;
   return launch_kernel((const void*)&gemm_stream_kernel<T, C, NT, W, U, LINES>, (unsigned)((p.n + C * NT - 1) / (C * NT)), W * 64, 0, stream, &q);
@@ -168,7 +173,7 @@ struct StreamRowsParams {
 };
 static_assert(sizeof(StreamRowsParams) <= 112, "a longer argument list costs every launch 0.7 us");
 
-template <class T, int W, int U> __global__ __launch_bounds__(W * 64) void gemm_stream_rows_kernel(StreamRowsParams p) {
+template <class T, int W, int U> __device__ __forceinline__ void stream_rows_block(const StreamRowsParams& p, int id) {
   static_assert(T::ES == 2, "16-bit element types only");
   typedef Mma<T, 16> MMA;
   typedef typename OutOf<T>::type O;
@@ -177,7 +182,7 @@ template <class T, int W, int U> __global__ __launch_bounds__(W * 64) void gemm_
   __shared__ int arrived;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, octet = (li >> 3) * 4 + (lane >> 4), c = li & 7;
-  const int tiles = (p.n + 63) / 64, id = xcd_remap(blockIdx.x, tiles * p.parts, 8), tile = id / p.parts, part = id - tile * p.parts, n0 = tile * 64;
+  const int tile = id / p.parts, part = id - tile * p.parts, n0 = tile * 64;
   // (the last run of 8 columns begins where it ends with the row)
   const int col = n0 + c * 8 < p.n - 8 ? n0 + c * 8 : p.n - 8;
   const raw* const xp = (const raw*)p.x + (int64_t)(c < p.m ? c : p.m - 1) * p.ldx + octet * 8;
@@ -278,6 +283,10 @@ template <class T, int W, int U> __global__ __launch_bounds__(W * 64) void gemm_
   }
 }
 
+template <class T, int W, int U> __global__ __launch_bounds__(W * 64) void gemm_stream_rows_kernel(StreamRowsParams p) {
+  stream_rows_block<T, W, U>(p, xcd_remap(blockIdx.x, (p.n + 63) / 64 * p.parts, 8));
+}
+
 // Workgroups to a block of 64 columns: one for each CU, twice as many where a wave then has no more than two steps (1 x 4096 x 4096, us: 4 parts 12.2, 8
 // parts 11.6; 1 x 8192 x 8192 2 parts 27.2, 4 parts 30.0), and a step at least for each wave.
 constexpr int STREAM_ROWS_WAVES = 8;
@@ -296,6 +305,51 @@ inline size_t stream_rows_workspace(int64_t m, int64_t n, int64_t k) {
 template <class T> hipError_t stream_rows(const StreamRowsParams& p, hipStream_t stream) {
   StreamRowsParams q = p;
   return launch_kernel((const void*)&gemm_stream_rows_kernel<T, STREAM_ROWS_WAVES, 2>, (unsigned)((p.n + 63) / 64 * p.parts), STREAM_ROWS_WAVES * 64, 0, stream, &q);
+}
+
+// The k-contiguous one by groups of rows, a weight to each (gemm_grouped.h): 8 rows of a group at a time, for few rows in all or few to a group.  A workgroup
+// finds its rows in the bounds, which are all that it waits for.  bf16, cold weights, us, against the tile kernels': 2 rows, 64 groups, 4096 x 2048 8.5 and 15.1,
+// 4 rows, 128 groups, 2048 x 768 5.5 and 11.8, 16 rows, 64 groups, 4096 x 2048 38 and 40, 64 rows, 128 groups, 2048 x 768 27 and 37.  (A row-major weight's 64
+// columns are too few workgroups here as well: even with the tile kernels at best, 1 row, 64 groups, 4096 x 2048 19.0 and 15.6.)
+template <class T, int NT, int W, int U, bool LINES> __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedParams q) {
+  constexpr int ES = T::ES, COLUMNS = 8 * NT;
+  const int across = (int)(((uint32_t)q.n + COLUMNS - 1) / COLUMNS), id = windowed<64>(blockIdx.x, gridDim.x), want = id / across, block = id - want * across;
+  int total = 0;
+  const GroupedFamily<false>::Stretch s = GroupedFamily<false>::stretch_of<8>(q, threadIdx.x & 63, want, &total);
+  if (s.number < 0) return;
+  const int skip = (want - s.before) * 8, m = s.rows - skip < 8 ? s.rows - skip : 8;
+  const int64_t row = s.first + skip;
+  uint8_t* const y = q.c + row * q.n * ES;
+  if (s.number == 0 || s.number == q.groups + 1) {
+    typedef typename OutOf<T>::type::raw raw;
+    for (int o = threadIdx.x; o < m * COLUMNS; o += W * 64) {
+      const int n = block * COLUMNS + o % COLUMNS;
+      if (n < q.n) ((raw*)y)[(int64_t)(o / COLUMNS) * q.n + n] = 0;
+    }
+    return;
+  }
+  const uint8_t* const x = q.a + row * q.lda * ES;
+  const uint8_t* const w = q.b + (int64_t)(s.number - 1) * q.group_stride * ES;
+  stream_block<T, 8, NT, W, U, LINES>({x, w, y, nullptr, nullptr, nullptr, q.lda, q.ldb, m, q.n, q.k, ACT_NONE, 0}, block);
+}
+
+// the most runs of 8 rows that there can be
+inline int64_t stream_runs(int64_t rows, int64_t groups) { return rows / 8 + (groups + 2 < rows ? groups + 2 : rows); }
+template <class T, int NT, int W, int U> hipError_t grouped_stream_launch(const GroupedParams& p, hipStream_t stream) {
+  GroupedParams q = p;
+  const unsigned grid = (unsigned)(stream_runs(p.rows, p.groups) * ((p.n + 8 * NT - 1) / (8 * NT)));
+  const bool lines = p.ldb % 64 == 0 && p.group_stride % 64 == 0 && ((uintptr_t)p.b & 127) == 0;
+  if (lines) return launch_kernel((const void*)&grouped_stream_kernel<T, NT, W, U, true>, grid, W * 64, 0, stream, &q);
+  return launch_kernel((const void*)&grouped_stream_kernel<T, NT, W, U, false>, grid, W * 64, 0, stream, &q);
+}
+// Columns and waves of a workgroup: blocks of 8 columns in pairs where workgroups are many and k is short, or where a group has two rows or more (us, single
+// and in pairs: 64 rows, 128 groups, 2048 x 768 29 and 27, 128 rows, 64 groups, 4096 x 2048 141 and 131; 8 rows, 32 groups, 4096 x 4096 38 and 41); 8 waves
+// for a long k (4 rows, 8 groups, 14336 x 4096: 4 waves 70, 8 waves 66; 4 rows, 128 groups, 2048 x 768 5.5 and 6.0).
+template <class T> hipError_t grouped_stream(const GroupedParams& p, hipStream_t stream) {
+  const int64_t used = p.rows < p.groups ? p.rows : p.groups;
+  const bool pairs = p.rows >= 2 * (int64_t)p.groups || (p.k < 4096 && used * p.n > 16384);
+  if (p.k >= 8192) return pairs ? grouped_stream_launch<T, 2, 8, 2>(p, stream) : grouped_stream_launch<T, 1, 8, 4>(p, stream);
+  return pairs ? grouped_stream_launch<T, 2, 4, 4>(p, stream) : grouped_stream_launch<T, 1, 4, 4>(p, stream);
 }
 
 }  // namespace tnx

@@ -9,6 +9,7 @@
 #include "registry.h"
 #include "gemm_linear.h"
 #include "gemm_grouped.h"
+#include "gemm_stream.h"
 
 using namespace tnx;
 
@@ -178,10 +179,22 @@ template <class O> __global__ __launch_bounds__(256) void join_kernel(const floa
   }
 }
 
+// Few rows by k-contiguous weights of 16 bits, which gemm_stream.h reads once a group for up to 8 rows: 8 rows in all, or 4 to a group on average (us,
+// against the tile kernels': 32 rows, 8 groups, 14336 x 4096 144 and 164, 64 rows 212 and 164; 128 rows, 32 groups, 4096 x 4096 153 and 173), but not many workgroups of a short k (256 rows, 64 groups, 1024 x 4096
+// 88 and 82; 4 rows 8.2 and 8.5, 64 rows, 16 groups, 700 x 1000 7.4 and 8.8).
+bool takes_stream(const tnx_grouped_args* a) {
+  if (gradient(a) || a->dtype == TNX_F32 || a->block_m > 0 || a->k == 0 || a->stride_ak != 1 || a->stride_ar < a->k) return false;
+  if (a->stride_bn == 1 || a->stride_bk != 1 || a->stride_bn < a->k) return false;
+  if (a->k < 2048 && (a->rows < a->groups ? a->rows : a->groups) * a->n > 16384) return false;
+  // (a grid's threads are counted in 32 bits)
+  return (a->rows <= 8 || a->rows <= 4 * (int64_t)a->groups) && stream_runs(a->rows, a->groups) * ((a->n + 7) / 8) < (1 << 23) - 1;
+}
+
 }  // namespace
 
 extern "C" size_t tnx_grouped_workspace_bytes(const tnx_grouped_args* a) {
   if (check(a) != TNX_OK || a->n == 0 || (gradient(a) ? a->k == 0 : a->rows == 0)) return 0;
+  if (takes_stream(a)) return 0;
   const Choice c = choose(a);
   return c.entry && c.parts > 1 ? (size_t)c.parts * sums_of(a) * 4 : 0;
 }
@@ -192,6 +205,18 @@ extern "C" int tnx_grouped(const tnx_grouped_args* a) {
   const bool at = gradient(a);
   if (a->n == 0 || (at ? a->k == 0 : a->rows == 0)) return TNX_OK;
   if (!a->offsets || !a->c || (a->rows > 0 && a->k > 0 && (!a->a || !a->b))) return TNX_E_INVALID;
+  if (takes_stream(a)) {
+    GroupedParams p = {};
+    p.a = (const uint8_t*)a->a; p.b = (const uint8_t*)a->b; p.c = (uint8_t*)a->c;
+    p.offsets = a->offsets;
+    p.lda = a->stride_ar; p.ldb = a->stride_bn;
+    p.group_stride = a->stride_group;
+    p.rows = (int32_t)a->rows; p.n = (int32_t)a->n; p.k = (int32_t)a->k;
+    p.groups = a->groups;
+    const hipError_t err = a->dtype == TNX_BF16 ? grouped_stream<TagBF16>(p, (hipStream_t)a->stream) : grouped_stream<TagF16>(p, (hipStream_t)a->stream);
+    if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
+    return TNX_OK;
+  }
   Choice c = choose(a);
   const GroupedEntry* e = c.entry;
   if (!e) return TNX_E_UNSUPPORTED;
@@ -236,6 +261,10 @@ extern "C" int tnx_grouped(const tnx_grouped_args* a) {
 
 extern "C" int tnx_grouped_route(const tnx_grouped_args* a, int32_t info[5]) {
   if (check(a) != TNX_OK) return 0;
+  if (takes_stream(a)) {
+    if (info) memset(info, 0, 5 * sizeof *info);
+    return 2;
+  }
   const Choice c = choose(a);
   const GroupedEntry* e = c.entry;
   Layout l;
