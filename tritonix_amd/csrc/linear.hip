@@ -4,7 +4,7 @@
 //
 // The product runs on the tile kernels with the epilogue of gemm_linear.h, float32 on the same kernels by heads and tails or, small ones, on
 // the binary32 matrix instruction.  Where no such kernel takes the operands as they lie (an x that is contiguous along m, rows shorter
-// than a 16-byte chunk, k = 0) the sums go to scratch in 32 bits and the epilogue is a launch of its own.  dx = dz w^T and dw = x^T dz are
+// than a 16-byte chunk, k = 0) the sums go to scratch in 32 bits and the epilogue is a launch of its own.  Few rows of 16-bit types: gemm_stream.h.  dx = dz w^T and dw = x^T dz are
 // products without an epilogue.
 #include <hip/hip_runtime.h>
 #include <string.h>
