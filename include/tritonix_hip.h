@@ -587,9 +587,9 @@ typedef struct tnx_grouped_args {
 /* scratch that a product is faster with (few tiles of a long k), or 0.  Host arithmetic on the sizes */
 size_t tnx_grouped_workspace_bytes(const tnx_grouped_args* args);
 int tnx_grouped(const tnx_grouped_args* args);
-/* For tests and tooling: 1, 2 where few rows by k-contiguous weights are streamed, or 0 where tnx_grouped would refuse these args (of the pointers only the
+/* For tests and tooling: 1, 2 where few rows are streamed past the tiles, or 0 where tnx_grouped would refuse these args (of the pointers only the
  * alignment counts).  info (may be NULL): rows and columns of a tile, waves, whether each group's last slab of k is loaded apart, parts of k (given a
- * workspace); all zero for 2. */
+ * workspace); for 2 only the parts, 0 where k is not cut. */
 int tnx_grouped_route(const tnx_grouped_args* args, int32_t info[5]);
 
 #ifdef __cplusplus

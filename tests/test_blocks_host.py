@@ -157,6 +157,14 @@ def test_grouped_entry_point_refuses():
     few = dict(rows=12, stride_bk=1, stride_bn=64)
     assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**few)), info) == 2 and list(info) == [0] * 5
     assert lib.tnx_grouped_workspace_bytes(ctypes.byref(grouped_args(**{**few, "k": 4096, "stride_ar": 4096, "stride_bn": 4096}))) == 0
+    long = dict(rows=8, k=4096, stride_ar=4096)
+    assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**long)), info) == 2 and list(info) == [0, 0, 0, 0, 8]
+    need = lib.tnx_grouped_workspace_bytes(ctypes.byref(grouped_args(**long)))
+    assert need == 8 * 8 * 64 * 4
+    for workspace, length in ((4096, need - 1), (4104, need)):
+        assert lib.tnx_grouped(ctypes.byref(grouped_args(**long, workspace=workspace, workspace_bytes=length))) == _C.E_WORKSPACE
+    for more in (dict(rows=9), dict(k=1023, stride_ar=1023), dict(n=4096 + 64, stride_bk=4096 + 64), dict(dtype=_C.F32)):
+        assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**{**long, **more})), info) == 1, more
     for more in (dict(rows=13), dict(dtype=_C.F32), dict(block_m=64, block_n=64), dict(form=_C.GROUPED_WEIGHT_GRADIENT, stride_bk=64, stride_bn=1)):
         assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**{**few, **more})), info) == 1, more
     for more in (dict(stride_ar=63), dict(stride_bn=63), dict(stride_ak=2)):

@@ -132,14 +132,15 @@ def test_k_in_parts(device, dtype, tile, parts, monkeypatch):
 
 # counts of the groups' rows, rows ahead and behind, k, n: a row each, runs longer than 8 rows, many groups, short and long k
 FEW = [([1], 0, 0, 1, 1), ([0, 3, 0], 0, 0, 7, 5), ([1, 0, 1], 1, 2, 65, 9), ([0, 8], 0, 0, 640, 200), ([2, 0, 9, 1, 0], 3, 2, 1024, 136), ([0, 0, 0, 17, 0, 0, 0], 1, 2, 300, 77),
-       ([1, 0] * 60, 0, 3, 520, 600), ([4] * 9, 0, 0, 1030, 70), ([0] * 130 + [25, 3], 9, 40, 72, 40), ([3, 5], 0, 0, 8200, 24), ([1, 2, 0, 8, 4, 5], 2, 1, 9000, 20),
+       ([1, 0] * 60, 0, 3, 520, 600), ([4] * 9, 0, 0, 1030, 70), ([0] * 130 + [25, 3], 9, 40, 72, 40), ([3, 5], 0, 0, 8200, 24), ([1, 2, 0, 8, 4, 5], 2, 1, 9000, 20), ([1, 0, 2], 1, 1, 2100, 210), ([0, 0, 1], 0, 0, 1029, 8), ([3, 1], 0, 4, 1090, 1029),
        ([1, 0] * 60, 0, 3, 2050, 600)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES[:2])
 @pytest.mark.parametrize("case", range(len(FEW)))
 @pytest.mark.parametrize("pad,offset", [(0, 0), (64, 64), (1, 3)])
-def test_few_rows_by_k_contiguous_weights(device, dtype, case, pad, offset):
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+def test_few_rows(device, dtype, case, pad, offset, layout):
     """Few rows, streamed: groups of none to 25 rows, rows of the weights on lines of memory and off them, NaN between them that nothing may read."""
     counts, ahead, behind, k, n = FEW[case]
     rows, groups = ahead + sum(counts) + behind, len(counts)
@@ -150,13 +151,15 @@ def test_few_rows_by_k_contiguous_weights(device, dtype, case, pad, offset):
         out.copy_(ref.draw(device, m, columns, dtype=dtype, seed=seed, scale=scale))
         return out
 
-    pitch = (k + 63) // 64 * 64 if pad == 64 else k + pad
-    x, flat = strided(rows, k, k + pad, 1), strided(groups * n, k, pitch, 2, k ** -0.5)
-    w = flat.as_strided((groups, k, n), (n * pitch, 1, pitch), flat.storage_offset())
+    own, inner = (n, k) if layout == "nt" else (k, n)
+    pitch = (inner + 63) // 64 * 64 if pad == 64 else inner + pad
+    x, flat = strided(rows, k, k + pad, 1), strided(groups * own, inner, pitch, 2, k ** -0.5)
+    w = flat.as_strided((groups, k, n), (own * pitch, 1, pitch) if layout == "nt" else (own * pitch, pitch, 1), flat.storage_offset())
     offsets = offsets_of(device, counts, ahead)
     if n > 1 and k > 1:
         g = module._args(_C.GROUPED_ROWS, x, w, None, offsets, n, k, *w.stride())
-        streamed = k >= 2048 or min(rows, groups) * n <= 16384
+        used = min(rows, groups)
+        streamed = k >= 2048 or used * n <= 16384 if layout == "nt" else rows <= 8 and n >= 8 and k >= 1024 and used * ((n + 63) // 64) <= 128
         assert _C.load().tnx_grouped_route(ctypes.byref(g), None) == (2 if streamed else 1)
     y = tritonix.grouped_matmul(x, w, offsets)
     ref.check("y", y, ref.grouped(x, w, offsets)["y"], dtype)

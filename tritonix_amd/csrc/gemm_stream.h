@@ -173,7 +173,8 @@ struct StreamRowsParams {
 };
 static_assert(sizeof(StreamRowsParams) <= 112, "a longer argument list costs every launch 0.7 us");
 
-template <class T, int W, int U> __device__ __forceinline__ void stream_rows_block(const StreamRowsParams& p, int id) {
+// APART: the sums of a part go to y as they are, in 32 bits, for a launch that adds them up.
+template <class T, int W, int U, bool APART> __device__ __forceinline__ void stream_rows_block(const StreamRowsParams& p, int id) {
   static_assert(T::ES == 2, "16-bit element types only");
   typedef Mma<T, 16> MMA;
   typedef typename OutOf<T>::type O;
@@ -247,6 +248,13 @@ template <class T, int W, int U> __device__ __forceinline__ void stream_rows_blo
       for (int g = 0; g < 2; ++g) v += ((const float*)&sums[w][e][(g * 2 + (cc >> 2)) * 8 + m])[cc & 3];
     return v;
   };
+  if constexpr (APART) {
+    for (int o = threadIdx.x; o < p.m * 64; o += W * 64) {
+      const int own = n0 + (o & 56), n = (own < p.n - 8 ? own : p.n - 8) + (o & 7);
+      if (n >= own && own < p.n) ((float*)p.y)[(int64_t)(o >> 6) * p.n + n] = sum_of(o);
+    }
+    return;
+  }
   float* const slab = p.workspace ? (float*)(p.workspace + WS_COUNTER_BYTES) + (int64_t)tile * p.parts * p.m * 64 : nullptr;
   if (p.parts > 1) {
     for (int o = threadIdx.x; o < p.m * 64; o += W * 64)
@@ -284,7 +292,7 @@ template <class T, int W, int U> __device__ __forceinline__ void stream_rows_blo
 }
 
 template <class T, int W, int U> __global__ __launch_bounds__(W * 64) void gemm_stream_rows_kernel(StreamRowsParams p) {
-  stream_rows_block<T, W, U>(p, xcd_remap(blockIdx.x, (p.n + 63) / 64 * p.parts, 8));
+  stream_rows_block<T, W, U, false>(p, xcd_remap(blockIdx.x, (p.n + 63) / 64 * p.parts, 8));
 }
 
 // Workgroups to a block of 64 columns: one for each CU, twice as many where a wave then has no more than two steps (1 x 4096 x 4096, us: 4 parts 12.2, 8
@@ -309,8 +317,7 @@ template <class T> hipError_t stream_rows(const StreamRowsParams& p, hipStream_t
 
 // The k-contiguous one by groups of rows, a weight to each (gemm_grouped.h): 8 rows of a group at a time, for few rows in all or few to a group.  A workgroup
 // finds its rows in the bounds, which are all that it waits for.  bf16, cold weights, us, against the tile kernels': 2 rows, 64 groups, 4096 x 2048 8.5 and 15.1,
-// 4 rows, 128 groups, 2048 x 768 5.5 and 11.8, 16 rows, 64 groups, 4096 x 2048 38 and 40, 64 rows, 128 groups, 2048 x 768 27 and 37.  (A row-major weight's 64
-// columns are too few workgroups here as well: even with the tile kernels at best, 1 row, 64 groups, 4096 x 2048 19.0 and 15.6.)
+// 4 rows, 128 groups, 2048 x 768 5.5 and 11.8, 16 rows, 64 groups, 4096 x 2048 38 and 40, 64 rows, 128 groups, 2048 x 768 27 and 37.
 template <class T, int NT, int W, int U, bool LINES> __global__ __launch_bounds__(W * 64) void grouped_stream_kernel(GroupedParams q) {
   constexpr int ES = T::ES, COLUMNS = 8 * NT;
   const int across = (int)(((uint32_t)q.n + COLUMNS - 1) / COLUMNS), id = windowed<64>(blockIdx.x, gridDim.x), want = id / across, block = id - want * across;
@@ -350,6 +357,33 @@ template <class T> hipError_t grouped_stream(const GroupedParams& p, hipStream_t
   const bool pairs = p.rows >= 2 * (int64_t)p.groups || (p.k < 4096 && used * p.n > 16384);
   if (p.k >= 8192) return pairs ? grouped_stream_launch<T, 2, 8, 2>(p, stream) : grouped_stream_launch<T, 1, 8, 4>(p, stream);
   return pairs ? grouped_stream_launch<T, 2, 4, 4>(p, stream) : grouped_stream_launch<T, 1, 4, 4>(p, stream);
+}
+
+// Row-major weights of a few groups, in parts of k whose sums another launch adds up.
+template <class T> __global__ __launch_bounds__(STREAM_ROWS_WAVES * 64) void grouped_stream_rows_kernel(GroupedParams q) {
+  constexpr int ES = T::ES;
+  const int across = (int)(((uint32_t)q.n + 63) / 64) * q.parts, id = windowed<64>(blockIdx.x, gridDim.x), want = id / across, block = id - want * across;
+  int total = 0;
+  const GroupedFamily<false>::Stretch s = GroupedFamily<false>::stretch_of<8>(q, threadIdx.x & 63, want, &total);
+  if (s.number < 0) return;
+  const int skip = (want - s.before) * 8, m = s.rows - skip < 8 ? s.rows - skip : 8, part = block % q.parts;
+  const int64_t row = s.first + skip;
+  float* const y = (float*)q.c + part * q.part_stride + row * q.n;
+  if (s.number == 0 || s.number == q.groups + 1) {
+    for (int o = threadIdx.x; o < m * 64; o += STREAM_ROWS_WAVES * 64) {
+      const int n = block / q.parts * 64 + o % 64;
+      if (n < q.n) y[(int64_t)(o / 64) * q.n + n] = 0.0f;
+    }
+    return;
+  }
+  const uint8_t* const x = q.a + row * q.lda * ES;
+  const uint8_t* const w = q.b + (int64_t)(s.number - 1) * q.group_stride * ES;
+  stream_rows_block<T, STREAM_ROWS_WAVES, 2, true>({x, w, (uint8_t*)y, nullptr, nullptr, nullptr, nullptr, q.lda, q.ldb, m, q.n, q.k, q.parts, ACT_NONE}, block);
+}
+template <class T> hipError_t grouped_stream_rows(const GroupedParams& p, hipStream_t stream) {
+  GroupedParams q = p;
+  const unsigned grid = (unsigned)(stream_runs(p.rows, p.groups) * ((p.n + 63) / 64) * p.parts);
+  return launch_kernel((const void*)&grouped_stream_rows_kernel<T>, grid, STREAM_ROWS_WAVES * 64, 0, stream, &q);
 }
 
 }  // namespace tnx

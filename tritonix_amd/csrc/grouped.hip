@@ -190,11 +190,34 @@ bool takes_stream(const tnx_grouped_args* a) {
   return (a->rows <= 8 || a->rows <= 4 * (int64_t)a->groups) && stream_runs(a->rows, a->groups) * ((a->n + 7) / 8) < (1 << 23) - 1;
 }
 
+// Up to 8 rows by row-major weights, while blocks of 64 columns times groups leave half of the CUs without a workgroup and k has parts for them: those
+// parts, a workgroup to a CU, or 0: not taken (us, against the tile kernels': 1 row, 64 groups, 4096 x 2048 9.5 and 15.7, 4 rows 17.4 and 21.2, 2 rows, 128
+// groups, 2048 x 768 7.4 and 14.2; a workgroup to every block without parts, 8 rows, 64 groups, 4096 x 2048: 26.4 and 24.9).
+int stream_rows_parts(const tnx_grouped_args* a) {
+  if (gradient(a) || a->dtype == TNX_F32 || a->block_m > 0 || a->stride_ak != 1 || a->stride_ar < a->k) return 0;
+  if (a->stride_bn != 1 || a->stride_bk < a->n || a->n < 8 || a->rows > 8) return 0;
+  const int64_t blocks = (a->rows < a->groups ? a->rows : a->groups) * ((a->n + 63) / 64), most = a->k / (64 * STREAM_ROWS_WAVES);
+  int64_t parts = blocks > 0 ? 256 / blocks : 0;
+  if (parts > most) parts = most;
+  return parts >= 2 ? (int)parts : 0;
+}
+
+hipError_t join(const tnx_grouped_args* a, int parts, int64_t sums) {
+  const dim3 grid((unsigned)((sums + 1023) / 1024));
+  const float* from = (const float*)a->workspace;
+  const hipStream_t stream = (hipStream_t)a->stream;
+  if (a->dtype == TNX_BF16) hipLaunchKernelGGL(join_kernel<OutBF16>, grid, dim3(256), 0, stream, from, parts, sums, sums, (uint8_t*)a->c);
+  else if (a->dtype == TNX_F16) hipLaunchKernelGGL(join_kernel<OutF16>, grid, dim3(256), 0, stream, from, parts, sums, sums, (uint8_t*)a->c);
+  else hipLaunchKernelGGL(join_kernel<OutF32>, grid, dim3(256), 0, stream, from, parts, sums, sums, (uint8_t*)a->c);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 extern "C" size_t tnx_grouped_workspace_bytes(const tnx_grouped_args* a) {
   if (check(a) != TNX_OK || a->n == 0 || (gradient(a) ? a->k == 0 : a->rows == 0)) return 0;
   if (takes_stream(a)) return 0;
+  if (const int parts = stream_rows_parts(a)) return (size_t)parts * sums_of(a) * 4;
   const Choice c = choose(a);
   return c.entry && c.parts > 1 ? (size_t)c.parts * sums_of(a) * 4 : 0;
 }
@@ -214,6 +237,22 @@ extern "C" int tnx_grouped(const tnx_grouped_args* a) {
     p.rows = (int32_t)a->rows; p.n = (int32_t)a->n; p.k = (int32_t)a->k;
     p.groups = a->groups;
     const hipError_t err = a->dtype == TNX_BF16 ? grouped_stream<TagBF16>(p, (hipStream_t)a->stream) : grouped_stream<TagF16>(p, (hipStream_t)a->stream);
+    if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
+    return TNX_OK;
+  }
+  if (const int parts = a->workspace && a->k > 0 ? stream_rows_parts(a) : 0) {
+    const int64_t sums = sums_of(a);
+    if (a->workspace_bytes < (size_t)parts * sums * 4 || ((uintptr_t)a->workspace & 15)) return TNX_E_WORKSPACE;
+    GroupedParams p = {};
+    p.a = (const uint8_t*)a->a; p.b = (const uint8_t*)a->b; p.c = (uint8_t*)a->workspace;
+    p.offsets = a->offsets;
+    p.lda = a->stride_ar; p.ldb = a->stride_bk;
+    p.group_stride = a->stride_group;
+    p.rows = (int32_t)a->rows; p.n = (int32_t)a->n; p.k = (int32_t)a->k;
+    p.groups = a->groups;
+    p.parts = parts; p.part_stride = sums;
+    hipError_t err = a->dtype == TNX_BF16 ? grouped_stream_rows<TagBF16>(p, (hipStream_t)a->stream) : grouped_stream_rows<TagF16>(p, (hipStream_t)a->stream);
+    if (err == hipSuccess) err = join(a, parts, sums);
     if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
     return TNX_OK;
   }
@@ -249,20 +288,19 @@ extern "C" int tnx_grouped(const tnx_grouped_args* a) {
   const hipError_t err = fn(p, (unsigned)(tiles_m * tiles_n * c.parts), (hipStream_t)a->stream);
   if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
   if (!cut) return TNX_OK;
-  const dim3 grid((unsigned)((sums + 1023) / 1024));
-  const float* from = (const float*)a->workspace;
-  if (a->dtype == TNX_BF16) hipLaunchKernelGGL(join_kernel<OutBF16>, grid, dim3(256), 0, (hipStream_t)a->stream, from, c.parts, sums, sums, (uint8_t*)a->c);
-  else if (a->dtype == TNX_F16) hipLaunchKernelGGL(join_kernel<OutF16>, grid, dim3(256), 0, (hipStream_t)a->stream, from, c.parts, sums, sums, (uint8_t*)a->c);
-  else hipLaunchKernelGGL(join_kernel<OutF32>, grid, dim3(256), 0, (hipStream_t)a->stream, from, c.parts, sums, sums, (uint8_t*)a->c);
-  const hipError_t joined = hipGetLastError();
+  const hipError_t joined = join(a, c.parts, sums);
   if (joined != hipSuccess) { note_hip_error((int)joined); return TNX_E_HIP; }
   return TNX_OK;
 }
 
 extern "C" int tnx_grouped_route(const tnx_grouped_args* a, int32_t info[5]) {
   if (check(a) != TNX_OK) return 0;
-  if (takes_stream(a)) {
-    if (info) memset(info, 0, 5 * sizeof *info);
+  const int parts = a->k > 0 ? stream_rows_parts(a) : 0;
+  if (parts || takes_stream(a)) {
+    if (info) {
+      memset(info, 0, 5 * sizeof *info);
+      info[4] = parts;
+    }
     return 2;
   }
   const Choice c = choose(a);
