@@ -74,7 +74,7 @@ def test_every_choice_of_tile_has_the_epilogue(dtype, layout):
                                      (8, 64, 72, 200, 512, 1000, 2048, 4096, 5000, 14336)):
         info = (ctypes.c_int32 * 5)()
         route = lib.tnx_linear_route(ctypes.byref(linear_args(m, n, k, dtype, layout)), info)
-        if dtype != _C.F32 and route == (_C.LINEAR_ROUTE_STREAM if layout == "nt" else _C.LINEAR_ROUTE_STREAM_ROWS) and m <= (16 if layout == "nt" else 8):
+        if route == (_C.LINEAR_ROUTE_STREAM if layout == "nt" else _C.LINEAR_ROUTE_STREAM_ROWS) and m <= (16 if layout == "nt" else 8):
             continue
         assert route == _C.LINEAR_ROUTE_FUSED, (m, n, k, list(info))
         tiles.add(tuple(info[:4]))
@@ -93,7 +93,10 @@ def test_routes_of_a_linear_layer():
         few = linear_args(m, n, k, layout="nt")
         assert route(few) == _C.LINEAR_ROUTE_STREAM and lib.tnx_linear_workspace_bytes(ctypes.byref(few)) == 0
     assert route(linear_args(17, 200, 304, layout="nt")) == route(linear_args(16, 512, 8192, layout="nt")) == _C.LINEAR_ROUTE_FUSED
-    assert route(linear_args(4, 200, 304, _C.F32, "nt")) == route(linear_args(4, 200, 304, _C.F32)) == _C.LINEAR_ROUTE_FUSED
+    assert route(linear_args(4, 200, 304, _C.F32, "nt")) == route(linear_args(8, 16384, 4096, _C.F32, "nt")) == _C.LINEAR_ROUTE_STREAM
+    assert route(linear_args(4, 20000, 304, _C.F32)) == _C.LINEAR_ROUTE_STREAM_ROWS
+    for other in (linear_args(9, 200, 304, _C.F32, "nt"), linear_args(8, 200, 4104, _C.F32, "nt"), linear_args(5, 200, 304, _C.F32), linear_args(4, 200, 4104, _C.F32)):
+        assert route(other) == _C.LINEAR_ROUTE_FUSED
     for m, n, k in ((1, 8, 1), (4, 200, 304), (4, 4096, 4096), (8, 16000, 2048)):
         few = linear_args(m, n, k)
         assert route(few) == _C.LINEAR_ROUTE_STREAM_ROWS
@@ -163,9 +166,10 @@ def test_grouped_entry_point_refuses():
     assert need == 8 * 8 * 64 * 4
     for workspace, length in ((4096, need - 1), (4104, need)):
         assert lib.tnx_grouped(ctypes.byref(grouped_args(**long, workspace=workspace, workspace_bytes=length))) == _C.E_WORKSPACE
-    for more in (dict(rows=9), dict(k=1023, stride_ar=1023), dict(n=4096 + 64, stride_bk=4096 + 64), dict(dtype=_C.F32)):
+    for more in (dict(rows=9), dict(k=1023, stride_ar=1023), dict(n=4096 + 64, stride_bk=4096 + 64)):
         assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**{**long, **more})), info) == 1, more
-    for more in (dict(rows=13), dict(dtype=_C.F32), dict(block_m=64, block_n=64), dict(form=_C.GROUPED_WEIGHT_GRADIENT, stride_bk=64, stride_bn=1)):
+    assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**few, dtype=_C.F32)), info) == 2
+    for more in (dict(rows=13), dict(block_m=64, block_n=64), dict(form=_C.GROUPED_WEIGHT_GRADIENT, stride_bk=64, stride_bn=1)):
         assert lib.tnx_grouped_route(ctypes.byref(grouped_args(**{**few, **more})), info) == 1, more
     for more in (dict(stride_ar=63), dict(stride_bn=63), dict(stride_ak=2)):
         assert lib.tnx_grouped(ctypes.byref(grouped_args(**{**few, **more}))) == _C.E_UNSUPPORTED, more

@@ -136,7 +136,7 @@ FEW = [([1], 0, 0, 1, 1), ([0, 3, 0], 0, 0, 7, 5), ([1, 0, 1], 1, 2, 65, 9), ([0
        ([1, 0] * 60, 0, 3, 2050, 600)]
 
 
-@pytest.mark.parametrize("dtype", DTYPES[:2])
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("case", range(len(FEW)))
 @pytest.mark.parametrize("pad,offset", [(0, 0), (64, 64), (1, 3)])
 @pytest.mark.parametrize("layout", ["nt", "nn"])

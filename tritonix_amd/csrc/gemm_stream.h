@@ -29,19 +29,18 @@ struct StreamParams {
 static_assert(sizeof(StreamParams) <= 112, "a longer argument list costs every launch 0.7 us");
 
 // C: columns of the weight and rows of x at most; W: waves; U: steps of 64 x 16 / C of k in flight; LINES: rows of the weight begin on lines of memory,
-// of which nothing is left for another instruction to read (with C = 8, us: 1 x 4096 x 4096 7.6 past the caches and 8.1 through them; rows that begin
+// of which nothing is left for another instruction to read (float32: half of these numbers, and the binary32 instruction four times; with C = 8, us: 1 x 4096 x 4096 7.6 past the caches and 8.1 through them; rows that begin
 // anywhere, 1 x 2050 x 4100 7.5 and 6.4).
 template <class T, int C, int NT, int W, int U, bool LINES> __device__ __forceinline__ void stream_block(const StreamParams& p, int block) {
-  static_assert(T::ES == 2, "16-bit element types only");
   typedef Mma<T, 16> MMA;
   typedef typename OutOf<T>::type O;
   typedef typename O::raw raw;
-  constexpr int G = 16 / C, STEP = 64 * G, HALF = 32 * G;
+  constexpr int V = 16 / T::ES, G = 16 / C, HALF = 4 * V * G, STEP = 2 * HALF;
   __shared__ f32x4 sums[W][NT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, kg = lane >> 4;
   const int n0 = block * (C * NT);
-  const int koff = li / C * 32 + kg * 8;
+  const int koff = li / C * (4 * V) + kg * V;
   const raw* const xp = (const raw*)p.x + (int64_t)(li % C < p.m ? li % C : p.m - 1) * p.ldx + koff;
   const raw* wp[NT];
 #pragma unroll
@@ -88,10 +87,10 @@ template <class T, int C, int NT, int W, int U, bool LINES> __device__ __forcein
       const int left = p.k - (int)at - koff;
       auto fetch = [&](const raw* from) __attribute__((always_inline)) {
         i32x4 v = {};
-        if (left >= 8) return (i32x4)*(const i32x4_loose*)(from + at);
-        raw e[8];
+        if (left >= V) return (i32x4)*(const i32x4_loose*)(from + at);
+        raw e[V];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = i < left ? from[at + i] : (raw)0;
+        for (int i = 0; i < V; ++i) e[i] = i < left ? from[at + i] : (raw)0;
         __builtin_memcpy(&v, e, 16);
         return v;
       };
@@ -118,7 +117,7 @@ template <class T, int C, int NT, int W, int U, bool LINES> __device__ __forcein
     if (p.bias) v += bias_value(p.bias, n0 + n, p.bias_dtype);
     if (p.z) ((raw*)p.z)[at] = O::cvt(v);
     v = activate(v, p.act);
-    if (p.residual) v += Run<O, 8>::widen(((const raw*)p.residual)[at]);
+    if (p.residual) v += Run<O, V>::widen(((const raw*)p.residual)[at]);
     ((raw*)p.y)[at] = O::cvt(v);
   }
 }
@@ -134,13 +133,13 @@ template <class T, int C, int NT, int W, int U, bool LINES> hipError_t stream_la
 
 // waves: 4 where k has no step for each of 8 (1 x 30000 x 512, us: 7.1 and 8.1)
 template <class T, int C, int NT, int U, bool LINES> hipError_t stream_waves(const StreamParams& p, hipStream_t stream) {
-  if (p.k < 8 * 64 * (16 / C)) return stream_launch<T, C, NT, 4, U, LINES>(p, stream);
+  if (p.k < 8 * (128 / T::ES) * (16 / C)) return stream_launch<T, C, NT, 4, U, LINES>(p, stream);
   return stream_launch<T, C, NT, 8, U, LINES>(p, stream);
 }
 
 template <class T, int C, int NT, int U> hipError_t stream_lines(const StreamParams& p, hipStream_t stream) {
   if constexpr (C < 16)
-    if (p.ldw % 64 == 0 && ((uintptr_t)p.w & 127) == 0) return stream_waves<T, C, NT, U, true>(p, stream);
+    if (p.ldw % (128 / T::ES) == 0 && ((uintptr_t)p.w & 127) == 0) return stream_waves<T, C, NT, U, true>(p, stream);
   return stream_waves<T, C, NT, U, false>(p, stream);
 }
 
@@ -153,7 +152,7 @@ template <class T> hipError_t stream_columns(const StreamParams& p, hipStream_t 
   return stream_lines<T, 16, 1, 4>(p, stream);
 }
 
-// The same for a row-major weight, up to 8 rows.  A workgroup owns 64 columns (a line of memory of each row of the weight), a step is 64 of k: a lane
+// The same for a row-major weight, up to 8 rows.  A workgroup owns 64 columns (float32: 32; a line of memory of each row of the weight), a step is 64 of k: a lane
 // reads 8 columns of 8 rows of the weight and picks the 8 numbers of a column together with v_perm_b32, half an instruction a number.  Column e of
 // every lane makes one matrix instruction: 8 columns in two groups, as C = 8 above.  64 columns are few workgroups (narrower ones would leave parts of
 // lines), so that `parts` of them share a block's k: each writes its sums through its L2, and the one that arrives last adds them up in the order of the parts.
@@ -175,39 +174,42 @@ static_assert(sizeof(StreamRowsParams) <= 112, "a longer argument list costs eve
 
 // APART: the sums of a part go to y as they are, in 32 bits, for a launch that adds them up.
 template <class T, int W, int U, bool APART> __device__ __forceinline__ void stream_rows_block(const StreamRowsParams& p, int id) {
-  static_assert(T::ES == 2, "16-bit element types only");
   typedef Mma<T, 16> MMA;
   typedef typename OutOf<T>::type O;
   typedef typename O::raw raw;
-  __shared__ f32x4 sums[W][8][32];
+  constexpr int V = 16 / T::ES, COLUMNS = 8 * V, STEP = 8 * V;
+  __shared__ f32x4 sums[W][V][32];
   __shared__ int arrived;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, octet = (li >> 3) * 4 + (lane >> 4), c = li & 7;
-  const int tile = id / p.parts, part = id - tile * p.parts, n0 = tile * 64;
-  // (the last run of 8 columns begins where it ends with the row)
-  const int col = n0 + c * 8 < p.n - 8 ? n0 + c * 8 : p.n - 8;
-  const raw* const xp = (const raw*)p.x + (int64_t)(c < p.m ? c : p.m - 1) * p.ldx + octet * 8;
-  const raw* const wp = (const raw*)p.w + (int64_t)(octet * 8) * p.ldw + col;
-  f32x4 acc[8] = {};
-  auto multiply = [&](const i32x4 (&b)[8], i32x4 a) __attribute__((always_inline)) {
+  const int tile = id / p.parts, part = id - tile * p.parts, n0 = tile * COLUMNS;
+  // (the last run of columns begins where it ends with the row)
+  const int col = n0 + c * V < p.n - V ? n0 + c * V : p.n - V;
+  const raw* const xp = (const raw*)p.x + (int64_t)(c < p.m ? c : p.m - 1) * p.ldx + octet * V;
+  const raw* const wp = (const raw*)p.w + (int64_t)(octet * V) * p.ldw + col;
+  f32x4 acc[V] = {};
+  auto multiply = [&](const i32x4 (&b)[V], i32x4 a) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < V; ++e) {
       i32x4 v;
 #pragma unroll
-      for (int d = 0; d < 4; ++d) v[d] = (int)__builtin_amdgcn_perm((uint32_t)b[2 * d + 1][e / 2], (uint32_t)b[2 * d][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+      for (int d = 0; d < 4; ++d) {
+        if constexpr (T::ES == 4) v[d] = b[d][e];
+        else v[d] = (int)__builtin_amdgcn_perm((uint32_t)b[2 * d + 1][e / 2], (uint32_t)b[2 * d][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+      }
       acc[e] = MMA::run(v, a, acc[e]);
     }
   };
-  const int whole = p.k / 64, turn = W * p.parts;
+  const int whole = p.k / STEP, turn = W * p.parts;
   auto steps = [&](int s, auto count) __attribute__((always_inline)) {
     constexpr int N = decltype(count)::value;
-    i32x4 b[N][8], a[N];
+    i32x4 b[N][V], a[N];
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const raw* const from = wp + (int64_t)(s + u * turn) * 64 * p.ldw;
+      const raw* const from = wp + (int64_t)(s + u * turn) * STEP * p.ldw;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[u][j] = (i32x4)__builtin_nontemporal_load((const i32x4_loose*)(from + j * p.ldw));
-      a[u] = *(const i32x4_loose*)(xp + (int64_t)(s + u * turn) * 64);
+      for (int j = 0; j < V; ++j) b[u][j] = (i32x4)__builtin_nontemporal_load((const i32x4_loose*)(from + j * p.ldw));
+      a[u] = *(const i32x4_loose*)(xp + (int64_t)(s + u * turn) * STEP);
     }
 #pragma unroll
     for (int u = 0; u < N; ++u) multiply(b[u], a[u]);
@@ -215,20 +217,20 @@ template <class T, int W, int U, bool APART> __device__ __forceinline__ void str
   int s = part * W + wave;
   for (; s + (U - 1) * turn < whole; s += U * turn) steps(s, std::integral_constant<int, U>());
   for (; s < whole; s += turn) steps(s, std::integral_constant<int, 1>());
-  if (s == whole && whole * 64 < p.k) {
-    const int left = p.k - whole * 64 - octet * 8;
-    i32x4 b[8], a = {};
+  if (s == whole && whole * STEP < p.k) {
+    const int left = p.k - whole * STEP - octet * V;
+    i32x4 b[V], a = {};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < V; ++j) {
       b[j] = i32x4{0, 0, 0, 0};
-      if (j < left) b[j] = *(const i32x4_loose*)(wp + ((int64_t)whole * 64 + j) * p.ldw);
+      if (j < left) b[j] = *(const i32x4_loose*)(wp + ((int64_t)whole * STEP + j) * p.ldw);
     }
-    const raw* const from = xp + (int64_t)whole * 64;
-    if (left >= 8) a = *(const i32x4_loose*)from;
+    const raw* const from = xp + (int64_t)whole * STEP;
+    if (left >= V) a = *(const i32x4_loose*)from;
     else {
-      raw e[8];
+      raw e[V];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = i < left ? from[i] : (raw)0;
+      for (int i = 0; i < V; ++i) e[i] = i < left ? from[i] : (raw)0;
       __builtin_memcpy(&a, e, 16);
     }
     multiply(b, a);
@@ -236,11 +238,11 @@ template <class T, int W, int U, bool APART> __device__ __forceinline__ void str
   // rows 0 to 7 of the sums are the first group's columns, whose x is in columns 0 to 7, the others the second's
   if ((lane >> 5) == (li >> 3)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[wave][e][(lane >> 4) * 8 + c] = acc[e];
+    for (int e = 0; e < V; ++e) sums[wave][e][(lane >> 4) * 8 + c] = acc[e];
   }
   __syncthreads();
   auto sum_of = [&](int o) __attribute__((always_inline)) {
-    const int m = o >> 6, cc = (o >> 3) & 7, e = o & 7;
+    const int m = o / COLUMNS, cc = o / V % 8, e = o % V;
     float v = 0.0f;
 #pragma unroll
     for (int w = 0; w < W; ++w)
@@ -248,17 +250,22 @@ template <class T, int W, int U, bool APART> __device__ __forceinline__ void str
       for (int g = 0; g < 2; ++g) v += ((const float*)&sums[w][e][(g * 2 + (cc >> 2)) * 8 + m])[cc & 3];
     return v;
   };
+  // the column of an output, or -1: not there, or another run's
+  auto column_of = [&](int o) __attribute__((always_inline)) {
+    const int own = n0 + o % COLUMNS / V * V, n = (own < p.n - V ? own : p.n - V) + o % V;
+    return n >= own && own < p.n ? n : -1;
+  };
   if constexpr (APART) {
-    for (int o = threadIdx.x; o < p.m * 64; o += W * 64) {
-      const int own = n0 + (o & 56), n = (own < p.n - 8 ? own : p.n - 8) + (o & 7);
-      if (n >= own && own < p.n) ((float*)p.y)[(int64_t)(o >> 6) * p.n + n] = sum_of(o);
+    for (int o = threadIdx.x; o < p.m * COLUMNS; o += W * 64) {
+      const int n = column_of(o);
+      if (n >= 0) ((float*)p.y)[(int64_t)(o / COLUMNS) * p.n + n] = sum_of(o);
     }
     return;
   }
-  float* const slab = p.workspace ? (float*)(p.workspace + WS_COUNTER_BYTES) + (int64_t)tile * p.parts * p.m * 64 : nullptr;
+  float* const slab = p.workspace ? (float*)(p.workspace + WS_COUNTER_BYTES) + (int64_t)tile * p.parts * p.m * COLUMNS : nullptr;
   if (p.parts > 1) {
-    for (int o = threadIdx.x; o < p.m * 64; o += W * 64)
-      __hip_atomic_store(slab + (int64_t)part * p.m * 64 + o, sum_of(o), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int o = threadIdx.x; o < p.m * COLUMNS; o += W * 64)
+      __hip_atomic_store(slab + (int64_t)part * p.m * COLUMNS + o, sum_of(o), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -272,13 +279,13 @@ template <class T, int W, int U, bool APART> __device__ __forceinline__ void str
     if (arrived != p.parts - 1) return;
   }
   const int act = p.flags & 255, bias_dtype = p.flags >> 8;
-  for (int o = threadIdx.x; o < p.m * 64; o += W * 64) {
-    const int m = o >> 6, own = n0 + (o & 56), n = (own < p.n - 8 ? own : p.n - 8) + (o & 7);
-    if (n < own || own >= p.n) continue;                   // (another lane's run has it)
+  for (int o = threadIdx.x; o < p.m * COLUMNS; o += W * 64) {
+    const int m = o / COLUMNS, n = column_of(o);
+    if (n < 0) continue;
     float v = 0.0f;
     if (p.parts > 1) {
 #pragma unroll 8
-      for (int q = 0; q < p.parts; ++q) v += __hip_atomic_load(slab + (int64_t)q * p.m * 64 + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int q = 0; q < p.parts; ++q) v += __hip_atomic_load(slab + (int64_t)q * p.m * COLUMNS + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     } else {
       v = sum_of(o);
     }
@@ -286,33 +293,33 @@ template <class T, int W, int U, bool APART> __device__ __forceinline__ void str
     if (p.bias) v += bias_value(p.bias, n, bias_dtype);
     if (p.z) ((raw*)p.z)[at] = O::cvt(v);
     v = activate(v, act);
-    if (p.residual) v += Run<O, 8>::widen(((const raw*)p.residual)[at]);
+    if (p.residual) v += Run<O, V>::widen(((const raw*)p.residual)[at]);
     ((raw*)p.y)[at] = O::cvt(v);
   }
 }
 
 template <class T, int W, int U> __global__ __launch_bounds__(W * 64) void gemm_stream_rows_kernel(StreamRowsParams p) {
-  stream_rows_block<T, W, U, false>(p, xcd_remap(blockIdx.x, (p.n + 63) / 64 * p.parts, 8));
+  stream_rows_block<T, W, U, false>(p, xcd_remap(blockIdx.x, (p.n + 128 / T::ES - 1) / (128 / T::ES) * p.parts, 8));
 }
 
 // Workgroups to a block of 64 columns: one for each CU, twice as many where a wave then has no more than two steps (1 x 4096 x 4096, us: 4 parts 12.2, 8
 // parts 11.6; 1 x 8192 x 8192 2 parts 27.2, 4 parts 30.0), and a step at least for each wave.
 constexpr int STREAM_ROWS_WAVES = 8;
-inline int stream_rows_parts(int64_t n, int64_t k) {
-  const int64_t tiles = (n + 63) / 64, most = k / (64 * STREAM_ROWS_WAVES);
+inline int stream_rows_parts(int64_t n, int64_t k, int es) {
+  const int64_t step = 128 / es, tiles = (n + step - 1) / step, most = k / (step * STREAM_ROWS_WAVES);
   int64_t parts = tiles < 256 ? 256 / tiles : 1;
-  if (k <= parts * STREAM_ROWS_WAVES * 128) parts *= 2;
+  if (k <= parts * STREAM_ROWS_WAVES * 2 * step) parts *= 2;
   if (parts > most) parts = most;
   return parts < 1 ? 1 : (int)parts;
 }
-inline size_t stream_rows_workspace(int64_t m, int64_t n, int64_t k) {
-  const int parts = stream_rows_parts(n, k);
-  return parts > 1 ? WS_COUNTER_BYTES + (size_t)((n + 63) / 64) * parts * m * 64 * 4 : 0;
+inline size_t stream_rows_workspace(int64_t m, int64_t n, int64_t k, int es) {
+  const int64_t columns = 128 / es, parts = stream_rows_parts(n, k, es);
+  return parts > 1 ? WS_COUNTER_BYTES + (size_t)((n + columns - 1) / columns) * parts * m * columns * 4 : 0;
 }
 
 template <class T> hipError_t stream_rows(const StreamRowsParams& p, hipStream_t stream) {
   StreamRowsParams q = p;
-  return launch_kernel((const void*)&gemm_stream_rows_kernel<T, STREAM_ROWS_WAVES, 2>, (unsigned)((p.n + 63) / 64 * p.parts), STREAM_ROWS_WAVES * 64, 0, stream, &q);
+  return launch_kernel((const void*)&gemm_stream_rows_kernel<T, STREAM_ROWS_WAVES, 2>, (unsigned)((p.n + 128 / T::ES - 1) / (128 / T::ES) * p.parts), STREAM_ROWS_WAVES * 64, 0, stream, &q);
 }
 
 // The k-contiguous one by groups of rows, a weight to each (gemm_grouped.h): 8 rows of a group at a time, for few rows in all or few to a group.  A workgroup
@@ -345,7 +352,7 @@ inline int64_t stream_runs(int64_t rows, int64_t groups) { return rows / 8 + (gr
 template <class T, int NT, int W, int U> hipError_t grouped_stream_launch(const GroupedParams& p, hipStream_t stream) {
   GroupedParams q = p;
   const unsigned grid = (unsigned)(stream_runs(p.rows, p.groups) * ((p.n + 8 * NT - 1) / (8 * NT)));
-  const bool lines = p.ldb % 64 == 0 && p.group_stride % 64 == 0 && ((uintptr_t)p.b & 127) == 0;
+  const bool lines = p.ldb % (128 / T::ES) == 0 && p.group_stride % (128 / T::ES) == 0 && ((uintptr_t)p.b & 127) == 0;
   if (lines) return launch_kernel((const void*)&grouped_stream_kernel<T, NT, W, U, true>, grid, W * 64, 0, stream, &q);
   return launch_kernel((const void*)&grouped_stream_kernel<T, NT, W, U, false>, grid, W * 64, 0, stream, &q);
 }
@@ -361,8 +368,8 @@ template <class T> hipError_t grouped_stream(const GroupedParams& p, hipStream_t
 
 // Row-major weights of a few groups, in parts of k whose sums another launch adds up.
 template <class T> __global__ __launch_bounds__(STREAM_ROWS_WAVES * 64) void grouped_stream_rows_kernel(GroupedParams q) {
-  constexpr int ES = T::ES;
-  const int across = (int)(((uint32_t)q.n + 63) / 64) * q.parts, id = windowed<64>(blockIdx.x, gridDim.x), want = id / across, block = id - want * across;
+  constexpr int ES = T::ES, COLUMNS = 128 / ES;
+  const int across = (int)(((uint32_t)q.n + COLUMNS - 1) / COLUMNS) * q.parts, id = windowed<64>(blockIdx.x, gridDim.x), want = id / across, block = id - want * across;
   int total = 0;
   const GroupedFamily<false>::Stretch s = GroupedFamily<false>::stretch_of<8>(q, threadIdx.x & 63, want, &total);
   if (s.number < 0) return;
@@ -370,9 +377,9 @@ template <class T> __global__ __launch_bounds__(STREAM_ROWS_WAVES * 64) void gro
   const int64_t row = s.first + skip;
   float* const y = (float*)q.c + part * q.part_stride + row * q.n;
   if (s.number == 0 || s.number == q.groups + 1) {
-    for (int o = threadIdx.x; o < m * 64; o += STREAM_ROWS_WAVES * 64) {
-      const int n = block / q.parts * 64 + o % 64;
-      if (n < q.n) y[(int64_t)(o / 64) * q.n + n] = 0.0f;
+    for (int o = threadIdx.x; o < m * COLUMNS; o += STREAM_ROWS_WAVES * 64) {
+      const int n = block / q.parts * COLUMNS + o % COLUMNS;
+      if (n < q.n) y[(int64_t)(o / COLUMNS) * q.n + n] = 0.0f;
     }
     return;
   }
@@ -382,7 +389,7 @@ template <class T> __global__ __launch_bounds__(STREAM_ROWS_WAVES * 64) void gro
 }
 template <class T> hipError_t grouped_stream_rows(const GroupedParams& p, hipStream_t stream) {
   GroupedParams q = p;
-  const unsigned grid = (unsigned)(stream_runs(p.rows, p.groups) * ((p.n + 63) / 64) * p.parts);
+  const unsigned grid = (unsigned)(stream_runs(p.rows, p.groups) * ((p.n + 128 / T::ES - 1) / (128 / T::ES)) * p.parts);
   return launch_kernel((const void*)&grouped_stream_rows_kernel<T>, grid, STREAM_ROWS_WAVES * 64, 0, stream, &q);
 }
 

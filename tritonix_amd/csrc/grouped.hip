@@ -179,11 +179,12 @@ template <class O> __global__ __launch_bounds__(256) void join_kernel(const floa
   }
 }
 
-// Few rows by k-contiguous weights of 16 bits, which gemm_stream.h reads once a group for up to 8 rows: 8 rows in all, or 4 to a group on average (us,
+// Few rows by k-contiguous weights, which gemm_stream.h reads once a group for up to 8 rows: 8 rows in all, or 4 to a group on average (us,
 // against the tile kernels': 32 rows, 8 groups, 14336 x 4096 144 and 164, 64 rows 212 and 164; 128 rows, 32 groups, 4096 x 4096 153 and 173), but not many workgroups of a short k (256 rows, 64 groups, 1024 x 4096
-// 88 and 82; 4 rows 8.2 and 8.5, 64 rows, 16 groups, 700 x 1000 7.4 and 8.8).
+// 88 and 82; 4 rows 8.2 and 8.5, 64 rows, 16 groups, 700 x 1000 7.4 and 8.8).  float32 gains more: 8 rows, 128 groups, 2048 x 768 12.5 and 18.6, 128 rows,
+// 32 groups, 4096 x 4096 318 and 339.
 bool takes_stream(const tnx_grouped_args* a) {
-  if (gradient(a) || a->dtype == TNX_F32 || a->block_m > 0 || a->k == 0 || a->stride_ak != 1 || a->stride_ar < a->k) return false;
+  if (gradient(a) || a->block_m > 0 || a->k == 0 || a->stride_ak != 1 || a->stride_ar < a->k) return false;
   if (a->stride_bn == 1 || a->stride_bk != 1 || a->stride_bn < a->k) return false;
   if (a->k < 2048 && (a->rows < a->groups ? a->rows : a->groups) * a->n > 16384) return false;
   // (a grid's threads are counted in 32 bits)
@@ -192,9 +193,10 @@ bool takes_stream(const tnx_grouped_args* a) {
 
 // Up to 8 rows by row-major weights, while blocks of 64 columns times groups leave half of the CUs without a workgroup and k has parts for them: those
 // parts, a workgroup to a CU, or 0: not taken (us, against the tile kernels': 1 row, 64 groups, 4096 x 2048 9.5 and 15.7, 4 rows 17.4 and 21.2, 2 rows, 128
-// groups, 2048 x 768 7.4 and 14.2; a workgroup to every block without parts, 8 rows, 64 groups, 4096 x 2048: 26.4 and 24.9).
+// groups, 2048 x 768 7.4 and 14.2; a workgroup to every block without parts, 8 rows, 64 groups, 4096 x 2048: 26.4 and 24.9).  float32 has blocks of 32 columns
+// and as many parts for each, two workgroups to a CU: 4 rows, 64 groups, 4096 x 2048 27.4 and 32.2, 2 rows, 128 groups, 2048 x 768 9.3 and 15.9.
 int stream_rows_parts(const tnx_grouped_args* a) {
-  if (gradient(a) || a->dtype == TNX_F32 || a->block_m > 0 || a->stride_ak != 1 || a->stride_ar < a->k) return 0;
+  if (gradient(a) || a->block_m > 0 || a->stride_ak != 1 || a->stride_ar < a->k) return 0;
   if (a->stride_bn != 1 || a->stride_bk < a->n || a->n < 8 || a->rows > 8) return 0;
   const int64_t blocks = (a->rows < a->groups ? a->rows : a->groups) * ((a->n + 63) / 64), most = a->k / (64 * STREAM_ROWS_WAVES);
   int64_t parts = blocks > 0 ? 256 / blocks : 0;
@@ -236,7 +238,8 @@ extern "C" int tnx_grouped(const tnx_grouped_args* a) {
     p.group_stride = a->stride_group;
     p.rows = (int32_t)a->rows; p.n = (int32_t)a->n; p.k = (int32_t)a->k;
     p.groups = a->groups;
-    const hipError_t err = a->dtype == TNX_BF16 ? grouped_stream<TagBF16>(p, (hipStream_t)a->stream) : grouped_stream<TagF16>(p, (hipStream_t)a->stream);
+    const hipStream_t s = (hipStream_t)a->stream;
+    const hipError_t err = a->dtype == TNX_F32 ? grouped_stream<TagF32>(p, s) : a->dtype == TNX_BF16 ? grouped_stream<TagBF16>(p, s) : grouped_stream<TagF16>(p, s);
     if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
     return TNX_OK;
   }
@@ -251,7 +254,8 @@ extern "C" int tnx_grouped(const tnx_grouped_args* a) {
     p.rows = (int32_t)a->rows; p.n = (int32_t)a->n; p.k = (int32_t)a->k;
     p.groups = a->groups;
     p.parts = parts; p.part_stride = sums;
-    hipError_t err = a->dtype == TNX_BF16 ? grouped_stream_rows<TagBF16>(p, (hipStream_t)a->stream) : grouped_stream_rows<TagF16>(p, (hipStream_t)a->stream);
+    const hipStream_t s = (hipStream_t)a->stream;
+    hipError_t err = a->dtype == TNX_F32 ? grouped_stream_rows<TagF32>(p, s) : a->dtype == TNX_BF16 ? grouped_stream_rows<TagBF16>(p, s) : grouped_stream_rows<TagF16>(p, s);
     if (err == hipSuccess) err = join(a, parts, sums);
     if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
     return TNX_OK;

@@ -141,20 +141,25 @@ struct Plan {
 
 bool with_epilogue(const tnx_linear_args* a) { return a->bias || a->residual || a->z || a->activation != TNX_ACT_NONE; }
 
-// Few rows of 16-bit numbers, k-contiguous on both sides: gemm_stream.h.  Up to 4 rows of any size; more rows take as long to fetch as the weight,
-// workgroup for workgroup, which a tile kernel fetches for many columns at once: 5 to 8 rows up to k = 8192 (us, against the tile kernels': 8 x 512 x 8192 9.6 and 10.5,
-// 8 x 4096 x 14336 26.3 and 25.1), 9 to 16 where n and k are small (16 x 2050 x 4100 8.1 and 13.6, 16 x 4096 x 4096 10.9 and 12.5; 16 x 512 x 8192
-// 16.4 and 10.6, 16 x 30000 x 512 10.8 and 9.2).
+// Few rows, k-contiguous on both sides: gemm_stream.h.  Up to 4 rows of any size; more rows take as long to fetch as the weight, workgroup for
+// workgroup, which a tile kernel fetches once for many columns: 5 to 8 rows up to k = 8192 (us, against the tile kernels': 8 x 512 x 8192 9.6 and
+// 10.5, 8 x 4096 x 14336 26.3 and 25.1), 9 to 16 where n and k are small (16 x 2050 x 4100 8.1 and 13.6, 16 x 4096 x 4096 10.9 and 12.5; 16 x 512 x
+// 8192 16.4 and 10.6, 16 x 30000 x 512 10.8 and 9.2).  float32: 1 x 14336 x 4096 41 and 123 (whose operands are cut into terms first), 4 x 512 x 8192 10.0 and
+// 12.9, 8 x 4096 x 4096 14.9 and 20.3, 8 x 512 x 8192 16.7 and 13.0, 16 x 4096 x 4096 21.2 and 20.7.
 bool takes_stream(const tnx_linear_args* a) {
-  if (a->dtype == TNX_F32 || a->stride_xk != 1 || a->stride_wk != 1 || a->m > 16 || a->n > 0x1000000 || a->k > 0x40000000) return false;
-  return a->m <= 4 || (a->m <= 8 && a->k <= 8192) || (a->n <= 4608 && a->k <= 4608);
+  if (a->stride_xk != 1 || a->stride_wk != 1 || a->m > 16 || a->n > 0x1000000 || a->k > 0x40000000) return false;
+  if (a->m <= 4) return true;
+  if (a->dtype == TNX_F32) return a->m <= 8 && a->k <= 4096 && a->n <= 16384;
+  return (a->m <= 8 && a->k <= 8192) || (a->n <= 4608 && a->k <= 4608);
 }
 
 // The same by a row-major weight, while the tile kernels' columns are fewer than the CUs (beyond, 1 x 16384 x 16384: 91 us and 88): up to 4 rows, and
-// to 8 of a long k (8 x 512 x 8192 9.4 and 11.1, 8 x 1024 x 1024 8.5 and 8.2).
+// to 8 of a long k (8 x 512 x 8192 9.4 and 11.1, 8 x 1024 x 1024 8.5 and 8.2).  float32: up to 4 rows of a k that few parts do (1 x 14336 x 4096 48 and 117,
+// 1 x 4096 x 4096 18.9 and 20.6, 1 x 512 x 8192 14.4 and 13.3).
 bool takes_stream_rows(const tnx_linear_args* a) {
-  if (a->dtype == TNX_F32 || a->stride_xk != 1 || a->stride_wn != 1 || a->n < 8 || a->n >= 16384 || a->k > 0x40000000) return false;
-  return a->m <= 4 || (a->m <= 8 && a->k >= 2048);
+  if (a->stride_xk != 1 || a->stride_wn != 1 || a->n < 8 || a->k > 0x40000000) return false;
+  if (a->dtype == TNX_F32) return a->m <= 4 && a->k <= 4096 && a->n <= 0x1000000;
+  return a->n < 16384 && (a->m <= 4 || (a->m <= 8 && a->k >= 2048));
 }
 
 Plan make_plan(const tnx_linear_args* a) {
@@ -177,7 +182,7 @@ Plan make_plan(const tnx_linear_args* a) {
   }
   if (takes_stream_rows(a)) {
     p.route = ROUTE_STREAM_ROWS;
-    p.workspace = stream_rows_workspace(a->m, a->n, a->k);
+    p.workspace = stream_rows_workspace(a->m, a->n, a->k, a->dtype == TNX_F32 ? 4 : 2);
     return p;
   }
   p.route = with_epilogue(a) ? ROUTE_FUSED : ROUTE_PRODUCT;
@@ -271,7 +276,8 @@ extern "C" int tnx_linear(const tnx_linear_args* a) {
   if (p.route == ROUTE_STREAM) {
     const StreamParams q = {(const uint8_t*)a->x, (const uint8_t*)a->w, (uint8_t*)a->y, (uint8_t*)a->z, (const uint8_t*)a->bias, (const uint8_t*)a->residual,
                             a->stride_xm, a->stride_wn, (int32_t)a->m, (int32_t)a->n, (int32_t)a->k, a->activation, a->bias_dtype};
-    const hipError_t err = a->dtype == TNX_BF16 ? stream_columns<TagBF16>(q, (hipStream_t)a->stream) : stream_columns<TagF16>(q, (hipStream_t)a->stream);
+    const hipStream_t s = (hipStream_t)a->stream;
+    const hipError_t err = a->dtype == TNX_BF16 ? stream_columns<TagBF16>(q, s) : a->dtype == TNX_F16 ? stream_columns<TagF16>(q, s) : stream_columns<TagF32>(q, s);
     if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
     return TNX_OK;
   }
@@ -279,8 +285,9 @@ extern "C" int tnx_linear(const tnx_linear_args* a) {
     if (p.workspace > 0 && (!a->workspace || a->workspace_bytes < p.workspace || ((uintptr_t)a->workspace & 15))) return TNX_E_WORKSPACE;
     const StreamRowsParams q = {(const uint8_t*)a->x, (const uint8_t*)a->w, (uint8_t*)a->y, (uint8_t*)a->z, (const uint8_t*)a->bias, (const uint8_t*)a->residual,
                                 p.workspace > 0 ? (uint8_t*)a->workspace : nullptr, a->stride_xm, a->stride_wk, (int32_t)a->m, (int32_t)a->n, (int32_t)a->k,
-                                stream_rows_parts(a->n, a->k), a->activation | a->bias_dtype << 8};
-    const hipError_t err = a->dtype == TNX_BF16 ? stream_rows<TagBF16>(q, (hipStream_t)a->stream) : stream_rows<TagF16>(q, (hipStream_t)a->stream);
+                                stream_rows_parts(a->n, a->k, a->dtype == TNX_F32 ? 4 : 2), a->activation | a->bias_dtype << 8};
+    const hipStream_t s = (hipStream_t)a->stream;
+    const hipError_t err = a->dtype == TNX_BF16 ? stream_rows<TagBF16>(q, s) : a->dtype == TNX_F16 ? stream_rows<TagF16>(q, s) : stream_rows<TagF32>(q, s);
     if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
     return TNX_OK;
   }
