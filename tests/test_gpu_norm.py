@@ -23,7 +23,7 @@ def compare(got, want, types):
 
 
 # (the last sizes of each kernel's range and the first of the next, both in 16 and in 32 bits)
-WIDTHS = [1, 2, 7, 8, 9, 64, 255, 256, 257, 500, 512, 513, 1023, 1024, 1025, 1501, 2048, 2056, 4095, 4096, 4104, 8192, 8200, 16384, 16385, 32768, 32769, 40000]
+WIDTHS = [1, 2, 7, 8, 9, 31, 32, 33, 63, 64, 65, 127, 128, 129, 130, 255, 256, 257, 500, 512, 513, 1023, 1024, 1025, 1501, 2048, 2056, 4095, 4096, 4104, 8192, 8200, 16384, 16385, 32768, 32769, 40000]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -39,7 +39,7 @@ def test_values_and_gradients(device, dtype, n):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,n", [(1, 1024), (3, 40), (600, 96), (2050, 130), (5000, 8), (1500, 2050), (700, 16400)])
+@pytest.mark.parametrize("rows,n", [(1, 1024), (3, 40), (600, 96), (2050, 130), (5000, 8), (4099, 61), (3001, 100), (2500, 250), (1500, 2050), (700, 16400)])
 def test_many_rows(device, dtype, rows, n):
     x, weight, bias, dy = (ref.draw(device, *s, dtype=dtype, seed=i) for i, s in enumerate(((rows, n), (n,), (n,), (rows, n))))
     types = {name: dtype for name in ("y", "dx", "dweight", "dbias")}

@@ -25,6 +25,7 @@ struct NormParams {
   int64_t rows, n, stride_x, stride_dy;
   int weight_dtype, bias_dtype;
   float eps;
+  int block;                     // rows of a workgroup that sums columns alone
 };
 
 
@@ -50,12 +51,12 @@ template <int L> __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// Sums over the TPR threads of a row of NS values; every thread gets them.  TPR is a wave or the whole workgroup.  `slot` alternates from call
+// Sums over the TPR threads of a row of NS values; every thread gets them.  TPR is a part of a wave, a wave or the whole workgroup.  `slot` alternates from call
 // to call, so that one barrier does.  The waves' sums are read a lane each and added up over lanes: read by every thread in turn they took 64
 // registers of 16 waves' four sums (16384 x 8192 bf16 backward: 1142 us, now 182).
 template <int TPR, int NS> __device__ __forceinline__ void row_sums(float (&v)[NS], float* lds, int slot) {
 #pragma unroll
-  for (int s = 0; s < NS; ++s) v[s] = lanes_sum<64>(v[s]);
+  for (int s = 0; s < NS; ++s) v[s] = lanes_sum<(TPR < 64 ? TPR : 64)>(v[s]);
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
     float* at = lds + slot * W * NS;
@@ -69,28 +70,41 @@ template <int TPR, int NS> __device__ __forceinline__ void row_sums(float (&v)[N
   }
 }
 
-// Runs of V columns, `cols` of which exist.  WHOLE: all or none, since n is a multiple of V.
-template <class O, int V, bool WHOLE = false> __device__ __forceinline__ void load_run(const typename O::raw* src, int cols, float (&f)[V]) {
+// V columns as they lie in memory, `cols` of which exist; past the row's end zeros.  WHOLE: all or none, since n is a multiple of V.  A run that is cut off
+// is the end of the 16 bytes that end with the row, shifted down (9613 x 4082 f16 forward 33.7 us by elements, 28.9 so; the backward pass of float32 and of
+// 1024 threads has no registers for it: 9613 x 6002 bf16 110 us by elements, 128 so); where it is the row's first (`first`: the row is shorter than a run) it
+// is loaded by elements.
+template <class O, bool WHOLE, bool SHIFT = true> __device__ __forceinline__ i32x4 load_packed(const typename O::raw* src, int cols, bool first) {
   typedef typename O::raw raw;
-  raw e[V];
-  if (WHOLE) {
-    const i32x4 v = cols ? *(const i32x4_loose*)src : i32x4{0, 0, 0, 0};
-    __builtin_memcpy(e, &v, 16);
-#pragma unroll
-    for (int x = 0; x < V; ++x) f[x] = Run<O, V>::widen(e[x]);
-    return;
-  }
-  if (cols == V) {
-    const i32x4 v = *(const i32x4_loose*)src;
-    __builtin_memcpy(e, &v, 16);
-  } else {
+  constexpr int V = 16 / sizeof(raw);
+  if (WHOLE) return cols ? *(const i32x4_loose*)src : i32x4{0, 0, 0, 0};
+  i32x4 v = {0, 0, 0, 0};
+  auto elements = [&]() __attribute__((always_inline)) {
+    raw e[V];
 #pragma unroll
     for (int x = 0; x < V; ++x) e[x] = x < cols ? src[x] : (raw)0;
+    __builtin_memcpy(&v, e, 16);
+    return v;
+  };
+  if (!SHIFT) return cols == V ? (i32x4)*(const i32x4_loose*)src : elements();
+  if (cols == V || (cols > 0 && !first)) {
+    v = *(const i32x4_loose*)(src + cols - V);
+    if (cols < V) v = __builtin_bit_cast(i32x4, __builtin_bit_cast(unsigned __int128, v) >> ((V - cols) * 8 * (int)sizeof(raw)));
+  } else if (cols > 0) {
+    elements();
   }
-#pragma unroll
-  for (int x = 0; x < V; ++x) f[x] = x < cols ? Run<O, V>::widen(e[x]) : 0.0f;
+  return v;
 }
-template <class O, int V, bool WHOLE = false> __device__ __forceinline__ void store_run(typename O::raw* dst, int cols, const float (&f)[V]) {
+template <class O, int V> __device__ __forceinline__ void unpack(i32x4 v, float (&f)[V]) {
+  typename O::raw e[V];
+  __builtin_memcpy(e, &v, 16);
+#pragma unroll
+  for (int x = 0; x < V; ++x) f[x] = Run<O, V>::widen(e[x]);
+}
+template <class O, int V, bool WHOLE = false, bool SHIFT = true> __device__ __forceinline__ void load_run(const typename O::raw* src, int cols, bool first, float (&f)[V]) {
+  unpack<O, V>(load_packed<O, WHOLE, SHIFT>(src, cols, first), f);
+}
+template <class O, int V, bool WHOLE = false, bool SHIFT = true> __device__ __forceinline__ void store_run(typename O::raw* dst, int cols, const float (&f)[V]) {
   typedef typename O::raw raw;
   raw e[V];
 #pragma unroll
@@ -100,26 +114,44 @@ template <class O, int V, bool WHOLE = false> __device__ __forceinline__ void st
     i32x4 v;
     __builtin_memcpy(&v, e, 16);
     *(i32x4_loose*)dst = v;
-  } else {
+  } else if (!SHIFT) {
 #pragma unroll
     for (int x = 0; x < V; ++x)
       if (x < cols) dst[x] = e[x];
+  } else {
+    // in pieces of half a run, a quarter and, of 16 bits, an eighth
+    struct __attribute__((packed, aligned(2))) Eight { uint64_t v; };
+    struct __attribute__((packed, aligned(2))) Four { uint32_t v; };
+    uint64_t half[2];
+    __builtin_memcpy(half, e, 16);
+    uint64_t left = half[0];
+    if (cols & V / 2) {
+      ((Eight*)dst)->v = left;
+      left = half[1];
+      dst += V / 2;
+    }
+    if (cols & V / 4) {
+      ((Four*)dst)->v = (uint32_t)left;
+      left >>= 32;
+      dst += V / 4;
+    }
+    if (V == 8 && cols & 1) *(uint16_t*)dst = (uint16_t)left;
   }
 }
 
 // V columns of weight or bias, of the rows' type or float32; null: `none` throughout
-template <class O, int V, bool WHOLE = false> __device__ __forceinline__ void load_param(const uint8_t* p, int dtype, int64_t col, int cols, float none, float (&f)[V]) {
+template <class O, int V, bool WHOLE = false, bool SHIFT = true> __device__ __forceinline__ void load_param(const uint8_t* p, int dtype, int64_t col, int cols, float none, float (&f)[V]) {
   if (!p) {
 #pragma unroll
     for (int x = 0; x < V; ++x) f[x] = none;
   } else if (dtype != DT_F32) {
-    load_run<O, V, WHOLE>((const typename O::raw*)p + col, cols, f);
+    load_run<O, V, WHOLE, SHIFT>((const typename O::raw*)p + col, cols, col == 0, f);
   } else {
     const float* src = (const float*)p + col;
 #pragma unroll
     for (int h = 0; h < V / 4; ++h) {
       float q[4];
-      load_run<OutF32, 4, WHOLE>(src + 4 * h, cols - 4 * h >= 4 ? 4 : cols - 4 * h > 0 ? cols - 4 * h : 0, q);
+      load_run<OutF32, 4, WHOLE, SHIFT>(src + 4 * h, cols - 4 * h >= 4 ? 4 : cols - 4 * h > 0 ? cols - 4 * h : 0, col + h == 0, q);
 #pragma unroll
       for (int x = 0; x < 4; ++x) f[4 * h + x] = q[x];
     }
@@ -140,7 +172,7 @@ template <class O, int TPR, int CH, bool WHOLE> __global__ __launch_bounds__(TPR
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int64_t col = (int64_t)(c * TPR + t) * V, left = p.n - col;
-    load_run<O, V, WHOLE>(src + (left > 0 ? col : 0), left >= V ? V : left > 0 ? (int)left : 0, f[c]);
+    load_run<O, V, WHOLE>(src + (left > 0 ? col : 0), left >= V ? V : left > 0 ? (int)left : 0, col == 0, f[c]);
 #pragma unroll
     for (int e = 0; e < V; ++e) s[0] += f[c][e];
   }
@@ -175,26 +207,6 @@ template <class O, int TPR, int CH, bool WHOLE> __global__ __launch_bounds__(TPR
   }
 }
 
-// V columns as they lie in memory; past the row's end zeros
-template <class O, bool WHOLE> __device__ __forceinline__ i32x4 load_packed(const typename O::raw* src, int cols) {
-  typedef typename O::raw raw;
-  constexpr int V = 16 / sizeof(raw);
-  if (WHOLE) return cols ? *(const i32x4_loose*)src : i32x4{0, 0, 0, 0};
-  if (cols == V) return *(const i32x4_loose*)src;
-  raw e[V];
-#pragma unroll
-  for (int x = 0; x < V; ++x) e[x] = x < cols ? src[x] : (raw)0;
-  i32x4 v;
-  __builtin_memcpy(&v, e, 16);
-  return v;
-}
-template <class O, int V> __device__ __forceinline__ void unpack(i32x4 v, float (&f)[V]) {
-  typename O::raw e[V];
-  __builtin_memcpy(e, &v, 16);
-#pragma unroll
-  for (int x = 0; x < V; ++x) f[x] = Run<O, V>::widen(e[x]);
-}
-
 // A workgroup walks over rows, R of them at a step (one barrier for their sums; two where a workgroup is alone on its CU or the
 // values are few: 16384 x 8192 bf16 214 us with one, 182 with two, float32 65536 x 1024 172 and 154; elsewhere two spill); x and dy of these and of the next R are in registers as they
 // lie in memory (widened twice: for the sums, then for dx), which leaves room for two sums per column and lets the loads run ahead of the
@@ -202,7 +214,7 @@ template <class O, int V> __device__ __forceinline__ void unpack(i32x4 v, float 
 template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_bounds__(TPR < 128 ? 256 : TPR, 4) void norm_backward_kernel(NormParams p) {
   typedef typename O::raw raw;
   constexpr int V = 16 / sizeof(raw), THREADS = TPR < 128 ? 256 : TPR, LINES = THREADS / TPR, R = CH == 1 && (V == 4 || TPR == 1024) ? 2 : 1;
-  constexpr bool AHEAD = CH <= 2;
+  constexpr bool AHEAD = CH <= 2, SHIFT = V == 8 && TPR < 1024;
   __shared__ float lds[2 * 2 * R * THREADS / 64];
   const int t = threadIdx.x % TPR, line = threadIdx.x / TPR;
   float dw[PARTS ? CH : 1][V], db[PARTS ? CH : 1][V];
@@ -227,8 +239,8 @@ template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_
       for (int c = 0; c < CH; ++c) {
         const int64_t at = cols[c] ? (int64_t)(c * TPR + t) * V : 0;
         const int count = there ? cols[c] : 0;
-        fx[r][c] = load_packed<O, WHOLE>((const raw*)p.x + (there ? row : 0) * p.stride_x + at, count);
-        fg[r][c] = load_packed<O, WHOLE>((const raw*)p.dy + (there ? row : 0) * p.stride_dy + at, count);
+        fx[r][c] = load_packed<O, WHOLE, SHIFT>((const raw*)p.x + (there ? row : 0) * p.stride_x + at, count, at == 0);
+        fg[r][c] = load_packed<O, WHOLE, SHIFT>((const raw*)p.dy + (there ? row : 0) * p.stride_dy + at, count, at == 0);
       }
       fmean[r] = there ? p.mean[row] : 0.0f;
       frstd[r] = there ? p.rstd[row] : 0.0f;
@@ -249,7 +261,7 @@ template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       float w[V];
-      load_param<O, V, WHOLE>(p.weight, p.weight_dtype, cols[c] ? (int64_t)(c * TPR + t) * V : 0, cols[c], 1.0f, w);
+      load_param<O, V, WHOLE, SHIFT>(p.weight, p.weight_dtype, cols[c] ? (int64_t)(c * TPR + t) * V : 0, cols[c], 1.0f, w);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float u[V], d[V];
@@ -274,7 +286,7 @@ template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         float w[V];
-        load_param<O, V, WHOLE>(p.weight, p.weight_dtype, cols[c] ? (int64_t)(c * TPR + t) * V : 0, cols[c], 1.0f, w);
+        load_param<O, V, WHOLE, SHIFT>(p.weight, p.weight_dtype, cols[c] ? (int64_t)(c * TPR + t) * V : 0, cols[c], 1.0f, w);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           float u[V], d[V];
@@ -285,7 +297,7 @@ template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_
 #pragma unroll
           for (int e = 0; e < V; ++e) d[e] = rstd[r] * (d[e] * w[e] - a - (u[e] - mean[r]) * rstd[r] * b);
           if (cols[c] && (R == 1 || row + r * step < p.rows))
-            store_run<O, V, WHOLE>((raw*)p.dx + (row + r * step) * p.n + (int64_t)(c * TPR + t) * V, cols[c], d);
+            store_run<O, V, WHOLE, SHIFT>((raw*)p.dx + (row + r * step) * p.n + (int64_t)(c * TPR + t) * V, cols[c], d);
         }
       }
     }
@@ -332,10 +344,10 @@ template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_
           float q[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) q[e] = dw[c][4 * h + e];
-          store_run<OutF32, 4, WHOLE>(out + col + 4 * h, left >= 4 ? 4 : left > 0 ? left : 0, q);
+          store_run<OutF32, 4, WHOLE, SHIFT>(out + col + 4 * h, left >= 4 ? 4 : left > 0 ? left : 0, q);
 #pragma unroll
           for (int e = 0; e < 4; ++e) q[e] = db[c][4 * h + e];
-          store_run<OutF32, 4, WHOLE>(out + p.n + col + 4 * h, left >= 4 ? 4 : left > 0 ? left : 0, q);
+          store_run<OutF32, 4, WHOLE, SHIFT>(out + p.n + col + 4 * h, left >= 4 ? 4 : left > 0 ? left : 0, q);
         }
       }
     }
@@ -355,13 +367,13 @@ template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_l
   if constexpr (!BACKWARD) {
     float s[1] = {0.0f}, q[1] = {0.0f}, f[V];
     over([&](int64_t col, int cols) __attribute__((always_inline)) {
-      load_run<O, V>(src + col, cols, f);
+      load_run<O, V>(src + col, cols, col == 0, f);
       for (int e = 0; e < V; ++e) s[0] += f[e];
     });
     row_sums<TPR, 1>(s, lds, 0);
     const float mean = s[0] / (float)p.n;
     over([&](int64_t col, int cols) __attribute__((always_inline)) {
-      load_run<O, V>(src + col, cols, f);
+      load_run<O, V>(src + col, cols, col == 0, f);
       for (int e = 0; e < V; ++e) q[0] += e < cols ? (f[e] - mean) * (f[e] - mean) : 0.0f;
     });
     row_sums<TPR, 1>(q, lds, 1);
@@ -371,7 +383,7 @@ template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_l
       p.rstd[row] = rstd;
     }
     over([&](int64_t col, int cols) __attribute__((always_inline)) {
-      load_run<O, V>(src + col, cols, f);
+      load_run<O, V>(src + col, cols, col == 0, f);
       float w[V], b[V];
       load_param<O, V>(p.weight, p.weight_dtype, col, cols, 1.0f, w);
       load_param<O, V>(p.bias, p.bias_dtype, col, cols, 0.0f, b);
@@ -383,8 +395,8 @@ template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_l
     const raw* dy = (const raw*)p.dy + row * p.stride_dy;
     float s[2] = {0.0f, 0.0f}, u[V], g[V];
     auto both = [&](int64_t col, int cols) __attribute__((always_inline)) {
-      load_run<O, V>(src + col, cols, u);
-      load_run<O, V>(dy + col, cols, g);
+      load_run<O, V>(src + col, cols, col == 0, u);
+      load_run<O, V>(dy + col, cols, col == 0, g);
       float w[V];
       load_param<O, V>(p.weight, p.weight_dtype, col, cols, 1.0f, w);
       for (int e = 0; e < V; ++e) {
@@ -410,26 +422,38 @@ template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_l
 }
 
 // dweight and dbias of such rows, and of those too long for a thread to keep its columns' sums too (sums_apart): a workgroup's 32 runs of columns down 256 rows, its 8 rows of threads meet in LDS
-constexpr int LONG_ROWS = 256;
 template <class O> __global__ __launch_bounds__(256) void norm_columns_kernel(NormParams p) {
   typedef typename O::raw raw;
   constexpr int V = 16 / sizeof(raw);
   __shared__ float sums[2][8][32 * V + 4];
   const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
-  const int64_t col = ((int64_t)blockIdx.x * 32 + lane) * V, row0 = (int64_t)blockIdx.y * LONG_ROWS;
+  const int64_t col = ((int64_t)blockIdx.x * 32 + lane) * V, row0 = (int64_t)blockIdx.y * p.block, end = row0 + p.block < p.rows ? row0 + p.block : p.rows;
   const int cols = p.n - col >= V ? V : p.n > col ? (int)(p.n - col) : 0;
   float dw[V] = {}, db[V] = {};
-  for (int r = line; r < LONG_ROWS; r += 8) {
-    const int64_t row = row0 + r;
-    if (row >= p.rows || cols == 0) break;
-    const float mean = p.mean[row], rstd = p.rstd[row];
-    float u[V], g[V];
-    load_run<O, V>((const raw*)p.x + row * p.stride_x + col, cols, u);
-    load_run<O, V>((const raw*)p.dy + row * p.stride_dy + col, cols, g);
+  constexpr int AHEAD = 4;                                // rows of a thread whose loads are on their way together
+  for (int64_t row = row0 + line; row < end && cols > 0; row += 8 * AHEAD) {
+    i32x4 x[AHEAD], d[AHEAD];
+    float mean[AHEAD], rstd[AHEAD];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      dw[e] += e < cols ? g[e] * (u[e] - mean) * rstd : 0.0f;
-      db[e] += g[e];
+    for (int r = 0; r < AHEAD; ++r) {
+      const bool there = row + 8 * r < end;
+      const int64_t at = there ? row + 8 * r : row;
+      x[r] = load_packed<O, false>((const raw*)p.x + at * p.stride_x + col, cols, col == 0);
+      d[r] = load_packed<O, false>((const raw*)p.dy + at * p.stride_dy + col, there ? cols : 0, col == 0);
+      mean[r] = p.mean[at];
+      rstd[r] = there ? p.rstd[at] : 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < AHEAD; ++r) {
+      float u[V], g[V];
+      unpack<O, V>(x[r], u);
+      unpack<O, V>(d[r], g);
+      if (row + 8 * r >= end) break;                      // (a row that is not there has no part, not even of a NaN)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        dw[e] += e < cols ? g[e] * (u[e] - mean[r]) * rstd[r] : 0.0f;
+        db[e] += g[e];
+      }
     }
   }
 #pragma unroll
@@ -450,27 +474,29 @@ template <class O> __global__ __launch_bounds__(256) void norm_columns_kernel(No
 }
 
 // out[c] = the sum of parts[i][c] in the order of i: the first n columns are dweight, the others dbias
-__global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, int64_t count, int64_t n, uint8_t* dweight, int weight_dtype, uint8_t* dbias,
+template <int ACROSS> __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, int64_t count, int64_t n, uint8_t* dweight, int weight_dtype, uint8_t* dbias,
                                                           int bias_dtype) {
-  __shared__ float sums[16][64];
-  const int lane = threadIdx.x & 63, line = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+  constexpr int LINES = 1024 / ACROSS;
+  __shared__ float sums[LINES][ACROSS];
+  const int lane = threadIdx.x % ACROSS, line = threadIdx.x / ACROSS;
+  const int64_t col = (int64_t)blockIdx.x * ACROSS + lane;
   float s = 0.0f;
   if (col < 2 * n) {
 #pragma unroll 8
-    for (int64_t i = line; i < count; i += 16) s += parts[i * 2 * n + col];
+    for (int64_t i = line; i < count; i += LINES) s += parts[i * 2 * n + col];
   }
   sums[line][lane] = s;
   __syncthreads();
   if (line == 0 && col < 2 * n) {
 #pragma unroll
-    for (int l = 1; l < 16; ++l) s += sums[l][lane];
+    for (int l = 1; l < LINES; ++l) s += sums[l][lane];
     if (col < n && dweight) store_out<float>(dweight, col, s, weight_dtype);
     if (col >= n && dbias) store_out<float>(dbias, col - n, s, bias_dtype);
   }
 }
 
-// Threads and runs of a row; 0: longer than the registers hold.
+// Threads and runs of a row; 0: longer than the registers hold.  Several short rows share a wave (45231 x 67 f16: a wave to a row 24 us forward, 42
+// backward, 16 lanes 9 and 23; 65536 x 128 bf16 22, 32 and 9, 23).
 struct Shape {
   int tpr, ch;
 };
@@ -479,15 +505,15 @@ Shape shape_of(const Shape* shapes, int count, int64_t n, int v) {
     if (n <= (int64_t)shapes[i].tpr * shapes[i].ch * v) return shapes[i];
   return {0, 0};
 }
-const Shape FORWARD[] = {{64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}};
-const Shape BACKWARD[] = {{64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
-#define TNX_NORM_FORWARD_SHAPES(DO) DO(64, 1) DO(64, 2) DO(64, 4) DO(256, 2) DO(256, 4) DO(512, 4) DO(1024, 4)
-#define TNX_NORM_BACKWARD_SHAPES(DO) DO(64, 1) DO(128, 1) DO(256, 1) DO(512, 1) DO(1024, 1) DO(1024, 2) DO(1024, 4)
+const Shape FORWARD[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}};
+const Shape BACKWARD[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {128, 1}, {256, 1}, {512, 1}, {1024, 1}, {1024, 2}, {1024, 4}};
+#define TNX_NORM_FORWARD_SHAPES(DO) DO(8, 1) DO(16, 1) DO(32, 1) DO(64, 1) DO(64, 2) DO(64, 4) DO(256, 2) DO(256, 4) DO(512, 4) DO(1024, 4)
+#define TNX_NORM_BACKWARD_SHAPES(DO) DO(8, 1) DO(16, 1) DO(32, 1) DO(64, 1) DO(128, 1) DO(256, 1) DO(512, 1) DO(1024, 1) DO(1024, 2) DO(1024, 4)
 Shape forward_shape(int64_t n, int v) { return shape_of(FORWARD, sizeof FORWARD / sizeof *FORWARD, n, v); }
 Shape backward_shape(int64_t n, int v) { return shape_of(BACKWARD, sizeof BACKWARD / sizeof *BACKWARD, n, v); }
 // rows that a workgroup has at a time
-int64_t lines_of(const Shape& s) { return s.tpr < 256 ? 256 / s.tpr : 1; }
-int64_t backward_lines(const Shape& s) { return s.tpr < 128 ? 256 / s.tpr : 1; }
+int64_t lines_of(const Shape& s) { return s.tpr > 0 && s.tpr < 256 ? 256 / s.tpr : 1; }
+int64_t backward_lines(const Shape& s) { return s.tpr > 0 && s.tpr < 128 ? 256 / s.tpr : 1; }
 // more columns' sums than that a thread's registers do not hold: they are a launch of their own
 bool sums_apart(const Shape& s, int v) { return s.tpr == 0 || s.ch * v > 8; }
 // Workgroups of the backward pass.  Each costs a share of 8 n bytes, written and read, where a row of 16 bits costs 6 n: so 16 rows or
@@ -498,9 +524,16 @@ int64_t groups_of(const tnx_norm_args* a, const Shape& s) {
   groups = groups < 256 ? 256 : groups > together ? together : groups;
   return groups < most ? groups : most;
 }
+// Rows of a workgroup of the launch of their own: 256, fewer while CUs are left without one (874 x 11520 bf16: 256 rows, loaded one after another, 20.0 us, 64 rows by fours 8.6).
+int columns_rows(const tnx_norm_args* a) {
+  const int64_t span = a->dtype == TNX_F32 ? 128 : 256, across = (a->n + span - 1) / span;
+  int rows = 256;
+  while (rows > 32 && (a->rows + rows - 1) / rows * across < 512) rows /= 2;
+  return rows;
+}
 int64_t shares_of(const tnx_norm_args* a) {
   const Shape s = backward_shape(a->n, a->dtype == TNX_F32 ? 4 : 8);
-  return sums_apart(s, a->dtype == TNX_F32 ? 4 : 8) ? (a->rows + LONG_ROWS - 1) / LONG_ROWS : groups_of(a, s);
+  return sums_apart(s, a->dtype == TNX_F32 ? 4 : 8) ? (a->rows + columns_rows(a) - 1) / columns_rows(a) : groups_of(a, s);
 }
 
 int check(const tnx_norm_args* a) {
@@ -520,6 +553,7 @@ NormParams params_of(const tnx_norm_args* a) {
   p.rows = a->rows; p.n = a->n; p.stride_x = a->stride_x; p.stride_dy = a->stride_dy;
   p.weight_dtype = a->weight_dtype; p.bias_dtype = a->bias_dtype;
   p.eps = a->eps;
+  p.block = columns_rows(a);
   return p;
 }
 int launched() {
@@ -542,6 +576,14 @@ template <class O> int forward_rows(const NormParams& p, hipStream_t stream) {
   TNX_NORM_FORWARD_SHAPES(TNX_NORM_FORWARD)
   hipLaunchKernelGGL((norm_long_kernel<O, false>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
   return launched();
+}
+
+// 16 columns to a workgroup while 64 leave CUs without one (25953 x 978 bf16, 1024 shares: 64 columns 8.5 us, 16 columns 5.5)
+void launch_parts(const NormParams& p, int64_t shares, const tnx_norm_args* a, hipStream_t stream) {
+  const int across = 2 * p.n <= 64 * 128 ? 16 : 64;
+  const dim3 grid((unsigned)((2 * p.n + across - 1) / across));
+  hipLaunchKernelGGL((across == 16 ? norm_parts_kernel<16> : norm_parts_kernel<64>), grid, dim3(1024), 0, stream, p.parts, shares, p.n, (uint8_t*)a->dweight,
+                     a->weight_dtype, (uint8_t*)a->dbias, a->bias_dtype);
 }
 
 template <class O> int forward(NormParams p, hipStream_t stream) {
@@ -582,8 +624,7 @@ template <class O> int backward(const tnx_norm_args* a, NormParams p, hipStream_
   if (apart && wanted)
     hipLaunchKernelGGL((norm_columns_kernel<O>), dim3((unsigned)((p.n + SPAN - 1) / SPAN), (unsigned)shares), dim3(256), 0, stream, p);
   if (wanted)
-    hipLaunchKernelGGL(norm_parts_kernel, dim3((unsigned)((2 * p.n + 63) / 64)), dim3(1024), 0, stream, p.parts, shares, p.n, (uint8_t*)a->dweight, a->weight_dtype,
-                       (uint8_t*)a->dbias, a->bias_dtype);
+    launch_parts(p, shares, a, stream);
   return launched();
 }
 
@@ -615,8 +656,7 @@ extern "C" int tnx_layer_norm_backward(const tnx_norm_args* a) {
   p.parts = (float*)a->workspace;
   const hipStream_t stream = (hipStream_t)a->stream;
   if (a->rows == 0) {                                     // sums of no rows
-    hipLaunchKernelGGL(norm_parts_kernel, dim3((unsigned)((2 * p.n + 63) / 64)), dim3(1024), 0, stream, p.parts, (int64_t)0, p.n, (uint8_t*)a->dweight, a->weight_dtype,
-                       (uint8_t*)a->dbias, a->bias_dtype);
+    launch_parts(p, 0, a, stream);
     return launched();
   }
   return a->dtype == TNX_BF16 ? backward<OutBF16>(a, p, stream) : a->dtype == TNX_F16 ? backward<OutF16>(a, p, stream) : backward<OutF32>(a, p, stream);
