@@ -89,27 +89,29 @@ def test_routes_of_a_linear_layer():
     a.stride_xm, a.stride_xk = 1, 100                         # contiguous along m
     assert route(a) == _C.LINEAR_ROUTE_APART and lib.tnx_linear_scratch_bytes(ctypes.byref(a)) >= 100 * 200 * 4
     assert route(linear_args(100, 200, 0)) == _C.LINEAR_ROUTE_APART
-    for m, n, k in ((1, 1, 1), (4, 100000, 64), (8, 200, 8192), (16, 4096, 4096)):
+    for m, n, k in ((1, 1, 1), (1, 100000, 4096), (4, 200, 8192), (8, 4096, 4096), (16, 2000, 2816), (4, 1000, 701)):
         few = linear_args(m, n, k, layout="nt")
         assert route(few) == _C.LINEAR_ROUTE_STREAM and lib.tnx_linear_workspace_bytes(ctypes.byref(few)) == 0
-    assert route(linear_args(17, 200, 304, layout="nt")) == route(linear_args(16, 512, 8192, layout="nt")) == _C.LINEAR_ROUTE_FUSED
-    assert route(linear_args(4, 200, 304, _C.F32, "nt")) == route(linear_args(8, 16384, 4096, _C.F32, "nt")) == _C.LINEAR_ROUTE_STREAM
+    for m, n, k in ((17, 200, 304), (16, 512, 8192), (16, 512, 2824), (8, 200, 8192), (4, 14336, 4096), (1, 4096, 14336), (4, 4096, 1001)):
+        assert route(linear_args(m, n, k, layout="nt")) == _C.LINEAR_ROUTE_FUSED, (m, n, k)
+    assert route(linear_args(4, 200, 304, _C.F32, "nt")) == route(linear_args(8, 4096, 4096, _C.F32, "nt")) == _C.LINEAR_ROUTE_STREAM
     assert route(linear_args(4, 20000, 304, _C.F32)) == _C.LINEAR_ROUTE_STREAM_ROWS
-    for other in (linear_args(9, 200, 304, _C.F32, "nt"), linear_args(8, 200, 4104, _C.F32, "nt"), linear_args(5, 200, 304, _C.F32), linear_args(4, 200, 4104, _C.F32)):
+    for other in (linear_args(9, 200, 304, _C.F32, "nt"), linear_args(8, 200, 4616, _C.F32, "nt"), linear_args(5, 20000, 304, _C.F32), linear_args(4, 20000, 4104, _C.F32), linear_args(4, 8192, 304, _C.F32),
+                  linear_args(16, 200, 304, _C.F32, "nt"), linear_args(4, 200, 8200, _C.F32, "nt")):
         assert route(other) == _C.LINEAR_ROUTE_FUSED
-    for m, n, k in ((1, 8, 1), (4, 200, 304), (4, 4096, 4096), (8, 16000, 2048)):
+    for m, n, k in ((1, 8, 4096), (8, 1024, 4100), (4, 200, 8192), (4, 8, 4096)):
         few = linear_args(m, n, k)
         assert route(few) == _C.LINEAR_ROUTE_STREAM_ROWS
         need = lib.tnx_linear_workspace_bytes(ctypes.byref(few))
-        assert (need >= _C.WS_COUNTER_BYTES + 4 * m * n) == (k >= 1024 and n < 16000), (m, n, k, need)
-        if need:                                              # refused before any launch: without its workspace, with one too short, with one off 16 bytes
-            few.y = 1 << 22
-            assert lib.tnx_linear(ctypes.byref(few)) == _C.E_WORKSPACE
-            few.workspace, few.workspace_bytes = 1 << 23, need - 1
-            assert lib.tnx_linear(ctypes.byref(few)) == _C.E_WORKSPACE
-            few.workspace, few.workspace_bytes = (1 << 23) + 8, need
-            assert lib.tnx_linear(ctypes.byref(few)) == _C.E_WORKSPACE
-    assert route(linear_args(9, 200, 4096)) == route(linear_args(8, 200, 304)) == route(linear_args(1, 16384, 64)) == route(linear_args(1, 7, 64)) == _C.LINEAR_ROUTE_FUSED
+        assert need >= _C.WS_COUNTER_BYTES + 8 * 4 * m * n, (m, n, k, need)
+        few.y = 1 << 22                                       # refused before any launch: without its workspace, with one too short, with one off 16 bytes
+        assert lib.tnx_linear(ctypes.byref(few)) == _C.E_WORKSPACE
+        few.workspace, few.workspace_bytes = 1 << 23, need - 1
+        assert lib.tnx_linear(ctypes.byref(few)) == _C.E_WORKSPACE
+        few.workspace, few.workspace_bytes = (1 << 23) + 8, need
+        assert lib.tnx_linear(ctypes.byref(few)) == _C.E_WORKSPACE
+    for m, n, k in ((9, 200, 4096), (1, 1025, 4096), (1, 200, 4095), (1, 7, 4096)):
+        assert route(linear_args(m, n, k)) == _C.LINEAR_ROUTE_FUSED, (m, n, k)
     assert route(linear_args(0, 200, 300)) == 0
     bad = linear_args(100, 200, 300)
     bad.activation = 5

@@ -159,7 +159,8 @@ def test_few_rows(device, dtype, case, pad, offset, layout):
     if n > 1 and k > 1:
         g = module._args(_C.GROUPED_ROWS, x, w, None, offsets, n, k, *w.stride())
         used = min(rows, groups)
-        streamed = k >= 2048 or used * n <= 16384 if layout == "nt" else rows <= 8 and n >= 8 and k >= 1024 and used * ((n + 63) // 64) <= 128
+        words = dtype == torch.float32 or (pitch | k + pad | offset) % 2 == 0 or used * n * k <= 8 << 20
+        streamed = (k >= 2048 or used * n <= 16384) and words if layout == "nt" else rows <= 8 and n >= 8 and k >= 1024 and used * ((n + 63) // 64) <= 128
         assert _C.load().tnx_grouped_route(ctypes.byref(g), None) == (2 if streamed else 1)
     y = tritonix.grouped_matmul(x, w, offsets)
     ref.check("y", y, ref.grouped(x, w, offsets)["y"], dtype)

@@ -192,7 +192,7 @@ def strided(device, rows, cols, dtype, seed, pitch, offset, scale=1.0):
     return out
 
 
-FEW = [(1, 1, 1), (1, 8, 1), (2, 64, 64), (1, 72, 4100), (8, 520, 2500), (6, 1001, 5000), (3, 9000, 1025), (1, 5, 7), (3, 9, 63), (4, 100, 257), (4, 4095, 520), (1, 4097, 136), (4, 4100, 1100), (5, 4104, 640), (8, 4099, 1026), (8, 33, 8192), (5, 17, 31), (8, 300, 2050),
+FEW = [(1, 1, 1), (1, 8, 1), (2, 64, 64), (1, 8, 4097), (7, 1024, 4099), (5, 130, 4600), (2, 8200, 77), (4, 9001, 1030), (8, 500, 4608), (1, 72, 4100), (8, 520, 2500), (6, 1001, 5000), (3, 9000, 1025), (1, 5, 7), (3, 9, 63), (4, 100, 257), (4, 4095, 520), (1, 4097, 136), (4, 4100, 1100), (5, 4104, 640), (8, 4099, 1026), (8, 33, 8192), (5, 17, 31), (8, 300, 2050),
        (9, 50, 64), (16, 129, 1025), (13, 4500, 513), (16, 16, 4608), (1, 70, 9000)]
 
 
@@ -209,10 +209,9 @@ def test_few_rows(device, dtype, m, n, k, pad, offset, layout):
     bias, residual = ref.draw(device, n, dtype=dtype, seed=3), ref.draw(device, m, n, dtype=dtype, seed=4)
     args = args_of(x, w, bias, "gelu")
     route = _C.load().tnx_linear_route(ctypes.byref(args), None)
-    f32 = dtype == torch.float32
-    if layout == "nt" and not f32 or m <= 4 and layout == "nt":
+    if layout == "nt" and (m == 1 or m <= 4 and k <= 8192) and (dtype == torch.float32 or n * k <= 1 << 20):
         assert route == _C.LINEAR_ROUTE_STREAM
-    elif layout == "nn" and m <= 4 and n >= 8 and (k <= 4096 or not f32):
+    elif layout == "nn" and m <= 8 and 8 <= n <= 1024 and k >= 4096 and dtype != torch.float32 or layout == "nn" and m <= 4 and n > 8192 and k <= 4096 and dtype == torch.float32:
         assert route == _C.LINEAR_ROUTE_STREAM_ROWS
     ref.check("y", tritonix.linear(x, w, bias, "gelu", residual), ref.linear(x, w, bias, "gelu", residual)["y"], dtype)
     plain = tritonix.linear(x, w)

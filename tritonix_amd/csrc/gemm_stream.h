@@ -7,8 +7,8 @@
 // groups of them take different parts of k, and of the 16 x 16 sums the blocks on the diagonal count.  That narrows a workgroup without an idle lane
 // among the loads, and a row's part of an instruction is 32 x 16 / C elements: from C = 8 on down whole lines of memory.  Rows of x come from the
 // caches.  The waves' and groups' sums meet in LDS, in order, where the epilogue runs on them: one launch, no workspace, the same bits every time.
-// bf16, cold weights, us: 1 x 4096 x 4096 7.6 (4.4 TB/s; the tile kernels, which cut k and hand slices over, 12.4), 1 x 14336 x 4096 19 (6.2 TB/s; 25),
-// 1 x 1024 x 1024 2.5 (7.4), 8 x 4096 x 4096 9.2 (12.5), 16 x 1024 x 1024 3.9 (7.5).
+// bf16, cold weights, us: 1 x 4096 x 4096 7.7 (4.4 TB/s; the tile kernels, which cut k and hand slices over, 9.5), 1 x 14336 x 4096 19 to 21 (22),
+// 1 x 16384 x 16384 78 (6.9 TB/s), 1 x 1000 x 704 3.1 (4.9), 8 x 1814 x 2752 5.5 (7.5).
 #pragma once
 #include "gemm_grouped.h"
 #include "gemm_linear.h"
@@ -156,8 +156,8 @@ template <class T> hipError_t stream_columns(const StreamParams& p, hipStream_t 
 // reads 8 columns of 8 rows of the weight and picks the 8 numbers of a column together with v_perm_b32, half an instruction a number.  Column e of
 // every lane makes one matrix instruction: 8 columns in two groups, as C = 8 above.  64 columns are few workgroups (narrower ones would leave parts of
 // lines), so that `parts` of them share a block's k: each writes its sums through its L2, and the one that arrives last adds them up in the order of the parts.
-// That costs 3 to 4 us, less than a CU's slow pace.  bf16, cold weights, us, against the tile kernels': 1 x 4096 x 4096 11.6 and 13.2, 1 x 8192 x 8192 27.2 (4.9 TB/s)
-// and 31.4, 1 x 512 x 8192 8.3 and 11.0, 8 x 4096 x 4096 12.8 and 13.7, 8 x 1024 x 1024 8.5 and 8.2; a k-contiguous weight's kernel 7.6, -, 4.9, 9.2 and 3.6.
+// That costs 3 us, less than a CU's slow pace.  bf16, cold weights, us, against the tile kernels': 1 x 512 x 8192 6.5 and 8.2, 1 x 1024 x 8192 8.6 and 10.2,
+// 8 x 128 x 4096 5.7 and 6.3.
 struct StreamRowsParams {
   const uint8_t* x;
   const uint8_t* w;
@@ -302,14 +302,10 @@ template <class T, int W, int U> __global__ __launch_bounds__(W * 64) void gemm_
   stream_rows_block<T, W, U, false>(p, xcd_remap(blockIdx.x, (p.n + 128 / T::ES - 1) / (128 / T::ES) * p.parts, 8));
 }
 
-// Workgroups to a block of 64 columns: one for each CU, twice as many where a wave then has no more than two steps (1 x 4096 x 4096, us: 4 parts 12.2, 8
-// parts 11.6; 1 x 8192 x 8192 2 parts 27.2, 4 parts 30.0), and a step at least for each wave.
+// Workgroups to a block of columns: a step for each of their waves, and not more than two workgroups to a CU (1 x 512 x 8192: 8 parts 1.2 us more than 16).
 constexpr int STREAM_ROWS_WAVES = 8;
 inline int stream_rows_parts(int64_t n, int64_t k, int es) {
-  const int64_t step = 128 / es, tiles = (n + step - 1) / step, most = k / (step * STREAM_ROWS_WAVES);
-  int64_t parts = tiles < 256 ? 256 / tiles : 1;
-  if (k <= parts * STREAM_ROWS_WAVES * 2 * step) parts *= 2;
-  if (parts > most) parts = most;
+  const int64_t step = 128 / es, tiles = (n + step - 1) / step, most = k / (step * STREAM_ROWS_WAVES), room = 512 / tiles, parts = most < room ? most : room;
   return parts < 1 ? 1 : (int)parts;
 }
 inline size_t stream_rows_workspace(int64_t m, int64_t n, int64_t k, int es) {

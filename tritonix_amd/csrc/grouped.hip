@@ -182,11 +182,15 @@ template <class O> __global__ __launch_bounds__(256) void join_kernel(const floa
 // Few rows by k-contiguous weights, which gemm_stream.h reads once a group for up to 8 rows: 8 rows in all, or 4 to a group on average (us,
 // against the tile kernels': 32 rows, 8 groups, 14336 x 4096 144 and 164, 64 rows 212 and 164; 128 rows, 32 groups, 4096 x 4096 153 and 173), but not many workgroups of a short k (256 rows, 64 groups, 1024 x 4096
 // 88 and 82; 4 rows 8.2 and 8.5, 64 rows, 16 groups, 700 x 1000 7.4 and 8.8).  float32 gains more: 8 rows, 128 groups, 2048 x 768 12.5 and 18.6, 128 rows,
-// 32 groups, 4096 x 4096 318 and 339.
+// 32 groups, 4096 x 4096 318 and 339.  Rows off whole words, whose loads take twice the time, while there is little of them (1 row, 64 groups, 4097 x 2048 10.9 and
+// 14.3, 4 rows 33 and 24).
 bool takes_stream(const tnx_grouped_args* a) {
   if (gradient(a) || a->block_m > 0 || a->k == 0 || a->stride_ak != 1 || a->stride_ar < a->k) return false;
   if (a->stride_bn == 1 || a->stride_bk != 1 || a->stride_bn < a->k) return false;
-  if (a->k < 2048 && (a->rows < a->groups ? a->rows : a->groups) * a->n > 16384) return false;
+  const int64_t columns = (a->rows < a->groups ? a->rows : a->groups) * a->n;
+  if (a->k < 2048 && columns > 16384) return false;
+  const bool words = a->dtype == TNX_F32 || (!(((uintptr_t)a->a | (uintptr_t)a->b) & 3) && a->stride_ar % 2 == 0 && a->stride_bn % 2 == 0 && a->stride_group % 2 == 0);
+  if (!words && columns * a->k > 8 << 20) return false;
   // (a grid's threads are counted in 32 bits)
   return (a->rows <= 8 || a->rows <= 4 * (int64_t)a->groups) && stream_runs(a->rows, a->groups) * ((a->n + 7) / 8) < (1 << 23) - 1;
 }

@@ -141,25 +141,37 @@ struct Plan {
 
 bool with_epilogue(const tnx_linear_args* a) { return a->bias || a->residual || a->z || a->activation != TNX_ACT_NONE; }
 
-// Few rows, k-contiguous on both sides: gemm_stream.h.  Up to 4 rows of any size; more rows take as long to fetch as the weight, workgroup for
-// workgroup, which a tile kernel fetches once for many columns: 5 to 8 rows up to k = 8192 (us, against the tile kernels': 8 x 512 x 8192 9.6 and
-// 10.5, 8 x 4096 x 14336 26.3 and 25.1), 9 to 16 where n and k are small (16 x 2050 x 4100 8.1 and 13.6, 16 x 4096 x 4096 10.9 and 12.5; 16 x 512 x
-// 8192 16.4 and 10.6, 16 x 30000 x 512 10.8 and 9.2).  float32: 1 x 14336 x 4096 41 and 123 (whose operands are cut into terms first), 4 x 512 x 8192 10.0 and
-// 12.9, 8 x 4096 x 4096 14.9 and 20.3, 8 x 512 x 8192 16.7 and 13.0, 16 x 4096 x 4096 21.2 and 20.7.
-bool takes_stream(const tnx_linear_args* a) {
-  if (a->stride_xk != 1 || a->stride_wk != 1 || a->m > 16 || a->n > 0x1000000 || a->k > 0x40000000) return false;
-  if (a->m <= 4) return true;
-  if (a->dtype == TNX_F32) return a->m <= 8 && a->k <= 4096 && a->n <= 16384;
-  return (a->m <= 8 && a->k <= 8192) || (a->n <= 4608 && a->k <= 4608);
+// rows that begin at whole words: 16-byte loads of others take twice the time
+bool whole_words(const tnx_linear_args* a) {
+  if (a->dtype == TNX_F32) return true;
+  return !(((uintptr_t)a->x | (uintptr_t)a->w) & 3) && a->stride_wn % 2 == 0 && (a->m == 1 || a->stride_xm % 2 == 0);
 }
 
-// The same by a row-major weight, while the tile kernels' columns are fewer than the CUs (beyond, 1 x 16384 x 16384: 91 us and 88): up to 4 rows, and
-// to 8 of a long k (8 x 512 x 8192 9.4 and 11.1, 8 x 1024 x 1024 8.5 and 8.2).  float32: up to 4 rows of a k that few parts do (1 x 14336 x 4096 48 and 117,
-// 1 x 4096 x 4096 18.9 and 20.6, 1 x 512 x 8192 14.4 and 13.3).
+// Few rows, k-contiguous on both sides: gemm_stream.h.  Rows of x are fetched for every block of columns, which counts the more the more rows there are and
+// the more blocks, and a long k by few workgroups is slower than the tile kernels' parts of it.  us, against the tile kernels', bf16: one row 1 x 1000 x 704
+// 3.1 and 4.9, 1 x 4096 x 4096 7.7 and 9.5, 1 x 8192 x 8192 25.4 and 26.7, 1 x 4096 x 14336 21.9 and 20.8; 4 x 4096 x 4096 9.1 and 9.4, 4 x 512 x 8192 6.0 and
+// 7.6, 4 x 14336 x 4096 25.2 and 21.2; 8 x 4096 x 4098 9.5 and 10.9, 8 x 512 x 8192 9.3 and 7.7; 16 x 1814 x 2746 7.2 and 8.1, 16 x 1024 x 4096 9.3 and 7.4.  Rows
+// of the weight off whole words: 4 x 1000 x 701 3.4 and 6.8, 1 x 4096 x 4097 16.4 and 10.8.  float32: 1 x 14336 x 4096 46 and 122 (whose operands are cut into
+// terms first), 4 x 8192 x 8192 52 and 56, 4 x 4096 x 14336 47 and 44, 8 x 4096 x 4096 13.9 and 18.1, 8 x 14336 x 4096 47 and 46.
+bool takes_stream(const tnx_linear_args* a) {
+  if (a->stride_xk != 1 || a->stride_wk != 1 || a->m > 16 || a->n > 0x1000000 || a->k > 0x40000000) return false;
+  const bool f32 = a->dtype == TNX_F32;
+  const int64_t weight = a->n * a->k;
+  if (!whole_words(a) && weight > 1 << 20) return false;
+  if (a->m == 1) return f32 || weight <= 1 << 24 || a->k <= 8192;
+  if (a->m <= 4) return a->k <= 8192 && (f32 || weight <= 1 << 24);
+  if (a->m <= 8) return a->k <= 4608 && weight <= 1 << 24;
+  return !f32 && a->k <= 2816 && weight <= 6 << 20;
+}
+
+// The same by a row-major weight.  Its blocks have 64 columns, which pays against the tile kernels where columns are few and k is long: bf16, us, 1 x 512 x 8192
+// 6.5 and 8.2, 8 x 512 x 8192 7.5 and 8.3, 1 x 1024 x 4096 6.4 and 7.5, 1 x 64 x 16384 6.1 and 8.6; 1 x 256 x 2048 5.5 and 5.3, 1 x 4096 x 4096 10.0 and 10.3,
+// 1 x 14336 x 4096 26.7 and 23.1.  float32, whose operands the tile kernels cut into terms where columns are many: 1 x 14336 x 4096 47 and 115, 4 x 30000 x 512
+// 22 and 38, 4 x 14336 x 4096 48 and 45; 1 x 1000 x 704 6.7 and 6.6.
 bool takes_stream_rows(const tnx_linear_args* a) {
   if (a->stride_xk != 1 || a->stride_wn != 1 || a->n < 8 || a->k > 0x40000000) return false;
-  if (a->dtype == TNX_F32) return a->m <= 4 && a->k <= 4096 && a->n <= 0x1000000;
-  return a->n < 16384 && (a->m <= 4 || (a->m <= 8 && a->k >= 2048));
+  if (a->dtype == TNX_F32) return a->m <= 4 && a->n > 8192 && a->n <= 0x1000000 && a->k <= 4096;
+  return a->m <= 8 && a->n <= 1024 && a->k >= 4096;
 }
 
 Plan make_plan(const tnx_linear_args* a) {
