@@ -262,6 +262,48 @@ def test_same_bits_every_time_and_from_a_graph(device, m):
                 assert torch.equal(a, c)
 
 
+def test_products_of_a_graph_share_their_counters(device):
+    """Several products that are cut along k in one graph, some on a second stream of it, eager ones and another graph of the same stream between:
+    every replay gives the eager bits."""
+    sizes = [(40, 1000, 2304), (24, 4096, 4096), (3, 512, 8192), (64, 700, 5000)]
+    w = [ref.draw(device, k, n, seed=i, scale=k ** -0.5) for i, (m, n, k) in enumerate(sizes)]
+    x = [ref.draw(device, m, k, seed=10 + i) for i, (m, n, k) in enumerate(sizes)]
+
+    def products(which):
+        return [tritonix.linear(x[i], w[i], activation="silu") for i in which]
+
+    side, second = torch.cuda.Stream(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        products(range(4))
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs = products((0, 1))
+            second.wait_stream(side)
+            with torch.cuda.stream(second):
+                outs += products((2, 3, 2))
+            outs += products((3, 2))
+            side.wait_stream(second)
+            outs += products((1, 0))
+        graphs.append((graph, outs))
+        with torch.cuda.stream(side):
+            products(range(4))
+        torch.cuda.synchronize()
+    for turn in range(4):
+        for i, t in enumerate(x):
+            t.copy_(ref.draw(device, *t.shape, seed=100 * turn + i))
+        want = [products((i,))[0] for i in (0, 1, 2, 3, 2, 3, 2, 1, 0)]
+        for graph, outs in graphs:
+            graph.replay()
+            products((turn % 4,))
+            torch.cuda.synchronize()
+            for a, c in zip(outs, want):
+                assert torch.equal(a, c)
+
+
 def test_on_another_stream(device):
     x, w, b = (ref.draw(device, *s, seed=i) for i, s in enumerate(((33, 2048), (2048, 512), (512,))))
     want = tritonix.linear(x, w, b, "silu")
