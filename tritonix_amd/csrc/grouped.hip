@@ -55,17 +55,19 @@ bool layout_of(const tnx_grouped_args* a, int bm, int bn, Layout* l) {
 
 // Modelled microseconds of a tile, as capi.hip has them (TileCost), and what streaming the weights with it costs against the best, row-major and
 // k-contiguous; four of the constants moved by up to 5 percent (one by a third) towards what 108 grouped problems measured, on which the choice
-// then takes 1.011x the best tile's time in the mean, 1.24x at most.
+// then takes 1.011x the best tile's time in the mean, 1.24x at most.  burst: of a short k the results are the time, and tiles of long rows write them
+// faster once they are more than a few MB (32768 rows, 32 groups, 128 x 2048 bf16: 256x256 44.7 us, 128x256 54, 128x128 79; 30000 rows, 4 groups, 64 x 3584 54, 65,
+// 95), by what each takes of the results' bytes at 5.05 TB/s beyond the fastest.
 struct Cost {
   int bm, bn, nw, stages;
-  double start, turn, slab, shared, crowd, tail, stream_nn, stream_nt;
+  double start, turn, slab, shared, crowd, tail, stream_nn, stream_nt, burst;
 };
-const Cost COST16[] = {{256, 256, 8, 2, 4.16, 0.001, 1.12, 1.89, 0.278, 2.8, 1.35, 1.45},    {256, 128, 8, 3, 4.24, 0.735, 0.575, 5.24, 0.439, 2.3, 1.2, 1.25},
-                       {128, 256, 8, 3, 4.5, 1.7, 0.545, 17.8, 0.442, 2.08, 1.1, 1.2},       {128, 128, 8, 3, 3.91, 0.51, 0.374, 2.18, 0.439, 1.32, 1.12, 1.15},
-                       {64, 128, 8, 3, 3.63, 1.11, 0.328, 0.975, 0.0551, 0.653, 1.0, 1.08},  {64, 64, 4, 4, 3.62, 0.794, 0.203, 0.656, 0.308, 0.896, 1.06, 1.03},
-                       {32, 128, 4, 3, 3.81, 0.918, 0.259, 0.495, 0.171, 0.983, 1.05, 1.1},  {32, 64, 4, 4, 3.48, 0.431, 0.143, 1.1, 0.276, 0.682, 1.1, 1.05}};
-const Cost COST32[] = {{64, 64, 4, 4, 3.78, 0.0015, 0.508, 0.815, 0.006, 0.611, 1.0, 1.0}, {32, 128, 4, 3, 4.29, 1.2, 0.535, 0.695, 0.151, 0.782, 1.0, 1.0},
-                       {32, 64, 4, 4, 3.68, 0.034, 0.279, 1.48, 0.133, 0.498, 1.0, 1.0}};
+const Cost COST16[] = {{256, 256, 8, 2, 4.16, 0.001, 1.12, 1.89, 0.278, 2.8, 1.35, 1.45, 0.0},    {256, 128, 8, 3, 4.24, 0.735, 0.575, 5.24, 0.439, 2.3, 1.2, 1.25, 0.27},
+                       {128, 256, 8, 3, 4.5, 1.7, 0.545, 17.8, 0.442, 2.08, 1.1, 1.2, 0.3},       {128, 128, 8, 3, 3.91, 0.51, 0.374, 2.18, 0.439, 1.32, 1.12, 1.15, 0.95},
+                       {64, 128, 8, 3, 3.63, 1.11, 0.328, 0.975, 0.0551, 0.653, 1.0, 1.08, 0.95},  {64, 64, 4, 4, 3.62, 0.794, 0.203, 0.656, 0.308, 0.896, 1.06, 1.03, 1.9},
+                       {32, 128, 4, 3, 3.81, 0.918, 0.259, 0.495, 0.171, 0.983, 1.05, 1.1, 2.3},  {32, 64, 4, 4, 3.48, 0.431, 0.143, 1.1, 0.276, 0.682, 1.1, 1.05, 2.6}};
+const Cost COST32[] = {{64, 64, 4, 4, 3.78, 0.0015, 0.508, 0.815, 0.006, 0.611, 1.0, 1.0, 0.0}, {32, 128, 4, 3, 4.29, 1.2, 0.535, 0.695, 0.151, 0.782, 1.0, 1.0, 0.0},
+                       {32, 64, 4, 4, 3.68, 0.034, 0.279, 1.48, 0.133, 0.498, 1.0, 1.0, 0.0}};
 
 constexpr double CUS = 256;
 
@@ -108,6 +110,7 @@ Choice make_choice(const tnx_grouped_args* a) {
   const double rows = (double)a->rows, groups = (double)a->groups, used = a->rows < a->groups ? rows : groups;
   const double active = groups * (1.0 - std::pow(1.0 - 1.0 / groups, rows));
   const double bytes = at ? (rows * (a->k + a->n) + groups * a->k * a->n) * es : (rows * (a->k + a->n) + active * a->k * a->n) * es;
+  const double written = rows * (double)a->n * es;
   const bool bt = !at && a->stride_bn != 1, tail = at || a->k % bk != 0 || a->n % 8 != 0;
   static const int cuts[] = {1, 2, 3, 4, 6, 8, 12, 16};
   double best = 1e300;
@@ -126,6 +129,7 @@ Choice make_choice(const tnx_grouped_args* a) {
       const double stream = bytes / 5.1e6 * (at ? 1.1 : bt ? t.stream_nt : t.stream_nn) + 2.5;
       const double p = at ? 2.0 : 4.0;
       us = std::pow(std::pow(us, p) + std::pow(stream, p), 1.0 / p);
+      if (!at) us += t.burst * (written > 3e6 ? written - 3e6 : 0.0) / 5.05e6 * (kt < 8 ? 1.0 : 8.0 / kt);
       if (s > 1) us += 3.0 + (2.0 * s * 4 + es) * sums_of(a) / 8e6;
       if (us < best * (s > 1 ? 0.95 : 1.0)) { best = us; pick = {e, s}; }
     }
