@@ -148,8 +148,9 @@ template <class T, int C, int NT, int U> hipError_t stream_lines(const StreamPar
 template <class T> hipError_t stream_columns(const StreamParams& p, hipStream_t stream) {
   if (p.m <= 4 && p.n < 4096) return stream_lines<T, 4, 1, 4>(p, stream);
   if (p.m <= 8 && (p.m <= 4 || p.n < 4096)) return stream_lines<T, 8, 1, 4>(p, stream);
-  if (p.m <= 8) return stream_lines<T, 8, 2, 2>(p, stream);
-  return stream_lines<T, 16, 1, 4>(p, stream);
+  if constexpr (T::ES == 2)
+    if (p.m > 8) return stream_lines<T, 16, 1, 4>(p, stream);
+  return stream_lines<T, 8, 2, 2>(p, stream);
 }
 
 // The same for a row-major weight, up to 8 rows.  A workgroup owns 64 columns (float32: 32; a line of memory of each row of the weight), a step is 64 of k: a lane
