@@ -175,6 +175,18 @@ def test_few_rows(device, dtype, case, pad, offset, layout):
     assert torch.equal(got[others], y[others]) and got[bad].isnan().all()
 
 
+def test_bounds_past_32_bits(device):
+    """int64 bounds that 32 bits do not hold are the nearest inside, as all that lie outside."""
+    x, w = ref.draw(device, 64, 256, seed=1), weights(device, 4, 256, 40, torch.bfloat16, "nn", 2)
+    wide = torch.tensor([-2 ** 40, 10, 2 ** 32 + 5, 7, 2 ** 62], device=device)
+    y = tritonix.grouped_matmul(x, w, wide)
+    ref.check("y", y, ref.grouped(x, w, torch.tensor([0, 10, 64, 64, 64]))["y"], torch.bfloat16)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w)]
+    got = torch.autograd.grad(tritonix.grouped_matmul(*leaves, wide), leaves, y)
+    want = torch.autograd.grad(tritonix.grouped_matmul(*leaves, torch.tensor([0, 10, 64, 64, 64], dtype=torch.int32, device=device)), leaves, y)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("bounds", [[-5, 10, 20, 30], [0, 30, 10, 40], [50, 40, 30, 20], [0, 2 ** 31 - 1, 5, 7], [7, 7, 7, 7], [-(2 ** 31), -1, 0, 0], [40, 40, 40, 99]])
 def test_bounds_outside_of_the_rows(device, bounds):
     """Whatever the bounds hold, they are taken into the rows and to a sequence that does not decrease."""

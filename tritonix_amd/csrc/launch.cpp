@@ -1270,9 +1270,14 @@ PyObject* grouped_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!here(args[0], 2, &x, &device) || !here(args[1], 3, &w, &device) || !here(args[2], 1, &offsets, &device)) Py_RETURN_NONE;
     // (rows shorter than a chunk may have to be padded)
     if (x->size(1) != w->size(1) || w->size(1) < 8 || w->size(2) < 8 || x->size(0) == 0 || w->size(0) < 1 || w->size(0) > TNX_GROUPED_MAX_GROUPS ||
-        offsets->size(0) != w->size(0) + 1 || offsets->scalar_type() != at::kInt || !offsets->is_contiguous() || float_code(x->scalar_type()) < 0 ||
-        w->scalar_type() != x->scalar_type() || !row_major(*x) || !grouped_weights(*w))
+        offsets->size(0) != w->size(0) + 1 || (offsets->scalar_type() != at::kInt && offsets->scalar_type() != at::kLong) || !offsets->is_contiguous() ||
+        float_code(x->scalar_type()) < 0 || w->scalar_type() != x->scalar_type() || !row_major(*x) || !grouped_weights(*w))
       Py_RETURN_NONE;
+    at::Tensor narrowed;
+    if (offsets->scalar_type() == at::kLong) {            // (past 32 bits: the nearest inside)
+      narrowed = at::clamp(*offsets, 0, x->size(0)).to(at::kInt);
+      offsets = &narrowed;
+    }
     if (at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad())) return THPVariable_Wrap(GroupedProduct::apply(*x, *w, *offsets));
     void* stream = c10::hip::getCurrentHIPStream(device).stream();
     at::Tensor y;
