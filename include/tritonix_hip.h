@@ -500,8 +500,8 @@ typedef struct tnx_linear_args {
   void* stream;
 } tnx_linear_args;
 
-/* Both depend on sizes, strides, types, the alignment of x and w, and on whether there is an epilogue (z counts as one).  Calls that share a
- * workspace or scratch must be ordered. */
+/* Both depend on sizes, strides, types, the alignment of x and w, on whether there is an epilogue (z counts as one) and on the activation.  Calls that
+ * share a workspace or scratch must be ordered. */
 size_t tnx_linear_workspace_bytes(const tnx_linear_args* args);
 size_t tnx_linear_scratch_bytes(const tnx_linear_args* args);
 int tnx_linear(const tnx_linear_args* args);

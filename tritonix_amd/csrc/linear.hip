@@ -141,6 +141,9 @@ struct Plan {
 
 bool with_epilogue(const tnx_linear_args* a) { return a->bias || a->residual || a->z || a->activation != TNX_ACT_NONE; }
 
+// an activation of an exponential and a division
+bool curved(const tnx_linear_args* a) { return a->activation > TNX_ACT_RELU; }
+
 // rows that begin at whole words: 16-byte loads of others take twice the time
 bool whole_words(const tnx_linear_args* a) {
   if (a->dtype == TNX_F32) return true;
@@ -202,6 +205,15 @@ Plan make_plan(const tnx_linear_args* a) {
   if (p.status != TNX_OK) return p;
   // (256x256 on four waves, the choice for long sums, has no registers left for this epilogue: 129 spilled, none on eight)
   if (p.route == ROUTE_FUSED && !p.f32 && g.block_m == 256 && g.block_n == 256) g.num_warps = 8;
+  // Of a short k the epilogue's arithmetic is the time: two workgroups to a CU, whose epilogues and products overlap (bf16, gelu, us, 256x256 and 128x128: 8192 x
+  // 4096 x 128 56 and 44, 4708 x 5248 x 352 63 and 49, 8192 x 4096 x 512 68 and 63, x 1024 84 and 88; writing z too 61 and 55 of a k of 256, 75 and 72, silu
+  // 63 and 70, of one of 512; bias alone 4708 x 5248 x 352 38 and 38)
+  if (p.route == ROUTE_FUSED && !p.f32 && curved(a) && a->k <= 384 && g.split_k <= 1 && g.block_m * g.block_n > 128 * 128) {
+    g.block_m = g.block_n = 128;
+    g.num_warps = 8;
+    g.num_stages = 2;
+    g.tail_tiles = 0;
+  }
   if (p.route == ROUTE_FUSED && !(p.f32 ? gemm_f32_linear_fused(&g) : gemm_linear_fused(&g, GEMM_PLAIN))) {
     p.route = ROUTE_APART;
     if (!p.f32) {
@@ -234,7 +246,7 @@ const Plan& plan_of(const tnx_linear_args* a) {
   int device = 0;
   (void)hipGetDevice(&device);
   const Key k = {{a->m, a->n, a->k, a->stride_xm, a->stride_xk, a->stride_wk, a->stride_wn, a->dtype, with_epilogue(a) ? 1 : 0,
-                  (int64_t)(((uintptr_t)a->x & 15) << 4 | ((uintptr_t)a->w & 15)), device, 0}};
+                  (int64_t)(((uintptr_t)a->x & 15) << 4 | ((uintptr_t)a->w & 15)), device, curved(a) ? 1 : 0}};
   const auto hit = plans.find(k);
   if (hit != plans.end()) return hit->second;
   if (plans.size() >= 512) plans.clear();
