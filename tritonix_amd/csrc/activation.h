@@ -29,16 +29,18 @@ __device__ __forceinline__ float erfc_abs(float z, float* e) {
 
 // gelu: z (1 + erf(z / sqrt 2)) / 2 is z q / 2 below zero and z - z q / 2 above, with q = erfc(|z| / sqrt 2): no cancellation next to -1.
 // gelu_tanh: z (1 + tanh u) / 2 = z / (1 + e^-2u), which keeps its relative precision where tanh is next to -1
+// The factor beside one that is zero in 32 bits past -128 (gelu's tail: past +-128) is held there, for the product of an infinity and a zero is no number: -inf gives zero and
+// +inf itself.  (fmaxf and fminf take a NaN for the bound: the other factor is NaN then.)
 __device__ __forceinline__ float activate(float z, int act) {
   switch (act) {
     case ACT_RELU: return z <= 0.0f ? 0.0f : z;          // (a NaN stays one)
-    case ACT_SILU: return z * logistic(z);
+    case ACT_SILU: return fmaxf(z, -128.0f) * logistic(z);
     case ACT_GELU: {
       float e;
-      const float half = 0.5f * z * erfc_abs(z, &e);
+      const float half = 0.5f * fminf(fmaxf(z, -128.0f), 128.0f) * erfc_abs(z, &e);
       return z > 0.0f ? z - half : half;
     }
-    case ACT_GELU_TANH: return z * logistic(2.0f * GELU_C * (z + GELU_A * z * z * z));
+    case ACT_GELU_TANH: return fmaxf(z, -128.0f) * logistic(2.0f * GELU_C * (z + GELU_A * z * z * z));
     default: return z;
   }
 }
