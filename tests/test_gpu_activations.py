@@ -1,4 +1,4 @@
-"""Activations of linear layers at the ends of their range: infinities and huge numbers."""
+"""Activations of linear layers at the ends of their range: infinities and huge numbers, and gelu where it is next to nothing."""
 import ctypes
 
 import pytest
@@ -60,3 +60,38 @@ def test_infinities_have_their_limits(device, dtype, act, m, n, k, layout, place
     for c in (0, n - 2):
         assert (dbias[c].double() - total[c]).abs() <= (m + 2) * ref.E * magnitude[c]
     assert dbias[5] == 0 and dbias[n - 1] == 0 and dbias[7].isnan()
+
+
+def gelu_exactly(z):
+    return 0.5 * z * torch.special.erfc(-z * 0.5 ** 0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("place", ["stream", "fused", "apart"])
+def test_gelu_below_zero_is_relatively_exact(device, dtype, place):
+    """From -12 to next to 0, where it falls to 1e-32, gelu and its slope are off by what 32-bit arithmetic costs, relative to themselves.
+
+    With e^-(z^2 / 2) from one exponential of a rounded argument: z^2 times half a step, times log2 e (rounded, and the constant's own 0.1 steps), is 1.11 z^2 / 2 steps of the result; the
+    exponential's and the reciprocal's last step, a polynomial of eight terms whose magnitudes add up to 1.65 (two half steps each) and four products come to 12 steps more, the polynomial's own error
+    to 1.6: in all (14 + 1.2 z^2 / 2) E.  The slope is the difference of two such terms, of 1.3 times its own size together from -3 on down."""
+    m, n, k = {"stream": (8 if dtype == torch.float32 else 16, 16, 16), "fused": (2048, 64, 64), "apart": (2048, 16, 33)}[place]
+    z = torch.linspace(-12, -0.01, m).to(dtype).double()
+    x, w = torch.zeros(m, k, dtype=dtype, device=device), torch.zeros(k, n, dtype=dtype, device=device)
+    x[:, 0], w[0, 0] = z.to(dtype).to(device), 1.0
+    if place == "apart":
+        x = x.t().contiguous().t()
+    elif place == "stream":
+        w = w.t().contiguous().t()
+    assert route_of(x, w, "gelu") == ROUTES[place]
+    x.requires_grad_(True)
+    y = tritonix.linear(x, w, None, "gelu")
+    dy = torch.zeros(m, n, dtype=dtype, device=device)
+    dy[:, 0] = 1.0
+    (dx,) = torch.autograd.grad(y, x, dy)
+    steps = (14 + 0.6 * z * z) * ref.E
+    want = gelu_exactly(z)
+    ref.check("gelu", y[:, 0], (want, steps * want.abs() + ref.rounding(want, dtype)))
+    slope = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5) + z * torch.exp(-0.5 * z * z) * (2 * torch.pi) ** -0.5
+    # (dz is rounded for the product dx = dz w^T, and dx once more; above -3 the terms cancel: their magnitudes)
+    terms = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5) + z.abs() * torch.exp(-0.5 * z * z) * (2 * torch.pi) ** -0.5
+    ref.check("slope", dx[:, 0], (slope, steps * torch.where(z <= -3, 1.3 * slope.abs(), terms) + 2 * ref.rounding(slope, dtype) + (k + 2) * ref.E * slope.abs()))

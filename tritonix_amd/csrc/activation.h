@@ -13,17 +13,21 @@ constexpr float GELU_A = 0.044715f;
 // instructions
 __device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
-// erfc(|z| / sqrt 2), and e = exp(-z^2 / 2) on the way: t P(t) e with t = 1 / (1 + p |z| / sqrt 2), the rational approximation of Hastings
-// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26), off by at most 1.5e-7.  A call of erff, with its branches, took the gated and
-// activated epilogues 6 to 10 percent of a launch (4096 x 14336 x 4096 bf16, gelu: 1.19 times the plain product's time, 1.12 with this).
+// erfc(|z| / sqrt 2), and e = exp(-z^2 / 2) on the way: t P(t) e with t = 1 / (1 + p |z| / sqrt 2), as Hastings' rational approximations are formed.  P is of degree 7 and p 0.44, fitted
+// here to the smallest largest error relative to the result, from 0 to |z| = 18 (weighted least squares, the weights raised where the error is largest, on 1200 Chebyshev points): 1.9e-7.
+// In 32 bits (14 + 0.6 z^2) 2^-23 of the result, the exponential's argument being rounded.  A fit of five terms to the error itself, 1.5e-7 of it, is 2e-2 off relative to the
+// result at |z| = 10, which gelu(-10) then is (4096 x 30000 x 768 bf16 with gelu: 281 us, with this 290; 8192 x 4096 x 4096 216 to 218 and 220).  A call of erff, with its branches,
+// took 4096 x 14336 x 4096 with gelu 1.19 times the plain product's time, this 1.13.
 __device__ __forceinline__ float erfc_abs(float z, float* e) {
-  const float x = __builtin_fabsf(z) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
-  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-  p = __builtin_fmaf(p, t, 1.421413741f);
-  p = __builtin_fmaf(p, t, -0.284496736f);
-  p = __builtin_fmaf(p, t, 0.254829592f);
-  *e = __expf(-x * x);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.311126984f, __builtin_fabsf(z), 1.0f));      // p / sqrt 2
+  float p = __builtin_fmaf(0.0715003982f, t, -0.279155076f);
+  p = __builtin_fmaf(p, t, 0.298870951f);
+  p = __builtin_fmaf(p, t, -0.0222975835f);
+  p = __builtin_fmaf(p, t, 0.216995254f);
+  p = __builtin_fmaf(p, t, 0.216934204f);
+  p = __builtin_fmaf(p, t, 0.248935491f);
+  p = __builtin_fmaf(p, t, 0.248216525f);
+  *e = __builtin_amdgcn_exp2f(z * z * -0.721347520f);                                                 // log2(e) / 2
   return p * t * *e;
 }
 
