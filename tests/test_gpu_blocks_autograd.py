@@ -1,0 +1,60 @@
+"""Linear layers, normalisation and grouped products in the autograd graph, natively and through the interpreter: which calls have no derivative."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import blocks_reference as ref
+import tritonix
+from tritonix_amd.ops import mx, native
+
+pytestmark = pytest.mark.gpu
+F32 = torch.float32
+
+
+@pytest.fixture(params=["native", "interpreter"])
+def side(request, monkeypatch, device):
+    tritonix.layer_norm(torch.zeros(2, 16, device=device))            # (finds the native side)
+    assert native.module is not mx._Interpreter, "the native side is not in use"
+    if request.param == "interpreter":
+        monkeypatch.setattr(native, "module", mx._Interpreter)
+    return request.param
+
+
+def inputs(device, op):
+    d = lambda i, *s, scale=1.0: ref.draw(device, *s, dtype=F32, seed=i, scale=scale)  # noqa: E731
+    if op == "linear":
+        return {"x": d(1, 40, 48), "w": d(2, 48, 64, scale=0.1), "bias": d(3, 64), "residual": d(4, 40, 64)}, d(5, 40, 64)
+    if op == "norm":
+        return {"x": d(1, 40, 300), "weight": d(2, 300), "bias": d(3, 300)}, d(4, 40, 300)
+    return {"x": d(1, 40, 48), "w": d(2, 3, 48, 64, scale=0.1), "offsets": torch.tensor([1, 20, 20, 38], dtype=torch.int32, device=device)}, d(3, 40, 64)
+
+
+def call(op, t, act):
+    if op == "linear":
+        return tritonix.linear(t["x"], t["w"], t["bias"], act, t["residual"])
+    return tritonix.layer_norm(t["x"], t["weight"], t["bias"]) if op == "norm" else tritonix.grouped_matmul(t["x"], t["w"], t["offsets"])
+
+
+@pytest.mark.parametrize("op", ["linear", "norm", "grouped"])
+def test_forward_mode_is_refused(device, side, op):
+    """A tangent is refused, with gradients asked for and without, on any of the floating operands and on the gradient that comes back."""
+    given, dy = inputs(device, op)
+    names = [name for name in given if name != "offsets"]
+    clean = call(op, given, "silu")
+    with forward_ad.dual_level():
+        for name in names:
+            for leaf in (False, True):
+                t = {k: v.detach().clone().requires_grad_(leaf and k != "offsets") for k, v in given.items()}
+                t[name] = forward_ad.make_dual(t[name], torch.ones_like(t[name]))
+                with pytest.raises(RuntimeError, match="forward"):
+                    call(op, t, "silu")
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+                    call(op, t, "silu")
+        t = {k: v.detach().clone() for k, v in given.items()}
+        t["x"].requires_grad_(True)
+        y = call(op, t, "silu")
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, t["x"], forward_ad.make_dual(dy, torch.ones_like(dy)))
+        # an operand without a tangent is as ever
+        assert torch.equal(call(op, given, "silu"), clean)
+    assert torch.equal(call(op, given, "silu"), clean)

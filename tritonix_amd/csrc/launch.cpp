@@ -90,9 +90,10 @@ struct Conv {
 std::unordered_map<Key, Product, Hash>& products = *new std::unordered_map<Key, Product, Hash>;
 std::unordered_map<Key, Conv, Hash>& convs = *new std::unordered_map<Key, Conv, Hash>;
 
-// an ordinary dense tensor on the GPU: nothing that intercepts the calls the Python path would make of it
+// an ordinary dense tensor on the GPU: nothing that intercepts the calls the Python path would make of it, no tangent of forward mode (which the Python
+// path refuses where an operator has gradients)
 bool plain(const at::Tensor& t, int64_t dim) {
-  if (!t.defined() || !t.is_cuda() || t.dim() != dim || t.layout() != at::kStrided) return false;
+  if (!t.defined() || !t.is_cuda() || t.dim() != dim || t.layout() != at::kStrided || t._fw_grad(0).defined()) return false;
   const c10::TensorImpl* impl = t.unsafeGetTensorImpl();
   if (impl->is_python_dispatch()) return false;
   static const c10::DispatchKeySet other({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::Functionalize,
@@ -995,7 +996,7 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &z = saved[2];
     const at::Tensor given = grads[0].detach();
-    TORCH_CHECK(plain(given, 2) && given.size(1) == w.size(1) && given.scalar_type() == w.scalar_type(),
+    TORCH_CHECK(plain(grads[0], 2) && given.size(1) == w.size(1) && given.scalar_type() == w.scalar_type(),
                 "linear: a gradient that is not an ordinary tensor of the result's size and type");
     const int act = (int)ctx->saved_data["act"].toInt();
     const int64_t bias_type = ctx->saved_data["bias"].toInt();
@@ -1117,7 +1118,7 @@ struct NormLayer : torch::autograd::Function<NormLayer> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &statistics = saved[3];
     const at::Tensor given = grads[0].detach();
-    TORCH_CHECK(plain(given, 2) && given.sizes() == x.sizes() && given.scalar_type() == x.scalar_type(),
+    TORCH_CHECK(plain(grads[0], 2) && given.sizes() == x.sizes() && given.scalar_type() == x.scalar_type(),
                 "layer_norm: a gradient that is not an ordinary tensor of the result's size and type");
     const at::Tensor dy = given.stride(1) == 1 || given.size(1) <= 1 ? given : given.contiguous();
     const c10::DeviceIndex device = (c10::DeviceIndex)dy.get_device();
@@ -1242,7 +1243,7 @@ struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
     at::Tensor dy = grads[0].detach();
-    TORCH_CHECK(plain(dy, 2) && dy.size(1) == w.size(2) && dy.scalar_type() == w.scalar_type(),
+    TORCH_CHECK(plain(grads[0], 2) && dy.size(1) == w.size(2) && dy.scalar_type() == w.scalar_type(),
                 "grouped_matmul: a gradient that is not an ordinary tensor of the result's size and type");
     if (!row_major(dy)) dy = dy.contiguous();
     const c10::DeviceIndex device = (c10::DeviceIndex)dy.get_device();

@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from tritonix_amd import _C
 from tritonix_amd.ops import native as _native
-from tritonix_amd.ops.mx import dtype_code, launch, on_device
+from tritonix_amd.ops.mx import dtype_code, launch, no_tangent, on_device
 
 __all__ = ["grouped_matmul"]
 
@@ -117,6 +117,7 @@ class _Grouped(torch.autograd.Function):
     def backward(ctx, dy):
         if dy is None:
             return None, None, None
+        no_tangent("grouped_matmul", dy)
         x, w, offsets = ctx.saved_tensors
         dx = dw = None
         if ctx.needs_input_grad[0]:

@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 from tritonix_amd import _C
 from tritonix_amd import kernel as _kernel
 from tritonix_amd.ops import native as _native
-from tritonix_amd.ops.mx import dtype_code, on_device, raise_for_status
+from tritonix_amd.ops.mx import dtype_code, no_tangent, on_device, raise_for_status
 
 _mm = importlib.import_module("tritonix_amd.ops.matmul")
 
@@ -114,6 +114,7 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         if dy is None:
             return None, None, None, None, None
+        no_tangent("linear", dy)
         x, w, z = ctx.saved_tensors
         wants_x, wants_w, wants_bias, wants_residual = ctx.needs_input_grad[:4]
         dresidual = dy if wants_residual else None

@@ -16,6 +16,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from tritonix_amd import _C
@@ -80,8 +81,16 @@ def raise_for_status(status: int, what: str) -> None:
     raise ValueError(f"{what}: {_C.strerror(status)}")
 
 
+def no_tangent(name: str, *tensors) -> None:
+    """Refuses tensors that carry a tangent of forward mode: the result would have none, silently."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
 def on_device(name: str, *tensors) -> int:
     """Index of the HIP device that all of them are on."""
+    no_tangent(name, *tensors)
     index = -1
     for t in tensors:
         if t is None:

@@ -16,7 +16,7 @@ from torch.autograd.function import once_differentiable
 from tritonix_amd import _C
 from tritonix_amd import kernel as _kernel
 from tritonix_amd.ops import native as _native
-from tritonix_amd.ops.mx import dtype_code, launch, on_device, raise_for_status
+from tritonix_amd.ops.mx import dtype_code, launch, no_tangent, on_device, raise_for_status
 
 __all__ = ["layer_norm"]
 
@@ -65,6 +65,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         if dy is None:
             return None, None, None, None
+        no_tangent("layer_norm", dy)
         x, weight, bias, mean, rstd = ctx.saved_tensors
         wants_x, wants_weight, wants_bias = ctx.needs_input_grad[:3]
         dy = _rows(dy)
