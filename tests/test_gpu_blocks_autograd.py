@@ -58,3 +58,26 @@ def test_forward_mode_is_refused(device, side, op):
         # an operand without a tangent is as ever
         assert torch.equal(call(op, given, "silu"), clean)
     assert torch.equal(call(op, given, "silu"), clean)
+
+
+@pytest.mark.parametrize("op", ["linear", "norm", "grouped"])
+def test_negated_views(device, side, op):
+    """A tensor that torch holds as the negative of its memory (the imaginary part of a conjugate) counts with its sign."""
+    given, dy = inputs(device, op)
+    names = [name for name in given if name != "offsets"]
+    for name in names:
+        negated = torch._neg_view(given[name])
+        assert negated.is_neg()
+        t = {**given, name: -given[name]}
+        want = call(op, t, "silu")
+        assert torch.equal(call(op, {**given, name: negated}, "silu"), want)
+        leaf = given[name].detach().clone().requires_grad_(True)
+        (g,) = torch.autograd.grad(call(op, {**given, name: torch._neg_view(leaf)}, "silu"), leaf, dy)
+        other = given[name].detach().clone().requires_grad_(True)
+        (h,) = torch.autograd.grad(call(op, {**given, name: -other}, "silu"), other, dy)
+        assert torch.equal(g.resolve_neg(), h.resolve_neg())
+    t = {k: v.detach().clone() for k, v in given.items()}
+    t["x"].requires_grad_(True)
+    (g,) = torch.autograd.grad(call(op, t, "silu"), t["x"], torch._neg_view(dy))
+    (h,) = torch.autograd.grad(call(op, t, "silu"), t["x"], -dy)
+    assert torch.equal(g, h)

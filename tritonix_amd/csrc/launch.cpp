@@ -98,7 +98,8 @@ bool plain(const at::Tensor& t, int64_t dim) {
   if (impl->is_python_dispatch()) return false;
   static const c10::DispatchKeySet other({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::Functionalize,
                                           c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                          c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::Batched});
+                                          c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::Batched,
+                                          c10::DispatchKey::Negative});      // (the negative of its memory)
   return !impl->key_set().has_any(other);
 }
 
@@ -995,8 +996,8 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
     if (!grads[0].defined()) return torch::autograd::variable_list(5);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &z = saved[2];
-    const at::Tensor given = grads[0].detach();
-    TORCH_CHECK(plain(grads[0], 2) && given.size(1) == w.size(1) && given.scalar_type() == w.scalar_type(),
+    const at::Tensor resolved = grads[0].resolve_neg(), given = resolved.detach();
+    TORCH_CHECK(plain(resolved, 2) && given.size(1) == w.size(1) && given.scalar_type() == w.scalar_type(),
                 "linear: a gradient that is not an ordinary tensor of the result's size and type");
     const int act = (int)ctx->saved_data["act"].toInt();
     const int64_t bias_type = ctx->saved_data["bias"].toInt();
@@ -1117,8 +1118,8 @@ struct NormLayer : torch::autograd::Function<NormLayer> {
     if (!grads[0].defined()) return torch::autograd::variable_list(4);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &statistics = saved[3];
-    const at::Tensor given = grads[0].detach();
-    TORCH_CHECK(plain(grads[0], 2) && given.sizes() == x.sizes() && given.scalar_type() == x.scalar_type(),
+    const at::Tensor resolved = grads[0].resolve_neg(), given = resolved.detach();
+    TORCH_CHECK(plain(resolved, 2) && given.sizes() == x.sizes() && given.scalar_type() == x.scalar_type(),
                 "layer_norm: a gradient that is not an ordinary tensor of the result's size and type");
     const at::Tensor dy = given.stride(1) == 1 || given.size(1) <= 1 ? given : given.contiguous();
     const c10::DeviceIndex device = (c10::DeviceIndex)dy.get_device();
@@ -1242,8 +1243,9 @@ struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
     if (!grads[0].defined()) return torch::autograd::variable_list(3);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
-    at::Tensor dy = grads[0].detach();
-    TORCH_CHECK(plain(grads[0], 2) && dy.size(1) == w.size(2) && dy.scalar_type() == w.scalar_type(),
+    const at::Tensor resolved = grads[0].resolve_neg();
+    at::Tensor dy = resolved.detach();
+    TORCH_CHECK(plain(resolved, 2) && dy.size(1) == w.size(2) && dy.scalar_type() == w.scalar_type(),
                 "grouped_matmul: a gradient that is not an ordinary tensor of the result's size and type");
     if (!row_major(dy)) dy = dy.contiguous();
     const c10::DeviceIndex device = (c10::DeviceIndex)dy.get_device();

@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from tritonix_amd import _C
 from tritonix_amd.ops import native as _native
-from tritonix_amd.ops.mx import dtype_code, launch, no_tangent, on_device
+from tritonix_amd.ops.mx import as_memory, dtype_code, launch, no_tangent, on_device
 
 __all__ = ["grouped_matmul"]
 
@@ -118,6 +118,7 @@ class _Grouped(torch.autograd.Function):
         if dy is None:
             return None, None, None
         no_tangent("grouped_matmul", dy)
+        (dy,) = as_memory(dy)
         x, w, offsets = ctx.saved_tensors
         dx = dw = None
         if ctx.needs_input_grad[0]:
@@ -151,6 +152,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> t
     if w.dtype != x.dtype:
         raise ValueError(f"grouped_matmul: x is {x.dtype}, w is {w.dtype}")
     on_device("grouped_matmul", x, w, offsets)
+    x, w, offsets = as_memory(x, w, offsets)
     if offsets.dtype == torch.int64:
         offsets = offsets.clamp(0, x.shape[0])             # (past 32 bits: the nearest inside)
     offsets = offsets.to(torch.int32).contiguous()

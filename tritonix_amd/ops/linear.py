@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 from tritonix_amd import _C
 from tritonix_amd import kernel as _kernel
 from tritonix_amd.ops import native as _native
-from tritonix_amd.ops.mx import dtype_code, no_tangent, on_device, raise_for_status
+from tritonix_amd.ops.mx import as_memory, dtype_code, no_tangent, on_device, raise_for_status
 
 _mm = importlib.import_module("tritonix_amd.ops.matmul")
 
@@ -115,6 +115,7 @@ class _Linear(torch.autograd.Function):
         if dy is None:
             return None, None, None, None, None
         no_tangent("linear", dy)
+        (dy,) = as_memory(dy)
         x, w, z = ctx.saved_tensors
         wants_x, wants_w, wants_bias, wants_residual = ctx.needs_input_grad[:4]
         dresidual = dy if wants_residual else None
@@ -164,6 +165,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     rows = 1
     for d in lead:
         rows *= d
+    x, w, bias, residual = as_memory(x, w, bias, residual)
     x = x if len(lead) == 1 else x.reshape(rows, k)
     if residual is not None:
         residual = residual.reshape(rows, n).contiguous()

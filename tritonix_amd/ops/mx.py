@@ -88,6 +88,11 @@ def no_tangent(name: str, *tensors) -> None:
             raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
+def as_memory(*tensors):
+    """The tensors with their values in memory: torch holds the negative of a tensor (the imaginary part of a conjugate) as a view that is marked so."""
+    return tuple(None if t is None else t.resolve_neg() for t in tensors)
+
+
 def on_device(name: str, *tensors) -> int:
     """Index of the HIP device that all of them are on."""
     no_tangent(name, *tensors)

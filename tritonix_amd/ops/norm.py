@@ -16,7 +16,7 @@ from torch.autograd.function import once_differentiable
 from tritonix_amd import _C
 from tritonix_amd import kernel as _kernel
 from tritonix_amd.ops import native as _native
-from tritonix_amd.ops.mx import dtype_code, launch, no_tangent, on_device, raise_for_status
+from tritonix_amd.ops.mx import as_memory, dtype_code, launch, no_tangent, on_device, raise_for_status
 
 __all__ = ["layer_norm"]
 
@@ -66,6 +66,7 @@ class _LayerNorm(torch.autograd.Function):
         if dy is None:
             return None, None, None, None
         no_tangent("layer_norm", dy)
+        (dy,) = as_memory(dy)
         x, weight, bias, mean, rstd = ctx.saved_tensors
         wants_x, wants_weight, wants_bias = ctx.needs_input_grad[:3]
         dy = _rows(dy)
@@ -111,6 +112,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     rows = 1
     for d in x.shape[:-1]:
         rows *= d
+    x, weight, bias = as_memory(x, weight, bias)
     given = x.shape
     x = _rows(x if x.dim() == 2 else x.reshape(rows, n))
     weight = None if weight is None else weight.contiguous()
