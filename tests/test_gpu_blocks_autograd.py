@@ -1,4 +1,6 @@
-"""Linear layers, normalisation and grouped products in the autograd graph, natively and through the interpreter: which calls have no derivative."""
+"""Linear layers, normalisation and grouped products in the autograd graph, natively and through the interpreter: which operands are kept, and which calls have no derivative."""
+import itertools
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -20,6 +22,10 @@ def side(request, monkeypatch, device):
     return request.param
 
 
+# what a gradient of each of the inputs reads of the others (and of itself)
+READS = {"linear": {"x": {"w"}, "w": {"x"}, "bias": set(), "residual": set()}, "norm": {"x": {"x", "weight"}, "weight": {"x"}, "bias": set()}, "grouped": {"x": {"w", "offsets"}, "w": {"x", "offsets"}}}
+
+
 def inputs(device, op):
     d = lambda i, *s, scale=1.0: ref.draw(device, *s, dtype=F32, seed=i, scale=scale)  # noqa: E731
     if op == "linear":
@@ -33,6 +39,48 @@ def call(op, t, act):
     if op == "linear":
         return tritonix.linear(t["x"], t["w"], t["bias"], act, t["residual"])
     return tritonix.layer_norm(t["x"], t["weight"], t["bias"]) if op == "norm" else tritonix.grouped_matmul(t["x"], t["w"], t["offsets"])
+
+
+def definition(op, t, dy, act):
+    if op == "linear":
+        return ref.linear(t["x"], t["w"], t["bias"], act, t["residual"], dy)
+    return ref.layer_norm(t["x"], t["weight"], t["bias"], 1e-5, dy) if op == "norm" else ref.grouped(t["x"], t["w"], t["offsets"], dy)
+
+
+@pytest.mark.parametrize("op,act", [("linear", None), ("linear", "gelu"), ("norm", None), ("grouped", None)])
+def test_operands_that_no_gradient_reads_may_change(device, side, op, act):
+    """Before the backward pass each operand that the gradients asked for do not read is changed in place: they are what they were.  One that they read
+    is missed."""
+    given, dy = inputs(device, op)
+    names = [name for name in given if name != "offsets"]
+    want = definition(op, given, dy, act)
+    for asked in itertools.chain.from_iterable(itertools.combinations(names, c) for c in range(1, len(names) + 1)):
+        read = set().union(*(READS[op][name] for name in asked))
+        for changed in given:
+            t = {name: v.detach().clone() for name, v in given.items()}
+            leaves = [t[name].requires_grad_(True) for name in asked]
+            y = call(op, t, act)
+            with torch.no_grad():
+                t[changed].mul_(3)
+            if changed in read:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    torch.autograd.grad(y, leaves, dy)
+                continue
+            for name, g in zip(asked, torch.autograd.grad(y, leaves, dy)):
+                ref.check(f"{asked}, {changed} changed: d{name}", g, want["d" + name])
+
+
+@pytest.mark.parametrize("layout", ["nn", "nt"])
+@pytest.mark.parametrize("op", ["linear", "grouped"])
+def test_a_weights_gradient_has_its_layout(device, side, op, layout):
+    """Also where x asks for no gradient, and the weight is not kept for one."""
+    given, dy = inputs(device, op)
+    last = given["w"] if layout == "nn" else given["w"].transpose(-1, -2).contiguous().transpose(-1, -2)
+    for x_too in (False, True):
+        t = {**given, "x": given["x"].detach().requires_grad_(x_too), "w": last.detach().requires_grad_(True)}
+        (dw,) = torch.autograd.grad(call(op, t, None), (t["w"],), dy)
+        ref.check("dw", dw, definition(op, given, dy, None)["dw"])
+        assert dw.stride() == last.stride()
 
 
 @pytest.mark.parametrize("op", ["linear", "norm", "grouped"])

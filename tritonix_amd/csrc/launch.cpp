@@ -973,6 +973,13 @@ at::Tensor product_of(const at::Tensor& a, const at::Tensor& b, c10::DeviceIndex
 
 typedef std::optional<at::Tensor> MaybeTensor;
 
+// What a node keeps of its forward call beside tensors: that it had a residual; that its weights are k-contiguous, transposes of row-major ones, and their gradient is to
+// lie so too; the result's type and columns.
+enum { HAS_RESIDUAL = 1, TRANSPOSED = 2 };
+bool transposed(const at::Tensor& w) { return w.stride(-2) == 1 && w.stride(-1) != 1; }
+int64_t what_of(const at::Tensor& y, int64_t flags) { return flags | (int64_t)y.scalar_type() << 8 | y.size(1) << 16; }
+bool fits(const at::Tensor& dy, int64_t what) { return plain(dy, 2) && dy.size(1) == what >> 16 && (int64_t)dy.scalar_type() == (what >> 8 & 255); }
+
 struct LinearLayer : torch::autograd::Function<LinearLayer> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const MaybeTensor& bias, const MaybeTensor& residual,
                             int64_t act) {
@@ -986,24 +993,25 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
     }
     if (r.status != TNX_OK) throw std::runtime_error("linear");
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), w, r.z});
+    // (what no gradient that is asked for reads is not kept: it may change before the backward pass)
+    ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), x.requires_grad() ? w : at::Tensor(), r.z});
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = bias ? (int64_t)bias->scalar_type() : (int64_t)-1;
-    ctx->saved_data["residual"] = residual.has_value();
+    ctx->saved_data["what"] = what_of(r.y, (residual ? HAS_RESIDUAL : 0) | (transposed(w) ? TRANSPOSED : 0));
     return r.y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     if (!grads[0].defined()) return torch::autograd::variable_list(5);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &z = saved[2];
+    const int64_t what = ctx->saved_data["what"].toInt();
     const at::Tensor resolved = grads[0].resolve_neg(), given = resolved.detach();
-    TORCH_CHECK(plain(resolved, 2) && given.size(1) == w.size(1) && given.scalar_type() == w.scalar_type(),
-                "linear: a gradient that is not an ordinary tensor of the result's size and type");
+    TORCH_CHECK(fits(resolved, what), "linear: a gradient that is not an ordinary tensor of the result's size and type");
     const int act = (int)ctx->saved_data["act"].toInt();
     const int64_t bias_type = ctx->saved_data["bias"].toInt();
     // (inputs that were not given are not counted)
     const bool wants_x = ctx->needs_input_grad(0), wants_w = ctx->needs_input_grad(1), wants_bias = bias_type >= 0 && ctx->needs_input_grad(2);
-    const bool wants_residual = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(bias_type >= 0 ? 3 : 2);
+    const bool wants_residual = (what & HAS_RESIDUAL) && ctx->needs_input_grad(bias_type >= 0 ? 3 : 2);
     const c10::DeviceIndex device = (c10::DeviceIndex)given.get_device();
     void* stream = c10::hip::getCurrentHIPStream(device).stream();
     at::Tensor dx, dw, dbias;
@@ -1039,7 +1047,7 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
       }
       if (wants_x) dx = product_of(dz, w.t(), device, stream);
       // (a weight that is the transpose of a row-major one has its gradient so too)
-      if (wants_w) dw = w.stride(0) == 1 && w.stride(1) != 1 ? product_of(dz.t(), x, device, stream).t() : product_of(x.t(), dz, device, stream);
+      if (wants_w) dw = what & TRANSPOSED ? product_of(dz.t(), x, device, stream).t() : product_of(x.t(), dz, device, stream);
     }
     torch::autograd::variable_list out = gradients({dx, dw, dbias}, 5, "linear has no second derivative");
     // (the gradient itself, not another tensor of its memory: who takes it as his own looks whether others hold the tensor)
@@ -1110,37 +1118,44 @@ struct NormLayer : torch::autograd::Function<NormLayer> {
     }
     if (status != TNX_OK) throw std::runtime_error("layer_norm");
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({x, weight ? *weight : at::Tensor(), bias ? *bias : at::Tensor(), statistics});
-    ctx->saved_data["eps"] = eps;
+    // (x where dx or dweight is asked for, weight where dx is: what neither reads may change before the backward pass)
+    const bool own = x.requires_grad();
+    ctx->save_for_backward({own || (weight && weight->requires_grad()) ? x : at::Tensor(), own && weight ? *weight : at::Tensor(), statistics});
+    ctx->saved_data["what"] = what_of(y, 0);
+    ctx->saved_data["weight"] = weight ? (int64_t)weight->scalar_type() : (int64_t)-1;
+    ctx->saved_data["bias"] = bias ? (int64_t)bias->scalar_type() : (int64_t)-1;
     return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     if (!grads[0].defined()) return torch::autograd::variable_list(4);
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &statistics = saved[3];
+    const at::Tensor &x = saved[0], &weight = saved[1], &statistics = saved[2];
+    const int64_t weight_type = ctx->saved_data["weight"].toInt(), bias_type = ctx->saved_data["bias"].toInt();
     const at::Tensor resolved = grads[0].resolve_neg(), given = resolved.detach();
-    TORCH_CHECK(plain(resolved, 2) && given.sizes() == x.sizes() && given.scalar_type() == x.scalar_type(),
+    TORCH_CHECK(fits(resolved, ctx->saved_data["what"].toInt()) && given.size(0) == statistics.size(1),
                 "layer_norm: a gradient that is not an ordinary tensor of the result's size and type");
     const at::Tensor dy = given.stride(1) == 1 || given.size(1) <= 1 ? given : given.contiguous();
     const c10::DeviceIndex device = (c10::DeviceIndex)dy.get_device();
-    tnx_norm_args a = norm_args(x, weight.defined() ? &weight : nullptr, bias.defined() ? &bias : nullptr, (float)ctx->saved_data["eps"].toDouble(),
-                                c10::hip::getCurrentHIPStream(device).stream());
+    // (where only the bias asks, dx and dweight are not written and their sums not looked at: dy stands in for x)
+    tnx_norm_args a = norm_args(x.defined() ? x : dy, weight.defined() ? &weight : nullptr, nullptr, 0.0f, c10::hip::getCurrentHIPStream(device).stream());
     a.mean = (float*)statistics.data_ptr();
     a.rstd = a.mean + a.rows;
     a.dy = dy.data_ptr();
     a.stride_dy = dy.stride(0);
     at::Tensor dx, dweight, dbias, scratch;
     if (ctx->needs_input_grad(0)) {
-      dx = fresh({a.rows, a.n}, x.scalar_type(), device);
+      dx = fresh({a.rows, a.n}, dy.scalar_type(), device);
       a.dx = dx.data_ptr();
     }
-    if (weight.defined() && ctx->needs_input_grad(1)) {
-      dweight = fresh({a.n}, weight.scalar_type(), device);
+    if (weight_type >= 0 && ctx->needs_input_grad(1)) {
+      dweight = fresh({a.n}, (at::ScalarType)weight_type, device);
       a.dweight = dweight.data_ptr();
+      a.weight_dtype = float_code((at::ScalarType)weight_type);
     }
-    if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1)) {       // (inputs that were not given are not counted)
-      dbias = fresh({a.n}, bias.scalar_type(), device);
+    if (bias_type >= 0 && ctx->needs_input_grad(weight_type >= 0 ? 2 : 1)) {       // (inputs that were not given are not counted)
+      dbias = fresh({a.n}, (at::ScalarType)bias_type, device);
       a.dbias = dbias.data_ptr();
+      a.bias_dtype = float_code((at::ScalarType)bias_type);
     }
     if (const size_t bytes = blocks.norm_workspace(&a)) {
       scratch = fresh({(int64_t)bytes}, at::kByte, device);
@@ -1236,17 +1251,18 @@ struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
     }
     if (status != TNX_OK) throw std::runtime_error("grouped_matmul");
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), w, offsets});
+    ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), x.requires_grad() ? w : at::Tensor(), offsets});
+    ctx->saved_data["what"] = what_of(y, transposed(w) ? TRANSPOSED : 0);
     return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     if (!grads[0].defined()) return torch::autograd::variable_list(3);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
+    const int64_t what = ctx->saved_data["what"].toInt();
     const at::Tensor resolved = grads[0].resolve_neg();
     at::Tensor dy = resolved.detach();
-    TORCH_CHECK(plain(resolved, 2) && dy.size(1) == w.size(2) && dy.scalar_type() == w.scalar_type(),
-                "grouped_matmul: a gradient that is not an ordinary tensor of the result's size and type");
+    TORCH_CHECK(fits(resolved, what), "grouped_matmul: a gradient that is not an ordinary tensor of the result's size and type");
     if (!row_major(dy)) dy = dy.contiguous();
     const c10::DeviceIndex device = (c10::DeviceIndex)dy.get_device();
     void* stream = c10::hip::getCurrentHIPStream(device).stream();
@@ -1255,9 +1271,9 @@ struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
     if (ctx->needs_input_grad(0)) status = rows_product(dy, w.transpose(1, 2), offsets, device, stream, &dx);
     if (status == TNX_OK && ctx->needs_input_grad(1)) {
       // (as a linear layer's)
-      const bool transposed = w.stride(1) == 1 && w.stride(2) != 1;
-      status = transposed ? weight_gradient(dy, x, offsets, device, stream, &dw) : weight_gradient(x, dy, offsets, device, stream, &dw);
-      if (transposed) dw = dw.transpose(1, 2);
+      const bool turned = what & TRANSPOSED;
+      status = turned ? weight_gradient(dy, x, offsets, device, stream, &dw) : weight_gradient(x, dy, offsets, device, stream, &dw);
+      if (turned) dw = dw.transpose(1, 2);
     }
     TORCH_CHECK(status == TNX_OK, "grouped_matmul: status ", status, " in the backward pass");
     return gradients({dx, dw}, 3, "grouped_matmul has no second derivative");

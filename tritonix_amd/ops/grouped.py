@@ -109,7 +109,9 @@ class _Grouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, w, offsets)
+        # (what no gradient that is asked for reads is not kept: it may change before the backward pass)
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, w if ctx.needs_input_grad[0] else None, offsets)
+        ctx.transposed = w.stride(1) == 1 and w.stride(2) != 1
         return _rows_product(x, w, offsets)
 
     @staticmethod
@@ -125,8 +127,7 @@ class _Grouped(torch.autograd.Function):
             dx = _rows_product(dy, w.transpose(1, 2), offsets)
         if ctx.needs_input_grad[1]:
             # (a transposed weight's gradient has its layout)
-            transposed = w.stride(1) == 1 and w.stride(2) != 1
-            dw = _weight_gradient(dy, x, offsets).transpose(1, 2) if transposed else _weight_gradient(x, dy, offsets)
+            dw = _weight_gradient(dy, x, offsets).transpose(1, 2) if ctx.transposed else _weight_gradient(x, dy, offsets)
         return dx, dw, None
 
 

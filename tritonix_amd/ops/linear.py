@@ -105,8 +105,9 @@ class _Linear(torch.autograd.Function):
         derived = activation != _C.ACT_NONE and any(ctx.needs_input_grad[:3])
         y, z = _run(x, w, bias, residual, activation, derived)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, w, z)
-        ctx.activation, ctx.bias_dtype = activation, None if bias is None else bias.dtype
+        # (what no gradient that is asked for reads is not kept: it may change before the backward pass)
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, w if ctx.needs_input_grad[0] else None, z)
+        ctx.activation, ctx.bias_dtype, ctx.transposed = activation, None if bias is None else bias.dtype, _transposed(w)
         return y
 
     @staticmethod
@@ -129,7 +130,7 @@ class _Linear(torch.autograd.Function):
             if wants_x:
                 dx = _run(dz, w.t())[0]
             if wants_w:
-                dw = _run(dz.t(), x)[0].t() if _transposed(w) else _run(x.t(), dz)[0]
+                dw = _run(dz.t(), x)[0].t() if ctx.transposed else _run(x.t(), dz)[0]
         return dx, dw, dbias, dresidual, None
 
 

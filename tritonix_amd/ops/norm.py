@@ -56,8 +56,10 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         y, mean, rstd = _forward(x, weight, bias, eps, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.eps = eps
+        # (x where dx or dweight is asked for, weight where dx is: what neither reads may change before the backward pass)
+        wants_x, wants_weight = ctx.needs_input_grad[:2]
+        ctx.save_for_backward(x if wants_x or wants_weight else None, weight if wants_x else None, mean, rstd)
+        ctx.weight_dtype, ctx.bias_dtype = (None if t is None else t.dtype for t in (weight, bias))
         return y
 
     @staticmethod
@@ -67,20 +69,25 @@ class _LayerNorm(torch.autograd.Function):
             return None, None, None, None
         no_tangent("layer_norm", dy)
         (dy,) = as_memory(dy)
-        x, weight, bias, mean, rstd = ctx.saved_tensors
+        x, weight, mean, rstd = ctx.saved_tensors
         wants_x, wants_weight, wants_bias = ctx.needs_input_grad[:3]
         dy = _rows(dy)
-        a = _args(x, weight, bias, ctx.eps)
+        # (where only the bias asks, dx and dweight are not written and their sums not looked at: dy stands in for x)
+        a = _args(dy if x is None else x, weight, None, 0.0)
         a.mean, a.rstd, a.dy, a.stride_dy = mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dy.stride(0)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if wants_x else None
-        dweight = torch.empty_like(weight) if wants_weight else None
-        dbias = torch.empty_like(bias) if wants_bias else None
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device) if wants_x else None
+        dweight = torch.empty(dy.shape[1], dtype=ctx.weight_dtype, device=dy.device) if wants_weight else None
+        dbias = torch.empty(dy.shape[1], dtype=ctx.bias_dtype, device=dy.device) if wants_bias else None
+        if wants_weight:
+            a.weight_dtype = dtype_code("layer_norm", ctx.weight_dtype)
+        if wants_bias:
+            a.bias_dtype = dtype_code("layer_norm", ctx.bias_dtype)
         a.dx, a.dweight, a.dbias = (None if t is None else t.data_ptr() for t in (dx, dweight, dbias))
         lib = _C.load()
         need = int(lib.tnx_layer_norm_workspace_bytes(ctypes.byref(a)))
-        index = x.get_device()
+        index = dy.get_device()
         with torch.cuda.device(index):
-            scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+            scratch = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
             if need:
                 a.workspace, a.workspace_bytes = scratch.data_ptr(), need
             a.stream = _kernel._stream_of(index)
