@@ -96,6 +96,22 @@ const GroupedEntry* entry_of(int dtype, int bm, int bn) {
   return nullptr;
 }
 
+// The most tiles that the rows can make.
+int64_t tiles_of(const tnx_grouped_args* a, int bm, int bn) {
+  const int64_t down = gradient(a) ? a->groups * ((a->k + bm - 1) / bm) : a->rows / bm + (a->groups + 2 < a->rows ? a->groups + 2 : a->rows);
+  return down * ((a->n + bn - 1) / bn);
+}
+// Parts of k, and slabs of each: none without a slab of its own.
+int parts_of(const tnx_grouped_args* a, int asked, int64_t* per) {
+  const int bk = a->dtype == TNX_F32 ? 32 : 64;
+  const int64_t slabs = gradient(a) ? a->rows / bk + 1 : (a->k + bk - 1) / bk;
+  const int parts = asked > slabs ? (int)slabs : asked;
+  *per = parts > 1 ? (slabs + parts - 1) / parts : slabs;
+  return parts > 1 && !gradient(a) ? (int)((slabs + *per - 1) / *per) : parts;
+}
+// A grid's threads are counted in 32 bits: what makes more is refused.
+bool launchable(const tnx_grouped_args* a, const GroupedEntry* e, int parts) { return (double)tiles_of(a, e->bm, e->bn) * parts * e->nw * 64 < 4294967296.0; }
+
 int64_t sums_of(const tnx_grouped_args* a) { return gradient(a) ? (int64_t)a->groups * a->k * a->n : a->rows * a->n; }
 constexpr int64_t MOST_PART_BYTES = 64 << 20;
 
@@ -125,6 +141,7 @@ Choice make_choice(const tnx_grouped_args* a) {
     const double kt = at ? std::ceil(each / bk) : std::ceil((double)a->k / bk);
     for (int s : cuts) {
       if (s > 1 && (!e->parts[at ? 2 : bt ? 1 : 0] || kt / s < 2 || tiles * s > 3 * CUS || (double)s * sums_of(a) * 4 > MOST_PART_BYTES)) break;
+      if (!launchable(a, e, s)) break;
       double us = compute_time(t, tiles * s, std::ceil(kt / s), tail, at);
       const double stream = bytes / 5.1e6 * (at ? 1.1 : bt ? t.stream_nt : t.stream_nn) + 2.5;
       const double p = at ? 2.0 : 4.0;
@@ -273,21 +290,16 @@ extern "C" int tnx_grouped(const tnx_grouped_args* a) {
   if (!e) return TNX_E_UNSUPPORTED;
   Layout l;
   if (!layout_of(a, e->bm, e->bn, &l)) return TNX_E_UNSUPPORTED;
-  const int which = at ? 2 : l.bt ? 1 : 0, bk = a->dtype == TNX_F32 ? 32 : 64;
-  const int64_t sums = sums_of(a), slabs = at ? a->rows / bk + 1 : (a->k + bk - 1) / bk;
-  // (no part without a slab of its own, and without a workspace no parts)
-  if (c.parts > slabs) c.parts = (int)slabs;
-  const int64_t per = c.parts > 1 ? (slabs + c.parts - 1) / c.parts : slabs;
-  if (c.parts > 1 && !at) c.parts = (int)((slabs + per - 1) / per);
+  const int which = at ? 2 : l.bt ? 1 : 0;
+  const int64_t sums = sums_of(a);
+  int64_t per;
+  c.parts = parts_of(a, a->workspace ? c.parts : 1, &per);                    // (without a workspace no parts)
   const size_t need = c.parts > 1 ? (size_t)c.parts * sums * 4 : 0;
-  if (!a->workspace) c.parts = 1;
-  else if (c.parts > 1 && (a->workspace_bytes < need || ((uintptr_t)a->workspace & 15))) return TNX_E_WORKSPACE;
+  if (c.parts > 1 && (a->workspace_bytes < need || ((uintptr_t)a->workspace & 15))) return TNX_E_WORKSPACE;
   const bool cut = c.parts > 1;
   const grouped_fn fn = cut ? e->parts[which] : which == 2 ? e->at : which == 1 ? e->bt : e->nn;
   if (!fn) return TNX_E_UNSUPPORTED;
-  const int64_t tiles_n = (a->n + e->bn - 1) / e->bn;
-  const int64_t tiles_m = at ? a->groups * ((a->k + e->bm - 1) / e->bm) : a->rows / e->bm + (a->groups + 2 < a->rows ? a->groups + 2 : a->rows);
-  if (tiles_m * tiles_n * c.parts > 0x7fffffff) return TNX_E_UNSUPPORTED;
+  if (!launchable(a, e, c.parts) || (cut && (sums + 1023) / 1024 > 0xffffffffll / 256)) return TNX_E_UNSUPPORTED;
   GroupedParams p;
   p.a = (const uint8_t*)a->a; p.b = (const uint8_t*)a->b; p.c = cut ? (uint8_t*)a->workspace : (uint8_t*)a->c;
   p.offsets = a->offsets;
@@ -297,7 +309,7 @@ extern "C" int tnx_grouped(const tnx_grouped_args* a) {
   p.groups = a->groups; p.group_m = 8;
   p.parts = c.parts; p.per_part = (int32_t)per; p.part_stride = sums;
   p.flags = l.tail ? PF_TAIL : 0u;
-  const hipError_t err = fn(p, (unsigned)(tiles_m * tiles_n * c.parts), (hipStream_t)a->stream);
+  const hipError_t err = fn(p, (unsigned)(tiles_of(a, e->bm, e->bn) * c.parts), (hipStream_t)a->stream);
   if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
   if (!cut) return TNX_OK;
   const hipError_t joined = join(a, c.parts, sums);
@@ -318,7 +330,8 @@ extern "C" int tnx_grouped_route(const tnx_grouped_args* a, int32_t info[5]) {
   const Choice c = choose(a);
   const GroupedEntry* e = c.entry;
   Layout l;
-  if (!e || !layout_of(a, e->bm, e->bn, &l) || !(gradient(a) ? e->at : l.bt ? e->bt : e->nn)) return 0;
+  int64_t per;
+  if (!e || !layout_of(a, e->bm, e->bn, &l) || !(gradient(a) ? e->at : l.bt ? e->bt : e->nn) || !launchable(a, e, parts_of(a, c.parts, &per))) return 0;
   if (info) { info[0] = e->bm; info[1] = e->bn; info[2] = e->nw; info[3] = l.tail; info[4] = c.parts; }
   return 1;
 }
