@@ -335,3 +335,19 @@ def test_route_of_short_rows(device):
     g.c = y.data_ptr()
     assert lib.tnx_grouped(ctypes.byref(g)) == _C.E_UNSUPPORTED
     ref.check("y", tritonix.grouped_matmul(x, w, offsets), ref.grouped(x, w, offsets)["y"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("workspace", [False, True])
+def test_no_k_through_the_entry_point(device, dtype, workspace):
+    """k of 0: every row is the sum of nothing, with a workspace to cut k in and without."""
+    rows, n = 70, 40
+    y = torch.full((rows, n), float("nan"), dtype=dtype, device=device)
+    offsets = torch.tensor([3, 20, 66], dtype=torch.int32, device=device)
+    scratch = torch.empty(1 << 16, dtype=torch.uint8, device=device)
+    g = _C.GroupedArgs(c=y.data_ptr(), offsets=offsets.data_ptr(), rows=rows, n=n, k=0, stride_ar=0, stride_ak=1, stride_group=0, stride_bk=n, stride_bn=1, groups=2,
+                       dtype={torch.float16: _C.F16, torch.bfloat16: _C.BF16, torch.float32: _C.F32}[dtype], stream=torch.cuda.current_stream().cuda_stream)
+    if workspace:
+        g.workspace, g.workspace_bytes = scratch.data_ptr(), scratch.numel()
+    assert _C.load().tnx_grouped(ctypes.byref(g)) == _C.OK
+    assert not y.isnan().any() and not y.any()

@@ -104,7 +104,7 @@ int64_t tiles_of(const tnx_grouped_args* a, int bm, int bn) {
 // Parts of k, and slabs of each: none without a slab of its own.
 int parts_of(const tnx_grouped_args* a, int asked, int64_t* per) {
   const int bk = a->dtype == TNX_F32 ? 32 : 64;
-  const int64_t slabs = gradient(a) ? a->rows / bk + 1 : (a->k + bk - 1) / bk;
+  const int64_t slabs = gradient(a) ? a->rows / bk + 1 : a->k > 0 ? (a->k + bk - 1) / bk : 1;
   const int parts = asked > slabs ? (int)slabs : asked;
   *per = parts > 1 ? (slabs + parts - 1) / parts : slabs;
   return parts > 1 && !gradient(a) ? (int)((slabs + *per - 1) / *per) : parts;
