@@ -1,4 +1,5 @@
 """Linear layers, layer normalisation and grouped products whose elements are past 32 bits, of very many rows, and from several threads at once."""
+import importlib
 import threading
 
 import pytest
@@ -154,3 +155,33 @@ def test_threads_on_streams_of_their_own(device):
     for t in threads:
         t.join()
     assert not failures, failures
+
+
+def test_sums_of_more_columns_than_a_launch_has_threads_for(device):
+    """The second launches of bias' and parameters' gradients, 16 threads to a column: past 2^28 columns of a linear layer, 2^27 of a normalisation."""
+    module = importlib.import_module("tritonix_amd.ops.linear")
+    m, n = 65, (1 << 28) + 200
+    dy = torch.ones(m, n, dtype=BF16, device=device)
+    odd = torch.tensor([0, 5, n // 2, (1 << 28) - 1, 1 << 28, n - 1], device=device)
+    dy[m - 1, odd] = 7.0
+    dbias = module._gradient(dy, None, 0, False, torch.float32)[1]
+    del dy
+    want = torch.full((n,), 65.0, device=device)
+    want[odd] = 71.0
+    assert torch.equal(dbias, want)
+    del dbias, want
+    # rows of 1 and -1 in turn: mean 0 and variance 1 without a rounding, so that unit is x / sqrt(1 + eps)
+    rows, n = 2, (1 << 27) + 200
+    x = torch.ones(rows, n, dtype=BF16, device=device)
+    x[:, 1::2] = -1.0
+    weight, bias = torch.ones(n, device=device, requires_grad=True), torch.zeros(n, device=device, requires_grad=True)
+    dy = torch.ones(rows, n, dtype=BF16, device=device)
+    odd = torch.tensor([1, 6, n // 2, (1 << 27) - 1, 1 << 27, n - 1], device=device)
+    dy[1, odd] = 3.0
+    dweight, dbias = torch.autograd.grad(tritonix.layer_norm(x, weight, bias), (weight, bias), dy)
+    total = torch.full((n,), 2.0, device=device)
+    total[odd] = 4.0
+    assert torch.equal(dbias, total)
+    # (the statistics: sums of n terms whose partial ones are whole numbers up to 2^18 a thread, then a tree of 1024 of them: 12 additions with a rounding each)
+    unit = (1 + 1e-5) ** -0.5
+    assert ((dweight.double() - total.double() * x[0].double() * unit).abs() <= 32 * ref.E * total).all()

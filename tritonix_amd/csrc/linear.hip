@@ -111,11 +111,11 @@ template <class O> __global__ __launch_bounds__(256) void grad_kernel(GradParams
   }
 }
 
-// out[c] = the sum of parts[i][c] in the order of i, 64 columns and 16 lines of threads to a workgroup
-__global__ __launch_bounds__(1024) void parts_kernel(const float* parts, int64_t count, int64_t n, uint8_t* out, int dtype) {
+// out[c] = the sum of parts[i][c] in the order of i, 64 columns from the `first` on and 16 lines of threads to a workgroup
+__global__ __launch_bounds__(1024) void parts_kernel(const float* parts, int64_t count, int64_t n, int64_t first, uint8_t* out, int dtype) {
   __shared__ float sums[16][64];
   const int lane = threadIdx.x & 63, line = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t col = first + (int64_t)blockIdx.x * 64 + lane;
   float s = 0.0f;
   if (col < n) {
 #pragma unroll 8
@@ -354,7 +354,7 @@ extern "C" int tnx_linear_gradient(const tnx_linear_gradient_args* a) {
   if (a->n == 0 || (!a->dz && !a->dbias) || (a->m == 0 && !a->dbias)) return TNX_OK;
   if ((a->m > 0 && !a->dy) || (a->m > 0 && a->activation != TNX_ACT_NONE && !a->z)) return TNX_E_INVALID;
   const int64_t blocks = a->m > 0 ? row_blocks(a) : 1, span = 32 * (a->dtype == TNX_F32 ? 4 : 8), cols = (a->n + span - 1) / span;
-  if (blocks > 65535 || cols > 0x7fffffff) return TNX_E_UNSUPPORTED;
+  if (blocks > 65535 || cols > 0xffffffffll / 256) return TNX_E_UNSUPPORTED;           // (a grid's threads are counted in 32 bits)
   const size_t need = tnx_linear_gradient_bytes(a);
   if (need && (!a->workspace || a->workspace_bytes < need || ((uintptr_t)a->workspace & 15))) return TNX_E_WORKSPACE;
   GradParams p = {(const uint8_t*)a->dy, (const uint8_t*)a->z, (uint8_t*)a->dz, (uint8_t*)a->dbias, need ? (float*)a->workspace : nullptr, a->m, a->n,
@@ -364,8 +364,13 @@ extern "C" int tnx_linear_gradient(const tnx_linear_gradient_args* a) {
   if (a->dtype == TNX_BF16) hipLaunchKernelGGL(grad_kernel<OutBF16>, grid, dim3(256), 0, stream, p);
   else if (a->dtype == TNX_F16) hipLaunchKernelGGL(grad_kernel<OutF16>, grid, dim3(256), 0, stream, p);
   else hipLaunchKernelGGL(grad_kernel<OutF32>, grid, dim3(256), 0, stream, p);
-  if (need)
-    hipLaunchKernelGGL(parts_kernel, dim3((unsigned)((a->n + 63) / 64)), dim3(1024), 0, stream, (const float*)a->workspace, blocks, a->n, (uint8_t*)a->dbias,
-                       a->bias_dtype);
+  if (need) {
+    constexpr int64_t MOST = 0xffffffffll / 1024;
+    for (int64_t first = 0; first < a->n; first += MOST * 64) {
+      const int64_t left = (a->n - first + 63) / 64;
+      hipLaunchKernelGGL(parts_kernel, dim3((unsigned)(left < MOST ? left : MOST)), dim3(1024), 0, stream, (const float*)a->workspace, blocks, a->n, first,
+                         (uint8_t*)a->dbias, a->bias_dtype);
+    }
+  }
   return launched();
 }

@@ -473,13 +473,13 @@ template <class O> __global__ __launch_bounds__(256) void norm_columns_kernel(No
   }
 }
 
-// out[c] = the sum of parts[i][c] in the order of i: the first n columns are dweight, the others dbias
-template <int ACROSS> __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, int64_t count, int64_t n, uint8_t* dweight, int weight_dtype, uint8_t* dbias,
-                                                          int bias_dtype) {
+// out[c] = the sum of parts[i][c] in the order of i, from column `first` on: the first n columns are dweight, the others dbias
+template <int ACROSS> __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, int64_t count, int64_t n, int64_t first, uint8_t* dweight, int weight_dtype,
+                                                                                 uint8_t* dbias, int bias_dtype) {
   constexpr int LINES = 1024 / ACROSS;
   __shared__ float sums[LINES][ACROSS];
   const int lane = threadIdx.x % ACROSS, line = threadIdx.x / ACROSS;
-  const int64_t col = (int64_t)blockIdx.x * ACROSS + lane;
+  const int64_t col = first + (int64_t)blockIdx.x * ACROSS + lane;
   float s = 0.0f;
   if (col < 2 * n) {
 #pragma unroll 8
@@ -578,12 +578,16 @@ template <class O> int forward_rows(const NormParams& p, hipStream_t stream) {
   return launched();
 }
 
-// 16 columns to a workgroup while 64 leave CUs without one (25953 x 978 bf16, 1024 shares: 64 columns 8.5 us, 16 columns 5.5)
+// 16 columns to a workgroup while 64 leave CUs without one (25953 x 978 bf16, 1024 shares: 64 columns 8.5 us, 16 columns 5.5).  In several launches where one has
+// not threads for all columns: a grid's are counted in 32 bits.
 void launch_parts(const NormParams& p, int64_t shares, const tnx_norm_args* a, hipStream_t stream) {
   const int across = 2 * p.n <= 64 * 128 ? 16 : 64;
-  const dim3 grid((unsigned)((2 * p.n + across - 1) / across));
-  hipLaunchKernelGGL((across == 16 ? norm_parts_kernel<16> : norm_parts_kernel<64>), grid, dim3(1024), 0, stream, p.parts, shares, p.n, (uint8_t*)a->dweight,
-                     a->weight_dtype, (uint8_t*)a->dbias, a->bias_dtype);
+  constexpr int64_t MOST = 0xffffffffll / 1024;
+  for (int64_t first = 0; first < 2 * p.n; first += MOST * across) {
+    const int64_t left = (2 * p.n - first + across - 1) / across;
+    hipLaunchKernelGGL((across == 16 ? norm_parts_kernel<16> : norm_parts_kernel<64>), dim3((unsigned)(left < MOST ? left : MOST)), dim3(1024), 0, stream, p.parts, shares, p.n,
+                       first, (uint8_t*)a->dweight, a->weight_dtype, (uint8_t*)a->dbias, a->bias_dtype);
+  }
 }
 
 template <class O> int forward(NormParams p, hipStream_t stream) {
