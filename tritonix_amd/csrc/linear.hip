@@ -297,9 +297,10 @@ extern "C" int tnx_linear(const tnx_linear_args* a) {
   if (!a->y || (a->k > 0 && (!a->x || !a->w))) return TNX_E_INVALID;
   const Plan& p = plan_of(a);
   if (p.status != TNX_OK) return p.status;
+  const int bias_dtype = a->bias ? a->bias_dtype : a->dtype;          // (packed beside other flags: without a bias it may hold anything)
   if (p.route == ROUTE_STREAM) {
     const StreamParams q = {(const uint8_t*)a->x, (const uint8_t*)a->w, (uint8_t*)a->y, (uint8_t*)a->z, (const uint8_t*)a->bias, (const uint8_t*)a->residual,
-                            a->stride_xm, a->stride_wn, (int32_t)a->m, (int32_t)a->n, (int32_t)a->k, a->activation, a->bias_dtype};
+                            a->stride_xm, a->stride_wn, (int32_t)a->m, (int32_t)a->n, (int32_t)a->k, a->activation, bias_dtype};
     const hipStream_t s = (hipStream_t)a->stream;
     const hipError_t err = a->dtype == TNX_BF16 ? stream_columns<TagBF16>(q, s) : a->dtype == TNX_F16 ? stream_columns<TagF16>(q, s) : stream_columns<TagF32>(q, s);
     if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
@@ -309,7 +310,7 @@ extern "C" int tnx_linear(const tnx_linear_args* a) {
     if (p.workspace > 0 && (!a->workspace || a->workspace_bytes < p.workspace || ((uintptr_t)a->workspace & 15))) return TNX_E_WORKSPACE;
     const StreamRowsParams q = {(const uint8_t*)a->x, (const uint8_t*)a->w, (uint8_t*)a->y, (uint8_t*)a->z, (const uint8_t*)a->bias, (const uint8_t*)a->residual,
                                 p.workspace > 0 ? (uint8_t*)a->workspace : nullptr, a->stride_xm, a->stride_wk, (int32_t)a->m, (int32_t)a->n, (int32_t)a->k,
-                                stream_rows_parts(a->n, a->k, a->dtype == TNX_F32 ? 4 : 2), a->activation | a->bias_dtype << 8};
+                                stream_rows_parts(a->n, a->k, a->dtype == TNX_F32 ? 4 : 2), a->activation | bias_dtype << 8};
     const hipStream_t s = (hipStream_t)a->stream;
     const hipError_t err = a->dtype == TNX_BF16 ? stream_rows<TagBF16>(q, s) : a->dtype == TNX_F16 ? stream_rows<TagF16>(q, s) : stream_rows<TagF32>(q, s);
     if (err != hipSuccess) { note_hip_error((int)err); return TNX_E_HIP; }
@@ -322,7 +323,7 @@ extern "C" int tnx_linear(const tnx_linear_args* a) {
   g.workspace = a->workspace; g.workspace_bytes = a->workspace_bytes;
   g.stream = a->stream;
   uint8_t* terms = (uint8_t*)a->scratch + p.sums;
-  const LinearParts x = {(const uint8_t*)a->bias, (const uint8_t*)a->residual, (uint8_t*)a->z, a->bias_dtype, a->activation};
+  const LinearParts x = {(const uint8_t*)a->bias, (const uint8_t*)a->residual, (uint8_t*)a->z, bias_dtype, a->activation};
   const LinearParts* fused = p.route == ROUTE_FUSED ? &x : nullptr;
   const int status = a->k == 0 ? TNX_OK : p.f32 ? gemm_f32(&g, p.scratch > p.sums ? terms : nullptr, p.scratch - p.sums, fused) : gemm_launch(&g, nullptr, GEMM_PLAIN, fused);
   if (status != TNX_OK || p.route != ROUTE_APART) return status;
