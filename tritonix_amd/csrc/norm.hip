@@ -539,7 +539,9 @@ int64_t shares_of(const tnx_norm_args* a) {
 int check(const tnx_norm_args* a) {
   if (!a || a->rows < 0 || a->n < 0 || !(a->eps >= 0.0f)) return TNX_E_INVALID;
   if (a->dtype != TNX_F16 && a->dtype != TNX_BF16 && a->dtype != TNX_F32) return TNX_E_UNSUPPORTED;
-  if ((a->weight && a->weight_dtype != a->dtype && a->weight_dtype != TNX_F32) || (a->bias && a->bias_dtype != a->dtype && a->bias_dtype != TNX_F32))
+  // (of a parameter's gradient too, which may be asked for where the parameter itself is not given)
+  if (((a->weight || a->dweight) && a->weight_dtype != a->dtype && a->weight_dtype != TNX_F32) ||
+      ((a->bias || a->dbias) && a->bias_dtype != a->dtype && a->bias_dtype != TNX_F32))
     return TNX_E_UNSUPPORTED;
   if (a->rows > 0x7fffffff || a->n > 0x3fffffff) return TNX_E_UNSUPPORTED;
   return TNX_OK;
