@@ -470,7 +470,7 @@ int tnx_moe_combine(const void* y, const int32_t* rows, const float* weights, vo
  * Linear layers.
  *
  * z[m, n] = x[m, k] w[k, n] + bias[n],  y = act(z) + residual.  Sums in 32 bits (float32 operands: as tnx_gemm_f32), each output rounded
- * once.  residual, y and z are row-major without gaps, of `dtype`; bias is of `dtype` or float32.  x and w take any strides; rows of x with w row-major or
+ * once.  An infinite z has the activation's limits.  residual, y and z are row-major without gaps, of `dtype`; bias is of `dtype` or float32.  x and w take any strides; rows of x with w row-major or
  * k-contiguous (stride_wk == 1, the transpose of a row-major weight) are the fast layouts.  Without bias, residual, z and activation it is a
  * product, with x also contiguous along m (stride_xm == 1): the gradients dx = dz w^T and dw = x^T dz. */
 enum tnx_activation {
@@ -490,7 +490,7 @@ typedef struct tnx_linear_args {
   int64_t m, n, k;
   int64_t stride_xm, stride_xk, stride_wk, stride_wn;
   int32_t dtype;               /* TNX_F16, TNX_BF16 or TNX_F32 */
-  int32_t bias_dtype;
+  int32_t bias_dtype;          /* without a bias it does not count */
   int32_t activation;          /* tnx_activation */
   int32_t reserved;
   void* workspace;             /* tnx_linear_workspace_bytes, 256-byte aligned; its first TNX_WS_COUNTER_BYTES zero when first used, and left zero */
@@ -536,7 +536,8 @@ int tnx_linear_gradient(const tnx_linear_gradient_args* args);
  * of x - mean.  In 32 bits throughout, outputs rounded once.  weight and bias (either or both may be null) are of `dtype` or float32.
  *
  * The backward pass takes mean and rstd as the forward pass wrote them: dx, and dweight and dbias of the parameters' types (each may be
- * null), summed over the rows in an order that depends on the sizes alone. */
+ * null), summed over the rows in an order that depends on the sizes alone.  Where dx is not asked for weight is not read (it may be null), where neither dx nor dweight is
+ * x's values do not count; bias is never read. */
 typedef struct tnx_norm_args {
   const void *x, *weight, *bias;
   void* y;                     /* [rows, n] without gaps */
@@ -565,7 +566,7 @@ int tnx_layer_norm_backward(const tnx_norm_args* args);
  * 32-bit sums (float32 on the binary32 matrix instruction), rounded once.  a has neighbouring columns (stride_ak == 1, stride_ar >= k).  b: row-major
  * (stride_bn == 1) or, in the first form, k-contiguous matrices (stride_bk == 1); in the second form rows of n, stride_bk apart.  c has no gaps.
  * Operands whose rows are too short for the loads (n, and in the second form k, of less than a 16-byte chunk) are refused with
- * TNX_E_UNSUPPORTED. */
+ * TNX_E_UNSUPPORTED, and so are a tile's rows that lie 4 GiB apart or more and products of more tiles than a grid's 2^32 threads. */
 #define TNX_GROUPED_MAX_GROUPS 4096
 enum tnx_grouped_form { TNX_GROUPED_ROWS = 0, TNX_GROUPED_WEIGHT_GRADIENT = 1 };
 

@@ -52,7 +52,6 @@ inline bool linear_params(const GemmParams& p, const LinearParts& x, bool bt, in
 // N neighbouring 16- or 32-bit floats in 32 bits
 template <class O, int N> struct Run {
   typedef typename O::raw raw;
-  static constexpr int WORDS = N * sizeof(raw) / 4;
   static __device__ __forceinline__ float widen(raw v) {
     if constexpr (std::is_same<O, OutBF16>::value) return __builtin_bit_cast(float, (uint32_t)v << 16);
     else if constexpr (std::is_same<O, OutF16>::value) return (float)__builtin_bit_cast(_Float16, v);
@@ -181,7 +180,8 @@ struct LinearFamily {
 #pragma unroll
         for (int e = 0; e < V; ++e) f[e] += bias[t][e];
         if (z) {
-          // (rounded to the output's type, as y is: the backward pass takes the derivative there)
+          // (rounded to the output's type, as y is: the backward pass takes the derivative there.  In 32 bits it would take dx and dw from 2.40e-3 to 2.34e-3 of their 2-norm (bf16, silu or gelu; the
+          // rest is dz's rounding and their own), for twice the memory that a layer holds between its passes and, at a copy's rate, 13 us more in both passes of 8192 x 4096)
 #pragma unroll
           for (int e = 0; e < V; ++e) out[e] = O::cvt(f[e]);
           put(z + at, l_cols[t], out);

@@ -4,7 +4,7 @@
 //
 // The product runs on the tile kernels with the epilogue of gemm_linear.h, float32 on the same kernels by heads and tails or, small ones, on
 // the binary32 matrix instruction.  Where no such kernel takes the operands as they lie (an x that is contiguous along m, rows shorter
-// than a 16-byte chunk, k = 0) the sums go to scratch in 32 bits and the epilogue is a launch of its own.  Few rows of 16-bit types: gemm_stream.h.  dx = dz w^T and dw = x^T dz are
+// than a 16-byte chunk, k = 0) the sums go to scratch in 32 bits and the epilogue is a launch of its own.  Few rows: gemm_stream.h.  dx = dz w^T and dw = x^T dz are
 // products without an epilogue.
 #include <hip/hip_runtime.h>
 #include <string.h>
@@ -51,6 +51,9 @@ struct GradParams {
 
 // A workgroup takes a block of rows of 32 runs of V columns; its 8 lines of threads take a row in turn, add up their columns and meet in
 // LDS.  Bound by memory: 8192 x 4096 bf16, dz of relu 38 us (5.3 TB/s).
+//
+// dz is rounded to the operands' type, for that is what the matrix instructions of dx = dz w^T and dw = x^T dz take; dbias sums it unrounded.  This rounding costs dx and dw as much as their own: off
+// by 2.4e-3 (2-norm, bf16; f16 3.0e-4) against 1.66e-3 (2.1e-4) for a result that is rounded once.  dz in two terms would halve the rate of both products, which are two thirds of a step.
 template <class O> __global__ __launch_bounds__(256) void grad_kernel(GradParams p) {
   typedef typename O::raw raw;
   constexpr int V = 16 / sizeof(raw);

@@ -5,7 +5,7 @@
 //
 // Bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  A row is read once, into registers (16-byte runs,
 // one after another over the threads), the mean before the variance from the same registers: no difference of large squares.  16384 x 8192
-// bf16: 107 us (5.0 TB/s; a copy reaches 5.1), backward 182 (4.4 TB/s, and 8 us for the parameters' shares).  In the backward pass a workgroup
+// bf16: 107 us (5.0 TB/s; a copy reaches 5.1), backward 182 (4.4 TB/s, 5 of them for the parameters' shares).  In the backward pass a workgroup
 // keeps its rows' share of dweight and dbias, in 32 bits per column, and a second launch adds the workgroups' shares up in order.
 #include <hip/hip_runtime.h>
 
@@ -165,7 +165,7 @@ template <class O, int TPR, int CH, bool WHOLE> __global__ __launch_bounds__(TPR
   __shared__ float lds[2 * THREADS / 64];
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
-  if (row >= p.rows) return;                             // (whole waves; with TPR = THREADS whole workgroups)
+  if (row >= p.rows) return;                             // (all lanes of a row together, and no sum leaves a row's lanes; with TPR = THREADS whole workgroups)
   const raw* src = (const raw*)p.x + row * p.stride_x;
   float f[CH][V];
   float s[1] = {0.0f};
@@ -354,7 +354,8 @@ template <class O, int TPR, int CH, bool PARTS, bool WHOLE> __global__ __launch_
   }
 }
 
-// Rows longer than the registers hold: read again for each of the passes.  A workgroup of 1024 threads to a row.
+// Rows longer than the registers hold: read again for each of the passes.  A workgroup of 1024 threads to a row, whose loads, reductions and stores take turns (2048 x 65536 bf16:
+// 160 us forward, 3.4 TB/s of x and y once; 4096 x 32768, in registers by the same workgroups, 142).
 template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_long_kernel(NormParams p) {
   typedef typename O::raw raw;
   constexpr int V = 16 / sizeof(raw), TPR = 1024;
@@ -421,7 +422,8 @@ template <class O, bool BACKWARD> __global__ __launch_bounds__(1024) void norm_l
   }
 }
 
-// dweight and dbias of such rows, and of those too long for a thread to keep its columns' sums too (sums_apart): a workgroup's 32 runs of columns down 256 rows, its 8 rows of threads meet in LDS
+// dweight and dbias of such rows, and of those too long for a thread to keep its columns' sums too (sums_apart): a workgroup's 32 runs of columns down 32 to 256 rows (columns_rows), its 8 rows of
+// threads meet in LDS.  x and dy are read a second time for them: 10 bytes an element of 16 bits where 6 would do (8192 x 16384 bf16 265 us backward, 160 at a copy's rate)
 template <class O> __global__ __launch_bounds__(256) void norm_columns_kernel(NormParams p) {
   typedef typename O::raw raw;
   constexpr int V = 16 / sizeof(raw);

@@ -2,7 +2,8 @@
 
     y = linear(x, w, bias, activation="gelu", residual=r)         # act(x @ w + bias) + r
 
-One launch where x is row-major and w row-major or k-contiguous (``weight.t()``); the tile is the library's built-in choice, no tuning.  For the backward
+One launch where x is row-major and w row-major or k-contiguous (``weight.t()``); the tile is the library's built-in choice, no tuning.  Matrices are launched by csrc/launch.cpp;
+x of other dimensions is reshaped here and goes through the interpreter, 8 us more a call and some 100 a training step.  For the backward
 pass z = x @ w + bias is written beside y where there is an activation.  Gradients: dz = dy * act'(z) and the bias' sums in one pass, then two
 products.  Tensors live on a HIP device; there is no CPU path.
 """
@@ -138,11 +139,13 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act(x @ w + bias) + residual`` with ``x[..., k]``, ``w[k, n]``, ``bias[n]`` and ``residual[..., n]``.
 
-    float16, bfloat16 and float32 (as ``matmul``: three bfloat16 products, few rows and small problems on the binary32 matrix
-    instruction); w and residual have x's dtype, the bias that or float32.  ``activation`` is None, "relu", "silu", "gelu" (with erf) or
+    float16, bfloat16 and float32 (as ``matmul``: three bfloat16 products, off by some 3e-6 of the result's 2-norm, few rows and small problems on the
+    binary32 matrix instruction; ``grouped_matmul`` takes that one always); w and residual have x's dtype, the bias that or float32.  ``activation`` is None, "relu", "silu", "gelu" (with erf) or
     "gelu_tanh".  Sums, bias, activation and residual are in 32 bits, the result is rounded once.
 
-    Differentiable in x, w, bias and residual.  act' is taken at z = x @ w + bias as it was kept, rounded to x's dtype; dz = dy * act'(z) is
+    An infinite x @ w + bias has the activation's limits, a NaN stays one.
+
+    Differentiable in x, w, bias and residual, once and backwards: second derivatives and tangents of forward mode are errors.  act' is taken at z = x @ w + bias as it was kept, rounded to x's dtype; dz = dy * act'(z) is
     rounded to it for the products dx = dz @ w.t() and dw = x.t() @ dz, the bias' gradient sums it in 32 bits, in an order that depends on the sizes alone."""
     act = ACTIVATIONS.get(activation)
     if act is not None:

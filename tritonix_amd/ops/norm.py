@@ -2,8 +2,9 @@
 
     y = layer_norm(x, weight, bias)              # (x - mean) / sqrt(variance + eps) * weight + bias over the last dimension
 
-A row is read once; mean, variance and sums are in 32 bits.  The gradients of weight and bias are summed over the rows in an order that depends on the
-sizes alone: the same call gives the same bits.  Tensors live on a HIP device; there is no CPU path.
+A row is read once (of more than 32768 elements of 16 bits, 16384 of 32, again for each pass); mean, variance and sums are in 32 bits.  The gradients of weight and bias are summed over the rows in an order that depends on the
+sizes alone: the same call gives the same bits.  Matrices are launched by csrc/launch.cpp; x of other dimensions is reshaped here and goes through the interpreter, 9 us more a call and some 80 a training step.
+Tensors live on a HIP device; there is no CPU path.
 """
 from __future__ import annotations
 
@@ -101,7 +102,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     variance being the mean of (x - mean)^2.
 
     ``weight[n]`` and ``bias[n]``, of x's dtype or float32, may be left out.  The result has x's dtype and shape, rounded once.  A row with a
-    NaN or an infinity is NaN.  Differentiable in x, weight and bias."""
+    NaN or an infinity is NaN.  Differentiable in x, weight and bias, once and backwards."""
     y = (_native.module or _native.find()).layer_norm(x, weight, bias, eps)
     if y is not None:
         return y
